@@ -59,8 +59,9 @@ extern "C" {
 /* 8: tfgfa_decode_splits, tfgfa_decode_scratch_bytes and tfgfa_stream_read added;
  * tfgfa_decode_noalloc splits only as far as its scratch holds instead of returning
  * TFGFA_ERR_SCRATCH.
- * 9: the six tfgpt2_* entry points added (tfgfa_gpt2.h). */
-#define TFGFA_ABI_VERSION 9
+ * 9: the six tfgpt2_* entry points added (tfgfa_gpt2.h).
+ * 10: the five tfserve_* entry points added (tfgfa_serving.h). */
+#define TFGFA_ABI_VERSION 10
 
 /* Status codes (> 0: invalid argument). */
 #define TFGFA_OK                 0
@@ -74,8 +75,9 @@ extern "C" {
 #define TFGFA_ERR_STRIDE         8  /* strides outside what the entry point takes         */
 #define TFGFA_ERR_CACHE          9  /* k_new/v_new given without cache_seqlens            */
 #define TFGFA_ERR_DTYPE         10  /* dtype is not a TFGFA_DTYPE_* value                 */
-#define TFGFA_ERR_SCRATCH       11  /* reserved: tfgfa_decode_noalloc limits its split to
-                                       its scratch and no longer returns it                */
+#define TFGFA_ERR_SCRATCH       11  /* tfserve_decode_paged: key_weights and a workspace that does not
+                                       hold its scores (tfgfa_decode_noalloc limits its split to its
+                                       scratch and does not return it)                      */
 
 /* Element types of q, k, v, o (fp32 accumulation and softmax either way). */
 #define TFGFA_DTYPE_BF16 0

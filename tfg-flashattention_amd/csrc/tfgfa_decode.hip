@@ -74,13 +74,17 @@
 #include <stdint.h>
 
 #include <algorithm>
-#include <atomic>
-#include <chrono>
 #include <mutex>
 
 #include "tfgfa.h"
+#include "tfgfa_arrive.h"
 
 namespace tfgfa_dec {
+
+using tfgfa::arrive_bytes;
+using tfgfa::kArriveStride;
+using tfgfa::kTagShift;
+using tfgfa::next_tag;
 
 constexpr int kD = 64;                         // head dim of tfgfa_decode_bf16
 constexpr int kMaxD = 128;                     // largest head dim of tfgfa_decode
@@ -96,8 +100,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kWorkspaceRows = 128;            // cache rows per split counted by the workspace
 static_assert(kSplitBlockKeys % kWorkspaceRows == 0, "splits must not outnumber workspace slots");
-constexpr int kArriveStride = 128;             // bytes between the arrival words of two heads
-constexpr int kTagShift = 16;                  // arrival word: tag << 16 | count (count < 2^16)
 // A buffer offset past any num_records this file builds (those stay below 2^31 - 2^24): the
 // load returns zero without a memory access.  Used for the prefetch after the last block and
 // for the pieces of a row past the head dim.
@@ -835,28 +837,6 @@ static int workspace_splits(size_t bytes, size_t ab, size_t per_split) {
   if (bytes <= ab) return 1;
   return (int)std::max((size_t)1, std::min((size_t)INT32_MAX, (bytes - ab) / per_split));
 }
-// Bytes of the arrival words at the start of a workspace: one per head, kArriveStride apart.
-static size_t arrive_bytes(long long bh) { return ((size_t)bh * kArriveStride + 255) / 256 * 256; }
-
-// A random nonzero 48-bit tag per call (splitmix64 over a process-wide counter and a seed from
-// the clock and an address), so that no word left in memory by anything else is likely to
-// carry it.
-static u64 splitmix64(u64 x) {
-  x += 0x9E3779B97F4A7C15ull;
-  x = (x ^ (x >> 30)) * 0xBF58476D1CE4E5B9ull;
-  x = (x ^ (x >> 27)) * 0x94D049BB133111EBull;
-  return x ^ (x >> 31);
-}
-static u64 next_tag() {
-  static std::atomic<u64> counter{0};
-  static const u64 seed =
-      splitmix64((u64)std::chrono::steady_clock::now().time_since_epoch().count() ^
-                 (u64)(uintptr_t)&counter);
-  const u64 t = splitmix64(seed + counter.fetch_add(1, std::memory_order_relaxed)) &
-                ((1ull << (64 - kTagShift)) - 1);
-  return t ? t : 1;
-}
-
 // The decode step for one element type: argument checks, split choice, launches.
 template <class T>
 static int decode_step(const void* q, const int64_t* q_strides, void* k_cache,

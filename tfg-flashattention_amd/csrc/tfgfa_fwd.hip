@@ -1659,7 +1659,7 @@ extern "C" const char* tfgfa_strerror(int status) {
     case TFGFA_ERR_ALIGNMENT: return "misaligned pointer (q/k/v/o need 16 B, lse 4 B)";
     case TFGFA_ERR_CACHE: return "k_new/v_new (cache append) need cache_seqlens";
     case TFGFA_ERR_SCRATCH:
-      return "reserved status (decode scratch): not returned by this library";
+      return "workspace too small for the scores that key weights are taken from";
     case TFGFA_ERR_STRIDE:
       return "unsupported strides (last dim 1; b, h, n non-negative multiples of 8; n >= head dim; "
              "o without overlapping elements)";

@@ -19,6 +19,7 @@
 #include "tfgfa.h"
 #include "tfgfa_gpt2.h"
 #include "tfgfa_plan.h"
+#include "tfgfa_serving.h"
 
 namespace py = pybind11;
 
@@ -221,6 +222,92 @@ void gpt2_linear_planes(std::uintptr_t x, std::uintptr_t w, std::uintptr_t bias,
   check(st, "tfgpt2_linear_planes");
 }
 
+using Strides2 = std::array<std::int64_t, 2>;
+
+void decode_paged(std::uintptr_t q, const Strides3& qs, std::uintptr_t k, const Strides4& ks,
+                  std::uintptr_t v, const Strides4& vs, std::uintptr_t table,
+                  std::int64_t table_stride, std::uintptr_t seqlens, std::uintptr_t kn,
+                  const Strides3& kns, std::uintptr_t vn, const Strides3& vns, std::uintptr_t o,
+                  const Strides3& os, std::uintptr_t lse, std::uintptr_t weights,
+                  const Strides2& ws, int B, int H, int H_kv, int P, int page, int M, int D,
+                  int dtype, float softmax_scale, std::uintptr_t workspace,
+                  std::size_t workspace_bytes, std::uintptr_t stream) {
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    st = tfserve_decode_paged(
+        reinterpret_cast<const void*>(q), qs.data(), reinterpret_cast<void*>(k), ks.data(),
+        reinterpret_cast<void*>(v), vs.data(), reinterpret_cast<const int*>(table), table_stride,
+        reinterpret_cast<const int*>(seqlens), reinterpret_cast<const void*>(kn), kns.data(),
+        reinterpret_cast<const void*>(vn), vns.data(), reinterpret_cast<void*>(o), os.data(),
+        reinterpret_cast<float*>(lse), reinterpret_cast<float*>(weights), ws.data(), B, H, H_kv, P,
+        page, M, D, dtype, softmax_scale, reinterpret_cast<void*>(workspace), workspace_bytes,
+        reinterpret_cast<void*>(stream));
+  }
+  check(st, "tfserve_decode_paged");
+}
+
+void key_weights(std::uintptr_t q, const Strides4& qs, std::uintptr_t k, const Strides4& ks,
+                 std::uintptr_t lse, const Strides2& ls, std::uintptr_t out, const Strides2& os,
+                 int B, int H, int H_kv, int N_q, int N_k, int D, int dtype, float softmax_scale,
+                 bool causal, std::int64_t first_query, std::uintptr_t stream) {
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    st = tfserve_key_weights(reinterpret_cast<const void*>(q), qs.data(),
+                             reinterpret_cast<const void*>(k), ks.data(),
+                             reinterpret_cast<const float*>(lse), ls.data(),
+                             reinterpret_cast<float*>(out), os.data(), B, H, H_kv, N_q, N_k, D,
+                             dtype, softmax_scale, causal ? 1 : 0, first_query,
+                             reinterpret_cast<void*>(stream));
+  }
+  check(st, "tfserve_key_weights");
+}
+
+void evict(std::uintptr_t k, const Strides4& ks, std::uintptr_t v, const Strides4& vs,
+           std::uintptr_t table, std::int64_t table_stride, std::uintptr_t seqlens,
+           std::uintptr_t weights, const Strides2& ws, std::uintptr_t new_table,
+           std::int64_t new_table_stride, std::uintptr_t kept, std::uintptr_t weights_out,
+           const Strides2& wos, int B, int H_kv, int P, int page, int M, int M_new, int D,
+           int budget, int recent, std::uintptr_t stream) {
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    st = tfserve_evict(reinterpret_cast<void*>(k), ks.data(), reinterpret_cast<void*>(v), vs.data(),
+                       reinterpret_cast<const int*>(table), table_stride,
+                       reinterpret_cast<const int*>(seqlens),
+                       reinterpret_cast<const float*>(weights), ws.data(),
+                       reinterpret_cast<const int*>(new_table), new_table_stride,
+                       reinterpret_cast<int*>(kept), reinterpret_cast<float*>(weights_out),
+                       wos.data(), B, H_kv, P, page, M, M_new, D, budget, recent,
+                       reinterpret_cast<void*>(stream));
+  }
+  check(st, "tfserve_evict");
+}
+
+// Each penalty: a device array of float32, one a row, or 0 and the scalar.
+void penalize(std::uintptr_t logits, std::int64_t logits_stride, std::uintptr_t out,
+              std::int64_t out_stride, int kind, std::uintptr_t tokens, int token_bytes,
+              std::int64_t tokens_stride, std::uintptr_t lengths, std::uintptr_t repetitions,
+              float repetition, std::uintptr_t presences, float presence,
+              std::uintptr_t frequencies, float frequency, std::uintptr_t bias,
+              std::int64_t bias_stride, std::uintptr_t allowed, std::int64_t allowed_stride, int B,
+              int V, int T, std::uintptr_t stream) {
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    st = tfserve_penalize(
+        reinterpret_cast<const void*>(logits), logits_stride, reinterpret_cast<void*>(out),
+        out_stride, kind, reinterpret_cast<const void*>(tokens), token_bytes, tokens_stride,
+        reinterpret_cast<const int*>(lengths), reinterpret_cast<const float*>(repetitions),
+        repetition, reinterpret_cast<const float*>(presences), presence,
+        reinterpret_cast<const float*>(frequencies), frequency,
+        reinterpret_cast<const float*>(bias), bias_stride, reinterpret_cast<const int*>(allowed),
+        allowed_stride, B, V, T, reinterpret_cast<void*>(stream));
+  }
+  check(st, "tfserve_penalize");
+}
+
 py::dict device_info() {
   int cu = 0, mhz = 0;
   char arch[128] = {0};
@@ -309,6 +396,39 @@ PYBIND11_MODULE(_C, m) {
     check(tfgfa_device_info(&cu, nullptr, nullptr, 0), "tfgfa_device_info");
     return tfgpt2_linear_planes_splits(M, N, K, cu);
   });
+  m.def("decode_paged", &decode_paged, "One decode step over a paged KV cache (element strides)",
+        py::arg("q"), py::arg("q_strides"), py::arg("k_pages"), py::arg("k_strides"),
+        py::arg("v_pages"), py::arg("v_strides"), py::arg("page_table"), py::arg("table_stride"),
+        py::arg("cache_seqlens"), py::arg("k_new"), py::arg("k_new_strides"), py::arg("v_new"),
+        py::arg("v_new_strides"), py::arg("o"), py::arg("o_strides"), py::arg("lse"),
+        py::arg("key_weights"), py::arg("weights_strides"), py::arg("B"), py::arg("H"),
+        py::arg("H_kv"), py::arg("P"), py::arg("page"), py::arg("M"), py::arg("D"),
+        py::arg("dtype"), py::arg("softmax_scale"), py::arg("workspace"),
+        py::arg("workspace_bytes"), py::arg("stream"));
+  m.def("decode_paged_workspace",
+        [](int B, int H, int H_kv, int page, int M, int D, bool with_weights) {
+          return tfserve_decode_paged_workspace(B, H, H_kv, page, M, D, with_weights ? 1 : 0);
+        });
+  m.def("key_weights", &key_weights, "The attention weight each key receives", py::arg("q"),
+        py::arg("q_strides"), py::arg("k"), py::arg("k_strides"), py::arg("lse"),
+        py::arg("lse_strides"), py::arg("out"), py::arg("out_strides"), py::arg("B"), py::arg("H"),
+        py::arg("H_kv"), py::arg("N_q"), py::arg("N_k"), py::arg("D"), py::arg("dtype"),
+        py::arg("softmax_scale"), py::arg("causal"), py::arg("first_query"), py::arg("stream"));
+  m.def("evict", &evict, "Eviction from a paged KV cache by accumulated weight",
+        py::arg("k_pages"), py::arg("k_strides"), py::arg("v_pages"), py::arg("v_strides"),
+        py::arg("page_table"), py::arg("table_stride"), py::arg("cache_seqlens"),
+        py::arg("key_weights"), py::arg("weights_strides"), py::arg("new_page_table"),
+        py::arg("new_table_stride"), py::arg("kept"), py::arg("weights_out"),
+        py::arg("weights_out_strides"), py::arg("B"), py::arg("H_kv"), py::arg("P"),
+        py::arg("page"), py::arg("M"), py::arg("M_new"), py::arg("D"), py::arg("budget"),
+        py::arg("recent"), py::arg("stream"));
+  m.def("penalize", &penalize, "Penalties, biases and masks on logits", py::arg("logits"),
+        py::arg("logits_stride"), py::arg("out"), py::arg("out_stride"), py::arg("kind"),
+        py::arg("tokens"), py::arg("token_bytes"), py::arg("tokens_stride"), py::arg("lengths"),
+        py::arg("repetitions"), py::arg("repetition"), py::arg("presences"), py::arg("presence"),
+        py::arg("frequencies"), py::arg("frequency"), py::arg("bias"), py::arg("bias_stride"),
+        py::arg("allowed"), py::arg("allowed_stride"), py::arg("B"), py::arg("V"), py::arg("T"),
+        py::arg("stream"));
   m.def("fwd_plan",
         [](long long heads, int cu_count, int Nq, int Nk, int D, bool causal) {
           static const char* const names[] = {"kWhole", "kHalves", "kGroups2", "kPairs", "kGroups4"};

@@ -30,8 +30,8 @@ except ImportError as exc:  # pragma: no cover - exercised only on a broken buil
         f"({exc}); run `make -C tfg-flashattention_amd/csrc` or __graft_entry__.build()"
     ) from exc
 
-__all__ = ["forward", "forward_lse", "attention", "flash_attn_forward", "decode", "device_info",
-           "HEAD_DIM", "MAX_HEAD_DIM", "library_path"]
+__all__ = ["forward", "forward_lse", "attention", "flash_attn_forward", "decode", "decode_paged",
+           "key_weights", "evict", "penalize_logits", "device_info", "HEAD_DIM", "MAX_HEAD_DIM", "library_path"]
 
 HEAD_DIM = 64  # the head dimension of forward() (common_types.hpp:33 fixes K = 64 too)
 MAX_HEAD_DIM = 128  # attention() / flash_attn_forward(): any head dim up to 128
@@ -399,3 +399,6 @@ def _decode_workspace(dev, nbytes: int) -> torch.Tensor:
 def device_info() -> dict:
     """CU count, shader clock (MHz) and gfx arch of the current device (cached per device)."""
     return _C.device_info()
+
+
+from .serving import decode_paged, evict, key_weights, penalize_logits  # noqa: E402,F401  (need the above)

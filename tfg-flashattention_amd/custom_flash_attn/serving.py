@@ -1,0 +1,307 @@
+"""The serving operators beside the attention (include/tfgfa_serving.h) on torch tensors: a decode step
+over a paged KV cache, the attention weight each key receives, eviction from the cache by that weight,
+and penalties, biases and grammar masks on logits.
+
+The reference's generate() has no cache and samples from unmodified logits
+(src/py/model_inference.py:199-228); nothing here has a counterpart in it.  The functions check their
+arguments (RuntimeError, before anything is launched), launch on the current stream of the tensors'
+device and do not synchronise.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _C, _DTYPES, MAX_HEAD_DIM, _check_vec, _current_stream, _decode_workspace, _launch_on, _WORKSPACES
+
+_ZERO3 = (0, 0, 0)
+_LOGITS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _check_pages(k_pages, v_pages) -> None:
+    for t, n in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if not t.is_cuda:
+            raise RuntimeError(f"{n} must be a CUDA tensor")
+        if t.dtype not in _DTYPES:
+            raise RuntimeError("Unsupported tensor dtype. Use bfloat16 or float16.")
+        if t.dim() != 4:
+            raise RuntimeError(f"{n} must be (P, H_kv, page, D), got {tuple(t.shape)}")
+        if t.stride(3) != 1:
+            raise RuntimeError(f"{n} must be dense in its last dimension (stride 1), got strides {t.stride()}")
+    if not (8 <= k_pages.shape[3] <= MAX_HEAD_DIM and k_pages.shape[3] % 8 == 0):
+        raise RuntimeError(f"head_dim must be a multiple of 8 in [8, {MAX_HEAD_DIM}], got {k_pages.shape[3]}")
+    if k_pages.shape[2] < 1:
+        raise RuntimeError("a page holds at least one row")
+    if v_pages.dtype != k_pages.dtype:
+        raise RuntimeError(f"v_pages must have dtype {k_pages.dtype}, got {v_pages.dtype}")
+    if v_pages.shape != k_pages.shape:
+        raise RuntimeError(f"v_pages must have shape {tuple(k_pages.shape)}, got {tuple(v_pages.shape)}")
+    if v_pages.device != k_pages.device:
+        raise RuntimeError(f"v_pages must be on {k_pages.device}, got {v_pages.device}")
+
+
+def _check_table(t, name: str, B: int, dev) -> None:
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != B:
+        raise RuntimeError(f"{name} must be int32 of shape ({B}, pages)")
+    if t.device != dev or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise RuntimeError(f"{name} must be on {dev} and dense in its last dimension")
+
+
+def _check_seqlens(t, B: int, dev) -> None:
+    if t.dtype != torch.int32 or tuple(t.shape) != (B,):
+        raise RuntimeError(f"cache_seqlens must be int32 of shape ({B},)")
+    if t.device != dev or not t.is_contiguous():
+        raise RuntimeError(f"cache_seqlens must be a contiguous tensor on {dev}")
+
+
+def _check_weights(t, name: str, B: int, H_kv: int, rows: int, dev) -> None:
+    if t.dtype != torch.float32 or t.dim() != 3 or tuple(t.shape[:2]) != (B, H_kv) or t.shape[2] < rows:
+        raise RuntimeError(f"{name} must be float32 of shape ({B}, {H_kv}, at least {rows}), got {t.dtype} "
+                           f"{tuple(t.shape)}")
+    if t.device != dev or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise RuntimeError(f"{name} must be on {dev} and dense in its last dimension")
+
+
+def decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                 cache_seqlens: torch.Tensor, k_new: torch.Tensor | None = None,
+                 v_new: torch.Tensor | None = None, *, key_weights: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None, softmax_scale: float | None = None, return_lse: bool = False,
+                 workspace: torch.Tensor | None = None):
+    """:func:`decode` over a paged cache, with query heads that may share key-value heads.
+
+    ``q``: (B, H, D).  ``k_pages``, ``v_pages``: (P, H_kv, page, D) pools (any strides with a dense last
+    dimension, e.g. (P, page, H_kv, D) buffers transposed); H a multiple of H_kv, query head h reading
+    key-value head ``h // (H // H_kv)``; any page size.  bf16 or fp16, all alike; D a multiple of 8 up to
+    128.  ``page_table``: int32 (B, M); row j of sequence b is row ``j % page`` of page
+    ``page_table[b, j // page]``.  ``cache_seqlens``: int32 (B,), the cached rows; entries of the table
+    past them are not read.  With ``k_new``/``v_new`` ((B, H_kv, D)) the new token becomes row
+    ``cache_seqlens[b]`` first (its page must be the sequence's own) and is attended too; the caller
+    advances ``cache_seqlens`` afterwards.  Pages may otherwise be shared by sequences.
+
+    ``key_weights``: float32 (B, H_kv, N >= M * page), the attention weight each row has received: this
+    step's softmax weights, summed over the query heads of each key-value head, are added in place (for
+    a new row: set).  A head whose log-sum-exp is not finite adds nothing.
+
+    Returns ``out`` ((B, H, D), new if not given), or ``(out, lse)`` with ``return_lse=True`` (lse (B, H)
+    float32, natural log).  A length that does not fit its table, or a page id outside the pool among a
+    sequence's rows, yields NaN for that batch row (checked on the device).  ``workspace`` as for
+    :func:`decode`, of ``_C.decode_paged_workspace(B, H, H_kv, page, M, D, with_weights)`` bytes; a smaller
+    one is refused with ``key_weights`` and otherwise runs each key-value head as one workgroup.
+    """
+    _check_pages(k_pages, v_pages)
+    P, H_kv, page, D = k_pages.shape
+    dev, dtype, index = k_pages.device, k_pages.dtype, k_pages.get_device()
+    if q.dim() != 3:
+        raise RuntimeError(f"q must be (B, H, D), got {tuple(q.shape)}")
+    B, H, _ = q.shape
+    if H_kv == 0 or H % H_kv:
+        raise RuntimeError(f"q's {H} heads must be a multiple of the cache's {H_kv}")
+    _check_vec(q, "q", B, H, D, dtype, dev)
+    _check_table(page_table, "page_table", B, dev)
+    _check_seqlens(cache_seqlens, B, dev)
+    if (k_new is None) != (v_new is None):
+        raise RuntimeError("k_new and v_new must be given together")
+    if k_new is not None:
+        _check_vec(k_new, "k_new", B, H_kv, D, dtype, dev)
+        _check_vec(v_new, "v_new", B, H_kv, D, dtype, dev)
+    if out is not None:
+        _check_vec(out, "out", B, H, D, dtype, dev)
+    M = page_table.shape[1]
+    if key_weights is not None:
+        _check_weights(key_weights, "key_weights", B, H_kv, M * page, dev)
+    if out is None:
+        out = torch.empty((B, H, D), dtype=dtype, device=dev)
+    scale = (1.0 / math.sqrt(D)) if softmax_scale is None else float(softmax_scale)
+    lse = torch.empty((B, H), dtype=torch.float32, device=dev) if return_lse else None
+    if workspace is None:
+        nbytes = _C.decode_paged_workspace(B, H, H_kv, page, M, D, key_weights is not None)
+        workspace = None if torch.cuda.is_current_stream_capturing() else _WORKSPACES.get((dev, _current_stream(index)))
+        if workspace is None or workspace.numel() < nbytes:
+            workspace = _decode_workspace(dev, nbytes)
+    elif not workspace.is_cuda or workspace.device != dev or not workspace.is_contiguous():
+        raise RuntimeError(f"workspace must be a contiguous tensor on {dev}")
+    _launch_on(index, _C.decode_paged,
+               q.data_ptr(), q.stride(), k_pages.data_ptr(), k_pages.stride(), v_pages.data_ptr(), v_pages.stride(),
+               page_table.data_ptr(), page_table.stride(0), cache_seqlens.data_ptr(),
+               0 if k_new is None else k_new.data_ptr(), _ZERO3 if k_new is None else k_new.stride(),
+               0 if v_new is None else v_new.data_ptr(), _ZERO3 if v_new is None else v_new.stride(),
+               out.data_ptr(), out.stride(), 0 if lse is None else lse.data_ptr(),
+               0 if key_weights is None else key_weights.data_ptr(),
+               (0, 0) if key_weights is None else key_weights.stride()[:2],
+               B, H, H_kv, P, page, M, D, _DTYPES[dtype], scale,
+               workspace.data_ptr() if workspace.numel() else 0, workspace.numel() * workspace.element_size())
+    return (out, lse) if return_lse else out
+
+
+def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, first_query: int = 0,
+                out: torch.Tensor | None = None, softmax_scale: float | None = None, causal: bool = True):
+    """The attention weight each key receives from given queries: what a cache's ``key_weights``
+    (:func:`decode_paged`) start from after a prompt.
+
+    ``out[b, h', j]`` is the sum, over the query heads h of key-value head h' and the queries i that see key
+    j, of ``exp(scale * q[b,h,i] . k[b,h',j] - lse[b,h,i])``.  ``q``: (B, H, N_q, D), ``k``: (B, H_kv, N_k,
+    D), bf16 or fp16 views as for :func:`attention`, D a multiple of 8 up to 128, H a multiple of H_kv.
+    ``lse``: float32 (B, H, N_q) with a dense last dimension, as :func:`attention` returned it for these
+    queries.  Query i stands at position ``first_query + i`` and with ``causal`` sees the keys up to it: the
+    last w queries of a prompt of N are ``q[:, :, -w:]``, ``lse[:, :, -w:]`` with ``first_query=N - w``.
+    A query whose lse is -inf adds nothing.  Returns ``out``, float32 (B, H_kv, N_k) (new if not given; a view
+    into a cache's weights with a dense last dimension is taken).  Sums are added in a fixed order.
+    """
+    for t, n in ((q, "q"), (k, "k")):
+        if not t.is_cuda:
+            raise RuntimeError(f"{n} must be a CUDA tensor")
+        if t.dtype not in _DTYPES:
+            raise RuntimeError("Unsupported tensor dtype. Use bfloat16 or float16.")
+        if t.dim() != 4:
+            raise RuntimeError(f"{n} must be 4-D (batch, heads, seq_len, head_dim), got shape {tuple(t.shape)}")
+        if t.stride(3) != 1:
+            raise RuntimeError(f"{n} must be dense in its last dimension (stride 1), got strides {t.stride()}")
+    B, H, N_q, D = q.shape
+    H_kv, N_k, dev = k.shape[1], k.shape[2], q.device
+    if k.dtype != q.dtype:
+        raise RuntimeError(f"k must have dtype {q.dtype}, got {k.dtype}")
+    if k.device != dev:
+        raise RuntimeError(f"k must be on {dev}, got {k.device}")
+    if k.shape[0] != B or k.shape[3] != D:
+        raise RuntimeError(f"k must have shape {(B, 'H_kv', 'N_k', D)}, got {tuple(k.shape)}")
+    if not (8 <= D <= MAX_HEAD_DIM and D % 8 == 0):
+        raise RuntimeError(f"head_dim must be a multiple of 8 in [8, {MAX_HEAD_DIM}], got {D}")
+    if H_kv == 0 or H == 0 or H % H_kv:
+        raise RuntimeError(f"q's {H} heads must be a multiple of k's {H_kv}")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (B, H, N_q):
+        raise RuntimeError(f"lse must be float32 of shape {(B, H, N_q)}, got {lse.dtype} {tuple(lse.shape)}")
+    if lse.device != dev or (N_q > 1 and lse.stride(2) != 1):
+        raise RuntimeError(f"lse must be on {dev} and dense in its last dimension")
+    if first_query < 0:
+        raise RuntimeError(f"first_query must not be negative, got {first_query}")
+    if out is None:
+        out = torch.empty((B, H_kv, N_k), dtype=torch.float32, device=dev)
+    else:
+        _check_weights(out, "out", B, H_kv, N_k, dev)
+        if out.shape[2] != N_k:
+            raise RuntimeError(f"out must have shape {(B, H_kv, N_k)}, got {tuple(out.shape)}")
+    scale = (1.0 / math.sqrt(D)) if softmax_scale is None else float(softmax_scale)
+    _launch_on(q.get_device(), _C.key_weights, q.data_ptr(), q.stride(), k.data_ptr(), k.stride(),
+               lse.data_ptr(), lse.stride()[:2], out.data_ptr(), out.stride()[:2], B, H, H_kv, N_q, N_k, D,
+               _DTYPES[q.dtype], scale, bool(causal), first_query)
+    return out
+
+
+def evict(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, cache_seqlens: torch.Tensor,
+          key_weights: torch.Tensor, new_page_table: torch.Tensor, budget: int, *, recent: int = 0,
+          weights_out: torch.Tensor | None = None):
+    """Cuts each sequence of a paged cache (:func:`decode_paged`) to ``budget`` rows by attention weight.
+
+    For each sequence and key-value head the last ``recent`` of its rows stay, then those of the largest
+    ``key_weights`` (float32 (B, H_kv, N >= M * page)), ties to the lowest row; NaN ranks below every
+    number.  The ``n = min(cache_seqlens[b], budget)`` rows kept are copied, in their order, to rows
+    0 .. n - 1 of the pages that ``new_page_table`` (int32 (B, M_new), ``M_new * page >= budget``) names;
+    entries past row n are not read.  Those pages must be ones that no row still reads.  The old pages
+    are left as they were, so that other sequences may go on sharing them.  Afterwards the caller takes
+    ``new_page_table`` for the sequences' and bounds ``cache_seqlens`` by ``budget``.
+
+    Returns ``(kept, weights)``: int32 (B, H_kv, budget), the kept rows, -1 from n on, and float32 (B,
+    H_kv, budget), their weights, 0 from n on.  With ``weights_out`` (float32 (B, H_kv, at least budget); it
+    may be ``key_weights`` itself) the weights are written to its first ``budget`` columns and it is returned
+    for them.  A length that does not fit its table, or a page id outside the pool among the ones a
+    sequence needs, yields -1 and NaN, and nothing is copied for it (checked on the device).
+    """
+    _check_pages(k_pages, v_pages)
+    P, H_kv, page, D = k_pages.shape
+    dev = k_pages.device
+    B = cache_seqlens.shape[0] if cache_seqlens.dim() == 1 else -1
+    _check_seqlens(cache_seqlens, B, dev)
+    _check_table(page_table, "page_table", B, dev)
+    _check_table(new_page_table, "new_page_table", B, dev)
+    _check_weights(key_weights, "key_weights", B, H_kv, page_table.shape[1] * page, dev)
+    if not 0 <= recent <= budget:
+        raise RuntimeError(f"recent must be between 0 and budget ({budget}), got {recent}")
+    if new_page_table.shape[1] * page < budget:
+        raise RuntimeError(f"new_page_table's {new_page_table.shape[1]} pages of {page} rows do not hold "
+                           f"{budget} rows")
+    if weights_out is None:
+        weights_out = torch.empty((B, H_kv, budget), dtype=torch.float32, device=dev)
+    else:
+        _check_weights(weights_out, "weights_out", B, H_kv, budget, dev)
+    kept = torch.empty((B, H_kv, budget), dtype=torch.int32, device=dev)
+    _launch_on(k_pages.get_device(), _C.evict, k_pages.data_ptr(), k_pages.stride(), v_pages.data_ptr(),
+               v_pages.stride(), page_table.data_ptr(), page_table.stride(0), cache_seqlens.data_ptr(),
+               key_weights.data_ptr(), key_weights.stride()[:2], new_page_table.data_ptr(), new_page_table.stride(0),
+               kept.data_ptr(), weights_out.data_ptr(), weights_out.stride()[:2], B, H_kv, P, page,
+               page_table.shape[1], new_page_table.shape[1], D, budget, recent)
+    return kept, weights_out
+
+
+def _penalty(p, name: str, B: int, dev):
+    """(device pointer or 0, scalar) of a penalty given as a number or as one float32 per row."""
+    if not isinstance(p, torch.Tensor):
+        p = float(p)
+        if not math.isfinite(p) or (name == "repetition" and p <= 0):
+            raise RuntimeError(f"{name} must be finite{' and positive' if name == 'repetition' else ''}, got {p}")
+        return 0, p
+    if p.dtype != torch.float32 or tuple(p.shape) != (B,) or p.device != dev or not p.is_contiguous():
+        raise RuntimeError(f"{name} must be a number or a contiguous float32 tensor of shape ({B},) on {dev}")
+    return p.data_ptr(), 1.0
+
+
+def penalize_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, *,
+                    lengths: torch.Tensor | None = None, repetition=1.0, presence=0.0, frequency=0.0,
+                    bias: torch.Tensor | None = None, allowed: torch.Tensor | None = None,
+                    out: torch.Tensor | None = None):
+    """Penalties for repeated tokens, biases and a grammar's mask on logits, in one pass.
+
+    ``logits``: (B, V) float32, bf16 or fp16, last dimension dense.  ``tokens``: int32 or int64 (B, T), the
+    text so far, of which row b counts its first ``lengths[b]`` (int32 (B,), taken into [0, T]; all
+    without it); ids outside [0, V) count for nothing, so padding may be -1.  A token that stands n > 0
+    times in it has its logit x divided (x > 0) or multiplied (x <= 0) by ``repetition``, then lowered by
+    ``n * frequency + presence``; each of the three is a number or a float32 (B,) tensor.  ``bias``: float32
+    (V,) or (B, V), added to all.  ``allowed``: int32 (ceil(V / 32),) or (B, ceil(V / 32)) words whose bit
+    ``v % 32`` of word ``v // 32`` allows token v; the others become -inf whatever they held.
+    Arithmetic is float32 with one rounding to the logits' type.  Returns ``out`` (new if not given;
+    ``logits`` itself is taken, other overlaps are not).
+    """
+    if not logits.is_cuda:
+        raise RuntimeError("logits must be a CUDA tensor")
+    if logits.dtype not in _LOGITS:
+        raise RuntimeError("Unsupported tensor dtype. Use float32, bfloat16 or float16.")
+    if logits.dim() != 2:
+        raise RuntimeError(f"logits must be (B, V), got {tuple(logits.shape)}")
+    B, V = logits.shape
+    dev = logits.device
+    if V > 1 and logits.stride(1) != 1:
+        raise RuntimeError(f"logits must be dense in its last dimension (stride 1), got strides {logits.stride()}")
+    T = 0
+    if tokens is not None:
+        if tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() != 2 or tokens.shape[0] != B:
+            raise RuntimeError(f"tokens must be int32 or int64 of shape ({B}, T), got {tokens.dtype} "
+                               f"{tuple(tokens.shape)}")
+        T = tokens.shape[1]
+        if tokens.device != dev or (T > 1 and tokens.stride(1) != 1):
+            raise RuntimeError(f"tokens must be on {dev} and dense in its last dimension")
+    if lengths is not None:
+        if tokens is None:
+            raise RuntimeError("lengths needs tokens")
+        if lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or lengths.device != dev \
+                or not lengths.is_contiguous():
+            raise RuntimeError(f"lengths must be a contiguous int32 tensor of shape ({B},) on {dev}")
+    penalties = [_penalty(p, n, B, dev) for p, n in ((repetition, "repetition"), (presence, "presence"),
+                                                     (frequency, "frequency"))]
+    for t, n, dtype, width in ((bias, "bias", torch.float32, V), (allowed, "allowed", torch.int32, -(-V // 32))):
+        if t is not None and (t.dtype != dtype or tuple(t.shape) not in ((width,), (B, width)) or t.device != dev
+                              or (width > 1 and t.stride(-1) != 1)):
+            raise RuntimeError(f"{n} must be {dtype} of shape ({width},) or ({B}, {width}) on {dev}, dense in its "
+                               "last dimension")
+    if out is None:
+        out = torch.empty((B, V), dtype=logits.dtype, device=dev)
+    elif out.dtype != logits.dtype or out.shape != logits.shape or out.device != dev \
+            or (V > 1 and out.stride(1) != 1):
+        raise RuntimeError(f"out must be {logits.dtype} of shape {(B, V)} on {dev}, dense in its last dimension")
+    _launch_on(logits.get_device(), _C.penalize, logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0),
+               _LOGITS[logits.dtype], 0 if tokens is None else tokens.data_ptr(),
+               8 if tokens is None else tokens.element_size(), 0 if tokens is None else tokens.stride(0),
+               0 if lengths is None else lengths.data_ptr(), *(x for p in penalties for x in p),
+               0 if bias is None else bias.data_ptr(), 0 if bias is None or bias.dim() == 1 else bias.stride(0),
+               0 if allowed is None else allowed.data_ptr(),
+               0 if allowed is None or allowed.dim() == 1 else allowed.stride(0), B, V, T)
+    return out
