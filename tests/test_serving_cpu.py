@@ -98,13 +98,13 @@ def test_decode_paged_workspace(lib):
     f = lib.tfserve_decode_paged_workspace
     f.restype = ctypes.c_size_t
     assert f(1, 12, 12, 16, 4, 64, 0) == 0                          # too short to be divided
-    a, b = f(1, 12, 12, 16, 64, 64, 0), f(1, 12, 12, 16, 64, 64, 1)
-    assert 0 < a < b and b - a >= 12 * 1024 * 4                     # a score for every head and row
+    a, b = f(1, 12, 12, 16, 128, 64, 0), f(1, 12, 12, 16, 128, 64, 1)
+    assert 0 < a < b and b - a >= 12 * 2048 * 4                     # a score for every head and row
     assert f(200, 32, 32, 64, 64, 64, 0) == 0                       # sequences enough to fill the device
     for bad in ((-1, 4, 4, 16, 8, 64), (2, 4, 3, 16, 8, 64), (2, 4, 4, 0, 8, 64), (2, 4, 4, 16, 8, 60),
                 (0, 4, 4, 16, 8, 64), (2, 4, 4, 16, 0, 64)):
         assert f(*bad, 1) == 0
-    assert _C.decode_paged_workspace(1, 12, 12, 16, 64, 64, True) == b
+    assert _C.decode_paged_workspace(1, 12, 12, 16, 128, 64, True) == b
 
 
 def _weights(lib, **kw):

@@ -7,14 +7,16 @@
 //
 // Bound: HBM.  Each K and V row is read once, 4D bytes for 4DG flops.  The 16 columns of a 16x16 matrix
 // tile are the query heads of one key-value head, so that up to 16 of them cost what one does:
-//   scores   S^T[key][head] = K Q^T     v_mfma_f32_16x16x32 (element type; products exact, fp32 sums)
-//   output   O^T[dim][head] += V^T P^T  v_mfma_f32_16x16x4_f32, P and V in fp32
-// The scores leave the first product with lane (g = lane / 16, i = lane % 16) holding keys 4g .. 4g + 3 of
-// head i.  The second product takes, per instruction, one key of each g: its B operand is such a register
-// as it stands, and its A operand is one dim of that key's V row per lane, i.e. the row in its natural
-// order (lane i: kDV neighbouring dims, one per instruction).  So neither P nor V is moved between
-// lanes, and P is not rounded.  The fp32 matrix rate (256 flops a CU and cycle) is 3 times what the
-// bytes of V ask for at HBM speed.
+//   scores   S^T[key][head] = K Q^T      v_mfma_f32_16x16x32 (products exact, float32 sums)
+//   output   O^T[dim][head] += V^T P^T   the same, P as two values of the element type
+// A wave takes 32 keys at a time.  The scores leave the first product with lane (g = lane / 16, i = lane % 16)
+// holding keys 4g .. 4g + 3 of each 16 for head i; two such sets are the second product's B operand as they stand (the
+// contraction runs over keys, whose order is free).  Its A operand wants 8 keys' values of one dim in a lane:
+// the lane loads kDV neighbouring dims of each of the 8 rows, and byte permutes put the keys of a dim side by side.
+// So neither P nor V moves between lanes.  P is split as hi + lo, each rounded to the element type, which keeps 16
+// (bf16) or 22 (fp16) of its bits; rounding it once would cost as much as the output's own rounding.  An infinite V
+// makes NaN of a lo of 0 or below; a wave whose sums hold NaN takes its keys again with hi alone.  (With P and V
+// as float32 on v_mfma_f32_16x16x4_f32 a block of 32 keys took 1024 matrix cycles at D = 64 instead of 192.)
 //
 // Division of the work.  A unit is a (sequence, key-value head, 16 query heads).  The lengths are known on
 // the device only, so every workgroup works the division out from them (plan, below): one chunk length C for
@@ -27,6 +29,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "tfgfa.h"
 #include "tfgfa_arrive.h"
@@ -55,135 +58,158 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kHeads = 16;                    // query heads of a unit
 constexpr int kTile = 16;                     // keys of a matrix tile
-constexpr int kTiles = 2;                     // tiles of a wave's block
+constexpr int kTiles = 2;                     // tiles of a wave's block (one contraction of P V)
 constexpr int kBlock = kTile * kTiles;        // keys of a wave's block
 constexpr int kGranule = kWaves * kBlock;     // keys of a workgroup's block
-constexpr int kMaxParts = 1024;               // workgroups of a unit (the arrival count has 16 bits)
+constexpr int kMaxParts = 64;                 // workgroups of a unit
+// A buffer offset past any num_records built here: the load returns zero without a memory access.
+constexpr uint32_t kOutOfRange = 0x7FFFFFF0u;
+constexpr float kSlack = 8.f;
+constexpr int kScoreTail = 4;                 // a head's scores end with a place for the new row's
+constexpr int kPolicyCoherent = 16;           // buffer loads from the device's coherence point (sc1)
 
 template <class T>
 struct Elem;
 template <>
 struct Elem<__bf16> {
+  typedef __bf16 x2 __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
                                                    c, 0, 0, 0);
   }
-  static __device__ __forceinline__ float lo(uint32_t x) { return __uint_as_float(x << 16); }
-  static __device__ __forceinline__ float hi(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 };
 template <>
 struct Elem<_Float16> {
+  typedef _Float16 x2 __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c,
                                                   0, 0, 0);
   }
-  static __device__ __forceinline__ float lo(uint32_t x) {
-    return (float)__builtin_bit_cast(_Float16, (unsigned short)(x & 0xffffu));
-  }
-  static __device__ __forceinline__ float hi(uint32_t x) {
-    return (float)__builtin_bit_cast(_Float16, (unsigned short)(x >> 16));
-  }
 };
+
+// Two values of the element type in 32 bits; *rest: what rounding left of them.
+template <class T>
+__device__ __forceinline__ uint32_t pack(float x, float y, float* rx, float* ry) {
+  const typename Elem<T>::x2 z = {(T)x, (T)y};
+  *rx = x - (float)z[0];
+  *ry = y - (float)z[1];
+  return __builtin_bit_cast(uint32_t, z);
+}
+// (x.lo16, y.lo16) and (x.hi16, y.hi16): one dim of two keys side by side (v_perm_b32).
+__device__ __forceinline__ uint32_t pair_lo(uint32_t x, uint32_t y) {
+  return __builtin_amdgcn_perm(y, x, 0x05040100u);
+}
+__device__ __forceinline__ uint32_t pair_hi(uint32_t x, uint32_t y) {
+  return __builtin_amdgcn_perm(y, x, 0x07060302u);
+}
 
 // e^x as 2^(x log2 e), the difference of two scores taken first: scores up to the largest float keep their place.
 // v_exp_f32: results below 2^-126 are 0.
 __device__ __forceinline__ float exp_(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 __device__ __forceinline__ float log_(float x) { return log2f(x) * kLn2; }
 
+// Floats of a part.
+__host__ __device__ constexpr long long part_floats(int D) { return (long long)kHeads * (D + 2); }
+
 struct Args {
-  const void* q;
   const char* k;
   const char* v;
-  const int* table;
-  const int* lens;
   const void* kn;
   const void* vn;
   void* o;
   float* lse;       // natural log, or null
   char* arrive;
-  float* part;      // per workgroup of a divided unit: [head][D] outputs, then [head] LSE
+  float* part;      // per workgroup of a divided unit: [head][D] sums, then [head] their offsets, [head] of weights
   float* lse_ws;    // (B, H) LSE for the weights, or null
-  float* scores;    // (B, H, n_pad) scores, or null
+  float* scores;    // (B, H, n_pad) scores, the new row's at n_pad - kScoreTail, or null
   u64 tag;
-  long long table_stride;
   Pages ks, vs;
   Vecs qs, os, kns, vns;
   long long n_pad;
-  float scale;
-  int B, H, Hkv, G, P, page, n_max, D;
+  float scale, scale_log2;
+  float slack;      // kSlack in scores without the scale
+  int H, G, P, page, D;
   int tiles;        // 16-head tiles of a key-value head
-  int units;        // Hkv * tiles: units of one sequence
-  int target;       // workgroups per unit of a sequence that the division aims at, in all sequences (0: no division)
-  int min_granules; // smallest chunk
-  uint32_t div_m;   // j / page = j * div_m >> div_s, j < 2^31
-  int div_s;
+  int min_granules; // smallest part
 };
 
-__device__ __forceinline__ uint32_t div_page(const Args& a, uint32_t j) {
-  return (uint32_t)(((u64)j * a.div_m) >> a.div_s);
-}
+// The arguments that a kernel has before Args.  units: of one sequence, Hkv * tiles; target: parts of a unit that the
+// division aims at over all sequences (0: none are divided); j / page = j * div_m >> div_s for j < 2^31.
+struct First {
+  const int* table;
+  const int* lens;
+  long long table_stride;
+  const void* q;
+  int n_max;
+  uint32_t div_m;
+  int div_s, target, units, B;
+};
 
-// Sum of x over the lanes up to and with this one.
-__device__ __forceinline__ int scan64(int x, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
-  return x;
+// Sum of x over the lanes up to and with this one (row shifts inside 16 lanes, then the rows' ends).
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int add_dpp(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xF, false);
+}
+__device__ __forceinline__ int scan64(int x) {
+  x = add_dpp<0x111, 0xF>(x);
+  x = add_dpp<0x112, 0xF>(x);
+  x = add_dpp<0x114, 0xF>(x);
+  x = add_dpp<0x118, 0xF>(x);
+  x = add_dpp<0x142, 0xA>(x);  // lane 15 of rows 0 and 2 to the row after
+  return add_dpp<0x143, 0xC>(x);  // lane 31 to rows 2 and 3
 }
 
 struct Piece {
   int b, unit, s, S;  // sequence, unit of it, part s of S
   int first;          // the unit's first workgroup
-  int chunk;          // granules of a part
+  int len;            // cache_seqlens[b]
 };
 
-__device__ __forceinline__ int row_length(const Args& a, int n, bool append, bool* valid) {
-  const bool ok = n >= 0 && n <= a.n_max - (append ? 1 : 0);
-  *valid = ok;
-  return ok ? n + (append ? 1 : 0) : 0;
+__device__ __forceinline__ int granules(int rows) { return (rows + kGranule - 1) / kGranule; }
+
+// x / y for 0 <= x < 2^21, y > 0: the product's error, 2^-22 of it, is below the 0.5 / y that x + 0.5 is away from the
+// next quotient.  (The compiler's exact division is some 40 instructions, a microsecond for a few of them in a row.)
+__device__ __forceinline__ int quot(int x, int y) {
+  return (int)(((float)x + 0.5f) * __builtin_amdgcn_rcpf((float)y));
 }
 
-// Granules of a sequence, at least one (a workgroup has to write the empty row).
-__device__ __forceinline__ int granules(const Args& a, int b, bool append) {
-  if (b >= a.B) return 0;
-  bool valid;
-  const int n = row_length(a, a.lens[b], append, &valid);
-  return max(1, (n + kGranule - 1) / kGranule);
-}
-
-// The piece of work of workgroup w: with C = ceil(all granules / target) granules to a chunk, sequence b
-// takes ceil(granules_b / C) workgroups for each of its units, in the order of (sequence, unit, part).
-// Every wave of every workgroup computes it alike; false where no work is left.
-__device__ __forceinline__ bool plan(const Args& a, int w, int lane, bool append, Piece* out) {
-  int C = INT32_MAX;
-  if (a.target > 0) {
-    int total = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-      const int mine = granules(a, b0 + lane, append);
-      total += __builtin_amdgcn_readlane(scan64(mine, lane), 63);
-    }
-    C = max(a.min_granules, (total + a.target - 1) / a.target);
-    C = max(C, (a.n_max + kGranule * kMaxParts - 1) / (kGranule * kMaxParts));
+// The piece of work of workgroup w of a batch whose sequences are divided: with C = ceil(all granules / target)
+// granules to a part, sequence b takes ceil(granules_b / C) workgroups (one at least, to write the empty row) for each
+// of its units, in the order of (sequence, unit, part).  Every wave works it out alike; false where no work is left.
+__device__ __forceinline__ bool plan(const int* lens, int B, int most, int append, int units, int target,
+                                     int min_granules, int w, int lane, Piece* out) {
+  // Granules of a sequence of n cached rows, of which more than `most` do not fit.
+  auto of = [&](int n) { return n >= 0 && n <= most ? granules(n + append) : 0; };
+  int total = 0;
+  int n0 = 0, g0 = 0;
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    const int n = b0 + lane < B ? lens[b0 + lane] : 0;
+    const int g = of(n);
+    total += __builtin_amdgcn_readlane(scan64(g), 63);
+    if (b0 == 0) n0 = n, g0 = g;
   }
+  const int C = max(min_granules, quot(total + target - 1, target));
   int before = 0;  // parts of one unit in the sequences before
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int g = granules(a, b0 + lane, append);
-    const int S = g == 0 ? 0 : C == INT32_MAX ? 1 : (g + C - 1) / C;
-    const int upto = before + scan64(S, lane);
-    const u64 done = __builtin_amdgcn_ballot_w64((long long)upto * a.units <= w);
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    int n = n0, g = g0;
+    if (b0 > 0) {
+      n = b0 + lane < B ? lens[b0 + lane] : 0;
+      g = of(n);
+    }
+    const int S = b0 + lane < B ? max(1, min(kMaxParts, quot(g + C - 1, C))) : 0;
+    const int upto = before + scan64(S);
+    const u64 done = __builtin_amdgcn_ballot_w64(upto * units <= w);
     const int at = __builtin_popcountll(done);
-    if (at < 64 && b0 + at < a.B) {
+    if (at < 64 && b0 + at < B) {
       const int Sb = __builtin_amdgcn_readlane(S, at);
-      const int first = (__builtin_amdgcn_readlane(upto, at) - Sb) * a.units;
+      const int first = (__builtin_amdgcn_readlane(upto, at) - Sb) * units;
       const int i = w - first;
       out->b = b0 + at;
-      out->unit = i / Sb;
+      out->unit = quot(i, Sb);
       out->s = i - out->unit * Sb;
       out->S = Sb;
       out->first = first + out->unit * Sb;
-      out->chunk = C;
+      out->len = __builtin_amdgcn_readlane(n, at);
       return true;
     }
     before = __builtin_amdgcn_readlane(upto, 63);
@@ -191,18 +217,25 @@ __device__ __forceinline__ bool plan(const Args& a, int w, int lane, bool append
   return false;
 }
 
-// A block of a wave: kTiles tiles of 16 keys.  k: row i of the tile, dims 32p + 8g of piece p (the A operand
-// of the scores); v: per register r of a tile's scores the row 4g + r, dims kDV i ...
-template <int kDV>
-struct KV {
-  u32x4 k[kTiles][kDV / 2];
-  uint32_t v[kTiles][4][kDV / 2];
-  bool bad[kTiles];
-};
-
-template <int kDV>
-__device__ __forceinline__ void load_v(uint32_t (&x)[kDV / 2], const char* p) {
-  if constexpr (kDV == 8) {
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, int nbytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, nbytes, 0x00020000);
+}
+__device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
+}
+template <int kN>
+__device__ __forceinline__ void load_v(uint32_t (&x)[kN], __amdgpu_buffer_rsrc_t r, uint32_t off) {
+  if constexpr (kN == 4) {
+    const u32x4 y = load16(r, off);
+    x[0] = y[0], x[1] = y[1], x[2] = y[2], x[3] = y[3];
+  } else {
+    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 0));
+    x[0] = y[0], x[1] = y[1];
+  }
+}
+template <int kN>
+__device__ __forceinline__ void load_v(uint32_t (&x)[kN], const char* p) {
+  if constexpr (kN == 4) {
     const u32x4 y = *reinterpret_cast<const u32x4*>(p);
     x[0] = y[0], x[1] = y[1], x[2] = y[2], x[3] = y[3];
   } else {
@@ -211,257 +244,393 @@ __device__ __forceinline__ void load_v(uint32_t (&x)[kDV / 2], const char* p) {
   }
 }
 
-// kDV: dims of a lane in V, 4 (D <= 64) or 8.  kFull: D == 16 kDV.  kAligned: pages are whole tiles, so that the
-// keys of a tile are in one page.
-template <class T, int kDV, bool kFull, bool kAligned>
-__global__ __launch_bounds__(kThreads, 2) void paged_kernel(const Args a) {
+// The sum (and the largest) of x over the four lanes of a head, in all of them: lanes 16 and 32 apart, by exchanges of
+// 16-lane rows between two registers.
+template <class F>
+__device__ __forceinline__ float over_rows(float x, F f) {
+  const uint32_t a = __float_as_uint(x);
+  const auto y = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  const uint32_t b = __float_as_uint(f(__uint_as_float(y[0]), __uint_as_float(y[1])));
+  const auto z = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return f(__uint_as_float(z[0]), __uint_as_float(z[1]));
+}
+
+// The same over the 64 lanes: rotations inside 16 lanes, then their rows.
+template <class F>
+__device__ __forceinline__ float over_lanes(float x, F f) {
+  auto turn = [&](auto c) {
+    x = f(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(c)::value, 0xF, 0xF, false)));
+  };
+  turn(std::integral_constant<int, 0x121>());
+  turn(std::integral_constant<int, 0x122>());
+  turn(std::integral_constant<int, 0x124>());
+  turn(std::integral_constant<int, 0x128>());
+  return over_rows(x, f);
+}
+
+// The tables and lengths are not written while a step runs: those at uniform places come by scalar loads.
+typedef const __attribute__((address_space(4))) int* uniform_ints;
+
+// kDV: dims of a lane in V, 4 (D <= 64) or 8.  kFull: D == 16 kDV.  kSpan: keys that are sure to be in one page: a
+// block (32), a tile (16) or 1, by the page size's multiples.  kDivide: sequences may be divided (grid: flat; otherwise units by sequences).
+// The first 14 dwords of the arguments are preloaded into scalar registers (-amdgpu-kernarg-preload-count): what the
+// first loads, of the length and of the first block's pages, wait for.
+template <class T, int kDV, bool kFull, int kSpan, bool kDivide>
+__global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restrict__ table, const int* __restrict__ lens,
+                                                            long long table_stride, const T* __restrict__ q, int n_max,
+                                                            uint32_t div_m, int div_s, int target, int units, int B,
+                                                            const Args a) {
   constexpr int kDP = kDV / 2;          // pieces of 32 dims
   constexpr int kDm = 16 * kDV;
-  __shared__ float sh_o[kWaves][kHeads][kDm + 4];
+  constexpr int kRow = kDm + 4;
+  // The waves' outputs; later the shares of a unit's parts and the sums of the groups that join them.
+  constexpr int kLds = kWaves * kHeads * kRow, kLdsJoin = kHeads * kMaxParts + 4 * kThreads;
+  __shared__ __attribute__((aligned(16))) float sh_o[kLds > kLdsJoin ? kLds : kLdsJoin];
   __shared__ float sh_m[kWaves][kHeads], sh_l[kWaves][kHeads];
   __shared__ int sh_last;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, i = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const bool append = a.kn != nullptr;
+  const int append = a.kn != nullptr;
+  auto page_of = [&](int j) { return (int)(((u64)(uint32_t)j * div_m) >> div_s); };
   Piece pc;
-  if (!plan(a, blockIdx.x, lane, append, &pc)) return;
+  if (!kDivide) {
+    pc.b = blockIdx.y, pc.unit = blockIdx.x;
+    pc.s = 0, pc.S = 1;
+  } else if (B == 1) {  // part s takes granules s, s + S, ..: where it starts does not depend on the length
+    pc.b = 0;
+    pc.unit = quot(blockIdx.x, target);
+    pc.first = pc.unit * target;
+    pc.s = blockIdx.x - pc.first;
+  } else if (!plan(lens, B, n_max - append, append, units, target, a.min_granules, blockIdx.x, lane, &pc)) {
+    return;
+  }
   const int b = __builtin_amdgcn_readfirstlane(pc.b), unit = __builtin_amdgcn_readfirstlane(pc.unit);
-  const int kv = unit / a.tiles, tile = unit - kv * a.tiles;
-  const int h0 = kv * a.G + tile * kHeads;               // first query head
-  const int nh = min(kHeads, a.G - tile * kHeads);       // query heads of the unit
-  const int Lc = a.lens[b];
-  bool valid;
-  const int L = row_length(a, Lc, append, &valid);
-  const int Lr = append ? L - 1 : L;  // rows that are in the cache (-1: an invalid appending row)
-  const int D = a.D;
-  const int c0 = pc.S > 1 ? pc.s * pc.chunk * kGranule : 0;
-  const int c1 = pc.S > 1 ? min(L, c0 + pc.chunk * kGranule) : L;
-  const int* const row = a.table + (long long)b * a.table_stride;
-  u64* const aw = reinterpret_cast<u64*>(a.arrive + ((long long)b * a.units + unit) * tfgfa::kArriveStride);
-  u64 aw_start = 0;
-  if (pc.S > 1 && wave == 0)
-    aw_start = __hip_atomic_load(aw, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const int s_mine = __builtin_amdgcn_readfirstlane(pc.s);
+
+  // The first block's pages are looked up beside the length: where it starts does not depend on it.
+  const int kb0 = (s_mine * kWaves + wave) * kBlock;
+  const int* const row = table + (long long)b * table_stride;
+  constexpr int kIds = kSpan == 1 ? 1 : kBlock / kSpan;
+  auto look_up = [&](int (&id)[kIds], int at) {
+    if constexpr (kSpan > 1) {
+#pragma unroll
+      for (int c = 0; c < kIds; ++c)
+        id[c] = __builtin_amdgcn_readfirstlane(at + c * kSpan < n_max ? ((uniform_ints)row)[page_of(at + c * kSpan)] : -1);
+    } else {  // lane l: key at + l % kBlock
+      const int key = at + (lane & (kBlock - 1));
+      id[0] = key < n_max ? row[page_of(key)] : -1;
+    }
+  };
+  int ids[kIds];
+  look_up(ids, kb0);
+  const int len = kDivide && B > 1 ? __builtin_amdgcn_readfirstlane(pc.len) : ((uniform_ints)lens)[b];
+
+  // The other arguments, needed next: their loads go out with the ones above rather than where they are used.
+  asm volatile("" ::"s"(a.k), "s"(a.v), "s"(a.ks.p), "s"(a.ks.h), "s"(a.ks.n), "s"(a.vs.p), "s"(a.vs.h), "s"(a.vs.n),
+               "s"(a.qs.b), "s"(a.qs.h));
 
   // Queries: the B operand, head i, zero past the unit's heads and past D.
+  const int D = a.D;
+  const int kv = a.tiles == 1 ? unit : __builtin_amdgcn_readfirstlane(quot(unit, a.tiles)), tile = unit - kv * a.tiles;
+  const int h0 = kv * a.G + tile * kHeads;               // first query head
+  const int nh = min(kHeads, a.G - tile * kHeads);       // query heads of the unit
   u32x4 qf[kDP];
+  {
+    const __amdgpu_buffer_rsrc_t qr = rows_rsrc(q + b * a.qs.b + h0 * a.qs.h, INT32_MAX / 2);
 #pragma unroll
-  for (int p = 0; p < kDP; ++p) {
-    qf[p] = u32x4{0, 0, 0, 0};
-    if (i < nh && (kFull || 32 * p + 8 * g < D))
-      qf[p] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.q) + b * a.qs.b + (h0 + i) * a.qs.h +
-                                              32 * p + 8 * g);
+    for (int p = 0; p < kDP; ++p)
+      qf[p] = load16(qr, i < nh && (kFull || 32 * p + 8 * g < D) ? (uint32_t)(i * (int)a.qs.h * 2 + 64 * p + 16 * g)
+                                                                 : kOutOfRange);
   }
+  u64* const aw = reinterpret_cast<u64*>(a.arrive + ((long long)b * units + unit) * tfgfa::kArriveStride);
+  const bool valid = len >= 0 && len <= n_max - append;
+  const int Lr = valid ? len : 0;                        // rows that are in the cache
+  const int L = valid ? len + append : 0;                // rows attended to
+  const int S = !kDivide   ? 1
+                : B == 1 ? max(1, min(target, quot(granules(L) + a.min_granules - 1, a.min_granules)))
+                         : __builtin_amdgcn_readfirstlane(pc.S);
+  if (kDivide && s_mine >= S) return;
+  u64 aw_start = 0;
+  if (kDivide && S > 1 && wave == 0) aw_start = __hip_atomic_load(aw, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+
+  // The blocks of this wave: those of its part's cached rows, and in the unit's last wave one more for the new row,
+  // which is read from the arguments (no wave reads its place in the cache, which this one writes).
+  const int stride = S * kGranule;
+  const int after = kb0 < Lr ? granules(Lr - kb0) : 0;
+  const int blocks = S == 1 ? after : quot(after + S - 1, S);
+  const int all = blocks + (append && valid && s_mine == S - 1 && wave == kWaves - 1 ? 1 : 0);
+  struct Block {
+    int at, rows;  // first key and how many of the block's keys there are
+    bool fresh;    // the new row
+  };
+  auto block = [&](int n) {
+    const int at = kb0 + n * stride;
+    return n < blocks ? Block{at, min(kBlock, Lr - at), false} : Block{Lr, 1, true};
+  };
 
   const char* const kh = a.k + kv * a.ks.h;
   const char* const vh = a.v + kv * a.vs.h;
-  const char* const kn = append ? reinterpret_cast<const char*>(static_cast<const T*>(a.kn) + b * a.kns.b +
-                                                                kv * a.kns.h)
-                                : nullptr;
-  const char* const vn = append ? reinterpret_cast<const char*>(static_cast<const T*>(a.vn) + b * a.vns.b +
-                                                                kv * a.vns.h)
-                                : nullptr;
-
-  float m = -INFINITY, l = 0.f;
-  f32x4 acc[kDV];
+  const char* const kn = append ? reinterpret_cast<const char*>(static_cast<const T*>(a.kn) + b * a.kns.b + kv * a.kns.h) : kh;
+  const char* const vn = append ? reinterpret_cast<const char*>(static_cast<const T*>(a.vn) + b * a.vns.b + kv * a.vns.h) : vh;
+  // Loads of a block.  Rows that are not there come as zeros (kSpan > 1: past the buffer, which for the new row ends
+  // before a second one; otherwise the loads go to a row that is there, and V is cleared below); so do dims past D in K.
+  u32x4 k[kTiles][kDP];           // row i of a tile, dims 32p + 8g .. of piece p: the A operand of the scores
+  uint32_t v[kTiles][4][kDP];     // row 4g + r of a tile, dims kDV i ..
+  const uint32_t k_lane = (uint32_t)(i * (int)a.ks.n + 16 * g);
+  const uint32_t v_lane = (uint32_t)(4 * g * (int)a.vs.n + 2 * kDV * i);
+  // Rows [at, at + kSpan) of the block in page id, as a buffer of those that there are.
+  auto span = [&](const Block& x, int c, int id, const char* base, const char* fresh, const Pages& st) {
+    const bool in = (uint32_t)id < (uint32_t)a.P;
+    const int key = x.at + c * kSpan, rows = max(0, min(kSpan, x.rows - c * kSpan));
+    const u64 pid = (uint32_t)(in ? id : 0), off = (uint32_t)(key - page_of(key) * a.page);
+    const u64 where = (u64)(uintptr_t)base + pid * (u64)st.p + off * (uint32_t)st.n;
+    const u64 start = x.fresh ? (u64)(uintptr_t)fresh : where;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)start);
+    const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(start >> 32));
+    return rows_rsrc(reinterpret_cast<const char*>((u64)hi << 32 | lo),
+                     __builtin_amdgcn_readfirstlane(in || x.fresh ? rows * (int)st.n : 0));
+  };
+  // The row of key l % kBlock of the block.
+  auto one = [&](const Block& x, int id, const char* base, const char* fresh, const Pages& st) {
+    const int key = lane & (kBlock - 1);
+    const bool in = (uint32_t)id < (uint32_t)a.P && key < x.rows;
+    const u64 pid = in ? id : 0, off = in ? x.at + key - page_of(x.at + key) * a.page : 0;
+    return x.fresh ? (u64)(uintptr_t)fresh : (u64)(uintptr_t)base + pid * (u64)st.p + off * (uint32_t)st.n;
+  };
+  auto load_keys = [&](const Block& x, const int (&id)[kIds]) {
+    if constexpr (kSpan > 1) {
 #pragma unroll
-  for (int j = 0; j < kDV; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  for (int kb = c0 + wave * kBlock; kb < c1; kb += kGranule) {
-    KV<kDV> x;
-    const bool tail = kb + kBlock > Lr;  // holds the new row, or rows past the length
-    float s[kTiles][4];
-    // Loads.  Rows at or past L of a page are inside it and may be read; their values are dropped below.
-    // A tile of nothing but such rows is left out: the table need not have a page for it.
-    bool new_ok = false;
-    long long new_row_k = 0, new_row_v = 0;
-    if constexpr (kAligned) {
+      for (int c = 0; c < kIds; ++c) {
+        const __amdgpu_buffer_rsrc_t kr = span(x, c, id[c], kh, kn, a.ks);
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        const int key0 = kb + t * kTile;
-        x.bad[t] = false;
-        if (key0 < c1) {
-          const uint32_t at = div_page(a, key0);
-          int pid = __builtin_amdgcn_readfirstlane(row[at]);
-          x.bad[t] = (uint32_t)pid >= (uint32_t)a.P;
-          pid = x.bad[t] ? 0 : pid;
-          const int off = key0 - at * a.page;
-          const char* kp = kh + pid * a.ks.p + (off + i) * a.ks.n + 16 * g;
-          if (tail && append && key0 + i == Lr) {
-            new_ok = !x.bad[t];
-            new_row_k = kp - kh;
-            kp = kn + 16 * g;
-          }
+        for (int t = c * kSpan / kTile; t < (c + 1) * kSpan / kTile; ++t)
 #pragma unroll
           for (int p = 0; p < kDP; ++p)
-            x.k[t][p] = kFull || 32 * p + 8 * g < D ? *reinterpret_cast<const u32x4*>(kp + 64 * p)
-                                                    : u32x4{0, 0, 0, 0};
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const char* vp = vh + pid * a.vs.p + (off + 4 * g + r) * a.vs.n + 2 * kDV * i;
-            if (tail && append && key0 + 4 * g + r == Lr) {
-              new_row_v = vp - vh;
-              vp = vn + 2 * kDV * i;
-            }
-#pragma unroll
-            for (int e = 0; e < kDP; ++e) x.v[t][r][e] = 0;
-            if (kFull || kDV * i < D) load_v<kDV>(x.v[t][r], vp);
-          }
-        } else {
-#pragma unroll
-          for (int p = 0; p < kDP; ++p) x.k[t][p] = u32x4{0, 0, 0, 0};
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int e = 0; e < kDP; ++e) x.v[t][r][e] = 0;
-        }
+            k[t][p] = load16(kr, kFull || 32 * p + 8 * g < D
+                                     ? k_lane + (t - c * kSpan / kTile) * kTile * (uint32_t)a.ks.n + 64 * p
+                                     : kOutOfRange);
       }
     } else {
-      // Lane l looks up key kb + l % 32; the rows of the lanes' keys come from there.
-      const int key = kb + (lane & (kBlock - 1));
-      const uint32_t at = div_page(a, key);
-      int pid = -1, off = 0;
-      if (key < c1) {
-        pid = row[at];
-        off = key - at * a.page;
-        if ((uint32_t)pid >= (uint32_t)a.P) pid = -1;
-      }
+      const u64 at = one(x, id[0], kh, kn, a.ks);
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
-        const int key0 = kb + t * kTile;
-        x.bad[t] = false;
-        const int kp_id = __shfl(pid, t * kTile + i), kp_off = __shfl(off, t * kTile + i);
-        const bool is_new = append && key0 + i == Lr;
-        const char* kp = kh + max(kp_id, 0) * a.ks.p + kp_off * a.ks.n + 16 * g;
-        if (is_new) {
-          new_ok = kp_id >= 0;
-          new_row_k = kp - kh;
-          kp = kn + 16 * g;
-        }
+        const char* const kr = reinterpret_cast<const char*>(__shfl(at, t * kTile + i));
 #pragma unroll
         for (int p = 0; p < kDP; ++p)
-          x.k[t][p] = key0 + i < c1 && (kp_id >= 0 || is_new) && (kFull || 32 * p + 8 * g < D)
-                          ? *reinterpret_cast<const u32x4*>(kp + 64 * p)
-                          : u32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int k2 = key0 + 4 * g + r;
-          const int id = __shfl(pid, t * kTile + 4 * g + r), of = __shfl(off, t * kTile + 4 * g + r);
-          const char* vp = vh + max(id, 0) * a.vs.p + of * a.vs.n + 2 * kDV * i;
-          const bool new_v = append && k2 == Lr;
-          if (new_v) {
-            new_row_v = vp - vh;
-            vp = vn + 2 * kDV * i;
-          }
-          // A key of a bad page: the score below is NaN (marked by s here).
-          s[t][r] = k2 < c1 && id < 0 ? __uint_as_float(0x7FC00000u) : 0.f;
-#pragma unroll
-          for (int e = 0; e < kDP; ++e) x.v[t][r][e] = 0;
-          if (k2 < c1 && (id >= 0 || new_v) && (kFull || kDV * i < D)) load_v<kDV>(x.v[t][r], vp);
-        }
+          k[t][p] = *reinterpret_cast<const u32x4*>(kr + (kFull || 32 * p + 8 * g < D ? 64 * p + 16 * g : 0));
       }
     }
-
-    // The new row goes to its page from the lanes that hold it, in the unit's first 16 heads only.
-    if (tail && append && tile == 0 && kb <= Lr && Lr < kb + kBlock) {
-      const u64 who = __builtin_amdgcn_ballot_w64(new_ok);
-      if (who != 0) {
+  };
+  auto load_values = [&](const Block& x, const int (&id)[kIds]) {
+    if constexpr (kSpan > 1) {
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          if (kb + t * kTile + i == Lr)
+      for (int c = 0; c < kIds; ++c) {
+        const __amdgpu_buffer_rsrc_t vr = span(x, c, id[c], vh, vn, a.vs);
 #pragma unroll
-            for (int p = 0; p < kDP; ++p)
-              if (kFull || 32 * p + 8 * g < D)
-                *reinterpret_cast<u32x4*>(const_cast<char*>(kh) + new_row_k + 64 * p) = x.k[t][p];
+        for (int t = c * kSpan / kTile; t < (c + 1) * kSpan / kTile; ++t)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (kb + t * kTile + 4 * g + r == Lr && (kFull || kDV * i < D)) {
-              uint32_t* to = reinterpret_cast<uint32_t*>(const_cast<char*>(vh) + new_row_v);
-#pragma unroll
-              for (int e = 0; e < kDP; ++e) to[e] = x.v[t][r][e];
-            }
-        }
+            load_v(v[t][r], vr, kFull || kDV * i < D
+                                    ? v_lane + ((t - c * kSpan / kTile) * kTile + r) * (uint32_t)a.vs.n
+                                    : kOutOfRange);
       }
+    } else {
+      const u64 at = one(x, id[0], vh, vn, a.vs);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          load_v(v[t][r], reinterpret_cast<const char*>(__shfl(at, t * kTile + 4 * g + r)) +
+                              (kFull || kDV * i < D ? 2 * kDV * i : 0));
     }
+  };
 
-    // Scores; -inf past the length, NaN through a bad page.
+  float m, l;
+  f32x4 acc[kDV];
+  bool both = true;  // hi and lo of P
+
+  // The arithmetic of block x.  kMore: another block follows, whose K goes out once the scores have read this one's, and
+  // its V once the output has, so that one of the two is always in flight with one set of registers.
+  auto step = [&](const Block& x, const Block& y, auto more) {
+      constexpr bool kMore = decltype(more)::value;
+      int next[kIds];
+      if constexpr (kMore) look_up(next, y.at);
+      if (!kFull && kSpan == 1)
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      f32x4 c = {0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-      for (int p = 0; p < kDP; ++p) c = Elem<T>::mfma(x.k[t][p], qf[p], c);
+          for (int p = 0; p < kDP; ++p)
+            if (32 * p + 8 * g >= D) k[t][p] = u32x4{0, 0, 0, 0};
+      // The new row goes to its page from the lanes of the block's first key; without a page its score is NaN.
+      const int home = x.fresh && tile == 0 ? __builtin_amdgcn_readfirstlane(ids[0]) : -1;
+      const bool write = (uint32_t)home < (uint32_t)a.P;
+      const u64 row_in = write ? Lr - page_of(Lr) * a.page : 0;
+      if (write && i == 0) {
+        char* const to = const_cast<char*>(kh) + (u64)home * (u64)a.ks.p + row_in * (uint32_t)a.ks.n + 16 * g;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float y = c[r] * a.scale;
-        if constexpr (kAligned) {
-          if (x.bad[t]) y = __uint_as_float(0x7FC00000u);
-        } else {
-          y += s[t][r];
-        }
-        if (tail) {
-          const bool in = kb + t * kTile + 4 * g + r < L;
-          y = in ? y : -INFINITY;
-          if (!in)
-#pragma unroll
-            for (int e = 0; e < kDP; ++e) x.v[t][r][e] = 0;
-        }
-        s[t][r] = y;
+        for (int p = 0; p < kDP; ++p)
+          if (kFull || 32 * p + 8 * g < D) *reinterpret_cast<u32x4*>(to + 64 * p) = k[0][p];
       }
-      if (a.scores != nullptr && i < nh && kb + t * kTile < c1)
-        *reinterpret_cast<f32x4*>(a.scores + ((long long)b * a.H + h0 + i) * a.n_pad + kb + t * kTile + 4 * g) =
-            f32x4{s[t][0], s[t][1], s[t][2], s[t][3]};
-    }
-    // Running maximum of each head over the wave's keys.
-    float mb = s[0][0];
+      float s[kTiles][4];
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t)
+      for (int t = 0; t < kTiles; ++t) {
+        f32x4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int r = 0; r < 4; ++r) mb = fmaxf(mb, s[t][r]);
-    mb = fmaxf(mb, __shfl_xor(mb, 16));
-    mb = fmaxf(mb, __shfl_xor(mb, 32));
-    if (__builtin_amdgcn_ballot_w64(mb > m)) {
-      const float mn = fmaxf(m, mb);
-      const float f = m == -INFINITY ? 0.f : exp_(m - mn);
-      l *= f;
+        for (int p = 0; p < kDP; ++p) c = Elem<T>::mfma(k[t][p], qf[p], c);
 #pragma unroll
-      for (int j = 0; j < kDV; ++j) acc[j] *= f;
-      m = mn;
-    }
-    const float mu = m == -INFINITY ? 0.f : m;
+        for (int r = 0; r < 4; ++r) s[t][r] = c[r];
+      }
+      if constexpr (kMore) load_keys(y, next);
+      __builtin_amdgcn_sched_barrier(0);
+      // (Scores without the scale.)  NaN through a page outside the pool (a bit each of the block's spans), -inf where
+      // there is no key.
+      u64 out = 0;
+      if constexpr (kSpan > 1) {
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t)
+        for (int c = 0; c < kIds; ++c) out |= (u64)((uint32_t)ids[c] >= (uint32_t)a.P) << c;
+      } else {
+        out = __builtin_amdgcn_ballot_w64((uint32_t)ids[0] >= (uint32_t)a.P);
+      }
+      if (x.rows < kBlock || out) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float p = exp_(s[t][r] - mu);
-        l += p;
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int key = t * kTile + 4 * g + r;
+            if ((out >> (kSpan > 1 ? t * kTile / kSpan : key)) & 1u) s[t][r] = __uint_as_float(0x7FC00000u);
+            if (key >= x.rows) s[t][r] = -INFINITY;
+          }
+      }
+      if (a.scores != nullptr && i < nh) {
+        float* const to = a.scores + ((long long)b * a.H + h0 + i) * a.n_pad;
+        if (x.fresh) {
+          if (g == 0) to[a.n_pad - kScoreTail] = s[0][0] * a.scale;
+        } else {
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t)
+            if (t * kTile < x.rows)
+              *reinterpret_cast<f32x4*>(to + x.at + t * kTile + 4 * g) =
+                  f32x4{s[t][0], s[t][1], s[t][2], s[t][3]} * a.scale;
+        }
+      }
+      // The offset of each head moves only when a score passes it by kSlack (weights up to e^kSlack leave the float32
+      // sums their range), so that lanes compare notes in few blocks.
+      float mb = s[0][0];
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mb = fmaxf(mb, s[t][r]);
+      if (__builtin_amdgcn_ballot_w64(mb > m + a.slack)) {
+        mb = over_rows(mb, [](float u, float w) { return fmaxf(u, w); });
+        const float mn = fmaxf(m, mb);
+        const float f = m == -INFINITY ? 0.f : exp_((m - mn) * a.scale);
+        l *= f;
+#pragma unroll
+        for (int j = 0; j < kDV; ++j) acc[j] *= f;
+        m = mn;
+      }
+      const float mu = m == -INFINITY ? 0.f : m;
+      u32x4 hi[kTiles / 2], lo[kTiles / 2];
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+          const float p0 = __builtin_amdgcn_exp2f((s[t][r] - mu) * a.scale_log2);
+          const float p1 = __builtin_amdgcn_exp2f((s[t][r + 1] - mu) * a.scale_log2);
+          l += p0 + p1;
+          float r0, r1, none;
+          hi[t / 2][2 * (t % 2) + r / 2] = pack<T>(p0, p1, &r0, &r1);
+          lo[t / 2][2 * (t % 2) + r / 2] = pack<T>(r0, r1, &none, &none);
+        }
+      if (write && g == 0 && (kFull || kDV * i < D)) {
+        char* const to = const_cast<char*>(vh) + (u64)home * (u64)a.vs.p + row_in * (uint32_t)a.vs.n + 2 * kDV * i;
+        if constexpr (kDV == 8)
+          *reinterpret_cast<u32x4*>(to) = u32x4{v[0][0][0], v[0][0][1], v[0][0][2], v[0][0][3]};
+        else
+          *reinterpret_cast<u32x2*>(to) = u32x2{v[0][0][0], v[0][0][1]};
+      }
+      if (kSpan == 1 && x.rows < kBlock)
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (t * kTile + 4 * g + r >= x.rows)
+#pragma unroll
+              for (int e = 0; e < kDP; ++e) v[t][r][e] = 0;
+#pragma unroll
+      for (int t = 0; t < kTiles; t += 2)
 #pragma unroll
         for (int e = 0; e < kDP; ++e) {
-          acc[2 * e] = __builtin_amdgcn_mfma_f32_16x16x4f32(Elem<T>::lo(x.v[t][r][e]), p, acc[2 * e], 0, 0, 0);
-          acc[2 * e + 1] =
-              __builtin_amdgcn_mfma_f32_16x16x4f32(Elem<T>::hi(x.v[t][r][e]), p, acc[2 * e + 1], 0, 0, 0);
+          const auto& va = v[t];
+          const auto& vb = v[t + 1];
+          const u32x4 v0 = {pair_lo(va[0][e], va[1][e]), pair_lo(va[2][e], va[3][e]), pair_lo(vb[0][e], vb[1][e]),
+                            pair_lo(vb[2][e], vb[3][e])};
+          const u32x4 v1 = {pair_hi(va[0][e], va[1][e]), pair_hi(va[2][e], va[3][e]), pair_hi(vb[0][e], vb[1][e]),
+                            pair_hi(vb[2][e], vb[3][e])};
+          acc[2 * e] = Elem<T>::mfma(v0, hi[t / 2], acc[2 * e]);
+          acc[2 * e + 1] = Elem<T>::mfma(v1, hi[t / 2], acc[2 * e + 1]);
+          if (both) {
+            acc[2 * e] = Elem<T>::mfma(v0, lo[t / 2], acc[2 * e]);
+            acc[2 * e + 1] = Elem<T>::mfma(v1, lo[t / 2], acc[2 * e + 1]);
+          }
         }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (kMore) {
+        load_values(y, next);
+#pragma unroll
+        for (int c = 0; c < kIds; ++c) ids[c] = next[c];
       }
+  };
+  for (;;) {
+    m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int j = 0; j < kDV; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (all == 0) break;
+    Block x = block(0);
+    if (x.fresh) look_up(ids, Lr);
+    load_keys(x, ids);
+    load_values(x, ids);
+#pragma unroll 1
+    for (int n = 1; n < all; ++n) {
+      const Block y = block(n);
+      step(x, y, std::true_type());
+      x = y;
+    }
+    step(x, x, std::false_type());
+    float any = 0.f;  // NaN if one of the sums is
+#pragma unroll
+    for (int j = 0; j < kDV; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) any = fmaf(acc[j][r], 0.f, any);
+    if (!both || !__builtin_amdgcn_ballot_w64(any != any)) break;
+    both = false;
+    look_up(ids, kb0);
   }
-  if (pc.S > 1 && wave == 0 && lane == 0 && (aw_start >> tfgfa::kTagShift) != a.tag) {
+  if (kDivide && S > 1 && wave == 0 && lane == 0 && (aw_start >> tfgfa::kTagShift) != a.tag) {
     u64 expected = aw_start;
     __hip_atomic_compare_exchange_strong(aw, &expected, a.tag << tfgfa::kTagShift, __ATOMIC_RELAXED,
                                          __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
 
+  m *= a.scale;
   // Join the waves.  acc[j], register r of lane (g, i): dim kDV (4g + r) + j of head i.
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
+  l = over_rows(l, [](float u, float w) { return u + w; });
   if (i < nh) {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int j = 0; j < kDV; ++j) sh_o[wave][i][kDV * (4 * g + r) + j] = acc[j][r];
+      for (int j = 0; j < kDV; j += 4)
+        *reinterpret_cast<f32x4*>(&sh_o[(wave * kHeads + i) * kRow + kDV * (4 * g + r) + j]) =
+            f32x4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]};
     if (g == 0) {
       sh_m[wave][i] = m;
       sh_l[wave][i] = l;
     }
   }
   __syncthreads();
-  float* const mine = a.part + (long long)blockIdx.x * kHeads * (D + 1);
+  const long long part = part_floats(D);
+  float* const mine = a.part + blockIdx.x * part;
+  const float nan = __uint_as_float(0x7FC00000u);
   for (int e = tid; e < nh * kDm; e += kThreads) {
     const int h = e / kDm, d = e % kDm;
     if (!kFull && d >= D) continue;
@@ -474,56 +643,105 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const Args a) {
     for (int w = 0; w < kWaves; ++w) {
       const float f = exp_(sh_m[w][h] - Mu);
       lt = fmaf(f, sh_l[w][h], lt);
-      ot = fmaf(f, sh_o[w][h][d], ot);
+      ot = fmaf(f, sh_o[(w * kHeads + h) * kRow + d], ot);
     }
-    const float on = lt == 0.f ? 0.f : ot / lt;
-    const float ls = lt == 0.f ? -INFINITY : Mu + log_(lt);
-    if (pc.S == 1) {
-      const float nan = __uint_as_float(0x7FC00000u);
+    if (S > 1) {
+      __hip_atomic_store(mine + h * D + d, ot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (d < 2)
+        __hip_atomic_store(mine + (D + d) * kHeads + h, d == 0 ? M : lt, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    } else {
+      const float on = lt == 0.f ? 0.f : ot * __builtin_amdgcn_rcpf(lt);
       static_cast<T*>(a.o)[b * a.os.b + (h0 + h) * a.os.h + d] = (T)(valid ? on : nan);
-      if (d == 0) {
+      if (d == 0 && (a.lse || a.lse_ws)) {
+        const float ls = lt == 0.f ? -INFINITY : Mu + log_(lt);
         if (a.lse) a.lse[(long long)b * a.H + h0 + h] = valid ? ls : nan;
         if (a.lse_ws) a.lse_ws[(long long)b * a.H + h0 + h] = ls;
       }
-    } else {
-      __hip_atomic_store(mine + h * D + d, on, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (d == 0) __hip_atomic_store(mine + kHeads * D + h, ls, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
-  if (pc.S == 1) return;
+  if (!kDivide || S == 1) return;
   // The part is at the coherence point once its stores are acknowledged; then the arrival is counted.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0) {
     const u64 old = __hip_atomic_fetch_add(aw, (u64)1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const int last = (old & ((1ull << tfgfa::kTagShift) - 1)) == (u64)(pc.S - 1);
+    const int last = (old & ((1ull << tfgfa::kTagShift) - 1)) == (u64)(S - 1);
     if (last) __hip_atomic_store(aw, (u64)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     sh_last = last;
   }
   __syncthreads();
   if (!sh_last) return;
   asm volatile("" ::: "memory");
-  const long long step = (long long)kHeads * (D + 1);
-  const float* const parts = a.part + pc.first * step;
-  for (int e = tid; e < nh * kDm; e += kThreads) {
-    const int h = e / kDm, d = e % kDm;
-    if (!kFull && d >= D) continue;
-    float M = -INFINITY, W = 0.f, o = 0.f;
-    for (int s = 0; s < pc.S; ++s) {
-      const float ls = __hip_atomic_load(parts + s * step + kHeads * D + h, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const float os = __hip_atomic_load(parts + s * step + h * D + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const float Mn = fmaxf(M, ls);
-      const float Mu = Mn == -INFINITY ? 0.f : Mn;
-      const float f = M == -INFINITY ? 0.f : exp_(M - Mu), w = exp_(ls - Mu);
-      W = fmaf(W, f, w);
-      o = fmaf(o, f, w * os);
-      M = Mn;
+  // Join the parts (sums with offset m): their shares e^(m_s - M) / sum into LDS, a wave a head; then 4 dims a thread,
+  // the parts dealt to groups of threads whose sums are added in order.  The first parts' loads go out before the
+  // shares are known.
+  const __amdgpu_buffer_rsrc_t parts = rows_rsrc(a.part + pc.first * part, (int)(S * part * 4));
+  auto coherent = [&](int at) {
+    return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(parts, at, 0, kPolicyCoherent));
+  };
+  constexpr int kQuads = kDm / 4, kBatch = 8;
+  const int quads = nh * kQuads;
+  const int join = max(1, kThreads / quads);  // groups
+  const int grp = join > 1 ? tid / quads : 0;
+  auto fetch = [&](u32x4 (&z)[kBatch], int e, int s0) {
+    const int h = e / kQuads, d = e % kQuads * 4;
+#pragma unroll
+    for (int n = 0; n < kBatch; ++n) {
+      const int s = s0 + n * join;
+      const bool in = grp < join && e < quads && (kFull || d < D) && s < S;
+      z[n] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                           parts, in ? (s * (int)part + h * D + d) * 4 : (int)kOutOfRange, 0,
+                                           kPolicyCoherent));
     }
-    const float ls = W == 0.f ? -INFINITY : M + log_(W);
-    static_cast<T*>(a.o)[b * a.os.b + (h0 + h) * a.os.h + d] = (T)(W == 0.f ? 0.f : o / W);
-    if (d == 0) {
-      if (a.lse) a.lse[(long long)b * a.H + h0 + h] = ls;
-      if (a.lse_ws) a.lse_ws[(long long)b * a.H + h0 + h] = ls;
+  };
+  u32x4 z[kBatch];
+  fetch(z, join > 1 ? tid - grp * quads : tid, grp);
+  float* const share = sh_o;                      // [head][S], at most kHeads * kMaxParts
+  float* const sums = sh_o + kHeads * kMaxParts;  // [group][quads] of 4, at most kThreads * 4
+  static_assert(kMaxParts <= 64, "a lane a part");
+  for (int h = wave; h < nh; h += kWaves) {
+    const int at = lane < S ? (lane * (int)part + D * kHeads + h) * 4 : (int)kOutOfRange;
+    const float ms = coherent(at), ls = coherent(at + kHeads * 4);
+    const float M = over_lanes(lane < S ? ms : -INFINITY, [](float u, float w) { return fmaxf(u, w); });
+    const float Mu = M == -INFINITY ? 0.f : M;
+    const float f = lane < S ? exp_(ms - Mu) : 0.f;
+    const float W = over_lanes(f * ls, [](float u, float w) { return u + w; });
+    if (lane < S) share[h * S + lane] = W == 0.f ? 0.f : f * __builtin_amdgcn_rcpf(W);
+    if (lane == 0 && (a.lse || a.lse_ws)) {
+      const float z = W == 0.f ? -INFINITY : Mu + log_(W);
+      if (a.lse) a.lse[(long long)b * a.H + h0 + h] = z;
+      if (a.lse_ws) a.lse_ws[(long long)b * a.H + h0 + h] = z;
+    }
+  }
+  __syncthreads();
+  for (int e0 = 0; e0 < quads; e0 += kThreads) {
+    const int e = join > 1 ? tid - grp * quads : e0 + tid;
+    const int h = e / kQuads, d = e % kQuads * 4;
+    const bool in = grp < join && e < quads && (kFull || d < D);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = grp; s0 < S; s0 += kBatch * join) {
+      if (e0 > 0 || s0 >= join) fetch(z, e, s0);
+#pragma unroll
+      for (int n = 0; n < kBatch; ++n) {
+        const int s = s0 + n * join;
+        if (in && s < S) {
+          const float w = share[h * S + s];
+          // A part of no weight adds nothing (its output may be infinite).
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[c] = w == 0.f ? o[c] : fmaf(w, __uint_as_float(z[n][c]), o[c]);
+        }
+      }
+    }
+    if (join > 1) {
+      if (grp < join) *reinterpret_cast<f32x4*>(sums + tid * 4) = o;
+      __syncthreads();
+      if (grp != 0) return;
+      for (int k = 1; k < join; ++k) o += *reinterpret_cast<const f32x4*>(sums + (k * quads + e) * 4);
+    }
+    if (in) {
+      T* const to = static_cast<T*>(a.o) + b * a.os.b + (h0 + h) * a.os.h + d;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) to[c] = (T)o[c];
     }
   }
 }
@@ -537,40 +755,46 @@ __global__ __launch_bounds__(256) void add_weights_kernel(const float* __restric
                                                           long long n_pad, int H, int G, int P, int page,
                                                           int n_max, int append) {
   const int b = blockIdx.z, kv = blockIdx.y;
-  const int Lc = lens[b];
-  if (Lc < 0 || Lc > n_max - append) return;
-  const int L = Lc + append;
+  const int L = lens[b];
+  if (L < 0 || L > n_max - append) return;
   const int j0 = (blockIdx.x * 256 + threadIdx.x) * 4;
-  if (j0 >= L) return;
-  float w[4] = {0.f, 0.f, 0.f, 0.f};
   const long long first = (long long)b * H + kv * G;
-  for (int h = 0; h < G; ++h) {
-    const float z = lse_ws[first + h];
-    if (!(fabsf(z) < INFINITY)) continue;
-    const f32x4 x = *reinterpret_cast<const f32x4*>(scores + (first + h) * n_pad + j0);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] += exp_(x[e] - z);
-  }
   float* const to = weights + b * wb + kv * wh;
+  if (j0 < L) {
+    float w[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int h = 0; h < G; ++h) {
+      const float z = lse_ws[first + h];
+      if (!(fabsf(z) < INFINITY)) continue;
+      const f32x4 x = *reinterpret_cast<const f32x4*>(scores + (first + h) * n_pad + j0);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int j = j0 + e;
-    if (j < Lc)
-      to[j] += w[e];
-    else if (j < L && (uint32_t)table[(long long)b * table_stride + j / page] < (uint32_t)P)
-      to[j] = w[e];
+      for (int e = 0; e < 4; ++e) w[e] += exp_(x[e] - z);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (j0 + e < L) to[j0 + e] += w[e];
+  }
+  if (append && j0 == 0 && (uint32_t)table[(long long)b * table_stride + L / page] < (uint32_t)P) {
+    float w = 0.f;
+    for (int h = 0; h < G; ++h) {
+      const float z = lse_ws[first + h];
+      if (fabsf(z) < INFINITY) w += exp_(scores[(first + h + 1) * n_pad - kScoreTail] - z);
+    }
+    to[L] = w;
   }
 }
 
 // ---------------------------------------------------------------------------------------
 // Host side.
 
-// A workgroup's chunk: about kSlots workgroups a CU, no chunk below kMinGranules.
+// About kSlots workgroups a CU.
 constexpr int kSlots = 2;
-constexpr int kMinGranules = 2;
+// Sequences of at most kWhole rows are not divided.
+constexpr int kWhole = 512;
+// A part writes and reads back its heads' outputs: a granule's worth of K and V for every 16 heads' 4 granules.
+static int min_granules(int G) { return std::max(1, std::min(kHeads, G) / 4); }
 constexpr int kMaxCu = 1024;  // for the workspace's size, which does not depend on the device
 
-static long long padded(long long n) { return (n + kGranule - 1) / kGranule * kGranule; }
+static long long padded(long long n) { return (n + kGranule - 1) / kGranule * kGranule + kScoreTail; }
 
 // Parts of the workspace for `wgs` workgroups and `units` units: arrival words, parts, LSE, scores.
 struct Layout {
@@ -579,7 +803,7 @@ struct Layout {
 static Layout layout(long long units, long long wgs, long long bh, long long n_max, int D, bool weights) {
   Layout x;
   x.part = tfgfa::arrive_bytes(units);
-  x.lse_ws = x.part + ((size_t)wgs * kHeads * (D + 1) * 4 + 255) / 256 * 256;
+  x.lse_ws = x.part + ((size_t)wgs * part_floats(D) * 4 + 255) / 256 * 256;
   x.scores = x.lse_ws + (weights ? ((size_t)bh * 4 + 255) / 256 * 256 : 0);
   x.bytes = x.scores + (weights ? (size_t)bh * padded(n_max) * 4 : 0);
   return x;
@@ -589,11 +813,16 @@ static Layout layout(long long units, long long wgs, long long bh, long long n_m
 // unit.  No division (target 0) where there are units enough, or where sequences are short.
 static int choose_target(long long units, int B, long long n_max, int cu_count) {
   const long long per = units * B;
-  if (n_max <= kMinGranules * kGranule || per >= (long long)kSlots * 2 * cu_count) return 0;
-  return (int)std::max(1LL, (long long)kSlots * cu_count / units);
+  // (Past 2^21 granules the plan's quotients are not exact.)
+  if (n_max <= kWhole || per >= (long long)kSlots * 2 * cu_count || (n_max / kGranule + 1) * B >= 1 << 20)
+    return 0;
+  const long long target = std::max(1LL, (long long)kSlots * cu_count / units);
+  if (B > 1) return (int)target;
+  return (int)std::min<long long>(std::min<long long>(target, kMaxParts), (n_max + kGranule - 1) / kGranule);
 }
 static long long workgroups(long long units, int B, long long n_max, int target) {
   if (target == 0) return units * B;
+  if (B == 1) return units * target;
   const long long most = (n_max + kGranule - 1) / kGranule;  // parts of a unit
   return units * std::min<long long>((long long)B * std::max(1LL, most), (long long)target + B);
 }
@@ -604,25 +833,36 @@ static bool sizes_ok(int B, int H, int Hkv, int page, int M, int D) {
   return true;
 }
 
-template <class T>
-static void launch(const Args& a, unsigned grid, hipStream_t stream) {
-  const bool aligned = a.page % kTile == 0;
-#define TFGFA_PAGED(kDV, kFull, kAligned) \
-  hipLaunchKernelGGL((paged_kernel<T, kDV, kFull, kAligned>), dim3(grid), dim3(kThreads), 0, stream, a)
-  if (a.D == 64) {
-    if (aligned) TFGFA_PAGED(4, true, true);
-    else TFGFA_PAGED(4, true, false);
-  } else if (a.D < 64) {
-    if (aligned) TFGFA_PAGED(4, false, true);
-    else TFGFA_PAGED(4, false, false);
-  } else if (a.D == 128) {
-    if (aligned) TFGFA_PAGED(8, true, true);
-    else TFGFA_PAGED(8, true, false);
-  } else {
-    if (aligned) TFGFA_PAGED(8, false, true);
-    else TFGFA_PAGED(8, false, false);
-  }
+template <class T, int kDV, bool kFull>
+static void launch_full(const First& f, const Args& a, unsigned wgs, hipStream_t stream) {
+  const dim3 grid = f.target ? dim3(wgs) : dim3(f.units, f.B);
+#define TFGFA_PAGED_(kSpan, kDivide) \
+  hipLaunchKernelGGL((paged_kernel<T, kDV, kFull, kSpan, kDivide>), grid, dim3(kThreads), 0, stream, f.table, f.lens, \
+                     f.table_stride, static_cast<const T*>(f.q), f.n_max, f.div_m, f.div_s, f.target, f.units, f.B, a)
+#define TFGFA_PAGED(kSpan)                 \
+  do {                                     \
+    if (f.target) TFGFA_PAGED_(kSpan, true); \
+    else TFGFA_PAGED_(kSpan, false);       \
+  } while (0)
+  if (a.page % kBlock == 0)
+    TFGFA_PAGED(kBlock);
+  else if (a.page % kTile == 0)
+    TFGFA_PAGED(kTile);
+  else
+    TFGFA_PAGED(1);
 #undef TFGFA_PAGED
+#undef TFGFA_PAGED_
+}
+template <class T>
+static void launch(const First& f, const Args& a, unsigned wgs, hipStream_t stream) {
+  if (a.D == 64)
+    launch_full<T, 4, true>(f, a, wgs, stream);
+  else if (a.D < 64)
+    launch_full<T, 4, false>(f, a, wgs, stream);
+  else if (a.D == 128)
+    launch_full<T, 8, true>(f, a, wgs, stream);
+  else
+    launch_full<T, 8, false>(f, a, wgs, stream);
 }
 
 }  // namespace tfgfa_paged
@@ -659,17 +899,22 @@ extern "C" int tfserve_decode_paged(
   if (P == 0) return TFGFA_ERR_BAD_SHAPE;
   const long long n_max = (long long)M * page;
   Args a = {};
+  First f = {};
   a.tiles = (H / H_kv + kHeads - 1) / kHeads;
   const long long units = (long long)H_kv * a.tiles;
-  // Granules of the whole batch and workgroups are counted in 32 bits; so are key indexes, with room for a block.
-  if (n_max > INT32_MAX - kGranule || units * B > INT32_MAX / 4 || (long long)B * H > INT32_MAX ||
-      (n_max / kGranule + 1) * B > INT32_MAX)
+  // Granules of the whole batch and workgroups are counted in 32 bits; so are key indexes, with room for the blocks
+  // that a loop looks ahead.
+  if (n_max > INT32_MAX - 128 * kMaxParts * kGranule || B > 65535 || units >= 1 << 20 || (long long)B * H > INT32_MAX ||
+      units * B > INT32_MAX)
     return TFGFA_ERR_TOO_LARGE;
   if (!q_strides || !k_strides || !v_strides || !o_strides) return TFGFA_ERR_NULL_POINTER;
   if (append && (!k_new_strides || !v_new_strides)) return TFGFA_ERR_NULL_POINTER;
   if (!vecs_ok(q_strides, B, H, &a.qs) || !vecs_ok(o_strides, B, H, &a.os) ||
       !pages_ok(k_strides, P, H_kv, page, D, &a.ks) || !pages_ok(v_strides, P, H_kv, page, D, &a.vs))
     return TFGFA_ERR_STRIDE;
+  // A block's rows, and a unit's queries, are one buffer of less than 2^30 bytes.
+  if (a.ks.n >= (1 << 30) / kBlock || a.vs.n >= (1 << 30) / kBlock || 2 * a.qs.h >= (1 << 30) / kHeads)
+    return TFGFA_ERR_TOO_LARGE;
   if (append && (!vecs_ok(k_new_strides, B, H_kv, &a.kns) || !vecs_ok(v_new_strides, B, H_kv, &a.vns)))
     return TFGFA_ERR_STRIDE;
   if (!apart(a.os.b, B, a.os.h, H, D)) return TFGFA_ERR_STRIDE;
@@ -685,52 +930,52 @@ extern "C" int tfserve_decode_paged(
     if (!weights_strides) return TFGFA_ERR_NULL_POINTER;
     wb = weights_strides[0], wh = weights_strides[1];
     if (!apart(wb, B, wh, H_kv, n_max)) return TFGFA_ERR_STRIDE;
-    if (B > 65535 || H_kv > 65535) return TFGFA_ERR_TOO_LARGE;
+    if (H_kv > 65535) return TFGFA_ERR_TOO_LARGE;
   }
 
   int cu = 0;
   const int st = tfgfa_device_info(&cu, nullptr, nullptr, 0);
   if (st != TFGFA_OK) return st;
   const bool weights = key_weights != nullptr && n_max > 0;
-  a.target = choose_target(units, B, n_max, std::min(cu, kMaxCu));
-  long long wgs = workgroups(units, B, n_max, a.target);
-  Layout lay = layout(units * B, a.target ? wgs : 0, (long long)B * H, n_max, D, weights);
+  f.target = choose_target(units, B, n_max, std::min(cu, kMaxCu));
+  long long wgs = workgroups(units, B, n_max, f.target);
+  Layout lay = layout(units * B, f.target ? wgs : 0, (long long)B * H, n_max, D, weights);
   if (lay.bytes > (workspace ? workspace_bytes : 0)) {
     if (weights) return TFGFA_ERR_SCRATCH;
     // Without a workspace that holds the division, each unit is one workgroup's.
-    a.target = 0;
+    f.target = 0;
     wgs = workgroups(units, B, n_max, 0);
   }
   if (wgs > INT32_MAX) return TFGFA_ERR_TOO_LARGE;
   char* const ws = static_cast<char*>(workspace);
-  a.q = q, a.k = static_cast<char*>(k_pages), a.v = static_cast<char*>(v_pages);
-  a.table = page_table, a.table_stride = B > 1 ? table_stride : 0, a.lens = cache_seqlens;
+  f.table = page_table, f.table_stride = B > 1 ? table_stride : 0, f.lens = cache_seqlens, f.q = q;
+  f.n_max = (int)n_max, f.units = (int)units, f.B = B;
+  a.k = static_cast<char*>(k_pages), a.v = static_cast<char*>(v_pages);
   a.kn = k_new, a.vn = v_new, a.o = o, a.lse = lse;
   a.arrive = ws;
   a.part = ws ? reinterpret_cast<float*>(ws + lay.part) : nullptr;
   a.lse_ws = weights ? reinterpret_cast<float*>(ws + lay.lse_ws) : nullptr;
   a.scores = weights ? reinterpret_cast<float*>(ws + lay.scores) : nullptr;
-  a.tag = a.target ? tfgfa::next_tag() : 0;
+  a.tag = f.target ? tfgfa::next_tag() : 0;
   a.n_pad = padded(n_max);
-  a.scale = softmax_scale;
-  a.B = B, a.H = H, a.Hkv = H_kv, a.G = H / H_kv, a.P = P, a.page = page, a.n_max = (int)n_max, a.D = D;
-  a.units = (int)units;
-  a.min_granules = kMinGranules;
+  a.scale = softmax_scale, a.scale_log2 = softmax_scale * kLog2e, a.slack = std::min(kSlack / softmax_scale, 1e30f);
+  a.H = H, a.G = H / H_kv, a.P = P, a.page = page, a.D = D;
+  a.min_granules = min_granules(a.G);
   // j / page by a product: with 2^(l-1) < page <= 2^l and m = floor(2^(31+l) / page) + 1 the error j (m page -
   // 2^(31+l)) / 2^(31+l) is below 1 / page for j < 2^31, and m < 2^32.
   int lg = 0;
   while ((1LL << lg) < page) ++lg;
-  a.div_m = (uint32_t)((1ULL << (31 + lg)) / (uint64_t)page + 1);
-  a.div_s = 31 + lg;
+  f.div_m = (uint32_t)((1ULL << (31 + lg)) / (uint64_t)page + 1);
+  f.div_s = 31 + lg;
   const hipStream_t stream = (hipStream_t)hip_stream;
   if (dtype == TFGFA_DTYPE_BF16)
-    launch<__bf16>(a, (unsigned)wgs, stream);
+    launch<__bf16>(f, a, (unsigned)wgs, stream);
   else
-    launch<_Float16>(a, (unsigned)wgs, stream);
+    launch<_Float16>(f, a, (unsigned)wgs, stream);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && weights) {
     hipLaunchKernelGGL(add_weights_kernel, dim3((unsigned)((n_max + 1023) / 1024), H_kv, B), dim3(256), 0, stream,
-                       a.scores, a.lse_ws, cache_seqlens, page_table, a.table_stride, key_weights, wb, wh, a.n_pad,
+                       a.scores, a.lse_ws, cache_seqlens, page_table, f.table_stride, key_weights, wb, wh, a.n_pad,
                        H, a.G, P, page, (int)n_max, append ? 1 : 0);
     e = hipGetLastError();
   }
