@@ -135,7 +135,7 @@ def _weights(lib, **kw):
     (dict(ls=(-1000, 10)), "ERR_STRIDE"),
     (dict(q=P + 4), "ERR_ALIGNMENT"),
     (dict(out=P + 2), "ERR_ALIGNMENT"),
-    (dict(B=70000), "ERR_TOO_LARGE"),
+    (dict(B=1 << 20), "ERR_TOO_LARGE"),
 ])
 def test_key_weights_refuses(lib, kw, code):
     assert _weights(lib, **kw) == _code(code)

@@ -2,20 +2,26 @@
 //     c_j = sum_h sum_i [j <= first + i] e^(scale q_hi . k_j - lse_hi)
 // over the query heads h of a key-value head, with the log-sum-exp of the attention that ran before.
 //
-// Bound: the exponentials.  A pair of query and key costs 2D flops on the matrix units (64 cycles a 32x32
-// tile and 32 dims) and one v_exp_f32, one v_fma and one v_add on the VALU, the first at a quarter of the rate:
-// about 384 cycles a tile against 128 at D = 64.
+// Bound: the exponentials.  A pair of query and key costs 2D flops on the matrix units (128 cycles a 32x32 tile at D =
+// 64) and a v_fma, a v_exp_f32 and a v_add on the VALU (16 x 15 cycles a tile).
 //
 // S^T[key][query] = K Q^T as v_mfma_f32_32x32x16 tiles: lane l holds 16 keys of query l % 32, so that the
 // query's lse is one register, the sums over queries stay in 16 registers of each lane, and lanes are
-// added once at the end.  A workgroup owns 32 keys of one key-value head, whose K rows stay in registers; its
-// waves take the (query head, 32 queries) tiles in turn, and their sums are added in wave order.
+// added once at the end.  A wave owns 32 keys of one key-value head, whose K rows stay in registers; the four waves of a
+// workgroup share tiles of 64 queries, which come through two LDS buffers by direct loads, the next tile's under this
+// one's arithmetic (an operand read straight from memory touches 32 rows an instruction, 32 bytes of each).
+// Under a causal mask the first keys are seen by most queries.  Their workgroups come first; where several share a CU,
+// every other round of workgroups over the CUs runs backwards, so that a CU's long and short ones add up alike (16 heads
+// of 8192 queries and keys: 1024 workgroups, all resident, of which one CU had 160 parts and another 100).
 #include <hip/hip_runtime.h>
 
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "tfgfa.h"
+#include "tfgfa_device.h"
 #include "tfgfa_layout.h"
 #include "tfgfa_serving.h"
 
@@ -32,8 +38,11 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxD = 128;
-constexpr int kTile = 32;
+constexpr int kTile = 32;              // keys of a wave, queries of a matrix tile
 constexpr int kWaves = 4;
+constexpr int kKeys = kTile * kWaves;  // keys of a workgroup
+constexpr int kQueries = 64;           // queries of an LDS buffer
+constexpr int kOutOfRange = 0x7FFFFFF0;  // a buffer offset past any num_records: the load gives zeros
 
 template <class T>
 __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c);
@@ -57,73 +66,148 @@ struct Args {
   long long lb, lh, ob, oh;
   long long first;
   float scale_log2;
-  int G, Nq, Nk, D, causal;
+  int Hkv, units, cu, G, Nq, Nk, D, causal;
 };
+
+// Rows of queries in LDS: kChunks chunks of 16 bytes, chunk c of row r at place c ^ turn(r), so that the rows of a
+// chunk that a read takes together lie in different banks.
+template <int kChunks>
+__device__ __forceinline__ int turn(int row) {
+  return kChunks == 8 ? tfgfa::swz_k(row) : row & 15;
+}
 
 // kP: pieces of 16 dims, D <= 16 kP; a lane holds dims 16p + 8 (l / 32) .. + 7 of row l % 32.
 template <class T, int kP>
-__global__ __launch_bounds__(64 * kWaves) void weights_kernel(const Args a) {
-  __shared__ float sums[kWaves][kTile];
+__global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(const Args a) {
+  constexpr int kChunks = 2 * kP, kRowBytes = 16 * kChunks, kBytes = kQueries * kRowBytes;
+  constexpr int kMoves = kBytes / 1024 / kWaves;  // 1-KiB transfers of a wave
+  __shared__ __attribute__((aligned(1024))) unsigned char buf[2][kBytes];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, i = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kv = blockIdx.y, b = blockIdx.z, j0 = blockIdx.x * kTile;
+  int id = blockIdx.x;
+  if (a.causal && id / a.cu % 2 != 0) {
+    const int first = id / a.cu * a.cu;
+    id = first + min(first + a.cu, (int)gridDim.x) - 1 - id;
+  }
+  const int y = id / a.units, unit = id - y * a.units;
+  const int b = unit / a.Hkv, kv = unit - b * a.Hkv;
+  const int jw = y * kKeys, j0 = jw + wave * kTile;  // first key of the workgroup, of the wave
   u32x4 kf[kP];
   const T* const kr = static_cast<const T*>(a.k) + b * a.ks.b + kv * a.ks.h + (long long)(j0 + i) * a.ks.n + 8 * half;
 #pragma unroll
   for (int p = 0; p < kP; ++p)
     kf[p] = j0 + i < a.Nk && 16 * p + 8 * half < a.D ? *reinterpret_cast<const u32x4*>(kr + 16 * p)
                                                      : u32x4{0, 0, 0, 0};
-  // First tile of queries that see a key of this workgroup.
-  const int tiles = (a.Nq + kTile - 1) / kTile;
+  // Tiles of queries that see a key of this workgroup, for each of the head's query heads in turn.
+  const int tiles = (a.Nq + kQueries - 1) / kQueries;
   int t0 = 0;
-  if (a.causal && j0 > a.first) t0 = (int)min((long long)tiles, (j0 - a.first) / kTile);
-  const int per = tiles - t0;
+  if (a.causal && jw > a.first) t0 = (int)min((long long)tiles, (jw - a.first) / kQueries);
+  const int per = tiles - t0, all = per * a.G;
+
+  const uint32_t at = tfgfa::lds_addr(&buf[0][0]);
+  const int row_bytes = (int)a.qs.n * 2;
+  float z[2], next[2];  // lse of the lane's query of each half of a tile; past the last query 0
+  // The next tile's queries and their lse, and how many there are from it on in this head.
+  const T* q = static_cast<const T*>(a.q) + b * a.qs.b + kv * a.G * a.qs.h + (long long)t0 * kQueries * a.qs.n;
+  const float* lse = a.lse + b * a.lb + kv * a.G * a.lh + t0 * kQueries;
+  const int left0 = a.Nq - t0 * kQueries;
+  const long long q_tile = kQueries * a.qs.n;
+  const long long q_head = a.qs.h - (long long)per * q_tile, lse_head = a.lh - (long long)per * kQueries;
+  int left = left0;
+  // The next tile into buffer n: lane l of a transfer writes 16 bytes at 16 l of its KiB.
+  auto load = [&](int n) {
+    const int rows = min(kQueries, left);
+    const __amdgpu_buffer_rsrc_t z = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(lse), (short)0, rows * 4,
+                                                                       0x00020000);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      next[u] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(z, (u * kTile + i) * 4, 0, 0));
+    const tfgfa::i32x4 desc = tfgfa::head_desc(q, rows, row_bytes);
+#pragma unroll
+    for (int m = 0; m < kMoves; ++m) {
+      const int first = (wave * kMoves + m) * (64 / kChunks), row = first + lane / kChunks;
+      const int chunk = (lane & (kChunks - 1)) ^ turn<kChunks>(row);
+      tfgfa::lds_transfer(desc, __builtin_amdgcn_readfirstlane(at + n * kBytes + first * kRowBytes),
+                          8 * chunk < a.D ? row * row_bytes + 16 * chunk : kOutOfRange);
+    }
+    q += q_tile, lse += kQueries, left -= kQueries;
+    if (left <= 0) q += q_head, lse += lse_head, left = left0;
+  };
+
   float sum[16];
 #pragma unroll
   for (int r = 0; r < 16; ++r) sum[r] = 0.f;
-  for (int w = wave; w < per * a.G; w += kWaves) {
-    const int g = w / per, t = t0 + (w - g * per), h = kv * a.G + g, q0 = t * kTile;
-    const bool in = q0 + i < a.Nq;
-    const T* const qr = static_cast<const T*>(a.q) + b * a.qs.b + h * a.qs.h + (long long)(q0 + i) * a.qs.n + 8 * half;
-    u32x4 qf[kP];
+  // The scale as a vector register: a v_fma with a scalar operand takes half as long again.
+  float scale = a.scale_log2;
+  asm("" : "+v"(scale));
+  // Tiles from `from` to `upto` are seen whole by the wave's keys.
+  int from = 0;
+  if (a.causal && j0 + kTile - 1 > a.first)
+    from = (int)min((long long)tiles, (j0 + kTile - 1 - a.first + kQueries - 1) / kQueries);
+  const int upto = a.Nq / kQueries;
+  int t = t0;
+  if (all > 0) load(0);
+#pragma unroll 1
+  for (int w = 0; w < all; ++w) {
+    const int n = w & 1;
+    tfgfa::wait_vmcnt<0>();
+    __syncthreads();
+    z[0] = next[0] * kLog2e, z[1] = next[1] * kLog2e;
+    if (w + 1 < all) load(n ^ 1);
+    f32x16 s[2];
 #pragma unroll
-    for (int p = 0; p < kP; ++p)
-      qf[p] = in && 16 * p + 8 * half < a.D ? *reinterpret_cast<const u32x4*>(qr + 16 * p) : u32x4{0, 0, 0, 0};
-    // Keys of the tile that this lane's query sees: up to `last`.  A row past the last, and one with nothing to
-    // see (lse -inf, or past the range in the log2 domain), sees none.
-    float z = in ? a.lse[b * a.lb + h * a.lh + q0 + i] * kLog2e : INFINITY;
-    const bool live = z != INFINITY && z != -INFINITY;
-    z = live ? z : 0.f;
-    int last = kTile - 1;
-    if (a.causal) last = (int)max(-1LL, min((long long)last, a.first + q0 + i - j0));
-    if (!live) last = -1;
-    f32x16 s;
+    for (int u = 0; u < 2; ++u) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+      for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+      const unsigned char* const row = &buf[n][(u * kTile + i) * kRowBytes];
 #pragma unroll
-    for (int p = 0; p < kP; ++p) s = mfma<T>(kf[p], qf[p], s);
-    // Register r: key 8 (r / 4) + 4 half + r % 4 of the tile, query i.
-    const bool edge = __builtin_amdgcn_ballot_w64(last < kTile - 1) != 0;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2, -z));
-      if (edge) p = 8 * (r / 4) + 4 * half + r % 4 <= last ? p : 0.f;
-      sum[r] += p;
+      for (int p = 0; p < kP; ++p)
+        s[u] = mfma<T>(kf[p], *reinterpret_cast<const u32x4*>(row + 16 * ((2 * p + half) ^ turn<kChunks>(u * kTile + i))),
+                       s[u]);
     }
+    // Register r: key 8 (r / 4) + 4 half + r % 4 of the wave's, query i.
+    const bool clear = t >= from && t < upto;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const bool live = fabsf(z[u]) != INFINITY;
+      if (clear && !__builtin_amdgcn_ballot_w64(!live)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[r] += __builtin_amdgcn_exp2f(fmaf(s[u][r], scale, -z[u]));
+      } else {
+        // Keys that the lane's query sees: up to `last`.  A row past the last, and one with nothing to see (lse -inf, or
+        // past the range in the log2 domain), sees none.
+        const int query = t * kQueries + u * kTile + i;
+        int last = kTile - 1;
+        if (a.causal) last = (int)max(-1LL, min((long long)last, a.first + query - j0));
+        if (!live || query >= a.Nq) last = -1;
+        const float zu = live ? z[u] : 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[u][r], scale, -zu));
+          sum[r] += 8 * (r / 4) + 4 * half + r % 4 <= last ? p : 0.f;
+        }
+      }
+    }
+    if (++t == tiles) t = t0;
   }
+  // Over the 32 queries of each half: rotations inside 16 lanes, then the two 16s.  Lane i < 16 keeps register i.
+  float x = 0.f;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) sum[r] += __shfl_xor(sum[r], o);
-    if (i == 0) sums[wave][8 * (r / 4) + 4 * half + r % 4] = sum[r];
+    float y = sum[r];
+    auto add = [&](auto c) {
+      y += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(y), decltype(c)::value, 0xF, 0xF, false));
+    };
+    add(std::integral_constant<int, 0x121>());
+    add(std::integral_constant<int, 0x122>());
+    add(std::integral_constant<int, 0x124>());
+    add(std::integral_constant<int, 0x128>());
+    const auto two = __builtin_amdgcn_permlane16_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+    y = __uint_as_float(two[0]) + __uint_as_float(two[1]);
+    x = i == r ? y : x;
   }
-  __syncthreads();
-  if (tid < kTile && j0 + tid < a.Nk) {
-    float x = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) x += sums[w][tid];
-    a.out[b * a.ob + kv * a.oh + j0 + tid] = x;
-  }
+  const int j = j0 + 8 * (i / 4) + 4 * half + i % 4;
+  if (i < 16 && j < a.Nk) a.out[b * a.ob + kv * a.oh + j] = x;
 }
 
 }  // namespace tfgfa_weights
@@ -141,13 +225,16 @@ extern "C" int tfserve_key_weights(const void* q, const int64_t* q_strides, cons
   if (!(softmax_scale > 0.f) || !isfinite(softmax_scale)) return TFGFA_ERR_SCALE;
   if (causal != 0 && causal != 1) return TFGFA_ERR_CAUSAL_FLAG;
   if (B == 0 || H == 0 || N_k == 0) return TFGFA_OK;
-  if (B > 65535 || H_kv > 65535 || N_q > INT32_MAX - kTile || N_k > INT32_MAX - kTile ||
-      first_query > INT64_MAX / 2 || (long long)(N_q / kTile + 1) * (H / H_kv) > INT32_MAX - kWaves)
+  const long long units = (long long)B * H_kv;
+  if (units > INT32_MAX / 4096 || N_k > INT32_MAX - kKeys || (N_k / kKeys + 1) * units > INT32_MAX || N_q > INT32_MAX - kQueries ||
+      first_query > INT64_MAX / 2 || (long long)(N_q / kQueries + 1) * (H / H_kv) > INT32_MAX)
     return TFGFA_ERR_TOO_LARGE;
   if (!q_strides || !k_strides || !lse_strides || !out_strides) return TFGFA_ERR_NULL_POINTER;
   Args a = {};
   if (!rows_ok(q_strides, B, H, N_q, D, &a.qs) || !rows_ok(k_strides, B, H_kv, N_k, D, &a.ks))
     return TFGFA_ERR_STRIDE;
+  // A tile's rows are one buffer of less than 2^31 bytes.
+  if (a.qs.n > INT32_MAX / (4 * kQueries)) return TFGFA_ERR_TOO_LARGE;
   if (!k || !out || (N_q > 0 && (!q || !lse))) return TFGFA_ERR_NULL_POINTER;
   if (((uintptr_t)q | (uintptr_t)k) & 15u) return TFGFA_ERR_ALIGNMENT;
   if (((uintptr_t)lse | (uintptr_t)out) & 3u) return TFGFA_ERR_ALIGNMENT;
@@ -158,8 +245,11 @@ extern "C" int tfserve_key_weights(const void* q, const int64_t* q_strides, cons
   a.q = q, a.k = k, a.lse = lse, a.out = out;
   a.first = first_query;
   a.scale_log2 = softmax_scale * kLog2e;
-  a.G = H / H_kv, a.Nq = N_q, a.Nk = N_k, a.D = D, a.causal = causal;
-  const dim3 grid((N_k + kTile - 1) / kTile, H_kv, B);
+  a.Hkv = H_kv, a.G = H / H_kv, a.Nq = N_q, a.Nk = N_k, a.D = D, a.causal = causal;
+  a.units = B * H_kv;
+  const int st = tfgfa_device_info(&a.cu, nullptr, nullptr, 0);
+  if (st != TFGFA_OK) return st;
+  const dim3 grid((unsigned)((N_k + kKeys - 1) / kKeys * units));
   const hipStream_t stream = (hipStream_t)hip_stream;
 #define TFGFA_WEIGHTS(T)                                                                            \
   do {                                                                                              \
