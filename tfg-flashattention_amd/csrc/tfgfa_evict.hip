@@ -3,17 +3,21 @@
 // Of the L rows of a (sequence, key-value head) the last `recent` stay, then those of the largest weight, ties to the
 // lowest row, n = min(L, budget) in all; they are copied in their order to rows 0 .. n - 1 of other pages.
 //
-// select_kernel: one workgroup a (sequence, key-value head).  Weights are ordered as 32-bit keys (the float's
-// bits, flipped so that unsigned order is float order; NaN lowest, protected rows highest).  The n-th largest key is
-// found digit by digit, 8 bits a pass: a histogram of the keys that share the digits found so far, then the
-// digit at which the count from above reaches n.  A last pass in row order writes the rows above that key, and the
-// first of those equal to it, behind one another (prefix sums over the workgroup).
+// select_kernel: one workgroup a (sequence, key-value head).  Bound: latency, a few passes over the head's weights, which
+// stay in registers (up to 32768 rows; longer ones are read again in each pass).  Weights are ordered as 32-bit keys (the
+// float's bits, flipped so that unsigned order is float order; NaN lowest).  The last key that is kept is found by its digits of 11, 11 and 10 bits: a histogram in LDS of the keys that share the digits found so far, and the
+// digit at which the count from above reaches the number kept.  (The first digit is sign, exponent and two bits of the mantissa: weights
+// spread over tens of its values, so that few of a wave's 64 additions meet.)  Then the rows above that key, and the first of
+// those equal to it, are written behind one another: a wave's rows stand in row order, register by register, so places are
+// counts of bits in ballots.
 // copy_kernel: 16 bytes a thread and step, rows of K and V through both page tables.  Bound: HBM, 4D bytes
-// read and 4D written a kept row.
+// read and 4D written a kept row.  Where a head has few rows to copy, the selecting workgroup copies them itself.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
 #include <stdint.h>
+
+#include <algorithm>
 
 #include "tfgfa.h"
 #include "tfgfa_layout.h"
@@ -28,54 +32,98 @@ using tfgfa::pages_ok;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxD = 128;
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / 64;
+constexpr int kBins = 2048;
+constexpr int kMaxFused = kBins;  // rows that a selecting workgroup may copy itself (their list is in LDS)
+constexpr int kCandidates = 4096;  // rows with the first digit of the last one kept that a list holds
+constexpr int kMaxRows = 32768;   // rows of a sequence whose weights stay in registers
+constexpr int kFusedValues = 16384;  // rows * D of a head up to which the selecting workgroup copies them
+constexpr int kCopy = 4;          // rows of a thread of the copying kernel
 
 struct Args {
+  char* k;
+  char* v;
   const int* table;
   const int* lens;
   const float* weights;
   const int* new_table;
   int* kept;
   float* out;
+  Pages ks, vs;
   long long table_stride, new_stride, wb, wh, ob, oh;
-  int Hkv, P, page, n_max, budget, recent;
+  tfgfa::Division by_page;
+  int Hkv, P, page, n_max, budget, recent, pieces, fused;
 };
 
-// Order of the weight of row j < L as an unsigned number.
-__device__ __forceinline__ uint32_t rank_key(float w, bool keep) {
+// Order of a weight as an unsigned number.
+__device__ __forceinline__ uint32_t rank_key(float w) {
   const uint32_t x = __float_as_uint(w + 0.f);  // -0 as 0
   const uint32_t y = x >> 31 ? ~x : x | 0x80000000u;
-  return keep ? 0xFFFFFFFFu : w != w ? 0u : y;
+  return w != w ? 0u : y;
 }
 
-// Sum of x over the workgroup's threads before this one; *all: over all of them.
-__device__ __forceinline__ int block_before(int x, int* sh, int* all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int y = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int z = __shfl_up(y, o);
-    if (lane >= o) y += z;
-  }
-  __syncthreads();
-  if (lane == 63) sh[wave] = y;
-  __syncthreads();
-  int before = 0, sum = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    before += w < wave ? sh[w] : 0;
-    sum += sh[w];
-  }
-  *all = sum;
-  return before + y - x;
+// Sum of x over the lanes up to and with this one (row shifts inside 16 lanes, then the rows' ends).
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int add_dpp(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xF, false);
+}
+__device__ __forceinline__ int scan64(int x) {
+  x = add_dpp<0x111, 0xF>(x);
+  x = add_dpp<0x112, 0xF>(x);
+  x = add_dpp<0x114, 0xF>(x);
+  x = add_dpp<0x118, 0xF>(x);
+  x = add_dpp<0x142, 0xA>(x);     // lane 15 of rows 0 and 2 to the row after
+  return add_dpp<0x143, 0xC>(x);  // lane 31 to rows 2 and 3
+}
+// Bits of m below this lane's.
+__device__ __forceinline__ int below(unsigned long long m) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
 }
 
-__global__ __launch_bounds__(kThreads) void select_kernel(const Args a) {
-  __shared__ int hist[256];
-  __shared__ int sh[kWaves];
-  __shared__ int sh_digit, sh_above, sh_bad;
-  const int tid = threadIdx.x, kv = blockIdx.x, b = blockIdx.y;
+__device__ __forceinline__ int page_of(const Args& a, int j) {
+  return (int)(((unsigned long long)(uint32_t)j * a.by_page.m) >> a.by_page.s);
+}
+
+// Rows i0, i0 + step, .. of the kept ones, 16-byte piece c of K and V, kUnroll at a time.  list(i): the row, or -1.
+template <int kUnroll, class List>
+__device__ __forceinline__ void copy_rows(const Args& a, int b, int kv, int i0, int step, int c, int n, List list) {
+  const int* const from = a.table + b * a.table_stride;
+  const int* const to = a.new_table + b * a.new_stride;
+  for (; i0 < n; i0 += step * kUnroll) {
+    u32x4 kx[kUnroll], vx[kUnroll];
+    int j[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) j[u] = i0 + u * step < n ? list(i0 + u * step) : -1;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (j[u] >= 0) {
+        const int at = page_of(a, j[u]);
+        const long long p = from[at], r = j[u] - at * a.page;
+        kx[u] = *reinterpret_cast<const u32x4*>(a.k + p * a.ks.p + kv * a.ks.h + r * a.ks.n + 16 * c);
+        vx[u] = *reinterpret_cast<const u32x4*>(a.v + p * a.vs.p + kv * a.vs.h + r * a.vs.n + 16 * c);
+      }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (j[u] >= 0) {
+        const int i = i0 + u * step, at = page_of(a, i);
+        const long long p = to[at], r = i - at * a.page;
+        *reinterpret_cast<u32x4*>(a.k + p * a.ks.p + kv * a.ks.h + r * a.ks.n + 16 * c) = kx[u];
+        *reinterpret_cast<u32x4*>(a.v + p * a.vs.p + kv * a.vs.h + r * a.vs.n + 16 * c) = vx[u];
+      }
+  }
+}
+
+// kW waves; kR weights a lane in registers (row of register r: (wave * kR + r) * 64 + lane), 0: read in each pass, wave by
+// wave in the same order.
+template <int kW, int kR>
+__global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
+  constexpr int kThreads = 64 * kW, kEach = kBins / kThreads;
+  constexpr bool kList = kR > 4;  // candidates of the second digit are put into a list where it holds them
+  __shared__ int hist[kBins];
+  __shared__ uint32_t list[kList ? kCandidates : 1];
+  __shared__ int sh_sum[kW], sh_tie[kW];
+  __shared__ int sh_digit, sh_above, sh_bad, sh_count;
+  const int tid = threadIdx.x, lane = tid & 63, kv = blockIdx.x, b = blockIdx.y;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const float* const w = a.weights + b * a.wb + kv * a.wh;
   int* const kept = a.kept + ((long long)b * a.Hkv + kv) * a.budget;
   float* const out = a.out + b * a.ob + kv * a.oh;
@@ -83,13 +131,129 @@ __global__ __launch_bounds__(kThreads) void select_kernel(const Args a) {
   bool bad = L < 0 || L > a.n_max;
   if (bad) L = 0;
   const int n = min(L, a.budget);
-  if (tid == 0) sh_bad = 0;
-  __syncthreads();
+  const bool every = L <= a.budget;
+  // The rows from `old` on are protected; of those before it, `chosen` are kept.
+  const int old = every ? 0 : L - min(L, a.recent), chosen = every ? 0 : n - (L - old);
+  // This wave's rows: from `first` on.
+  const int regs = kR > 0 ? kR : (L + kThreads - 1) / kThreads;
+  const int first = wave * regs * 64;
+  float x[kR > 0 ? kR : 1];
+  uint32_t q[kR > 0 ? kR : 1];
+  if constexpr (kR > 0) {
+#pragma unroll
+    for (int r = 0; r < kR; ++r) x[r] = first + r * 64 + lane < L ? w[first + r * 64 + lane] : 0.f;
+  }
   for (int c = tid; c < (L + a.page - 1) / a.page; c += kThreads)
     bad |= (uint32_t)a.table[b * a.table_stride + c] >= (uint32_t)a.P;
   for (int c = tid; c < (n + a.page - 1) / a.page; c += kThreads)
     bad |= (uint32_t)a.new_table[b * a.new_stride + c] >= (uint32_t)a.P;
+  if (tid == 0) sh_bad = sh_count = 0;
+  __syncthreads();
   if (bad) sh_bad = 1;
+  if constexpr (kR > 0) {
+#pragma unroll
+    for (int r = 0; r < kR; ++r) q[r] = rank_key(x[r]);
+  }
+  // f(row, key, whether it is one to choose from) for this wave's rows in order.
+  auto rows = [&](auto f) {
+    if constexpr (kR > 0) {
+#pragma unroll
+      for (int r = 0; r < kR; ++r) {
+        if (first + r * 64 >= old) break;
+        const int j = first + r * 64 + lane;
+        f(j, q[r], j < old);
+      }
+    } else {
+      for (int r = 0; r < regs; ++r) {
+        if (first + r * 64 >= old) break;
+        const int j = first + r * 64 + lane;
+        f(j, j < old ? rank_key(w[j]) : 0u, j < old);
+      }
+    }
+  };
+  auto clear = [&]() {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) hist[e * kThreads + tid] = 0;
+    __syncthreads();
+  };
+  // One more of a digit, in the lanes that are in; a wave whose keys all have one digit (equal weights) adds them at once.
+  auto count = [&](bool in, int digit) {
+    const unsigned long long who = __builtin_amdgcn_ballot_w64(in);
+    if (who == 0) return;
+    const int lead = __builtin_amdgcn_readlane(digit, __builtin_ctzll(who));
+    if (__builtin_amdgcn_ballot_w64(in && digit != lead) == 0) {
+      if (lane == 0) atomicAdd(&hist[lead], __builtin_popcountll(who));
+    } else if (in) {
+      atomicAdd(&hist[digit], 1);
+    }
+  };
+  // The chosen-th largest key, and how many of the keys equal to it are wanted.
+  uint32_t key = 0;
+  int want = chosen;
+  // The digit at which the count of the histogram from above reaches `want`.
+  auto find = [&](int shift) {
+    __syncthreads();
+    // Thread t: bins from kBins - 1 - t kEach down.
+    int mine = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) mine += hist[kBins - 1 - tid * kEach - e];
+    const int upto = scan64(mine);
+    if (lane == 63) sh_sum[wave] = upto;
+    __syncthreads();
+    int above = upto - mine;
+#pragma unroll
+    for (int c = 0; c < kW; ++c) above += c < wave ? sh_sum[c] : 0;
+    if (above < want && above + mine >= want) {
+      int e = 0;
+      for (; e < kEach - 1; ++e) {
+        const int here = hist[kBins - 1 - tid * kEach - e];
+        if (above + here >= want) break;
+        above += here;
+      }
+      sh_digit = kBins - 1 - tid * kEach - e;
+      sh_above = above;
+    }
+    __syncthreads();
+    key |= (uint32_t)sh_digit << shift;
+    want -= sh_above;
+  };
+  if (chosen > 0 && chosen < old) {
+    clear();
+    rows([&](int j, uint32_t y, bool in) { count(in, y >> 21); });
+    find(21);
+    const int same = hist[key >> 21];
+    if (kList && same <= kCandidates) {
+      __syncthreads();  // (the histogram has been read)
+      rows([&](int j, uint32_t y, bool in) {
+        if (in && y >> 21 == key >> 21) list[atomicAdd(&sh_count, 1) & (kCandidates - 1)] = y;
+      });
+#pragma unroll 1
+      for (int shift = 10; shift >= 0; shift -= 10) {
+        clear();
+        for (int c = tid; c < (same + 63) / 64 * 64; c += kThreads) {
+          const uint32_t y = c < same ? list[c] : 0u;
+          const int top = shift == 10 ? 21 : 10;
+          count(c < same && y >> top == key >> top, (y >> shift) & ((1 << (top - shift)) - 1));
+        }
+        find(shift);
+      }
+    } else {
+#pragma unroll 1
+      for (int shift = 10; shift >= 0; shift -= 10) {
+        const int top = shift == 10 ? 21 : 10;
+        __syncthreads();
+        clear();
+        rows([&](int j, uint32_t y, bool in) {
+          count(in && y >> top == key >> top, (y >> shift) & ((1 << (top - shift)) - 1));
+        });
+        find(shift);
+      }
+    }
+  } else if (chosen == 0) {
+    key = 0xFFFFFFFFu;  // (no key is above it, and no tie is wanted)
+  } else {
+    want = old;  // all of them: those above 0, and of 0 (NaN) as many as there are
+  }
   __syncthreads();
   if (sh_bad) {
     for (int i = tid; i < a.budget; i += kThreads) {
@@ -98,78 +262,97 @@ __global__ __launch_bounds__(kThreads) void select_kernel(const Args a) {
     }
     return;
   }
-  // The n-th largest key: its digits, and how many of the keys equal to it are wanted.
-  uint32_t key = 0;
-  int want = n;
-  const int old = L - min(L, a.recent);
-  if (L > a.budget) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
+  auto keep = [&](int at, int j, float y) {
+    kept[at] = j;
+    out[at] = y;
+    if (kR > 0 && a.fused) hist[at & (kBins - 1)] = j;
+  };
+  if constexpr (kR > 0) {
+    // Rows above the key, and ties, of the waves before.  (Every weight is in a register by now: `out` may be `w`.)
+    int taken = 0, ties = 0;
+    rows([&](int j, uint32_t y, bool in) {
+      taken += __builtin_popcountll(__builtin_amdgcn_ballot_w64(in && y > key));
+      ties += __builtin_popcountll(__builtin_amdgcn_ballot_w64(in && y == key));
+    });
+    if (lane == 0) {
+      sh_sum[wave] = taken;
+      sh_tie[wave] = ties;
+    }
+    __syncthreads();
+    taken = ties = 0;
+#pragma unroll
+    for (int c = 0; c < kW; ++c) {
+      taken += c < wave ? sh_sum[c] : 0;
+      ties += c < wave ? sh_tie[c] : 0;
+    }
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+      if (first + r * 64 >= L) break;
+      const int j = first + r * 64 + lane;
+      const bool in = j < old;
+      const unsigned long long mo = __builtin_amdgcn_ballot_w64(in && q[r] > key);
+      const unsigned long long mt = __builtin_amdgcn_ballot_w64(in && q[r] == key);
+      if (mo | mt) {
+        const int t = ties + below(mt);
+        if (in && (q[r] > key || (q[r] == key && t < want))) keep(taken + below(mo) + min(t, want), j, x[r]);
+        taken += __builtin_popcountll(mo);
+        ties += __builtin_popcountll(mt);
+      }
+      if (!in && j < L) keep(chosen + j - old, j, x[r]);
+    }
+  } else {
+    // `out` may be `w`: rows move down only, and a step's rows, of all waves, are read before any is written.
+    int done = 0, seen = 0;
+    for (int j0 = 0; j0 < L; j0 += kThreads) {
+      const int j = j0 + tid;
+      const bool in = j < old;
+      const float y = j < L ? w[j] : 0.f;
+      const uint32_t z = rank_key(y);
+      const unsigned long long mo = __builtin_amdgcn_ballot_w64(in && z > key);
+      const unsigned long long mt = __builtin_amdgcn_ballot_w64(in && z == key);
       __syncthreads();
-      for (int j = tid; j < L; j += kThreads) {
-        const uint32_t x = rank_key(w[j], j >= old);
-        if (shift == 24 || (x >> (shift + 8)) == (key >> (shift + 8))) atomicAdd(&hist[(x >> shift) & 255], 1);
+      if (lane == 0) {
+        sh_sum[wave] = __builtin_popcountll(mo);
+        sh_tie[wave] = __builtin_popcountll(mt);
       }
       __syncthreads();
-      int all;
-      const int mine = tid < 256 ? hist[255 - tid] : 0;  // from the highest digit down
-      const int above = block_before(mine, sh, &all);
-      if (tid < 256 && above < want && above + mine >= want) {
-        sh_digit = 255 - tid;
-        sh_above = above;
+      int o = done, s = seen;
+#pragma unroll
+      for (int c = 0; c < kW; ++c) {
+        o += c < wave ? sh_sum[c] : 0;
+        s += c < wave ? sh_tie[c] : 0;
+        done += sh_sum[c];
+        seen += sh_tie[c];
       }
-      __syncthreads();
-      key |= (uint32_t)sh_digit << shift;
-      want -= sh_above;
+      const int t = s + below(mt);
+      if (in && (z > key || (z == key && t < want))) keep(o + below(mo) + min(t, want), j, y);
+      if (!in && j < L) keep(chosen + j - old, j, y);
     }
+    __syncthreads();
   }
-  // In row order: the rows above the key, and the first `want` of those equal to it.
-  int done = 0, ties = 0;
-  for (int j0 = 0; j0 < L; j0 += kThreads) {
-    const int j = j0 + tid;
-    const float x = j < L ? w[j] : 0.f;
-    bool take = j < L;
-    int all;
-    if (L > a.budget) {
-      const uint32_t y = rank_key(x, j >= old);
-      const bool tie = j < L && y == key;
-      const int t = block_before(tie ? 1 : 0, sh, &all);
-      take = j < L && (y > key || (tie && ties + t < want));
-      ties += all;
-    }
-    const int at = done + block_before(take ? 1 : 0, sh, &all);
-    done += all;
-    // Every row of this step has been read (the barriers above), and rows move down only: `out` may be `w`.
-    if (take) {
-      kept[at] = j;
-      out[at] = x;
-    }
-  }
-  __syncthreads();
   for (int i = n + tid; i < a.budget; i += kThreads) {
     kept[i] = -1;
     out[i] = 0.f;
   }
+  if (!a.fused) return;
+  __syncthreads();
+  const int per = kThreads / a.pieces, row = tid / a.pieces;
+  if (row < per) copy_rows<4>(a, b, kv, row, per, tid - row * a.pieces, n, [&](int i) { return hist[i]; });
 }
 
-__global__ __launch_bounds__(256) void copy_kernel(char* k, char* v, Pages ks, Pages vs,
-                                                   const int* __restrict__ table, long long table_stride,
-                                                   const int* __restrict__ new_table, long long new_stride,
-                                                   const int* __restrict__ kept, int Hkv, int page, int budget,
-                                                   int pieces) {
+__global__ __launch_bounds__(256) void copy_kernel(const Args a) {
   const int kv = blockIdx.y, b = blockIdx.z;
-  const int* const rows = kept + ((long long)b * Hkv + kv) * budget;
-  const long long x = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int i = (int)(x / pieces), c = (int)(x - (long long)i * pieces);
-  if (i >= budget) return;
-  const int j = rows[i];
-  if (j < 0) return;
-  const long long from = table[b * table_stride + j / page], to = new_table[b * new_stride + i / page];
-  const int fo = j % page, ti = i % page;
-  const u32x4 kx = *reinterpret_cast<const u32x4*>(k + from * ks.p + kv * ks.h + fo * ks.n + 16 * c);
-  const u32x4 vx = *reinterpret_cast<const u32x4*>(v + from * vs.p + kv * vs.h + fo * vs.n + 16 * c);
-  *reinterpret_cast<u32x4*>(k + to * ks.p + kv * ks.h + ti * ks.n + 16 * c) = kx;
-  *reinterpret_cast<u32x4*>(v + to * vs.p + kv * vs.h + ti * vs.n + 16 * c) = vx;
+  const int* const rows = a.kept + ((long long)b * a.Hkv + kv) * a.budget;
+  const int per = 256 / a.pieces, row = threadIdx.x / a.pieces;
+  const int i0 = blockIdx.x * per * kCopy;
+  if (row < per)
+    copy_rows<kCopy>(a, b, kv, i0 + row, per, threadIdx.x - row * a.pieces, min(a.budget, i0 + per * kCopy),
+                     [&](int i) { return rows[i]; });
+}
+
+template <int kW, int kR>
+static void launch(const Args& a, int B, hipStream_t stream) {
+  hipLaunchKernelGGL((select_kernel<kW, kR>), dim3(a.Hkv, B), dim3(64 * kW), 0, stream, a);
 }
 
 }  // namespace tfgfa_evict
@@ -188,16 +371,14 @@ extern "C" int tfserve_evict(void* k_pages, const int64_t* k_strides, void* v_pa
   if (B == 0 || H_kv == 0 || budget == 0) return TFGFA_OK;
   if (P == 0) return TFGFA_ERR_BAD_SHAPE;
   const long long n_max = (long long)M * page;
-  const long long grid = ((long long)budget * (D / 8) + 255) / 256;
-  if (n_max > INT32_MAX - kThreads || (long long)M_new * page > INT32_MAX || budget > INT32_MAX - kThreads ||
-      B > 65535 || H_kv > 65535 || grid > INT32_MAX / 256)
+  if (n_max > INT32_MAX - 65536 || (long long)M_new * page > INT32_MAX || budget > INT32_MAX - 65536 || B > 65535 ||
+      H_kv > 65535)
     return TFGFA_ERR_TOO_LARGE;
   if (!k_strides || !v_strides || !weights_strides || !weights_out_strides) return TFGFA_ERR_NULL_POINTER;
-  Pages ks, vs;
-  if (!pages_ok(k_strides, P, H_kv, page, D, &ks) || !pages_ok(v_strides, P, H_kv, page, D, &vs))
-    return TFGFA_ERR_STRIDE;
   if (B > 1 && (table_stride < 0 || new_table_stride < M_new)) return TFGFA_ERR_STRIDE;
   Args a = {};
+  if (!pages_ok(k_strides, P, H_kv, page, D, &a.ks) || !pages_ok(v_strides, P, H_kv, page, D, &a.vs))
+    return TFGFA_ERR_STRIDE;
   a.wb = B > 1 ? weights_strides[0] : 0, a.wh = H_kv > 1 ? weights_strides[1] : 0;
   a.ob = B > 1 ? weights_out_strides[0] : 0, a.oh = H_kv > 1 ? weights_out_strides[1] : 0;
   if (a.wb < 0 || a.wh < 0 || !apart(a.ob, B, a.oh, H_kv, budget))
@@ -210,17 +391,30 @@ extern "C" int tfserve_evict(void* k_pages, const int64_t* k_strides, void* v_pa
   if (((uintptr_t)page_table | (uintptr_t)cache_seqlens | (uintptr_t)key_weights | (uintptr_t)new_page_table |
        (uintptr_t)kept | (uintptr_t)weights_out) & 3u)
     return TFGFA_ERR_ALIGNMENT;
+  a.k = static_cast<char*>(k_pages), a.v = static_cast<char*>(v_pages);
   a.table = page_table, a.lens = cache_seqlens, a.weights = key_weights, a.new_table = new_page_table;
   a.kept = kept, a.out = weights_out;
   a.table_stride = B > 1 ? table_stride : 0, a.new_stride = B > 1 ? new_table_stride : 0;
   a.Hkv = H_kv, a.P = P, a.page = page, a.n_max = (int)n_max, a.budget = budget, a.recent = recent;
+  a.by_page = tfgfa::division_by(page);
+  a.pieces = D / 8;
+  const int rows = std::min<long long>(budget, n_max);
+  a.fused = n_max <= kMaxRows && rows <= kMaxFused && (long long)rows * D <= kFusedValues;
   const hipStream_t stream = (hipStream_t)hip_stream;
-  hipLaunchKernelGGL(select_kernel, dim3(H_kv, B), dim3(kThreads), 0, stream, a);
+  if (n_max <= 1024)
+    launch<4, 4>(a, B, stream);
+  else if (n_max <= 4096)
+    launch<16, 4>(a, B, stream);
+  else if (n_max <= kMaxRows)
+    launch<16, 32>(a, B, stream);
+  else
+    launch<16, 0>(a, B, stream);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return -(int)e;
-  hipLaunchKernelGGL(copy_kernel, dim3((unsigned)grid, H_kv, B), dim3(256), 0, stream, static_cast<char*>(k_pages),
-                     static_cast<char*>(v_pages), ks, vs, page_table, a.table_stride, new_page_table, a.new_stride,
-                     kept, H_kv, page, budget, D / 8);
-  e = hipGetLastError();
+  if (!a.fused) {
+    const int per = 256 / a.pieces * kCopy;
+    hipLaunchKernelGGL(copy_kernel, dim3((rows + per - 1) / per, H_kv, B), dim3(256), 0, stream, a);
+    e = hipGetLastError();
+  }
   return e == hipSuccess ? TFGFA_OK : -(int)e;
 }

@@ -54,6 +54,18 @@ inline bool apart(long long sa, long long na, long long sb, long long nb, long l
   return nb <= 1 || sb > reach;
 }
 
+// j / page = j * m >> s for 0 <= j < 2^31: with 2^(l-1) < page <= 2^l and m = floor(2^(31+l) / page) + 1 the error j (m
+// page - 2^(31+l)) / (page 2^(31+l)) is below 1 / page, and m < 2^32.
+struct Division {
+  uint32_t m;
+  int s;
+};
+inline Division division_by(int page) {
+  int l = 0;
+  while ((1LL << l) < page) ++l;
+  return {(uint32_t)((1ULL << (31 + l)) / (uint64_t)page + 1), 31 + l};
+}
+
 }  // namespace tfgfa
 
 #endif  // TFGFA_LAYOUT_H

@@ -961,12 +961,8 @@ extern "C" int tfserve_decode_paged(
   a.scale = softmax_scale, a.scale_log2 = softmax_scale * kLog2e, a.slack = std::min(kSlack / softmax_scale, 1e30f);
   a.H = H, a.G = H / H_kv, a.P = P, a.page = page, a.D = D;
   a.min_granules = min_granules(a.G);
-  // j / page by a product: with 2^(l-1) < page <= 2^l and m = floor(2^(31+l) / page) + 1 the error j (m page -
-  // 2^(31+l)) / 2^(31+l) is below 1 / page for j < 2^31, and m < 2^32.
-  int lg = 0;
-  while ((1LL << lg) < page) ++lg;
-  f.div_m = (uint32_t)((1ULL << (31 + lg)) / (uint64_t)page + 1);
-  f.div_s = 31 + lg;
+  const tfgfa::Division by_page = tfgfa::division_by(page);
+  f.div_m = by_page.m, f.div_s = by_page.s;
   const hipStream_t stream = (hipStream_t)hip_stream;
   if (dtype == TFGFA_DTYPE_BF16)
     launch<__bf16>(f, a, (unsigned)wgs, stream);
