@@ -1,9 +1,9 @@
 // tfgfa_logits.hip - penalties for repeated tokens, biases and grammar masks on logits, MI355X (gfx950).
 //
-// Bound: HBM, the logits read and written once.  A workgroup owns kChunk tokens of one row: it counts the
-// row's history into LDS (only its own tokens; integer adds, so their order is no matter), then passes over its
-// logits once.  The history is read by every workgroup of the row (from L2), which costs less than a counting
-// kernel before this one.
+// Bound: HBM, the logits read and written once.  A workgroup owns kChunk tokens of one row, whose logits, biases and mask
+// words it asks for first; while they come it counts the row's history into LDS (its own tokens only; integer adds, so their
+// order is no matter), which every workgroup of the row reads from L2.  Rows of odd lengths begin at any element: a lane
+// takes four neighbouring logits as one load of the elements' own alignment.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -15,7 +15,10 @@
 namespace tfgfa_logits {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 4096;
+constexpr int kEach = 4;              // neighbouring logits of a lane
+constexpr int kSteps = 4;
+constexpr int kChunk = kThreads * kEach * kSteps;
+constexpr int kTokens = 4;            // tokens of the history that a lane loads at once
 
 struct Args {
   const void* x;
@@ -32,34 +35,81 @@ struct Args {
   int token_bytes, V, T;
 };
 
+// kEach neighbouring values of type E at any element.
+template <class E>
+struct Pack {
+  typedef E v __attribute__((ext_vector_type(kEach)));
+  typedef v __attribute__((aligned(sizeof(E)))) any;
+};
+
 template <class E>
 __global__ __launch_bounds__(kThreads) void penalize_kernel(const Args a) {
   __shared__ int count[kChunk];
   const int tid = threadIdx.x, b = blockIdx.y, v0 = blockIdx.x * kChunk;
-  for (int i = tid; i < kChunk; i += kThreads) count[i] = 0;
-  __syncthreads();
-  int T = a.T;
-  if (a.lengths) T = max(0, min(T, a.lengths[b]));
-  for (int t = tid; t < T; t += kThreads) {
-    const long long v = (a.token_bytes == 8 ? static_cast<const long long*>(a.tokens)[b * a.ts + t]
-                                            : (long long)static_cast<const int*>(a.tokens)[b * a.ts + t]) -
-                        v0;
-    if (v >= 0 && v < kChunk) atomicAdd(&count[(int)v], 1);
-  }
-  __syncthreads();
-  const float rep = a.reps ? a.reps[b] : a.rep, pres = a.press ? a.press[b] : a.pres,
-              freq = a.freqs ? a.freqs[b] : a.freq;
   const E* const x = static_cast<const E*>(a.x) + b * a.xs;
   E* const y = static_cast<E*>(a.y) + b * a.ys;
-  for (int i = tid; i < kChunk; i += kThreads) {
-    const int v = v0 + i;
-    if (v >= a.V) break;
-    float z = (float)x[v];
-    const int n = count[i];
-    if (n > 0) z = (z > 0.f ? z / rep : z * rep) - freq * (float)n - pres;
-    if (a.bias) z += a.bias[b * a.bs + v];
-    if (a.allowed && !((a.allowed[b * a.as + (v >> 5)] >> (v & 31)) & 1u)) z = -INFINITY;
-    y[v] = (E)z;
+  const float* const bias = a.bias ? a.bias + b * a.bs : nullptr;
+  const uint32_t* const allowed = a.allowed ? a.allowed + b * a.as : nullptr;
+  typename Pack<E>::v z[kSteps];
+  typename Pack<float>::v w[kSteps];
+  uint32_t bits[kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int v = v0 + (s * kThreads + tid) * kEach;  // (a multiple of 4: its four bits are in one word)
+    if (v + kEach <= a.V) {
+      z[s] = *reinterpret_cast<const typename Pack<E>::any*>(x + v);
+      if (bias) w[s] = *reinterpret_cast<const typename Pack<float>::any*>(bias + v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        z[s][e] = v + e < a.V ? x[v + e] : (E)0.f;
+        if (bias) w[s][e] = v + e < a.V ? bias[v + e] : 0.f;
+      }
+    }
+    bits[s] = allowed && v < a.V ? allowed[v >> 5] >> (v & 31) : 0xFu;
+  }
+  int T = a.T;
+  if (a.lengths) T = max(0, min(T, a.lengths[b]));
+  const float rep = a.reps ? a.reps[b] : a.rep, pres = a.press ? a.press[b] : a.pres,
+              freq = a.freqs ? a.freqs[b] : a.freq;
+#pragma unroll
+  for (int s = 0; s < kSteps * kEach; ++s) count[s * kThreads + tid] = 0;
+  __syncthreads();
+  for (int t0 = 0; t0 < T; t0 += kThreads * kTokens) {
+    long long id[kTokens];
+#pragma unroll
+    for (int c = 0; c < kTokens; ++c) {
+      const int t = t0 + c * kThreads + tid;
+      id[c] = -1;
+      if (t < T)
+        id[c] = a.token_bytes == 8 ? static_cast<const long long*>(a.tokens)[b * a.ts + t]
+                                   : (long long)static_cast<const int*>(a.tokens)[b * a.ts + t];
+    }
+#pragma unroll
+    for (int c = 0; c < kTokens; ++c)
+      if (id[c] >= v0 && id[c] < v0 + kChunk) atomicAdd(&count[(int)(id[c] - v0)], 1);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int at = (s * kThreads + tid) * kEach, v = v0 + at;
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const i32x4 n = *reinterpret_cast<const i32x4*>(&count[at]);
+    typename Pack<E>::v out;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      float f = (float)z[s][e];
+      if (n[e] > 0) f = (f > 0.f ? f / rep : f * rep) - freq * (float)n[e] - pres;
+      if (bias) f += w[s][e];
+      out[e] = (E)((bits[s] >> e) & 1u ? f : -INFINITY);
+    }
+    if (v + kEach <= a.V) {
+      *reinterpret_cast<typename Pack<E>::any*>(y + v) = out;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (v + e < a.V) y[v + e] = out[e];
+    }
   }
 }
 
