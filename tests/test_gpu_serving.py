@@ -638,3 +638,113 @@ def test_empty_calls():
     assert (kept == -1).all() and (ws == 0).all()
     assert fa.penalize_logits(torch.zeros(0, 9, device=DEV)).shape == (0, 9)
     assert fa.penalize_logits(torch.zeros(3, 0, device=DEV)).shape == (3, 0)
+
+
+def test_prompt_steps_and_cuts_run_together():
+    """A paged cache as a generation uses it: the prompt's attention and key weights, steps that append and sum weights,
+    cuts to the budget in between; against the same in 64 bits.  (Which rows a cut keeps is checked on the sums that the
+    cache holds, which are themselves within their bound.)"""
+    import model_inference as mi
+
+    g = _gen(30)
+    B, H, D, N, steps = 2, 3, 64, 150, 60
+    cache = mi.PagedKVCache({"n_heads": H, "emb_dim": H * D, "n_layers": 1}, B, 256, DEV, page_size=16, budget=64, recent=20,
+                            slack=17)
+    q, k, v = (_randn((B, N, H, D), g, BF, 1.5) for _ in range(3))
+    ctx = torch.empty(B, N, H, D, dtype=BF, device=DEV)
+    cache.prompt(0, q, k, v, ctx)
+    cache.advance(N)
+    qd, kd = q.double().cpu(), k.double().cpu()
+    rows = [[(k[b, :, :].transpose(0, 1).cpu(), v[b, :, :].transpose(0, 1).cpu()) for _ in (0,)][0] for b in range(B)]
+    sums, err = torch.zeros(B, H, N, dtype=torch.float64), torch.zeros(B, H, N, dtype=torch.float64)
+    for b in range(B):
+        for h in range(H):
+            x = (qd[b, :, h] @ kd[b, :, h].T) * D ** -0.5
+            x.masked_fill_(torch.ones(N, N).triu(1).bool(), -INF)
+            p = torch.softmax(x, 1)
+            sums[b, h] = p.sum(0)
+            X = (qd[b, :, h].abs() @ kd[b, :, h].abs().T * D ** -0.5).max()
+            # The attention's lse is off by its scores' error and its bf16-weighted sum's 2^-8 at most.
+            err[b, h] = sums[b, h] * (2.1 * ((D + 4) * U * X + 8 * U * x[x > -INF].abs().max()) + 2.0 ** -8 + N * U)
+    for step in range(steps):
+        assert torch.equal(cache.seqlens.cpu(), torch.full((B,), cache.length, dtype=torch.int32))
+        assert (cache.positions == N + step).all()
+        n = cache.length
+        held = cache.weights[0][:, :, :n].double().cpu()
+        assert ((held - sums).abs() <= err).all(), f"sums before step {step}"
+        if cache.over():
+            _say(f"step {step}: cut from {n} rows")
+            w = cache.weights[0][:, :, :n].clone()
+            cache.evict()
+            assert cache.length == 64 and not cache.over()
+            for b in range(B):
+                for h in range(H):
+                    keep = torch.from_numpy(_evict_ref(w[b, h], n, 64, 20))
+                    sums[b, h, :64], err[b, h, :64] = sums[b, h, keep].clone(), err[b, h, keep].clone()
+                    for t in rows[b]:
+                        t[h, :64] = t[h, keep].clone()
+            sums, err = sums[..., :64], err[..., :64]
+            rows = [(kk[:, :64], vv[:, :64]) for kk, vv in rows]
+        q1, k1, v1 = (_randn((B, H, D), g, BF, 1.5) for _ in range(3))
+        o = cache.attend(0, q1, k1, v1)
+        cache.advance(1)
+        rows = [(torch.cat([rows[b][0], k1[b].cpu()[:, None]], 1), torch.cat([rows[b][1], v1[b].cpu()[:, None]], 1))
+                for b in range(B)]
+        zero = torch.zeros(B, H, 1, dtype=torch.float64)
+        sums, err = torch.cat([sums, zero], 2), torch.cat([err, zero], 2)
+        for b in range(B):
+            ro, _, w, eo, _, ew = attend(q1[b], *rows[b], D ** -0.5)
+            d = (o[b].double().cpu() - ro).abs()
+            assert (d <= eo + _half(BF) * (ro.abs() + eo)).all(), step
+            sums[b] += w
+            err[b] += ew + 2 * U * sums[b]
+    pages = torch.cat([cache.table.cpu().flatten(), torch.tensor(cache._free, dtype=torch.int32)])
+    assert sorted(pages.tolist()) == list(range(cache.k[0].shape[0])), "every page is held or free once"
+    cache.reset()
+    assert cache.length == 0 and (cache.positions == 0).all() and cache.table.shape[1] == 16
+
+
+def test_generation_with_paged_caches_and_penalties():
+    """generate_cached over pages gives the logits of the contiguous cache (both bf16 attentions of one model); with a
+    budget it runs past it; penalties forbid and demand tokens in every loop."""
+    import model_inference as mi
+
+    cfg = dict(mi.GPT_CONFIG_124M)
+    cfg.update({"emb_dim": 256, "n_layers": 2, "n_heads": 4, "vocab_size": 1000, "context_length": 256, "drop_rate": 0.0,
+                "qkv_bias": True, "impl_type": "hip"})
+    model = mi.GPTModel(cfg).eval()
+    mi.init_gpt2_weights(model, 5)
+    model.to(DEV)
+    small = {"n_heads": 4, "emb_dim": 256, "n_layers": 2}
+    idx = torch.randint(0, 1000, (3, 90), generator=_gen(1)).to(DEV)
+    tokens = torch.randint(0, 1000, (3, 20), generator=_gen(2)).to(DEV)
+    caches = [mi.KVCache(small, 3, 128, DEV), mi.PagedKVCache(small, 3, 128, DEV, page_size=16),
+              mi.PagedKVCache(small, 3, 128, DEV, page_size=48, budget=100, slack=28)]
+    with torch.no_grad():
+        got = [[model(idx, kv_cache=c)[:, -1]] + [model(tokens[:, i:i + 1], kv_cache=c)[:, -1] for i in range(20)]
+               for c in caches]
+    for other in got[1:]:
+        for a, b in zip(got[0], other):
+            assert (a - b).norm() / a.norm() <= 1e-2   # the gate of the cached path against the full forward
+    cut = mi.PagedKVCache(small, 3, 200, DEV, page_size=16, budget=32, recent=8, slack=16)
+    out = mi.generate_cached(model, idx, 100, 256, temperature=0.0, cache=cut)
+    assert out.shape == (3, 190) and cut.length <= 48 and int(cut.positions[0]) == 189
+    again = mi.generate_cached(model, idx, 100, 256, temperature=0.0, cache=cut)
+    assert torch.equal(out, again)
+    with pytest.raises(ValueError, match="shorter than prompt"):
+        mi.generate_cached(model, idx, 111, 256, cache=cut)
+    with pytest.raises(ValueError, match="for 3 sequences"):
+        mi.generate_cached(model, idx[:1], 5, 256, cache=cut)
+    # Only even tokens, none twice.
+    even = torch.full((32,), 0x55555555, dtype=torch.int32, device=DEV)
+    loops = (lambda p: mi.generate(model, idx, 12, 256, temperature=0.0, penalties=p),
+             lambda p: mi.generate_cached(model, idx, 12, 256, temperature=0.0, penalties=p),
+             lambda p: mi.generate_graphed(model, idx, 12, 256, temperature=0.0, penalties=p))
+    for loop in loops:
+        new = loop(mi.LogitPenalties(presence=1e4, allowed=even))[:, 90:]
+        assert (new % 2 == 0).all()
+        for b in range(3):
+            assert len(set(new[b].tolist())) == 12 and not set(new[b].tolist()) & set(idx[b].tolist())
+        bias = torch.zeros(1000, device=DEV)
+        bias[77] = 1e4
+        assert (loop(mi.LogitPenalties(bias=bias))[:, 90:] == 77).all()

@@ -4,7 +4,8 @@ Mirrors the reference's model classes (src/py/model_inference.py:39-190) with th
 names, constructor arguments and config keys, so code written against the reference's
 ``GPTModel(cfg)`` runs unchanged, and its token loop ``generate`` (:199-228).  Added:
 ``KVCache`` and ``generate_cached``, the same loop with a KV cache (prefill once, then one
-decode-kernel step per token).  The reference's data loader, training helpers, tokenizer and
+decode-kernel step per token); ``PagedKVCache``, a cache in pages that may be cut to the rows whose
+attention weight is largest; ``LogitPenalties``, what a loop does to the logits before sampling.  The reference's data loader, training helpers, tokenizer and
 pretrained-weight download (model_inference.py:23-37, :193-197, :229-376; gpt_download.py)
 are not here.
 
@@ -222,31 +223,23 @@ class MultiHeadAttention(nn.Module):
         """Attention against a KV cache (no counterpart in the reference, whose generate()
         re-runs the whole prefix, model_inference.py:199-228).
 
-        Prefill (the cache is empty): the new tokens' K/V are copied into the cache and the
-        causal forward kernel reads Q from the projection and K/V from the cache through their
-        strides.  Decode (one new token): the decode kernel appends the token's K/V to the cache
-        and attends over the cached prefix.  Both write the context straight into a
-        (B, N, H*d) buffer.
+        Prefill (the cache is empty): the cache stores the new tokens' K/V and runs the causal
+        forward kernel over them.  Decode (one new token): its decode kernel appends the token's K/V
+        and attends over the cached prefix.  Both write the context straight into a (B, N, H*d)
+        buffer.
         """
-        import custom_flash_attn  # raises if the native extension is not built
-
         if self.impl_type not in ("hip", "cuda"):
             raise ValueError(f"cached attention runs on the HIP kernels; impl_type is {self.impl_type!r}")
         b, n, _ = x.shape
         H, hd = self.num_heads, self.head_dim
         q, k, v, out_proj = self._project(x)
-        kc, vc = cache.k[layer], cache.v[layer]
         ctx = torch.empty(b, n, H, hd, dtype=q.dtype, device=q.device)
         if cache.length == 0:
-            if n > kc.shape[2]:
-                raise ValueError(f"{n} tokens do not fit a cache of {kc.shape[2]}")
-            kc[:, :, :n].copy_(k.transpose(1, 2))
-            vc[:, :, :n].copy_(v.transpose(1, 2))
-            custom_flash_attn.attention(q.transpose(1, 2), kc[:, :, :n], vc[:, :, :n],
-                                        out=ctx.transpose(1, 2))
+            if n > cache.max_len:
+                raise ValueError(f"{n} tokens do not fit a cache of {cache.max_len}")
+            cache.prompt(layer, q, k, v, ctx)
         elif n == 1:
-            custom_flash_attn.decode(q[:, 0], kc, vc, cache.seqlens, k[:, 0], v[:, 0],
-                                     out=ctx[:, 0], workspace=cache.workspace)
+            cache.attend(layer, q[:, 0], k[:, 0], v[:, 0], out=ctx[:, 0])
         else:
             raise NotImplementedError("a cache that already holds tokens takes one new token per step")
         return out_proj(ctx.view(b, n, self.d_out))
@@ -274,6 +267,29 @@ class KVCache:
         nbytes = custom_flash_attn._C.decode_workspace_bytes(batch, H, max_len)
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
 
+    @property
+    def positions(self):
+        """The position of the next token, per batch row."""
+        return self.seqlens
+
+    def prompt(self, layer, q, k, v, ctx) -> None:
+        """The prompt's (B, N, H, d) projections: K and V into the cache, the attention into ``ctx``.
+        The causal forward kernel reads Q from the projection and K/V from the cache through their
+        strides."""
+        import custom_flash_attn
+
+        n, kc, vc = k.shape[1], self.k[layer], self.v[layer]
+        kc[:, :, :n].copy_(k.transpose(1, 2))
+        vc[:, :, :n].copy_(v.transpose(1, 2))
+        custom_flash_attn.attention(q.transpose(1, 2), kc[:, :, :n], vc[:, :, :n], out=ctx.transpose(1, 2))
+
+    def attend(self, layer, q, k, v, out=None):
+        """One decode step of (B, H, d) projections: the new row appended, the attention over all rows."""
+        import custom_flash_attn
+
+        return custom_flash_attn.decode(q, self.k[layer], self.v[layer], self.seqlens, k, v, out=out,
+                                        workspace=self.workspace)
+
     def advance(self, n: int) -> None:
         self.length += n
         self.seqlens.add_(n)
@@ -281,6 +297,113 @@ class KVCache:
     def reset(self) -> None:
         self.length = 0
         self.seqlens.zero_()
+
+
+class PagedKVCache:
+    """K/V caches of a GPTModel in pages, optionally cut to the rows that matter.
+
+    ``k[layer]``, ``v[layer]``: pools of (pages, H, page_size, head_dim) bf16; ``table``: int32 (B,
+    columns), the pages of each sequence's rows, the same in every layer; ``seqlens``: int32 (B,), the
+    rows of each sequence, and ``length`` the same on the host; ``positions``: int32 (B,), the tokens
+    seen.  With ``budget`` the attention weight that every row receives is summed in
+    ``weights[layer]`` (float32 (B, H, rows)), and :meth:`evict` keeps, in each layer and head, the last
+    ``recent`` rows (default half the budget) and those of the largest sums, ``budget`` in all;
+    :meth:`over` says when ``slack`` more rows than that are held.  Rows carry their positions in their
+    keys, so the others stay what they are.  Pages are handed out and taken back on the host.
+    """
+
+    def __init__(self, cfg: dict, batch: int, max_len: int, device, dtype=torch.bfloat16, page_size: int = 64,
+                 budget: int | None = None, recent: int | None = None, slack: int = 64):
+        import custom_flash_attn
+
+        if budget is not None and not 0 < budget:
+            raise ValueError(f"budget must be positive, got {budget}")
+        self.recent = (0 if budget is None else budget // 2) if recent is None else recent
+        if budget is not None and not 0 <= self.recent <= budget:
+            raise ValueError(f"recent must be between 0 and budget ({budget}), got {recent}")
+        H = cfg["n_heads"]
+        hd = cfg["emb_dim"] // H
+        self.max_len, self.page_size, self.budget, self.slack = max_len, page_size, budget, slack
+        self._columns = -(-max_len // page_size)
+        self._cut_columns = 0 if budget is None else -(-(budget + slack) // page_size)
+        pages = batch * (self._columns + self._cut_columns)
+        layers = range(cfg["n_layers"])
+        self.k = [torch.zeros(pages, H, page_size, hd, dtype=dtype, device=device) for _ in layers]
+        self.v = [torch.zeros(pages, H, page_size, hd, dtype=dtype, device=device) for _ in layers]
+        self.seqlens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.positions = torch.zeros(batch, dtype=torch.int32, device=device)
+        columns = max(self._columns, self._cut_columns)
+        self.weights = None if budget is None else [
+            torch.zeros(batch, H, columns * page_size, dtype=torch.float32, device=device) for _ in layers]
+        nbytes = custom_flash_attn._C.decode_paged_workspace(batch, H, H, page_size, columns, hd, budget is not None)
+        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        self._pages = pages
+        self.reset()
+
+    def _take(self, columns: int):
+        """A table of ``columns`` free pages for each sequence."""
+        batch = self.seqlens.shape[0]
+        ids, self._free = self._free[:batch * columns], self._free[batch * columns:]
+        return torch.tensor(ids, dtype=torch.int32).view(batch, columns).to(self.seqlens.device), ids
+
+    def prompt(self, layer, q, k, v, ctx) -> None:
+        """The prompt's (B, N, H, d) projections: K and V into the pages, the attention into ``ctx``, and
+        the weight each key received into ``weights``."""
+        import custom_flash_attn
+
+        b, n, H, hd = k.shape
+        pages = -(-n // self.page_size)
+        at = self.table[:, :pages].long()
+        for pool, rows in ((self.k[layer], k), (self.v[layer], v)):
+            rows = F.pad(rows, (0, 0, 0, 0, 0, pages * self.page_size - n))
+            pool[at] = rows.view(b, pages, self.page_size, H, hd).transpose(2, 3)
+        q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
+        if self.weights is None:
+            custom_flash_attn.attention(q, k, v, out=ctx.transpose(1, 2))
+        else:
+            _, lse = custom_flash_attn.attention(q, k, v, out=ctx.transpose(1, 2), return_lse=True)
+            custom_flash_attn.key_weights(q, k, lse, out=self.weights[layer][:, :, :n])
+
+    def attend(self, layer, q, k, v, out=None):
+        """One decode step of (B, H, d) projections: the new row appended, the attention over all rows."""
+        import custom_flash_attn
+
+        return custom_flash_attn.decode_paged(q, self.k[layer], self.v[layer], self.table, self.seqlens, k, v, out=out,
+                                              key_weights=None if self.weights is None else self.weights[layer],
+                                              workspace=self.workspace)
+
+    def advance(self, n: int) -> None:
+        self.length += n
+        self.seqlens.add_(n)
+        self.positions.add_(n)
+
+    def over(self) -> bool:
+        """Whether the cache holds ``slack`` rows more than its budget (and the next token needs a cut)."""
+        return self.budget is not None and self.length >= self.budget + self.slack
+
+    def evict(self) -> None:
+        """Cuts every sequence to ``budget`` rows in each layer and head, into other pages."""
+        import custom_flash_attn
+
+        if self.budget is None:
+            raise ValueError("the cache has no budget to be cut to")
+        if self.length <= self.budget:
+            return
+        table, ids = self._take(self._cut_columns)
+        for k, v, w in zip(self.k, self.v, self.weights):
+            custom_flash_attn.evict(k, v, self.table, self.seqlens, w, table, self.budget, recent=self.recent,
+                                    weights_out=w)
+        self._free += self._held
+        self.table, self._held = table, ids
+        self.length = self.budget
+        self.seqlens.clamp_(max=self.budget)
+
+    def reset(self) -> None:
+        self.length = 0
+        self.seqlens.zero_()
+        self.positions.zero_()
+        self._free = list(range(self._pages))
+        self.table, self._held = self._take(self._columns)
 
 
 class GraphedDecoder:
@@ -457,16 +580,13 @@ class TransformerBlock(nn.Module):
         """One decode step as five kernels: norm1 + query/key/value, attention, output projection
         + residual, norm2 + MLP up + GELU, MLP down + residual.  The weights are read in place, so
         the bf16 roundings autocast makes of the attention's weights, input and output fall away."""
-        import custom_flash_attn
-
         g, att, norm1, norm2 = _gpt2(), self.att, self.norm1, self.norm2
         b, _, d = x.shape
         H, hd = att.num_heads, att.head_dim
         q, k, v = (t.view(b, H, hd) for t in g.linear_rows(
             x, [(m.weight, m.bias) for m in (att.W_query, att.W_key, att.W_value)], torch.bfloat16,
             norm=(norm1.scale, norm1.shift, norm1.eps)))
-        ctx = custom_flash_attn.decode(q, cache.k[layer], cache.v[layer], cache.seqlens, k, v,
-                                       workspace=cache.workspace)
+        ctx = cache.attend(layer, q, k, v)
         x, = g.linear_rows(ctx.view(b, 1, d), [(att.out_proj.weight, att.out_proj.bias)], torch.float32, residual=x)
         up, down = self.ff.layers[0], self.ff.layers[2]
         h, = g.linear_rows(x, [(up.weight, up.bias)], torch.float32, norm=(norm2.scale, norm2.shift, norm2.eps), gelu=True)
@@ -530,14 +650,14 @@ class GPTModel(nn.Module):
 
     def _hidden(self, in_idx, kv_cache=None):
         """The last block's output for ``in_idx`` (forward without final norm and head).  With ``kv_cache`` the tokens continue the cached sequence:
-        positions start at the cached length, read from ``kv_cache.seqlens`` on the device (so a
+        positions start at the cached length, read from ``kv_cache.positions`` on the device (so a
         captured decode step stays correct on replay), and the cache advances by the token
         count."""
         _, seq_len = in_idx.shape
         tok_embeds = self.tok_emb(in_idx)
         pos = torch.arange(seq_len, device=in_idx.device)
         if kv_cache is not None:
-            pos = kv_cache.seqlens[:, None].long() + pos  # (B, T)
+            pos = kv_cache.positions[:, None].long() + pos  # (B, T)
         pos_embeds = self.pos_emb(pos)
         x = self.drop_emb(tok_embeds + pos_embeds)
         if kv_cache is None:
@@ -584,14 +704,50 @@ def _next_token(logits, temperature, top_k):
     return torch.argmax(logits, dim=-1, keepdim=True)
 
 
-def generate(model, idx, max_new_tokens, context_size, temperature=1.0, top_k=None, eos_id=None):
+def _penalized(logits, idx, penalties):
+    return logits if penalties is None else penalties(logits, idx)
+
+
+class LogitPenalties:
+    """What a generation loop does to the logits before it samples from them (custom_flash_attn.
+    penalize_logits): tokens that the text holds already have their logit divided (positive) or multiplied by
+    ``repetition`` and lowered by ``presence`` and, for each time, ``frequency`` (numbers, or one float32 per row);
+    ``bias`` ((V,) or (B, V) float32) is added; tokens whose bit is not set in ``allowed`` (int32 words, (ceil(V / 32),)
+    or one row per text, or a function of the text that returns them, as a grammar needs it) are ruled out."""
+
+    def __init__(self, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None):
+        self.repetition, self.presence, self.frequency = repetition, presence, frequency
+        self.bias, self.allowed = bias, allowed
+
+    def __call__(self, logits, idx):
+        allowed = self.allowed(idx) if callable(self.allowed) else self.allowed
+        if logits.is_cuda:
+            import custom_flash_attn  # raises if the native extension is not built
+
+            return custom_flash_attn.penalize_logits(logits, idx, repetition=self.repetition, presence=self.presence,
+                                                     frequency=self.frequency, bias=self.bias, allowed=allowed)
+        column = lambda p: p[:, None] if isinstance(p, torch.Tensor) else p  # noqa: E731
+        x = logits.float()
+        n = torch.zeros_like(x).scatter_add_(1, idx, torch.ones_like(idx, dtype=x.dtype))
+        r = column(self.repetition)
+        x = torch.where(n > 0, torch.where(x > 0, x / r, x * r) - column(self.frequency) * n - column(self.presence), x)
+        if self.bias is not None:
+            x = x + self.bias
+        if allowed is not None:
+            v = torch.arange(x.shape[1], device=x.device)
+            x = x.masked_fill((allowed[..., v // 32] >> (v % 32)) & 1 == 0, float("-inf"))
+        return x.to(logits.dtype)
+
+
+def generate(model, idx, max_new_tokens, context_size, temperature=1.0, top_k=None, eos_id=None, penalties=None):
     """The reference's token loop (model_inference.py:199-228): every step re-runs the model
-    over the last ``context_size`` tokens and samples from the last position's logits."""
+    over the last ``context_size`` tokens and samples from the last position's logits.
+    ``penalties``: a :class:`LogitPenalties` applied to them first, or None."""
     for _ in range(max_new_tokens):
         idx_cond = idx[:, -context_size:]
         with torch.no_grad():
             logits = _last_logits(model, idx_cond)
-        idx_next = _next_token(logits, temperature, top_k)
+        idx_next = _next_token(_penalized(logits, idx, penalties), temperature, top_k)
         if idx_next == eos_id:
             break
         idx = torch.cat((idx, idx_next), dim=1)
@@ -599,22 +755,34 @@ def generate(model, idx, max_new_tokens, context_size, temperature=1.0, top_k=No
 
 
 def generate_cached(model, idx, max_new_tokens, context_size, temperature=1.0, top_k=None,
-                    eos_id=None):
+                    eos_id=None, penalties=None, cache=None):
     """:func:`generate` with a KV cache: one prefill over the prompt, then one decode step per
     new token (the decode kernel, which appends the token's K/V and attends over the cache).
     Same sampling.  The whole sequence must fit ``context_size`` (no sliding window: shifting
-    positions would invalidate the cache)."""
+    positions would invalidate the cache).  ``cache``: a :class:`PagedKVCache` (or another
+    :class:`KVCache`) for this batch to use, from its reset on; one with a budget is cut to it
+    whenever it holds its slack more."""
     if idx.shape[1] + max_new_tokens > context_size:
         raise ValueError(f"prompt ({idx.shape[1]}) + max_new_tokens ({max_new_tokens}) exceeds "
                          f"context_size ({context_size})")
-    cfg = {"n_heads": model.trf_blocks[0].att.num_heads, "emb_dim": model.tok_emb.embedding_dim,
-           "n_layers": len(model.trf_blocks)}
-    cache = KVCache(cfg, idx.shape[0], idx.shape[1] + max_new_tokens, idx.device)
+    if cache is None:
+        cfg = {"n_heads": model.trf_blocks[0].att.num_heads, "emb_dim": model.tok_emb.embedding_dim,
+               "n_layers": len(model.trf_blocks)}
+        cache = KVCache(cfg, idx.shape[0], idx.shape[1] + max_new_tokens, idx.device)
+    else:
+        if cache.seqlens.shape[0] != idx.shape[0]:
+            raise ValueError(f"the cache is for {cache.seqlens.shape[0]} sequences, not {idx.shape[0]}")
+        if cache.max_len < idx.shape[1] + max_new_tokens:
+            raise ValueError("the cache is shorter than prompt + max_new_tokens")
+        cache.reset()
+    paged = isinstance(cache, PagedKVCache)
     step_in = idx
     for _ in range(max_new_tokens):
         with torch.no_grad():
+            if paged and cache.over():
+                cache.evict()
             logits = _last_logits(model, step_in, cache)
-        idx_next = _next_token(logits, temperature, top_k)
+        idx_next = _next_token(_penalized(logits, idx, penalties), temperature, top_k)
         if idx_next == eos_id:
             break
         idx = torch.cat((idx, idx_next), dim=1)
@@ -623,7 +791,7 @@ def generate_cached(model, idx, max_new_tokens, context_size, temperature=1.0, t
 
 
 def generate_graphed(model, idx, max_new_tokens, context_size, temperature=1.0, top_k=None,
-                     eos_id=None, decoder: GraphedDecoder | None = None):
+                     eos_id=None, decoder: GraphedDecoder | None = None, penalties=None):
     """:func:`generate_cached` with every decode step replayed from a :class:`GraphedDecoder`
     (built here unless one for this batch and length is passed in).  Same sampling."""
     if idx.shape[1] + max_new_tokens > context_size:
@@ -636,7 +804,7 @@ def generate_graphed(model, idx, max_new_tokens, context_size, temperature=1.0, 
     decoder.cache.reset()
     logits = decoder.prefill(idx)
     for i in range(max_new_tokens):
-        idx_next = _next_token(logits, temperature, top_k)
+        idx_next = _next_token(_penalized(logits, idx, penalties), temperature, top_k)
         if idx_next == eos_id:
             break
         idx = torch.cat((idx, idx_next), dim=1)
