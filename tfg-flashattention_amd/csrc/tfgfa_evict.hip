@@ -219,7 +219,16 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
   };
   if (chosen > 0 && chosen < old) {
     clear();
-    rows([&](int j, uint32_t y, bool in) { count(in, y >> 21); });
+    rows([&](int j, uint32_t y, bool in) {
+      // (Of most registers every row is in: then a compare says whether all have one digit.)
+      const int digit = y >> 21;
+      if (__builtin_amdgcn_ballot_w64(!in) != 0)
+        count(in, digit);
+      else if (__builtin_amdgcn_ballot_w64(digit != __builtin_amdgcn_readfirstlane(digit)) != 0)
+        atomicAdd(&hist[digit], 1);
+      else if (lane == 0)
+        atomicAdd(&hist[digit], 64);
+    });
     find(21);
     const int same = hist[key >> 21];
     if (kList && same <= kCandidates) {
@@ -262,7 +271,7 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
     }
     return;
   }
-  auto keep = [&](int at, int j, float y) {
+  auto keep = [&](uint32_t at, int j, float y) {
     kept[at] = j;
     out[at] = y;
     if (kR > 0 && a.fused) hist[at & (kBins - 1)] = j;
@@ -271,10 +280,11 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
     // Rows above the key, and ties, of the waves before.  (Every weight is in a register by now: `out` may be `w`.)
     int taken = 0, ties = 0;
     rows([&](int j, uint32_t y, bool in) {
-      taken += __builtin_popcountll(__builtin_amdgcn_ballot_w64(in && y > key));
-      ties += __builtin_popcountll(__builtin_amdgcn_ballot_w64(in && y == key));
+      taken += in && y > key ? 1 : 0;
+      ties += in && y == key ? 1 : 0;
     });
-    if (lane == 0) {
+    taken = scan64(taken), ties = scan64(ties);
+    if (lane == 63) {
       sh_sum[wave] = taken;
       sh_tie[wave] = ties;
     }
@@ -292,7 +302,10 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
       const bool in = j < old;
       const unsigned long long mo = __builtin_amdgcn_ballot_w64(in && q[r] > key);
       const unsigned long long mt = __builtin_amdgcn_ballot_w64(in && q[r] == key);
-      if (mo | mt) {
+      if (mt == 0) {
+        if (in && q[r] > key) keep(taken + min(ties, want) + below(mo), j, x[r]);
+        taken += __builtin_popcountll(mo);
+      } else {
         const int t = ties + below(mt);
         if (in && (q[r] > key || (q[r] == key && t < want))) keep(taken + below(mo) + min(t, want), j, x[r]);
         taken += __builtin_popcountll(mo);
