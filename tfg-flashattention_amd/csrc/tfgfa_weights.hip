@@ -76,6 +76,35 @@ __device__ __forceinline__ int turn(int row) {
   return kChunks == 8 ? tfgfa::swz_k(row) : row & 15;
 }
 
+// The sums over the 32 queries (lanes) of each half of the registers of s, 16 of them: halves of the registers change sides
+// with the lanes that differ in one bit of their number (of the last ones three: any pairing does that flips the bit), so
+// that each step adds half as many.  Lane l ends with register l / 2 % 16.
+__device__ __forceinline__ float over_queries(const float (&sum)[16], int lane) {
+  float s[8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    const auto two = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum[r]), __float_as_uint(sum[r + 8]), false, false);
+    s[r] = __uint_as_float(two[0]) + __uint_as_float(two[1]);
+  }
+  auto halve = [&](auto n, auto turned, int bit) {
+#pragma unroll
+    for (int r = 0; r < decltype(n)::value; ++r) {
+      const float mine = lane & bit ? s[r + decltype(n)::value] : s[r], other = lane & bit ? s[r] : s[r + decltype(n)::value];
+      s[r] = mine + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(other), decltype(turned)::value, 0xF, 0xF,
+                                                               false));
+    }
+  };
+  halve(std::integral_constant<int, 4>(), std::integral_constant<int, 0x128>(), 8);  // 8 lanes on
+  halve(std::integral_constant<int, 2>(), std::integral_constant<int, 0x141>(), 4);  // mirrored in 8 lanes
+  halve(std::integral_constant<int, 1>(), std::integral_constant<int, 0x4E>(), 2);   // 2 lanes on in 4
+  return s[0] + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(s[0]), 0xB1, 0xF, 0xF, false));
+}
+// The key of a wave's 32 whose sum the lane ends with: register r of half h is key 8 (r / 4) + 4 h + r % 4.
+__device__ __forceinline__ int key_of(int lane) {
+  const int r = lane / 2 % 16;
+  return 8 * (r / 4) + 4 * (lane / 32) + r % 4;
+}
+
 // kP: pieces of 16 dims, D <= 16 kP; a lane holds dims 16p + 8 (l / 32) .. + 7 of row l % 32.
 template <class T, int kP>
 __global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(const Args a) {
@@ -154,60 +183,49 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(const Args a) {
     __syncthreads();
     z[0] = next[0] * kLog2e, z[1] = next[1] * kLog2e;
     if (w + 1 < all) load(n ^ 1);
-    f32x16 s[2];
+    // Register r: key 8 (r / 4) + 4 half + r % 4 of the wave's, query i.
+    auto scores = [&](int u) {
+      f32x16 s;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+      for (int r = 0; r < 16; ++r) s[r] = 0.f;
       const unsigned char* const row = &buf[n][(u * kTile + i) * kRowBytes];
 #pragma unroll
       for (int p = 0; p < kP; ++p)
-        s[u] = mfma<T>(kf[p], *reinterpret_cast<const u32x4*>(row + 16 * ((2 * p + half) ^ turn<kChunks>(u * kTile + i))),
-                       s[u]);
-    }
-    // Register r: key 8 (r / 4) + 4 half + r % 4 of the wave's, query i.
-    const bool clear = t >= from && t < upto;
+        s = mfma<T>(kf[p], *reinterpret_cast<const u32x4*>(row + 16 * ((2 * p + half) ^ turn<kChunks>(u * kTile + i))), s);
+      return s;
+    };
+    if (t >= from && t < upto && !__builtin_amdgcn_ballot_w64(fmaxf(fabsf(z[0]), fabsf(z[1])) == INFINITY)) {
+      const f32x16 s[2] = {scores(0), scores(1)};
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const bool live = fabsf(z[u]) != INFINITY;
-      if (clear && !__builtin_amdgcn_ballot_w64(!live)) {
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) sum[r] += __builtin_amdgcn_exp2f(fmaf(s[u][r], scale, -z[u]));
-      } else {
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        // Half a tile without a query, or whose last one sees none of the wave's keys.
+        const int q0 = t * kQueries + u * kTile;
+        if (q0 >= a.Nq || (a.causal && a.first + q0 + kTile - 1 < j0)) continue;
+        const f32x16 s = scores(u);
         // Keys that the lane's query sees: up to `last`.  A row past the last, and one with nothing to see (lse -inf, or
         // past the range in the log2 domain), sees none.
-        const int query = t * kQueries + u * kTile + i;
+        const bool live = fabsf(z[u]) != INFINITY && q0 + i < a.Nq;
         int last = kTile - 1;
-        if (a.causal) last = (int)max(-1LL, min((long long)last, a.first + query - j0));
-        if (!live || query >= a.Nq) last = -1;
+        if (a.causal) last = (int)max(-1LL, min((long long)last, a.first + q0 + i - j0));
+        if (!live) last = -1;
         const float zu = live ? z[u] : 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[u][r], scale, -zu));
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[r], scale, -zu));
           sum[r] += 8 * (r / 4) + 4 * half + r % 4 <= last ? p : 0.f;
         }
       }
     }
     if (++t == tiles) t = t0;
   }
-  // Over the 32 queries of each half: rotations inside 16 lanes, then the two 16s.  Lane i < 16 keeps register i.
-  float x = 0.f;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    float y = sum[r];
-    auto add = [&](auto c) {
-      y += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(y), decltype(c)::value, 0xF, 0xF, false));
-    };
-    add(std::integral_constant<int, 0x121>());
-    add(std::integral_constant<int, 0x122>());
-    add(std::integral_constant<int, 0x124>());
-    add(std::integral_constant<int, 0x128>());
-    const auto two = __builtin_amdgcn_permlane16_swap(__float_as_uint(y), __float_as_uint(y), false, false);
-    y = __uint_as_float(two[0]) + __uint_as_float(two[1]);
-    x = i == r ? y : x;
-  }
-  const int j = j0 + 8 * (i / 4) + 4 * half + i % 4;
-  if (i < 16 && j < a.Nk) a.out[b * a.ob + kv * a.oh + j] = x;
+  const int j = j0 + key_of(lane);
+  const float x = over_queries(sum, lane);
+  if ((lane & 1) == 0 && j < a.Nk) a.out[b * a.ob + kv * a.oh + j] = x;
 }
 
 }  // namespace tfgfa_weights
@@ -249,8 +267,8 @@ extern "C" int tfserve_key_weights(const void* q, const int64_t* q_strides, cons
   a.units = B * H_kv;
   const int st = tfgfa_device_info(&a.cu, nullptr, nullptr, 0);
   if (st != TFGFA_OK) return st;
-  const dim3 grid((unsigned)((N_k + kKeys - 1) / kKeys * units));
   const hipStream_t stream = (hipStream_t)hip_stream;
+  const dim3 grid((unsigned)((N_k + kKeys - 1) / kKeys * units));
 #define TFGFA_WEIGHTS(T)                                                                            \
   do {                                                                                              \
     if (D <= 64)                                                                                    \
