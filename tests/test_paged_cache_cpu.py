@@ -36,11 +36,23 @@ def test_pages_are_held_or_free_once(monkeypatch):
     assert c.table.shape == (3, 7) and c.length == 0
 
 
+def test_cuts_again_where_budget_and_slack_pass_the_longest_text(monkeypatch):
+    monkeypatch.setattr(custom_flash_attn, "evict", lambda *a, **kw: None)
+    c = mi.PagedKVCache(CFG, 2, 50, "cpu", page_size=8, budget=10, slack=1000)
+    for _ in range(4):
+        c.advance(9)
+        c.evict()
+        assert c.table.shape == (2, 7) and c.length == min(10, int(c.positions[0]))
+        assert sorted(c.table.flatten().tolist() + c._free) == list(range(28))
+
+
 def test_paged_cache_refuses_budgets_that_make_no_sense():
     with pytest.raises(ValueError, match="budget must be positive"):
         mi.PagedKVCache(CFG, 1, 50, "cpu", budget=0)
     with pytest.raises(ValueError, match="recent must be between"):
         mi.PagedKVCache(CFG, 1, 50, "cpu", budget=10, recent=11)
+    with pytest.raises(ValueError, match="slack must be positive"):  # the row after a cut needs a place
+        mi.PagedKVCache(CFG, 1, 50, "cpu", budget=16, page_size=8, slack=0)
     with pytest.raises(ValueError, match="no budget"):
         mi.PagedKVCache(CFG, 1, 50, "cpu").evict()
 

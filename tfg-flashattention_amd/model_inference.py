@@ -321,21 +321,23 @@ class PagedKVCache:
         self.recent = (0 if budget is None else budget // 2) if recent is None else recent
         if budget is not None and not 0 <= self.recent <= budget:
             raise ValueError(f"recent must be between 0 and budget ({budget}), got {recent}")
+        if budget is not None and slack < 1:
+            raise ValueError(f"slack must be positive, got {slack}")
         H = cfg["n_heads"]
         hd = cfg["emb_dim"] // H
         self.max_len, self.page_size, self.budget, self.slack = max_len, page_size, budget, slack
         self._columns = -(-max_len // page_size)
-        self._cut_columns = 0 if budget is None else -(-(budget + slack) // page_size)
+        # (A text of max_len tokens never needs more rows than that, cut or not.)
+        self._cut_columns = 0 if budget is None else min(self._columns, -(-(budget + slack) // page_size))
         pages = batch * (self._columns + self._cut_columns)
         layers = range(cfg["n_layers"])
         self.k = [torch.zeros(pages, H, page_size, hd, dtype=dtype, device=device) for _ in layers]
         self.v = [torch.zeros(pages, H, page_size, hd, dtype=dtype, device=device) for _ in layers]
         self.seqlens = torch.zeros(batch, dtype=torch.int32, device=device)
         self.positions = torch.zeros(batch, dtype=torch.int32, device=device)
-        columns = max(self._columns, self._cut_columns)
         self.weights = None if budget is None else [
-            torch.zeros(batch, H, columns * page_size, dtype=torch.float32, device=device) for _ in layers]
-        nbytes = custom_flash_attn._C.decode_paged_workspace(batch, H, H, page_size, columns, hd, budget is not None)
+            torch.zeros(batch, H, self._columns * page_size, dtype=torch.float32, device=device) for _ in layers]
+        nbytes = custom_flash_attn._C.decode_paged_workspace(batch, H, H, page_size, self._columns, hd, budget is not None)
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
         self._pages = pages
         self.reset()
