@@ -197,6 +197,7 @@ def _penalize(lib, **kw):
     (dict(kind=3), "ERR_DTYPE"),
     (dict(tb=2), "ERR_DTYPE"),
     (dict(T=-1), "ERR_BAD_SHAPE"),
+    (dict(T=2 ** 31 - 300), "ERR_TOO_LARGE"),   # a loop's step past the last token passes 2^31
     (dict(rep=0.0), "ERR_SCALE"),
     (dict(rep=float("nan")), "ERR_SCALE"),
     (dict(pres=float("inf")), "ERR_SCALE"),

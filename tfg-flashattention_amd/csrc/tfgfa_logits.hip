@@ -128,7 +128,7 @@ extern "C" int tfserve_penalize(const void* logits, int64_t logits_stride, void*
   if (!repetitions && (!(repetition > 0.f) || !isfinite(repetition))) return TFGFA_ERR_SCALE;
   if ((!presences && !isfinite(presence)) || (!frequencies && !isfinite(frequency))) return TFGFA_ERR_SCALE;
   if (B == 0 || V == 0) return TFGFA_OK;
-  if (B > 65535 || V > INT32_MAX - kChunk || T > INT32_MAX - kThreads) return TFGFA_ERR_TOO_LARGE;
+  if (B > 65535 || V > INT32_MAX - kChunk || T > INT32_MAX - kThreads * kTokens) return TFGFA_ERR_TOO_LARGE;
   if (B > 1 && (logits_stride < 0 || out_stride < V || (T > 0 && tokens_stride < 0) || bias_stride < 0 ||
                 allowed_stride < 0))
     return TFGFA_ERR_STRIDE;
