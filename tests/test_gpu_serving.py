@@ -247,6 +247,84 @@ def test_decode_paged_rows_without_a_finite_score(page):
     _near(o[2, 0], mean, _half(BF) * (mean.abs() + 200 * U * a) + 200 * U * a, "equal lowest scores")
 
 
+@pytest.mark.parametrize("page,dtype,D", [(16, BF, 64), (5, BF, 64), (64, HF, 64), (7, HF, 128), (128, BF, 128), (3, BF, 40)])
+def test_decode_paged_infinite_values_and_nan_queries(page, dtype, D):
+    """An infinite value with weight makes its dim infinite; a query of NaN makes its own head NaN.  The other dims, and
+    the other heads of the key-value head, keep their accuracy."""
+    g = _gen(20 + page)
+    H, H_kv, L = 8, 2, 700
+    c = Paged(g, [L, L, 0], H_kv, D, page, dtype, sigma=0.5)
+    q = _randn((3, H, D), g, dtype)
+    rows = [[t.clone() for t in r] for r in c.rows]
+    for j, d, x in ((3, 7, INF), (600, 9, -INF), (650, 9, -INF)):
+        rows[0][1][1, j, d] = x
+        c.row(c.v, 0, j)[1, d] = x
+    q[1, 2, 5] = NAN
+    o, lse = fa.decode_paged(q, c.k, c.v, c.table, c.seqlens, return_lse=True)
+    torch.cuda.synchronize()
+    finite = rows[0][1].clone()
+    finite[torch.isinf(finite)] = 0
+    ro, rl, _, eo, el, _ = attend(q[0], rows[0][0], finite, D ** -0.5)
+    assert (o[0, 4:, 7] == INF).all() and (o[0, 4:, 9] == -INF).all()
+    got = o[0].clone()
+    got[4:, 7], got[4:, 9] = ro[4:, 7].to(got), ro[4:, 9].to(got)
+    _near(got, ro, eo + _half(dtype) * (ro.abs() + eo), "beside infinite values")
+    _near(lse[0], rl, el, "lse")
+    assert torch.isnan(o[1, 2]).all() and torch.isnan(lse[1, 2])
+    clean = q[1].clone()
+    clean[2] = 0
+    ro, rl, _, eo, el, _ = attend(clean, *rows[1], D ** -0.5)
+    others = [h for h in range(H) if h != 2]
+    _near(o[1, others], ro[others], (eo + _half(dtype) * (ro.abs() + eo))[others], "beside a head of NaN")
+    _near(lse[1, others], rl[others], el[others], "lse")
+    assert (o[2] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_decode_paged_many_small_weights(dtype):
+    """20000 rows of weight e^-17.4 beside one of weight 1, whose values are 0: fp16's smallest number is 6e-8, these
+    weights 3e-8.  A weight below 2^-24 is kept to 2^-38 of the largest."""
+    g = _gen(31)
+    D, L, page = 64, 20000, 64
+    c = Paged(g, [L], 1, D, page, dtype)
+    (k, v), = c.rows
+    k.zero_()
+    k[0, 1:, 0] = -17.4
+    v.add_(1.0)
+    v[0, 0] = 0
+    for j in range(0, L, page):
+        m = min(page, L - j)
+        c.k[int(c.table[0, j // page]), :, :m] = k[:, j:j + m]
+        c.v[int(c.table[0, j // page]), :, :m] = v[:, j:j + m]
+    q = torch.zeros(1, 1, D, dtype=dtype, device=DEV)
+    q[..., 0] = 1
+    ws = torch.empty(0, dtype=torch.uint8, device=DEV)   # (not divided: a quarter of the rows beside the first)
+    o = fa.decode_paged(q, c.k, c.v, c.table, c.seqlens, softmax_scale=1.0, workspace=ws)
+    ro, _, _, eo, _, _ = attend(q[0], k, v, 1.0)
+    small = 2.0 ** -38 * v[0].double().abs().sum(0).cpu()
+    _near(o[0], ro, eo + small + _half(dtype) * (ro.abs() + eo + small) + 2.0 ** -25, "o")
+
+
+def test_decode_paged_divides_more_than_64_sequences():
+    """The division of the work takes lengths 64 at a time."""
+    g = _gen(32)
+    B, H, D, page = 150, 1, 64, 32
+    lens = torch.randint(0, 700, (B,), generator=g).tolist()
+    lens[3], lens[70], lens[149], lens[64], lens[127] = 5000, 3000, 2500, 0, 1
+    c = Paged(g, lens, H, D, page, BF, spare=1)
+    q, kn, vn = (_randn((B, H, D), g, BF) for _ in range(3))
+    assert _C.decode_paged_workspace(B, H, H, page, c.table.shape[1], D, False) > 0
+    sums = torch.zeros(B, H, c.table.shape[1] * page, device=DEV)
+    o, lse = fa.decode_paged(q, c.k, c.v, c.table, c.seqlens, kn, vn, return_lse=True, key_weights=sums)
+    torch.cuda.synchronize()
+    for b in range(B):
+        k, v = (torch.cat([t, n[b][:, None]], 1) for t, n in zip(c.rows[b], (kn, vn)))
+        ro, rl, w, eo, el, ew = attend(q[b], k, v, D ** -0.5)
+        for got, want, bound in ((o[b], ro, eo + _half(BF) * (ro.abs() + eo)), (lse[b], rl, el),
+                                 (sums[b, :, :lens[b] + 1], w, ew + 2 * U * w)):
+            assert ((got.double().cpu() - want).abs() <= bound).all(), (b, lens[b])
+
+
 @pytest.mark.parametrize("H,H_kv,D,page,dtype,append", [
     (12, 12, 64, 16, BF, True), (8, 2, 128, 64, HF, True), (20, 1, 64, 10, BF, False), (4, 4, 40, 32, BF, True)])
 def test_decode_paged_adds_key_weights(H, H_kv, D, page, dtype, append):

@@ -14,8 +14,9 @@
 // contraction runs over keys, whose order is free).  Its A operand wants 8 keys' values of one dim in a lane:
 // the lane loads kDV neighbouring dims of each of the 8 rows, and byte permutes put the keys of a dim side by side.
 // So neither P nor V moves between lanes.  P is split as hi + lo, each rounded to the element type, which keeps 16
-// (bf16) or 22 (fp16) of its bits; rounding it once would cost as much as the output's own rounding.  An infinite V
-// makes NaN of a lo of 0 or below; a wave whose sums hold NaN takes its keys again with hi alone.  (With P and V
+// (bf16) or 22 (fp16) of its bits; rounding it once would cost as much as the output's own rounding.  (fp16 ends at 2^-24:
+// its P is carried times 2^13, so that weights are kept to 2^-38 of the largest.)  An infinite V
+// makes NaN of a lo of 0 or below; a wave whose sums hold NaN takes its keys again with hi alone, for those sums.  (With P and V
 // as float32 on v_mfma_f32_16x16x4_f32 a block of 32 keys took 1024 matrix cycles at D = 64 instead of 192.)
 //
 // Division of the work.  A unit is a (sequence, key-value head, 16 query heads).  The lengths are known on
@@ -64,14 +65,17 @@ constexpr int kGranule = kWaves * kBlock;     // keys of a workgroup's block
 constexpr int kMaxParts = 64;                 // workgroups of a unit
 // A buffer offset past any num_records built here: the load returns zero without a memory access.
 constexpr uint32_t kOutOfRange = 0x7FFFFFF0u;
-constexpr float kSlack = 8.f;
 constexpr int kScoreTail = 4;                 // a head's scores end with a place for the new row's
 constexpr int kPolicyCoherent = 16;           // buffer loads from the device's coherence point (sc1)
 
 template <class T>
 struct Elem;
+// kShift: P is carried times 2^kShift.  kSlack: how far a score may pass its head's offset; e^kSlack 2^kShift is a number
+// of the type.
 template <>
 struct Elem<__bf16> {
+  static constexpr int kShift = 0;
+  static constexpr float kSlack = 8.f;
   typedef __bf16 x2 __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
@@ -80,6 +84,8 @@ struct Elem<__bf16> {
 };
 template <>
 struct Elem<_Float16> {
+  static constexpr int kShift = 13;
+  static constexpr float kSlack = 2.f;
   typedef _Float16 x2 __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c,
@@ -127,7 +133,7 @@ struct Args {
   Vecs qs, os, kns, vns;
   long long n_pad;
   float scale, scale_log2;
-  float slack;      // kSlack in scores without the scale
+  float slack;      // Elem::kSlack in scores without the scale
   int H, G, P, page, D;
   int tiles;        // 16-head tiles of a key-value head
   int min_granules; // smallest part
@@ -447,7 +453,20 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
 
   float m, l;
   f32x4 acc[kDV];
-  bool both = true;  // hi and lo of P
+  // Hi and lo of P: 1 or 0, kept in a scalar register.  (A branch on what the compiler takes for a value of each lane only
+  // masks lanes, and a matrix instruction runs whatever the mask.)
+  int both = __builtin_amdgcn_readfirstlane(1);
+  // The wave's sums into LDS.  acc[j], register r of lane (g, i): dim kDV (4g + r) + j of head i.
+  auto leave = [&]() {
+    if (i < nh) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < kDV; j += 4)
+          *reinterpret_cast<f32x4*>(&sh_o[(wave * kHeads + i) * kRow + kDV * (4 * g + r) + j]) =
+              f32x4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]};
+    }
+  };
 
   // The arithmetic of block x.  kMore: another block follows, whose K goes out once the scores have read this one's, and
   // its V once the output has, so that one of the two is always in flight with one set of registers.
@@ -513,8 +532,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
                   f32x4{s[t][0], s[t][1], s[t][2], s[t][3]} * a.scale;
         }
       }
-      // The offset of each head moves only when a score passes it by kSlack (weights up to e^kSlack leave the float32
-      // sums their range), so that lanes compare notes in few blocks.
+      // The offset of each head moves only when a score passes it by the slack, so that lanes compare notes in few blocks.
       float mb = s[0][0];
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)
@@ -535,8 +553,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
       for (int t = 0; t < kTiles; ++t)
 #pragma unroll
         for (int r = 0; r < 4; r += 2) {
-          const float p0 = __builtin_amdgcn_exp2f((s[t][r] - mu) * a.scale_log2);
-          const float p1 = __builtin_amdgcn_exp2f((s[t][r + 1] - mu) * a.scale_log2);
+          float x0 = (s[t][r] - mu) * a.scale_log2, x1 = (s[t][r + 1] - mu) * a.scale_log2;
+          if constexpr (Elem<T>::kShift != 0) x0 += Elem<T>::kShift, x1 += Elem<T>::kShift;
+          const float p0 = __builtin_amdgcn_exp2f(x0), p1 = __builtin_amdgcn_exp2f(x1);
           l += p0 + p1;
           float r0, r1, none;
           hi[t / 2][2 * (t % 2) + r / 2] = pack<T>(p0, p1, &r0, &r1);
@@ -569,7 +588,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
                             pair_hi(vb[2][e], vb[3][e])};
           acc[2 * e] = Elem<T>::mfma(v0, hi[t / 2], acc[2 * e]);
           acc[2 * e + 1] = Elem<T>::mfma(v1, hi[t / 2], acc[2 * e + 1]);
-          if (both) {
+          if (__builtin_amdgcn_readfirstlane(both)) {
             acc[2 * e] = Elem<T>::mfma(v0, lo[t / 2], acc[2 * e]);
             acc[2 * e + 1] = Elem<T>::mfma(v1, lo[t / 2], acc[2 * e + 1]);
           }
@@ -602,8 +621,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
     for (int j = 0; j < kDV; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) any = fmaf(acc[j][r], 0.f, any);
-    if (!both || !__builtin_amdgcn_ballot_w64(any != any)) break;
-    both = false;
+    if (!__builtin_amdgcn_readfirstlane(both) || !__builtin_amdgcn_ballot_w64(any != any)) break;
+    leave();  // (the sums that are not NaN are kept)
+    both = __builtin_amdgcn_readfirstlane(0);
     look_up(ids, kb0);
   }
   if (kDivide && S > 1 && wave == 0 && lane == 0 && (aw_start >> tfgfa::kTagShift) != a.tag) {
@@ -613,19 +633,21 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
   }
 
   m *= a.scale;
-  // Join the waves.  acc[j], register r of lane (g, i): dim kDV (4g + r) + j of head i.
+  // Join the waves.
   l = over_rows(l, [](float u, float w) { return u + w; });
-  if (i < nh) {
+  if (!both && i < nh) {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int j = 0; j < kDV; j += 4)
-        *reinterpret_cast<f32x4*>(&sh_o[(wave * kHeads + i) * kRow + kDV * (4 * g + r) + j]) =
-            f32x4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]};
-    if (g == 0) {
-      sh_m[wave][i] = m;
-      sh_l[wave][i] = l;
-    }
+      for (int j = 0; j < kDV; ++j) {
+        const float first = sh_o[(wave * kHeads + i) * kRow + kDV * (4 * g + r) + j];
+        if (first == first) acc[j][r] = first;
+      }
+  }
+  leave();
+  if (i < nh && g == 0) {
+    sh_m[wave][i] = m;
+    sh_l[wave][i] = l;
   }
   __syncthreads();
   const long long part = part_floats(D);
@@ -645,6 +667,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
       lt = fmaf(f, sh_l[w][h], lt);
       ot = fmaf(f, sh_o[(w * kHeads + h) * kRow + d], ot);
     }
+    constexpr float kBack = 1.f / (1 << Elem<T>::kShift);
+    lt *= kBack, ot *= kBack;
     if (S > 1) {
       __hip_atomic_store(mine + h * D + d, ot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       if (d < 2)
@@ -958,7 +982,7 @@ extern "C" int tfserve_decode_paged(
   a.scores = weights ? reinterpret_cast<float*>(ws + lay.scores) : nullptr;
   a.tag = f.target ? tfgfa::next_tag() : 0;
   a.n_pad = padded(n_max);
-  a.scale = softmax_scale, a.scale_log2 = softmax_scale * kLog2e, a.slack = std::min(kSlack / softmax_scale, 1e30f);
+  a.scale = softmax_scale, a.scale_log2 = softmax_scale * kLog2e, a.slack = std::min((dtype == TFGFA_DTYPE_BF16 ? Elem<__bf16>::kSlack : Elem<_Float16>::kSlack) / softmax_scale, 1e30f);
   a.H = H, a.G = H / H_kv, a.P = P, a.page = page, a.D = D;
   a.min_granules = min_granules(a.G);
   const tfgfa::Division by_page = tfgfa::division_by(page);
