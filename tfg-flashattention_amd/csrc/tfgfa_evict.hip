@@ -415,7 +415,7 @@ extern "C" int tfserve_evict(void* k_pages, const int64_t* k_strides, void* v_pa
   a.fused = n_max <= kMaxRows && rows <= kMaxFused && (long long)rows * D <= kFusedValues;
   const hipStream_t stream = (hipStream_t)hip_stream;
   if (n_max <= 1024)
-    launch<4, 4>(a, B, stream);
+    launch<8, 2>(a, B, stream);
   else if (n_max <= 4096)
     launch<16, 4>(a, B, stream);
   else if (n_max <= kMaxRows)

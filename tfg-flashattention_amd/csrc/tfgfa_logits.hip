@@ -16,8 +16,8 @@ namespace tfgfa_logits {
 
 constexpr int kThreads = 256;
 constexpr int kEach = 4;              // neighbouring logits of a lane
-constexpr int kSteps = 4;
-constexpr int kChunk = kThreads * kEach * kSteps;
+constexpr int kMaxSteps = 4;
+constexpr int kFewSteps = 1;
 constexpr int kTokens = 4;            // tokens of the history that a lane loads at once
 
 struct Args {
@@ -42,8 +42,10 @@ struct Pack {
   typedef v __attribute__((aligned(sizeof(E)))) any;
 };
 
-template <class E>
+// kSteps: of kThreads * kEach logits in a workgroup's chunk.
+template <class E, int kSteps>
 __global__ __launch_bounds__(kThreads) void penalize_kernel(const Args a) {
+  constexpr int kChunk = kThreads * kEach * kSteps;
   __shared__ int count[kChunk];
   const int tid = threadIdx.x, b = blockIdx.y, v0 = blockIdx.x * kChunk;
   const E* const x = static_cast<const E*>(a.x) + b * a.xs;
@@ -128,7 +130,7 @@ extern "C" int tfserve_penalize(const void* logits, int64_t logits_stride, void*
   if (!repetitions && (!(repetition > 0.f) || !isfinite(repetition))) return TFGFA_ERR_SCALE;
   if ((!presences && !isfinite(presence)) || (!frequencies && !isfinite(frequency))) return TFGFA_ERR_SCALE;
   if (B == 0 || V == 0) return TFGFA_OK;
-  if (B > 65535 || V > INT32_MAX - kChunk || T > INT32_MAX - kThreads * kTokens) return TFGFA_ERR_TOO_LARGE;
+  if (B > 65535 || V > INT32_MAX - kThreads * kEach * kMaxSteps || T > INT32_MAX - kThreads * kTokens) return TFGFA_ERR_TOO_LARGE;
   if (B > 1 && (logits_stride < 0 || out_stride < V || (T > 0 && tokens_stride < 0) || bias_stride < 0 ||
                 allowed_stride < 0))
     return TFGFA_ERR_STRIDE;
@@ -146,14 +148,27 @@ extern "C" int tfserve_penalize(const void* logits, int64_t logits_stride, void*
   if (B > 1) a.xs = logits_stride, a.ys = out_stride, a.ts = tokens_stride, a.bs = bias_stride, a.as = allowed_stride;
   a.rep = repetition, a.pres = presence, a.freq = frequency;
   a.token_bytes = token_bytes, a.V = V, a.T = T;
-  const dim3 grid((V + kChunk - 1) / kChunk, B);
+  int cu = 0;
+  const int st = tfgfa_device_info(&cu, nullptr, nullptr, 0);
+  if (st != TFGFA_OK) return st;
+  // Long chunks where they make workgroups enough, four a CU: each reads its row's history.
+  const int steps = (long long)B * (V / (kThreads * kEach * kMaxSteps)) >= 4LL * cu ? kMaxSteps : kFewSteps;
+  const dim3 grid((V + kThreads * kEach * steps - 1) / (kThreads * kEach * steps), B);
   const hipStream_t stream = (hipStream_t)hip_stream;
+#define TFGFA_PENALIZE(E)                                                                            \
+  do {                                                                                               \
+    if (steps == kMaxSteps)                                                                          \
+      hipLaunchKernelGGL((penalize_kernel<E, kMaxSteps>), grid, dim3(kThreads), 0, stream, a);       \
+    else                                                                                             \
+      hipLaunchKernelGGL((penalize_kernel<E, kFewSteps>), grid, dim3(kThreads), 0, stream, a);       \
+  } while (0)
   if (kind == TFSERVE_LOGITS_F32)
-    hipLaunchKernelGGL((penalize_kernel<float>), grid, dim3(kThreads), 0, stream, a);
+    TFGFA_PENALIZE(float);
   else if (kind == TFSERVE_LOGITS_BF16)
-    hipLaunchKernelGGL((penalize_kernel<__bf16>), grid, dim3(kThreads), 0, stream, a);
+    TFGFA_PENALIZE(__bf16);
   else
-    hipLaunchKernelGGL((penalize_kernel<_Float16>), grid, dim3(kThreads), 0, stream, a);
+    TFGFA_PENALIZE(_Float16);
+#undef TFGFA_PENALIZE
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? TFGFA_OK : -(int)e;
 }

@@ -815,7 +815,7 @@ constexpr int kSlots = 2;
 // Sequences of at most kWhole rows are not divided.
 constexpr int kWhole = 512;
 // A part writes and reads back its heads' outputs: a granule's worth of K and V for every 16 heads' 4 granules.
-static int min_granules(int G) { return std::max(1, std::min(kHeads, G) / 4); }
+static int min_granules(int G) { return (int)lround(sqrt((double)std::min(kHeads, G))); }
 constexpr int kMaxCu = 1024;  // for the workspace's size, which does not depend on the device
 
 static long long padded(long long n) { return (n + kGranule - 1) / kGranule * kGranule + kScoreTail; }
@@ -838,7 +838,7 @@ static Layout layout(long long units, long long wgs, long long bh, long long n_m
 static int choose_target(long long units, int B, long long n_max, int cu_count) {
   const long long per = units * B;
   // (Past 2^21 granules the plan's quotients are not exact.)
-  if (n_max <= kWhole || per >= (long long)kSlots * 2 * cu_count || (n_max / kGranule + 1) * B >= 1 << 20)
+  if (n_max <= (B == 1 ? kWhole : 2 * kWhole) || per >= (long long)kSlots * 2 * cu_count || (n_max / kGranule + 1) * B >= 1 << 20)
     return 0;
   const long long target = std::max(1LL, (long long)kSlots * cu_count / units);
   if (B > 1) return (int)target;
@@ -868,9 +868,7 @@ static void launch_full(const First& f, const Args& a, unsigned wgs, hipStream_t
     if (f.target) TFGFA_PAGED_(kSpan, true); \
     else TFGFA_PAGED_(kSpan, false);       \
   } while (0)
-  if (a.page % kBlock == 0)
-    TFGFA_PAGED(kBlock);
-  else if (a.page % kTile == 0)
+  if (a.page % kTile == 0)
     TFGFA_PAGED(kTile);
   else
     TFGFA_PAGED(1);
