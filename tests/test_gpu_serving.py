@@ -353,6 +353,45 @@ def test_decode_paged_adds_key_weights(H, H_kv, D, page, dtype, append):
         _near(sums[b], want, bound, f"L={n} sums")
 
 
+@pytest.mark.parametrize("H,H_kv,D,page,dtype,append,lens", [
+    (12, 12, 64, 16, BF, True, [3000, 0, 1, 1023, 1025]),
+    (6, 2, 40, 100, HF, True, [5000, 130, 0]),
+    (8, 2, 128, 64, BF, False, [4000, 128]),
+    (16, 1, 64, 32, BF, True, [1000]),
+    (2, 2, 64, 7, HF, True, [2300, 17]),        # a table of rows that are no multiple of 4
+    (4, 4, 64, 64, BF, True, [9000, 2048, 40]),
+    (16, 1, 64, 64, BF, True, [3000, 700]),
+    (3, 3, 64, 64, BF, True, [4097]),
+])
+def test_decode_paged_adds_key_weights_of_long_caches(H, H_kv, D, page, dtype, append, lens):
+    """The same where a cache is divided over workgroups, twice over; sums that were there stay under the new ones."""
+    g = _gen(40 + H + page)
+    c = Paged(g, lens, H_kv, D, page, dtype, spare=1 if append else 0)
+    B, M = len(lens), c.table.shape[1]
+    q = _randn((B, H, D), g, dtype)
+    kn, vn = (_randn((B, H_kv, D), g, dtype), _randn((B, H_kv, D), g, dtype)) if append else (None, None)
+    sums = torch.rand(B, H_kv, M * page, generator=g).to(DEV)
+    before = sums.double().cpu()
+    other = sums.clone()
+    o, lse = fa.decode_paged(q, c.k, c.v, c.table, c.seqlens, kn, vn, key_weights=sums, return_lse=True)
+    fa.decode_paged(q, c.k, c.v, c.table, c.seqlens, kn, vn, key_weights=other)
+    plain, plain_lse = fa.decode_paged(q, c.k, c.v, c.table, c.seqlens, kn, vn, return_lse=True)
+    torch.cuda.synchronize()
+    assert torch.equal(sums, other) and torch.equal(o, plain) and torch.equal(lse, plain_lse)
+    for b, n in enumerate(lens):
+        k, v = c.rows[b]
+        if append:
+            k, v = torch.cat([k, kn[b][:, None]], 1), torch.cat([v, vn[b][:, None]], 1)
+        _, _, w, _, _, ew = attend(q[b], k, v, D ** -0.5)
+        want = before[b].clone()
+        if append:
+            want[:, n] = 0
+        want[:, :w.shape[1]] += w
+        bound = torch.zeros_like(want)
+        bound[:, :w.shape[1]] = ew + (H // H_kv + 2) * U * want[:, :w.shape[1]]
+        _near(sums[b], want, bound, f"L={n} sums")
+
+
 def test_decode_paged_workspaces():
     """A workspace of any content and size: the division needs the whole of it, key weights refuse less."""
     g = _gen(8)

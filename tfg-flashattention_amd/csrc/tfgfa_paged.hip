@@ -137,6 +137,8 @@ struct Args {
   int H, G, P, page, D;
   int tiles;        // 16-head tiles of a key-value head
   int min_granules; // smallest part
+  float* weights;   // key_weights where the workgroup that ends a unit adds them, or null; strides
+  long long wb, wh;
 };
 
 // The arguments that a kernel has before Args.  units: of one sequence, Hkv * tiles; target: parts of a unit that the
@@ -281,7 +283,7 @@ typedef const __attribute__((address_space(4))) int* uniform_ints;
 // block (32), a tile (16) or 1, by the page size's multiples.  kDivide: sequences may be divided (grid: flat; otherwise units by sequences).
 // The first 14 dwords of the arguments are preloaded into scalar registers (-amdgpu-kernarg-preload-count): what the
 // first loads, of the length and of the first block's pages, wait for.
-template <class T, int kDV, bool kFull, int kSpan, bool kDivide>
+template <class T, int kDV, bool kFull, int kSpan, bool kDivide, bool kFused>
 __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restrict__ table, const int* __restrict__ lens,
                                                             long long table_stride, const T* __restrict__ q, int n_max,
                                                             uint32_t div_m, int div_s, int target, int units, int B,
@@ -292,7 +294,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
   // The waves' outputs; later the shares of a unit's parts and the sums of the groups that join them.
   constexpr int kLds = kWaves * kHeads * kRow, kLdsJoin = kHeads * kMaxParts + 4 * kThreads;
   __shared__ __attribute__((aligned(16))) float sh_o[kLds > kLdsJoin ? kLds : kLdsJoin];
-  __shared__ float sh_m[kWaves][kHeads], sh_l[kWaves][kHeads];
+  __shared__ float sh_m[kWaves][kHeads], sh_l[kWaves][kHeads], sh_lse[kHeads];
   __shared__ int sh_last;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, i = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -521,15 +523,28 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
           }
       }
       if (a.scores != nullptr && i < nh) {
-        float* const to = a.scores + ((long long)b * a.H + h0 + i) * a.n_pad;
-        if (x.fresh) {
-          if (g == 0) to[a.n_pad - kScoreTail] = s[0][0] * a.scale;
-        } else {
+        if constexpr (kFused) {  // for the workgroup that ends the unit, to the coherence point
+          const __amdgpu_buffer_rsrc_t sr = rows_rsrc(a.scores + ((long long)b * a.H + h0) * a.n_pad, INT32_MAX / 2);
+          const int head = i * (int)a.n_pad;
 #pragma unroll
-          for (int t = 0; t < kTiles; ++t)
-            if (t * kTile < x.rows)
-              *reinterpret_cast<f32x4*>(to + x.at + t * kTile + 4 * g) =
-                  f32x4{s[t][0], s[t][1], s[t][2], s[t][3]} * a.scale;
+          for (int t = 0; t < kTiles; ++t) {
+            const f32x4 y = f32x4{s[t][0], s[t][1], s[t][2], s[t][3]} * a.scale;
+            const int at = x.fresh ? (t == 0 && g == 0 ? head + (int)a.n_pad - kScoreTail : -1)
+                                   : (t * kTile < x.rows ? head + x.at + t * kTile + 4 * g : -1);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), sr,
+                                                   at < 0 ? (int)kOutOfRange : at * 4, 0, kPolicyCoherent);
+          }
+        } else {
+          float* const to = a.scores + ((long long)b * a.H + h0 + i) * a.n_pad;
+          if (x.fresh) {
+            if (g == 0) to[a.n_pad - kScoreTail] = s[0][0] * a.scale;
+          } else {
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+              if (t * kTile < x.rows)
+                *reinterpret_cast<f32x4*>(to + x.at + t * kTile + 4 * g) =
+                    f32x4{s[t][0], s[t][1], s[t][2], s[t][3]} * a.scale;
+          }
         }
       }
       // The offset of each head moves only when a score passes it by the slack, so that lanes compare notes in few blocks.
@@ -632,6 +647,53 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
                                          __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
 
+  // key_weights of the unit's heads (no other unit has this key-value head), by the workgroup that ends it and has left
+  // their LSE in LDS.
+  auto add_weights = [&]() {
+    const __amdgpu_buffer_rsrc_t wr = rows_rsrc(a.weights + b * a.wb + kv * a.wh, INT32_MAX / 2);
+    const __amdgpu_buffer_rsrc_t sr = rows_rsrc(a.scores + ((long long)b * a.H + h0) * a.n_pad, INT32_MAX / 2);
+    auto store = [&](float x, int at) {
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), wr, at < 0 ? (int)kOutOfRange : at * 4, 0, 0);
+    };
+    if (append && wave == kWaves - 1) {  // the new row's
+      const float z = lane < nh ? sh_lse[lane] : INFINITY;
+      const float x = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+          sr, lane < nh ? (lane * (int)a.n_pad + (int)a.n_pad - kScoreTail) * 4 : (int)kOutOfRange, 0, kPolicyCoherent));
+      const float w = over_lanes(fabsf(z) < INFINITY ? exp_(x - z) : 0.f, [](float u, float v) { return u + v; });
+      store(w, lane == 0 && (uint32_t)((uniform_ints)row)[page_of(Lr)] < (uint32_t)a.P ? Lr : -1);
+    }
+    // Four rows a thread; kItems heads of such blocks of rows in flight at once.
+    constexpr int kItems = 8;
+    const int items = (Lr + 4 * kThreads - 1) / (4 * kThreads) * nh;
+    float w[4] = {0.f, 0.f, 0.f, 0.f};
+    int h = 0, j = 4 * tid;
+    for (int n = 0; n < items; n += kItems) {
+      u32x4 x[kItems], y[kItems];
+      int hx = h, jx = j;
+#pragma unroll
+      for (int u = 0; u < kItems; ++u) {
+        x[u] = __builtin_amdgcn_raw_buffer_load_b128(sr, jx < Lr ? (hx * (int)a.n_pad + jx) * 4 : (int)kOutOfRange, 0,
+                                                     kPolicyCoherent);
+        y[u] = load16(wr, jx < Lr && hx == nh - 1 ? jx * 4 : kOutOfRange);
+        if (++hx == nh) hx = 0, jx += 4 * kThreads;
+      }
+#pragma unroll
+      for (int u = 0; u < kItems; ++u) {
+        const float z = sh_lse[h];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] += fabsf(z) < INFINITY ? exp_(__uint_as_float(x[u][e]) - z) : 0.f;
+        if (++h == nh) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            store(__uint_as_float(y[u][e]) + w[e], j + e < Lr ? j + e : -1);
+            w[e] = 0.f;
+          }
+          h = 0, j += 4 * kThreads;
+        }
+      }
+    }
+  };
+
   m *= a.scale;
   // Join the waves.
   l = over_rows(l, [](float u, float w) { return u + w; });
@@ -676,14 +738,22 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
     } else {
       const float on = lt == 0.f ? 0.f : ot * __builtin_amdgcn_rcpf(lt);
       static_cast<T*>(a.o)[b * a.os.b + (h0 + h) * a.os.h + d] = (T)(valid ? on : nan);
-      if (d == 0 && (a.lse || a.lse_ws)) {
+      if (d == 0 && (a.lse || a.lse_ws || kFused)) {
         const float ls = lt == 0.f ? -INFINITY : Mu + log_(lt);
         if (a.lse) a.lse[(long long)b * a.H + h0 + h] = valid ? ls : nan;
         if (a.lse_ws) a.lse_ws[(long long)b * a.H + h0 + h] = ls;
+        if (kFused) sh_lse[h] = ls;
       }
     }
   }
-  if (!kDivide || S == 1) return;
+  if (!kDivide || S == 1) {
+    if (kFused && valid) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's scores
+      __syncthreads();
+      add_weights();
+    }
+    return;
+  }
   // The part is at the coherence point once its stores are acknowledged; then the arrival is counted.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
@@ -731,13 +801,15 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
     const float f = lane < S ? exp_(ms - Mu) : 0.f;
     const float W = over_lanes(f * ls, [](float u, float w) { return u + w; });
     if (lane < S) share[h * S + lane] = W == 0.f ? 0.f : f * __builtin_amdgcn_rcpf(W);
-    if (lane == 0 && (a.lse || a.lse_ws)) {
+    if (lane == 0 && (a.lse || a.lse_ws || kFused)) {
       const float z = W == 0.f ? -INFINITY : Mu + log_(W);
       if (a.lse) a.lse[(long long)b * a.H + h0 + h] = z;
       if (a.lse_ws) a.lse_ws[(long long)b * a.H + h0 + h] = z;
+      if (kFused) sh_lse[h] = z;
     }
   }
   __syncthreads();
+  if (kFused) add_weights();
   for (int e0 = 0; e0 < quads; e0 += kThreads) {
     const int e = join > 1 ? tid - grp * quads : e0 + tid;
     const int h = e / kQuads, d = e % kQuads * 4;
@@ -770,7 +842,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
   }
 }
 
-// key_weights: four keys a thread, the heads of the key-value head added in order.
+// key_weights after the step: four keys a thread, the heads of the key-value head added in order.
 __global__ __launch_bounds__(256) void add_weights_kernel(const float* __restrict__ scores,
                                                           const float* __restrict__ lse_ws,
                                                           const int* __restrict__ lens,
@@ -810,12 +882,21 @@ __global__ __launch_bounds__(256) void add_weights_kernel(const float* __restric
 // ---------------------------------------------------------------------------------------
 // Host side.
 
-// About kSlots workgroups a CU.
+// About kSlots workgroups a CU (a step of 4 sequences, 32 heads on 8, D = 128, 32768 rows: 80 us; with 1 102, with 4 83.5).
 constexpr int kSlots = 2;
-// Sequences of at most kWhole rows are not divided.
+// A sequence by itself of at most kWhole rows, and a batch's of twice as many, is not divided (12 heads of 400 rows 6.4 us,
+// divided 8.1; 1024 rows 8.5 divided, 9.7 not; 8 sequences of 1024, whose division takes the plan, 11.3 divided, 10.2 not).
 constexpr int kWhole = 512;
-// A part writes and reads back its heads' outputs: a granule's worth of K and V for every 16 heads' 4 granules.
+// The smallest part, in granules.  A unit of n granules in S parts takes a time of a n / S for its rows and b G S for writing and
+// joining S outputs of G heads, least at parts n / S = sqrt(b / a) sqrt(n G): longer with G (28 heads on 4, D = 128, 8192 rows 14.6
+// us, with parts of 1 granule 18.4; 16 on 1, D = 64, 8192 rows 12.7 and 17.0, with parts of 8 14.3).
 static int min_granules(int G) { return (int)lround(sqrt((double)std::min(kHeads, G))); }
+// key_weights of a key-value head of at most kFusedRows rows and kFusedScores scores are added by the workgroup that ends
+// it; more of them, and those of several units, by a kernel of their own, which takes the host another 2.5 us.
+// One kernel against two: 12 heads of 300 rows 9.1 and 9.2 us, 16 heads on 1 of 1000 rows, 4 sequences, 15.1 and 18.8, 32
+// on 8 heads of 4000 20.4 and 21.2; but 16 heads of 8000 rows 18.0 and 16.6, 4 sequences of 32 on 8 heads of 8000 35.0 and
+// 30.9.
+constexpr long long kFusedRows = 6144, kFusedScores = 16384;
 constexpr int kMaxCu = 1024;  // for the workspace's size, which does not depend on the device
 
 static long long padded(long long n) { return (n + kGranule - 1) / kGranule * kGranule + kScoreTail; }
@@ -837,7 +918,8 @@ static Layout layout(long long units, long long wgs, long long bh, long long n_m
 // unit.  No division (target 0) where there are units enough, or where sequences are short.
 static int choose_target(long long units, int B, long long n_max, int cu_count) {
   const long long per = units * B;
-  // (Past 2^21 granules the plan's quotients are not exact.)
+  // (64 sequences of 8 heads of 4096 rows, 512 units: 65.7 us divided, 67.7 not.  Past 2^21 granules the plan's quotients are
+  // not exact.)
   if (n_max <= (B == 1 ? kWhole : 2 * kWhole) || per >= (long long)kSlots * 2 * cu_count || (n_max / kGranule + 1) * B >= 1 << 20)
     return 0;
   const long long target = std::max(1LL, (long long)kSlots * cu_count / units);
@@ -860,13 +942,16 @@ static bool sizes_ok(int B, int H, int Hkv, int page, int M, int D) {
 template <class T, int kDV, bool kFull>
 static void launch_full(const First& f, const Args& a, unsigned wgs, hipStream_t stream) {
   const dim3 grid = f.target ? dim3(wgs) : dim3(f.units, f.B);
-#define TFGFA_PAGED_(kSpan, kDivide) \
-  hipLaunchKernelGGL((paged_kernel<T, kDV, kFull, kSpan, kDivide>), grid, dim3(kThreads), 0, stream, f.table, f.lens, \
-                     f.table_stride, static_cast<const T*>(f.q), f.n_max, f.div_m, f.div_s, f.target, f.units, f.B, a)
-#define TFGFA_PAGED(kSpan)                 \
-  do {                                     \
-    if (f.target) TFGFA_PAGED_(kSpan, true); \
-    else TFGFA_PAGED_(kSpan, false);       \
+#define TFGFA_PAGED_(kSpan, kDivide, kFused)                                                                     \
+  hipLaunchKernelGGL((paged_kernel<T, kDV, kFull, kSpan, kDivide, kFused>), grid, dim3(kThreads), 0, stream, f.table, \
+                     f.lens, f.table_stride, static_cast<const T*>(f.q), f.n_max, f.div_m, f.div_s, f.target, f.units, \
+                     f.B, a)
+#define TFGFA_PAGED(kSpan)                                           \
+  do {                                                               \
+    if (a.weights && f.target) TFGFA_PAGED_(kSpan, true, true);      \
+    else if (a.weights) TFGFA_PAGED_(kSpan, false, true);            \
+    else if (f.target) TFGFA_PAGED_(kSpan, true, false);             \
+    else TFGFA_PAGED_(kSpan, false, false);                          \
   } while (0)
   if (a.page % kTile == 0)
     TFGFA_PAGED(kTile);
@@ -976,7 +1061,10 @@ extern "C" int tfserve_decode_paged(
   a.kn = k_new, a.vn = v_new, a.o = o, a.lse = lse;
   a.arrive = ws;
   a.part = ws ? reinterpret_cast<float*>(ws + lay.part) : nullptr;
-  a.lse_ws = weights ? reinterpret_cast<float*>(ws + lay.lse_ws) : nullptr;
+  const bool fused = weights && a.tiles == 1 && n_max % 4 == 0 && n_max <= kFusedRows &&
+                     n_max * (H / H_kv) <= kFusedScores;
+  if (fused) a.weights = key_weights, a.wb = wb, a.wh = wh;
+  a.lse_ws = weights && !fused ? reinterpret_cast<float*>(ws + lay.lse_ws) : nullptr;
   a.scores = weights ? reinterpret_cast<float*>(ws + lay.scores) : nullptr;
   a.tag = f.target ? tfgfa::next_tag() : 0;
   a.n_pad = padded(n_max);
@@ -991,7 +1079,7 @@ extern "C" int tfserve_decode_paged(
   else
     launch<_Float16>(f, a, (unsigned)wgs, stream);
   hipError_t e = hipGetLastError();
-  if (e == hipSuccess && weights) {
+  if (e == hipSuccess && weights && !fused) {
     hipLaunchKernelGGL(add_weights_kernel, dim3((unsigned)((n_max + 1023) / 1024), H_kv, B), dim3(256), 0, stream,
                        a.scores, a.lse_ws, cache_seqlens, page_table, f.table_stride, key_weights, wb, wh, a.n_pad,
                        H, a.G, P, page, (int)n_max, append ? 1 : 0);
