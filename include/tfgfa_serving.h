@@ -26,7 +26,7 @@ extern "C" {
  * tfgfa_decode (last dimension dense, the others non-negative multiples of 8 elements, n >= D).  Row j
  * of sequence b is row j % page of page page_table[b * table_stride + j / page]; page_table is int32
  * (B, M), cache_seqlens B int32, both in device memory, so a sequence holds at most N_max = M * page
- * rows.  Entries of the table past a sequence's last row are not read.  H is a multiple of H_kv: query
+ * rows.  Entries of the table past a sequence's last row are not used.  H is a multiple of H_kv: query
  * head h reads key-value head h / (H / H_kv).
  *
  * One decode step, attention of one new query per (batch, head):

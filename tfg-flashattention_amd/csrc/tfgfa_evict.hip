@@ -3,15 +3,21 @@
 // Of the L rows of a (sequence, key-value head) the last `recent` stay, then those of the largest weight, ties to the
 // lowest row, n = min(L, budget) in all; they are copied in their order to rows 0 .. n - 1 of other pages.
 //
-// select_kernel: one workgroup a (sequence, key-value head).  Bound: latency, a few passes over the head's weights, which
-// stay in registers (up to 32768 rows; longer ones are read again in each pass).  Weights are ordered as 32-bit keys (the
-// float's bits, flipped so that unsigned order is float order; NaN lowest).  The last key that is kept is found by its digits of 11, 11 and 10 bits: a histogram in LDS of the keys that share the digits found so far, and the
-// digit at which the count from above reaches the number kept.  (The first digit is sign, exponent and two bits of the mantissa: weights
-// spread over tens of its values, so that few of a wave's 64 additions meet.)  Then the rows above that key, and the first of
-// those equal to it, are written behind one another: a wave's rows stand in row order, register by register, so places are
-// counts of bits in ballots.
-// copy_kernel: 16 bytes a thread and step, rows of K and V through both page tables.  Bound: HBM, 4D bytes
-// read and 4D written a kept row.  Where a head has few rows to copy, the selecting workgroup copies them itself.
+// select_kernel: one workgroup a (sequence, key-value head).  Bound: latency, a few passes over the head's weights,
+// which stay in registers (up to 32768 rows; longer ones are read again in each pass).  Weights are ordered as 32-bit
+// keys (the float's bits, flipped so that unsigned order is float order; NaN lowest).  The last key that is kept is
+// found by its digits of 11, 11 and 10 bits: a histogram in LDS of the keys that share the digits found so far, and
+// the digit at which the count from above reaches the number kept.  (The first digit is sign, exponent and two bits
+// of the mantissa: weights spread over tens of its values, so that few of a wave's 64 additions meet.)  Then the rows
+// above that key, and the first of those equal to it, are written behind one another: a wave's rows stand in row
+// order, register by register, so places are counts of bits in ballots.
+// copy_kernel: 16 bytes a thread and step, rows of K and V through both page tables.  Bound: HBM, 4D bytes read and
+// 4D written a kept row.  Where a head has few rows to copy, the selecting workgroup copies them itself.
+//
+// Measured: 32 heads of up to 32768 rows, D = 128, cut to 4096: selection 27 us (32 of 256 CUs have work; loads 3,
+// first histogram 5, candidates 4, places and stores 8), copies 22.5 us, 6 TB/s of reads and writes; 16 sequences of
+// 25 heads of up to 1024 rows cut to 512: 8 and 15.3 us; one sequence of 12 heads, 300 rows cut to 130, 7.7 us in one
+// launch.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -34,9 +40,13 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kMaxD = 128;
 constexpr int kBins = 2048;
 constexpr int kMaxFused = kBins;  // rows that a selecting workgroup may copy itself (their list is in LDS)
-constexpr int kCandidates = 4096;  // rows with the first digit of the last one kept that a list holds
+// Rows with the first digit of the last one kept that a list holds, for the other digits (63.8 us at 32768 rows, 68.6
+// with the registers gone through again).
+constexpr int kCandidates = 4096;
 constexpr int kMaxRows = 32768;   // rows of a sequence whose weights stay in registers
-constexpr int kFusedValues = 16384;  // rows * D of a head up to which the selecting workgroup copies them
+// rows * D of a head up to which the selecting workgroup copies them (12 heads, 130 rows: 7.7 us, with two kernels
+// 9.8; 400 heads of 512 rows: 28.4 and 26.4).
+constexpr int kFusedValues = 16384;
 constexpr int kCopy = 4;          // rows of a thread of the copying kernel
 
 struct Args {
@@ -112,8 +122,8 @@ __device__ __forceinline__ void copy_rows(const Args& a, int b, int kv, int i0, 
   }
 }
 
-// kW waves; kR weights a lane in registers (row of register r: (wave * kR + r) * 64 + lane), 0: read in each pass, wave by
-// wave in the same order.
+// kW waves; kR weights a lane in registers (row of register r: (wave * kR + r) * 64 + lane), 0: read in each pass,
+// wave by wave in the same order.
 template <int kW, int kR>
 __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
   constexpr int kThreads = 64 * kW, kEach = kBins / kThreads;
@@ -176,7 +186,8 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
     for (int e = 0; e < kEach; ++e) hist[e * kThreads + tid] = 0;
     __syncthreads();
   };
-  // One more of a digit, in the lanes that are in; a wave whose keys all have one digit (equal weights) adds them at once.
+  // One more of a digit, in the lanes that are in; a wave whose keys all have one digit (equal weights) adds them at
+  // once.
   auto count = [&](bool in, int digit) {
     const unsigned long long who = __builtin_amdgcn_ballot_w64(in);
     if (who == 0) return;
@@ -414,6 +425,9 @@ extern "C" int tfserve_evict(void* k_pages, const int64_t* k_strides, void* v_pa
   const int rows = std::min<long long>(budget, n_max);
   a.fused = n_max <= kMaxRows && rows <= kMaxFused && (long long)rows * D <= kFusedValues;
   const hipStream_t stream = (hipStream_t)hip_stream;
+  // The fewest registers that hold a head's weights, in waves that still leave other heads room (400 heads of 1024
+  // rows: 26.4 us with 8 waves of 2 a lane, 28.1 with 4 of 4, 30.2 with 16 of 1; 32 heads of 32768: 63.3 with 16 of
+  // 32, 80.5 with 8 of 64).
   if (n_max <= 1024)
     launch<8, 2>(a, B, stream);
   else if (n_max <= 4096)

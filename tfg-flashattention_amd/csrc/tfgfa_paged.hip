@@ -1,29 +1,38 @@
-// tfgfa_paged.hip - one decode step of attention over a paged key-value cache, MI355X (gfx950), bf16
-// or fp16, head dims that are multiples of 8 up to 128, query heads sharing key-value heads.
+// tfgfa_paged.hip - one decode step of attention over a paged key-value cache, MI355X (gfx950), bf16 or fp16, head
+// dims that are multiples of 8 up to 128, query heads sharing key-value heads.
 //
 // For each query head h of key-value head h' (G = H / H_kv of them):
 //     x_j = scale q_h . k_j,   o_h = sum_j e^(x_j) v_j / sum_j e^(x_j),   lse_h = log sum_j e^(x_j)
 // over the rows j < L of the sequence, row j being row j % page of page table[j / page].
 //
-// Bound: HBM.  Each K and V row is read once, 4D bytes for 4DG flops.  The 16 columns of a 16x16 matrix
-// tile are the query heads of one key-value head, so that up to 16 of them cost what one does:
+// Bound: HBM.  Each K and V row is read once, 4D bytes for 4DG flops.  The 16 columns of a 16x16 matrix tile are the
+// query heads of one key-value head, so that up to 16 of them cost what one does:
 //   scores   S^T[key][head] = K Q^T      v_mfma_f32_16x16x32 (products exact, float32 sums)
 //   output   O^T[dim][head] += V^T P^T   the same, P as two values of the element type
 // A wave takes 32 keys at a time.  The scores leave the first product with lane (g = lane / 16, i = lane % 16)
-// holding keys 4g .. 4g + 3 of each 16 for head i; two such sets are the second product's B operand as they stand (the
-// contraction runs over keys, whose order is free).  Its A operand wants 8 keys' values of one dim in a lane:
+// holding keys 4g .. 4g + 3 of each 16 for head i; two such sets are the second product's B operand as they stand
+// (the contraction runs over keys, whose order is free).  Its A operand wants 8 keys' values of one dim in a lane:
 // the lane loads kDV neighbouring dims of each of the 8 rows, and byte permutes put the keys of a dim side by side.
 // So neither P nor V moves between lanes.  P is split as hi + lo, each rounded to the element type, which keeps 16
-// (bf16) or 22 (fp16) of its bits; rounding it once would cost as much as the output's own rounding.  (fp16 ends at 2^-24:
-// its P is carried times 2^13, so that weights are kept to 2^-38 of the largest.)  An infinite V
-// makes NaN of a lo of 0 or below; a wave whose sums hold NaN takes its keys again with hi alone, for those sums.  (With P and V
+// (bf16) or 22 (fp16) of its bits; rounding it once would cost as much as the output's own rounding.  (fp16 ends at
+// 2^-24: its P is carried times 2^13, so that weights are kept to 2^-38 of the largest.)  An infinite V makes NaN of
+// a lo of 0 or below; a wave whose sums hold NaN takes its keys again with hi alone, for those sums.  (With P and V
 // as float32 on v_mfma_f32_16x16x4_f32 a block of 32 keys took 1024 matrix cycles at D = 64 instead of 192.)
 //
-// Division of the work.  A unit is a (sequence, key-value head, 16 query heads).  The lengths are known on
-// the device only, so every workgroup works the division out from them (plan, below): one chunk length C for
-// all units, with about `target` workgroups in all; a unit of more than C rows is divided over
-// several workgroups.  Each leaves its part (normalised output and log-sum-exp) in the workspace, and the
-// one that arrives last joins them (arrival words and memory order as in tfgfa_decode.hip).
+// Division of the work.  A unit is a (sequence, key-value head, 16 query heads).  The lengths are known on the device
+// only, so every workgroup works the division out from them (plan, below): one chunk length C for all units, with
+// about `target` workgroups in all; a unit of more than C rows is divided over several workgroups.  Each leaves its
+// part (sums of weighted values and of weights, and their offset) in the workspace, and the one that arrives last
+// joins them (arrival words and memory order as in tfgfa_decode.hip) and, where it is asked for, adds the unit's key
+// weights from the scores that the parts have left.
+//
+// Measured: 32 sequences of 25 heads, D = 64, lengths to 1024, 120 MB in 24.9 us (a plain read of as many bytes
+// 21.6); 4 sequences of 32 heads on 8, D = 128, to 32768 rows, 385 MB in 78 us (67); one sequence of 12 heads, 400
+// rows, 6.4 us (the chain length - pages - K - V - output; 1.6 us are the launch); 4 sequences of 16 heads to 4096
+// rows with key weights, 50 MB, 21 us, 4 of them the weights (10).  Matrix units busy 5%, VALU issue
+// 19%, 80% of the wave cycles in waits at the first: loads under way bound it, and their number is what the registers
+// hold (a second set of them 192 to 256 VGPRs, slower; 4 waves a SIMD spill; blocks of 64 keys, 8 or 16 waves a
+// workgroup, slower).
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -70,8 +79,8 @@ constexpr int kPolicyCoherent = 16;           // buffer loads from the device's 
 
 template <class T>
 struct Elem;
-// kShift: P is carried times 2^kShift.  kSlack: how far a score may pass its head's offset; e^kSlack 2^kShift is a number
-// of the type.
+// kShift: P is carried times 2^kShift.  kSlack: how far a score may pass its head's offset; e^kSlack 2^kShift is a
+// number of the type.
 template <>
 struct Elem<__bf16> {
   static constexpr int kShift = 0;
@@ -280,9 +289,10 @@ __device__ __forceinline__ float over_lanes(float x, F f) {
 typedef const __attribute__((address_space(4))) int* uniform_ints;
 
 // kDV: dims of a lane in V, 4 (D <= 64) or 8.  kFull: D == 16 kDV.  kSpan: keys that are sure to be in one page: a
-// block (32), a tile (16) or 1, by the page size's multiples.  kDivide: sequences may be divided (grid: flat; otherwise units by sequences).
-// The first 14 dwords of the arguments are preloaded into scalar registers (-amdgpu-kernarg-preload-count): what the
-// first loads, of the length and of the first block's pages, wait for.
+// tile (16) where the page size is a multiple of it, otherwise 1, whose lanes have an address each (5 to 20% slower
+// on pages that allow both).  kFused: this kernel adds key weights.  kDivide: sequences may be divided (grid: flat;
+// otherwise units by sequences). The first 14 dwords of the arguments are preloaded into scalar registers
+// (-amdgpu-kernarg-preload-count): what the first loads, of the length and of the first block's pages, wait for.
 template <class T, int kDV, bool kFull, int kSpan, bool kDivide, bool kFused>
 __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restrict__ table, const int* __restrict__ lens,
                                                             long long table_stride, const T* __restrict__ q, int n_max,
@@ -381,7 +391,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
   const char* const kn = append ? reinterpret_cast<const char*>(static_cast<const T*>(a.kn) + b * a.kns.b + kv * a.kns.h) : kh;
   const char* const vn = append ? reinterpret_cast<const char*>(static_cast<const T*>(a.vn) + b * a.vns.b + kv * a.vns.h) : vh;
   // Loads of a block.  Rows that are not there come as zeros (kSpan > 1: past the buffer, which for the new row ends
-  // before a second one; otherwise the loads go to a row that is there, and V is cleared below); so do dims past D in K.
+  // before a second one; otherwise the loads go to a row that is there, and V is cleared below); so do dims past D
+  // in K.
   u32x4 k[kTiles][kDP];           // row i of a tile, dims 32p + 8g .. of piece p: the A operand of the scores
   uint32_t v[kTiles][4][kDP];     // row 4g + r of a tile, dims kDV i ..
   const uint32_t k_lane = (uint32_t)(i * (int)a.ks.n + 16 * g);
@@ -455,8 +466,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
 
   float m, l;
   f32x4 acc[kDV];
-  // Hi and lo of P: 1 or 0, kept in a scalar register.  (A branch on what the compiler takes for a value of each lane only
-  // masks lanes, and a matrix instruction runs whatever the mask.)
+  // Hi and lo of P: 1 or 0, kept in a scalar register.  (A branch on what the compiler takes for a value of each lane
+  // only masks lanes, and a matrix instruction runs whatever the mask.)
   int both = __builtin_amdgcn_readfirstlane(1);
   // The wave's sums into LDS.  acc[j], register r of lane (g, i): dim kDV (4g + r) + j of head i.
   auto leave = [&]() {
@@ -470,8 +481,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
     }
   };
 
-  // The arithmetic of block x.  kMore: another block follows, whose K goes out once the scores have read this one's, and
-  // its V once the output has, so that one of the two is always in flight with one set of registers.
+  // The arithmetic of block x.  kMore: another block follows, whose K goes out once the scores have read this one's,
+  // and its V once the output has, so that one of the two is always in flight with one set of registers.
   auto step = [&](const Block& x, const Block& y, auto more) {
       constexpr bool kMore = decltype(more)::value;
       int next[kIds];
@@ -547,7 +558,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
           }
         }
       }
-      // The offset of each head moves only when a score passes it by the slack, so that lanes compare notes in few blocks.
+      // The offset of each head moves only when a score passes it by the slack, so that lanes compare notes in few
+      // blocks.
       float mb = s[0][0];
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)
@@ -882,20 +894,23 @@ __global__ __launch_bounds__(256) void add_weights_kernel(const float* __restric
 // ---------------------------------------------------------------------------------------
 // Host side.
 
-// About kSlots workgroups a CU (a step of 4 sequences, 32 heads on 8, D = 128, 32768 rows: 80 us; with 1 102, with 4 83.5).
+// About kSlots workgroups a CU (a step of 4 sequences, 32 heads on 8, D = 128, 32768 rows: 80 us; with 1 102, with 4
+// 83.5).
 constexpr int kSlots = 2;
-// A sequence by itself of at most kWhole rows, and a batch's of twice as many, is not divided (12 heads of 400 rows 6.4 us,
-// divided 8.1; 1024 rows 8.5 divided, 9.7 not; 8 sequences of 1024, whose division takes the plan, 11.3 divided, 10.2 not).
+// A sequence by itself of at most kWhole rows, and a batch's of twice as many, is not divided (12 heads of 400 rows
+// 6.4 us, divided 8.1; 1024 rows 8.5 divided, 9.7 not; 8 sequences of 1024, whose division takes the plan, 11.3
+// divided, 10.2 not).
 constexpr int kWhole = 512;
-// The smallest part, in granules.  A unit of n granules in S parts takes a time of a n / S for its rows and b G S for writing and
-// joining S outputs of G heads, least at parts n / S = sqrt(b / a) sqrt(n G): longer with G (28 heads on 4, D = 128, 8192 rows 14.6
-// us, with parts of 1 granule 18.4; 16 on 1, D = 64, 8192 rows 12.7 and 17.0, with parts of 8 14.3).
+// The smallest part, in granules.  A unit of n granules in S parts takes a time of a n / S for its rows and b G S for
+// writing and joining S outputs of G heads, least at parts n / S = sqrt(b / a) sqrt(n G): longer with G (28 heads on
+// 4, D = 128, 8192 rows 14.6 us, with parts of 1 granule 18.4; 16 on 1, D = 64, 8192 rows 12.7 and 17.0, with parts
+// of 8 14.3).
 static int min_granules(int G) { return (int)lround(sqrt((double)std::min(kHeads, G))); }
-// key_weights of a key-value head of at most kFusedRows rows and kFusedScores scores are added by the workgroup that ends
-// it; more of them, and those of several units, by a kernel of their own, which takes the host another 2.5 us.
-// One kernel against two: 12 heads of 300 rows 9.1 and 9.2 us, 16 heads on 1 of 1000 rows, 4 sequences, 15.1 and 18.8, 32
-// on 8 heads of 4000 20.4 and 21.2; but 16 heads of 8000 rows 18.0 and 16.6, 4 sequences of 32 on 8 heads of 8000 35.0 and
-// 30.9.
+// key_weights of a key-value head of at most kFusedRows rows and kFusedScores scores are added by the workgroup that
+// ends it; more of them, and those of several units, by a kernel of their own, which takes the host another 2.5 us.
+// One kernel against two: 12 heads of 300 rows 9.1 and 9.2 us, 16 heads on 1 of 1000 rows, 4 sequences, 15.1 and
+// 18.8, 32 on 8 heads of 4000 20.4 and 21.2; but 16 heads of 8000 rows 18.0 and 16.6, 4 sequences of 32 on 8 heads of
+// 8000 35.0 and 30.9.
 constexpr long long kFusedRows = 6144, kFusedScores = 16384;
 constexpr int kMaxCu = 1024;  // for the workspace's size, which does not depend on the device
 
@@ -918,9 +933,10 @@ static Layout layout(long long units, long long wgs, long long bh, long long n_m
 // unit.  No division (target 0) where there are units enough, or where sequences are short.
 static int choose_target(long long units, int B, long long n_max, int cu_count) {
   const long long per = units * B;
-  // (64 sequences of 8 heads of 4096 rows, 512 units: 65.7 us divided, 67.7 not.  Past 2^21 granules the plan's quotients are
-  // not exact.)
-  if (n_max <= (B == 1 ? kWhole : 2 * kWhole) || per >= (long long)kSlots * 2 * cu_count || (n_max / kGranule + 1) * B >= 1 << 20)
+  // (64 sequences of 8 heads of 4096 rows, 512 units: 65.7 us divided, 67.7 not.  Past 2^21 granules the plan's
+  // quotients are not exact.)
+  if (n_max <= (B == 1 ? kWhole : 2 * kWhole) || per >= (long long)kSlots * 2 * cu_count ||
+      (n_max / kGranule + 1) * B >= 1 << 20)
     return 0;
   const long long target = std::max(1LL, (long long)kSlots * cu_count / units);
   if (B > 1) return (int)target;
@@ -1068,7 +1084,9 @@ extern "C" int tfserve_decode_paged(
   a.scores = weights ? reinterpret_cast<float*>(ws + lay.scores) : nullptr;
   a.tag = f.target ? tfgfa::next_tag() : 0;
   a.n_pad = padded(n_max);
-  a.scale = softmax_scale, a.scale_log2 = softmax_scale * kLog2e, a.slack = std::min((dtype == TFGFA_DTYPE_BF16 ? Elem<__bf16>::kSlack : Elem<_Float16>::kSlack) / softmax_scale, 1e30f);
+  a.scale = softmax_scale, a.scale_log2 = softmax_scale * kLog2e;
+  const float slack = dtype == TFGFA_DTYPE_BF16 ? Elem<__bf16>::kSlack : Elem<_Float16>::kSlack;
+  a.slack = std::min(slack / softmax_scale, 1e30f);
   a.H = H, a.G = H / H_kv, a.P = P, a.page = page, a.D = D;
   a.min_granules = min_granules(a.G);
   const tfgfa::Division by_page = tfgfa::division_by(page);

@@ -2,17 +2,26 @@
 //     c_j = sum_h sum_i [j <= first + i] e^(scale q_hi . k_j - lse_hi)
 // over the query heads h of a key-value head, with the log-sum-exp of the attention that ran before.
 //
-// Bound: the exponentials.  A pair of query and key costs 2D flops on the matrix units (128 cycles a 32x32 tile at D =
-// 64) and a v_fma, a v_exp_f32 and a v_add on the VALU (16 x 15 cycles a tile).
+// Bound: VALU issue.  A pair of query and key costs 2D flops on the matrix units (128 cycles a 32x32 tile at D = 64)
+// and a v_fma, a v_exp_f32 and a v_add on the VALU (16 x 15 cycles a tile).
+// Measured: 16 heads of 8192 causal queries and keys, D = 64, 99-102 us, 670-690 TFLOP/s; VALU issue 65% of the
+// cycles, matrix units 26%, 37% of the wave cycles waiting to issue (without the exponentials 90 us, without the
+// matrix products 73.5, without LDS reads 83).  D = 128, 4 x 16 heads of 4096: 157 us, 876 TFLOP/s.  64 queries
+// against 16001 keys, 2 x 32 heads on 8, D = 128, 27-30 us, 12 of them a plain read of K: a workgroup's first loads
+// are not covered.
 //
-// S^T[key][query] = K Q^T as v_mfma_f32_32x32x16 tiles: lane l holds 16 keys of query l % 32, so that the
-// query's lse is one register, the sums over queries stay in 16 registers of each lane, and lanes are
-// added once at the end.  A wave owns 32 keys of one key-value head, whose K rows stay in registers; the four waves of a
-// workgroup share tiles of 64 queries, which come through two LDS buffers by direct loads, the next tile's under this
-// one's arithmetic (an operand read straight from memory touches 32 rows an instruction, 32 bytes of each).
-// Under a causal mask the first keys are seen by most queries.  Their workgroups come first; where several share a CU,
-// every other round of workgroups over the CUs runs backwards, so that a CU's long and short ones add up alike (16 heads
-// of 8192 queries and keys: 1024 workgroups, all resident, of which one CU had 160 parts and another 100).
+// S^T[key][query] = K Q^T as v_mfma_f32_32x32x16 tiles: lane l holds 16 keys of query l % 32, so that the query's lse
+// is one register, the sums over queries stay in 16 registers of each lane, and lanes are added once at the end.  A
+// wave owns 32 keys of one key-value head, whose K rows stay in registers; the four waves of a workgroup share tiles
+// of 64 queries, which come through two LDS buffers by direct loads, the next tile's under this one's arithmetic (an
+// operand read straight from memory touches 32 rows an instruction, 32 bytes of each). Under a causal mask the first
+// keys are seen by most queries.  Their workgroups come first; where several share a CU, every other round of
+// workgroups over the CUs runs backwards, so that a CU's long and short ones add up alike (16 heads of 8192 queries
+// and keys: 1024 workgroups, all resident, of which one CU had 160 parts and another 100; 100 us, in plain order
+// 106).
+// Tried and slower: 8 waves a workgroup (114 us), two key tiles a wave (139), the causal ends paired in one wave
+// (163); for few queries, all of them in LDS and waves that go through the keys (27 -> 19 us for 32 queries, but 8.3
+// -> 10.5 and 13.4 -> 15 at other sizes).
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -76,9 +85,9 @@ __device__ __forceinline__ int turn(int row) {
   return kChunks == 8 ? tfgfa::swz_k(row) : row & 15;
 }
 
-// The sums over the 32 queries (lanes) of each half of the registers of s, 16 of them: halves of the registers change sides
-// with the lanes that differ in one bit of their number (of the last ones three: any pairing does that flips the bit), so
-// that each step adds half as many.  Lane l ends with register l / 2 % 16.
+// The sums over the 32 queries (lanes) of each half of the registers of s, 16 of them: halves of the registers change
+// sides with the lanes that differ in one bit of their number (of the last ones three: any pairing does that flips
+// the bit), so that each step adds half as many.  Lane l ends with register l / 2 % 16.
 __device__ __forceinline__ float over_queries(const float (&sum)[16], int lane) {
   float s[8];
 #pragma unroll
@@ -207,8 +216,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(const Args a) {
         const int q0 = t * kQueries + u * kTile;
         if (q0 >= a.Nq || (a.causal && a.first + q0 + kTile - 1 < j0)) continue;
         const f32x16 s = scores(u);
-        // Keys that the lane's query sees: up to `last`.  A row past the last, and one with nothing to see (lse -inf, or
-        // past the range in the log2 domain), sees none.
+        // Keys that the lane's query sees: up to `last`.  A row past the last, and one with nothing to see (lse -inf,
+        // or past the range in the log2 domain), sees none.
         const bool live = fabsf(z[u]) != INFINITY && q0 + i < a.Nq;
         int last = kTile - 1;
         if (a.causal) last = (int)max(-1LL, min((long long)last, a.first + q0 + i - j0));

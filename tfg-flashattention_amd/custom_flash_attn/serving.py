@@ -139,7 +139,7 @@ def decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     key-value head ``h // (H // H_kv)``; any page size.  bf16 or fp16, all alike; D a multiple of 8 up to
     128.  ``page_table``: int32 (B, M); row j of sequence b is row ``j % page`` of page
     ``page_table[b, j // page]``.  ``cache_seqlens``: int32 (B,), the cached rows; entries of the table
-    past them are not read.  With ``k_new``/``v_new`` ((B, H_kv, D)) the new token becomes row
+    past them are not used.  With ``k_new``/``v_new`` ((B, H_kv, D)) the new token becomes row
     ``cache_seqlens[b]`` first (its page must be the sequence's own) and is attended too; the caller
     advances ``cache_seqlens`` afterwards.  Pages may otherwise be shared by sequences.
 
