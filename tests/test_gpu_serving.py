@@ -305,6 +305,29 @@ def test_decode_paged_many_small_weights(dtype):
     _near(o[0], ro, eo + small + _half(dtype) * (ro.abs() + eo + small) + 2.0 ** -25, "o")
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_decode_paged_large_scores(dtype):
+    """Scores near 2^23, where float32 holds integers only: a later row passes the first ones by 7, 2.1 with the scale.  The scores
+    are exact, and so are their differences, which the weights come from: (L + 32) u for their sums, 2^-16 for the
+    weights' own bits."""
+    g = _gen(33)
+    D, L, page = 64, 300, 16
+    c = Paged(g, [L], 1, D, page, dtype)
+    (k, v), = c.rows
+    k.zero_()
+    k[0, :, 0] = 256
+    k[0, 128, 1] = 7
+    for j in range(0, L, page):
+        c.k[int(c.table[0, j // page]), :, :min(page, L - j)] = k[:, j:j + page]
+    q = torch.zeros(1, 1, D, dtype=dtype, device=DEV)
+    q[..., 0], q[..., 1] = 32768, 1
+    o = fa.decode_paged(q, c.k, c.v, c.table, c.seqlens, softmax_scale=0.3)
+    p = torch.softmax(k[0, :, 1].double().cpu() * 0.3, 0)
+    vv = v[0].double().cpu()
+    ro, eo = (p @ vv)[None], (((L + 32) * U + 2.0 ** -16) * (p @ vv.abs()))[None]
+    _near(o[0], ro, eo + _half(dtype) * (ro.abs() + eo), "o")
+
+
 def test_decode_paged_divides_more_than_64_sequences():
     """The division of the work takes lengths 64 at a time."""
     g = _gen(32)

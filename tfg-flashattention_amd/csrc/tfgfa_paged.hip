@@ -559,13 +559,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
         }
       }
       // The offset of each head moves only when a score passes it by the slack, so that lanes compare notes in few
-      // blocks.
+      // blocks.  (By the difference, which is exact for near scores: m + slack may round up by more than fp16 has room.)
       float mb = s[0][0];
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) mb = fmaxf(mb, s[t][r]);
-      if (__builtin_amdgcn_ballot_w64(mb > m + a.slack)) {
+      if (__builtin_amdgcn_ballot_w64(mb - m > a.slack)) {
         mb = over_rows(mb, [](float u, float w) { return fmaxf(u, w); });
         const float mn = fmaxf(m, mb);
         const float f = m == -INFINITY ? 0.f : exp_((m - mn) * a.scale);
@@ -706,8 +706,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
     }
   };
 
-  m *= a.scale;
-  // Join the waves.
+  // Join the waves.  (Offsets without the scale: differences first, here too.)
   l = over_rows(l, [](float u, float w) { return u + w; });
   if (!both && i < nh) {
 #pragma unroll
@@ -737,7 +736,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
     float lt = 0.f, ot = 0.f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const float f = exp_(sh_m[w][h] - Mu);
+      const float f = exp_((sh_m[w][h] - Mu) * a.scale);
       lt = fmaf(f, sh_l[w][h], lt);
       ot = fmaf(f, sh_o[(w * kHeads + h) * kRow + d], ot);
     }
@@ -751,7 +750,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
       const float on = lt == 0.f ? 0.f : ot * __builtin_amdgcn_rcpf(lt);
       static_cast<T*>(a.o)[b * a.os.b + (h0 + h) * a.os.h + d] = (T)(valid ? on : nan);
       if (d == 0 && (a.lse || a.lse_ws || kFused)) {
-        const float ls = lt == 0.f ? -INFINITY : Mu + log_(lt);
+        const float ls = lt == 0.f ? -INFINITY : fmaf(Mu, a.scale, log_(lt));
         if (a.lse) a.lse[(long long)b * a.H + h0 + h] = valid ? ls : nan;
         if (a.lse_ws) a.lse_ws[(long long)b * a.H + h0 + h] = ls;
         if (kFused) sh_lse[h] = ls;
@@ -810,11 +809,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
     const float ms = coherent(at), ls = coherent(at + kHeads * 4);
     const float M = over_lanes(lane < S ? ms : -INFINITY, [](float u, float w) { return fmaxf(u, w); });
     const float Mu = M == -INFINITY ? 0.f : M;
-    const float f = lane < S ? exp_(ms - Mu) : 0.f;
+    const float f = lane < S ? exp_((ms - Mu) * a.scale) : 0.f;
     const float W = over_lanes(f * ls, [](float u, float w) { return u + w; });
     if (lane < S) share[h * S + lane] = W == 0.f ? 0.f : f * __builtin_amdgcn_rcpf(W);
     if (lane == 0 && (a.lse || a.lse_ws || kFused)) {
-      const float z = W == 0.f ? -INFINITY : Mu + log_(W);
+      const float z = W == 0.f ? -INFINITY : fmaf(Mu, a.scale, log_(W));
       if (a.lse) a.lse[(long long)b * a.H + h0 + h] = z;
       if (a.lse_ws) a.lse_ws[(long long)b * a.H + h0 + h] = z;
       if (kFused) sh_lse[h] = z;
