@@ -43,6 +43,7 @@ constexpr int kMaxFused = kBins;  // rows that a selecting workgroup may copy it
 // Rows with the first digit of the last one kept that a list holds, for the other digits (63.8 us at 32768 rows, 68.6
 // with the registers gone through again).
 constexpr int kCandidates = 4096;
+constexpr int kFewRows = 4096;    // rows of a sequence that four weights a lane hold
 constexpr int kMaxRows = 32768;   // rows of a sequence whose weights stay in registers
 // rows * D of a head up to which the selecting workgroup copies them (12 heads, 130 rows: 7.7 us, with two kernels
 // 9.8; 400 heads of 512 rows: 28.4 and 26.4).
@@ -84,9 +85,9 @@ __device__ __forceinline__ int scan64(int x) {
   x = add_dpp<0x142, 0xA>(x);     // lane 15 of rows 0 and 2 to the row after
   return add_dpp<0x143, 0xC>(x);  // lane 31 to rows 2 and 3
 }
-// Bits of m below this lane's.
-__device__ __forceinline__ int below(unsigned long long m) {
-  return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+// Bits of m below this lane's, and n.
+__device__ __forceinline__ int below(unsigned long long m, int n) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, n));
 }
 
 __device__ __forceinline__ int page_of(const Args& a, int j) {
@@ -127,6 +128,7 @@ __device__ __forceinline__ void copy_rows(const Args& a, int b, int kv, int i0, 
 template <int kW, int kR>
 __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
   constexpr int kThreads = 64 * kW, kEach = kBins / kThreads;
+  constexpr bool kFuses = kR > 0 && kR <= 4;  // may copy the rows too
   constexpr bool kList = kR > 4;  // candidates of the second digit are put into a list where it holds them
   __shared__ int hist[kBins];
   __shared__ uint32_t list[kList ? kCandidates : 1];
@@ -269,10 +271,8 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
         find(shift);
       }
     }
-  } else if (chosen == 0) {
-    key = 0xFFFFFFFFu;  // (no key is above it, and no tie is wanted)
-  } else {
-    want = old;  // all of them: those above 0, and of 0 (NaN) as many as there are
+  } else {  // (none is chosen: chosen < old wherever the budget does not hold every row)
+    key = 0xFFFFFFFEu;  // no weight's key is it or above it
   }
   __syncthreads();
   if (sh_bad) {
@@ -282,18 +282,22 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
     }
     return;
   }
-  auto keep = [&](uint32_t at, int j, float y) {
-    kept[at] = j;
-    out[at] = y;
-    if (kR > 0 && a.fused) hist[at & (kBins - 1)] = j;
-  };
   if constexpr (kR > 0) {
-    // Rows above the key, and ties, of the waves before.  (Every weight is in a register by now: `out` may be `w`.)
+    // Protected rows count as above every key, so that a kept row's place is the number of rows above the key before it,
+    // and of the wanted ties.  Rows past the last have the lowest key: as ties they come after all that are wanted.
+    auto key_of = [&](int r) {
+      const int j = first + r * 64 + lane;
+      return j < old ? q[r] : j < L ? 0xFFFFFFFFu : 0u;
+    };
+    // Those of the waves before.  (Every weight is in a register by now: `out` may be `w`.)
     int taken = 0, ties = 0;
-    rows([&](int j, uint32_t y, bool in) {
-      taken += in && y > key ? 1 : 0;
-      ties += in && y == key ? 1 : 0;
-    });
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+      if (first + r * 64 >= L) break;
+      q[r] = key_of(r);
+      taken += q[r] > key ? 1 : 0;
+      ties += q[r] == key ? 1 : 0;
+    }
     taken = scan64(taken), ties = scan64(ties);
     if (lane == 63) {
       sh_sum[wave] = taken;
@@ -306,25 +310,26 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
       taken += c < wave ? sh_sum[c] : 0;
       ties += c < wave ? sh_tie[c] : 0;
     }
+    taken = __builtin_amdgcn_readfirstlane(taken), ties = __builtin_amdgcn_readfirstlane(ties);
+    const __amdgpu_buffer_rsrc_t to_kept = __builtin_amdgcn_make_buffer_rsrc(kept, (short)0, INT32_MAX, 0x00020000);
+    const __amdgpu_buffer_rsrc_t to_out = __builtin_amdgcn_make_buffer_rsrc(out, (short)0, INT32_MAX, 0x00020000);
 #pragma unroll
     for (int r = 0; r < kR; ++r) {
       if (first + r * 64 >= L) break;
-      const int j = first + r * 64 + lane;
-      const bool in = j < old;
-      const unsigned long long mo = __builtin_amdgcn_ballot_w64(in && q[r] > key);
-      const unsigned long long mt = __builtin_amdgcn_ballot_w64(in && q[r] == key);
-      if (mt == 0) {
-        if (in && q[r] > key) keep(taken + min(ties, want) + below(mo), j, x[r]);
-        taken += __builtin_popcountll(mo);
-      } else {
-        const int t = ties + below(mt);
-        if (in && (q[r] > key || (q[r] == key && t < want))) keep(taken + below(mo) + min(t, want), j, x[r]);
-        taken += __builtin_popcountll(mo);
-        ties += __builtin_popcountll(mt);
+      const unsigned long long mo = __builtin_amdgcn_ballot_w64(q[r] > key);
+      const unsigned long long mt = __builtin_amdgcn_ballot_w64(q[r] == key);
+      const int t = below(mt, ties), at = below(mo, taken) + min(t, want);
+      if (q[r] > key || (q[r] == key && t < want)) {
+        const int j = first + r * 64 + lane;
+        __builtin_amdgcn_raw_buffer_store_b32((uint32_t)j, to_kept, at * 4, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[r]), to_out, at * 4, 0, 0);
+        if (kFuses && a.fused) hist[at & (kBins - 1)] = j;
       }
-      if (!in && j < L) keep(chosen + j - old, j, x[r]);
+      taken += __builtin_popcountll(mo);
+      ties += __builtin_popcountll(mt);
     }
   } else {
+    auto keep = [&](int at, int j, float y) { kept[at] = j, out[at] = y; };
     // `out` may be `w`: rows move down only, and a step's rows, of all waves, are read before any is written.
     int done = 0, seen = 0;
     for (int j0 = 0; j0 < L; j0 += kThreads) {
@@ -348,8 +353,8 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
         done += sh_sum[c];
         seen += sh_tie[c];
       }
-      const int t = s + below(mt);
-      if (in && (z > key || (z == key && t < want))) keep(o + below(mo) + min(t, want), j, y);
+      const int t = below(mt, s);
+      if (in && (z > key || (z == key && t < want))) keep(below(mo, o) + min(t, want), j, y);
       if (!in && j < L) keep(chosen + j - old, j, y);
     }
     __syncthreads();
@@ -358,7 +363,7 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
     kept[i] = -1;
     out[i] = 0.f;
   }
-  if (!a.fused) return;
+  if (!kFuses || !a.fused) return;
   __syncthreads();
   const int per = kThreads / a.pieces, row = tid / a.pieces;
   if (row < per) copy_rows<4>(a, b, kv, row, per, tid - row * a.pieces, n, [&](int i) { return hist[i]; });
@@ -423,14 +428,14 @@ extern "C" int tfserve_evict(void* k_pages, const int64_t* k_strides, void* v_pa
   a.by_page = tfgfa::division_by(page);
   a.pieces = D / 8;
   const int rows = std::min<long long>(budget, n_max);
-  a.fused = n_max <= kMaxRows && rows <= kMaxFused && (long long)rows * D <= kFusedValues;
+  a.fused = n_max <= kFewRows && rows <= kMaxFused && (long long)rows * D <= kFusedValues;
   const hipStream_t stream = (hipStream_t)hip_stream;
   // The fewest registers that hold a head's weights, in waves that still leave other heads room (400 heads of 1024
   // rows: 26.4 us with 8 waves of 2 a lane, 28.1 with 4 of 4, 30.2 with 16 of 1; 32 heads of 32768: 63.3 with 16 of
   // 32, 80.5 with 8 of 64).
   if (n_max <= 1024)
     launch<8, 2>(a, B, stream);
-  else if (n_max <= 4096)
+  else if (n_max <= kFewRows)
     launch<16, 4>(a, B, stream);
   else if (n_max <= kMaxRows)
     launch<16, 32>(a, B, stream);
