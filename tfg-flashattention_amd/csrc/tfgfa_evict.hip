@@ -164,22 +164,22 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
   if (bad) sh_bad = 1;
   if constexpr (kR > 0) {
 #pragma unroll
-    for (int r = 0; r < kR; ++r) q[r] = rank_key(x[r]);
+    for (int r = 0; r < kR; ++r) q[r] = first + r * 64 + lane < old ? rank_key(x[r]) : 0u;
   }
-  // f(row, key, whether it is one to choose from) for this wave's rows in order.
+  // f(key) for this wave's rows in order.  Rows that are not to be chosen from have the lowest key, which as the last one
+  // in every order changes no count from above.
   auto rows = [&](auto f) {
     if constexpr (kR > 0) {
 #pragma unroll
       for (int r = 0; r < kR; ++r) {
         if (first + r * 64 >= old) break;
-        const int j = first + r * 64 + lane;
-        f(j, q[r], j < old);
+        f(q[r]);
       }
     } else {
       for (int r = 0; r < regs; ++r) {
         if (first + r * 64 >= old) break;
         const int j = first + r * 64 + lane;
-        f(j, j < old ? rank_key(w[j]) : 0u, j < old);
+        f(j < old ? rank_key(w[j]) : 0u);
       }
     }
   };
@@ -232,12 +232,9 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
   };
   if (chosen > 0 && chosen < old) {
     clear();
-    rows([&](int j, uint32_t y, bool in) {
-      // (Of most registers every row is in: then a compare says whether all have one digit.)
+    rows([&](uint32_t y) {
       const int digit = y >> 21;
-      if (__builtin_amdgcn_ballot_w64(!in) != 0)
-        count(in, digit);
-      else if (__builtin_amdgcn_ballot_w64(digit != __builtin_amdgcn_readfirstlane(digit)) != 0)
+      if (__builtin_amdgcn_ballot_w64(digit != __builtin_amdgcn_readfirstlane(digit)) != 0)
         atomicAdd(&hist[digit], 1);
       else if (lane == 0)
         atomicAdd(&hist[digit], 64);
@@ -246,8 +243,13 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
     const int same = hist[key >> 21];
     if (kList && same <= kCandidates) {
       __syncthreads();  // (the histogram has been read)
-      rows([&](int j, uint32_t y, bool in) {
-        if (in && y >> 21 == key >> 21) list[atomicAdd(&sh_count, 1) & (kCandidates - 1)] = y;
+      int mine = 0;
+      rows([&](uint32_t y) { mine += y >> 21 == key >> 21 ? 1 : 0; });
+      const int upto = scan64(mine);
+      int at = lane == 63 ? atomicAdd(&sh_count, upto) : 0;
+      at = __builtin_amdgcn_readlane(at, 63) + upto - mine;
+      rows([&](uint32_t y) {
+        if (y >> 21 == key >> 21) list[at++ & (kCandidates - 1)] = y;
       });
 #pragma unroll 1
       for (int shift = 10; shift >= 0; shift -= 10) {
@@ -265,9 +267,7 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
         const int top = shift == 10 ? 21 : 10;
         __syncthreads();
         clear();
-        rows([&](int j, uint32_t y, bool in) {
-          count(in && y >> top == key >> top, (y >> shift) & ((1 << (top - shift)) - 1));
-        });
+        rows([&](uint32_t y) { count(y >> top == key >> top, (y >> shift) & ((1 << (top - shift)) - 1)); });
         find(shift);
       }
     }
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
     // and of the wanted ties.  Rows past the last have the lowest key: as ties they come after all that are wanted.
     auto key_of = [&](int r) {
       const int j = first + r * 64 + lane;
-      return j < old ? q[r] : j < L ? 0xFFFFFFFFu : 0u;
+      return j >= old && j < L ? 0xFFFFFFFFu : q[r];
     };
     // Those of the waves before.  (Every weight is in a register by now: `out` may be `w`.)
     int taken = 0, ties = 0;
