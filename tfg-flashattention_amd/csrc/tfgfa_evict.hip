@@ -152,8 +152,11 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
   float x[kR > 0 ? kR : 1];
   uint32_t q[kR > 0 ? kR : 1];
   if constexpr (kR > 0) {
+    // (Past the last row the buffer gives zeros.)
+    const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(w), (short)0, 4 * L, 0x00020000);
 #pragma unroll
-    for (int r = 0; r < kR; ++r) x[r] = first + r * 64 + lane < L ? w[first + r * 64 + lane] : 0.f;
+    for (int r = 0; r < kR; ++r)
+      x[r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(from, (first + lane) * 4 + r * 256, 0, 0));
   }
   for (int c = tid; c < (L + a.page - 1) / a.page; c += kThreads)
     bad |= (uint32_t)a.table[b * a.table_stride + c] >= (uint32_t)a.P;
