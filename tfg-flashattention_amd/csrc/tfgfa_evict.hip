@@ -14,9 +14,9 @@
 // copy_kernel: 16 bytes a thread and step, rows of K and V through both page tables.  Bound: HBM, 4D bytes read and
 // 4D written a kept row.  Where a head has few rows to copy, the selecting workgroup copies them itself.
 //
-// Measured: 32 heads of up to 32768 rows, D = 128, cut to 4096: selection 27 us (32 of 256 CUs have work; loads 3,
-// first histogram 5, candidates 4, places and stores 8), copies 22.5 us, 6 TB/s of reads and writes; 16 sequences of
-// 25 heads of up to 1024 rows cut to 512: 8 and 15.3 us; one sequence of 12 heads, 300 rows cut to 130, 7.7 us in one
+// Measured: 32 heads of up to 32768 rows, D = 128, cut to 4096: selection 23 us (32 of 256 CUs have work; 56% of the
+// wave cycles in waits, for loads and at 17 barriers), copies 22 us, 6 TB/s of reads and writes; 16 sequences of 25
+// heads of up to 1024 rows cut to 512: 7.4 and 15.4 us; one sequence of 12 heads, 300 rows cut to 130, 7.5 us in one
 // launch.
 #include <hip/hip_runtime.h>
 
@@ -40,13 +40,13 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kMaxD = 128;
 constexpr int kBins = 2048;
 constexpr int kMaxFused = kBins;  // rows that a selecting workgroup may copy itself (their list is in LDS)
-// Rows with the first digit of the last one kept that a list holds, for the other digits (63.8 us at 32768 rows, 68.6
+// Rows with the first digit of the last one kept that a list holds, for the other digits (59.2 us at 32768 rows, 61.8
 // with the registers gone through again).
 constexpr int kCandidates = 4096;
 constexpr int kFewRows = 4096;    // rows of a sequence that four weights a lane hold
 constexpr int kMaxRows = 32768;   // rows of a sequence whose weights stay in registers
-// rows * D of a head up to which the selecting workgroup copies them (12 heads, 130 rows: 7.7 us, with two kernels
-// 9.8; 400 heads of 512 rows: 28.4 and 26.4).
+// rows * D of a head up to which the selecting workgroup copies them (12 heads, 130 rows: 7.6 us, with two kernels
+// 9.7; 400 heads of 512 rows: 28.2 and 26.4).
 constexpr int kFusedValues = 16384;
 constexpr int kCopy = 4;          // rows of a thread of the copying kernel
 
@@ -434,8 +434,8 @@ extern "C" int tfserve_evict(void* k_pages, const int64_t* k_strides, void* v_pa
   a.fused = n_max <= kFewRows && rows <= kMaxFused && (long long)rows * D <= kFusedValues;
   const hipStream_t stream = (hipStream_t)hip_stream;
   // The fewest registers that hold a head's weights, in waves that still leave other heads room (400 heads of 1024
-  // rows: 26.4 us with 8 waves of 2 a lane, 28.1 with 4 of 4, 30.2 with 16 of 1; 32 heads of 32768: 63.3 with 16 of
-  // 32, 80.5 with 8 of 64).
+  // rows: 26.4 us with 8 waves of 2 a lane, 26.8 with 4 of 4, 30.2 with 16 of 1; 12 heads: 8.8, 10.8 and 9.1; 32 heads
+  // of 32768: 59.2 with 16 of 32, 63.3 with 8 of 64).
   if (n_max <= 1024)
     launch<8, 2>(a, B, stream);
   else if (n_max <= kFewRows)
