@@ -76,14 +76,21 @@ size_t tfserve_decode_paged_workspace(int B, int H, int H_kv, int page, int M, i
  * q: (B, H, N_q, D), k: (B, H_kv, N_k, D), strides [b, h, n, d] as for tfgfa_fwd; lse: float32
  * (B, H, N_q), strides [b, h], last dimension dense, the log-sum-exp the attention returned; out: float32
  * (B, H_kv, N_k), strides [b, h], last dimension dense, written whole.  A query whose lse is -inf (or
- * past 2^127 in magnitude) adds nothing; hidden pairs add nothing whatever they hold.  The result does not depend on the device's
- * scheduling: sums are added in a fixed order.
+ * past 2^127 in magnitude) adds nothing; hidden pairs add nothing whatever they hold.  The result does
+ * not depend on the device's scheduling: sums are added in a fixed order.
+ *
+ * workspace (16-byte aligned, device memory, no initialisation): tfserve_key_weights_workspace bytes let the
+ * queries of a block of keys be divided over several workgroups where there are few keys; fewer (or NULL) is
+ * correct but slower.  Calls sharing a workspace must be ordered on one stream.
  */
 int tfserve_key_weights(const void* q, const int64_t* q_strides, const void* k,
                         const int64_t* k_strides, const float* lse, const int64_t* lse_strides,
                         float* out, const int64_t* out_strides, int B, int H, int H_kv, int N_q,
                         int N_k, int D, int dtype, float softmax_scale, int causal,
-                        int64_t first_query, void* hip_stream);
+                        int64_t first_query, void* workspace, size_t workspace_bytes, void* hip_stream);
+
+/* Workspace bytes for the above (0 where nothing is divided, and for sizes out of range). */
+size_t tfserve_key_weights_workspace(int B, int H, int H_kv, int N_q, int N_k, int causal);
 
 /*
  * Eviction from a paged cache (laid out as above) by accumulated weight.  Of the L = cache_seqlens[b] rows

@@ -521,6 +521,53 @@ def test_key_weights_match_64_bits(H, H_kv, Nq, Nk, D, dtype, causal, first):
     assert torch.equal(fa.key_weights(q, k, lse, first_query=first, causal=causal), out), "another run"
 
 
+@pytest.mark.parametrize("B,H,H_kv,Nq,Nk,D,dtype,causal", [
+    (1, 16, 1, 1000, 1000, 64, BF, True),
+    (2, 24, 3, 700, 333, 128, HF, False),
+    (1, 32, 4, 65, 300, 80, BF, True),
+    (1, 3, 3, 2000, 129, 64, HF, True),      # the queries past the keys' positions see them all
+    (1, 16, 1, 129, 2000, 40, BF, False),
+])
+def test_key_weights_divided_queries(B, H, H_kv, Nq, Nk, D, dtype, causal):
+    """Few keys and many queries: the queries go to several workgroups, whose sums are added in order."""
+    g = _gen(Nq + Nk)
+    q, k = _randn((B, H, Nq, D), g, dtype), _randn((B, H_kv, Nk, D), g, dtype)
+    G, scale = H // H_kv, D ** -0.5
+    hide = (torch.arange(Nk)[None, :] > torch.arange(Nq)[:, None]) if causal else torch.zeros(Nq, Nk, dtype=torch.bool)
+    lse, want, bound = torch.empty(B, H, Nq), torch.zeros(B, H_kv, Nk, dtype=torch.float64), torch.zeros(B, H_kv, Nk, dtype=torch.float64)
+    for b in range(B):
+        for h in range(H):
+            qd, kd = q[b, h].double().cpu(), k[b, h // G].double().cpu()
+            x = (scale * qd @ kd.T.contiguous()).masked_fill(hide, -INF)
+            lse[b, h] = torch.logsumexp(x, 1).float()
+            p = torch.exp(x - lse[b, h].double()[:, None])
+            big = float((scale * qd.abs() @ kd.abs().T.contiguous()).max())
+            e = 2.1 * ((D + 4) * U * big + 4 * U * (2 * big + float(lse[b, h].abs().max())))
+            want[b, h // G] += p.sum(0)
+            bound[b, h // G] += (e + (Nq * G + 80) * U) * p.sum(0)
+    lse = lse.to(DEV)
+    n = _C.key_weights_workspace(B, H, H_kv, Nq, Nk, causal)
+    assert n > 0
+    got = fa.key_weights(q, k, lse, causal=causal)
+    _near(got, want, bound, "divided")
+    _near(fa.key_weights(q, k, lse, causal=causal, workspace=torch.empty(64, dtype=torch.uint8, device=DEV)), want, bound, "whole")
+    for fill in (0, 0x5A, 0xFF):
+        ws = torch.full((n,), fill, dtype=torch.uint8, device=DEV)
+        for _ in range(3):
+            assert torch.equal(fa.key_weights(q, k, lse, causal=causal, workspace=ws), got), fill
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        held = fa.key_weights(q, k, lse, causal=causal)
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(3):
+        held.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, got) and torch.equal(fa.key_weights(q, k, lse, causal=causal), got)
+
+
 def test_key_weights_of_hidden_and_empty_rows():
     """Keys that no query sees get 0 whatever they hold; a query whose lse is -inf adds nothing; NaN in a query
     reaches only the keys it sees; no queries at all give zeros."""

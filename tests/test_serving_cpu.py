@@ -30,7 +30,7 @@ def test_library_exports_the_serving_entry_points(lib):
     text = re.sub(r"/\*.*?\*/", "", open(os.path.join(INCLUDE, "tfgfa_serving.h")).read(), flags=re.S)
     names = sorted(set(re.findall(r"\b(tfserve_\w+)\s*\(", text)))
     assert names == ["tfserve_decode_paged", "tfserve_decode_paged_workspace", "tfserve_evict", "tfserve_key_weights",
-                     "tfserve_penalize"]
+                     "tfserve_key_weights_workspace", "tfserve_penalize"]
     assert all(hasattr(lib, n) for n in names) and lib.tfgfa_abi_version() >= 10
 
 
@@ -94,6 +94,16 @@ def test_decode_paged_refuses(lib, kw, code):
     assert _paged(lib, **kw) == _code(code)
 
 
+def test_key_weights_workspace(lib):
+    size = lib.tfserve_key_weights_workspace
+    size.restype = ctypes.c_size_t
+    assert size(1, 12, 12, 256, 256, 1) == 0 and size(1, 16, 1, 0, 100, 1) == 0 and size(1, 16, 3, 100, 100, 1) == 0
+    assert size(8, 64, 64, 4096, 32768, 1) == 0   # keys enough
+    n = size(1, 16, 1, 2930, 2930, 1)
+    assert 23 * 128 + 2 * 23 * 512 <= n <= 1 << 20
+    assert size(1, 16, 1, 2930, 2930, 0) >= n // 2 and n == _C.key_weights_workspace(1, 16, 1, 2930, 2930, True)
+
+
 def test_decode_paged_workspace(lib):
     f = lib.tfserve_decode_paged_workspace
     f.restype = ctypes.c_size_t
@@ -109,12 +119,13 @@ def test_decode_paged_workspace(lib):
 
 def _weights(lib, **kw):
     a = dict(q=P, qs=(6400, 64, 640, 1), k=P, ks=(6400, 64, 640, 1), lse=P, ls=(1000, 10), out=P, os=(1000, 20), B=2,
-             H=10, Hkv=10, Nq=10, Nk=20, D=64, dtype=0, scale=0.125, causal=1, first=0)
+             H=10, Hkv=10, Nq=10, Nk=20, D=64, dtype=0, scale=0.125, causal=1, first=0, work=0, bytes=0)
     a.update(kw)
     return lib.tfserve_key_weights(
         _ptr(a["q"]), _strides(*a["qs"]), _ptr(a["k"]), _strides(*a["ks"]), _ptr(a["lse"]), _strides(*a["ls"]),
         _ptr(a["out"]), _strides(*a["os"]), a["B"], a["H"], a["Hkv"], a["Nq"], a["Nk"], a["D"], a["dtype"],
-        ctypes.c_float(a["scale"]), a["causal"], I64(a["first"]), _ptr(0))
+        ctypes.c_float(a["scale"]), a["causal"], I64(a["first"]), _ptr(a["work"]),
+        ctypes.c_size_t(a["bytes"]), _ptr(0))
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -125,6 +136,7 @@ def _weights(lib, **kw):
     (dict(D=12), "ERR_HEAD_DIM"),
     (dict(scale=-1.0), "ERR_SCALE"),
     (dict(causal=2), "ERR_CAUSAL_FLAG"),
+    (dict(work=P + 8, bytes=1 << 20), "ERR_ALIGNMENT"),
     (dict(Nk=0), "OK"),
     (dict(B=0), "OK"),
     (dict(k=0), "ERR_NULL_POINTER"),

@@ -250,7 +250,8 @@ void decode_paged(std::uintptr_t q, const Strides3& qs, std::uintptr_t k, const 
 void key_weights(std::uintptr_t q, const Strides4& qs, std::uintptr_t k, const Strides4& ks,
                  std::uintptr_t lse, const Strides2& ls, std::uintptr_t out, const Strides2& os,
                  int B, int H, int H_kv, int N_q, int N_k, int D, int dtype, float softmax_scale,
-                 bool causal, std::int64_t first_query, std::uintptr_t stream) {
+                 bool causal, std::int64_t first_query, std::uintptr_t workspace,
+                 std::size_t workspace_bytes, std::uintptr_t stream) {
   int st;
   {
     py::gil_scoped_release nogil;
@@ -259,6 +260,7 @@ void key_weights(std::uintptr_t q, const Strides4& qs, std::uintptr_t k, const S
                              reinterpret_cast<const float*>(lse), ls.data(),
                              reinterpret_cast<float*>(out), os.data(), B, H, H_kv, N_q, N_k, D,
                              dtype, softmax_scale, causal ? 1 : 0, first_query,
+                             reinterpret_cast<void*>(workspace), workspace_bytes,
                              reinterpret_cast<void*>(stream));
   }
   check(st, "tfserve_key_weights");
@@ -413,7 +415,11 @@ PYBIND11_MODULE(_C, m) {
         py::arg("q_strides"), py::arg("k"), py::arg("k_strides"), py::arg("lse"),
         py::arg("lse_strides"), py::arg("out"), py::arg("out_strides"), py::arg("B"), py::arg("H"),
         py::arg("H_kv"), py::arg("N_q"), py::arg("N_k"), py::arg("D"), py::arg("dtype"),
-        py::arg("softmax_scale"), py::arg("causal"), py::arg("first_query"), py::arg("stream"));
+        py::arg("softmax_scale"), py::arg("causal"), py::arg("first_query"), py::arg("workspace"),
+        py::arg("workspace_bytes"), py::arg("stream"));
+  m.def("key_weights_workspace", [](int B, int H, int H_kv, int N_q, int N_k, bool causal) {
+    return tfserve_key_weights_workspace(B, H, H_kv, N_q, N_k, causal ? 1 : 0);
+  });
   m.def("evict", &evict, "Eviction from a paged KV cache by accumulated weight",
         py::arg("k_pages"), py::arg("k_strides"), py::arg("v_pages"), py::arg("v_strides"),
         py::arg("page_table"), py::arg("table_stride"), py::arg("cache_seqlens"),

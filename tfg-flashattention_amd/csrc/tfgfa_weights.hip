@@ -27,9 +27,11 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "tfgfa.h"
+#include "tfgfa_arrive.h"
 #include "tfgfa_device.h"
 #include "tfgfa_layout.h"
 #include "tfgfa_serving.h"
@@ -41,6 +43,7 @@ using tfgfa::Rows;
 using tfgfa::rows_ok;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned long long u64;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -76,6 +79,11 @@ struct Args {
   long long first;
   float scale_log2;
   int Hkv, units, cu, G, Nq, Nk, D, causal;
+  // Where the queries of a block of keys are divided: parts, tiles of a part, arrival words and sums of parts.
+  int splits, part_tiles;
+  char* arrive;
+  float* part;
+  u64 tag;
 };
 
 // Rows of queries in LDS: kChunks chunks of 16 bytes, chunk c of row r at place c ^ turn(r), so that the rows of a
@@ -115,43 +123,63 @@ __device__ __forceinline__ int key_of(int lane) {
 }
 
 // kP: pieces of 16 dims, D <= 16 kP; a lane holds dims 16p + 8 (l / 32) .. + 7 of row l % 32.
-template <class T, int kP>
+// kSplit: a block of keys is several workgroups', each with part_tiles tiles of its queries; they leave their sums in the
+// workspace, and the one that arrives last adds them in order (arrival words and memory order as in tfgfa_decode.hip).
+template <class T, int kP, bool kSplit>
 __global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(const Args a) {
   constexpr int kChunks = 2 * kP, kRowBytes = 16 * kChunks, kBytes = kQueries * kRowBytes;
   constexpr int kMoves = kBytes / 1024 / kWaves;  // 1-KiB transfers of a wave
   __shared__ __attribute__((aligned(1024))) unsigned char buf[2][kBytes];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, i = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int id = blockIdx.x;
-  if (a.causal && id / a.cu % 2 != 0) {
+  int id = blockIdx.x, piece = 0;
+  if constexpr (kSplit) {
+    id = blockIdx.x / a.splits;
+    piece = blockIdx.x - id * a.splits;
+  } else if (a.causal && id / a.cu % 2 != 0) {
     const int first = id / a.cu * a.cu;
     id = first + min(first + a.cu, (int)gridDim.x) - 1 - id;
   }
   const int y = id / a.units, unit = id - y * a.units;
   const int b = unit / a.Hkv, kv = unit - b * a.Hkv;
   const int jw = y * kKeys, j0 = jw + wave * kTile;  // first key of the workgroup, of the wave
+  // Tiles of queries that see a key of this workgroup, for each of the head's query heads in turn.
+  const int tiles = (a.Nq + kQueries - 1) / kQueries;
+  int t0 = 0;
+  if (a.causal && jw > a.first) t0 = (int)min((long long)tiles, (jw - a.first) / kQueries);
+  const int per = tiles - t0;
+  int all = per * a.G, parts = 1, from_tile = 0;
+  u64* const aw = reinterpret_cast<u64*>(a.arrive + (long long)id * tfgfa::kArriveStride);
+  u64 aw_start = 0;
+  if constexpr (kSplit) {
+    parts = max(1, (all + a.part_tiles - 1) / a.part_tiles);
+    if (piece >= parts) return;
+    from_tile = piece * a.part_tiles;
+    all = min(a.part_tiles, all - from_tile);
+    if (parts > 1 && tid == 0) aw_start = __hip_atomic_load(aw, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
   u32x4 kf[kP];
   const T* const kr = static_cast<const T*>(a.k) + b * a.ks.b + kv * a.ks.h + (long long)(j0 + i) * a.ks.n + 8 * half;
 #pragma unroll
   for (int p = 0; p < kP; ++p)
     kf[p] = j0 + i < a.Nk && 16 * p + 8 * half < a.D ? *reinterpret_cast<const u32x4*>(kr + 16 * p)
                                                      : u32x4{0, 0, 0, 0};
-  // Tiles of queries that see a key of this workgroup, for each of the head's query heads in turn.
-  const int tiles = (a.Nq + kQueries - 1) / kQueries;
-  int t0 = 0;
-  if (a.causal && jw > a.first) t0 = (int)min((long long)tiles, (jw - a.first) / kQueries);
-  const int per = tiles - t0, all = per * a.G;
 
   const uint32_t at = tfgfa::lds_addr(&buf[0][0]);
   const int row_bytes = (int)a.qs.n * 2;
   float z[2], next[2];  // lse of the lane's query of each half of a tile; past the last query 0
   // The next tile's queries and their lse, and how many there are from it on in this head.
-  const T* q = static_cast<const T*>(a.q) + b * a.qs.b + kv * a.G * a.qs.h + (long long)t0 * kQueries * a.qs.n;
-  const float* lse = a.lse + b * a.lb + kv * a.G * a.lh + t0 * kQueries;
+  int t = t0, h = kv * a.G;
+  if (kSplit && per > 0) {
+    const int g = __builtin_amdgcn_readfirstlane(from_tile / per);
+    h += g, t += from_tile - g * per;
+  }
+  const T* q = static_cast<const T*>(a.q) + b * a.qs.b + h * a.qs.h + (long long)t * kQueries * a.qs.n;
+  const float* lse = a.lse + b * a.lb + h * a.lh + t * kQueries;
   const int left0 = a.Nq - t0 * kQueries;
   const long long q_tile = kQueries * a.qs.n;
   const long long q_head = a.qs.h - (long long)per * q_tile, lse_head = a.lh - (long long)per * kQueries;
-  int left = left0;
+  int left = a.Nq - t * kQueries;
   // The next tile into buffer n: lane l of a transfer writes 16 bytes at 16 l of its KiB.
   auto load = [&](int n) {
     const int rows = min(kQueries, left);
@@ -183,7 +211,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(const Args a) {
   if (a.causal && j0 + kTile - 1 > a.first)
     from = (int)min((long long)tiles, (j0 + kTile - 1 - a.first + kQueries - 1) / kQueries);
   const int upto = a.Nq / kQueries;
-  int t = t0;
   if (all > 0) load(0);
 #pragma unroll 1
   for (int w = 0; w < all; ++w) {
@@ -234,16 +261,96 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(const Args a) {
   }
   const int j = j0 + key_of(lane);
   const float x = over_queries(sum, lane);
-  if ((lane & 1) == 0 && j < a.Nk) a.out[b * a.ob + kv * a.oh + j] = x;
+  float* const out = a.out + b * a.ob + kv * a.oh;
+  if (!kSplit || parts == 1) {
+    if ((lane & 1) == 0 && j < a.Nk) out[j] = x;
+    return;
+  }
+  if constexpr (kSplit) {
+    __shared__ int sh_last;
+    float* const mine = a.part + (long long)id * a.splits * kKeys;
+    if ((lane & 1) == 0)
+      __hip_atomic_store(mine + piece * kKeys + (j - jw), x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // The part is at the coherence point once its stores are acknowledged; then the arrival is counted.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) {
+      if ((aw_start >> tfgfa::kTagShift) != a.tag) {
+        u64 expected = aw_start;
+        __hip_atomic_compare_exchange_strong(aw, &expected, a.tag << tfgfa::kTagShift, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
+                                             __HIP_MEMORY_SCOPE_AGENT);
+      }
+      const u64 old = __hip_atomic_fetch_add(aw, (u64)1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int last = (old & ((1ull << tfgfa::kTagShift) - 1)) == (u64)(parts - 1);
+      if (last) __hip_atomic_store(aw, (u64)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      sh_last = last;
+    }
+    __syncthreads();
+    if (!sh_last || tid >= kKeys || jw + tid >= a.Nk) return;
+    asm volatile("" ::: "memory");
+    float total = 0.f;
+    constexpr int kBatch = 8;
+    for (int s0 = 0; s0 < parts; s0 += kBatch) {
+      float z[kBatch];
+#pragma unroll
+      for (int s = 0; s < kBatch; ++s)
+        z[s] = s0 + s < parts
+                   ? __hip_atomic_load(mine + (s0 + s) * kKeys + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                   : 0.f;
+#pragma unroll
+      for (int s = 0; s < kBatch; ++s) total += z[s];
+    }
+    out[jw + tid] = total;
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Host side.
+
+constexpr int kMaxCu = 1024;    // for the workspace's size, which does not depend on the device
+// The least tiles of a part (16 heads on 1, 727 queries and keys, 3 sequences: 12.3 us, with 2 12.8, with 8 15.0; 512
+// queries of 12 heads 7.6, 6.4, 8.7; 1369 of 16, D = 128, 15.7, 18.5, 16.3).
+constexpr int kMinTiles = 4;
+constexpr int kMaxSplits = 64;
+// Workgroups of a CU that a division aims at (32 heads on 4, D = 80, 2081 queries: 36 us, with 2 49, with 8 38; 32 on 8, D
+// = 128, 2 x 1504: 39.7, 38.7 and 45.9).
+constexpr int kSlots = 4;
+
+// Parts of a block of keys and tiles of a part on a device of `cu` CUs: 1 and 0 where the blocks of keys fill it, or have
+// few queries.  (16 heads on 1, 2930 queries and keys: 26.5 us, not divided 482; 32 on 4, 1792: 23 and 145; 12 heads of
+// 1024: 9.7 and 13.2.  Twice as many blocks as CUs divided too: 200 heads of 512, 13.4 -> 19.0.)
+struct Split {
+  int splits, tiles;
+};
+static Split choose_split(long long units, int G, int N_q, int N_k, int causal, int cu) {
+  const long long blocks = (N_k + kKeys - 1) / kKeys * units, tiles = (long long)((N_q + kQueries - 1) / kQueries) * G;
+  if (blocks >= 2LL * cu || tiles < 2 * kMinTiles) return {1, 0};
+  // (Under a causal mask about half the tiles are seen.)
+  const long long share = blocks * tiles / (causal ? 2 : 1) / ((long long)kSlots * cu);
+  const long long part = std::max<long long>({kMinTiles, share, (tiles + kMaxSplits - 1) / kMaxSplits});
+  return {(int)((tiles + part - 1) / part), (int)part};
+}
+static size_t split_bytes(long long blocks, int splits) {
+  return splits > 1 ? tfgfa::arrive_bytes(blocks) + (size_t)blocks * splits * kKeys * 4 : 0;
 }
 
 }  // namespace tfgfa_weights
+
+extern "C" size_t tfserve_key_weights_workspace(int B, int H, int H_kv, int N_q, int N_k, int causal) {
+  using namespace tfgfa_weights;
+  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || N_q <= 0 || N_k <= 0) return 0;
+  const long long units = (long long)B * H_kv;
+  if (units > INT32_MAX / 4096 || (N_k / kKeys + 1) * units > INT32_MAX) return 0;
+  // (A device of fewer CUs divides less.)
+  const Split s = choose_split(units, H / H_kv, N_q, N_k, causal, kMaxCu);
+  return split_bytes((long long)((N_k + kKeys - 1) / kKeys) * units, s.splits);
+}
 
 extern "C" int tfserve_key_weights(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                                    const float* lse, const int64_t* lse_strides, float* out,
                                    const int64_t* out_strides, int B, int H, int H_kv, int N_q, int N_k, int D,
                                    int dtype, float softmax_scale, int causal, int64_t first_query,
-                                   void* hip_stream) {
+                                   void* workspace, size_t workspace_bytes, void* hip_stream) {
   using namespace tfgfa_weights;
   if (dtype != TFGFA_DTYPE_BF16 && dtype != TFGFA_DTYPE_F16) return TFGFA_ERR_DTYPE;
   if (B < 0 || H < 0 || H_kv < 0 || N_q < 0 || N_k < 0 || first_query < 0) return TFGFA_ERR_BAD_SHAPE;
@@ -264,7 +371,7 @@ extern "C" int tfserve_key_weights(const void* q, const int64_t* q_strides, cons
   if (a.qs.n > INT32_MAX / (4 * kQueries)) return TFGFA_ERR_TOO_LARGE;
   if (!k || !out || (N_q > 0 && (!q || !lse))) return TFGFA_ERR_NULL_POINTER;
   if (((uintptr_t)q | (uintptr_t)k) & 15u) return TFGFA_ERR_ALIGNMENT;
-  if (((uintptr_t)lse | (uintptr_t)out) & 3u) return TFGFA_ERR_ALIGNMENT;
+  if ((((uintptr_t)lse | (uintptr_t)out) & 3u) || ((uintptr_t)workspace & 15u)) return TFGFA_ERR_ALIGNMENT;
   a.lb = B > 1 ? lse_strides[0] : 0, a.lh = H > 1 ? lse_strides[1] : 0;
   a.ob = B > 1 ? out_strides[0] : 0, a.oh = H_kv > 1 ? out_strides[1] : 0;
   if (a.lb < 0 || a.lh < 0 || !apart(a.ob, B, a.oh, H_kv, N_k))
@@ -277,19 +384,32 @@ extern "C" int tfserve_key_weights(const void* q, const int64_t* q_strides, cons
   const int st = tfgfa_device_info(&a.cu, nullptr, nullptr, 0);
   if (st != TFGFA_OK) return st;
   const hipStream_t stream = (hipStream_t)hip_stream;
-  const dim3 grid((unsigned)((N_k + kKeys - 1) / kKeys * units));
-#define TFGFA_WEIGHTS(T)                                                                            \
-  do {                                                                                              \
-    if (D <= 64)                                                                                    \
-      hipLaunchKernelGGL((weights_kernel<T, 4>), grid, dim3(64 * kWaves), 0, stream, a);            \
-    else                                                                                            \
-      hipLaunchKernelGGL((weights_kernel<T, 8>), grid, dim3(64 * kWaves), 0, stream, a);            \
+  const long long blocks = (long long)((N_k + kKeys - 1) / kKeys) * units;
+  Split s = choose_split(units, a.G, N_q, N_k, causal, std::min(a.cu, kMaxCu));
+  // Without a workspace that holds the parts, a block of keys is one workgroup's.
+  if (split_bytes(blocks, s.splits) > (workspace ? workspace_bytes : 0)) s = {1, 0};
+  a.splits = s.splits, a.part_tiles = s.tiles;
+  a.arrive = static_cast<char*>(workspace);
+  if (s.splits > 1) {
+    a.part = reinterpret_cast<float*>(a.arrive + tfgfa::arrive_bytes(blocks));
+    a.tag = tfgfa::next_tag();
+  }
+  const dim3 grid((unsigned)(blocks * s.splits));
+#define TFGFA_WEIGHTS_(T, kP, kSplit) \
+  hipLaunchKernelGGL((weights_kernel<T, kP, kSplit>), grid, dim3(64 * kWaves), 0, stream, a)
+#define TFGFA_WEIGHTS(T)                                       \
+  do {                                                         \
+    if (D <= 64 && s.splits > 1) TFGFA_WEIGHTS_(T, 4, true);   \
+    else if (D <= 64) TFGFA_WEIGHTS_(T, 4, false);             \
+    else if (s.splits > 1) TFGFA_WEIGHTS_(T, 8, true);         \
+    else TFGFA_WEIGHTS_(T, 8, false);                          \
   } while (0)
   if (dtype == TFGFA_DTYPE_BF16)
     TFGFA_WEIGHTS(__bf16);
   else
     TFGFA_WEIGHTS(_Float16);
 #undef TFGFA_WEIGHTS
+#undef TFGFA_WEIGHTS_
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? TFGFA_OK : -(int)e;
 }

@@ -63,6 +63,23 @@ def _check_weights(t, name: str, B: int, H_kv: int, rows: int, dev) -> None:
         raise RuntimeError(f"{name} must be on {dev} and dense in its last dimension")
 
 
+def _workspace(index: int, nbytes: int) -> tuple[int, int]:
+    """(pointer, bytes) of the workspace of device ``index``'s current stream, of at least ``nbytes``."""
+    if not nbytes:
+        return 0, 0
+    dev = torch.device("cuda", index)
+    workspace = None if torch.cuda.is_current_stream_capturing() else _WORKSPACES.get((dev, _current_stream(index)))
+    if workspace is None or workspace.numel() < nbytes:
+        workspace = _decode_workspace(dev, nbytes)
+    return workspace.data_ptr(), workspace.numel()
+
+
+def _given_workspace(workspace, like) -> tuple[int, int]:
+    if not workspace.is_cuda or workspace.get_device() != like.get_device() or not workspace.is_contiguous():
+        raise RuntimeError(f"workspace must be a contiguous tensor on {like.device}")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
 def _accepts_pages(k_pages, v_pages, index) -> bool:
     """Everything _check_pages checks, as one test."""
     ks, dtype = k_pages.shape, k_pages.dtype
@@ -162,19 +179,10 @@ def decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, H, D))
     scale = (1.0 / math.sqrt(D)) if softmax_scale is None else float(softmax_scale)
     lse = q.new_empty((B, H), dtype=torch.float32) if return_lse else None
-    work, nbytes = 0, 0
-    if workspace is not None:
-        if not workspace.is_cuda or workspace.get_device() != index or not workspace.is_contiguous():
-            raise RuntimeError(f"workspace must be a contiguous tensor on {k_pages.device}")
-        work, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    if workspace is None:
+        work, nbytes = _workspace(index, _C.decode_paged_workspace(B, H, H_kv, page, M, D, key_weights is not None))
     else:
-        nbytes = _C.decode_paged_workspace(B, H, H_kv, page, M, D, key_weights is not None)
-        if nbytes:
-            dev = k_pages.device
-            workspace = None if torch.cuda.is_current_stream_capturing() else _WORKSPACES.get((dev, _current_stream(index)))
-            if workspace is None or workspace.numel() < nbytes:
-                workspace = _decode_workspace(dev, nbytes)
-            work, nbytes = workspace.data_ptr(), workspace.numel()
+        work, nbytes = _given_workspace(workspace, k_pages)
     _launch_on(index, _C.decode_paged,
                q.data_ptr(), q.stride(), k_pages.data_ptr(), k_pages.stride(), v_pages.data_ptr(), v_pages.stride(),
                page_table.data_ptr(), page_table.stride(0), cache_seqlens.data_ptr(),
@@ -235,7 +243,8 @@ def _check_key_weights(q, k, lse, first_query, out) -> None:
 
 
 def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, first_query: int = 0,
-                out: torch.Tensor | None = None, softmax_scale: float | None = None, causal: bool = True):
+                out: torch.Tensor | None = None, softmax_scale: float | None = None, causal: bool = True,
+                workspace: torch.Tensor | None = None):
     """The attention weight each key receives from given queries: what a cache's ``key_weights``
     (:func:`decode_paged`) start from after a prompt.
 
@@ -247,6 +256,8 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, first_qu
     last w queries of a prompt of N are ``q[:, :, -w:]``, ``lse[:, :, -w:]`` with ``first_query=N - w``.
     A query whose lse is -inf adds nothing.  Returns ``out``, float32 (B, H_kv, N_k) (new if not given; a view
     into a cache's weights with a dense last dimension is taken).  Sums are added in a fixed order.
+    ``workspace`` as for :func:`decode`, of ``_C.key_weights_workspace(B, H, H_kv, N_q, N_k, causal)`` bytes (0 where
+    the keys fill the device); with a smaller one a block of keys is one workgroup's, whatever its queries.
     """
     if not _accepts_weights(q, k, lse, first_query, out):
         _check_key_weights(q, k, lse, first_query, out)
@@ -255,9 +266,14 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, first_qu
     if out is None:
         out = lse.new_empty((B, H_kv, N_k))
     scale = (1.0 / math.sqrt(D)) if softmax_scale is None else float(softmax_scale)
-    _launch_on(q.get_device(), _C.key_weights, q.data_ptr(), q.stride(), k.data_ptr(), k.stride(),
+    index = q.get_device()
+    if workspace is None:
+        work, nbytes = _workspace(index, _C.key_weights_workspace(B, H, H_kv, N_q, N_k, bool(causal)))
+    else:
+        work, nbytes = _given_workspace(workspace, q)
+    _launch_on(index, _C.key_weights, q.data_ptr(), q.stride(), k.data_ptr(), k.stride(),
                lse.data_ptr(), lse.stride()[:2], out.data_ptr(), out.stride()[:2], B, H, H_kv, N_q, N_k, D,
-               _DTYPES[q.dtype], scale, bool(causal), first_query)
+               _DTYPES[q.dtype], scale, bool(causal), first_query, work, nbytes)
     return out
 
 
