@@ -869,12 +869,12 @@ __global__ __launch_bounds__(256) void add_weights_kernel(const float* __restric
   float* const to = weights + b * wb + kv * wh;
   if (j0 < L) {
     float w[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8  // (no branch on z: the heads' loads go out together)
     for (int h = 0; h < G; ++h) {
       const float z = lse_ws[first + h];
-      if (!(fabsf(z) < INFINITY)) continue;
       const f32x4 x = *reinterpret_cast<const f32x4*>(scores + (first + h) * n_pad + j0);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] += exp_(x[e] - z);
+      for (int e = 0; e < 4; ++e) w[e] += fabsf(z) < INFINITY ? exp_(x[e] - z) : 0.f;
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -882,9 +882,10 @@ __global__ __launch_bounds__(256) void add_weights_kernel(const float* __restric
   }
   if (append && j0 == 0 && (uint32_t)table[(long long)b * table_stride + L / page] < (uint32_t)P) {
     float w = 0.f;
+#pragma unroll 8
     for (int h = 0; h < G; ++h) {
-      const float z = lse_ws[first + h];
-      if (fabsf(z) < INFINITY) w += exp_(scores[(first + h + 1) * n_pad - kScoreTail] - z);
+      const float z = lse_ws[first + h], x = scores[(first + h + 1) * n_pad - kScoreTail];
+      w += fabsf(z) < INFINITY ? exp_(x - z) : 0.f;
     }
     to[L] = w;
   }
