@@ -908,9 +908,8 @@ constexpr int kWhole = 512;
 static int min_granules(int G) { return (int)lround(sqrt((double)std::min(kHeads, G))); }
 // key_weights of a key-value head of at most kFusedRows rows and kFusedScores scores are added by the workgroup that
 // ends it; more of them, and those of several units, by a kernel of their own, which takes the host another 2.5 us.
-// One kernel against two: 12 heads of 300 rows 9.1 and 9.2 us, 16 heads on 1 of 1000 rows, 4 sequences, 15.1 and
-// 18.8, 32 on 8 heads of 4000 20.4 and 21.2; but 16 heads of 8000 rows 18.0 and 16.6, 4 sequences of 32 on 8 heads of
-// 8000 35.0 and 30.9.
+// One kernel against two: 32 heads on 8, D = 128, 4 sequences of 1000 rows 17.6 and 18.9 us, of 4000 20.4 and 21.2; 16
+// heads on 1 of 1000 15.3 and 15.0; but 16 heads of 8000 rows 18.0 and 16.6, 32 on 8 heads of 8000 35.0 and 30.9.
 constexpr long long kFusedRows = 6144, kFusedScores = 16384;
 constexpr int kMaxCu = 1024;  // for the workspace's size, which does not depend on the device
 

@@ -311,6 +311,10 @@ constexpr int kMaxCu = 1024;    // for the workspace's size, which does not depe
 // The least tiles of a part (16 heads on 1, 727 queries and keys, 3 sequences: 12.3 us, with 2 12.8, with 8 15.0; 512
 // queries of 12 heads 7.6, 6.4, 8.7; 1369 of 16, D = 128, 15.7, 18.5, 16.3).
 constexpr int kMinTiles = 4;
+// The same where every CU has a block of keys already (16 heads of 2300 queries and keys: 20.0 us, not divided 26.1, with 4
+// 26.5; 2 x 12 heads of 1500 15.4, 19.0, 17.7; 13 queries of 32 heads on 4 against 4415 keys, 3 sequences, not
+// divided 13.5, with 4 17.4).
+constexpr int kManyTiles = 8;
 constexpr int kMaxSplits = 64;
 // Workgroups of a CU that a division aims at (32 heads on 4, D = 80, 2081 queries: 36 us, with 2 49, with 8 38; 32 on 8, D
 // = 128, 2 x 1504: 39.7, 38.7 and 45.9).
@@ -324,10 +328,11 @@ struct Split {
 };
 static Split choose_split(long long units, int G, int N_q, int N_k, int causal, int cu) {
   const long long blocks = (N_k + kKeys - 1) / kKeys * units, tiles = (long long)((N_q + kQueries - 1) / kQueries) * G;
-  if (blocks >= 2LL * cu || tiles < 2 * kMinTiles) return {1, 0};
+  const int least = blocks < cu ? kMinTiles : kManyTiles;
+  if (blocks >= 2LL * cu || tiles < 2 * least) return {1, 0};
   // (Under a causal mask about half the tiles are seen.)
   const long long share = blocks * tiles / (causal ? 2 : 1) / ((long long)kSlots * cu);
-  const long long part = std::max<long long>({kMinTiles, share, (tiles + kMaxSplits - 1) / kMaxSplits});
+  const long long part = std::max<long long>({least, share, (tiles + kMaxSplits - 1) / kMaxSplits});
   return {(int)((tiles + part - 1) / part), (int)part};
 }
 static size_t split_bytes(long long blocks, int splits) {
