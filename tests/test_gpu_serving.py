@@ -328,6 +328,36 @@ def test_decode_paged_large_scores(dtype):
     _near(o[0], ro, eo + _half(dtype) * (ro.abs() + eo), "o")
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("L,at", [(3, (0, 1, 2)), (300, (7, 40, 290)), (2500, (2499, 0, 1300))])
+def test_decode_paged_weights_keep_their_bits(dtype, L, at):
+    """Two rows of weight 1 whose values are minus the first and second 16-bit part of a third row's weight p, and that row
+    with the value 1: the output is what two parts leave of p, over 2 + p.  (The other rows weigh e^-256.)  An exponential
+    is off by 2 u of itself, its argument by another, and the sums of six products of at most 1 by 2 u each: 16 u in all."""
+    g = _gen(35)
+    H, D, page = 16, 64, 16
+    c = Paged(g, [L], H, D, page, dtype)
+    (k, v), = c.rows
+    q = torch.zeros(1, H, D, dtype=dtype, device=DEV)
+    q[0, :, 0] = (0.05 + 0.6 * torch.rand(H, generator=g)).to(dtype).to(DEV)
+    q[..., 1] = 1
+    p = torch.exp(-q[0, :, 0].double())
+    hi = p.to(dtype)
+    lo = (p - hi.double()).to(dtype)
+    k.zero_()
+    k[..., 1] = -256
+    k[:, at, 1] = 0
+    k[:, at[2], 0] = -1
+    v[:, at[0]], v[:, at[1]], v[:, at[2]] = -hi[:, None], -lo[:, None], 1
+    for j in range(0, L, page):
+        m, pid = min(page, L - j), int(c.table[0, j // page])
+        c.k[pid, :, :m], c.v[pid, :, :m] = k[:, j:j + m], v[:, j:j + m]
+    o = fa.decode_paged(q, c.k, c.v, c.table, c.seqlens, softmax_scale=1.0)
+    ro = ((p - hi.double() - lo.double()) / (2 + p)).cpu()[:, None].expand(H, D)
+    eo = (16 * U / (2 + p)).cpu()[:, None]
+    _near(o[0], ro, eo + _half(dtype) * (ro.abs() + eo) + 2.0 ** -25, "o")
+
+
 def test_decode_paged_divides_more_than_64_sequences():
     """The division of the work takes lengths 64 at a time."""
     g = _gen(32)

@@ -8,16 +8,19 @@
 // Bound: HBM.  Each K and V row is read once, 4D bytes for 4DG flops.  The 16 columns of a 16x16 matrix tile are the
 // query heads of one key-value head, so that up to 16 of them cost what one does:
 //   scores   S^T[key][head] = K Q^T      v_mfma_f32_16x16x32 (products exact, float32 sums)
-//   output   O^T[dim][head] += V^T P^T   the same, P as two values of the element type
+//   output   O^T[dim][head] += V^T P^T   the same, P as a sum of three bf16 or two fp16
 // A wave takes 32 keys at a time.  The scores leave the first product with lane (g = lane / 16, i = lane % 16)
 // holding keys 4g .. 4g + 3 of each 16 for head i; two such sets are the second product's B operand as they stand
 // (the contraction runs over keys, whose order is free).  Its A operand wants 8 keys' values of one dim in a lane:
 // the lane loads kDV neighbouring dims of each of the 8 rows, and byte permutes put the keys of a dim side by side.
-// So neither P nor V moves between lanes.  P is split as hi + lo, each rounded to the element type, which keeps 16
-// (bf16) or 22 (fp16) of its bits; rounding it once would cost as much as the output's own rounding.  (fp16 ends at
-// 2^-24: its P is carried times 2^13, so that weights are kept to 2^-38 of the largest.)  An infinite V makes NaN of
-// a lo of 0 or below; a wave whose sums hold NaN takes its keys again with hi alone, for those sums.  (With P and V
-// as float32 on v_mfma_f32_16x16x4_f32 a block of 32 keys took 1024 matrix cycles at D = 64 instead of 192.)
+// So neither P nor V moves between lanes.  P is split into parts of the element type, each what rounding left of the
+// ones before: three of bf16 hold all 24 bits of a float32, two of fp16 miss 2^-23 of it at most, twice a float32's
+// rounding.  (fp16 ends at 2^-24: its P goes in times 2^13, so that weights are kept to 2^-38 of the
+// largest.)  An infinite V makes NaN of a part of 0 or below; a wave whose sums hold NaN takes its keys again with the
+// first part alone, for those sums.  (With P and V as float32 on v_mfma_f32_16x16x4_f32 a block of 32 keys took 1024
+// matrix cycles at D = 64 instead of 192 with two parts.  Two of bf16, 16 bits, gave one output in a thousand another
+// rounding than the definition's; the third takes 32 sequences of 25 heads of 1024 rows from 28.7 to 29.3 us, one of 12
+// heads of 400 from 6.45 to 6.65, and caches that are divided nothing.)
 //
 // Division of the work.  A unit is a (sequence, key-value head, 16 query heads).  The lengths are known on the device
 // only, so every workgroup works the division out from them (plan, below): one chunk length C for all units, with
@@ -79,11 +82,11 @@ constexpr int kPolicyCoherent = 16;           // buffer loads from the device's 
 
 template <class T>
 struct Elem;
-// kShift: P is carried times 2^kShift.  kSlack: how far a score may pass its head's offset; e^kSlack 2^kShift is a
-// number of the type.
+// kParts: of the type that a P is split into; kShift: it goes in times 2^kShift.  kSlack: how far a score may pass its
+// head's offset; e^kSlack 2^kShift is a number of the type.
 template <>
 struct Elem<__bf16> {
-  static constexpr int kShift = 0;
+  static constexpr int kParts = 3, kShift = 0;
   static constexpr float kSlack = 8.f;
   typedef __bf16 x2 __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
@@ -93,7 +96,7 @@ struct Elem<__bf16> {
 };
 template <>
 struct Elem<_Float16> {
-  static constexpr int kShift = 13;
+  static constexpr int kParts = 2, kShift = 13;
   static constexpr float kSlack = 2.f;
   typedef _Float16 x2 __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
@@ -102,9 +105,16 @@ struct Elem<_Float16> {
   }
 };
 
-// Two values of the element type in 32 bits; *rest: what rounding left of them.
+// Two values of the element type in 32 bits; *rest: what rounding left of them.  (bf16 by cutting off, which is two
+// operations less in a row and leaves no part below 0.)
 template <class T>
 __device__ __forceinline__ uint32_t pack(float x, float y, float* rx, float* ry) {
+  if constexpr (std::is_same_v<T, __bf16>) {
+    const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+    *rx = x - __uint_as_float(a & 0xFFFF0000u);
+    *ry = y - __uint_as_float(b & 0xFFFF0000u);
+    return __builtin_amdgcn_perm(b, a, 0x07060302u);
+  }
   const typename Elem<T>::x2 z = {(T)x, (T)y};
   *rx = x - (float)z[0];
   *ry = y - (float)z[1];
@@ -122,6 +132,12 @@ __device__ __forceinline__ uint32_t pair_hi(uint32_t x, uint32_t y) {
 // v_exp_f32: results below 2^-126 are 0.
 __device__ __forceinline__ float exp_(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 __device__ __forceinline__ float log_(float x) { return log2f(x) * kLn2; }
+// 1 / x to a rounding for the normal x > 0 whose inverse is normal: v_rcp_f32 is off by one unit, a Newton step takes it
+// away.  (The compiler's division is 10 instructions one after another.)
+__device__ __forceinline__ float inverse(float x) {
+  const float y = __builtin_amdgcn_rcpf(x);
+  return fmaf(fmaf(-x, y, 1.f), y, y);
+}
 
 // Floats of a part.
 __host__ __device__ constexpr long long part_floats(int D) { return (long long)kHeads * (D + 2); }
@@ -466,9 +482,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
 
   float m, l;
   f32x4 acc[kDV];
-  // Hi and lo of P: 1 or 0, kept in a scalar register.  (A branch on what the compiler takes for a value of each lane
+  // All parts of P: 1 or 0, kept in a scalar register.  (A branch on what the compiler takes for a value of each lane
   // only masks lanes, and a matrix instruction runs whatever the mask.)
-  int both = __builtin_amdgcn_readfirstlane(1);
+  int every = __builtin_amdgcn_readfirstlane(1);
   // The wave's sums into LDS.  acc[j], register r of lane (g, i): dim kDV (4g + r) + j of head i.
   auto leave = [&]() {
     if (i < nh) {
@@ -575,18 +591,18 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
         m = mn;
       }
       const float mu = m == -INFINITY ? 0.f : m;
-      u32x4 hi[kTiles / 2], lo[kTiles / 2];
+      constexpr int kParts = Elem<T>::kParts;
+      u32x4 part[kParts][kTiles / 2];
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)
 #pragma unroll
         for (int r = 0; r < 4; r += 2) {
-          float x0 = (s[t][r] - mu) * a.scale_log2, x1 = (s[t][r + 1] - mu) * a.scale_log2;
-          if constexpr (Elem<T>::kShift != 0) x0 += Elem<T>::kShift, x1 += Elem<T>::kShift;
-          const float p0 = __builtin_amdgcn_exp2f(x0), p1 = __builtin_amdgcn_exp2f(x1);
+          float p0 = __builtin_amdgcn_exp2f((s[t][r] - mu) * a.scale_log2);
+          float p1 = __builtin_amdgcn_exp2f((s[t][r + 1] - mu) * a.scale_log2);
           l += p0 + p1;
-          float r0, r1, none;
-          hi[t / 2][2 * (t % 2) + r / 2] = pack<T>(p0, p1, &r0, &r1);
-          lo[t / 2][2 * (t % 2) + r / 2] = pack<T>(r0, r1, &none, &none);
+          p0 *= 1 << Elem<T>::kShift, p1 *= 1 << Elem<T>::kShift;
+#pragma unroll
+          for (int c = 0; c < kParts; ++c) part[c][t / 2][2 * (t % 2) + r / 2] = pack<T>(p0, p1, &p0, &p1);
         }
       if (write && g == 0 && (kFull || kDV * i < D)) {
         char* const to = const_cast<char*>(vh) + (u64)home * (u64)a.vs.p + row_in * (uint32_t)a.vs.n + 2 * kDV * i;
@@ -613,11 +629,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
                             pair_lo(vb[2][e], vb[3][e])};
           const u32x4 v1 = {pair_hi(va[0][e], va[1][e]), pair_hi(va[2][e], va[3][e]), pair_hi(vb[0][e], vb[1][e]),
                             pair_hi(vb[2][e], vb[3][e])};
-          acc[2 * e] = Elem<T>::mfma(v0, hi[t / 2], acc[2 * e]);
-          acc[2 * e + 1] = Elem<T>::mfma(v1, hi[t / 2], acc[2 * e + 1]);
-          if (__builtin_amdgcn_readfirstlane(both)) {
-            acc[2 * e] = Elem<T>::mfma(v0, lo[t / 2], acc[2 * e]);
-            acc[2 * e + 1] = Elem<T>::mfma(v1, lo[t / 2], acc[2 * e + 1]);
+          acc[2 * e] = Elem<T>::mfma(v0, part[0][t / 2], acc[2 * e]);
+          acc[2 * e + 1] = Elem<T>::mfma(v1, part[0][t / 2], acc[2 * e + 1]);
+          if (__builtin_amdgcn_readfirstlane(every)) {
+#pragma unroll
+            for (int c = 1; c < kParts; ++c) {
+              acc[2 * e] = Elem<T>::mfma(v0, part[c][t / 2], acc[2 * e]);
+              acc[2 * e + 1] = Elem<T>::mfma(v1, part[c][t / 2], acc[2 * e + 1]);
+            }
           }
         }
       __builtin_amdgcn_sched_barrier(0);
@@ -648,9 +667,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
     for (int j = 0; j < kDV; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) any = fmaf(acc[j][r], 0.f, any);
-    if (!__builtin_amdgcn_readfirstlane(both) || !__builtin_amdgcn_ballot_w64(any != any)) break;
+    if (!__builtin_amdgcn_readfirstlane(every) || !__builtin_amdgcn_ballot_w64(any != any)) break;
     leave();  // (the sums that are not NaN are kept)
-    both = __builtin_amdgcn_readfirstlane(0);
+    every = __builtin_amdgcn_readfirstlane(0);
     look_up(ids, kb0);
   }
   if (kDivide && S > 1 && wave == 0 && lane == 0 && (aw_start >> tfgfa::kTagShift) != a.tag) {
@@ -708,7 +727,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
 
   // Join the waves.  (Offsets without the scale: differences first, here too.)
   l = over_rows(l, [](float u, float w) { return u + w; });
-  if (!both && i < nh) {
+  if (!every && i < nh) {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -740,14 +759,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
       lt = fmaf(f, sh_l[w][h], lt);
       ot = fmaf(f, sh_o[(w * kHeads + h) * kRow + d], ot);
     }
-    constexpr float kBack = 1.f / (1 << Elem<T>::kShift);
-    lt *= kBack, ot *= kBack;
+    ot *= 1.f / (1 << Elem<T>::kShift);
     if (S > 1) {
       __hip_atomic_store(mine + h * D + d, ot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       if (d < 2)
         __hip_atomic_store(mine + (D + d) * kHeads + h, d == 0 ? M : lt, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     } else {
-      const float on = lt == 0.f ? 0.f : ot * __builtin_amdgcn_rcpf(lt);
+      const float on = lt == 0.f ? 0.f : ot * inverse(lt);
       static_cast<T*>(a.o)[b * a.os.b + (h0 + h) * a.os.h + d] = (T)(valid ? on : nan);
       if (d == 0 && (a.lse || a.lse_ws || kFused)) {
         const float ls = lt == 0.f ? -INFINITY : fmaf(Mu, a.scale, log_(lt));
@@ -811,7 +829,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
     const float Mu = M == -INFINITY ? 0.f : M;
     const float f = lane < S ? exp_((ms - Mu) * a.scale) : 0.f;
     const float W = over_lanes(f * ls, [](float u, float w) { return u + w; });
-    if (lane < S) share[h * S + lane] = W == 0.f ? 0.f : f * __builtin_amdgcn_rcpf(W);
+    if (lane < S) share[h * S + lane] = W == 0.f ? 0.f : f * inverse(W);
     if (lane == 0 && (a.lse || a.lse_ws || kFused)) {
       const float z = W == 0.f ? -INFINITY : fmaf(Mu, a.scale, log_(W));
       if (a.lse) a.lse[(long long)b * a.H + h0 + h] = z;
