@@ -445,6 +445,40 @@ def test_decode_paged_adds_key_weights_of_long_caches(H, H_kv, D, page, dtype, a
         _near(sums[b], want, bound, f"L={n} sums")
 
 
+@pytest.mark.parametrize("H,H_kv,L,page,append,dtype", [
+    (2, 1, 300, 16, True, BF),       # added by the step's own workgroup
+    (4, 2, 5000, 64, True, HF),      # by the one that joins a cache's parts
+    (2, 1, 300, 7, False, BF),       # by a second kernel: a table of rows that are no multiple of 4,
+    (20, 1, 500, 16, True, BF),      # two tiles of query heads,
+    (3, 3, 9000, 64, True, HF),      # a long cache
+])
+def test_decode_paged_key_weights_of_large_scores(H, H_kv, L, page, append, dtype):
+    """Scores near 2^23, exact, whose differences 0 to 12 are exact too: their weights are float32's to (L + 64) u, as the
+    definition's exp(x_j) / sum exp(x_i) has them; scores and log-sum-exp by themselves are rounded to 0.25 here."""
+    g = _gen(36 + L)
+    c = Paged(g, [L], H_kv, 64, page, dtype, spare=1 if append else 0)
+    (k, v), = c.rows
+    k.zero_()
+    k[..., 0] = 256
+    k[..., 1] = torch.randint(0, 13, (H_kv, L), generator=g).to(dtype).to(DEV)
+    for j in range(0, L, page):
+        c.k[int(c.table[0, j // page]), :, :min(page, L - j)] = k[:, j:j + page]
+    q = torch.zeros(1, H, 64, dtype=dtype, device=DEV)
+    q[..., 0], q[..., 1] = 32768, 1
+    kn = vn = None
+    if append:
+        kn, vn = torch.zeros(1, H_kv, 64, dtype=dtype, device=DEV), _randn((1, H_kv, 64), g, dtype)
+        kn[..., 0], kn[..., 1] = 256, 9
+        k = torch.cat([k, kn[0][:, None]], 1)
+    sums = torch.zeros(1, H_kv, c.table.shape[1] * page, device=DEV)
+    scale = 0.375
+    fa.decode_paged(q, c.k, c.v, c.table, c.seqlens, kn, vn, key_weights=sums, softmax_scale=scale)
+    n = k.shape[1]
+    want = H // H_kv * torch.softmax(k[..., 1].double().cpu() * scale, 1)
+    _near(sums[0, :, :n], want, (L + 64) * U * want, "sums")
+    assert (sums[0, :, n:] == 0).all()
+
+
 def test_decode_paged_workspaces():
     """A workspace of any content and size: the division needs the whole of it, key weights refuse less."""
     g = _gen(8)

@@ -27,7 +27,9 @@
 // about `target` workgroups in all; a unit of more than C rows is divided over several workgroups.  Each leaves its
 // part (sums of weighted values and of weights, and their offset) in the workspace, and the one that arrives last
 // joins them (arrival words and memory order as in tfgfa_decode.hip) and, where it is asked for, adds the unit's key
-// weights from the scores that the parts have left.
+// weights from the scores that the parts have left: e^(scale (s - m)) / W, s without the scale, m the offset of the
+// joined sums and W their sum of weights, so that s - m is exact for near scores of any size (with e^(x - lse) of
+// rounded x and lse, weights of scores near 2^23 were off by tens of percent).
 //
 // Measured: 32 sequences of 25 heads, D = 64, lengths to 1024, 120 MB in 24.9 us (a plain read of as many bytes
 // 21.6); 4 sequences of 32 heads on 8, D = 128, to 32768 rows, 385 MB in 78 us (67); one sequence of 12 heads, 400
@@ -139,6 +141,17 @@ __device__ __forceinline__ float inverse(float x) {
   return fmaf(fmaf(-x, y, 1.f), y, y);
 }
 
+// What turns a head's scores into its key weights: their offset, and one over the sum of e^(scale (s - offset)); 0 for
+// a head whose log-sum-exp is not finite, which adds nothing.
+struct alignas(8) Share {
+  float offset, inverse;
+};
+// w and the key weight of score s.
+__device__ __forceinline__ float add_weight(float w, float s, Share head, float scale_log2) {
+  const float p = __builtin_amdgcn_exp2f((s - head.offset) * scale_log2);
+  return head.inverse != 0.f ? fmaf(p, head.inverse, w) : w;
+}
+
 // Floats of a part.
 __host__ __device__ constexpr long long part_floats(int D) { return (long long)kHeads * (D + 2); }
 
@@ -151,8 +164,8 @@ struct Args {
   float* lse;       // natural log, or null
   char* arrive;
   float* part;      // per workgroup of a divided unit: [head][D] sums, then [head] their offsets, [head] of weights
-  float* lse_ws;    // (B, H) LSE for the weights, or null
-  float* scores;    // (B, H, n_pad) scores, the new row's at n_pad - kScoreTail, or null
+  Share* shares;    // (B, H) for the weights, or null
+  float* scores;    // (B, H, n_pad) scores without the scale, the new row's at n_pad - kScoreTail, or null
   u64 tag;
   Pages ks, vs;
   Vecs qs, os, kns, vns;
@@ -320,7 +333,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
   // The waves' outputs; later the shares of a unit's parts and the sums of the groups that join them.
   constexpr int kLds = kWaves * kHeads * kRow, kLdsJoin = kHeads * kMaxParts + 4 * kThreads;
   __shared__ __attribute__((aligned(16))) float sh_o[kLds > kLdsJoin ? kLds : kLdsJoin];
-  __shared__ float sh_m[kWaves][kHeads], sh_l[kWaves][kHeads], sh_lse[kHeads];
+  __shared__ float sh_m[kWaves][kHeads], sh_l[kWaves][kHeads];
+  __shared__ Share sh_share[kHeads];
   __shared__ int sh_last;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, i = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -555,7 +569,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
           const int head = i * (int)a.n_pad;
 #pragma unroll
           for (int t = 0; t < kTiles; ++t) {
-            const f32x4 y = f32x4{s[t][0], s[t][1], s[t][2], s[t][3]} * a.scale;
+            const f32x4 y = {s[t][0], s[t][1], s[t][2], s[t][3]};
             const int at = x.fresh ? (t == 0 && g == 0 ? head + (int)a.n_pad - kScoreTail : -1)
                                    : (t * kTile < x.rows ? head + x.at + t * kTile + 4 * g : -1);
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), sr,
@@ -564,13 +578,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
         } else {
           float* const to = a.scores + ((long long)b * a.H + h0 + i) * a.n_pad;
           if (x.fresh) {
-            if (g == 0) to[a.n_pad - kScoreTail] = s[0][0] * a.scale;
+            if (g == 0) to[a.n_pad - kScoreTail] = s[0][0];
           } else {
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
               if (t * kTile < x.rows)
                 *reinterpret_cast<f32x4*>(to + x.at + t * kTile + 4 * g) =
-                    f32x4{s[t][0], s[t][1], s[t][2], s[t][3]} * a.scale;
+                    f32x4{s[t][0], s[t][1], s[t][2], s[t][3]};
           }
         }
       }
@@ -679,7 +693,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
   }
 
   // key_weights of the unit's heads (no other unit has this key-value head), by the workgroup that ends it and has left
-  // their LSE in LDS.
+  // their shares in LDS.
   auto add_weights = [&]() {
     const __amdgpu_buffer_rsrc_t wr = rows_rsrc(a.weights + b * a.wb + kv * a.wh, INT32_MAX / 2);
     const __amdgpu_buffer_rsrc_t sr = rows_rsrc(a.scores + ((long long)b * a.H + h0) * a.n_pad, INT32_MAX / 2);
@@ -687,10 +701,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
       __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), wr, at < 0 ? (int)kOutOfRange : at * 4, 0, 0);
     };
     if (append && wave == kWaves - 1) {  // the new row's
-      const float z = lane < nh ? sh_lse[lane] : INFINITY;
+      const Share head = lane < nh ? sh_share[lane] : Share{0.f, 0.f};
       const float x = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
           sr, lane < nh ? (lane * (int)a.n_pad + (int)a.n_pad - kScoreTail) * 4 : (int)kOutOfRange, 0, kPolicyCoherent));
-      const float w = over_lanes(fabsf(z) < INFINITY ? exp_(x - z) : 0.f, [](float u, float v) { return u + v; });
+      const float w = over_lanes(add_weight(0.f, x, head, a.scale_log2), [](float u, float v) { return u + v; });
       store(w, lane == 0 && (uint32_t)((uniform_ints)row)[page_of(Lr)] < (uint32_t)a.P ? Lr : -1);
     }
     // Four rows a thread; kItems heads of such blocks of rows in flight at once.
@@ -710,9 +724,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
       }
 #pragma unroll
       for (int u = 0; u < kItems; ++u) {
-        const float z = sh_lse[h];
+        const Share head = sh_share[h];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] += fabsf(z) < INFINITY ? exp_(__uint_as_float(x[u][e]) - z) : 0.f;
+        for (int e = 0; e < 4; ++e) w[e] = add_weight(w[e], __uint_as_float(x[u][e]), head, a.scale_log2);
         if (++h == nh) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -767,11 +781,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
     } else {
       const float on = lt == 0.f ? 0.f : ot * inverse(lt);
       static_cast<T*>(a.o)[b * a.os.b + (h0 + h) * a.os.h + d] = (T)(valid ? on : nan);
-      if (d == 0 && (a.lse || a.lse_ws || kFused)) {
+      if (d == 0 && (a.lse || a.shares || kFused)) {
         const float ls = lt == 0.f ? -INFINITY : fmaf(Mu, a.scale, log_(lt));
+        const Share mine = {Mu, fabsf(ls) < INFINITY ? inverse(lt) : 0.f};
         if (a.lse) a.lse[(long long)b * a.H + h0 + h] = valid ? ls : nan;
-        if (a.lse_ws) a.lse_ws[(long long)b * a.H + h0 + h] = ls;
-        if (kFused) sh_lse[h] = ls;
+        if (a.shares) a.shares[(long long)b * a.H + h0 + h] = mine;
+        if (kFused) sh_share[h] = mine;
       }
     }
   }
@@ -830,11 +845,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
     const float f = lane < S ? exp_((ms - Mu) * a.scale) : 0.f;
     const float W = over_lanes(f * ls, [](float u, float w) { return u + w; });
     if (lane < S) share[h * S + lane] = W == 0.f ? 0.f : f * inverse(W);
-    if (lane == 0 && (a.lse || a.lse_ws || kFused)) {
+    if (lane == 0 && (a.lse || a.shares || kFused)) {
       const float z = W == 0.f ? -INFINITY : fmaf(Mu, a.scale, log_(W));
+      const Share mine = {Mu, fabsf(z) < INFINITY ? inverse(W) : 0.f};
       if (a.lse) a.lse[(long long)b * a.H + h0 + h] = z;
-      if (a.lse_ws) a.lse_ws[(long long)b * a.H + h0 + h] = z;
-      if (kFused) sh_lse[h] = z;
+      if (a.shares) a.shares[(long long)b * a.H + h0 + h] = mine;
+      if (kFused) sh_share[h] = mine;
     }
   }
   __syncthreads();
@@ -873,12 +889,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
 
 // key_weights after the step: four keys a thread, the heads of the key-value head added in order.
 __global__ __launch_bounds__(256) void add_weights_kernel(const float* __restrict__ scores,
-                                                          const float* __restrict__ lse_ws,
+                                                          const Share* __restrict__ shares,
                                                           const int* __restrict__ lens,
                                                           const int* __restrict__ table, long long table_stride,
                                                           float* weights, long long wb, long long wh,
                                                           long long n_pad, int H, int G, int P, int page,
-                                                          int n_max, int append) {
+                                                          int n_max, int append, float scale_log2) {
   const int b = blockIdx.z, kv = blockIdx.y;
   const int L = lens[b];
   if (L < 0 || L > n_max - append) return;
@@ -887,12 +903,12 @@ __global__ __launch_bounds__(256) void add_weights_kernel(const float* __restric
   float* const to = weights + b * wb + kv * wh;
   if (j0 < L) {
     float w[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8  // (no branch on z: the heads' loads go out together)
+#pragma unroll 8  // (no branch on the head: the heads' loads go out together)
     for (int h = 0; h < G; ++h) {
-      const float z = lse_ws[first + h];
+      const Share head = shares[first + h];
       const f32x4 x = *reinterpret_cast<const f32x4*>(scores + (first + h) * n_pad + j0);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] += fabsf(z) < INFINITY ? exp_(x[e] - z) : 0.f;
+      for (int e = 0; e < 4; ++e) w[e] = add_weight(w[e], x[e], head, scale_log2);
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -902,8 +918,7 @@ __global__ __launch_bounds__(256) void add_weights_kernel(const float* __restric
     float w = 0.f;
 #pragma unroll 8
     for (int h = 0; h < G; ++h) {
-      const float z = lse_ws[first + h], x = scores[(first + h + 1) * n_pad - kScoreTail];
-      w += fabsf(z) < INFINITY ? exp_(x - z) : 0.f;
+      w = add_weight(w, scores[(first + h + 1) * n_pad - kScoreTail], shares[first + h], scale_log2);
     }
     to[L] = w;
   }
@@ -933,15 +948,15 @@ constexpr int kMaxCu = 1024;  // for the workspace's size, which does not depend
 
 static long long padded(long long n) { return (n + kGranule - 1) / kGranule * kGranule + kScoreTail; }
 
-// Parts of the workspace for `wgs` workgroups and `units` units: arrival words, parts, LSE, scores.
+// Parts of the workspace for `wgs` workgroups and `units` units: arrival words, parts, shares, scores.
 struct Layout {
-  size_t part, lse_ws, scores, bytes;
+  size_t part, shares, scores, bytes;
 };
 static Layout layout(long long units, long long wgs, long long bh, long long n_max, int D, bool weights) {
   Layout x;
   x.part = tfgfa::arrive_bytes(units);
-  x.lse_ws = x.part + ((size_t)wgs * part_floats(D) * 4 + 255) / 256 * 256;
-  x.scores = x.lse_ws + (weights ? ((size_t)bh * 4 + 255) / 256 * 256 : 0);
+  x.shares = x.part + ((size_t)wgs * part_floats(D) * 4 + 255) / 256 * 256;
+  x.scores = x.shares + (weights ? ((size_t)bh * sizeof(Share) + 255) / 256 * 256 : 0);
   x.bytes = x.scores + (weights ? (size_t)bh * padded(n_max) * 4 : 0);
   return x;
 }
@@ -1097,7 +1112,7 @@ extern "C" int tfserve_decode_paged(
   const bool fused = weights && a.tiles == 1 && n_max % 4 == 0 && n_max <= kFusedRows &&
                      n_max * (H / H_kv) <= kFusedScores;
   if (fused) a.weights = key_weights, a.wb = wb, a.wh = wh;
-  a.lse_ws = weights && !fused ? reinterpret_cast<float*>(ws + lay.lse_ws) : nullptr;
+  a.shares = weights && !fused ? reinterpret_cast<Share*>(ws + lay.shares) : nullptr;
   a.scores = weights ? reinterpret_cast<float*>(ws + lay.scores) : nullptr;
   a.tag = f.target ? tfgfa::next_tag() : 0;
   a.n_pad = padded(n_max);
@@ -1116,8 +1131,8 @@ extern "C" int tfserve_decode_paged(
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && weights && !fused) {
     hipLaunchKernelGGL(add_weights_kernel, dim3((unsigned)((n_max + 1023) / 1024), H_kv, B), dim3(256), 0, stream,
-                       a.scores, a.lse_ws, cache_seqlens, page_table, f.table_stride, key_weights, wb, wh, a.n_pad,
-                       H, a.G, P, page, (int)n_max, append ? 1 : 0);
+                       a.scores, a.shares, cache_seqlens, page_table, f.table_stride, key_weights, wb, wh, a.n_pad,
+                       H, a.G, P, page, (int)n_max, append ? 1 : 0, a.scale_log2);
     e = hipGetLastError();
   }
   return e == hipSuccess ? TFGFA_OK : -(int)e;
