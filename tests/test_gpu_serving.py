@@ -632,6 +632,28 @@ def test_key_weights_divided_queries(B, H, H_kv, Nq, Nk, D, dtype, causal):
         assert torch.equal(held, got) and torch.equal(fa.key_weights(q, k, lse, causal=causal), got)
 
 
+@pytest.mark.parametrize("H,H_kv,Nq,Nk,dtype,causal", [(4, 2, 200, 300, BF, True), (2, 2, 64, 64, HF, False),
+                                                       (16, 1, 700, 700, BF, True)])
+def test_key_weights_of_large_scores(H, H_kv, Nq, Nk, dtype, causal):
+    """Scores near 2^23, which are exact, and a log-sum-exp near 786432 (scale 0.09375) or 838861 (0.1) as float32 holds it:
+    exp(scale s - lse) is a function of those numbers, off by 4 u |scale s - lse| + 16 u of itself, sums by Nq u."""
+    g = _gen(37)
+    for scale in (0.09375, float(np.float32(0.1))):
+        q, k = (torch.zeros(1, h, n, 64, dtype=dtype, device=DEV) for h, n in ((H, Nq), (H_kv, Nk)))
+        q[..., 0], q[..., 1] = 32768, 1
+        k[..., 0] = 256
+        k[..., 1] = torch.randint(0, 13, (1, H_kv, Nk), generator=g).to(dtype).to(DEV)
+        x = scale * (2.0 ** 23 + k[..., 1].double().cpu())
+        lse = (torch.logsumexp(x, -1).repeat_interleave(H // H_kv, 1)[..., None] + torch.rand(1, H, Nq, generator=g)).float()
+        d = x.repeat_interleave(H // H_kv, 1)[:, :, None] - lse.double()[..., None]
+        see = torch.arange(Nk) <= torch.arange(Nq)[:, None] if causal else torch.ones(Nq, Nk, dtype=torch.bool)
+        p = torch.where(see, torch.exp(d), 0.0)
+        fold = lambda t: t.view(1, H_kv, -1, Nk).sum(2)  # noqa: E731
+        want = fold(p)
+        bound = fold(p * (4 * U * d.abs() + 16 * U)) + H // H_kv * Nq * U * want
+        _near(fa.key_weights(q, k, lse.to(DEV), softmax_scale=scale, causal=causal), want, bound, f"scale {scale}")
+
+
 def test_key_weights_of_hidden_and_empty_rows():
     """Keys that no query sees get 0 whatever they hold; a query whose lse is -inf adds nothing; NaN in a query
     reaches only the keys it sees; no queries at all give zeros."""

@@ -2,6 +2,10 @@
 //     c_j = sum_h sum_i [j <= first + i] e^(scale q_hi . k_j - lse_hi)
 // over the query heads h of a key-value head, with the log-sum-exp of the attention that ran before.
 //
+// e^(x - lse) is 2^(c s - z) in one v_fma, c the scale times log2 e and z = lse log2 e, both rounded: off by 2^-24 (|c s| +
+// |z|), as x - lse in float32 is.  Where a tile's |z| pass kCoarse, 64, what their roundings left is added (lse near 786432:
+// sums 7% off without; a factor for it in every tile took 16 heads of 8192 from 101 to 112 us).
+//
 // Bound: VALU issue.  A pair of query and key costs 2D flops on the matrix units (128 cycles a 32x32 tile at D = 64)
 // and a v_fma, a v_exp_f32 and a v_add on the VALU (16 x 15 cycles a tile).
 // Measured: 16 heads of 8192 causal queries and keys, D = 64, 99-102 us, 670-690 TFLOP/s; VALU issue 65% of the
@@ -48,7 +52,9 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLog2e = 1.4426950408889634;
+constexpr float kLog2eHi = (float)kLog2e, kLog2eLo = (float)(kLog2e - kLog2eHi);
+constexpr float kCoarse = 64.f;  // the largest |z| whose rounding is left at that
 constexpr int kMaxD = 128;
 constexpr int kTile = 32;              // keys of a wave, queries of a matrix tile
 constexpr int kWaves = 4;
@@ -77,7 +83,7 @@ struct Args {
   Rows qs, ks;
   long long lb, lh, ob, oh;
   long long first;
-  float scale_log2;
+  float scale_log2, scale_log2_rest;  // c, and what its rounding left
   int Hkv, units, cu, G, Nq, Nk, D, causal;
   // Where the queries of a block of keys are divided: parts, tiles of a part, arrival words and sums of parts.
   int splits, part_tiles;
@@ -167,7 +173,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(const Args a) {
 
   const uint32_t at = tfgfa::lds_addr(&buf[0][0]);
   const int row_bytes = (int)a.qs.n * 2;
-  float z[2], next[2];  // lse of the lane's query of each half of a tile; past the last query 0
+  // lse of the lane's query of each half of a tile, past the last query 0, and in the log2 domain; the next tile's.
+  float lse_i[2], z[2], next[2];
   // The next tile's queries and their lse, and how many there are from it on in this head.
   int t = t0, h = kv * a.G;
   if (kSplit && per > 0) {
@@ -217,7 +224,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(const Args a) {
     const int n = w & 1;
     tfgfa::wait_vmcnt<0>();
     __syncthreads();
-    z[0] = next[0] * kLog2e, z[1] = next[1] * kLog2e;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) lse_i[u] = next[u], z[u] = next[u] * kLog2eHi;
     if (w + 1 < all) load(n ^ 1);
     // Register r: key 8 (r / 4) + 4 half + r % 4 of the wave's, query i.
     auto scores = [&](int u) {
@@ -230,7 +238,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(const Args a) {
         s = mfma<T>(kf[p], *reinterpret_cast<const u32x4*>(row + 16 * ((2 * p + half) ^ turn<kChunks>(u * kTile + i))), s);
       return s;
     };
-    if (t >= from && t < upto && !__builtin_amdgcn_ballot_w64(fmaxf(fabsf(z[0]), fabsf(z[1])) == INFINITY)) {
+    const bool coarse = __builtin_amdgcn_ballot_w64(fmaxf(fabsf(z[0]), fabsf(z[1])) > kCoarse) != 0;
+    if (t >= from && t < upto && !coarse) {
       const f32x16 s[2] = {scores(0), scores(1)};
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -250,10 +259,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weights_kernel(const Args a) {
         if (a.causal) last = (int)max(-1LL, min((long long)last, a.first + q0 + i - j0));
         if (!live) last = -1;
         const float zu = live ? z[u] : 0.f;
+        auto add = [&](auto exponent) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[r], scale, -zu));
-          sum[r] += 8 * (r / 4) + 4 * half + r % 4 <= last ? p : 0.f;
+          for (int r = 0; r < 16; ++r)
+            sum[r] += 8 * (r / 4) + 4 * half + r % 4 <= last ? __builtin_amdgcn_exp2f(exponent(s[r])) : 0.f;
+        };
+        if (coarse) {
+          const float rest = live ? fmaf(lse_i[u], kLog2eLo, fmaf(lse_i[u], kLog2eHi, -z[u])) : 0.f;
+          add([&](float x) { return fmaf(x, scale, -zu) + fmaf(x, a.scale_log2_rest, -rest); });
+        } else {
+          add([&](float x) { return fmaf(x, scale, -zu); });
         }
       }
     }
@@ -383,7 +398,7 @@ extern "C" int tfserve_key_weights(const void* q, const int64_t* q_strides, cons
     return TFGFA_ERR_STRIDE;
   a.q = q, a.k = k, a.lse = lse, a.out = out;
   a.first = first_query;
-  a.scale_log2 = softmax_scale * kLog2e;
+  a.scale_log2 = (float)(softmax_scale * kLog2e), a.scale_log2_rest = (float)(softmax_scale * kLog2e - a.scale_log2);
   a.Hkv = H_kv, a.G = H / H_kv, a.Nq = N_q, a.Nk = N_k, a.D = D, a.causal = causal;
   a.units = B * H_kv;
   const int st = tfgfa_device_info(&a.cu, nullptr, nullptr, 0);
