@@ -4,6 +4,7 @@ call, and every call here fails them or has nothing to do."""
 import ctypes
 import os
 import re
+import weakref
 
 import pytest
 import torch
@@ -345,3 +346,40 @@ def test_penalize_logits_python_refuses(kw, match):
     a.update(kw)
     with pytest.raises(RuntimeError, match=match):
         fa.penalize_logits(a.pop("logits"), a.pop("tokens"), **a)
+
+
+class _OnDevice0(_Dev):
+    def get_device(self):
+        return 0
+
+
+@pytest.mark.parametrize("op", ["decode_paged", "key_weights"])
+def test_workspace_lives_until_the_launch(monkeypatch, op):
+    """Another thread's call on the same stream may replace the kept workspace by a larger one before this call
+    launches: the buffer whose address the launch gets is still held then."""
+    from custom_flash_attn import serving
+
+    kept, first, launched = {}, [], []
+
+    def make(dev, nbytes):
+        buffer = kept["it"] = torch.empty(nbytes, dtype=torch.uint8)
+        first.append(weakref.ref(buffer))
+        return buffer
+
+    def launch(index, fn, *args):
+        kept["it"] = None   # (what the other thread does)
+        launched.append(args)
+        assert first[0]() is not None, "the workspace was let go before the launch"
+        assert args[-2:] == (first[0]().data_ptr(), first[0]().numel())
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(serving, "_current_stream", lambda index: 7)
+    monkeypatch.setattr(serving, "_decode_workspace", make)
+    monkeypatch.setattr(serving, "_launch_on", launch)
+    t = lambda *shape, dtype=torch.bfloat16: torch.zeros(shape, dtype=dtype).as_subclass(_OnDevice0)  # noqa: E731
+    if op == "decode_paged":
+        fa.decode_paged(t(1, 4, 64), t(3, 2, 16, 64), t(3, 2, 16, 64), t(1, 100, dtype=I32), t(1, dtype=I32),
+                        key_weights=t(1, 2, 1600, dtype=torch.float32))
+    else:
+        fa.key_weights(t(1, 16, 700, 64), t(1, 1, 700, 64), t(1, 16, 700, dtype=torch.float32))
+    assert len(launched) == len(first) == 1

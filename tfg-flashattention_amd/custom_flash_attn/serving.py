@@ -63,21 +63,26 @@ def _check_weights(t, name: str, B: int, H_kv: int, rows: int, dev) -> None:
         raise RuntimeError(f"{name} must be on {dev} and dense in its last dimension")
 
 
-def _workspace(index: int, nbytes: int) -> tuple[int, int]:
-    """(pointer, bytes) of the workspace of device ``index``'s current stream, of at least ``nbytes``."""
+def _workspace(given, index: int, nbytes: int):
+    """The caller's workspace, checked, or one of at least ``nbytes`` for device ``index``'s current stream; None where
+    none is needed.  The caller keeps it until after the launch: another thread's call on the stream may replace the
+    kept one by a larger one in between, and its memory would go to the next tensor."""
+    if given is not None:
+        if not given.is_cuda or given.get_device() != index or not given.is_contiguous():
+            raise RuntimeError(f"workspace must be a contiguous tensor on cuda:{index}")
+        return given
     if not nbytes:
-        return 0, 0
+        return None
     dev = torch.device("cuda", index)
     workspace = None if torch.cuda.is_current_stream_capturing() else _WORKSPACES.get((dev, _current_stream(index)))
     if workspace is None or workspace.numel() < nbytes:
         workspace = _decode_workspace(dev, nbytes)
-    return workspace.data_ptr(), workspace.numel()
+    return workspace
 
 
-def _given_workspace(workspace, like) -> tuple[int, int]:
-    if not workspace.is_cuda or workspace.get_device() != like.get_device() or not workspace.is_contiguous():
-        raise RuntimeError(f"workspace must be a contiguous tensor on {like.device}")
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+def _extent(workspace) -> tuple[int, int]:
+    """(pointer, bytes) of a workspace or None."""
+    return (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
 
 
 def _accepts_pages(k_pages, v_pages, index) -> bool:
@@ -179,10 +184,8 @@ def decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, H, D))
     scale = (1.0 / math.sqrt(D)) if softmax_scale is None else float(softmax_scale)
     lse = q.new_empty((B, H), dtype=torch.float32) if return_lse else None
-    if workspace is None:
-        work, nbytes = _workspace(index, _C.decode_paged_workspace(B, H, H_kv, page, M, D, key_weights is not None))
-    else:
-        work, nbytes = _given_workspace(workspace, k_pages)
+    workspace = _workspace(workspace, index, 0 if workspace is not None else
+                           _C.decode_paged_workspace(B, H, H_kv, page, M, D, key_weights is not None))
     _launch_on(index, _C.decode_paged,
                q.data_ptr(), q.stride(), k_pages.data_ptr(), k_pages.stride(), v_pages.data_ptr(), v_pages.stride(),
                page_table.data_ptr(), page_table.stride(0), cache_seqlens.data_ptr(),
@@ -191,7 +194,7 @@ def decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
                out.data_ptr(), out.stride(), 0 if lse is None else lse.data_ptr(),
                0 if key_weights is None else key_weights.data_ptr(),
                _ZERO2 if key_weights is None else key_weights.stride()[:2],
-               B, H, H_kv, P, page, M, D, _DTYPES[q.dtype], scale, work, nbytes)
+               B, H, H_kv, P, page, M, D, _DTYPES[q.dtype], scale, *_extent(workspace))
     return (out, lse) if return_lse else out
 
 
@@ -267,13 +270,11 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, first_qu
         out = lse.new_empty((B, H_kv, N_k))
     scale = (1.0 / math.sqrt(D)) if softmax_scale is None else float(softmax_scale)
     index = q.get_device()
-    if workspace is None:
-        work, nbytes = _workspace(index, _C.key_weights_workspace(B, H, H_kv, N_q, N_k, bool(causal)))
-    else:
-        work, nbytes = _given_workspace(workspace, q)
+    workspace = _workspace(workspace, index, 0 if workspace is not None else
+                           _C.key_weights_workspace(B, H, H_kv, N_q, N_k, bool(causal)))
     _launch_on(index, _C.key_weights, q.data_ptr(), q.stride(), k.data_ptr(), k.stride(),
                lse.data_ptr(), lse.stride()[:2], out.data_ptr(), out.stride()[:2], B, H, H_kv, N_q, N_k, D,
-               _DTYPES[q.dtype], scale, bool(causal), first_query, work, nbytes)
+               _DTYPES[q.dtype], scale, bool(causal), first_query, *_extent(workspace))
     return out
 
 
