@@ -50,7 +50,8 @@ extern "C" {
  * workspace (16-byte aligned, device memory, no initialisation): tfserve_decode_paged_workspace bytes let
  * the step divide the rows of long sequences over several workgroups; fewer (or NULL) is correct but
  * slower, except that key_weights needs the whole of it (TFGFA_ERR_SCRATCH).  Calls sharing a workspace
- * must be ordered on one stream.
+ * must be ordered on one stream, and a call with key_weights, which may be two launches, must not have
+ * another thread's between them.
  */
 int tfserve_decode_paged(const void* q, const int64_t* q_strides,
                          void* k_pages, const int64_t* k_strides,

@@ -897,6 +897,41 @@ def test_serving_operators_on_streams_of_their_own():
         assert all(torch.equal(o, r) for got, r in zip(outs, refs) for o in got)
 
 
+def test_threads_share_a_stream_and_its_workspace():
+    """Steps of two threads on one stream, which shares one workspace between its calls: key weights that a second kernel
+    adds from scores in it are those of the step by itself."""
+    import threading
+
+    g = _gen(22)
+    sets = []
+    for L, H, H_kv, page in ((9000, 3, 3, 64), (1500, 20, 1, 7)):
+        c = Paged(g, [L], H_kv, 64, page, BF)
+        sets.append((_randn((1, H, 64), g, BF), c.k, c.v, c.table, c.seqlens))
+    fresh = lambda s: torch.zeros(1, s[1].shape[1], s[3].shape[1] * s[1].shape[2], device=DEV)  # noqa: E731
+    refs = []
+    for s in sets:
+        w = fresh(s)
+        refs.append((fa.decode_paged(*s, key_weights=w), w))
+    torch.cuda.synchronize()
+    got, stream = [[], []], torch.cuda.current_stream()
+
+    def steps(n):
+        with torch.cuda.stream(stream):
+            for _ in range(100):
+                w = fresh(sets[n])
+                got[n].append((fa.decode_paged(*sets[n], key_weights=w), w))
+
+    threads = [threading.Thread(target=steps, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for n in range(2):
+        assert len(got[n]) == 100
+        assert all(torch.equal(o, refs[n][0]) and torch.equal(w, refs[n][1]) for o, w in got[n]), n
+
+
 def test_empty_calls():
     k = torch.zeros(2, 1, 16, 64, dtype=BF, device=DEV)
     i32 = dict(dtype=torch.int32, device=DEV)

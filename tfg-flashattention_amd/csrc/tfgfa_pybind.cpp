@@ -232,18 +232,16 @@ void decode_paged(std::uintptr_t q, const Strides3& qs, std::uintptr_t k, const 
                   const Strides2& ws, int B, int H, int H_kv, int P, int page, int M, int D,
                   int dtype, float softmax_scale, std::uintptr_t workspace,
                   std::size_t workspace_bytes, std::uintptr_t stream) {
-  int st;
-  {
-    py::gil_scoped_release nogil;
-    st = tfserve_decode_paged(
-        reinterpret_cast<const void*>(q), qs.data(), reinterpret_cast<void*>(k), ks.data(),
-        reinterpret_cast<void*>(v), vs.data(), reinterpret_cast<const int*>(table), table_stride,
-        reinterpret_cast<const int*>(seqlens), reinterpret_cast<const void*>(kn), kns.data(),
-        reinterpret_cast<const void*>(vn), vns.data(), reinterpret_cast<void*>(o), os.data(),
-        reinterpret_cast<float*>(lse), reinterpret_cast<float*>(weights), ws.data(), B, H, H_kv, P,
-        page, M, D, dtype, softmax_scale, reinterpret_cast<void*>(workspace), workspace_bytes,
-        reinterpret_cast<void*>(stream));
-  }
+  // The GIL is kept: a step with key weights may be two launches with scores in the workspace between them, and another
+  // Python thread's call on the same stream, which shares the workspace kept for it, must not come in between.
+  const int st = tfserve_decode_paged(
+      reinterpret_cast<const void*>(q), qs.data(), reinterpret_cast<void*>(k), ks.data(),
+      reinterpret_cast<void*>(v), vs.data(), reinterpret_cast<const int*>(table), table_stride,
+      reinterpret_cast<const int*>(seqlens), reinterpret_cast<const void*>(kn), kns.data(),
+      reinterpret_cast<const void*>(vn), vns.data(), reinterpret_cast<void*>(o), os.data(),
+      reinterpret_cast<float*>(lse), reinterpret_cast<float*>(weights), ws.data(), B, H, H_kv, P,
+      page, M, D, dtype, softmax_scale, reinterpret_cast<void*>(workspace), workspace_bytes,
+      reinterpret_cast<void*>(stream));
   check(st, "tfserve_decode_paged");
 }
 
