@@ -95,6 +95,26 @@ def test_decode_paged_refuses(lib, kw, code):
     assert _paged(lib, **kw) == _code(code)
 
 
+# (A call that its strides pass is refused for its misaligned lengths.)
+@pytest.mark.parametrize("strides,apart", [
+    ((4096, 1024, 64, 1), True),                   # dense
+    ((4096, 64, 256, 1), True),                    # a row's heads together
+    ((1024, 10240, 64, 1), True),                  # a head's pages together
+    ((8192, 2048, 128, 1), True),                  # K and V rows in turn
+    ((0, 1024, 64, 1), False),                     # one page for all
+    ((4096, 0, 64, 1), False),                     # one head for all
+    ((4032, 1024, 64, 1), False),                  # the last row of a page is the next one's first
+    ((1024, 4096, 64, 1), False),                  # ten pages, four of which reach the next head
+])
+def test_written_pools_hold_rows_apart(lib, strides, apart):
+    code = _code("ERR_ALIGNMENT" if apart else "ERR_STRIDE")
+    for name in ("ks", "vs"):
+        assert _paged(lib, kn=P, vn=P, lens=P + 2, **{name: strides}) == code
+        assert _paged(lib, lens=P + 2, **{name: strides}) == _code("ERR_ALIGNMENT")   # read only
+        assert _evict(lib, lens=P + 2, pages=10, out=2 * P, **{name: strides}) == code
+    assert _paged(lib, kn=P, vn=P, lens=P + 2, pages=1, ks=(0, 1024, 64, 1)) == _code("ERR_ALIGNMENT")
+
+
 def test_key_weights_workspace(lib):
     size = lib.tfserve_key_weights_workspace
     size.restype = ctypes.c_size_t

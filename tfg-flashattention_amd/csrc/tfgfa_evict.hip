@@ -33,6 +33,7 @@ namespace tfgfa_evict {
 
 using tfgfa::apart;
 using tfgfa::Pages;
+using tfgfa::pages_apart;
 using tfgfa::pages_ok;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -409,7 +410,8 @@ extern "C" int tfserve_evict(void* k_pages, const int64_t* k_strides, void* v_pa
   if (!k_strides || !v_strides || !weights_strides || !weights_out_strides) return TFGFA_ERR_NULL_POINTER;
   if (B > 1 && (table_stride < 0 || new_table_stride < M_new)) return TFGFA_ERR_STRIDE;
   Args a = {};
-  if (!pages_ok(k_strides, P, H_kv, page, D, &a.ks) || !pages_ok(v_strides, P, H_kv, page, D, &a.vs))
+  if (!pages_ok(k_strides, P, H_kv, page, D, &a.ks) || !pages_ok(v_strides, P, H_kv, page, D, &a.vs) ||
+      !pages_apart(a.ks, P, H_kv, page, D) || !pages_apart(a.vs, P, H_kv, page, D))
     return TFGFA_ERR_STRIDE;
   a.wb = B > 1 ? weights_strides[0] : 0, a.wh = H_kv > 1 ? weights_strides[1] : 0;
   a.ob = B > 1 ? weights_out_strides[0] : 0, a.oh = H_kv > 1 ? weights_out_strides[1] : 0;

@@ -1662,7 +1662,7 @@ extern "C" const char* tfgfa_strerror(int status) {
       return "workspace too small for the scores that key weights are taken from";
     case TFGFA_ERR_STRIDE:
       return "unsupported strides (last dim 1; b, h, n non-negative multiples of 8; n >= head dim; "
-             "o without overlapping elements)";
+             "what is written without overlapping elements)";
     default: break;
   }
   if (status < 0) return hipGetErrorString((hipError_t)(-status));

@@ -4,6 +4,7 @@
 
 #include <stdint.h>
 
+#include <algorithm>
 #include <utility>
 
 namespace tfgfa {
@@ -52,6 +53,20 @@ inline bool apart(long long sa, long long na, long long sb, long long nb, long l
     reach += (na - 1) * sa;
   }
   return nb <= 1 || sb > reach;
+}
+
+// The rows of a pool (one that is written to) share none: of its strides from the smallest on, each is past the span of
+// those before it.
+inline bool pages_apart(const Pages& st, int P, int H_kv, int page, int D) {
+  std::pair<long long, long long> dims[3] = {{st.p, P}, {st.h, H_kv}, {st.n, page}};
+  std::sort(dims, dims + 3);
+  __int128 reach = 2 * D - 1;
+  for (const auto& d : dims) {
+    if (d.second <= 1) continue;
+    if (d.first <= reach) return false;
+    reach += (__int128)(d.second - 1) * d.first;
+  }
+  return true;
 }
 
 // j / page = j * m >> s for 0 <= j < 2^31: with 2^(l-1) < page <= 2^l and m = floor(2^(31+l) / page) + 1 the error j (m

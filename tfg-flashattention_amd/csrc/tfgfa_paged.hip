@@ -55,6 +55,7 @@ namespace tfgfa_paged {
 
 using tfgfa::apart;
 using tfgfa::Pages;
+using tfgfa::pages_apart;
 using tfgfa::pages_ok;
 using tfgfa::Vecs;
 using tfgfa::vecs_ok;
@@ -1073,6 +1074,7 @@ extern "C" int tfserve_decode_paged(
   if (append && (!vecs_ok(k_new_strides, B, H_kv, &a.kns) || !vecs_ok(v_new_strides, B, H_kv, &a.vns)))
     return TFGFA_ERR_STRIDE;
   if (!apart(a.os.b, B, a.os.h, H, D)) return TFGFA_ERR_STRIDE;
+  if (append && (!pages_apart(a.ks, P, H_kv, page, D) || !pages_apart(a.vs, P, H_kv, page, D))) return TFGFA_ERR_STRIDE;
   if (B > 1 && table_stride < 0) return TFGFA_ERR_STRIDE;
   if (!q || !k_pages || !v_pages || !o || !cache_seqlens || (!page_table && M > 0)) return TFGFA_ERR_NULL_POINTER;
   if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)o | (uintptr_t)k_new |
