@@ -765,6 +765,24 @@ def test_evict_marks_bad_lengths_and_pages():
     assert torch.equal(c.k.view(torch.int16), k0.view(torch.int16))
 
 
+def test_evict_checks_pages_of_more_than_2_to_30_rows():
+    """L + page passes 2^31: the page ids are checked all the same, and a good one's last rows are found."""
+    page, L = 1200 * 10 ** 6, 1100 * 10 ** 6
+    k = torch.empty(2, 1, page, 8, dtype=BF, device=DEV)
+    w = torch.empty(1, 1, page, device=DEV)
+    k[0, 0, L - 4:L] = _randn((4, 8), _gen(16), BF)
+    w[0, 0, L - 4:L] = torch.arange(4, device=DEV).float()
+    new = torch.ones(1, 1, dtype=torch.int32, device=DEV)
+    lens = torch.tensor([L], dtype=torch.int32, device=DEV)
+    for pid in (2, -1):
+        k[1, 0, :4] = 7
+        kept, ws = fa.evict(k, k, new * pid, lens, w, new, 4, recent=4)
+        assert (kept == -1).all() and torch.isnan(ws).all() and (k[1, 0, :4] == 7).all(), pid
+    kept, ws = fa.evict(k, k, new * 0, lens, w, new, 4, recent=4)
+    assert kept[0, 0].tolist() == list(range(L - 4, L)) and ws[0, 0].tolist() == [0, 1, 2, 3]
+    assert torch.equal(k[1, 0, :4], k[0, 0, L - 4:L])
+
+
 def _penalize_ref(x, tokens, lengths, rep, pres, freq, bias, allowed):
     B, V = x.shape
     x = x.double().cpu().numpy().copy()

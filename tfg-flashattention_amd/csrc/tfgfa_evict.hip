@@ -95,6 +95,9 @@ __device__ __forceinline__ int page_of(const Args& a, int j) {
   return (int)(((unsigned long long)(uint32_t)j * a.by_page.m) >> a.by_page.s);
 }
 
+// Pages of the first n rows (n + page may pass 2^31).
+__device__ __forceinline__ int pages_of(const Args& a, int n) { return n > 0 ? page_of(a, n - 1) + 1 : 0; }
+
 // Rows i0, i0 + step, .. of the kept ones, 16-byte piece c of K and V, kUnroll at a time.  list(i): the row, or -1.
 template <int kUnroll, class List>
 __device__ __forceinline__ void copy_rows(const Args& a, int b, int kv, int i0, int step, int c, int n, List list) {
@@ -159,9 +162,9 @@ __global__ __launch_bounds__(64 * kW) void select_kernel(const Args a) {
     for (int r = 0; r < kR; ++r)
       x[r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(from, (first + lane) * 4 + r * 256, 0, 0));
   }
-  for (int c = tid; c < (L + a.page - 1) / a.page; c += kThreads)
+  for (int c = tid; c < pages_of(a, L); c += kThreads)
     bad |= (uint32_t)a.table[b * a.table_stride + c] >= (uint32_t)a.P;
-  for (int c = tid; c < (n + a.page - 1) / a.page; c += kThreads)
+  for (int c = tid; c < pages_of(a, n); c += kThreads)
     bad |= (uint32_t)a.new_table[b * a.new_stride + c] >= (uint32_t)a.P;
   if (tid == 0) sh_bad = sh_count = 0;
   __syncthreads();
