@@ -138,6 +138,19 @@ def test_decode_paged_workspace(lib):
     assert _C.decode_paged_workspace(1, 12, 12, 16, 128, 64, True) == b
 
 
+def test_workspaces_of_sizes_that_are_refused(lib):
+    """Sizes that a call refuses as too large ask for no workspace (nothing is allocated before the refusal)."""
+    f, g = lib.tfserve_decode_paged_workspace, lib.tfserve_key_weights_workspace
+    f.restype = g.restype = ctypes.c_size_t
+    top = 2 ** 31 - 1
+    for B, H, H_kv, page, M in ((1, 4, 4, 1, top), (1, 4, 4, 2 ** 20, 2 ** 12), (70000, 4, 4, 16, 8), (top, top, 1, 16, 8)):
+        assert f(B, H, H_kv, page, M, 64, 1) == 0
+        assert _paged(lib, B=B, H=H, Hkv=H_kv, page=page, M=M) == _code("ERR_TOO_LARGE")
+    for H, N_q, N_k in ((16, top, 100), (16, top - 63, 100), (2 ** 20, 2 ** 30, 100), (16, 700, top)):
+        assert g(1, H, 1, N_q, N_k, 0) == 0
+        assert _weights(lib, B=1, H=H, Hkv=1, Nq=N_q, Nk=N_k) == _code("ERR_TOO_LARGE")
+
+
 def _weights(lib, **kw):
     a = dict(q=P, qs=(6400, 64, 640, 1), k=P, ks=(6400, 64, 640, 1), lse=P, ls=(1000, 10), out=P, os=(1000, 20), B=2,
              H=10, Hkv=10, Nq=10, Nk=20, D=64, dtype=0, scale=0.125, causal=1, first=0, work=0, bytes=0)

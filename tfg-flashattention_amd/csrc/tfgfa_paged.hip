@@ -988,6 +988,13 @@ static bool sizes_ok(int B, int H, int Hkv, int page, int M, int D) {
   return true;
 }
 
+// Granules of the whole batch and workgroups are counted in 32 bits; so are key indexes, with room for the blocks that a
+// loop looks ahead.
+static bool too_large(long long units, int B, int H, long long n_max) {
+  return n_max > INT32_MAX - 128 * kMaxParts * kGranule || B > 65535 || units >= 1 << 20 || (long long)B * H > INT32_MAX ||
+         units * B > INT32_MAX;
+}
+
 template <class T, int kDV, bool kFull>
 static void launch_full(const First& f, const Args& a, unsigned wgs, hipStream_t stream) {
   const dim3 grid = f.target ? dim3(wgs) : dim3(f.units, f.B);
@@ -1030,6 +1037,7 @@ extern "C" size_t tfserve_decode_paged_workspace(int B, int H, int H_kv, int pag
   if (B == 0 || H == 0 || M == 0) return 0;
   const long long n_max = (long long)M * page, tiles = (H / H_kv + kHeads - 1) / kHeads;
   const long long units = H_kv * tiles;
+  if (too_large(units, B, H, n_max)) return 0;
   long long wgs = 0;  // the most that any device of up to kMaxCu CUs starts
   const int target = choose_target(units, B, n_max, kMaxCu);
   if (target) wgs = workgroups(units, B, n_max, target);
@@ -1058,11 +1066,7 @@ extern "C" int tfserve_decode_paged(
   First f = {};
   a.tiles = (H / H_kv + kHeads - 1) / kHeads;
   const long long units = (long long)H_kv * a.tiles;
-  // Granules of the whole batch and workgroups are counted in 32 bits; so are key indexes, with room for the blocks
-  // that a loop looks ahead.
-  if (n_max > INT32_MAX - 128 * kMaxParts * kGranule || B > 65535 || units >= 1 << 20 || (long long)B * H > INT32_MAX ||
-      units * B > INT32_MAX)
-    return TFGFA_ERR_TOO_LARGE;
+  if (too_large(units, B, H, n_max)) return TFGFA_ERR_TOO_LARGE;
   if (!q_strides || !k_strides || !v_strides || !o_strides) return TFGFA_ERR_NULL_POINTER;
   if (append && (!k_new_strides || !v_new_strides)) return TFGFA_ERR_NULL_POINTER;
   if (!vecs_ok(q_strides, B, H, &a.qs) || !vecs_ok(o_strides, B, H, &a.os) ||

@@ -350,6 +350,11 @@ static Split choose_split(long long units, int G, int N_q, int N_k, int causal, 
   const long long part = std::max<long long>({least, share, (tiles + kMaxSplits - 1) / kMaxSplits});
   return {(int)((tiles + part - 1) / part), (int)part};
 }
+// Blocks of keys, and tiles of queries of a key-value head, are counted in 32 bits.
+static bool too_large(long long units, int G, int N_q, int N_k) {
+  return units > INT32_MAX / 4096 || N_k > INT32_MAX - kKeys || (N_k / kKeys + 1) * units > INT32_MAX ||
+         N_q > INT32_MAX - kQueries || (long long)(N_q / kQueries + 1) * G > INT32_MAX;
+}
 static size_t split_bytes(long long blocks, int splits) {
   return splits > 1 ? tfgfa::arrive_bytes(blocks) + (size_t)blocks * splits * kKeys * 4 : 0;
 }
@@ -360,7 +365,7 @@ extern "C" size_t tfserve_key_weights_workspace(int B, int H, int H_kv, int N_q,
   using namespace tfgfa_weights;
   if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || N_q <= 0 || N_k <= 0) return 0;
   const long long units = (long long)B * H_kv;
-  if (units > INT32_MAX / 4096 || (N_k / kKeys + 1) * units > INT32_MAX) return 0;
+  if (too_large(units, H / H_kv, N_q, N_k)) return 0;
   // (A device of fewer CUs divides less.)
   const Split s = choose_split(units, H / H_kv, N_q, N_k, causal, kMaxCu);
   return split_bytes((long long)((N_k + kKeys - 1) / kKeys) * units, s.splits);
@@ -380,9 +385,7 @@ extern "C" int tfserve_key_weights(const void* q, const int64_t* q_strides, cons
   if (causal != 0 && causal != 1) return TFGFA_ERR_CAUSAL_FLAG;
   if (B == 0 || H == 0 || N_k == 0) return TFGFA_OK;
   const long long units = (long long)B * H_kv;
-  if (units > INT32_MAX / 4096 || N_k > INT32_MAX - kKeys || (N_k / kKeys + 1) * units > INT32_MAX || N_q > INT32_MAX - kQueries ||
-      first_query > INT64_MAX / 2 || (long long)(N_q / kQueries + 1) * (H / H_kv) > INT32_MAX)
-    return TFGFA_ERR_TOO_LARGE;
+  if (too_large(units, H / H_kv, N_q, N_k) || first_query > INT64_MAX / 2) return TFGFA_ERR_TOO_LARGE;
   if (!q_strides || !k_strides || !lse_strides || !out_strides) return TFGFA_ERR_NULL_POINTER;
   Args a = {};
   if (!rows_ok(q_strides, B, H, N_q, D, &a.qs) || !rows_ok(k_strides, B, H_kv, N_k, D, &a.ks))
