@@ -93,3 +93,13 @@ def test_generate_applies_penalties_on_the_cpu():
     out = mi.generate(model, idx, 20, 256, temperature=0.0, penalties=mi.LogitPenalties(presence=1e4))
     for row in out.tolist():
         assert len(set(row[5:])) == 20 and not set(row[5:]) & set(row[:5])
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_logit_penalties_on_the_cpu_take_what_the_device_takes(dtype):
+    """int32 texts, and ids outside the vocabulary, which count for nothing."""
+    x = torch.tensor([[2.0, -1.0, 3.0, 0.5]])
+    idx = torch.tensor([[2, -1, 2, 4, 1, 100]], dtype=dtype)
+    got = mi.LogitPenalties(repetition=2.0, presence=0.25, frequency=0.5)(x, idx)
+    assert got.tolist() == [[2.0, -1.0 * 2 - 0.5 - 0.25, 3.0 / 2 - 2 * 0.5 - 0.25, 0.5]]
+    assert mi.LogitPenalties(presence=1.0)(x, idx[:, :0]).tolist() == x.tolist()

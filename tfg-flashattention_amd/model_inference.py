@@ -730,7 +730,8 @@ class LogitPenalties:
                                                      frequency=self.frequency, bias=self.bias, allowed=allowed)
         column = lambda p: p[:, None] if isinstance(p, torch.Tensor) else p  # noqa: E731
         x = logits.float()
-        n = torch.zeros_like(x).scatter_add_(1, idx, torch.ones_like(idx, dtype=x.dtype))
+        inside = (idx >= 0) & (idx < x.shape[1])
+        n = torch.zeros_like(x).scatter_add_(1, torch.where(inside, idx, 0).long(), inside.to(x.dtype))
         r = column(self.repetition)
         x = torch.where(n > 0, torch.where(x > 0, x / r, x * r) - column(self.frequency) * n - column(self.presence), x)
         if self.bias is not None:
