@@ -103,3 +103,22 @@ def test_logit_penalties_on_the_cpu_take_what_the_device_takes(dtype):
     got = mi.LogitPenalties(repetition=2.0, presence=0.25, frequency=0.5)(x, idx)
     assert got.tolist() == [[2.0, -1.0 * 2 - 0.5 - 0.25, 3.0 / 2 - 2 * 0.5 - 0.25, 0.5]]
     assert mi.LogitPenalties(presence=1.0)(x, idx[:, :0]).tolist() == x.tolist()
+
+
+def test_a_token_past_the_table_is_refused(monkeypatch):
+    """A cut leaves a table for budget + slack rows; a loop that does not cut again is told so (the step itself would
+    give NaN)."""
+    steps = []
+    monkeypatch.setattr(custom_flash_attn, "evict", lambda *a, **kw: None)
+    monkeypatch.setattr(custom_flash_attn, "decode_paged", lambda *a, **kw: steps.append(a))
+    c = mi.PagedKVCache(CFG, 2, 50, "cpu", page_size=8, budget=10, slack=5)
+    c.advance(20)
+    c.evict()
+    for _ in range(6):   # two pages
+        c.attend(0, None, None, None)
+        c.advance(1)
+    with pytest.raises(ValueError, match="16 rows"):
+        c.attend(0, None, None, None)
+    c.evict()
+    c.attend(0, None, None, None)
+    assert len(steps) == 7

@@ -370,6 +370,10 @@ class PagedKVCache:
         """One decode step of (B, H, d) projections: the new row appended, the attention over all rows."""
         import custom_flash_attn
 
+        rows = self.table.shape[1] * self.page_size
+        if self.length >= rows:
+            raise ValueError(f"the cache's tables hold {rows} rows and have no place for another token"
+                             + ("" if self.budget is None else ": evict() first"))
         return custom_flash_attn.decode_paged(q, self.k[layer], self.v[layer], self.table, self.seqlens, k, v, out=out,
                                               key_weights=None if self.weights is None else self.weights[layer],
                                               workspace=self.workspace)
