@@ -378,6 +378,25 @@ def test_decode_paged_divides_more_than_64_sequences():
             assert ((got.double().cpu() - want).abs() <= bound).all(), (b, lens[b])
 
 
+def test_decode_paged_many_units_and_one_long_sequence():
+    """More units than four a CU, one sequence of 20000 rows among short ones, whose weights are summed too."""
+    g = _gen(34)
+    B, H, D, page = 130, 8, 64, 64
+    lens = torch.randint(0, 60, (B,), generator=g).tolist()
+    lens[77] = 20000
+    c = Paged(g, lens, H, D, page, BF, spare=1)
+    q, kn, vn = (_randn((B, H, D), g, BF) for _ in range(3))
+    sums = torch.zeros(B, H, c.table.shape[1] * page, device=DEV)
+    o, lse = fa.decode_paged(q, c.k, c.v, c.table, c.seqlens, kn, vn, return_lse=True, key_weights=sums)
+    torch.cuda.synchronize()
+    for b in (0, 1, 76, 77, 78, 129):
+        k, v = (torch.cat([t, n[b][:, None]], 1) for t, n in zip(c.rows[b], (kn, vn)))
+        ro, rl, w, eo, el, ew = attend(q[b], k, v, D ** -0.5)
+        _near(o[b], ro, eo + _half(BF) * (ro.abs() + eo), f"o of {lens[b]}")
+        _near(lse[b], rl, el, "lse")
+        _near(sums[b, :, :lens[b] + 1], w, ew + 2 * U * w, "sums")
+
+
 @pytest.mark.parametrize("H,H_kv,D,page,dtype,append", [
     (12, 12, 64, 16, BF, True), (8, 2, 128, 64, HF, True), (20, 1, 64, 10, BF, False), (4, 4, 40, 32, BF, True)])
 def test_decode_paged_adds_key_weights(H, H_kv, D, page, dtype, append):

@@ -966,8 +966,11 @@ static Layout layout(long long units, long long wgs, long long bh, long long n_m
 // unit.  No division (target 0) where there are units enough, or where sequences are short.
 static int choose_target(long long units, int B, long long n_max, int cu_count) {
   const long long per = units * B;
-  // (64 sequences of 8 heads of 4096 rows, 512 units: 65.7 us divided, 67.7 not.  Past 2^21 granules the plan's
-  // quotients are not exact.)
+  // Sequences of like lengths take 1 to 2% longer divided from 4 units a CU on (128 of 8 heads of 4096 rows 188 us, divided
+  // 189; 256 of 2048 180.4 and 183; 64 of 25 heads of 188 to 1500 64.6 and 66; below, 64 of 8 heads of 4096: 67.7 and
+  // 65.7).  The lengths are not known here, and a very long one among that many pays for it: 128 sequences of 8 heads, D =
+  // 128, one of 32768 rows and the others of 512, take 380 us, divided 75.  (Past 2^21 granules the plan's quotients are
+  // not exact.)
   if (n_max <= (B == 1 ? kWhole : 2 * kWhole) || per >= (long long)kSlots * 2 * cu_count ||
       (n_max / kGranule + 1) * B >= 1 << 20)
     return 0;
