@@ -46,6 +46,8 @@ extern "C" {
  * gives NaN in O and LSE for that batch row, which is otherwise left alone; a page id outside [0, P)
  * among a sequence's rows gives NaN in O and LSE too, and nothing is written through it.
  * Values of rows at or past the length never reach the result.
+ * Sums of weighted values are float32 before the sum of weights, up to e^8 L, divides them: bf16 values past
+ * 3.4e38 / (2981 L_b) can make them infinite.
  *
  * workspace (16-byte aligned, device memory, no initialisation): tfserve_decode_paged_workspace bytes let
  * the step divide the rows of long sequences over several workgroups; fewer (or NULL) is correct but

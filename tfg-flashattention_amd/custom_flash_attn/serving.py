@@ -163,7 +163,9 @@ def decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     ``page_table[b, j // page]``.  ``cache_seqlens``: int32 (B,), the cached rows; entries of the table
     past them are not used.  With ``k_new``/``v_new`` ((B, H_kv, D)) the new token becomes row
     ``cache_seqlens[b]`` first (its page must be the sequence's own) and is attended too; the caller
-    advances ``cache_seqlens`` afterwards.  Pages may otherwise be shared by sequences.
+    advances ``cache_seqlens`` afterwards.  Pages may otherwise be shared by sequences.  Pools that are appended to
+    hold each row in a place of its own (no expanded views).  bf16 values past 3.4e38 / (2981 rows) can make float32's
+    sums infinite.
 
     ``key_weights``: float32 (B, H_kv, N >= M * page), the attention weight each row has received: this
     step's softmax weights, summed over the query heads of each key-value head, are added in place (for
@@ -305,7 +307,8 @@ def evict(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor
     ``key_weights`` (float32 (B, H_kv, N >= M * page)), ties to the lowest row; NaN ranks below every
     number.  The ``n = min(cache_seqlens[b], budget)`` rows kept are copied, in their order, to rows
     0 .. n - 1 of the pages that ``new_page_table`` (int32 (B, M_new), ``M_new * page >= budget``) names;
-    entries past row n are not read.  Those pages must be ones that no row still reads.  The old pages
+    entries past row n are not read.  Those pages must be ones that no row still reads, in pools that hold each row in a
+    place of its own.  The old pages
     are left as they were, so that other sequences may go on sharing them.  Afterwards the caller takes
     ``new_page_table`` for the sequences' and bounds ``cache_seqlens`` by ``budget``.
 

@@ -309,7 +309,9 @@ class PagedKVCache:
     ``weights[layer]`` (float32 (B, H, rows)), and :meth:`evict` keeps, in each layer and head, the last
     ``recent`` rows (default half the budget) and those of the largest sums, ``budget`` in all;
     :meth:`over` says when ``slack`` more rows than that are held.  Rows carry their positions in their
-    keys, so the others stay what they are.  Pages are handed out and taken back on the host.
+    keys, so the others stay what they are.  Pages are handed out and taken back on the host, and a cut's table is copied
+    from there, which waits for the copy.  A budget bounds the rows that a step reads, not the pools: they hold the
+    longest text's pages and a cut's beside them, for every sequence.
     """
 
     def __init__(self, cfg: dict, batch: int, max_len: int, device, dtype=torch.bfloat16, page_size: int = 64,
@@ -719,7 +721,9 @@ class LogitPenalties:
     penalize_logits): tokens that the text holds already have their logit divided (positive) or multiplied by
     ``repetition`` and lowered by ``presence`` and, for each time, ``frequency`` (numbers, or one float32 per row);
     ``bias`` ((V,) or (B, V) float32) is added; tokens whose bit is not set in ``allowed`` (int32 words, (ceil(V / 32),)
-    or one row per text, or a function of the text that returns them, as a grammar needs it) are ruled out."""
+    or one row per text, or a function of the text that returns them, as a grammar needs it) are ruled out.
+    The three penalties count one history, the prompt included; a loop that counts generated text alone for the last two
+    gives it to custom_flash_attn.penalize_logits in a call of its own."""
 
     def __init__(self, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None):
         self.repetition, self.presence, self.frequency = repetition, presence, frequency
