@@ -105,7 +105,7 @@ size_t tfserve_key_weights_workspace(int B, int H, int H_kv, int N_q, int N_k, i
  *   weights_out[b,h',i] = its key_weights, 0 from n on          float32, strides [b, h], i < budget
  * Pools whose strides put rows over one another are refused.
  * Table entries past a sequence's last row, old and new, are not read.  The pages of new_page_table must
- * be none that any row still reads (the caller afterwards takes it for its page_table and bounds
+ * be none that any row still reads, and each named once (the caller afterwards takes it for its page_table and bounds
  * cache_seqlens by budget); the old pages are left as they were.  weights_out may be key_weights
  * itself (same strides).
  * A row whose length does not fit (L < 0 or > M * page), or with a page id outside [0, P) among the

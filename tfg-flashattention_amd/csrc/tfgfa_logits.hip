@@ -4,8 +4,8 @@
 // words it asks for first; while they come it counts the row's history into LDS (its own tokens only; integer adds,
 // so their order is no matter), which every workgroup of the row reads from L2.  Rows of odd lengths begin at any
 // element: a lane takes four neighbouring logits as one load of the elements' own alignment.
-// Measured: 128 rows of 50257 float32 logits with biases, masks and 1024 tokens each, 53.5 MB in 11.7 us (4.6 TB/s);
-// one row 3.5 us.
+// Measured: 128 rows of 50257 float32 logits with biases, masks and 1024 tokens each, 53.5 MB in 12.8 us (4.2 TB/s;
+// 11.7 where the Infinity Cache holds them); one row 3.0 us.
 #include <hip/hip_runtime.h>
 
 #include <math.h>

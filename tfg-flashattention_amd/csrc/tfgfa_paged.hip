@@ -31,12 +31,12 @@
 // joined sums and W their sum of weights, so that s - m is exact for near scores of any size (with e^(x - lse) of
 // rounded x and lse, weights of scores near 2^23 were off by tens of percent).
 //
-// Measured: 32 sequences of 25 heads, D = 64, lengths to 1024, 120 MB in 24.9 us (a plain read of as many bytes
-// 21.6); 4 sequences of 32 heads on 8, D = 128, to 32768 rows, 385 MB in 78 us (67); one sequence of 12 heads, 400
-// rows, 6.4 us (the chain length - pages - K - V - output; 1.6 us are the launch); 4 sequences of 16 heads to 4096
-// rows with key weights, 50 MB, 21 us, 4 of them the weights (10).  Matrix units busy 5%, VALU issue
-// 19%, 80% of the wave cycles in waits at the first: loads under way bound it, and their number is what the registers
-// hold (a second set of them 192 to 256 VGPRs, slower; 4 waves a SIMD spill; blocks of 64 keys, 8 or 16 waves a
+// Measured, inputs that no cache holds: 32 sequences of 25 heads, D = 64, lengths to 1024, 120 MB in 28.6 us (24.5 from
+// the Infinity Cache; a plain read of as many bytes 21.6); 4 sequences of 32 heads on 8, D = 128, to 32768 rows, 385 MB
+// in 80 us (67); one sequence of 12 heads, 400 rows, 6.5 us (the chain length - pages - K - V - output; 1.6 us are the
+// launch); 4 sequences of 16 heads to 4096 rows with key weights, 50 MB, 23 us, 4 of them the weights (10).  Matrix
+// units busy 7%, VALU issue 19%, 76% of the wave cycles in waits at the first: loads under way bound it, and their number
+// is what the registers hold (a second set of them 192 to 256 VGPRs, slower; 4 waves a SIMD spill; blocks of 64 keys, 8 or 16 waves a
 // workgroup, slower).
 #include <hip/hip_runtime.h>
 
@@ -784,10 +784,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
       static_cast<T*>(a.o)[b * a.os.b + (h0 + h) * a.os.h + d] = (T)(valid ? on : nan);
       if (d == 0 && (a.lse || a.shares || kFused)) {
         const float ls = lt == 0.f ? -INFINITY : fmaf(Mu, a.scale, log_(lt));
-        const Share mine = {Mu, fabsf(ls) < INFINITY ? inverse(lt) : 0.f};
+        const Share head = {Mu, fabsf(ls) < INFINITY ? inverse(lt) : 0.f};
         if (a.lse) a.lse[(long long)b * a.H + h0 + h] = valid ? ls : nan;
-        if (a.shares) a.shares[(long long)b * a.H + h0 + h] = mine;
-        if (kFused) sh_share[h] = mine;
+        if (a.shares) a.shares[(long long)b * a.H + h0 + h] = head;
+        if (kFused) sh_share[h] = head;
       }
     }
   }
@@ -848,10 +848,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(const int* __restric
     if (lane < S) share[h * S + lane] = W == 0.f ? 0.f : f * inverse(W);
     if (lane == 0 && (a.lse || a.shares || kFused)) {
       const float z = W == 0.f ? -INFINITY : fmaf(Mu, a.scale, log_(W));
-      const Share mine = {Mu, fabsf(z) < INFINITY ? inverse(W) : 0.f};
+      const Share head = {Mu, fabsf(z) < INFINITY ? inverse(W) : 0.f};
       if (a.lse) a.lse[(long long)b * a.H + h0 + h] = z;
-      if (a.shares) a.shares[(long long)b * a.H + h0 + h] = mine;
-      if (kFused) sh_share[h] = mine;
+      if (a.shares) a.shares[(long long)b * a.H + h0 + h] = head;
+      if (kFused) sh_share[h] = head;
     }
   }
   __syncthreads();

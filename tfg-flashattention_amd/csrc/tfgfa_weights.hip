@@ -8,11 +8,11 @@
 //
 // Bound: VALU issue.  A pair of query and key costs 2D flops on the matrix units (128 cycles a 32x32 tile at D = 64)
 // and a v_fma, a v_exp_f32 and a v_add on the VALU (16 x 15 cycles a tile).
-// Measured: 16 heads of 8192 causal queries and keys, D = 64, 99-102 us, 670-690 TFLOP/s; VALU issue 65% of the
-// cycles, matrix units 26%, 37% of the wave cycles waiting to issue (without the exponentials 90 us, without the
-// matrix products 73.5, without LDS reads 83).  D = 128, 4 x 16 heads of 4096: 157 us, 876 TFLOP/s.  64 queries
-// against 16001 keys, 2 x 32 heads on 8, D = 128, 27-30 us, 12 of them a plain read of K: a workgroup's first loads
-// are not covered.
+// Measured: 16 heads of 8192 causal queries and keys, D = 64, 101-106 us (on different cards), 650-680 TFLOP/s; VALU issue 66% of
+// the cycles, matrix units 25%, 38% of the wave cycles waiting to issue (without the exponentials 90 us, without the
+// matrix products 73.5, without LDS reads 83, where the whole took 101).  D = 128, 4 x 16 heads of 4096: 163 us, 845
+// TFLOP/s.  64 queries against 16001 keys, 2 x 32 heads on 8, D = 128, 36 us, 28 where K is in the Infinity Cache, 12
+// of them a plain read of K: a workgroup's first loads are not covered.
 //
 // S^T[key][query] = K Q^T as v_mfma_f32_32x32x16 tiles: lane l holds 16 keys of query l % 32, so that the query's lse
 // is one register, the sums over queries stay in 16 registers of each lane, and lanes are added once at the end.  A
