@@ -35,7 +35,8 @@ extern "C" {
  *   LSE[b,h] = log sum_{j < L_b} exp(scale * q[b,h,:] . K[b,h',j,:])
  * q, o: (B, H, D) strides [b, h, d]; k_new, v_new: (B, H_kv, D), both NULL or both set: they become row
  * cache_seqlens[b] of the sequence first (the caller advances cache_seqlens afterwards, and gives no
- * two sequences one page for their new rows; a pool whose strides put rows over one another is refused).  lse: (B, H) contiguous or NULL.
+ * two sequences one page for their new rows; a pool whose strides put rows over one another is
+ * refused).  lse: (B, H) contiguous or NULL.
  * key_weights: NULL, or float32 (B, H_kv, N >= N_max), strides [b, h] in weights_strides, last dimension
  * dense:
  *   key_weights[b,h',j] += sum over the heads h of h' of softmax_j(...)     j < L_b
@@ -105,8 +106,8 @@ size_t tfserve_key_weights_workspace(int B, int H, int H_kv, int N_q, int N_k, i
  *   weights_out[b,h',i] = its key_weights, 0 from n on          float32, strides [b, h], i < budget
  * Pools whose strides put rows over one another are refused.
  * Table entries past a sequence's last row, old and new, are not read.  The pages of new_page_table must
- * be none that any row still reads, and each named once (the caller afterwards takes it for its page_table and bounds
- * cache_seqlens by budget); the old pages are left as they were.  weights_out may be key_weights
+ * be none that any row still reads, and each named once (the caller afterwards takes it for its
+ * page_table and bounds cache_seqlens by budget); the old pages are left as they were.  weights_out may be key_weights
  * itself (same strides).
  * A row whose length does not fit (L < 0 or > M * page), or with a page id outside [0, P) among the
  * ones it needs, gets kept = -1 and weights_out = NaN, and nothing is copied for it.

@@ -15,9 +15,9 @@
 // 4D written a kept row.  Where a head has few rows to copy, the selecting workgroup copies them itself.
 //
 // Measured: 32 heads of up to 32768 rows, D = 128, cut to 4096: selection 23 us (32 of 256 CUs have work; 53% of the
-// wave cycles in waits, for loads and at 17 barriers), copies 35 us, 3.9 TB/s of reads and writes (22, 6 TB/s, from the
-// Infinity Cache); 16 sequences of 25 heads of up to 1024 rows cut to 512: 7.4 and 23 us (15.4); one sequence of 12 heads,
-// 300 rows cut to 130, 7.5 us in one launch.
+// wave cycles in waits, for loads and at 17 barriers), copies 35 us, 3.9 TB/s of reads and writes (22, 6 TB/s, from
+// the Infinity Cache); 16 sequences of 25 heads of up to 1024 rows cut to 512: 7.4 and 23 us (15.4); one sequence of
+// 12 heads, 300 rows cut to 130, 7.5 us in one launch.
 #include <hip/hip_runtime.h>
 
 #include <math.h>

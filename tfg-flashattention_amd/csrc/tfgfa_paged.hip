@@ -15,12 +15,12 @@
 // the lane loads kDV neighbouring dims of each of the 8 rows, and byte permutes put the keys of a dim side by side.
 // So neither P nor V moves between lanes.  P is split into parts of the element type, each what rounding left of the
 // ones before: three of bf16 hold all 24 bits of a float32, two of fp16 miss 2^-23 of it at most, twice a float32's
-// rounding.  (fp16 ends at 2^-24: its P goes in times 2^13, so that weights are kept to 2^-38 of the
-// largest.)  An infinite V makes NaN of a part of 0 or below; a wave whose sums hold NaN takes its keys again with the
-// first part alone, for those sums.  (With P and V as float32 on v_mfma_f32_16x16x4_f32 a block of 32 keys took 1024
-// matrix cycles at D = 64 instead of 192 with two parts.  Two of bf16, 16 bits, gave one output in a thousand another
-// rounding than the definition's; the third takes 32 sequences of 25 heads of 1024 rows from 28.7 to 29.3 us, one of 12
-// heads of 400 from 6.45 to 6.65, and caches that are divided nothing.)
+// rounding.  (fp16 ends at 2^-24: its P goes in times 2^13, so that weights are kept to 2^-38 of the largest.)  An
+// infinite V makes NaN of a part of 0 or below; a wave whose sums hold NaN takes its keys again with the first part
+// alone, for those sums.  (With P and V as float32 on v_mfma_f32_16x16x4_f32 a block of 32 keys took 1024 matrix
+// cycles at D = 64 instead of 192 with two parts.  Two of bf16, 16 bits, gave one output in a thousand another
+// rounding than the definition's; the third takes 32 sequences of 25 heads of 1024 rows from 28.7 to 29.3 us, one of
+// 12 heads of 400 from 6.45 to 6.65, and caches that are divided nothing.)
 //
 // Division of the work.  A unit is a (sequence, key-value head, 16 query heads).  The lengths are known on the device
 // only, so every workgroup works the division out from them (plan, below): one chunk length C for all units, with
@@ -31,13 +31,13 @@
 // joined sums and W their sum of weights, so that s - m is exact for near scores of any size (with e^(x - lse) of
 // rounded x and lse, weights of scores near 2^23 were off by tens of percent).
 //
-// Measured, inputs that no cache holds: 32 sequences of 25 heads, D = 64, lengths to 1024, 120 MB in 28.6 us (24.5 from
-// the Infinity Cache; a plain read of as many bytes 21.6); 4 sequences of 32 heads on 8, D = 128, to 32768 rows, 385 MB
-// in 80 us (67); one sequence of 12 heads, 400 rows, 6.5 us (the chain length - pages - K - V - output; 1.6 us are the
-// launch); 4 sequences of 16 heads to 4096 rows with key weights, 50 MB, 23 us, 4 of them the weights (10).  Matrix
-// units busy 7%, VALU issue 19%, 76% of the wave cycles in waits at the first: loads under way bound it, and their number
-// is what the registers hold (a second set of them 192 to 256 VGPRs, slower; 4 waves a SIMD spill; blocks of 64 keys, 8 or 16 waves a
-// workgroup, slower).
+// Measured, inputs that no cache holds: 32 sequences of 25 heads, D = 64, lengths to 1024, 120 MB in 28.6 us (24.5
+// from the Infinity Cache; a plain read of as many bytes 21.6); 4 sequences of 32 heads on 8, D = 128, to 32768 rows,
+// 385 MB in 80 us (67); one sequence of 12 heads, 400 rows, 6.5 us (the chain length - pages - K - V - output; 1.6 us
+// are the launch); 4 sequences of 16 heads to 4096 rows with key weights, 50 MB, 23 us, 4 of them the weights (10).
+// Matrix units busy 7%, VALU issue 19%, 76% of the wave cycles in waits at the first: loads under way bound it, and
+// their number is what the registers hold (a second set of them 192 to 256 VGPRs, slower; 4 waves a SIMD spill; blocks
+// of 64 keys, 8 or 16 waves a workgroup, slower).
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -135,8 +135,8 @@ __device__ __forceinline__ uint32_t pair_hi(uint32_t x, uint32_t y) {
 // v_exp_f32: results below 2^-126 are 0.
 __device__ __forceinline__ float exp_(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 __device__ __forceinline__ float log_(float x) { return log2f(x) * kLn2; }
-// 1 / x to a rounding for the normal x > 0 whose inverse is normal: v_rcp_f32 is off by one unit, a Newton step takes it
-// away.  (The compiler's division is 10 instructions one after another.)
+// 1 / x to a rounding for the normal x > 0 whose inverse is normal: v_rcp_f32 is off by one unit, a Newton step takes
+// it away.  (The compiler's division is 10 instructions one after another.)
 __device__ __forceinline__ float inverse(float x) {
   const float y = __builtin_amdgcn_rcpf(x);
   return fmaf(fmaf(-x, y, 1.f), y, y);
@@ -966,11 +966,11 @@ static Layout layout(long long units, long long wgs, long long bh, long long n_m
 // unit.  No division (target 0) where there are units enough, or where sequences are short.
 static int choose_target(long long units, int B, long long n_max, int cu_count) {
   const long long per = units * B;
-  // Sequences of like lengths take 1 to 2% longer divided from 4 units a CU on (128 of 8 heads of 4096 rows 188 us, divided
-  // 189; 256 of 2048 180.4 and 183; 64 of 25 heads of 188 to 1500 64.6 and 66; below, 64 of 8 heads of 4096: 67.7 and
-  // 65.7).  The lengths are not known here, and a very long one among that many pays for it: 128 sequences of 8 heads, D =
-  // 128, one of 32768 rows and the others of 512, take 380 us, divided 75.  (Past 2^21 granules the plan's quotients are
-  // not exact.)
+  // Sequences of like lengths take 1 to 2% longer divided from 4 units a CU on (128 of 8 heads of 4096 rows 188 us,
+  // divided 189; 256 of 2048 180.4 and 183; 64 of 25 heads of 188 to 1500 64.6 and 66; below, 64 of 8 heads of 4096:
+  // 67.7 and 65.7).  The lengths are not known here, and a very long one among that many pays for it: 128 sequences of
+  // 8 heads, D = 128, one of 32768 rows and the others of 512, take 380 us, divided 75.  (Past 2^21 granules the
+  // plan's quotients are not exact.)
   if (n_max <= (B == 1 ? kWhole : 2 * kWhole) || per >= (long long)kSlots * 2 * cu_count ||
       (n_max / kGranule + 1) * B >= 1 << 20)
     return 0;
@@ -991,11 +991,11 @@ static bool sizes_ok(int B, int H, int Hkv, int page, int M, int D) {
   return true;
 }
 
-// Granules of the whole batch and workgroups are counted in 32 bits; so are key indexes, with room for the blocks that a
-// loop looks ahead.
+// Granules of the whole batch and workgroups are counted in 32 bits; so are key indexes, with room for the blocks that
+// a loop looks ahead.
 static bool too_large(long long units, int B, int H, long long n_max) {
-  return n_max > INT32_MAX - 128 * kMaxParts * kGranule || B > 65535 || units >= 1 << 20 || (long long)B * H > INT32_MAX ||
-         units * B > INT32_MAX;
+  return n_max > INT32_MAX - 128 * kMaxParts * kGranule || B > 65535 || units >= 1 << 20 ||
+         (long long)B * H > INT32_MAX || units * B > INT32_MAX;
 }
 
 template <class T, int kDV, bool kFull>

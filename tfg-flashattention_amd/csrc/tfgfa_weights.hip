@@ -2,17 +2,17 @@
 //     c_j = sum_h sum_i [j <= first + i] e^(scale q_hi . k_j - lse_hi)
 // over the query heads h of a key-value head, with the log-sum-exp of the attention that ran before.
 //
-// e^(x - lse) is 2^(c s - z) in one v_fma, c the scale times log2 e and z = lse log2 e, both rounded: off by 2^-24 (|c s| +
-// |z|), as x - lse in float32 is.  Where a tile's |z| pass kCoarse, 64, what their roundings left is added (lse near 786432:
-// sums 7% off without; a factor for it in every tile took 16 heads of 8192 from 101 to 112 us).
+// e^(x - lse) is 2^(c s - z) in one v_fma, c the scale times log2 e and z = lse log2 e, both rounded: off by 2^-24 (|c
+// s| + |z|), as x - lse in float32 is.  Where a tile's |z| pass kCoarse, 64, what their roundings left is added (lse
+// near 786432: sums 7% off without; a factor for it in every tile took 16 heads of 8192 from 101 to 112 us).
 //
 // Bound: VALU issue.  A pair of query and key costs 2D flops on the matrix units (128 cycles a 32x32 tile at D = 64)
 // and a v_fma, a v_exp_f32 and a v_add on the VALU (16 x 15 cycles a tile).
-// Measured: 16 heads of 8192 causal queries and keys, D = 64, 101-106 us (on different cards), 650-680 TFLOP/s; VALU issue 66% of
-// the cycles, matrix units 25%, 38% of the wave cycles waiting to issue (without the exponentials 90 us, without the
-// matrix products 73.5, without LDS reads 83, where the whole took 101).  D = 128, 4 x 16 heads of 4096: 163 us, 845
-// TFLOP/s.  64 queries against 16001 keys, 2 x 32 heads on 8, D = 128, 36 us, 28 where K is in the Infinity Cache, 12
-// of them a plain read of K: a workgroup's first loads are not covered.
+// Measured: 16 heads of 8192 causal queries and keys, D = 64, 101-106 us (on different cards), 650-680 TFLOP/s; VALU
+// issue 66% of the cycles, matrix units 25%, 38% of the wave cycles waiting to issue (without the exponentials 90 us,
+// without the matrix products 73.5, without LDS reads 83, where the whole took 101).  D = 128, 4 x 16 heads of 4096:
+// 163 us, 845 TFLOP/s.  64 queries against 16001 keys, 2 x 32 heads on 8, D = 128, 36 us, 28 where K is in the
+// Infinity Cache, 12 of them a plain read of K: a workgroup's first loads are not covered.
 //
 // S^T[key][query] = K Q^T as v_mfma_f32_32x32x16 tiles: lane l holds 16 keys of query l % 32, so that the query's lse
 // is one register, the sums over queries stay in 16 registers of each lane, and lanes are added once at the end.  A

@@ -307,10 +307,10 @@ def evict(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor
     ``key_weights`` (float32 (B, H_kv, N >= M * page)), ties to the lowest row; NaN ranks below every
     number.  The ``n = min(cache_seqlens[b], budget)`` rows kept are copied, in their order, to rows
     0 .. n - 1 of the pages that ``new_page_table`` (int32 (B, M_new), ``M_new * page >= budget``) names;
-    entries past row n are not read.  Those pages must be ones that no row still reads, each named once, in pools that hold each row in a
-    place of its own.  The old pages
-    are left as they were, so that other sequences may go on sharing them.  Afterwards the caller takes
-    ``new_page_table`` for the sequences' and bounds ``cache_seqlens`` by ``budget``.
+    entries past row n are not read.  Those pages must be ones that no row still reads, each named once, in pools that
+    hold each row in a place of its own.  The old pages are left as they were, so that other sequences may go on
+    sharing them.  Afterwards the caller takes ``new_page_table`` for the sequences' and bounds ``cache_seqlens`` by
+    ``budget``.
 
     Returns ``(kept, weights)``: int32 (B, H_kv, budget), the kept rows, -1 from n on, and float32 (B,
     H_kv, budget), their weights, 0 from n on.  With ``weights_out`` (float32 (B, H_kv, at least budget); it
