@@ -935,8 +935,8 @@ def test_serving_operators_on_streams_of_their_own():
 
 
 def test_threads_share_a_stream_and_its_workspace():
-    """Steps of two threads on one stream, which shares one workspace between its calls: key weights that a second kernel
-    adds from scores in it are those of the step by itself."""
+    """Steps of four threads on one stream, whose calls share one workspace: each gives what it gives by itself, key
+    weights that a second kernel adds from scores in the workspace among them."""
     import threading
 
     g = _gen(22)
@@ -944,29 +944,33 @@ def test_threads_share_a_stream_and_its_workspace():
     for L, H, H_kv, page in ((9000, 3, 3, 64), (1500, 20, 1, 7)):
         c = Paged(g, [L], H_kv, 64, page, BF)
         sets.append((_randn((1, H, 64), g, BF), c.k, c.v, c.table, c.seqlens))
-    fresh = lambda s: torch.zeros(1, s[1].shape[1], s[3].shape[1] * s[1].shape[2], device=DEV)  # noqa: E731
-    refs = []
-    for s in sets:
-        w = fresh(s)
-        refs.append((fa.decode_paged(*s, key_weights=w), w))
-    torch.cuda.synchronize()
-    got, stream = [[], []], torch.cuda.current_stream()
 
-    def steps(n):
+    def paged(n):
+        w = torch.zeros(1, sets[n][1].shape[1], sets[n][3].shape[1] * sets[n][1].shape[2], device=DEV)
+        return fa.decode_paged(*sets[n], key_weights=w), w
+
+    step = [_randn((1, 4, 64), g, BF)] + [_randn((1, 4, 6000, 64), g, BF) for _ in range(2)]
+    prompt = [_randn((1, h, 700, 64), g, BF) for h in (16, 1)] + [torch.full((1, 16, 700), 6.0, device=DEV)]
+    assert _C.decode_workspace_size(1, 4, 6000, 64) > 0 and _C.key_weights_workspace(1, 16, 1, 700, 700, True) > 0
+    calls = [lambda: paged(0), lambda: paged(1), lambda: (fa.decode(*step),), lambda: (fa.key_weights(*prompt),)]
+    refs = [call() for call in calls]
+    torch.cuda.synchronize()
+    got, stream = [[] for _ in calls], torch.cuda.current_stream()
+
+    def run(n):
         with torch.cuda.stream(stream):
             for _ in range(100):
-                w = fresh(sets[n])
-                got[n].append((fa.decode_paged(*sets[n], key_weights=w), w))
+                got[n].append(calls[n]())
 
-    threads = [threading.Thread(target=steps, args=(n,)) for n in range(2)]
+    threads = [threading.Thread(target=run, args=(n,)) for n in range(len(calls))]
     for t in threads:
         t.start()
     for t in threads:
         t.join()
     torch.cuda.synchronize()
-    for n in range(2):
+    for n, ref in enumerate(refs):
         assert len(got[n]) == 100
-        assert all(torch.equal(o, refs[n][0]) and torch.equal(w, refs[n][1]) for o, w in got[n]), n
+        assert all(torch.equal(a, b) for outs in got[n] for a, b in zip(outs, ref)), n
 
 
 def test_empty_calls():

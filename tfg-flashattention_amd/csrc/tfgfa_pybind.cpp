@@ -11,6 +11,7 @@
 
 #include <array>
 #include <cstdint>
+#include <mutex>
 #include <stdexcept>
 #include <string>
 #include <tuple>
@@ -24,6 +25,11 @@
 namespace py = pybind11;
 
 namespace {
+
+// Held by the calls that take a workspace.  The Python package keeps one for each stream, which all threads on the
+// stream share: a paged step with key weights may be two launches, with scores in the workspace between them, and no
+// other call's launch on it may come in between.
+std::mutex workspace_calls;
 
 void fwd(std::uintptr_t q, std::uintptr_t k, std::uintptr_t v, std::uintptr_t o, std::uintptr_t lse,
          int B, int H, int N, int D, float softmax_scale, bool causal, std::uintptr_t stream) {
@@ -91,6 +97,7 @@ void decode(std::uintptr_t q, const Strides3& qs, std::uintptr_t kc, const Strid
   int st;
   {
     py::gil_scoped_release nogil;
+    const std::lock_guard<std::mutex> alone(workspace_calls);
     st = tfgfa_decode_bf16(
         reinterpret_cast<const void*>(q), qs.data(), reinterpret_cast<void*>(kc), ks.data(),
         reinterpret_cast<void*>(vc), vs.data(), reinterpret_cast<const void*>(kn), kns.data(),
@@ -114,6 +121,7 @@ void decode_general(std::uintptr_t q, const Strides3& qs, std::uintptr_t kc, con
   int st;
   {
     py::gil_scoped_release nogil;
+    const std::lock_guard<std::mutex> alone(workspace_calls);
     st = tfgfa_decode(
         reinterpret_cast<const void*>(q), qs.data(), reinterpret_cast<void*>(kc), ks.data(),
         reinterpret_cast<void*>(vc), vs.data(), reinterpret_cast<const void*>(kn), kns.data(),
@@ -232,16 +240,19 @@ void decode_paged(std::uintptr_t q, const Strides3& qs, std::uintptr_t k, const 
                   const Strides2& ws, int B, int H, int H_kv, int P, int page, int M, int D,
                   int dtype, float softmax_scale, std::uintptr_t workspace,
                   std::size_t workspace_bytes, std::uintptr_t stream) {
-  // The GIL is kept: a step with key weights may be two launches with scores in the workspace between them, and another
-  // Python thread's call on the same stream, which shares the workspace kept for it, must not come in between.
-  const int st = tfserve_decode_paged(
-      reinterpret_cast<const void*>(q), qs.data(), reinterpret_cast<void*>(k), ks.data(),
-      reinterpret_cast<void*>(v), vs.data(), reinterpret_cast<const int*>(table), table_stride,
-      reinterpret_cast<const int*>(seqlens), reinterpret_cast<const void*>(kn), kns.data(),
-      reinterpret_cast<const void*>(vn), vns.data(), reinterpret_cast<void*>(o), os.data(),
-      reinterpret_cast<float*>(lse), reinterpret_cast<float*>(weights), ws.data(), B, H, H_kv, P,
-      page, M, D, dtype, softmax_scale, reinterpret_cast<void*>(workspace), workspace_bytes,
-      reinterpret_cast<void*>(stream));
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    const std::lock_guard<std::mutex> alone(workspace_calls);
+    st = tfserve_decode_paged(
+        reinterpret_cast<const void*>(q), qs.data(), reinterpret_cast<void*>(k), ks.data(),
+        reinterpret_cast<void*>(v), vs.data(), reinterpret_cast<const int*>(table), table_stride,
+        reinterpret_cast<const int*>(seqlens), reinterpret_cast<const void*>(kn), kns.data(),
+        reinterpret_cast<const void*>(vn), vns.data(), reinterpret_cast<void*>(o), os.data(),
+        reinterpret_cast<float*>(lse), reinterpret_cast<float*>(weights), ws.data(), B, H, H_kv, P,
+        page, M, D, dtype, softmax_scale, reinterpret_cast<void*>(workspace), workspace_bytes,
+        reinterpret_cast<void*>(stream));
+  }
   check(st, "tfserve_decode_paged");
 }
 
@@ -253,6 +264,7 @@ void key_weights(std::uintptr_t q, const Strides4& qs, std::uintptr_t k, const S
   int st;
   {
     py::gil_scoped_release nogil;
+    const std::lock_guard<std::mutex> alone(workspace_calls);
     st = tfserve_key_weights(reinterpret_cast<const void*>(q), qs.data(),
                              reinterpret_cast<const void*>(k), ks.data(),
                              reinterpret_cast<const float*>(lse), ls.data(),
