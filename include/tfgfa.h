@@ -60,8 +60,9 @@ extern "C" {
  * tfgfa_decode_noalloc splits only as far as its scratch holds instead of returning
  * TFGFA_ERR_SCRATCH.
  * 9: the six tfgpt2_* entry points added (tfgfa_gpt2.h).
- * 10: the five tfserve_* entry points added (tfgfa_serving.h). */
-#define TFGFA_ABI_VERSION 10
+ * 10: the five tfserve_* entry points added (tfgfa_serving.h).
+ * 11: the tfpages_* entry points added (tfgfa_pages.h). */
+#define TFGFA_ABI_VERSION 11
 
 /* Status codes (> 0: invalid argument). */
 #define TFGFA_OK                 0

@@ -15,10 +15,12 @@
 #include <stdexcept>
 #include <string>
 #include <tuple>
+#include <utility>
 #include <vector>
 
 #include "tfgfa.h"
 #include "tfgfa_gpt2.h"
+#include "tfgfa_pages.h"
 #include "tfgfa_plan.h"
 #include "tfgfa_serving.h"
 
@@ -320,6 +322,51 @@ void penalize(std::uintptr_t logits, std::int64_t logits_stride, std::uintptr_t 
   check(st, "tfserve_penalize");
 }
 
+// A tensor as (device pointer or 0, element strides).
+using View = std::pair<std::uintptr_t, Strides4>;
+template <class T>
+T* pointer(std::uintptr_t p) {
+  return reinterpret_cast<T*>(p);
+}
+
+void rotate(const View& q, const View& q_out, int H, const View& k, const View& k_out, int H_kv,
+            std::uintptr_t positions, int position_bytes, const Strides2& position_strides,
+            std::int64_t first, std::uintptr_t turns, int rot, bool interleaved, float magnitude,
+            bool transposed, int B, int N, int D, int dtype, std::uintptr_t stream) {
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    st = tfpages_rotate(pointer<void>(q.first), q.second.data(), pointer<void>(q_out.first),
+                        q_out.second.data(), H, pointer<void>(k.first), k.second.data(),
+                        pointer<void>(k_out.first), k_out.second.data(), H_kv,
+                        pointer<void>(positions), position_bytes, position_strides.data(), first,
+                        pointer<std::uint64_t>(turns), rot, interleaved ? 1 : 0, magnitude,
+                        transposed ? 1 : 0, B, N, D, dtype, pointer<void>(stream));
+  }
+  check(st, "tfpages_rotate");
+}
+
+void append(const View& k, const View& v, const View& k_pages, const View& v_pages,
+            std::uintptr_t table, std::int64_t table_stride, std::uintptr_t seqlens,
+            std::uintptr_t lengths, std::uintptr_t positions, const View& q, const View& q_out,
+            bool pad, std::uintptr_t turns, int rot, bool interleaved, float magnitude, int B,
+            int H, int H_kv, int N, int P, int page, int M, int D, int dtype,
+            std::uintptr_t stream) {
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    st = tfpages_append(pointer<void>(k.first), k.second.data(), pointer<void>(v.first),
+                        v.second.data(), pointer<void>(k_pages.first), k_pages.second.data(),
+                        pointer<void>(v_pages.first), v_pages.second.data(), pointer<int>(table),
+                        table_stride, pointer<int>(seqlens), pointer<int>(lengths),
+                        pointer<int>(positions), pointer<void>(q.first), q.second.data(),
+                        pointer<void>(q_out.first), q_out.second.data(), pad ? 1 : 0,
+                        pointer<std::uint64_t>(turns), rot, interleaved ? 1 : 0, magnitude, B, H,
+                        H_kv, N, P, page, M, D, dtype, pointer<void>(stream));
+  }
+  check(st, "tfpages_append");
+}
+
 py::dict device_info() {
   int cu = 0, mhz = 0;
   char arch[128] = {0};
@@ -445,6 +492,20 @@ PYBIND11_MODULE(_C, m) {
         py::arg("frequencies"), py::arg("frequency"), py::arg("bias"), py::arg("bias_stride"),
         py::arg("allowed"), py::arg("allowed_stride"), py::arg("B"), py::arg("V"), py::arg("T"),
         py::arg("stream"));
+  m.def("rotate", &rotate, "Rotary positions; tensors as (pointer or 0, element strides)",
+        py::arg("q"), py::arg("q_out"), py::arg("H"), py::arg("k"), py::arg("k_out"),
+        py::arg("H_kv"), py::arg("positions"), py::arg("position_bytes"),
+        py::arg("position_strides"), py::arg("first"), py::arg("turns"), py::arg("rot"),
+        py::arg("interleaved"), py::arg("magnitude"), py::arg("transposed"), py::arg("B"),
+        py::arg("N"), py::arg("D"), py::arg("dtype"), py::arg("stream"));
+  m.attr("DTYPE_F32") = TFPAGES_DTYPE_F32;
+  m.def("append", &append, "New tokens' keys and values into a paged KV cache", py::arg("k"),
+        py::arg("v"), py::arg("k_pages"), py::arg("v_pages"), py::arg("page_table"),
+        py::arg("table_stride"), py::arg("cache_seqlens"), py::arg("lengths"),
+        py::arg("positions"), py::arg("q"), py::arg("q_out"), py::arg("pad"), py::arg("turns"),
+        py::arg("rot"), py::arg("interleaved"), py::arg("magnitude"), py::arg("B"), py::arg("H"),
+        py::arg("H_kv"), py::arg("N"), py::arg("P"), py::arg("page"), py::arg("M"), py::arg("D"),
+        py::arg("dtype"), py::arg("stream"));
   m.def("fwd_plan",
         [](long long heads, int cu_count, int Nq, int Nk, int D, bool causal) {
           static const char* const names[] = {"kWhole", "kHalves", "kGroups2", "kPairs", "kGroups4"};

@@ -1,0 +1,359 @@
+"""The operators around a paged KV cache (include/tfgfa_pages.h) on torch tensors: rotary positions, new tokens' keys
+and values into the pages, attention of several new tokens over them, and a decode step for sequences that share a
+prefix.
+
+The reference's model has learned positions and keeps no cache (src/py/model_inference.py:166-228); nothing here has
+a counterpart in it.  The functions check their arguments (RuntimeError, before anything is launched), launch on the
+current stream of the tensors' device and do not synchronise.  :func:`rotate` has a gradient; the others are inference
+operators, whose results carry none.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+from torch.autograd import forward_ad
+
+from . import _C, _DTYPES, MAX_HEAD_DIM, _launch_on
+from .serving import (_accepts_pages, _check_pages, _check_seqlens, _check_table, _is_seqlens, _is_table)
+
+_NONE = (0, (0, 0, 0, 0))
+_ROTATED = {torch.bfloat16: _C.DTYPE_BF16, torch.float16: _C.DTYPE_F16, torch.float32: _C.DTYPE_F32}
+_INTS = (torch.int32, torch.int64)
+
+
+def _view(t):
+    return _NONE if t is None else (t.data_ptr(), t.stride())
+
+
+class Rotary:
+    """A model's rotary positions: of each head's first ``dim`` dims (even, the whole head or a part of it) pair i is
+    turned by ``position * frequencies[i]`` radians.  Pairs are dims (i, i + dim / 2), or with ``interleaved`` (2i, 2i + 1).
+
+    Frequencies are ``base ** (-2 i / dim)``, for contexts longer than the trained ones scaled by ``factor``:
+      * ``scaling="linear"``: divided by it;
+      * ``scaling="base"``: of base ``base * factor ** (dim / (dim - 2))``, which divides the last by it and keeps the first;
+      * ``scaling="bands"``: those that turn at least ``high`` times within ``trained_length`` positions are kept, those
+        that turn at most ``low`` times divided, those between mixed in proportion to their turns;
+    or ``frequencies`` (dim / 2 numbers, radians a position) gives them.  ``magnitude`` multiplies what is rotated.
+    They are kept on ``device`` as 64-bit fractions of a turn, so that an angle is exact at any position.
+    """
+
+    def __init__(self, dim: int, base: float = 10000.0, *, interleaved: bool = False, scaling: str | None = None,
+                 factor: float = 1.0, trained_length: int | None = None, low: float = 1.0, high: float = 32.0,
+                 magnitude: float = 1.0, frequencies=None, device="cuda"):
+        if not (isinstance(dim, int) and 2 <= dim <= MAX_HEAD_DIM and dim % 2 == 0):
+            raise RuntimeError(f"dim must be even, in [2, {MAX_HEAD_DIM}], got {dim}")
+        if not (math.isfinite(magnitude) and magnitude > 0):
+            raise RuntimeError(f"magnitude must be finite and positive, got {magnitude}")
+        if frequencies is not None:
+            if scaling is not None:
+                raise RuntimeError("frequencies are given as they are: no scaling beside them")
+            f = [float(x) for x in frequencies]
+            if len(f) != dim // 2 or not all(math.isfinite(x) for x in f):
+                raise RuntimeError(f"frequencies must be {dim // 2} finite numbers")
+        else:
+            if not (math.isfinite(base) and base > 0):
+                raise RuntimeError(f"base must be finite and positive, got {base}")
+            if scaling not in (None, "linear", "base", "bands"):
+                raise RuntimeError(f"scaling must be None, 'linear', 'base' or 'bands', got {scaling!r}")
+            if not (math.isfinite(factor) and factor > 0) or (scaling is None and factor != 1.0):
+                raise RuntimeError(f"factor must be finite and positive, and 1 without scaling, got {factor}")
+            if scaling == "base" and dim > 2:
+                base = base * factor ** (dim / (dim - 2))
+            f = [base ** (-2 * i / dim) for i in range(dim // 2)]
+            if scaling == "linear":
+                f = [x / factor for x in f]
+            elif scaling == "bands":
+                if trained_length is None or trained_length <= 0 or not 0 <= low < high < math.inf:
+                    raise RuntimeError("scaling='bands' needs a positive trained_length and 0 <= low < high, got "
+                                       f"{trained_length}, {low} and {high}")
+                for i, x in enumerate(f):
+                    keep = min(1.0, max(0.0, (trained_length * x / (2 * math.pi) - low) / (high - low)))
+                    f[i] = x / factor * (1 - keep) + x * keep
+        self.dim, self.interleaved, self.magnitude, self.frequencies = dim, bool(interleaved), float(magnitude), tuple(f)
+        self._turns = torch.tensor([_turn(x) for x in f], dtype=torch.int64).to(device)
+
+    def to(self, device) -> "Rotary":
+        """The same on another device."""
+        return Rotary(self.dim, interleaved=self.interleaved, magnitude=self.magnitude, frequencies=self.frequencies,
+                      device=device)
+
+
+def _turn(frequency: float) -> int:
+    """The frequency as turns in 2^-64, modulo a turn, as a signed 64-bit integer (the nearest to the float64 quotient)."""
+    n = round(math.fmod(frequency / (2 * math.pi), 1.0) * 2.0 ** 64) % 2 ** 64
+    return n - 2 ** 64 if n >= 2 ** 63 else n
+
+
+def _is_rotary(rotary, index: int, D: int) -> bool:
+    return type(rotary) is Rotary and rotary._turns.get_device() == index and rotary.dim <= D
+
+
+def _check_rotary(rotary, dev, D: int) -> None:
+    if not isinstance(rotary, Rotary):
+        raise RuntimeError(f"rotary must be a Rotary, got {type(rotary).__name__}")
+    if rotary._turns.device != dev:
+        raise RuntimeError(f"rotary must be on {dev}, got {rotary._turns.device}")
+    if rotary.dim > D:
+        raise RuntimeError(f"rotary rotates {rotary.dim} dims of a head of {D}")
+
+
+def _are_positions(p, B: int, N: int, index: int) -> bool:
+    return p.dtype in _INTS and p.get_device() == index and p.shape in ((N,), (B, N), (1, N))
+
+
+def _accepts_rotate(q, k, positions, rotary, outs) -> bool:
+    """Everything _check_rotate checks, as one test."""
+    qs, index, dtype = q.shape, q.get_device(), q.dtype
+    if not (index >= 0 and q.is_cuda and dtype in _ROTATED and len(qs) == 4 and 1 <= qs[3] <= MAX_HEAD_DIM
+            and (q.stride(3) == 1 or qs[3] == 1) and _is_rotary(rotary, index, qs[3])):
+        return False
+    if k is not None:
+        ks = k.shape
+        if not (k.dtype is dtype and k.get_device() == index and len(ks) == 4 and ks[0] == qs[0] and ks[2] == qs[2]
+                and ks[3] == qs[3] and (k.stride(3) == 1 or qs[3] == 1)):
+            return False
+    for x, out in zip((q, k), outs):
+        if out is not None and not (x is not None and out.shape == x.shape and out.dtype is dtype
+                                    and out.get_device() == index and (out.stride(3) == 1 or qs[3] == 1)):
+            return False
+    return type(positions) is int or (isinstance(positions, torch.Tensor) and _are_positions(positions, qs[0], qs[2], index))
+
+
+def _check_rotate(q, k, positions, rotary, outs) -> None:
+    for x, n in ((q, "q"), (k, "k"), (outs[0], "q_out"), (outs[1], "k_out")):
+        if x is None:
+            continue
+        if not x.is_cuda:
+            raise RuntimeError(f"{n} must be a CUDA tensor")
+        if x.dtype not in _ROTATED:
+            raise RuntimeError("Unsupported tensor dtype. Use float32, bfloat16 or float16.")
+        if x.dim() != 4:
+            raise RuntimeError(f"{n} must be 4-D (batch, heads, seq_len, head_dim), got shape {tuple(x.shape)}")
+        if x.stride(3) != 1 and x.shape[3] > 1:
+            raise RuntimeError(f"{n} must be dense in its last dimension (stride 1), got strides {x.stride()}")
+        if x.dtype != q.dtype:
+            raise RuntimeError(f"{n} must have dtype {q.dtype}, got {x.dtype}")
+        if x.device != q.device:
+            raise RuntimeError(f"{n} must be on {q.device}, got {x.device}")
+    B, _, N, D = q.shape
+    if not 1 <= D <= MAX_HEAD_DIM:
+        raise RuntimeError(f"head_dim must be in [1, {MAX_HEAD_DIM}], got {D}")
+    if k is not None and (k.shape[0], k.shape[2], k.shape[3]) != (B, N, D):
+        raise RuntimeError(f"k must have shape {(B, 'H_kv', N, D)}, got {tuple(k.shape)}")
+    for x, out, n in ((q, outs[0], "q_out"), (k, outs[1], "k_out")):
+        if out is not None and (x is None or out.shape != x.shape):
+            raise RuntimeError(f"{n} must have the shape of what is rotated into it")
+    _check_rotary(rotary, q.device, D)
+    if isinstance(positions, torch.Tensor):
+        if positions.dtype not in _INTS or tuple(positions.shape) not in ((N,), (B, N), (1, N)):
+            raise RuntimeError(f"positions must be int32 or int64 of shape ({N},) or ({B}, {N}), got {positions.dtype} "
+                               f"{tuple(positions.shape)}")
+        if positions.device != q.device:
+            raise RuntimeError(f"positions must be on {q.device}, got {positions.device}")
+    elif not isinstance(positions, int):
+        raise RuntimeError(f"positions must be a tensor or the first position, got {type(positions).__name__}")
+
+
+def _rotate(q, k, positions, rotary, q_out, k_out, transposed: bool) -> None:
+    """Launches the rotation of what _check_rotate takes."""
+    B, H, N, D = q.shape
+    if isinstance(positions, torch.Tensor):
+        strides = positions.stride()
+        # (A single row of positions is every sequence's.)
+        strides = (0, strides[-1]) if len(strides) == 1 or positions.shape[0] == 1 else strides
+        where, size, first = positions.data_ptr(), positions.element_size(), 0
+    else:
+        where, size, strides, first = 0, 4, (0, 0), int(positions)
+    _launch_on(q.get_device(), _C.rotate, _view(q), _view(q_out), H, _view(k), _view(k_out), 0 if k is None else k.shape[1],
+               where, size, strides, first, rotary._turns.data_ptr(), rotary.dim, rotary.interleaved, rotary.magnitude,
+               transposed, B, N, D, _ROTATED[q.dtype])
+
+
+def _dense(x):
+    """A gradient as the kernel takes it: an expanded last dimension, for one, is copied."""
+    return x if x.shape[-1] <= 1 or x.stride(-1) == 1 else x.contiguous()
+
+
+class _Rotate(torch.autograd.Function):
+    """The rotation as a differentiable function: linear in q and k, its gradient the transposed rotation."""
+
+    @staticmethod
+    def forward(q, k, positions, rotary, transposed):
+        q_out, k_out = torch.empty_like(q), None if k is None else torch.empty_like(k)
+        _rotate(q, k, positions, rotary, q_out, k_out, transposed)
+        return q_out, k_out
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _, _, positions, ctx.rotary, ctx.transposed = inputs
+        ctx.first = None
+        if isinstance(positions, torch.Tensor):
+            ctx.save_for_backward(positions)
+            ctx.save_for_forward(positions)
+        else:
+            ctx.first = positions
+        ctx.set_materialize_grads(False)
+
+    @staticmethod
+    def _apply(ctx, q, k, transposed):
+        positions = ctx.saved_tensors[0] if ctx.first is None else ctx.first
+        q, k = (None if x is None else _dense(x) for x in (q, k))
+        if q is None:
+            return None, None if k is None else _Rotate.apply(k, None, positions, ctx.rotary, transposed)[0]
+        return _Rotate.apply(q, k, positions, ctx.rotary, transposed)
+
+    @staticmethod
+    def backward(ctx, q, k):
+        q, k = _Rotate._apply(ctx, q if ctx.needs_input_grad[0] else None, k if ctx.needs_input_grad[1] else None,
+                              not ctx.transposed)
+        return q, k, None, None, None
+
+    @staticmethod
+    def jvp(ctx, q, k, *_):
+        return _Rotate._apply(ctx, q, k, ctx.transposed)
+
+
+def rotate(q: torch.Tensor, k: torch.Tensor | None, positions, rotary: Rotary, *, q_out: torch.Tensor | None = None,
+           k_out: torch.Tensor | None = None):
+    """Rotary positions on queries and keys, in one launch.
+
+    ``q``: (B, H, N, D), ``k``: (B, H_kv, N, D) or None; float32, bf16 or fp16 alike, any strides whose last dimension is
+    dense (16-byte pieces are moved whole where strides, D and the rotated dims allow it), D up to 128.  ``positions``:
+    int32 or int64 of shape (N,) or (B, N), or an int, the first of N positions in a row.  ``rotary``: a
+    :class:`Rotary`; dims past ``rotary.dim`` are copied.  Arithmetic is float32 with one rounding.
+
+    Returns (q', k'), or q' for ``k=None``: new tensors, or ``q_out`` and ``k_out``, of which ``q_out`` may be ``q`` and
+    ``k_out`` ``k`` (other overlaps are not taken).  Differentiable with respect to q and k, to any order; with outputs
+    given it is not, and refuses inputs that need a gradient.  A captured backward pass needs, as torch's own do, that no
+    eager graph of the same leaves lives.
+    """
+    outs = (q_out, k_out)
+    if not _accepts_rotate(q, k, positions, rotary, outs):
+        _check_rotate(q, k, positions, rotary, outs)
+    grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
+    if grad or forward_ad._current_level >= 0 or torch._C._functorch.peek_interpreter_stack() is not None:
+        if q_out is not None or k_out is not None:
+            raise RuntimeError("q_out and k_out are not differentiable: rotate without them, or under torch.no_grad()")
+        q_out, k_out = _Rotate.apply(q, k, positions, rotary, False)
+    else:
+        if q_out is None:
+            q_out = torch.empty_like(q)
+        if k is not None and k_out is None:
+            k_out = torch.empty_like(k)
+        _rotate(q, k, positions, rotary, q_out, k_out, False)
+    return q_out if k is None else (q_out, k_out)
+
+
+def _are_rows(x, B: int, H: int, N: int, D: int, dtype, index: int) -> bool:
+    return x.shape == (B, H, N, D) and x.dtype is dtype and x.get_device() == index and x.stride(3) == 1
+
+
+def _check_rows(x, name: str, B: int, H: int, N: int, D: int, dtype, dev) -> None:
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if x.dtype != dtype:
+        raise RuntimeError(f"{name} must have dtype {dtype}, got {x.dtype}")
+    if tuple(x.shape) != (B, H, N, D):
+        raise RuntimeError(f"{name} must have shape {(B, H, N, D)}, got {tuple(x.shape)}")
+    if x.device != dev:
+        raise RuntimeError(f"{name} must be on {dev}, got {x.device}")
+    if x.stride(3) != 1:
+        raise RuntimeError(f"{name} must be dense in its last dimension (stride 1), got strides {x.stride()}")
+
+
+def _check_counts(t, name: str, B: int, dev) -> None:
+    if t.dtype != torch.int32 or tuple(t.shape) != (B,) or t.device != dev or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous int32 tensor of shape ({B},) on {dev}")
+
+
+def _accepts_append(k, v, k_pages, v_pages, page_table, cache_seqlens, lengths, rotary, positions, q, q_out) -> bool:
+    """Everything _check_append checks, as one test."""
+    index, ks = k_pages.get_device(), k.shape
+    if not (_accepts_pages(k_pages, v_pages, index) and len(ks) == 4):
+        return False
+    _, H_kv, _, D = k_pages.shape
+    B, N, dtype = ks[0], ks[2], k_pages.dtype
+    if not (_are_rows(k, B, H_kv, N, D, dtype, index) and _are_rows(v, B, H_kv, N, D, dtype, index)
+            and _is_table(page_table, B, index) and _is_seqlens(cache_seqlens, B, index)):
+        return False
+    if rotary is None:
+        if q is not None or positions is not None:
+            return False
+    elif not _is_rotary(rotary, index, D):
+        return False
+    for x in (lengths, positions):
+        if x is not None and not _is_seqlens(x, B, index):
+            return False
+    if q is None:
+        return q_out is None
+    qs = q.shape
+    if len(qs) != 4:
+        return False
+    return all(x is None or _are_rows(x, B, qs[1], N, D, dtype, index) for x in (q, q_out))
+
+
+def _check_append(k, v, k_pages, v_pages, page_table, cache_seqlens, lengths, rotary, positions, q, q_out) -> None:
+    _check_pages(k_pages, v_pages)
+    _, H_kv, _, D = k_pages.shape
+    dev, dtype = k_pages.device, k_pages.dtype
+    if k.dim() != 4:
+        raise RuntimeError(f"k must be 4-D (batch, heads, seq_len, head_dim), got shape {tuple(k.shape)}")
+    B, _, N, _ = k.shape
+    _check_rows(k, "k", B, H_kv, N, D, dtype, dev)
+    _check_rows(v, "v", B, H_kv, N, D, dtype, dev)
+    _check_table(page_table, "page_table", B, dev)
+    _check_seqlens(cache_seqlens, B, dev)
+    if lengths is not None:
+        _check_counts(lengths, "lengths", B, dev)
+    if rotary is None:
+        for x, n in ((q, "q"), (positions, "positions")):
+            if x is not None:
+                raise RuntimeError(f"{n} needs a rotary")
+    else:
+        _check_rotary(rotary, dev, D)
+    if positions is not None:
+        _check_counts(positions, "positions", B, dev)
+    if q is None:
+        if q_out is not None:
+            raise RuntimeError("q_out needs q")
+    else:
+        if q.dim() != 4:
+            raise RuntimeError(f"q must be 4-D (batch, heads, seq_len, head_dim), got shape {tuple(q.shape)}")
+        _check_rows(q, "q", B, q.shape[1], N, D, dtype, dev)
+        if q_out is not None:
+            _check_rows(q_out, "q_out", B, q.shape[1], N, D, dtype, dev)
+
+
+def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 page_table: torch.Tensor, cache_seqlens: torch.Tensor, *, lengths: torch.Tensor | None = None,
+                 rotary: Rotary | None = None, positions: torch.Tensor | None = None, q: torch.Tensor | None = None,
+                 q_out: torch.Tensor | None = None):
+    """New tokens' keys and values into a paged cache (:func:`decode_paged`), rotated on the way, in one launch.
+
+    ``k``, ``v``: (B, H_kv, N, D) of the pools' type, any strides as for :func:`attention`.  Token i of sequence b becomes
+    its row ``cache_seqlens[b] + i``; with ``lengths`` (int32 (B,)) only the first ``lengths[b]`` of its N tokens do.
+    The rows' pages must be the sequence's own, in pools that hold each row in a place of its own; the caller advances
+    ``cache_seqlens`` afterwards (after :func:`attend_paged`, which counts the rows before the new tokens too).
+    With ``rotary`` the keys are rotated, token i at position ``positions[b] + i`` (int32 (B,); ``cache_seqlens[b] + i``
+    without), and so are the queries ``q`` (B, H, N, D), if given: they are returned, in ``q_out`` if given (``q`` itself is
+    taken).  Rows of tokens past ``lengths[b]`` are left as they were in ``q_out``, and zeros in a new tensor.
+
+    A sequence whose length or number of new tokens does not fit its table gets no row, and NaN for its queries; a row
+    whose page id is outside the pool is not written (checked on the device).
+    """
+    if not _accepts_append(k, v, k_pages, v_pages, page_table, cache_seqlens, lengths, rotary, positions, q, q_out):
+        _check_append(k, v, k_pages, v_pages, page_table, cache_seqlens, lengths, rotary, positions, q, q_out)
+    P, H_kv, page, D = k_pages.shape
+    B, _, N, _ = k.shape
+    pad = q_out is None
+    if q is not None and pad:
+        q_out = torch.empty_like(q)
+    turns, rot, interleaved, magnitude = (0, 0, False, 1.0) if rotary is None else (
+        rotary._turns.data_ptr(), rotary.dim, rotary.interleaved, rotary.magnitude)
+    _launch_on(k_pages.get_device(), _C.append, _view(k), _view(v), _view(k_pages), _view(v_pages), page_table.data_ptr(),
+               page_table.stride(0), cache_seqlens.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
+               0 if positions is None else positions.data_ptr(), _view(q), _view(q_out), pad, turns, rot, interleaved,
+               magnitude, B, 0 if q is None else q.shape[1], H_kv, N, P, page, page_table.shape[1], D, _DTYPES[k.dtype])
+    return q_out
