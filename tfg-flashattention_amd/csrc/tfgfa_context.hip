@@ -1,0 +1,1261 @@
+// tfgfa_context.hip - attention of several query rows over a paged key-value cache, MI355X (gfx950), bf16 or fp16, head
+// dims that are multiples of 8 up to 128, query heads sharing key-value heads: new tokens of a sequence (tfpages_attend),
+// and a decode step of sequences that share a prefix (tfpages_decode_shared).
+//
+//     o_r = sum_{j < L_r} softmax_j(scale q_r . k_j) v_j,   lse_r = log sum_{j < L_r} e^(scale q_r . k_j)
+// The rows r that meet the same keys are one job: a key-value head's query heads, times the new tokens of a sequence, or
+// times the sequences behind a prefix.  Bound: HBM for few rows (4 D bytes a key, 4 D flops a key and row), the VALU's
+// exponentials beside the matrix units for many.
+//
+// A block is 32 keys by 32 rows, on v_mfma_f32_32x32x16 (layouts as in tfgfa_fwd.hip):
+//   S^T[key][row] = K Q^T: lane (h, i) holds 16 keys of row i, so the softmax of a row is two lanes' own registers;
+//   O^T[dim][row] += V^T P^T: those 16 values are the B operand as they stand (the keys' order in the contraction is
+//   free), V's operand comes by transposing LDS reads.
+// K and V rows go from their pages to LDS by direct loads, 8 keys a transfer.  Where a page is a multiple of 8 keys, a
+// transfer has one page: its id and address are scalars, and rows past the end are past its descriptor, which gives zeros.
+// Other pages: each lane has an address, of a row of zeros where there is no key.  A page id outside the pool gives a
+// row of NaN for K, so that NaN reaches the rows that see the key, and zeros for V.
+//
+// Few rows (up to 64 a job): each wave streams blocks of its own (wave w of a workgroup takes blocks w, w + 4, ..) through
+// a ring of its own, with no barrier, all rows in its registers; the four are joined through LDS.  Many rows: four waves
+// of 32 rows share tiles of 64 keys.  A job's keys may be divided over workgroups, whose parts a second kernel joins.
+//
+// Hidden keys have weight 0, but 0 times an infinite or NaN value is NaN: a wave whose sums hold NaN at the end takes its
+// keys again with products on the VALU that leave weights of 0 out (so the common path checks nothing).
+#include <hip/hip_runtime.h>
+
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "tfgfa.h"
+#include "tfgfa_device.h"
+#include "tfgfa_layout.h"
+#include "tfgfa_pages.h"
+
+namespace tfgfa_context {
+
+using tfgfa::Division;
+using tfgfa::i32x4;
+using tfgfa::Pages;
+using tfgfa::Rows;
+using tfgfa::Vecs;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kMaxD = 128;
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kBlock = 32;                    // keys of a block; rows of a wave's tile
+constexpr int kGroup = 8;                     // keys of a transfer
+constexpr int kHalfBytes = kBlock * 128;      // K or V of a block, 64 dims
+constexpr int kManyRows = kWaves * kBlock;    // rows of a workgroup for many rows
+constexpr int kTile = 2 * kBlock;             // keys of its tile
+constexpr int kMaxParts = 64;                 // workgroups of a job
+constexpr int kOutOfRange = 0x7FFFFFF0;       // a buffer offset past any num_records: the load gives zeros
+
+// kHead: weights are 2^(c (s - m)), s a score without the scale, c the scale times log2 e.  A row's offset m puts the
+// largest weight at 2^kHead, and moves when one would pass 2^(kHead + kMargin).  fp16 ends at 2^-24: with the largest at
+// 2^13, weights are kept to 2^-37 of it.
+template <class T>
+struct Elem;
+template <>
+struct Elem<__bf16> {
+  typedef bf16x8 v8;
+  typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+  static constexpr float kHead = 0.f, kMargin = 8.f;
+  static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float add2(v2 x, float acc) {
+    return __builtin_amdgcn_fdot2_f32_bf16(x, v2{(__bf16)1.f, (__bf16)1.f}, acc, false);
+  }
+};
+template <>
+struct Elem<_Float16> {
+  typedef f16x8 v8;
+  typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+  static constexpr float kHead = 13.f, kMargin = 2.f;
+  static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float add2(v2 x, float acc) {
+    return __builtin_amdgcn_fdot2(x, v2{(_Float16)1.f, (_Float16)1.f}, acc, false);
+  }
+};
+
+// The value of the other half's lane, with the own: a row's two lanes.
+template <class F>
+__device__ __forceinline__ float over_pair(float x, F f) {
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return f(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+__device__ __forceinline__ int divide(int x, Division d) { return (int)(((uint64_t)(uint32_t)x * d.m) >> d.s); }
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+__device__ const uint32_t kNanRow[kMaxD / 2] = {
+#define TFGFA_8(x) x, x, x, x, x, x, x, x
+    TFGFA_8(0x7FFF7FFFu), TFGFA_8(0x7FFF7FFFu), TFGFA_8(0x7FFF7FFFu), TFGFA_8(0x7FFF7FFFu),
+    TFGFA_8(0x7FFF7FFFu), TFGFA_8(0x7FFF7FFFu), TFGFA_8(0x7FFF7FFFu), TFGFA_8(0x7FFF7FFFu)};
+__device__ const uint32_t kZeroRow[kMaxD / 2] = {};
+
+typedef const __attribute__((address_space(4))) int* uniform_ints;
+
+// A sequence's keys in one key-value head.
+struct Source {
+  const char* k;  // the pools, at the head
+  const char* v;
+  Pages ks, vs;
+  const int* table;
+  Division by_page;
+  int page, P;
+  int keys;       // keys that there are
+};
+
+// 1 KiB from 64 addresses to LDS, as tfgfa::lds_transfer does from a buffer.
+__device__ __forceinline__ void lds_gather(uint64_t from, uint32_t lds_base) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %2, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(lds_base), "v"(from)
+      : "memory");
+}
+
+__device__ __forceinline__ int swz_v(int row) { return (row & 3) << 1; }
+
+// Loads of kGroups groups of 8 keys, from group g0 of a block on.  A block in LDS: K's halves of 64 dims, then V's, each 32
+// rows of 128 bytes; chunk c of row r at place c ^ swz (tfgfa_fwd.hip says why).  Lane l of a transfer fills chunk l % 8
+// of row l / 8 of the group.
+template <int kDH, bool kAligned, int kGroups>
+struct Loader {
+  int koff[kGroups][kDH], voff[kDH];  // aligned: byte offsets from the group's first row; otherwise in a row, or out of range
+  int id[kAligned ? kGroups : 1];     // pages of the block that is loaded next
+  int g0, lane;
+
+  __device__ __forceinline__ void init(const Source& s, int D, int g0_, int lane_) {
+    g0 = g0_, lane = lane_;
+    const int r = lane >> 3, chunks = D >> 3;
+#pragma unroll
+    for (int dh = 0; dh < kDH; ++dh) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const int c = 8 * dh + ((lane & 7) ^ tfgfa::swz_k((g0 + g) * kGroup + r));
+        koff[g][dh] = c < chunks ? (kAligned ? r * (int)s.ks.n : 0) + 16 * c : kOutOfRange;
+      }
+      const int c = 8 * dh + ((lane & 7) ^ swz_v(r));
+      voff[dh] = c < chunks ? (kAligned ? r * (int)s.vs.n : 0) + 16 * c : kOutOfRange;
+    }
+  }
+  // The pages of the block at key `at`.
+  __device__ __forceinline__ void look_up(const Source& s, int at) {
+    if constexpr (kAligned) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const int key = at + (g0 + g) * kGroup;
+        id[g] = uniform(key < s.keys ? ((uniform_ints)s.table)[divide(key, s.by_page)] : 0);
+      }
+    } else {
+      const int key = at + (lane & 31);
+      id[0] = key < s.keys ? s.table[divide(key, s.by_page)] : 0;
+    }
+  }
+  // The block at key `at`, whose pages were looked up, to LDS byte `to`.
+  __device__ __forceinline__ void issue(const Source& s, int at, uint32_t to) {
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const uint32_t k_to = to + (g0 + g) * 1024, v_to = k_to + kDH * kHalfBytes;
+      if constexpr (kAligned) {
+        const int key = at + (g0 + g) * kGroup, rows = uniform(min(kGroup, max(0, s.keys - key)));
+        const bool in = (uint32_t)id[g] < (uint32_t)s.P;
+        const int there = uniform(in ? rows : 0);
+        const uint64_t pid = (uint32_t)(in ? id[g] : 0), off = (uint32_t)(key - divide(key, s.by_page) * s.page);
+        const i32x4 kd = tfgfa::head_desc(s.k + pid * (uint64_t)s.ks.p + off * (uint64_t)s.ks.n, there, (int)s.ks.n);
+        const i32x4 vd = tfgfa::head_desc(s.v + pid * (uint64_t)s.vs.p + off * (uint64_t)s.vs.n, there, (int)s.vs.n);
+        if (in || rows == 0) {
+#pragma unroll
+          for (int dh = 0; dh < kDH; ++dh) tfgfa::lds_transfer(kd, k_to + dh * kHalfBytes, koff[g][dh]);
+        } else {
+          const i32x4 nd = tfgfa::head_desc(kNanRow, 1, sizeof(kNanRow));
+#pragma unroll
+          for (int dh = 0; dh < kDH; ++dh)
+            tfgfa::lds_transfer(nd, k_to + dh * kHalfBytes,
+                                koff[g][dh] == kOutOfRange || (lane >> 3) >= rows ? kOutOfRange : koff[g][dh] - (lane >> 3) * (int)s.ks.n);
+        }
+#pragma unroll
+        for (int dh = 0; dh < kDH; ++dh) tfgfa::lds_transfer(vd, v_to + dh * kHalfBytes, voff[dh]);
+      } else {
+        const int r = (g0 + g) * kGroup + (lane >> 3), key = at + r;
+        const int page = __shfl(id[0], r);
+        const bool there = key < s.keys, in = there && (uint32_t)page < (uint32_t)s.P;
+        const uint64_t pid = (uint32_t)(in ? page : 0), off = (uint32_t)(in ? key - divide(key, s.by_page) * s.page : 0);
+        const uint64_t kr = in ? (uint64_t)(uintptr_t)s.k + pid * (uint64_t)s.ks.p + off * (uint64_t)s.ks.n
+                               : (uint64_t)(uintptr_t)(there ? kNanRow : kZeroRow);
+        const uint64_t vr = in ? (uint64_t)(uintptr_t)s.v + pid * (uint64_t)s.vs.p + off * (uint64_t)s.vs.n
+                               : (uint64_t)(uintptr_t)kZeroRow;
+        const uint64_t zero = (uint64_t)(uintptr_t)kZeroRow;
+#pragma unroll
+        for (int dh = 0; dh < kDH; ++dh) {
+          lds_gather(koff[g][dh] == kOutOfRange ? zero : kr + koff[g][dh], k_to + dh * kHalfBytes);
+          lds_gather(voff[dh] == kOutOfRange ? zero : vr + voff[dh], v_to + dh * kHalfBytes);
+        }
+      }
+    }
+  }
+};
+
+// A wave's rows: kRT tiles of 32, row i of tile t in lanes i and i + 32.
+// kParts: of the element type that a weight is split into for the product with V, each what rounding left of the ones
+// before (2: all but 2^-16 of a weight in bf16, 2^-22 in fp16).  With 1 the output is divided by the sum of the rounded weights, so that the
+// rounding of a weight that stands alone cancels; the log-sum-exp takes the unrounded ones.
+template <class T, int kDH, int kRT, int kParts>
+struct State {
+  typedef typename Elem<T>::v8 v8;
+  typedef typename Elem<T>::v2 v2;
+  static constexpr int kC = 4 * kDH;   // pieces of 16 dims
+  static constexpr int kOT = 2 * kDH;  // output tiles of 32
+  v8 q[kRT][kC];
+  f32x16 o[kRT][kOT];
+  float m[kRT], thr[kRT];   // offset, and how far a score may pass it (-inf: the row has no weight yet)
+  f32x16 below[kRT];        // -m, what the products start from
+  float l[kRT], lp[kRT];    // this lane's sums of weights; kParts 1: of the rounded ones
+  int seen[kRT];            // keys that the row sees
+  int koff[4], voff[2][2];  // LDS offsets of the operands, in a block's first 64 dims
+
+  __device__ __forceinline__ void init(int lane) {
+    const int i = lane & 31, h = lane >> 5, g = lane >> 4, j = lane & 15;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) koff[c] = i * 128 + (((2 * c + h) ^ tfgfa::swz_k(i)) << 4);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int row = 8 * s + 4 * (g >> 1) + (j >> 2), d = 32 * t + 16 * (g & 1) + 4 * (j & 3);
+        voff[t][s] = row * 128 + (((d >> 3) ^ swz_v(row)) << 4) + (d & 7) * 2;
+      }
+    clear();
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int t = 0; t < kRT; ++t) {
+      m[t] = l[t] = lp[t] = 0.f, thr[t] = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) below[t][r] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kOT; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[t][j][r] = 0.f;
+    }
+  }
+
+  // S^T of the block in LDS, from c on.
+  __device__ __forceinline__ void scores(f32x16 (&s)[kRT], const unsigned char* block, bool offset) const {
+#pragma unroll
+    for (int t = 0; t < kRT; ++t) {
+      if (offset) {
+        s[t] = below[t];
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const v8 a = *reinterpret_cast<const v8*>(block + (c >> 2) * kHalfBytes + koff[c & 3]);
+#pragma unroll
+      for (int t = 0; t < kRT; ++t) s[t] = Elem<T>::mfma(a, q[t][c], s[t]);
+    }
+  }
+
+  static __device__ __forceinline__ float largest(const f32x16& s) {
+    float x = fmaxf(s[0], fmaxf(s[1], s[2]));
+#pragma unroll
+    for (int r = 3; r < 15; r += 2) x = fmaxf(fmaxf(x, s[r]), s[r + 1]);
+    return fmaxf(x, s[15]);
+  }
+
+  // Scores less their offsets.  The matrix products start from -m, so the difference costs nothing and is exact for near
+  // scores of any size.  Where an offset has to move, the scores are taken again from 0: what a far offset left of them
+  // may be coarse.  c: scale_log2.
+  __device__ __forceinline__ void offset_scores(f32x16 (&s)[kRT], const unsigned char* block, int at, int least, float c,
+                                                float inv_c, int lane) {
+    const bool some = at + kBlock > least;
+    auto hide = [&]() {
+      if (some)
+#pragma unroll
+        for (int t = 0; t < kRT; ++t) mask(s[t], t, at, lane);
+    };
+    scores(s, block, true);
+    hide();
+    bool over = false;
+#pragma unroll
+    for (int t = 0; t < kRT; ++t) over = over || largest(s[t]) >= thr[t];
+    if (__builtin_amdgcn_ballot_w64(over)) {
+      scores(s, block, false);
+      hide();
+#pragma unroll
+      for (int t = 0; t < kRT; ++t) {
+        const float top = over_pair(largest(s[t]), [](float x, float y) { return fmaxf(x, y); });
+        const bool fresh = thr[t] == -INFINITY, none = top == -INFINITY;  // no weight so far; none here
+        const float to = none ? m[t] : fmaxf(fresh ? -INFINITY : m[t], top - fminf(Elem<T>::kHead * inv_c, 1e30f));
+        const float f = fresh ? 0.f : __builtin_amdgcn_exp2f((m[t] - to) * c);
+        m[t] = to;
+        if (!none) thr[t] = fminf((Elem<T>::kHead + Elem<T>::kMargin) * inv_c, 1e30f);
+        l[t] *= f, lp[t] *= f;
+#pragma unroll
+        for (int j = 0; j < kOT; ++j) o[t][j] *= f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] -= to, below[t][r] = -to;
+      }
+    }
+  }
+
+  // Scores of keys that a row does not see; at: the block's first key.
+  __device__ __forceinline__ void mask(f32x16& s, int t, int at, int lane) const {
+    const int left = seen[t] - at - 4 * (lane >> 5);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 8 * (r / 4) + r % 4 < left ? s[r] : -INFINITY;
+  }
+
+  __device__ __forceinline__ v8 values(const unsigned char* v, int j, int c) const {
+    const unsigned char* const at = v + (j >> 1) * kHalfBytes + c * 16 * 128;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4*)(at + voff[j & 1][0]));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4*)(at + voff[j & 1][1]));
+    return __builtin_bit_cast(v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+
+  // Weights p of tile t as operands, and their sums.
+  __device__ __forceinline__ void split(const f32x16& p, int t, v8 (&part)[kParts][2], bool want_l) {
+    if (kParts > 1 || want_l) {
+      float a = p[0], b = p[1];
+#pragma unroll
+      for (int r = 2; r < 16; r += 2) a += p[r], b += p[r + 1];
+      l[t] += a + b;
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float x = p[8 * c + e];
+#pragma unroll
+        for (int n = 0; n < kParts; ++n) {
+          T y;
+          if (std::is_same_v<T, __bf16> && n + 1 < kParts)  // cut off: two operations less than rounding, and no part below 0
+            y = __builtin_bit_cast(T, (unsigned short)(__float_as_uint(x) >> 16));
+          else
+            y = (T)x;
+          part[n][c][e] = y;
+          if (n + 1 < kParts) x -= (float)y;
+        }
+      }
+    if (kParts == 1) {
+      float a = lp[t], b = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        a = Elem<T>::add2(v2{part[0][0][e], part[0][0][e + 1]}, a);
+        b = Elem<T>::add2(v2{part[0][1][e], part[0][1][e + 1]}, b);
+      }
+      lp[t] = a + b;
+    }
+  }
+
+  // O^T += V^T P^T.
+  __device__ __forceinline__ void output(const unsigned char* v, const v8 (&part)[kRT][kParts][2]) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int j = 0; j < kOT; ++j) {
+        const v8 a = values(v, j, c);
+#pragma unroll
+        for (int t = 0; t < kRT; ++t)
+#pragma unroll
+          for (int n = 0; n < kParts; ++n) o[t][j] = Elem<T>::mfma(a, part[t][n][c], o[t][j]);
+      }
+  }
+
+  // The same with float32 products that leave weights of 0 out.
+  __device__ __forceinline__ void output_exact(const unsigned char* v, const f32x16 (&p)[kRT], int lane) {
+    const int h = lane >> 5;
+#pragma unroll 1
+    for (int r = 0; r < 16; ++r) {
+      float both[kRT][2];
+#pragma unroll
+      for (int t = 0; t < kRT; ++t) {
+        float x = p[t][0];
+#pragma unroll
+        for (int u = 1; u < 16; ++u) x = r == u ? p[t][u] : x;
+        const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        both[t][0] = __uint_as_float(y[0]), both[t][1] = __uint_as_float(y[1]);
+        l[t] += x, lp[t] += x;
+      }
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const int key = 8 * (r / 4) + 4 * hh + r % 4;
+#pragma unroll
+        for (int j = 0; j < kOT; ++j)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int d = (32 * j + 8 * g) & 63;
+            typedef T v4 __attribute__((ext_vector_type(4)));
+            const v4 x = *reinterpret_cast<const v4*>(v + (j >> 1) * kHalfBytes + key * 128 + (((d >> 3) ^ swz_v(key)) << 4) + 8 * h);
+#pragma unroll
+            for (int t = 0; t < kRT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float y = both[t][hh];
+                o[t][j][4 * g + e] = y == 0.f ? o[t][j][4 * g + e] : fmaf(y, (float)x[e], o[t][j][4 * g + e]);
+              }
+          }
+      }
+    }
+  }
+
+  // One block; at: its first key; least: keys that every row of the wave sees.
+  template <bool kExact>
+  __device__ __forceinline__ void step(const unsigned char* block, int at, int least, float c, float inv_c, bool want_l,
+                                       int lane) {
+    f32x16 s[kRT];
+    offset_scores(s, block, at, least, c, inv_c, lane);
+#pragma unroll
+    for (int t = 0; t < kRT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[t][r] = __builtin_amdgcn_exp2f(s[t][r] * c);
+    if constexpr (kExact) {
+      output_exact(block + kDH * kHalfBytes, s, lane);
+    } else {
+      v8 part[kRT][kParts][2];
+#pragma unroll
+      for (int t = 0; t < kRT; ++t) split(s[t], t, part[t], want_l);
+      output(block + kDH * kHalfBytes, part);
+    }
+  }
+
+  // Whether some sum of the wave is NaN.
+  __device__ __forceinline__ bool any_nan() const {
+    float x = 0.f;
+#pragma unroll
+    for (int t = 0; t < kRT; ++t)
+#pragma unroll
+      for (int j = 0; j < kOT; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x = fmaf(o[t][j][r], 0.f, x);
+    return __builtin_amdgcn_ballot_w64(x != x) != 0;
+  }
+
+  // Into LDS: rows of 64 kDH floats, 16-byte piece c of row r at place c ^ r % pieces; statistics beside.
+  __device__ __forceinline__ void publish(unsigned char* rows, float* sm, float* sl, float* slp, int lane) const {
+    constexpr int kPieces = 16 * kDH;
+    const int i = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int t = 0; t < kRT; ++t) {
+      const int r = t * kBlock + i;
+      const float lt = over_pair(l[t], [](float x, float y) { return x + y; });
+      const float lpt = kParts == 1 ? over_pair(lp[t], [](float x, float y) { return x + y; }) : lt;
+#pragma unroll
+      for (int j = 0; j < kOT; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int c = 8 * j + 2 * g + h;
+          *reinterpret_cast<f32x4*>(rows + (r * kPieces + (c ^ (r % kPieces))) * 16) =
+              f32x4{o[t][j][4 * g], o[t][j][4 * g + 1], o[t][j][4 * g + 2], o[t][j][4 * g + 3]};
+        }
+      if (h == 0) sm[r] = thr[t] == -INFINITY ? -INFINITY : m[t], sl[r] = lt, slp[r] = lpt;
+    }
+  }
+};
+
+// A piece of work: rows [row0, row0 + 32 kRT or 128) of a job, blocks [first, last) of its keys.
+struct Job {
+  const void* q;                  // the job's first row; row r is r / G steps and r % G heads on
+  long long q_step, q_head;
+  Division by_group;
+  int G, row0, rows;              // rows: of the job
+  int seen, causal;               // row r sees the keys below seen (+ r / G + 1, causal)
+  int first, last;
+  float scale, scale_log2;
+  bool want_l;
+};
+
+// Where its rows go: the outputs, or (part) its part of them: D floats a row of sums, and of each row the offset and the
+// sums of weights.
+struct Sink {
+  void* o;
+  long long o_step, o_head;       // elements
+  float* lse;
+  long long l_step, l_head;
+  float* part;
+  int fill_to, fill;              // rows from Job::rows up to here get zeros (fill 1) or NaN (fill 2)
+};
+
+constexpr int few_lds(int kDH, int kRT, int stages) {
+  const int ring = kWaves * stages * 2 * kDH * kHalfBytes, rows = kWaves * kRT * kBlock * 64 * kDH * 4;
+  return ring > rows ? ring : rows;
+}
+constexpr int many_lds(int kDH, int stages) {
+  const int ring = stages * 4 * kDH * kHalfBytes, rows = kManyRows * 64 * kDH * 4;
+  return ring > rows ? ring : rows;
+}
+constexpr int kMaxRows = kWaves * 2 * kBlock;  // of statistics: four waves of 64 rows
+
+struct Stats {
+  float m[kMaxRows], l[kMaxRows], lp[kMaxRows];
+};
+
+template <class T, int kDH, int kRT, int kParts>
+__device__ __forceinline__ void load_rows(State<T, kDH, kRT, kParts>& w, const Job& job, int first, int D, int lane) {
+  typedef typename Elem<T>::v8 v8;
+  const int i = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int t = 0; t < kRT; ++t) {
+    const int r = first + t * kBlock + i, step = divide(r, job.by_group);
+    const T* const at = static_cast<const T*>(job.q) + step * job.q_step + (r - step * job.G) * job.q_head;
+    w.seen[t] = r < job.rows ? job.seen + (job.causal ? step + 1 : 0) : 0;
+#pragma unroll
+    for (int c = 0; c < 4 * kDH; ++c) {
+      const int d = 16 * c + 8 * h;
+      w.q[t][c] = __builtin_bit_cast(v8, u32x4{0, 0, 0, 0});
+      if (r < job.rows && d < D) w.q[t][c] = *reinterpret_cast<const v8*>(at + d);
+    }
+    // Here, before the loop: the waits that the compiler places for these loads would empty the pipeline of direct ones.
+#pragma unroll
+    for (int c = 0; c < 4 * kDH; ++c) asm volatile("" ::"v"(w.q[t][c]));
+  }
+}
+
+// Row `row` of the workgroup's kRows rows, 8 dims from 8 c8 on, joined over kJoin waves' states (stride: rows apart), to its
+// place.
+template <class T, int kDH, int kJoin>
+__device__ __forceinline__ void put(const unsigned char* rows, const Stats& st, int stride, int row, int c8, const Job& job,
+                                    const Sink& to, int D, int kRows) {
+  constexpr int kPieces = 16 * kDH;
+  const int r = job.row0 + row;
+  const bool real = r < job.rows;
+  if (!real && !(to.part == nullptr && to.fill != 0 && r < to.fill_to)) return;
+  float M = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kJoin; ++w) M = fmaxf(M, st.m[w * stride + row]);
+  float l = 0.f, lp = 0.f;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < kJoin; ++w) {
+    const int at = w * stride + row;
+    const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((st.m[at] - M) * job.scale_log2);
+    l = fmaf(f, st.l[at], l), lp = fmaf(f, st.lp[at], lp);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(rows + (at * kPieces + ((2 * c8) ^ (at % kPieces))) * 16);
+    const f32x4 y = *reinterpret_cast<const f32x4*>(rows + (at * kPieces + ((2 * c8 + 1) ^ (at % kPieces))) * 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {  // (a wave without weight has no sums; its offset may be NaN's)
+      a[e] = f == 0.f ? a[e] : fmaf(f, x[e], a[e]);
+      b[e] = f == 0.f ? b[e] : fmaf(f, y[e], b[e]);
+    }
+  }
+  if (to.part) {
+    float* const at = to.part + (long long)row * D + 8 * c8;
+    *reinterpret_cast<f32x4*>(at) = a;
+    *reinterpret_cast<f32x4*>(at + 4) = b;
+    if (c8 == 0) {
+      float* const stats = to.part + (long long)kRows * D + row;
+      stats[0] = M, stats[kRows] = l, stats[2 * kRows] = lp;
+    }
+    return;
+  }
+  const int step = divide(r, job.by_group), head = r - step * job.G;
+  const float nan = __uint_as_float(0x7FC00000u);
+  const float inv = lp == 0.f ? 0.f : 1.f / lp;
+  typename Elem<T>::v8 out;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    out[e] = (T)(real ? (lp == 0.f ? 0.f : a[e] * inv) : to.fill == 2 ? nan : 0.f);
+    out[4 + e] = (T)(real ? (lp == 0.f ? 0.f : b[e] * inv) : to.fill == 2 ? nan : 0.f);
+  }
+  *reinterpret_cast<typename Elem<T>::v8*>(static_cast<T*>(to.o) + step * to.o_step + head * to.o_head + 8 * c8) = out;
+  if (c8 == 0 && to.lse)
+    to.lse[step * to.l_step + head * to.l_head] =
+        !real ? (to.fill == 2 ? nan : -INFINITY) : l == 0.f ? -INFINITY : fmaf(M, job.scale, log2f(l) * kLn2);
+}
+
+// Few rows.
+template <class T, int kDH, bool kAligned, int kRT, int kStages>
+__device__ __forceinline__ void run_few(const Source& src, const Job& job, const Sink& to, int D, unsigned char* lds, Stats& st) {
+  constexpr int kLoads = 8 * kDH;                       // transfers of a block
+  constexpr int kBytes = 2 * kDH * kHalfBytes;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  unsigned char* const ring = lds + wave * kStages * kBytes;
+  const uint32_t ring_at = tfgfa::lds_addr(ring);
+  const int count = max(0, (job.last - job.first - wave + kWaves - 1) / kWaves);
+  auto key = [&](int n) { return (job.first + wave + n * kWaves) * kBlock; };
+  State<T, kDH, kRT, 2> w;
+  const float inv = 1.f / job.scale_log2;
+  w.init(lane);
+  Loader<kDH, kAligned, 4> in;
+  in.init(src, D, 0, lane);
+  auto pass = [&](auto exact) {
+    if (count > 0) in.look_up(src, key(0));
+#pragma unroll
+    for (int n = 0; n < kStages - 1; ++n)
+      if (n < count) {
+        in.issue(src, key(n), ring_at + n * kBytes);
+        if (n + 1 < count) in.look_up(src, key(n + 1));
+      }
+    if (!decltype(exact)::value) load_rows(w, job, job.row0, D, lane);
+    const int least = job.causal ? job.seen + divide(job.row0, job.by_group) + 1 : job.seen;
+    int stage = 0;
+#pragma unroll 1
+    for (int n = 0; n < count; ++n) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of the stage that is filled next
+      if (n + kStages - 1 < count) {
+        in.issue(src, key(n + kStages - 1), ring_at + (stage == 0 ? kStages - 1 : stage - 1) * kBytes);
+        if (n + kStages < count) in.look_up(src, key(n + kStages));
+        tfgfa::wait_vmcnt<(kStages - 1) * kLoads>();
+      } else {
+        tfgfa::wait_vmcnt<0>();
+      }
+      w.template step<decltype(exact)::value>(ring + stage * kBytes, key(n), least, job.scale_log2, inv, true, lane);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
+  pass(std::false_type());
+  if (w.any_nan()) {
+    w.clear();
+    pass(std::true_type());
+  }
+  constexpr int kRows = kRT * kBlock;
+  __syncthreads();  // (the rows' places are the rings')
+  w.publish(lds + wave * kRows * 64 * kDH * 4, st.m + wave * kRows, st.l + wave * kRows, st.lp + wave * kRows, lane);
+  __syncthreads();
+  for (int e = tid; e < kRows * 8 * kDH; e += kThreads)
+    if (e % (8 * kDH) * 8 < D) put<T, kDH, kWaves>(lds, st, kRows, e / (8 * kDH), e % (8 * kDH), job, to, D, kRows);
+}
+
+// Many rows.
+template <class T, int kDH, bool kAligned, int kParts, int kStages>
+__device__ __forceinline__ void run_many(const Source& src, const Job& job, const Sink& to, int D, unsigned char* lds, Stats& st) {
+  constexpr int kLoads = 4 * kDH;                       // transfers of a wave and tile
+  constexpr int kBytes = 2 * kDH * kHalfBytes;          // of a block
+  __shared__ int sh_nan;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const uint32_t ring_at = tfgfa::lds_addr(lds);
+  const int tiles = (job.last - job.first + 1) / 2;
+  auto key = [&](int n) { return job.first * kBlock + n * kTile; };
+  State<T, kDH, 1, kParts> w;
+  const float inv = 1.f / job.scale_log2;
+  w.init(lane);
+  if (tid == 0) sh_nan = 0;
+  Loader<kDH, kAligned, 2> in;                          // 16 keys of a tile: half a block
+  in.init(src, D, (wave & 1) * 2, lane);
+  const int mine = (wave >> 1) * kBlock;                // the block's first key in the tile
+  const int r0 = job.row0 + wave * kBlock, r1 = min(job.rows, r0 + kBlock) - 1;
+  const int least = r0 >= job.rows ? 0 : job.causal ? job.seen + divide(r0, job.by_group) + 1 : job.seen;
+  const int most = r0 >= job.rows ? 0 : job.causal ? job.seen + divide(r1, job.by_group) + 1 : job.seen;
+  auto issue = [&](int n, int stage) {
+    in.issue(src, key(n) + mine, ring_at + (2 * stage + (wave >> 1)) * kBytes);
+    if (n + 1 < tiles) in.look_up(src, key(n + 1) + mine);
+  };
+  auto pass = [&](auto exact) {
+    if (tiles > 0) in.look_up(src, key(0) + mine);
+#pragma unroll
+    for (int n = 0; n < kStages - 1; ++n)
+      if (n < tiles) issue(n, n);
+    if (!decltype(exact)::value) load_rows(w, job, r0, D, lane);
+    int stage = 0;
+#pragma unroll 1
+    for (int n = 0; n < tiles; ++n) {
+      if (n + kStages - 2 < tiles && kStages > 2)
+        tfgfa::wait_vmcnt<(kStages - 2) * kLoads>();
+      else
+        tfgfa::wait_vmcnt<0>();
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (n + kStages - 1 < tiles) issue(n + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int at = key(n) + b * kBlock;
+        if (at < most)
+          w.template step<decltype(exact)::value>(lds + (2 * stage + b) * kBytes, at, least, job.scale_log2, inv, job.want_l, lane);
+      }
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  pass(std::false_type());
+  if (w.any_nan() && lane == 0) sh_nan = 1;
+  __syncthreads();
+  if (uniform(sh_nan)) {
+    w.clear();
+    pass(std::true_type());
+  }
+  w.publish(lds + wave * kBlock * 64 * kDH * 4, st.m + wave * kBlock, st.l + wave * kBlock, st.lp + wave * kBlock, lane);
+  __syncthreads();
+  for (int e = tid; e < kManyRows * 8 * kDH; e += kThreads)
+    if (e % (8 * kDH) * 8 < D) put<T, kDH, 1>(lds, st, 0, e / (8 * kDH), e % (8 * kDH), job, to, D, kManyRows);
+}
+
+// ---------------------------------------------------------------------------------------
+// Joining the parts of a job's rows: 16 lanes a row, 8 dims a lane.
+
+constexpr int kLanes = kMaxD / 8;
+constexpr int kMine = kMaxParts / kLanes;  // parts whose statistics a lane has
+constexpr int kAtOnce = 4;                 // parts whose sums are loaded together (divides kLanes)
+
+// A row's parts: `count` of them, `stride` floats apart, the sums of part 0 at `sums` (this lane's dims) and its offset at
+// `stats` (the sums of weights kRows and 2 kRows further).
+struct Parts {
+  const float* sums;
+  const float* stats;
+  long long stride;
+  int count, rows;
+};
+__device__ __forceinline__ Parts parts_of(const float* part, long long job, int count, int rows, int row, int D, int c8) {
+  const long long stride = (long long)rows * (D + 3);
+  const float* const at = part + job * count * stride;
+  return {at + (long long)row * D + 8 * c8, at + (long long)rows * D + row, stride, count, rows};
+}
+
+template <class F>
+__device__ __forceinline__ float over_lanes(float x, F f) {
+#pragma unroll
+  for (int n = kLanes / 2; n > 0; n /= 2) x = f(x, __shfl_xor(x, n, kLanes));
+  return x;
+}
+
+struct Joined {
+  f32x4 a, b;
+  float M, l, lp;
+};
+
+// The sum over kSources lists of parts; c: the lane of the row.  (Dims past D: any that are there.)
+template <int kSources>
+__device__ __forceinline__ Joined join(const Parts (&from)[kSources], int c, float scale_log2) {
+  Joined y = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}, -INFINITY, 0.f, 0.f};
+  float f[kSources][kMine], l[kSources][kMine], lp[kSources][kMine];
+#pragma unroll
+  for (int n = 0; n < kSources; ++n)
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int s = i * kLanes + c;
+      const float* const at = from[n].stats + s * from[n].stride;
+      const bool in = s < from[n].count;
+      f[n][i] = in ? at[0] : -INFINITY;
+      l[n][i] = in ? at[from[n].rows] : 0.f;
+      lp[n][i] = in ? at[2 * from[n].rows] : 0.f;
+      y.M = fmaxf(y.M, f[n][i]);
+    }
+  y.M = over_lanes(y.M, [](float u, float v) { return fmaxf(u, v); });
+#pragma unroll
+  for (int n = 0; n < kSources; ++n)
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      f[n][i] = f[n][i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((f[n][i] - y.M) * scale_log2);
+      y.l = fmaf(f[n][i], l[n][i], y.l), y.lp = fmaf(f[n][i], lp[n][i], y.lp);
+    }
+  y.l = over_lanes(y.l, [](float u, float v) { return u + v; });
+  y.lp = over_lanes(y.lp, [](float u, float v) { return u + v; });
+#pragma unroll
+  for (int n = 0; n < kSources; ++n)
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int here = min(kLanes, from[n].count - i * kLanes);
+      const float* const first = from[n].sums + i * kLanes * from[n].stride;
+      for (int s0 = 0; s0 < here; s0 += kAtOnce) {
+        f32x4 u[kAtOnce], v[kAtOnce];
+        float w[kAtOnce];
+#pragma unroll
+        for (int s = 0; s < kAtOnce; ++s) {
+          const float* const at = first + min(s0 + s, here - 1) * from[n].stride;
+          u[s] = *reinterpret_cast<const f32x4*>(at), v[s] = *reinterpret_cast<const f32x4*>(at + 4);
+          w[s] = __shfl(f[n][i], s0 + s, kLanes);  // (past `here` there is a weight of 0: no part)
+        }
+#pragma unroll
+        for (int s = 0; s < kAtOnce; ++s)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y.a[e] = w[s] == 0.f ? y.a[e] : fmaf(w[s], u[s][e], y.a[e]);
+            y.b[e] = w[s] == 0.f ? y.b[e] : fmaf(w[s], v[s][e], y.b[e]);
+          }
+      }
+    }
+  return y;
+}
+
+template <class T>
+__device__ __forceinline__ void store_row(T* to, const Joined& y, bool zero, bool nan) {
+  const float inv = y.lp == 0.f ? 0.f : 1.f / y.lp, bad = __uint_as_float(0x7FC00000u);
+  typename Elem<T>::v8 out;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    out[e] = (T)(nan ? bad : zero || y.lp == 0.f ? 0.f : y.a[e] * inv);
+    out[4 + e] = (T)(nan ? bad : zero || y.lp == 0.f ? 0.f : y.b[e] * inv);
+  }
+  *reinterpret_cast<typename Elem<T>::v8*>(to) = out;
+}
+__device__ __forceinline__ float row_lse(const Joined& y, float scale, bool zero, bool nan) {
+  return nan ? __uint_as_float(0x7FC00000u) : zero || y.l == 0.f ? -INFINITY : fmaf(y.M, scale, log2f(y.l) * kLn2);
+}
+
+// ---------------------------------------------------------------------------------------
+// New tokens of each sequence.
+
+struct AttendArgs {
+  const void* q;
+  void* o;
+  float* lse;
+  float* part;
+  const char* k;
+  const char* v;
+  Pages ks, vs;
+  Rows qs, os;
+  const int* table;
+  long long table_stride;
+  const int* lens;
+  const int* lengths;
+  Division by_page, by_group;
+  int page, P, n_max, N, G, Hkv, heads, D, causal, pad, tiles, parts;
+  float scale, scale_log2;
+};
+
+// How many rows a workgroup takes, and how.
+enum class Kind { kFew1, kFew2, kMany };
+__host__ __device__ constexpr int rows_of(Kind kind) {
+  return kind == Kind::kFew1 ? kBlock : kind == Kind::kFew2 ? 2 * kBlock : kManyRows;
+}
+constexpr int kFewStages = 2, kManyStages = 2;
+constexpr int lds_of(Kind kind, int kDH) {
+  return kind == Kind::kMany ? many_lds(kDH, kManyStages) : few_lds(kDH, kind == Kind::kFew1 ? 1 : 2, kFewStages);
+}
+
+template <class T, int kDH, bool kAligned, Kind kKind, int kParts>
+__device__ __forceinline__ void run(const Source& src, const Job& job, const Sink& to, int D, unsigned char* lds, Stats& st) {
+  if constexpr (kKind == Kind::kMany)
+    run_many<T, kDH, kAligned, kParts, kManyStages>(src, job, to, D, lds, st);
+  else
+    run_few<T, kDH, kAligned, kKind == Kind::kFew1 ? 1 : 2, kFewStages>(src, job, to, D, lds, st);
+}
+
+// Part s of S of `blocks` blocks: whole rounds of the workgroup.
+template <Kind kKind>
+__device__ __forceinline__ void share(Job* job, int blocks, int s, int S) {
+  constexpr int kRound = kKind == Kind::kMany ? 2 : kWaves;
+  const int rounds = (blocks + kRound - 1) / kRound;
+  job->first = kRound * (int)((long long)rounds * s / S);
+  job->last = min(blocks, kRound * (int)((long long)rounds * (s + 1) / S));
+}
+
+template <class T, int kDH, bool kAligned, Kind kKind>
+__global__ __launch_bounds__(kThreads) void attend_kernel(const AttendArgs a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[lds_of(kKind, kDH)];
+  __shared__ Stats st;
+  constexpr int kRows = rows_of(kKind);
+  // The longest first (the last tiles of a causal sequence); a key-value head's workgroups on one XCD where 8 divides
+  // their number.
+  const int idx = blockIdx.x, rest = idx / a.heads, head = idx - rest * a.heads;
+  const int from_end = rest / a.parts, s = rest - from_end * a.parts, tile = a.tiles - 1 - from_end;
+  const int b = head / a.Hkv, kv = head - b * a.Hkv;
+  const int len = ((uniform_ints)a.lens)[b], n = a.lengths ? ((uniform_ints)a.lengths)[b] : a.N;
+  const bool fits = len >= 0 && n >= 0 && n <= a.N && (long long)len + (a.causal ? n : 0) <= a.n_max;
+  const long long first_head = (long long)kv * a.G;
+  Job job;
+  job.q = static_cast<const T*>(a.q) + b * a.qs.b + first_head * a.qs.h;
+  job.q_step = a.qs.n, job.q_head = a.qs.h;
+  job.by_group = a.by_group, job.G = a.G, job.row0 = tile * kRows, job.rows = fits ? n * a.G : 0;
+  job.seen = fits ? len : 0, job.causal = a.causal;
+  job.scale = a.scale, job.scale_log2 = a.scale_log2, job.want_l = a.lse != nullptr;
+  const int top = min(job.rows, job.row0 + kRows) - 1;
+  const int keys = job.row0 >= job.rows ? 0 : a.causal ? len + divide(top, a.by_group) + 1 : len;
+  share<kKind>(&job, (keys + kBlock - 1) / kBlock, s, a.parts);
+  const Source src = {a.k + kv * a.ks.h, a.v + kv * a.vs.h, a.ks, a.vs, a.table + b * a.table_stride, a.by_page, a.page, a.P, keys};
+  const long long unit = (long long)head * a.tiles + tile;
+  Sink to;
+  to.o = static_cast<T*>(a.o) + b * a.os.b + first_head * a.os.h;
+  to.o_step = a.os.n, to.o_head = a.os.h;
+  to.lse = a.lse ? a.lse + ((long long)b * a.Hkv * a.G + first_head) * a.N : nullptr;
+  to.l_step = 1, to.l_head = a.N;
+  to.part = a.parts > 1 ? a.part + (unit * a.parts + s) * kRows * (a.D + 3) : nullptr;
+  to.fill_to = a.N * a.G, to.fill = !fits ? 2 : a.pad;
+  run<T, kDH, kAligned, kKind, 1>(src, job, to, a.D, lds, st);
+}
+
+template <class T, Kind kKind>
+__global__ __launch_bounds__(kThreads) void attend_join_kernel(const AttendArgs a) {
+  constexpr int kRows = rows_of(kKind), kEach = kThreads / kLanes;
+  const int c = threadIdx.x % kLanes;
+  const int unit = blockIdx.x / (kRows / kEach), row = (int)(blockIdx.x % (kRows / kEach)) * kEach + (int)threadIdx.x / kLanes;
+  const int head = unit / a.tiles, tile = unit - head * a.tiles, b = head / a.Hkv, kv = head - b * a.Hkv;
+  const int r = tile * kRows + row, step = divide(r, a.by_group), h = kv * a.G + r - step * a.G;
+  if (step >= a.N) return;
+  const int len = a.lens[b], n = a.lengths ? a.lengths[b] : a.N;
+  const bool fits = len >= 0 && n >= 0 && n <= a.N && (long long)len + (a.causal ? n : 0) <= a.n_max;
+  const bool past = fits && step >= n;
+  if (past && !a.pad) return;
+  const bool real = fits && !past;
+  const int d = 8 * c < a.D ? c : 0;
+  Parts p[1] = {parts_of(a.part, unit, a.parts, kRows, row, a.D, d)};
+  if (!real) p[0].count = 0;
+  const Joined y = join(p, c, a.scale_log2);
+  if (8 * c < a.D) store_row(static_cast<T*>(a.o) + b * a.os.b + h * a.os.h + step * a.os.n + 8 * c, y, past, !fits);
+  if (c == 0 && a.lse) a.lse[((long long)b * a.Hkv * a.G + h) * a.N + step] = row_lse(y, a.scale, past, !fits);
+}
+
+// ---------------------------------------------------------------------------------------
+// A decode step of sequences that share a prefix.
+
+struct SharedArgs {
+  const void* q;
+  void* o;
+  float* lse;
+  float* prefix_part;
+  float* own_part;
+  char* k;
+  char* v;
+  const void* kn;
+  const void* vn;
+  Pages ks, vs;
+  Vecs qs, os, kns, vns;
+  const int* prefix_table;
+  const int* prefix_lens;
+  const int* table;
+  const int* lens;
+  long long prefix_stride, table_stride;
+  Division by_page, by_group;
+  int page, P, prefix_max, n_max, G, Hkv, R, each, D;   // each: sequences of a group
+  int prefix_heads, prefix_tiles, prefix_parts, prefix_jobs;
+  int own_heads, own_tiles, own_parts;
+  float scale, scale_log2;
+};
+
+template <class T, int kDH, bool kAligned, Kind kKind>
+__global__ __launch_bounds__(kThreads) void shared_kernel(const SharedArgs a) {
+  constexpr int kPrefixLds = lds_of(kKind, kDH), kOwnLds = lds_of(Kind::kFew1, kDH);
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[kPrefixLds > kOwnLds ? kPrefixLds : kOwnLds];
+  __shared__ Stats st;
+  Job job;
+  Sink to;
+  job.by_group = a.by_group, job.G = a.G, job.causal = 0;
+  job.q_step = a.qs.b, job.q_head = a.qs.h;
+  job.scale = a.scale, job.scale_log2 = a.scale_log2, job.want_l = true;
+  to.o = nullptr, to.o_step = to.o_head = 0, to.lse = nullptr, to.l_step = to.l_head = 0, to.fill_to = to.fill = 0;
+  const bool prefix = (int)blockIdx.x < a.prefix_jobs;
+  const int idx = prefix ? blockIdx.x : blockIdx.x - a.prefix_jobs;
+  const int heads = prefix ? a.prefix_heads : a.own_heads, parts = prefix ? a.prefix_parts : a.own_parts;
+  const int rest = idx / heads, head = idx - rest * heads, tile = rest / parts, s = rest - tile * parts;
+  const int b = head / a.Hkv, kv = head - b * a.Hkv;   // group or sequence
+  Source src = {a.k + kv * a.ks.h, a.v + kv * a.vs.h, a.ks, a.vs, nullptr, a.by_page, a.page, a.P, 0};
+  const long long first_head = (long long)kv * a.G;
+  if (prefix) {
+    constexpr int kRows = rows_of(kKind);
+    const int len = ((uniform_ints)a.prefix_lens)[b];
+    src.table = a.prefix_table + b * a.prefix_stride;
+    src.keys = len >= 0 && len <= a.prefix_max ? len : 0;
+    job.q = static_cast<const T*>(a.q) + (long long)b * a.each * a.qs.b + first_head * a.qs.h;
+    job.row0 = tile * kRows, job.rows = a.each * a.G, job.seen = src.keys;
+    share<kKind>(&job, (src.keys + kBlock - 1) / kBlock, s, parts);
+    to.part = a.prefix_part + (((long long)head * a.prefix_tiles + tile) * parts + s) * kRows * (a.D + 3);
+    run<T, kDH, kAligned, kKind, 2>(src, job, to, a.D, lds, st);
+  } else {
+    constexpr int kRows = rows_of(Kind::kFew1);
+    const int append = a.kn != nullptr, len = ((uniform_ints)a.lens)[b];
+    const bool fits = len >= 0 && len <= a.n_max - append;
+    src.table = a.table + b * a.table_stride;
+    src.keys = fits ? len + append : 0;
+    // The new row goes to its page first; this workgroup alone reads it (or another with rows of the same head, which
+    // writes the same bytes before it reads them).
+    if (append && fits && s == parts - 1) {
+      const int at = divide(len, a.by_page), id = ((uniform_ints)src.table)[at], tid = threadIdx.x;
+      const bool value = tid >= kMaxD / 8;
+      const int c = value ? tid - kMaxD / 8 : tid;
+      if ((uint32_t)id < (uint32_t)a.P && 8 * c < a.D && tid < kMaxD / 4) {
+        const Pages& ps = value ? a.vs : a.ks;
+        const T* const from = value ? static_cast<const T*>(a.vn) + b * a.vns.b + kv * a.vns.h
+                                    : static_cast<const T*>(a.kn) + b * a.kns.b + kv * a.kns.h;
+        char* const row = (value ? a.v : a.k) + kv * ps.h + (uint64_t)(uint32_t)id * (uint64_t)ps.p + (uint64_t)(len - at * a.page) * (uint64_t)ps.n;
+        *reinterpret_cast<u32x4*>(row + 16 * c) = *reinterpret_cast<const u32x4*>(from + 8 * c);
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+    }
+    job.q = static_cast<const T*>(a.q) + b * a.qs.b + first_head * a.qs.h;
+    job.row0 = tile * kRows, job.rows = a.G, job.seen = src.keys;
+    share<Kind::kFew1>(&job, (src.keys + kBlock - 1) / kBlock, s, parts);
+    to.part = a.own_part + (((long long)head * a.own_tiles + tile) * parts + s) * kRows * (a.D + 3);
+    run<T, kDH, kAligned, Kind::kFew1, 2>(src, job, to, a.D, lds, st);
+  }
+}
+
+template <class T, Kind kKind>
+__global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs a, int rows) {
+  constexpr int kRows = rows_of(kKind);
+  const int c = threadIdx.x % kLanes, at = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  if (at >= rows) return;
+  const int H = a.Hkv * a.G, b = at / H, h = at - b * H, kv = h / a.G, g = h - kv * a.G, r = b / a.each;
+  const int plen = a.prefix_lens[r], len = a.lens[b];
+  const bool fits = plen >= 0 && plen <= a.prefix_max && len >= 0 && len <= a.n_max - (a.kn ? 1 : 0);
+  const int d = 8 * c < a.D ? c : 0;
+  const int row = (b - r * a.each) * a.G + g;
+  Parts p[2] = {
+      parts_of(a.prefix_part, ((long long)r * a.Hkv + kv) * a.prefix_tiles + row / kRows, a.prefix_parts, kRows, row % kRows, a.D, d),
+      parts_of(a.own_part, ((long long)b * a.Hkv + kv) * a.own_tiles + g / kBlock, a.own_parts, kBlock, g % kBlock, a.D, d)};
+  const Joined y = join(p, c, a.scale_log2);
+  if (8 * c < a.D) store_row(static_cast<T*>(a.o) + b * a.os.b + h * a.os.h + 8 * c, y, false, !fits);
+  if (c == 0 && a.lse) a.lse[at] = row_lse(y, a.scale, false, !fits);
+}
+
+// ---------------------------------------------------------------------------------------
+// Host side.
+
+constexpr int kCu = 256;  // workgroups are counted for this many CUs, so that a workspace's size does not depend on the device
+
+static Kind choose_kind(long long rows) {
+  return rows <= kBlock ? Kind::kFew1 : rows <= 2 * kBlock ? Kind::kFew2 : Kind::kMany;
+}
+// Workgroups that a job of up to n_max keys is divided over, where there are `jobs` of them.
+static int choose_parts(Kind kind, long long jobs, long long n_max) {
+  const long long least = kind == Kind::kMany ? 512 : 256;  // keys of a part
+  const long long want = 2 * kCu / std::max(1LL, jobs), most = n_max / least;
+  return (int)std::max(1LL, std::min({want, most, (long long)kMaxParts}));
+}
+static size_t part_bytes(Kind kind, long long jobs, int parts, int D) {
+  return ((size_t)jobs * parts * rows_of(kind) * (D + 3) * 4 + 255) / 256 * 256;
+}
+
+static bool heads_ok(int B, int H, int Hkv, int page, int M) {
+  if (B < 0 || H < 0 || Hkv < 0 || page < 1 || M < 0) return false;
+  return Hkv == 0 ? H == 0 : H % Hkv == 0;
+}
+
+struct AttendPlan {
+  Kind kind;
+  long long tiles, jobs;
+  int parts;
+  size_t bytes;
+};
+// False: too large.
+static bool attend_plan(int B, int H, int Hkv, int N, int page, int M, int D, AttendPlan* x) {
+  const long long n_max = (long long)M * page, rows = (long long)N * (H / Hkv);
+  if (n_max > INT32_MAX - (1 << 20) || rows > INT32_MAX - kManyRows || (long long)B * Hkv > INT32_MAX) return false;
+  x->kind = choose_kind(rows);
+  const int each = rows_of(x->kind);
+  x->tiles = (rows + each - 1) / each;
+  if (x->tiles > INT32_MAX / ((long long)B * Hkv)) return false;
+  x->jobs = x->tiles * B * Hkv;
+  x->parts = choose_parts(x->kind, x->jobs, n_max);
+  x->bytes = x->parts > 1 ? part_bytes(x->kind, x->jobs, x->parts, D) : 0;
+  return x->jobs * x->parts <= INT32_MAX && x->jobs <= INT32_MAX / kManyRows;
+}
+
+template <class T, int kDH, bool kAligned>
+static void launch_attend(const AttendArgs& a, const AttendPlan& x, hipStream_t stream) {
+  const dim3 grid((unsigned)(x.jobs * x.parts));
+  if (x.kind == Kind::kFew1)
+    hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kFew1>), grid, dim3(kThreads), 0, stream, a);
+  else if (x.kind == Kind::kFew2)
+    hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kFew2>), grid, dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kMany>), grid, dim3(kThreads), 0, stream, a);
+}
+template <class T>
+static hipError_t launch_attend(const AttendArgs& a, const AttendPlan& x, hipStream_t stream) {
+  const bool aligned = a.page % kGroup == 0;
+  if (a.D <= 64)
+    aligned ? launch_attend<T, 1, true>(a, x, stream) : launch_attend<T, 1, false>(a, x, stream);
+  else
+    aligned ? launch_attend<T, 2, true>(a, x, stream) : launch_attend<T, 2, false>(a, x, stream);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || x.parts == 1) return e;
+  const dim3 grid((unsigned)(x.jobs * (rows_of(x.kind) / (kThreads / kLanes))));
+  if (x.kind == Kind::kFew1)
+    hipLaunchKernelGGL((attend_join_kernel<T, Kind::kFew1>), grid, dim3(kThreads), 0, stream, a);
+  else if (x.kind == Kind::kFew2)
+    hipLaunchKernelGGL((attend_join_kernel<T, Kind::kFew2>), grid, dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((attend_join_kernel<T, Kind::kMany>), grid, dim3(kThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+struct SharedPlan {
+  Kind kind;
+  long long prefix_tiles, prefix_jobs, own_tiles, own_jobs;  // jobs: without their parts
+  int prefix_parts, own_parts;
+  size_t own_at, bytes;
+};
+static bool shared_plan(int R, int B, int H, int Hkv, int page, int Mp, int M, int D, SharedPlan* x) {
+  const long long n_max = (long long)M * page, p_max = (long long)Mp * page, G = H / Hkv, rows = B / R * G;
+  if (n_max > INT32_MAX - (1 << 20) || p_max > INT32_MAX - (1 << 20) || rows > INT32_MAX - kManyRows ||
+      (long long)B * H > INT32_MAX - kThreads)
+    return false;
+  x->kind = choose_kind(rows);
+  x->prefix_tiles = (rows + rows_of(x->kind) - 1) / rows_of(x->kind);
+  x->own_tiles = (G + kBlock - 1) / kBlock;
+  x->prefix_jobs = x->prefix_tiles * R * Hkv;
+  x->own_jobs = x->own_tiles * B * Hkv;
+  x->prefix_parts = choose_parts(x->kind, x->prefix_jobs, p_max);
+  x->own_parts = choose_parts(Kind::kFew1, x->own_jobs, n_max);
+  x->own_at = part_bytes(x->kind, x->prefix_jobs, x->prefix_parts, D);
+  x->bytes = x->own_at + part_bytes(Kind::kFew1, x->own_jobs, x->own_parts, D);
+  return x->prefix_jobs * x->prefix_parts + x->own_jobs * x->own_parts <= INT32_MAX;
+}
+
+template <class T, int kDH, bool kAligned>
+static void launch_shared(const SharedArgs& a, const SharedPlan& x, hipStream_t stream) {
+  const dim3 grid((unsigned)(x.prefix_jobs * x.prefix_parts + x.own_jobs * x.own_parts));
+  if (x.kind == Kind::kFew1)
+    hipLaunchKernelGGL((shared_kernel<T, kDH, kAligned, Kind::kFew1>), grid, dim3(kThreads), 0, stream, a);
+  else if (x.kind == Kind::kFew2)
+    hipLaunchKernelGGL((shared_kernel<T, kDH, kAligned, Kind::kFew2>), grid, dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((shared_kernel<T, kDH, kAligned, Kind::kMany>), grid, dim3(kThreads), 0, stream, a);
+}
+template <class T>
+static hipError_t launch_shared(const SharedArgs& a, const SharedPlan& x, int rows, hipStream_t stream) {
+  const bool aligned = a.page % kGroup == 0;
+  if (a.D <= 64)
+    aligned ? launch_shared<T, 1, true>(a, x, stream) : launch_shared<T, 1, false>(a, x, stream);
+  else
+    aligned ? launch_shared<T, 2, true>(a, x, stream) : launch_shared<T, 2, false>(a, x, stream);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const dim3 grid((rows + kThreads / kLanes - 1) / (kThreads / kLanes));
+  if (x.kind == Kind::kFew1)
+    hipLaunchKernelGGL((shared_join_kernel<T, Kind::kFew1>), grid, dim3(kThreads), 0, stream, a, rows);
+  else if (x.kind == Kind::kFew2)
+    hipLaunchKernelGGL((shared_join_kernel<T, Kind::kFew2>), grid, dim3(kThreads), 0, stream, a, rows);
+  else
+    hipLaunchKernelGGL((shared_join_kernel<T, Kind::kMany>), grid, dim3(kThreads), 0, stream, a, rows);
+  return hipGetLastError();
+}
+
+// A pool's rows of a transfer are one buffer of less than 2^30 bytes.
+static bool rows_fit(const Pages& st) { return st.n < (1 << 30) / kGroup; }
+
+}  // namespace tfgfa_context
+
+extern "C" size_t tfpages_attend_workspace(int B, int H, int H_kv, int N, int page, int M, int D) {
+  using namespace tfgfa_context;
+  if (!heads_ok(B, H, H_kv, page, M) || N < 0 || D < 8 || D > kMaxD || (D & 7)) return 0;
+  if (B == 0 || H == 0 || N == 0) return 0;
+  AttendPlan x;
+  return attend_plan(B, H, H_kv, N, page, M, D, &x) ? x.bytes : 0;
+}
+
+extern "C" int tfpages_attend(const void* q, const int64_t* q_strides, const void* k_pages, const int64_t* k_strides,
+                              const void* v_pages, const int64_t* v_strides, const int* page_table,
+                              int64_t table_stride, const int* cache_seqlens, const int* lengths, void* o,
+                              const int64_t* o_strides, float* lse, int pad, int causal, int B, int H, int H_kv,
+                              int N, int P, int page, int M, int D, int dtype, float softmax_scale, void* workspace,
+                              size_t workspace_bytes, void* hip_stream) {
+  using namespace tfgfa_context;
+  if (dtype != TFGFA_DTYPE_BF16 && dtype != TFGFA_DTYPE_F16) return TFGFA_ERR_DTYPE;
+  if (!heads_ok(B, H, H_kv, page, M) || N < 0 || P < 0) return TFGFA_ERR_BAD_SHAPE;
+  if (D < 8 || D > kMaxD || (D & 7)) return TFGFA_ERR_HEAD_DIM;
+  if (!(softmax_scale > 0.f) || !isfinite(softmax_scale)) return TFGFA_ERR_SCALE;
+  if (causal != 0 && causal != 1) return TFGFA_ERR_CAUSAL_FLAG;
+  if (B == 0 || H == 0 || N == 0) return TFGFA_OK;
+  if (P == 0) return TFGFA_ERR_BAD_SHAPE;
+  AttendPlan x;
+  if (!attend_plan(B, H, H_kv, N, page, M, D, &x)) return TFGFA_ERR_TOO_LARGE;
+  if (!q || !k_pages || !v_pages || !o || !cache_seqlens || (!page_table && M > 0) || !q_strides || !k_strides ||
+      !v_strides || !o_strides)
+    return TFGFA_ERR_NULL_POINTER;
+  AttendArgs a = {};
+  if (!tfgfa::rows_ok(q_strides, B, H, N, D, &a.qs) || !tfgfa::rows_ok(o_strides, B, H, N, D, &a.os) ||
+      !tfgfa::pages_ok(k_strides, P, H_kv, page, D, &a.ks) || !tfgfa::pages_ok(v_strides, P, H_kv, page, D, &a.vs) ||
+      !tfgfa::pages_apart({2 * a.os.b, 2 * a.os.h, 2 * a.os.n}, B, H, N, D))
+    return TFGFA_ERR_STRIDE;
+  if (B > 1 && table_stride < 0) return TFGFA_ERR_STRIDE;
+  if (!rows_fit(a.ks) || !rows_fit(a.vs)) return TFGFA_ERR_TOO_LARGE;
+  if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)o | (uintptr_t)workspace) & 15u)
+    return TFGFA_ERR_ALIGNMENT;
+  if (((uintptr_t)page_table | (uintptr_t)cache_seqlens | (uintptr_t)lengths | (uintptr_t)lse) & 3u) return TFGFA_ERR_ALIGNMENT;
+  if (x.bytes > (workspace ? workspace_bytes : 0)) x.parts = 1;
+  a.q = q, a.o = o, a.lse = lse, a.part = static_cast<float*>(workspace);
+  a.k = static_cast<const char*>(k_pages), a.v = static_cast<const char*>(v_pages);
+  a.table = page_table, a.table_stride = B > 1 ? table_stride : 0, a.lens = cache_seqlens, a.lengths = lengths;
+  a.by_page = tfgfa::division_by(page), a.by_group = tfgfa::division_by(H / H_kv);
+  a.page = page, a.P = P, a.n_max = M * page, a.N = N, a.G = H / H_kv, a.Hkv = H_kv, a.heads = B * H_kv, a.D = D;
+  a.causal = causal, a.pad = pad != 0, a.tiles = (int)x.tiles, a.parts = x.parts;
+  a.scale = softmax_scale, a.scale_log2 = softmax_scale * kLog2e;
+  const hipStream_t stream = (hipStream_t)hip_stream;
+  const hipError_t e = dtype == TFGFA_DTYPE_BF16 ? launch_attend<__bf16>(a, x, stream) : launch_attend<_Float16>(a, x, stream);
+  return e == hipSuccess ? TFGFA_OK : -(int)e;
+}
+
+extern "C" size_t tfpages_decode_shared_workspace(int R, int B, int H, int H_kv, int page, int M_prefix, int M, int D) {
+  using namespace tfgfa_context;
+  if (!heads_ok(B, H, H_kv, page, M) || M_prefix < 0 || D < 8 || D > kMaxD || (D & 7) || R < 1 || B % R) return 0;
+  if (B == 0 || H == 0) return 0;
+  SharedPlan x;
+  return shared_plan(R, B, H, H_kv, page, M_prefix, M, D, &x) ? x.bytes : 0;
+}
+
+extern "C" int tfpages_decode_shared(const void* q, const int64_t* q_strides, void* k_pages, const int64_t* k_strides,
+                                     void* v_pages, const int64_t* v_strides, const int* prefix_table,
+                                     int64_t prefix_stride, const int* prefix_lens, const int* page_table,
+                                     int64_t table_stride, const int* cache_seqlens, const void* k_new,
+                                     const int64_t* k_new_strides, const void* v_new, const int64_t* v_new_strides,
+                                     void* o, const int64_t* o_strides, float* lse, int R, int B, int H, int H_kv,
+                                     int P, int page, int M_prefix, int M, int D, int dtype, float softmax_scale,
+                                     void* workspace, size_t workspace_bytes, void* hip_stream) {
+  using namespace tfgfa_context;
+  if (dtype != TFGFA_DTYPE_BF16 && dtype != TFGFA_DTYPE_F16) return TFGFA_ERR_DTYPE;
+  if (!heads_ok(B, H, H_kv, page, M) || M_prefix < 0 || P < 0 || R < 0 || (R == 0 ? B != 0 : B % R != 0))
+    return TFGFA_ERR_BAD_SHAPE;
+  if (D < 8 || D > kMaxD || (D & 7)) return TFGFA_ERR_HEAD_DIM;
+  if (!(softmax_scale > 0.f) || !isfinite(softmax_scale)) return TFGFA_ERR_SCALE;
+  if ((k_new == nullptr) != (v_new == nullptr)) return TFGFA_ERR_NULL_POINTER;
+  if (B == 0 || H == 0) return TFGFA_OK;
+  if (P == 0) return TFGFA_ERR_BAD_SHAPE;
+  SharedPlan x;
+  if (!shared_plan(R, B, H, H_kv, page, M_prefix, M, D, &x)) return TFGFA_ERR_TOO_LARGE;
+  if (!q || !k_pages || !v_pages || !o || !prefix_lens || !cache_seqlens || (!page_table && M > 0) ||
+      (!prefix_table && M_prefix > 0) || !q_strides || !k_strides || !v_strides || !o_strides ||
+      (k_new && (!k_new_strides || !v_new_strides)))
+    return TFGFA_ERR_NULL_POINTER;
+  SharedArgs a = {};
+  if (!tfgfa::vecs_ok(q_strides, B, H, &a.qs) || !tfgfa::vecs_ok(o_strides, B, H, &a.os) ||
+      !tfgfa::pages_ok(k_strides, P, H_kv, page, D, &a.ks) || !tfgfa::pages_ok(v_strides, P, H_kv, page, D, &a.vs) ||
+      !tfgfa::apart(a.os.b, B, a.os.h, H, D))
+    return TFGFA_ERR_STRIDE;
+  if (k_new && (!tfgfa::vecs_ok(k_new_strides, B, H_kv, &a.kns) || !tfgfa::vecs_ok(v_new_strides, B, H_kv, &a.vns) ||
+                !tfgfa::pages_apart(a.ks, P, H_kv, page, D) || !tfgfa::pages_apart(a.vs, P, H_kv, page, D)))
+    return TFGFA_ERR_STRIDE;
+  if ((B > 1 && table_stride < 0) || (R > 1 && prefix_stride < 0)) return TFGFA_ERR_STRIDE;
+  if (!rows_fit(a.ks) || !rows_fit(a.vs)) return TFGFA_ERR_TOO_LARGE;
+  if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)o | (uintptr_t)k_new | (uintptr_t)v_new |
+       (uintptr_t)workspace) & 15u)
+    return TFGFA_ERR_ALIGNMENT;
+  if (((uintptr_t)prefix_table | (uintptr_t)prefix_lens | (uintptr_t)page_table | (uintptr_t)cache_seqlens |
+       (uintptr_t)lse) & 3u)
+    return TFGFA_ERR_ALIGNMENT;
+  if (x.bytes > (workspace ? workspace_bytes : 0)) return TFGFA_ERR_SCRATCH;
+  a.q = q, a.o = o, a.lse = lse;
+  a.prefix_part = static_cast<float*>(workspace);
+  a.own_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + x.own_at);
+  a.k = static_cast<char*>(k_pages), a.v = static_cast<char*>(v_pages), a.kn = k_new, a.vn = v_new;
+  a.prefix_table = prefix_table, a.prefix_lens = prefix_lens, a.table = page_table, a.lens = cache_seqlens;
+  a.prefix_stride = R > 1 ? prefix_stride : 0, a.table_stride = B > 1 ? table_stride : 0;
+  a.by_page = tfgfa::division_by(page), a.by_group = tfgfa::division_by(H / H_kv);
+  a.page = page, a.P = P, a.prefix_max = M_prefix * page, a.n_max = M * page, a.G = H / H_kv, a.Hkv = H_kv, a.R = R;
+  a.each = B / R, a.D = D;
+  a.prefix_heads = R * H_kv, a.prefix_tiles = (int)x.prefix_tiles, a.prefix_parts = x.prefix_parts;
+  a.prefix_jobs = (int)(x.prefix_jobs * x.prefix_parts);
+  a.own_heads = B * H_kv, a.own_tiles = (int)x.own_tiles, a.own_parts = x.own_parts;
+  a.scale = softmax_scale, a.scale_log2 = softmax_scale * kLog2e;
+  const hipStream_t stream = (hipStream_t)hip_stream;
+  const hipError_t e = dtype == TFGFA_DTYPE_BF16 ? launch_shared<__bf16>(a, x, B * H, stream)
+                                                 : launch_shared<_Float16>(a, x, B * H, stream);
+  return e == hipSuccess ? TFGFA_OK : -(int)e;
+}

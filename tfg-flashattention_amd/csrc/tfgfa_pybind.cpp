@@ -367,6 +367,52 @@ void append(const View& k, const View& v, const View& k_pages, const View& v_pag
   check(st, "tfpages_append");
 }
 
+void attend(const View& q, const View& k, const View& v, std::uintptr_t table,
+            std::int64_t table_stride, std::uintptr_t seqlens, std::uintptr_t lengths,
+            const View& o, std::uintptr_t lse, bool pad, bool causal, int B, int H, int H_kv,
+            int N, int P, int page, int M, int D, int dtype, float softmax_scale,
+            std::uintptr_t workspace, std::size_t workspace_bytes, std::uintptr_t stream) {
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    const std::lock_guard<std::mutex> alone(workspace_calls);
+    st = tfpages_attend(pointer<void>(q.first), q.second.data(), pointer<void>(k.first),
+                        k.second.data(), pointer<void>(v.first), v.second.data(),
+                        pointer<int>(table), table_stride, pointer<int>(seqlens),
+                        pointer<int>(lengths), pointer<void>(o.first), o.second.data(),
+                        pointer<float>(lse), pad ? 1 : 0, causal ? 1 : 0, B, H, H_kv, N, P, page,
+                        M, D, dtype, softmax_scale, pointer<void>(workspace), workspace_bytes,
+                        pointer<void>(stream));
+  }
+  check(st, "tfpages_attend");
+}
+
+// A (B, H, D) tensor.
+using View3 = std::pair<std::uintptr_t, Strides3>;
+
+void decode_shared(const View3& q, const View& k, const View& v, std::uintptr_t prefix_table,
+                   std::int64_t prefix_stride, std::uintptr_t prefix_lens, std::uintptr_t table,
+                   std::int64_t table_stride, std::uintptr_t seqlens, const View3& k_new,
+                   const View3& v_new, const View3& o, std::uintptr_t lse, int R, int B, int H,
+                   int H_kv, int P, int page, int M_prefix, int M, int D, int dtype,
+                   float softmax_scale, std::uintptr_t workspace, std::size_t workspace_bytes,
+                   std::uintptr_t stream) {
+  int st;
+  {
+    py::gil_scoped_release nogil;
+    const std::lock_guard<std::mutex> alone(workspace_calls);
+    st = tfpages_decode_shared(
+        pointer<void>(q.first), q.second.data(), pointer<void>(k.first), k.second.data(),
+        pointer<void>(v.first), v.second.data(), pointer<int>(prefix_table), prefix_stride,
+        pointer<int>(prefix_lens), pointer<int>(table), table_stride, pointer<int>(seqlens),
+        pointer<void>(k_new.first), k_new.second.data(), pointer<void>(v_new.first),
+        v_new.second.data(), pointer<void>(o.first), o.second.data(), pointer<float>(lse), R, B,
+        H, H_kv, P, page, M_prefix, M, D, dtype, softmax_scale, pointer<void>(workspace),
+        workspace_bytes, pointer<void>(stream));
+  }
+  check(st, "tfpages_decode_shared");
+}
+
 py::dict device_info() {
   int cu = 0, mhz = 0;
   char arch[128] = {0};
@@ -506,6 +552,25 @@ PYBIND11_MODULE(_C, m) {
         py::arg("rot"), py::arg("interleaved"), py::arg("magnitude"), py::arg("B"), py::arg("H"),
         py::arg("H_kv"), py::arg("N"), py::arg("P"), py::arg("page"), py::arg("M"), py::arg("D"),
         py::arg("dtype"), py::arg("stream"));
+  m.def("attend", &attend, "Attention of several new tokens over a paged KV cache", py::arg("q"),
+        py::arg("k_pages"), py::arg("v_pages"), py::arg("page_table"), py::arg("table_stride"),
+        py::arg("cache_seqlens"), py::arg("lengths"), py::arg("o"), py::arg("lse"), py::arg("pad"),
+        py::arg("causal"), py::arg("B"), py::arg("H"), py::arg("H_kv"), py::arg("N"), py::arg("P"),
+        py::arg("page"), py::arg("M"), py::arg("D"), py::arg("dtype"), py::arg("softmax_scale"),
+        py::arg("workspace"), py::arg("workspace_bytes"), py::arg("stream"));
+  m.def("attend_workspace", &tfpages_attend_workspace, py::arg("B"), py::arg("H"), py::arg("H_kv"),
+        py::arg("N"), py::arg("page"), py::arg("M"), py::arg("D"));
+  m.def("decode_shared", &decode_shared, "One decode step of sequences that share a prefix",
+        py::arg("q"), py::arg("k_pages"), py::arg("v_pages"), py::arg("prefix_table"),
+        py::arg("prefix_stride"), py::arg("prefix_lens"), py::arg("page_table"),
+        py::arg("table_stride"), py::arg("cache_seqlens"), py::arg("k_new"), py::arg("v_new"),
+        py::arg("o"), py::arg("lse"), py::arg("R"), py::arg("B"), py::arg("H"), py::arg("H_kv"),
+        py::arg("P"), py::arg("page"), py::arg("M_prefix"), py::arg("M"), py::arg("D"),
+        py::arg("dtype"), py::arg("softmax_scale"), py::arg("workspace"),
+        py::arg("workspace_bytes"), py::arg("stream"));
+  m.def("decode_shared_workspace", &tfpages_decode_shared_workspace, py::arg("R"), py::arg("B"),
+        py::arg("H"), py::arg("H_kv"), py::arg("page"), py::arg("M_prefix"), py::arg("M"),
+        py::arg("D"));
   m.def("fwd_plan",
         [](long long heads, int cu_count, int Nq, int Nk, int D, bool causal) {
           static const char* const names[] = {"kWhole", "kHalves", "kGroups2", "kPairs", "kGroups4"};

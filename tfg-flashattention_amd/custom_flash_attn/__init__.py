@@ -31,8 +31,8 @@ except ImportError as exc:  # pragma: no cover - exercised only on a broken buil
     ) from exc
 
 __all__ = ["forward", "forward_lse", "attention", "flash_attn_forward", "decode", "decode_paged",
-           "key_weights", "evict", "penalize_logits", "Rotary", "rotate", "append_paged", "device_info", "HEAD_DIM",
-           "MAX_HEAD_DIM", "library_path"]
+           "key_weights", "evict", "penalize_logits", "Rotary", "rotate", "append_paged", "attend_paged",
+           "decode_shared", "device_info", "HEAD_DIM", "MAX_HEAD_DIM", "library_path"]
 
 HEAD_DIM = 64  # the head dimension of forward() (common_types.hpp:33 fixes K = 64 too)
 MAX_HEAD_DIM = 128  # attention() / flash_attn_forward(): any head dim up to 128
@@ -403,4 +403,4 @@ def device_info() -> dict:
 
 
 from .serving import decode_paged, evict, key_weights, penalize_logits  # noqa: E402,F401  (need the above)
-from .pages import Rotary, append_paged, rotate  # noqa: E402,F401
+from .pages import Rotary, append_paged, attend_paged, decode_shared, rotate  # noqa: E402,F401

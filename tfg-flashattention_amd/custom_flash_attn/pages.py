@@ -14,10 +14,11 @@ import math
 import torch
 from torch.autograd import forward_ad
 
-from . import _C, _DTYPES, MAX_HEAD_DIM, _launch_on
-from .serving import (_accepts_pages, _check_pages, _check_seqlens, _check_table, _is_seqlens, _is_table)
+from . import _C, _check_vec, _DTYPES, MAX_HEAD_DIM, _launch_on
+from .serving import (_accepts_pages, _check_pages, _check_seqlens, _check_table, _extent, _is_seqlens, _is_table,
+                      _workspace)
 
-_NONE = (0, (0, 0, 0, 0))
+_NONE, _NONE3 = (0, (0, 0, 0, 0)), (0, (0, 0, 0))
 _ROTATED = {torch.bfloat16: _C.DTYPE_BF16, torch.float16: _C.DTYPE_F16, torch.float32: _C.DTYPE_F32}
 _INTS = (torch.int32, torch.int64)
 
@@ -357,3 +358,155 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
                0 if positions is None else positions.data_ptr(), _view(q), _view(q_out), pad, turns, rot, interleaved,
                magnitude, B, 0 if q is None else q.shape[1], H_kv, N, P, page, page_table.shape[1], D, _DTYPES[k.dtype])
     return q_out
+
+
+def _accepts_attend(q, k_pages, v_pages, page_table, cache_seqlens, lengths, out) -> bool:
+    """Everything _check_attend checks, as one test."""
+    index, qs = k_pages.get_device(), q.shape
+    if not (_accepts_pages(k_pages, v_pages, index) and len(qs) == 4):
+        return False
+    _, H_kv, _, D = k_pages.shape
+    B, H, N, _ = qs
+    return (H_kv > 0 and H % H_kv == 0 and _are_rows(q, B, H, N, D, k_pages.dtype, index)
+            and (out is None or _are_rows(out, B, H, N, D, k_pages.dtype, index)) and _is_table(page_table, B, index)
+            and _is_seqlens(cache_seqlens, B, index) and (lengths is None or _is_seqlens(lengths, B, index)))
+
+
+def _check_attend(q, k_pages, v_pages, page_table, cache_seqlens, lengths, out) -> None:
+    _check_pages(k_pages, v_pages)
+    _, H_kv, _, D = k_pages.shape
+    dev, dtype = k_pages.device, k_pages.dtype
+    if q.dim() != 4:
+        raise RuntimeError(f"q must be 4-D (batch, heads, seq_len, head_dim), got shape {tuple(q.shape)}")
+    B, H, N, _ = q.shape
+    if H_kv == 0 or H % H_kv:
+        raise RuntimeError(f"q's {H} heads must be a multiple of the cache's {H_kv}")
+    _check_rows(q, "q", B, H, N, D, dtype, dev)
+    if out is not None:
+        _check_rows(out, "out", B, H, N, D, dtype, dev)
+    _check_table(page_table, "page_table", B, dev)
+    _check_seqlens(cache_seqlens, B, dev)
+    if lengths is not None:
+        _check_counts(lengths, "lengths", B, dev)
+
+
+def attend_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                 cache_seqlens: torch.Tensor, *, lengths: torch.Tensor | None = None, causal: bool = True,
+                 out: torch.Tensor | None = None, softmax_scale: float | None = None, return_lse: bool = False,
+                 workspace: torch.Tensor | None = None):
+    """Attention of several new tokens over a paged cache (:func:`decode_paged`) that holds their keys already
+    (:func:`append_paged`): a chunk of a prompt, or drafted tokens that are checked together.
+
+    ``q``: (B, H, N, D), any strides as for :func:`attention`, H a multiple of the cache's H_kv.  With ``causal`` token i of
+    sequence b sees the ``cache_seqlens[b]`` rows before the new tokens and the new tokens' up to its own; without, every
+    token sees the ``cache_seqlens[b]`` rows, all there are (cross attention to cached states of another length).  With
+    ``lengths`` (int32 (B,)) only the first ``lengths[b]`` tokens count; rows of the others are left as they were in
+    ``out``, and in a new tensor are zeros.  The caller advances ``cache_seqlens`` afterwards.
+
+    Returns ``out`` ((B, H, N, D), new if not given), or ``(out, lse)`` with ``return_lse=True`` (lse (B, H, N) float32,
+    natural log, -inf for tokens that do not count).  A token that sees no row, or scores of -inf alone, has output 0 and
+    lse -inf.  A sequence whose length or number of new tokens does not fit its table yields NaN for its tokens, a page id
+    outside the pool for those that see its rows (checked on the device).  ``workspace`` as for :func:`decode`, of
+    ``_C.attend_workspace(B, H, H_kv, N, page, M, D)`` bytes; with a smaller one a tile of rows is one workgroup's.
+    """
+    if not _accepts_attend(q, k_pages, v_pages, page_table, cache_seqlens, lengths, out):
+        _check_attend(q, k_pages, v_pages, page_table, cache_seqlens, lengths, out)
+    P, H_kv, page, D = k_pages.shape
+    B, H, N, _ = q.shape
+    M, index = page_table.shape[1], k_pages.get_device()
+    pad = out is None
+    if pad:
+        out = torch.empty_like(q)
+    lse = None
+    if return_lse:
+        lse = q.new_empty((B, H, N), dtype=torch.float32)
+        if not pad and lengths is not None:
+            lse.fill_(-math.inf)  # (with the caller's output the kernel leaves such rows alone)
+    scale = (1.0 / math.sqrt(D)) if softmax_scale is None else float(softmax_scale)
+    workspace = _workspace(workspace, index, 0 if workspace is not None else
+                           _C.attend_workspace(B, H, H_kv, N, page, M, D))
+    _launch_on(index, _C.attend, _view(q), _view(k_pages), _view(v_pages), page_table.data_ptr(), page_table.stride(0),
+               cache_seqlens.data_ptr(), 0 if lengths is None else lengths.data_ptr(), _view(out),
+               0 if lse is None else lse.data_ptr(), pad, bool(causal), B, H, H_kv, N, P, page, M, D, _DTYPES[q.dtype], scale,
+               *_extent(workspace))
+    return (out, lse) if return_lse else out
+
+
+def _accepts_shared(q, k_pages, v_pages, prefix_table, prefix_lens, page_table, cache_seqlens, k_new, v_new, out) -> bool:
+    """Everything _check_shared checks, as one test."""
+    index, qs = k_pages.get_device(), q.shape
+    if not (_accepts_pages(k_pages, v_pages, index) and len(qs) == 3 and (k_new is None) == (v_new is None)
+            and len(prefix_table.shape) == 2):
+        return False
+    _, H_kv, _, D = k_pages.shape
+    B, H, _ = qs
+    R, dtype = prefix_table.shape[0], k_pages.dtype
+    if H_kv == 0 or H % H_kv or R == 0 or B % R:
+        return False
+    for x, h in ((q, H), (out, H), (k_new, H_kv), (v_new, H_kv)):
+        if x is not None and not (x.shape == (B, h, D) and x.dtype is dtype and x.get_device() == index and x.stride(2) == 1):
+            return False
+    return (_is_table(prefix_table, R, index) and _is_seqlens(prefix_lens, R, index) and _is_table(page_table, B, index)
+            and _is_seqlens(cache_seqlens, B, index))
+
+
+def _check_shared(q, k_pages, v_pages, prefix_table, prefix_lens, page_table, cache_seqlens, k_new, v_new, out) -> None:
+    _check_pages(k_pages, v_pages)
+    _, H_kv, _, D = k_pages.shape
+    dev, dtype = k_pages.device, k_pages.dtype
+    if q.dim() != 3:
+        raise RuntimeError(f"q must be (B, H, D), got {tuple(q.shape)}")
+    B, H, _ = q.shape
+    if H_kv == 0 or H % H_kv:
+        raise RuntimeError(f"q's {H} heads must be a multiple of the cache's {H_kv}")
+    _check_vec(q, "q", B, H, D, dtype, dev)
+    R = prefix_table.shape[0] if prefix_table.dim() == 2 else 0
+    if R == 0 or B % R:
+        raise RuntimeError(f"prefix_table must be int32 of shape (R, pages) with {B} sequences a multiple of R, got "
+                           f"{prefix_table.dtype} {tuple(prefix_table.shape)}")
+    _check_table(prefix_table, "prefix_table", R, dev)
+    _check_counts(prefix_lens, "prefix_lens", R, dev)
+    _check_table(page_table, "page_table", B, dev)
+    _check_seqlens(cache_seqlens, B, dev)
+    if (k_new is None) != (v_new is None):
+        raise RuntimeError("k_new and v_new must be given together")
+    if k_new is not None:
+        _check_vec(k_new, "k_new", B, H_kv, D, dtype, dev)
+        _check_vec(v_new, "v_new", B, H_kv, D, dtype, dev)
+    if out is not None:
+        _check_vec(out, "out", B, H, D, dtype, dev)
+
+
+def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, prefix_table: torch.Tensor,
+                  prefix_lens: torch.Tensor, page_table: torch.Tensor, cache_seqlens: torch.Tensor,
+                  k_new: torch.Tensor | None = None, v_new: torch.Tensor | None = None, *,
+                  out: torch.Tensor | None = None, softmax_scale: float | None = None, return_lse: bool = False,
+                  workspace: torch.Tensor | None = None):
+    """:func:`decode_paged` for sequences that share their first rows, which are read once for all of them.
+
+    The B sequences of ``q`` (B, H, D) are R groups of B / R, one after the other: sequence b attends to the
+    ``prefix_lens[r]`` rows (int32 (R,)) that ``prefix_table`` (int32 (R, M_prefix)) names for its group r = b // (B / R),
+    then to the ``cache_seqlens[b]`` rows of its own in ``page_table`` (int32 (B, M)); neither needs to fill its last page.
+    Everything else is as for :func:`decode_paged`: the pools, head layouts and types, ``k_new``/``v_new`` ((B, H_kv, D)),
+    which become row ``cache_seqlens[b]`` of the sequence's own, ``out``, the lse.  A length that does not fit its table or a
+    page id outside the pool yields NaN for the sequence, or for the whole group if it is the prefix's (checked on the
+    device).  ``workspace``: at least ``_C.decode_shared_workspace(R, B, H, H_kv, page, M_prefix, M, D)`` bytes, kept per
+    device and stream where none is given.
+    """
+    if not _accepts_shared(q, k_pages, v_pages, prefix_table, prefix_lens, page_table, cache_seqlens, k_new, v_new, out):
+        _check_shared(q, k_pages, v_pages, prefix_table, prefix_lens, page_table, cache_seqlens, k_new, v_new, out)
+    P, H_kv, page, D = k_pages.shape
+    B, H, _ = q.shape
+    (R, M_prefix), M, index = prefix_table.shape, page_table.shape[1], k_pages.get_device()
+    if out is None:
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, H, D))
+    lse = q.new_empty((B, H), dtype=torch.float32) if return_lse else None
+    scale = (1.0 / math.sqrt(D)) if softmax_scale is None else float(softmax_scale)
+    workspace = _workspace(workspace, index, 0 if workspace is not None else
+                           _C.decode_shared_workspace(R, B, H, H_kv, page, M_prefix, M, D))
+    _launch_on(index, _C.decode_shared, _view(q), _view(k_pages), _view(v_pages), prefix_table.data_ptr(),
+               prefix_table.stride(0), prefix_lens.data_ptr(), page_table.data_ptr(), page_table.stride(0),
+               cache_seqlens.data_ptr(), _NONE3 if k_new is None else _view(k_new), _NONE3 if v_new is None else _view(v_new),
+               _view(out), 0 if lse is None else lse.data_ptr(), R, B, H, H_kv, P, page, M_prefix, M, D, _DTYPES[q.dtype],
+               scale, *_extent(workspace))
+    return (out, lse) if return_lse else out
