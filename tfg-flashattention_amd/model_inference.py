@@ -5,7 +5,8 @@ names, constructor arguments and config keys, so code written against the refere
 ``GPTModel(cfg)`` runs unchanged, and its token loop ``generate`` (:199-228).  Added:
 ``KVCache`` and ``generate_cached``, the same loop with a KV cache (prefill once, then one
 decode-kernel step per token); ``PagedKVCache``, a cache in pages that may be cut to the rows whose
-attention weight is largest; ``LogitPenalties``, what a loop does to the logits before sampling.  The reference's data loader, training helpers, tokenizer and
+attention weight is largest; ``SampledKVCache`` and ``generate_samples``, several continuations of each
+prompt, whose keys they share; ``LogitPenalties``, what a loop does to the logits before sampling.  The reference's data loader, training helpers, tokenizer and
 pretrained-weight download (model_inference.py:23-37, :193-197, :229-376; gpt_download.py)
 are not here.
 
@@ -225,8 +226,9 @@ class MultiHeadAttention(nn.Module):
 
         Prefill (the cache is empty): the cache stores the new tokens' K/V and runs the causal
         forward kernel over them.  Decode (one new token): its decode kernel appends the token's K/V
-        and attends over the cached prefix.  Both write the context straight into a (B, N, H*d)
-        buffer.
+        and attends over the cached prefix.  Several tokens on a cache that holds some (a paged one
+        without a budget): appended, then attended to together.  All write the context straight into a
+        (B, N, H*d) buffer.
         """
         if self.impl_type not in ("hip", "cuda"):
             raise ValueError(f"cached attention runs on the HIP kernels; impl_type is {self.impl_type!r}")
@@ -240,8 +242,11 @@ class MultiHeadAttention(nn.Module):
             cache.prompt(layer, q, k, v, ctx)
         elif n == 1:
             cache.attend(layer, q[:, 0], k[:, 0], v[:, 0], out=ctx[:, 0])
+        elif getattr(cache, "extends", False):
+            cache.extend(layer, q, k, v, ctx)
         else:
-            raise NotImplementedError("a cache that already holds tokens takes one new token per step")
+            raise NotImplementedError("a cache that already holds tokens takes one new token per step (a PagedKVCache "
+                                      "without a budget takes more)")
         return out_proj(ctx.view(b, n, self.d_out))
 
 
@@ -310,12 +315,13 @@ class PagedKVCache:
     ``recent`` rows (default half the budget) and those of the largest sums, ``budget`` in all;
     :meth:`over` says when ``slack`` more rows than that are held.  Rows carry their positions in their
     keys, so the others stay what they are.  Pages are handed out and taken back on the host, and a cut's table is copied
-    from there, which waits for the copy.  A budget bounds the rows that a step reads, not the pools: they hold the
+    from there, which waits for the copy.  Without a budget a cache that holds tokens takes several more at a time
+    (:meth:`extend`).  A budget bounds the rows that a step reads, not the pools: they hold the
     longest text's pages and a cut's beside them, for every sequence.
     """
 
     def __init__(self, cfg: dict, batch: int, max_len: int, device, dtype=torch.bfloat16, page_size: int = 64,
-                 budget: int | None = None, recent: int | None = None, slack: int = 64):
+                 budget: int | None = None, recent: int | None = None, slack: int = 64, more_pages: int = 0):
         import custom_flash_attn
 
         if budget is not None and not 0 < budget:
@@ -331,7 +337,7 @@ class PagedKVCache:
         self._columns = -(-max_len // page_size)
         # (A text of max_len tokens never needs more rows than that, cut or not.)
         self._cut_columns = 0 if budget is None else min(self._columns, -(-(budget + slack) // page_size))
-        pages = batch * (self._columns + self._cut_columns)
+        pages = batch * (self._columns + self._cut_columns) + more_pages
         layers = range(cfg["n_layers"])
         self.k = [torch.zeros(pages, H, page_size, hd, dtype=dtype, device=device) for _ in layers]
         self.v = [torch.zeros(pages, H, page_size, hd, dtype=dtype, device=device) for _ in layers]
@@ -355,27 +361,44 @@ class PagedKVCache:
         the weight each key received into ``weights``."""
         import custom_flash_attn
 
-        b, n, H, hd = k.shape
-        pages = -(-n // self.page_size)
-        at = self.table[:, :pages].long()
-        for pool, rows in ((self.k[layer], k), (self.v[layer], v)):
-            rows = F.pad(rows, (0, 0, 0, 0, 0, pages * self.page_size - n))
-            pool[at] = rows.view(b, pages, self.page_size, H, hd).transpose(2, 3)
+        n = k.shape[1]
         q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
+        custom_flash_attn.append_paged(k, v, self.k[layer], self.v[layer], self.table, self.seqlens)
         if self.weights is None:
             custom_flash_attn.attention(q, k, v, out=ctx.transpose(1, 2))
         else:
             _, lse = custom_flash_attn.attention(q, k, v, out=ctx.transpose(1, 2), return_lse=True)
             custom_flash_attn.key_weights(q, k, lse, out=self.weights[layer][:, :, :n])
 
+    @property
+    def extends(self) -> bool:
+        """Whether :meth:`extend` may be called (the sums of a budget need one token at a time)."""
+        return self.budget is None
+
+    def extend(self, layer, q, k, v, ctx) -> None:
+        """More tokens' (B, N, H, d) projections: K and V behind the rows there are, and the attention of each token over
+        those and the new ones up to it into ``ctx``."""
+        import custom_flash_attn
+
+        if not self.extends:
+            raise ValueError("a cache with a budget takes one new token per step")
+        self._check_room(k.shape[1])
+        q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
+        custom_flash_attn.append_paged(k, v, self.k[layer], self.v[layer], self.table, self.seqlens)
+        custom_flash_attn.attend_paged(q, self.k[layer], self.v[layer], self.table, self.seqlens, out=ctx.transpose(1, 2))
+
+    def _check_room(self, n: int) -> None:
+        rows = self.table.shape[1] * self.page_size
+        if self.length + n > rows:
+            raise ValueError(f"the cache's tables hold {rows} rows and have no place for "
+                             f"{'another token' if n == 1 else f'{n} more tokens'}"
+                             + ("" if self.budget is None else ": evict() first"))
+
     def attend(self, layer, q, k, v, out=None):
         """One decode step of (B, H, d) projections: the new row appended, the attention over all rows."""
         import custom_flash_attn
 
-        rows = self.table.shape[1] * self.page_size
-        if self.length >= rows:
-            raise ValueError(f"the cache's tables hold {rows} rows and have no place for another token"
-                             + ("" if self.budget is None else ": evict() first"))
+        self._check_room(1)
         return custom_flash_attn.decode_paged(q, self.k[layer], self.v[layer], self.table, self.seqlens, k, v, out=out,
                                               key_weights=None if self.weights is None else self.weights[layer],
                                               workspace=self.workspace)
@@ -412,6 +435,66 @@ class PagedKVCache:
         self.positions.zero_()
         self._free = list(range(self._pages))
         self.table, self._held = self._take(self._columns)
+
+
+class SampledKVCache(PagedKVCache):
+    """A paged cache of ``batch`` prompts and, after :meth:`share`, of ``samples`` continuations of each: sequences
+    b * samples .. (b + 1) * samples - 1 are prompt b's.  Their prompts' rows stay where they are, once for all of them,
+    and are read once a step for all of them (custom_flash_attn.decode_shared); each continuation holds up to
+    ``new_len`` rows of its own.  ``seqlens`` counts the prompts' rows, ``own_lens`` (int32 (batch * samples,)) the
+    continuations', ``positions`` the tokens that each sequence has seen."""
+
+    def __init__(self, cfg: dict, batch: int, samples: int, max_len: int, new_len: int, device, dtype=torch.bfloat16,
+                 page_size: int = 64):
+        if samples < 1 or new_len < 1:
+            raise ValueError(f"samples and new_len must be positive, got {samples} and {new_len}")
+        self.samples, self.new_len = samples, new_len
+        self._own_columns = -(-new_len // page_size)
+        super().__init__(cfg, batch, max_len, device, dtype, page_size, more_pages=batch * samples * self._own_columns)
+
+    @property
+    def extends(self) -> bool:
+        return not self.shared
+
+    def share(self) -> None:
+        """From here on every prompt is ``samples`` sequences."""
+        if self.shared:
+            raise ValueError("the prompts are shared already")
+        self.shared = True
+        self.positions = self.seqlens.repeat_interleave(self.samples)
+
+    def extend(self, layer, q, k, v, ctx) -> None:
+        if self.shared:
+            raise ValueError("continuations take one new token per step")
+        super().extend(layer, q, k, v, ctx)
+
+    def attend(self, layer, q, k, v, out=None):
+        import custom_flash_attn
+
+        if not self.shared:
+            return super().attend(layer, q, k, v, out)
+        if self.own_length >= self.new_len:
+            raise ValueError(f"the continuations hold up to {self.new_len} tokens and have no place for another one")
+        return custom_flash_attn.decode_shared(q, self.k[layer], self.v[layer], self.table, self.seqlens, self.own_table,
+                                               self.own_lens, k, v, out=out)
+
+    def advance(self, n: int) -> None:
+        if not self.shared:
+            super().advance(n)
+            return
+        self.own_length += n
+        self.own_lens.add_(n)
+        self.positions.add_(n)
+
+    def reset(self) -> None:
+        batch = self.seqlens.shape[0]
+        self.positions = torch.zeros_like(self.seqlens)
+        super().reset()
+        self.shared, self.own_length = False, 0
+        own = batch * self.samples
+        ids = self._free[:own * self._own_columns]
+        self.own_table = torch.tensor(ids, dtype=torch.int32).view(own, self._own_columns).to(self.seqlens.device)
+        self.own_lens = torch.zeros(own, dtype=torch.int32, device=self.seqlens.device)
 
 
 class GraphedDecoder:
@@ -798,6 +881,41 @@ def generate_cached(model, idx, max_new_tokens, context_size, temperature=1.0, t
             break
         idx = torch.cat((idx, idx_next), dim=1)
         step_in = idx_next
+    return idx
+
+
+def generate_samples(model, idx, samples, max_new_tokens, context_size, temperature=1.0, top_k=None, eos_id=None,
+                     penalties=None, cache=None):
+    """``samples`` continuations of each prompt of ``idx`` (B, N): (B * samples, N + new), prompt b's in rows b * samples ..
+    The prompts are run once, and their cached rows are shared by their continuations (:class:`SampledKVCache`; ``cache``,
+    if given, is one for this batch, from its reset on).  Sampling as in :func:`generate_cached`; ends when every
+    continuation's token is ``eos_id``."""
+    B, N = idx.shape
+    if N + max_new_tokens > context_size:
+        raise ValueError(f"prompt ({N}) + max_new_tokens ({max_new_tokens}) exceeds context_size ({context_size})")
+    if cache is None:
+        cfg = {"n_heads": model.trf_blocks[0].att.num_heads, "emb_dim": model.tok_emb.embedding_dim,
+               "n_layers": len(model.trf_blocks)}
+        cache = SampledKVCache(cfg, B, samples, N, max(1, max_new_tokens), idx.device)
+    else:
+        if cache.seqlens.shape[0] != B or cache.samples != samples:
+            raise ValueError(f"the cache is for {cache.seqlens.shape[0]} prompts and {cache.samples} samples, not {B} and "
+                             f"{samples}")
+        if cache.max_len < N or cache.new_len < max_new_tokens - 1:
+            raise ValueError("the cache is shorter than the prompt or max_new_tokens")
+        cache.reset()
+    with torch.no_grad():
+        logits = _last_logits(model, idx, cache).repeat_interleave(samples, 0)
+    cache.share()
+    idx = idx.repeat_interleave(samples, 0)
+    for i in range(max_new_tokens):
+        idx_next = _next_token(_penalized(logits, idx, penalties), temperature, top_k)
+        if eos_id is not None and bool((idx_next == eos_id).all()):
+            break
+        idx = torch.cat((idx, idx_next), dim=1)
+        if i + 1 < max_new_tokens:
+            with torch.no_grad():
+                logits = _last_logits(model, idx_next, cache)
     return idx
 
 
