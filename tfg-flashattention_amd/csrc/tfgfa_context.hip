@@ -62,6 +62,8 @@ constexpr int kManyRows = kWaves * kBlock;    // rows of a workgroup for many ro
 constexpr int kTile = 2 * kBlock;             // keys of its tile
 constexpr int kMaxParts = 64;                 // workgroups of a job
 constexpr int kOutOfRange = 0x7FFFFFF0;       // a buffer offset past any num_records: the load gives zeros
+// Many rows: an offset is no lower, so that scores of -inf have weight 0 beside it.
+constexpr float kLowest = -0x1.fffffep127f;
 
 // kHead: weights are 2^(c (s - m)), s a score without the scale, c the scale times log2 e.  A row's offset m puts the
 // largest weight at 2^kHead, and moves when one would pass 2^(kHead + kMargin).  fp16 ends at 2^-24: with the largest at
@@ -143,8 +145,12 @@ __device__ __forceinline__ int swz_v(int row) { return (row & 3) << 1; }
 template <int kDH, bool kAligned, int kGroups>
 struct Loader {
   int koff[kGroups][kDH], voff[kDH];  // aligned: byte offsets from the group's first row; otherwise in a row, or out of range
-  int id[kAligned ? kGroups : 1];     // pages of the block that is loaded next
   int g0, lane;
+
+  // Pages of a block's groups (one for each), or of its keys (lane l: key l % 32).
+  struct Ids {
+    int id[kAligned ? kGroups : 1];
+  };
 
   __device__ __forceinline__ void init(const Source& s, int D, int g0_, int lane_) {
     g0 = g0_, lane = lane_;
@@ -161,56 +167,56 @@ struct Loader {
     }
   }
   // The pages of the block at key `at`.
-  __device__ __forceinline__ void look_up(const Source& s, int at) {
+  __device__ __forceinline__ Ids look_up(const Source& s, int at) const {
+    Ids x;
     if constexpr (kAligned) {
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         const int key = at + (g0 + g) * kGroup;
-        id[g] = uniform(key < s.keys ? ((uniform_ints)s.table)[divide(key, s.by_page)] : 0);
+        x.id[g] = uniform(key < s.keys ? ((uniform_ints)s.table)[divide(key, s.by_page)] : 0);
       }
     } else {
       const int key = at + (lane & 31);
-      id[0] = key < s.keys ? s.table[divide(key, s.by_page)] : 0;
+      x.id[0] = key < s.keys ? s.table[divide(key, s.by_page)] : 0;
     }
+    return x;
   }
-  // The block at key `at`, whose pages were looked up, to LDS byte `to`.
-  __device__ __forceinline__ void issue(const Source& s, int at, uint32_t to) {
+  // K (kValue: V) of the block at key `at` to LDS byte `to`.
+  template <bool kValue>
+  __device__ __forceinline__ void issue(const Source& s, int at, const Ids& x, uint32_t to) const {
+    const Pages& st = kValue ? s.vs : s.ks;
+    const char* const base = kValue ? s.v : s.k;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      const uint32_t k_to = to + (g0 + g) * 1024, v_to = k_to + kDH * kHalfBytes;
+      const uint32_t there = to + (g0 + g) * 1024;
       if constexpr (kAligned) {
         const int key = at + (g0 + g) * kGroup, rows = uniform(min(kGroup, max(0, s.keys - key)));
-        const bool in = (uint32_t)id[g] < (uint32_t)s.P;
-        const int there = uniform(in ? rows : 0);
-        const uint64_t pid = (uint32_t)(in ? id[g] : 0), off = (uint32_t)(key - divide(key, s.by_page) * s.page);
-        const i32x4 kd = tfgfa::head_desc(s.k + pid * (uint64_t)s.ks.p + off * (uint64_t)s.ks.n, there, (int)s.ks.n);
-        const i32x4 vd = tfgfa::head_desc(s.v + pid * (uint64_t)s.vs.p + off * (uint64_t)s.vs.n, there, (int)s.vs.n);
-        if (in || rows == 0) {
+        const bool in = (uint32_t)x.id[g] < (uint32_t)s.P;
+        const uint64_t pid = (uint32_t)(in ? x.id[g] : 0), off = (uint32_t)(key - divide(key, s.by_page) * s.page);
+        const i32x4 desc = tfgfa::head_desc(base + pid * (uint64_t)st.p + off * (uint64_t)st.n, uniform(in ? rows : 0), (int)st.n);
+        if (kValue || in || rows == 0) {
 #pragma unroll
-          for (int dh = 0; dh < kDH; ++dh) tfgfa::lds_transfer(kd, k_to + dh * kHalfBytes, koff[g][dh]);
+          for (int dh = 0; dh < kDH; ++dh) tfgfa::lds_transfer(desc, there + dh * kHalfBytes, kValue ? voff[dh] : koff[g][dh]);
         } else {
-          const i32x4 nd = tfgfa::head_desc(kNanRow, 1, sizeof(kNanRow));
+          const i32x4 nan = tfgfa::head_desc(kNanRow, 1, sizeof(kNanRow));
+          const int r = lane >> 3;
 #pragma unroll
           for (int dh = 0; dh < kDH; ++dh)
-            tfgfa::lds_transfer(nd, k_to + dh * kHalfBytes,
-                                koff[g][dh] == kOutOfRange || (lane >> 3) >= rows ? kOutOfRange : koff[g][dh] - (lane >> 3) * (int)s.ks.n);
+            tfgfa::lds_transfer(nan, there + dh * kHalfBytes,
+                                koff[g][dh] == kOutOfRange || r >= rows ? kOutOfRange : koff[g][dh] - r * (int)st.n);
         }
-#pragma unroll
-        for (int dh = 0; dh < kDH; ++dh) tfgfa::lds_transfer(vd, v_to + dh * kHalfBytes, voff[dh]);
       } else {
         const int r = (g0 + g) * kGroup + (lane >> 3), key = at + r;
-        const int page = __shfl(id[0], r);
-        const bool there = key < s.keys, in = there && (uint32_t)page < (uint32_t)s.P;
+        const int page = __shfl(x.id[0], r);
+        const bool seen = key < s.keys, in = seen && (uint32_t)page < (uint32_t)s.P;
         const uint64_t pid = (uint32_t)(in ? page : 0), off = (uint32_t)(in ? key - divide(key, s.by_page) * s.page : 0);
-        const uint64_t kr = in ? (uint64_t)(uintptr_t)s.k + pid * (uint64_t)s.ks.p + off * (uint64_t)s.ks.n
-                               : (uint64_t)(uintptr_t)(there ? kNanRow : kZeroRow);
-        const uint64_t vr = in ? (uint64_t)(uintptr_t)s.v + pid * (uint64_t)s.vs.p + off * (uint64_t)s.vs.n
-                               : (uint64_t)(uintptr_t)kZeroRow;
         const uint64_t zero = (uint64_t)(uintptr_t)kZeroRow;
+        const uint64_t row = in ? (uint64_t)(uintptr_t)base + pid * (uint64_t)st.p + off * (uint64_t)st.n
+                                : !kValue && seen ? (uint64_t)(uintptr_t)kNanRow : zero;
 #pragma unroll
         for (int dh = 0; dh < kDH; ++dh) {
-          lds_gather(koff[g][dh] == kOutOfRange ? zero : kr + koff[g][dh], k_to + dh * kHalfBytes);
-          lds_gather(voff[dh] == kOutOfRange ? zero : vr + voff[dh], v_to + dh * kHalfBytes);
+          const int at_lane = kValue ? voff[dh] : koff[g][dh];
+          lds_gather(at_lane == kOutOfRange ? zero : row + at_lane, there + dh * kHalfBytes);
         }
       }
     }
@@ -339,14 +345,8 @@ struct State {
     return __builtin_bit_cast(v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 
-  // Weights p of tile t as operands, and their sums.
-  __device__ __forceinline__ void split(const f32x16& p, int t, v8 (&part)[kParts][2], bool want_l) {
-    if (kParts > 1 || want_l) {
-      float a = p[0], b = p[1];
-#pragma unroll
-      for (int r = 2; r < 16; r += 2) a += p[r], b += p[r + 1];
-      l[t] += a + b;
-    }
+  // Weights as operands.
+  static __device__ __forceinline__ void parts_of(const float* p, v8 (&part)[kParts][2]) {
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -363,15 +363,29 @@ struct State {
           if (n + 1 < kParts) x -= (float)y;
         }
       }
-    if (kParts == 1) {
-      float a = lp[t], b = 0.f;
+  }
+  static __device__ __forceinline__ float sum16(const float* p) {
+    float a = p[0], b = p[1];
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        a = Elem<T>::add2(v2{part[0][0][e], part[0][0][e + 1]}, a);
-        b = Elem<T>::add2(v2{part[0][1][e], part[0][1][e + 1]}, b);
-      }
-      lp[t] = a + b;
+    for (int r = 2; r < 16; r += 2) a += p[r], b += p[r + 1];
+    return a + b;
+  }
+  // x and the sum of the weights as rounded (of two parts: the first).
+  static __device__ __forceinline__ float add_rounded(const v8 (&part)[kParts][2], float x) {
+    float y = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      x = Elem<T>::add2(v2{part[0][0][e], part[0][0][e + 1]}, x);
+      y = Elem<T>::add2(v2{part[0][1][e], part[0][1][e + 1]}, y);
     }
+    return x + y;
+  }
+  __device__ __forceinline__ void split(const f32x16& w, int t, v8 (&part)[kParts][2]) {
+    float p[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) p[r] = w[r];
+    l[t] += sum16(p);
+    parts_of(p, part);
   }
 
   // O^T += V^T P^T.
@@ -427,22 +441,100 @@ struct State {
 
   // One block; at: its first key; least: keys that every row of the wave sees.
   template <bool kExact>
-  __device__ __forceinline__ void step(const unsigned char* block, int at, int least, float c, float inv_c, bool want_l,
+  __device__ __forceinline__ void step(const unsigned char* k, const unsigned char* v, int at, int least, float c, float inv_c,
                                        int lane) {
     f32x16 s[kRT];
-    offset_scores(s, block, at, least, c, inv_c, lane);
+    offset_scores(s, k, at, least, c, inv_c, lane);
 #pragma unroll
     for (int t = 0; t < kRT; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[t][r] = __builtin_amdgcn_exp2f(s[t][r] * c);
     if constexpr (kExact) {
-      output_exact(block + kDH * kHalfBytes, s, lane);
+      output_exact(v, s, lane);
     } else {
       v8 part[kRT][kParts][2];
 #pragma unroll
-      for (int t = 0; t < kRT; ++t) split(s[t], t, part[t], want_l);
-      output(block + kDH * kHalfBytes, part);
+      for (int t = 0; t < kRT; ++t) split(s[t], t, part[t]);
+      output(v, part);
     }
+  }
+
+  // Many rows (kRT = 1): blocks in a pipeline.  s: the scores of block u; part: the weights of block u - 1; v, k: V of block
+  // u - 1 and K of block u + 1 in LDS.  The products of V run beside the exponentials, those of K beside the weights' sums
+  // and rounding, one matrix instruction and a share of them at a time (a wave's VALU work overlaps its own matrix
+  // instructions).  Offsets are in the log2 domain (m = thr): 2^(c s - m) is one v_fma and one v_exp.
+  // The sum of the rounded weights tells when an offset has to move: a weight past the type's range, or a sum past kBound,
+  // is infinite, NaN or above it.  Where c s passes float32's range (scores past 2.3e38 / scale), `far` asks for the exact
+  // pass.
+  static constexpr float kBound = std::is_same_v<T, __bf16> ? 0x1p64f : 0x1.fffffep127f;
+  template <bool kPV, bool kLse>
+  __device__ __forceinline__ void fused(const unsigned char* v, const unsigned char* k, f32x16& s, v8 (&part)[kParts][2],
+                                        float c, float head, bool* far) {
+    constexpr int kPairs = 2 * kOT;
+    v8 vo[2], ko[2];
+    if constexpr (kPV) vo[0] = values(v, 0, 0), vo[1] = values(v, 1, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    float p[16];
+    const float neg = -m[0];
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const int cc = i / kOT, j = i % kOT;
+      if constexpr (kPV)
+#pragma unroll
+        for (int n = 0; n < kParts; ++n) o[0][j] = Elem<T>::mfma(vo[i & 1], part[n][cc], o[0][j]);
+      if (i + 2 < kPairs) {
+        if constexpr (kPV) vo[i & 1] = values(v, (i + 2) % kOT, (i + 2) / kOT);
+      } else {
+        ko[i + 2 - kPairs] = key_operand(k, i + 2 - kPairs);
+      }
+#pragma unroll
+      for (int r = 16 * i / kPairs; r < 16 * (i + 1) / kPairs; ++r) {
+        p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, neg));
+        asm volatile("" : "+v"(p[r]));  // (here, though the rare branch takes them again)
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    f32x16 next;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) next[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kC; ++i) {
+      next = Elem<T>::mfma(ko[i & 1], q[0][i], next);
+      if (i + 2 < kC) ko[i & 1] = key_operand(k, i + 2);
+      if (i == 0) {
+        parts_of(p, part);
+#pragma unroll
+        for (int n = 0; n < kParts; ++n) asm volatile("" : "+v"(part[n][0]), "+v"(part[n][1]));
+      } else if (i == 1) {
+        float sum = add_rounded(part, lp[0]);
+        // (As integers: past the bound, infinite or NaN.)
+        if (__builtin_amdgcn_ballot_w64(__float_as_uint(sum) > __float_as_uint(kBound))) {
+          const float top = over_pair(largest(s), [](float x, float y) { return fmaxf(x, y); });
+          const float at = top * c;
+          *far = *far || (fabsf(top) < INFINITY && !(fabsf(at) < INFINITY));
+          const float to = fmaxf(fmaxf(m[0], kLowest), at - head);
+          const float f = __builtin_amdgcn_exp2f(m[0] - to);
+          m[0] = to, lp[0] *= f, l[0] *= f;
+#pragma unroll
+          for (int j = 0; j < kOT; ++j) o[0][j] *= f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -to));
+          parts_of(p, part);
+          sum = add_rounded(part, lp[0]);
+        }
+        lp[0] = sum;
+        asm volatile("" : "+v"(lp[0]));
+      }
+      if (i == 2 && kLse) {
+        l[0] += sum16(p);
+        asm volatile("" : "+v"(l[0]));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    s = next;
+  }
+  __device__ __forceinline__ v8 key_operand(const unsigned char* k, int c) const {
+    return *reinterpret_cast<const v8*>(k + (c >> 2) * kHalfBytes + koff[c & 3]);
   }
 
   // Whether some sum of the wave is NaN.
@@ -455,6 +547,20 @@ struct State {
 #pragma unroll
         for (int r = 0; r < 16; ++r) x = fmaf(o[t][j][r], 0.f, x);
     return __builtin_amdgcn_ballot_w64(x != x) != 0;
+  }
+
+  // Many rows: the offset from the log2 domain to scores without the scale.  What rounding it there leaves, m c - to, goes
+  // into the sums, so that it is exact.
+  __device__ __forceinline__ void rescale(float c) {
+    if (!(fabsf(m[0]) < INFINITY)) return;
+    if (m[0] <= kLowest) {  // scores of -inf alone
+      m[0] = -INFINITY;
+      return;
+    }
+    const float to = m[0] / c, f = __builtin_amdgcn_exp2f(-fmaf(to, c, -m[0]));
+    m[0] = to, l[0] *= f, lp[0] *= f;
+#pragma unroll
+    for (int j = 0; j < kOT; ++j) o[0][j] *= f;
   }
 
   // Into LDS: rows of 64 kDH floats, 16-byte piece c of row r at place c ^ r % pieces; statistics beside.
@@ -488,7 +594,6 @@ struct Job {
   int seen, causal;               // row r sees the keys below seen (+ r / G + 1, causal)
   int first, last;
   float scale, scale_log2;
-  bool want_l;
 };
 
 // Where its rows go: the outputs, or (part) its part of them: D floats a row of sums, and of each row the offset and the
@@ -506,10 +611,7 @@ constexpr int few_lds(int kDH, int kRT, int stages) {
   const int ring = kWaves * stages * 2 * kDH * kHalfBytes, rows = kWaves * kRT * kBlock * 64 * kDH * 4;
   return ring > rows ? ring : rows;
 }
-constexpr int many_lds(int kDH, int stages) {
-  const int ring = stages * 4 * kDH * kHalfBytes, rows = kManyRows * 64 * kDH * 4;
-  return ring > rows ? ring : rows;
-}
+constexpr int many_lds(int kDH) { return kManyRows * 64 * kDH * 4; }  // the rows, and four tiles of 64 keys
 constexpr int kMaxRows = kWaves * 2 * kBlock;  // of statistics: four waves of 64 rows
 
 struct Stats {
@@ -603,29 +705,32 @@ __device__ __forceinline__ void run_few(const Source& src, const Job& job, const
   const float inv = 1.f / job.scale_log2;
   w.init(lane);
   Loader<kDH, kAligned, 4> in;
+  typename Loader<kDH, kAligned, 4>::Ids ids = {};
   in.init(src, D, 0, lane);
+  auto issue = [&](int n, uint32_t to) {
+    in.template issue<false>(src, key(n), ids, to);
+    in.template issue<true>(src, key(n), ids, to + kBytes / 2);
+    if (n + 1 < count) ids = in.look_up(src, key(n + 1));
+  };
+  const int least = job.causal ? job.seen + divide(job.row0, job.by_group) + 1 : job.seen;
   auto pass = [&](auto exact) {
-    if (count > 0) in.look_up(src, key(0));
+    if (count > 0) ids = in.look_up(src, key(0));
 #pragma unroll
     for (int n = 0; n < kStages - 1; ++n)
-      if (n < count) {
-        in.issue(src, key(n), ring_at + n * kBytes);
-        if (n + 1 < count) in.look_up(src, key(n + 1));
-      }
+      if (n < count) issue(n, ring_at + n * kBytes);
     if (!decltype(exact)::value) load_rows(w, job, job.row0, D, lane);
-    const int least = job.causal ? job.seen + divide(job.row0, job.by_group) + 1 : job.seen;
     int stage = 0;
 #pragma unroll 1
     for (int n = 0; n < count; ++n) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of the stage that is filled next
       if (n + kStages - 1 < count) {
-        in.issue(src, key(n + kStages - 1), ring_at + (stage == 0 ? kStages - 1 : stage - 1) * kBytes);
-        if (n + kStages < count) in.look_up(src, key(n + kStages));
+        issue(n + kStages - 1, ring_at + (stage == 0 ? kStages - 1 : stage - 1) * kBytes);
         tfgfa::wait_vmcnt<(kStages - 1) * kLoads>();
       } else {
         tfgfa::wait_vmcnt<0>();
       }
-      w.template step<decltype(exact)::value>(ring + stage * kBytes, key(n), least, job.scale_log2, inv, true, lane);
+      const unsigned char* const block = ring + stage * kBytes;
+      w.template step<decltype(exact)::value>(block, block + kBytes / 2, key(n), least, job.scale_log2, inv, lane);
       stage = stage + 1 == kStages ? 0 : stage + 1;
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -643,63 +748,126 @@ __device__ __forceinline__ void run_few(const Source& src, const Job& job, const
     if (e % (8 * kDH) * 8 < D) put<T, kDH, kWaves>(lds, st, kRows, e / (8 * kDH), e % (8 * kDH), job, to, D, kRows);
 }
 
-// Many rows.
-template <class T, int kDH, bool kAligned, int kParts, int kStages>
+// Many rows.  Two K tiles and two V tiles of 64 keys in LDS.  Step j of the workgroup: block 2j; wait for K of tile j + 1 and
+// V of tile j, barrier, load V of tile j + 1 and K of tile j + 2; block 2j + 1.
+template <class T, int kDH, bool kAligned, int kParts, bool kLse>
 __device__ __forceinline__ void run_many(const Source& src, const Job& job, const Sink& to, int D, unsigned char* lds, Stats& st) {
-  constexpr int kLoads = 4 * kDH;                       // transfers of a wave and tile
-  constexpr int kBytes = 2 * kDH * kHalfBytes;          // of a block
-  __shared__ int sh_nan;
+  constexpr int kHalf = kDH * kHalfBytes, kSlot = 2 * kHalf;  // K (or V) of a block, of a tile
+  constexpr bool kKeepL = kLse || kParts > 1;                 // the sum of unrounded weights
+  typedef State<T, kDH, 1, kParts> W;
+  __shared__ int sh_again;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const uint32_t ring_at = tfgfa::lds_addr(lds);
-  const int tiles = (job.last - job.first + 1) / 2;
-  auto key = [&](int n) { return job.first * kBlock + n * kTile; };
-  State<T, kDH, 1, kParts> w;
-  const float inv = 1.f / job.scale_log2;
+  const int blocks = max(0, job.last - job.first), tiles = (blocks + 1) / 2;
+  auto key = [&](int tile) { return job.first * kBlock + tile * kTile; };
+  W w;
+  const float c = job.scale_log2;
   w.init(lane);
-  if (tid == 0) sh_nan = 0;
-  Loader<kDH, kAligned, 2> in;                          // 16 keys of a tile: half a block
+  if (tid == 0) sh_again = 0;
+  typedef Loader<kDH, kAligned, 2> In;                        // 16 keys of a tile: half a block
+  In in;
   in.init(src, D, (wave & 1) * 2, lane);
-  const int mine = (wave >> 1) * kBlock;                // the block's first key in the tile
+  const int mine = (wave >> 1) * kBlock;                      // the block's first key in the tile
   const int r0 = job.row0 + wave * kBlock, r1 = min(job.rows, r0 + kBlock) - 1;
   const int least = r0 >= job.rows ? 0 : job.causal ? job.seen + divide(r0, job.by_group) + 1 : job.seen;
   const int most = r0 >= job.rows ? 0 : job.causal ? job.seen + divide(r1, job.by_group) + 1 : job.seen;
-  auto issue = [&](int n, int stage) {
-    in.issue(src, key(n) + mine, ring_at + (2 * stage + (wave >> 1)) * kBytes);
-    if (n + 1 < tiles) in.look_up(src, key(n + 1) + mine);
+  // Blocks with a key that some row of the wave sees, and those with none that one does not.
+  const int act = min(blocks, max(0, (most + kBlock - 1) / kBlock - job.first));
+  const int full = min(act, max(0, least / kBlock - job.first));
+  auto issue = [&](auto value, int tile, const typename In::Ids& ids) {
+    constexpr bool kValue = decltype(value)::value;
+    in.template issue<kValue>(src, key(tile) + mine, ids, ring_at + ((kValue ? 2 : 0) + (tile & 1)) * kSlot + (wave >> 1) * kHalf);
   };
-  auto pass = [&](auto exact) {
-    if (tiles > 0) in.look_up(src, key(0) + mine);
-#pragma unroll
-    for (int n = 0; n < kStages - 1; ++n)
-      if (n < tiles) issue(n, n);
-    if (!decltype(exact)::value) load_rows(w, job, r0, D, lane);
-    int stage = 0;
+  auto look_up = [&](int tile) { return in.look_up(src, key(tile) + mine); };
+  const std::false_type keys{};
+  const std::true_type values{};
+
+  typename In::Ids k_ids = {}, v_ids = {};
+  if (tiles > 0) {
+    v_ids = look_up(0);
+    issue(keys, 0, v_ids);
+    issue(values, 0, v_ids);
+  }
+  if (tiles > 1) {
+    v_ids = look_up(1);
+    issue(keys, 1, v_ids);
+  }
+  if (tiles > 2) k_ids = look_up(2);
+  load_rows(w, job, r0, D, lane);
+  tfgfa::wait_vmcnt<0>();
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  w.m[0] = -INFINITY;
+  const float head = fminf(Elem<T>::kHead, 1e30f * c);
+  bool far = false;
+  f32x16 s[1];
+  typename W::v8 part[kParts][2];
+  if (act > 0) w.scores(s, lds, false);
+  // Half a step: block u, V of the one before it and K of the one after it in LDS.
+  auto half = [&](int u, const unsigned char* v, const unsigned char* k, auto first) {
+    constexpr bool kPV = !decltype(first)::value;
+    if (u < act) {
+      if (u >= full) w.mask(s[0], 0, (job.first + u) * kBlock, lane);
+      w.template fused<kPV, kKeepL>(v, k, s[0], part, c, head, &far);
+    } else if (kPV && u == act && u > 0) {
+      typename W::v8 (*const all)[kParts][2] = &part;
+      w.output(v, *reinterpret_cast<typename W::v8 (*)[1][kParts][2]>(all));
+    }
+  };
+  auto step = [&](int j, auto slot, auto first) {
+    constexpr int kS = decltype(slot)::value;
+    unsigned char* const k_here = lds + kS * kSlot;
+    unsigned char* const k_next = lds + (kS ^ 1) * kSlot;
+    unsigned char* const v_here = lds + (2 + kS) * kSlot;
+    unsigned char* const v_last = lds + (2 + (kS ^ 1)) * kSlot;
+    half(2 * j, v_last + kHalf, k_here + kHalf, first);
+    tfgfa::wait_vmcnt<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (j + 1 < tiles) issue(values, j + 1, v_ids);
+    if (j + 2 < tiles) issue(keys, j + 2, k_ids);
+    v_ids = k_ids;
+    if (j + 3 < tiles) k_ids = look_up(j + 3);
+    half(2 * j + 1, v_here, k_next, std::false_type());
+  };
+  const std::integral_constant<int, 0> even{};
+  const std::integral_constant<int, 1> odd{};
+  if (tiles > 0) step(0, even, std::true_type());
+  int j = 1;
+#pragma unroll 1
+  for (; j + 1 < tiles; j += 2) {
+    step(j, odd, std::false_type());
+    step(j + 1, even, std::false_type());
+  }
+  if (j < tiles) step(j, odd, std::false_type());
+  if (act > 0 && act == 2 * tiles) {
+    typename W::v8 (*const all)[kParts][2] = &part;
+    w.output(lds + (2 + ((tiles - 1) & 1)) * kSlot + kHalf, *reinterpret_cast<typename W::v8 (*)[1][kParts][2]>(all));
+  }
+  w.rescale(c);
+  if (kParts > 1) w.lp[0] = w.l[0];
+  w.thr[0] = 0.f;
+  if ((__builtin_amdgcn_ballot_w64(far) != 0 || w.any_nan()) && lane == 0) sh_again = 1;
+  __syncthreads();
+  if (uniform(sh_again)) {
+    // The exact pass: a tile at a time.
+    const float inv = 1.f / c;
+    w.clear();
 #pragma unroll 1
     for (int n = 0; n < tiles; ++n) {
-      if (n + kStages - 2 < tiles && kStages > 2)
-        tfgfa::wait_vmcnt<(kStages - 2) * kLoads>();
-      else
-        tfgfa::wait_vmcnt<0>();
+      const typename In::Ids ids = look_up(n);
+      issue(keys, n, ids);
+      issue(values, n, ids);
+      tfgfa::wait_vmcnt<0>();
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (n + kStages - 1 < tiles) issue(n + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
-#pragma unroll
+#pragma unroll 1
       for (int b = 0; b < 2; ++b) {
         const int at = key(n) + b * kBlock;
-        if (at < most)
-          w.template step<decltype(exact)::value>(lds + (2 * stage + b) * kBytes, at, least, job.scale_log2, inv, job.want_l, lane);
+        if (at < most && 2 * n + b < blocks)
+          w.template step<true>(lds + (n & 1) * kSlot + b * kHalf, lds + (2 + (n & 1)) * kSlot + b * kHalf, at, least, c, inv, lane);
       }
-      stage = stage + 1 == kStages ? 0 : stage + 1;
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __syncthreads();
-  };
-  pass(std::false_type());
-  if (w.any_nan() && lane == 0) sh_nan = 1;
-  __syncthreads();
-  if (uniform(sh_nan)) {
-    w.clear();
-    pass(std::true_type());
   }
+  __syncthreads();
   w.publish(lds + wave * kBlock * 64 * kDH * 4, st.m + wave * kBlock, st.l + wave * kBlock, st.lp + wave * kBlock, lane);
   __syncthreads();
   for (int e = tid; e < kManyRows * 8 * kDH; e += kThreads)
@@ -834,15 +1002,15 @@ enum class Kind { kFew1, kFew2, kMany };
 __host__ __device__ constexpr int rows_of(Kind kind) {
   return kind == Kind::kFew1 ? kBlock : kind == Kind::kFew2 ? 2 * kBlock : kManyRows;
 }
-constexpr int kFewStages = 2, kManyStages = 2;
+constexpr int kFewStages = 2;
 constexpr int lds_of(Kind kind, int kDH) {
-  return kind == Kind::kMany ? many_lds(kDH, kManyStages) : few_lds(kDH, kind == Kind::kFew1 ? 1 : 2, kFewStages);
+  return kind == Kind::kMany ? many_lds(kDH) : few_lds(kDH, kind == Kind::kFew1 ? 1 : 2, kFewStages);
 }
 
-template <class T, int kDH, bool kAligned, Kind kKind, int kParts>
+template <class T, int kDH, bool kAligned, Kind kKind, int kParts, bool kLse>
 __device__ __forceinline__ void run(const Source& src, const Job& job, const Sink& to, int D, unsigned char* lds, Stats& st) {
   if constexpr (kKind == Kind::kMany)
-    run_many<T, kDH, kAligned, kParts, kManyStages>(src, job, to, D, lds, st);
+    run_many<T, kDH, kAligned, kParts, kLse>(src, job, to, D, lds, st);
   else
     run_few<T, kDH, kAligned, kKind == Kind::kFew1 ? 1 : 2, kFewStages>(src, job, to, D, lds, st);
 }
@@ -856,8 +1024,8 @@ __device__ __forceinline__ void share(Job* job, int blocks, int s, int S) {
   job->last = min(blocks, kRound * (int)((long long)rounds * (s + 1) / S));
 }
 
-template <class T, int kDH, bool kAligned, Kind kKind>
-__global__ __launch_bounds__(kThreads) void attend_kernel(const AttendArgs a) {
+template <class T, int kDH, bool kAligned, Kind kKind, bool kLse>
+__global__ __launch_bounds__(kThreads, kKind == Kind::kMany ? 2 : 1) void attend_kernel(const AttendArgs a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[lds_of(kKind, kDH)];
   __shared__ Stats st;
   constexpr int kRows = rows_of(kKind);
@@ -874,7 +1042,7 @@ __global__ __launch_bounds__(kThreads) void attend_kernel(const AttendArgs a) {
   job.q_step = a.qs.n, job.q_head = a.qs.h;
   job.by_group = a.by_group, job.G = a.G, job.row0 = tile * kRows, job.rows = fits ? n * a.G : 0;
   job.seen = fits ? len : 0, job.causal = a.causal;
-  job.scale = a.scale, job.scale_log2 = a.scale_log2, job.want_l = a.lse != nullptr;
+  job.scale = a.scale, job.scale_log2 = a.scale_log2;
   const int top = min(job.rows, job.row0 + kRows) - 1;
   const int keys = job.row0 >= job.rows ? 0 : a.causal ? len + divide(top, a.by_group) + 1 : len;
   share<kKind>(&job, (keys + kBlock - 1) / kBlock, s, a.parts);
@@ -887,7 +1055,7 @@ __global__ __launch_bounds__(kThreads) void attend_kernel(const AttendArgs a) {
   to.l_step = 1, to.l_head = a.N;
   to.part = a.parts > 1 ? a.part + (unit * a.parts + s) * kRows * (a.D + 3) : nullptr;
   to.fill_to = a.N * a.G, to.fill = !fits ? 2 : a.pad;
-  run<T, kDH, kAligned, kKind, 1>(src, job, to, a.D, lds, st);
+  run<T, kDH, kAligned, kKind, 1, kLse>(src, job, to, a.D, lds, st);
 }
 
 template <class T, Kind kKind>
@@ -947,7 +1115,7 @@ __global__ __launch_bounds__(kThreads) void shared_kernel(const SharedArgs a) {
   Sink to;
   job.by_group = a.by_group, job.G = a.G, job.causal = 0;
   job.q_step = a.qs.b, job.q_head = a.qs.h;
-  job.scale = a.scale, job.scale_log2 = a.scale_log2, job.want_l = true;
+  job.scale = a.scale, job.scale_log2 = a.scale_log2;
   to.o = nullptr, to.o_step = to.o_head = 0, to.lse = nullptr, to.l_step = to.l_head = 0, to.fill_to = to.fill = 0;
   const bool prefix = (int)blockIdx.x < a.prefix_jobs;
   const int idx = prefix ? blockIdx.x : blockIdx.x - a.prefix_jobs;
@@ -965,7 +1133,7 @@ __global__ __launch_bounds__(kThreads) void shared_kernel(const SharedArgs a) {
     job.row0 = tile * kRows, job.rows = a.each * a.G, job.seen = src.keys;
     share<kKind>(&job, (src.keys + kBlock - 1) / kBlock, s, parts);
     to.part = a.prefix_part + (((long long)head * a.prefix_tiles + tile) * parts + s) * kRows * (a.D + 3);
-    run<T, kDH, kAligned, kKind, 2>(src, job, to, a.D, lds, st);
+    run<T, kDH, kAligned, kKind, 2, true>(src, job, to, a.D, lds, st);
   } else {
     constexpr int kRows = rows_of(Kind::kFew1);
     const int append = a.kn != nullptr, len = ((uniform_ints)a.lens)[b];
@@ -992,7 +1160,7 @@ __global__ __launch_bounds__(kThreads) void shared_kernel(const SharedArgs a) {
     job.row0 = tile * kRows, job.rows = a.G, job.seen = src.keys;
     share<Kind::kFew1>(&job, (src.keys + kBlock - 1) / kBlock, s, parts);
     to.part = a.own_part + (((long long)head * a.own_tiles + tile) * parts + s) * kRows * (a.D + 3);
-    run<T, kDH, kAligned, Kind::kFew1, 2>(src, job, to, a.D, lds, st);
+    run<T, kDH, kAligned, Kind::kFew1, 2, true>(src, job, to, a.D, lds, st);
   }
 }
 
@@ -1061,11 +1229,13 @@ template <class T, int kDH, bool kAligned>
 static void launch_attend(const AttendArgs& a, const AttendPlan& x, hipStream_t stream) {
   const dim3 grid((unsigned)(x.jobs * x.parts));
   if (x.kind == Kind::kFew1)
-    hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kFew1>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kFew1, true>), grid, dim3(kThreads), 0, stream, a);
   else if (x.kind == Kind::kFew2)
-    hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kFew2>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kFew2, true>), grid, dim3(kThreads), 0, stream, a);
+  else if (a.lse)
+    hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kMany, true>), grid, dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kMany>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kMany, false>), grid, dim3(kThreads), 0, stream, a);
 }
 template <class T>
 static hipError_t launch_attend(const AttendArgs& a, const AttendPlan& x, hipStream_t stream) {
