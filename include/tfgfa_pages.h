@@ -74,7 +74,8 @@ int tfpages_append(const void* k, const int64_t* k_strides, const void* v, const
  * rows do not fit M * page, O and LSE of the sequence's N tokens are NaN; a page id outside [0, P) among the rows that a
  * token sees gives it NaN.
  * Weights are rounded to the element type for the product with V where there are more than 64 query rows (tokens x H /
- * H_kv), as tfgfa_fwd does; with fewer, and for the sums, they are float32.
+ * H_kv), as tfgfa_fwd does, and divided by the sum of the rounded ones; with fewer they go through the product in two parts
+ * (all but 2^-16 of a weight in bf16, 2^-22 in fp16).  LSE takes the unrounded ones.
  * workspace (16-byte aligned, device memory, no initialisation): tfpages_attend_workspace bytes let the rows of long
  * caches be divided over several workgroups; fewer (or NULL) is correct but slower.  Calls sharing a workspace must be
  * ordered on one stream, without another thread's call between the launches of one.
@@ -96,6 +97,8 @@ size_t tfpages_attend_workspace(int B, int H, int H_kv, int N, int page, int M, 
  * empty rows are as for tfserve_decode_paged.  B is a multiple of R.
  * Visible on the device only: a length that does not fit, or a page id outside [0, P) among the rows, gives NaN to
  * the sequence, or to the whole group if it is the prefix's.
+ * Weights of a prefix are rounded to the element type for the product with V, as tfpages_attend does, where a group has
+ * more than 64 query rows (B / R x H / H_kv).
  * workspace (16-byte aligned, device memory, no initialisation): tfpages_decode_shared_workspace bytes, which the call
  * needs (TFGFA_ERR_SCRATCH otherwise).  Calls sharing a workspace must be ordered on one stream, without another
  * thread's call between the launches of one.

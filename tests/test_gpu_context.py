@@ -7,7 +7,8 @@ type, as worst cases of the sums:
     X is the row's largest scale * sum |q_d k_d|, and the offset (scaled) is a score of the row, so within X, less 13 ln 2 or
     0; scale, log2 e and their product add 4 u (|x| + |lse|).  Together ex.
   * a weight relative to its row's sum is off by twice e^ex - 1, at most 4.2 ex; sums of L terms by (L + 16) u.
-  * the weights' rounding for the product with V: with up to 64 rows a key-value head two parts, 2^-16 (bf16: cut off at 2^-7,
+  * the weights' rounding for the product with V: with up to 64 rows a key-value head (tokens, or a group's sequences, times
+    the query heads it is shared by) two parts, 2^-16 (bf16: cut off at 2^-7,
     the rest rounded) or 2^-22 (fp16) of each; with more rows one rounding, half, of each and of their sum: 2 half.  fp16 keeps
     weights to 2^-38 of the largest."""
 import math
@@ -420,7 +421,7 @@ def _run_shared(H, H_kv, D, page, dtype, prefix, own, append, rows_first=False, 
             k, v = torch.cat([k, kn[b][:, None]], 1), torch.cat([v, vn[b][:, None]], 1)
             pid, off = int(table[b, own[b] // page]), own[b] % page
             k0[pid, :, off], v0[pid, :, off] = kn[b], vn[b]
-        ro, rl, eo, el = attend(q[b][:, None], k, v, [k.shape[1]], D ** -0.5, dtype, False)
+        ro, rl, eo, el = attend(q[b][:, None], k, v, [k.shape[1]], D ** -0.5, dtype, n * H // H_kv > 64)
         _near_o(o[b][:, None], ro, eo, dtype, f"{b}: {prefix[b // n]} + {own[b]} o")
         _near(lse[b][:, None], rl, el, "lse")
     assert torch.equal(_bits(pool.k), _bits(k0)) and torch.equal(_bits(pool.v), _bits(v0)), "pool"
@@ -516,7 +517,7 @@ def test_decode_shared_infinite_values_and_nan_queries(n):
     texts[2][1][0, 3, 6] = 0
     for b, heads in ((0, [0]), (1, [0, 1]), (2, [0, 1]), (n - 1, [0, 1])):
         ro, rl, eo, el = attend(q[b, heads][:, None], torch.cat([k, texts[b][0]], 1), torch.cat([v, texts[b][1]], 1), [509],
-                                D ** -0.5, BF, False)
+                                D ** -0.5, BF, n * H // H_kv > 64)
         got = o[b, heads].clone()
         assert (got[:, 5] == INF).all() and (b != 2 or (got[:, 6] == -INF).all())
         bad = [5, 6] if b == 2 else [5]

@@ -60,7 +60,7 @@ constexpr int kGroup = 8;                     // keys of a transfer
 constexpr int kHalfBytes = kBlock * 128;      // K or V of a block, 64 dims
 constexpr int kManyRows = kWaves * kBlock;    // rows of a workgroup for many rows
 constexpr int kTile = 2 * kBlock;             // keys of its tile
-constexpr int kMaxParts = 64;                 // workgroups of a job
+constexpr int kMaxParts = 32;                 // workgroups of a job
 constexpr int kOutOfRange = 0x7FFFFFF0;       // a buffer offset past any num_records: the load gives zeros
 // Many rows: an offset is no lower, so that scores of -inf have weight 0 beside it.
 constexpr float kLowest = -0x1.fffffep127f;
@@ -236,7 +236,6 @@ struct State {
   v8 q[kRT][kC];
   f32x16 o[kRT][kOT];
   float m[kRT], thr[kRT];   // offset, and how far a score may pass it (-inf: the row has no weight yet)
-  f32x16 below[kRT];        // -m, what the products start from
   float l[kRT], lp[kRT];    // this lane's sums of weights; kParts 1: of the rounded ones
   int seen[kRT];            // keys that the row sees
   int koff[4], voff[2][2];  // LDS offsets of the operands, in a block's first 64 dims
@@ -259,28 +258,21 @@ struct State {
     for (int t = 0; t < kRT; ++t) {
       m[t] = l[t] = lp[t] = 0.f, thr[t] = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) below[t][r] = 0.f;
-#pragma unroll
       for (int j = 0; j < kOT; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[t][j][r] = 0.f;
     }
   }
 
-  // S^T of the block in LDS, from c on.
-  __device__ __forceinline__ void scores(f32x16 (&s)[kRT], const unsigned char* block, bool offset) const {
+  // S^T of the block in LDS.
+  __device__ __forceinline__ void scores(f32x16 (&s)[kRT], const unsigned char* block) const {
 #pragma unroll
-    for (int t = 0; t < kRT; ++t) {
-      if (offset) {
-        s[t] = below[t];
-      } else {
+    for (int t = 0; t < kRT; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
-      }
-    }
+      for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
-      const v8 a = *reinterpret_cast<const v8*>(block + (c >> 2) * kHalfBytes + koff[c & 3]);
+      const v8 a = key_operand(block, c);
 #pragma unroll
       for (int t = 0; t < kRT; ++t) s[t] = Elem<T>::mfma(a, q[t][c], s[t]);
     }
@@ -293,40 +285,23 @@ struct State {
     return fmaxf(x, s[15]);
   }
 
-  // Scores less their offsets.  The matrix products start from -m, so the difference costs nothing and is exact for near
-  // scores of any size.  Where an offset has to move, the scores are taken again from 0: what a far offset left of them
-  // may be coarse.  c: scale_log2.
-  __device__ __forceinline__ void offset_scores(f32x16 (&s)[kRT], const unsigned char* block, int at, int least, float c,
-                                                float inv_c, int lane) {
-    const bool some = at + kBlock > least;
-    auto hide = [&]() {
-      if (some)
+  // Few rows, and the exact pass: weights 2^(c (s - m)) of tile t in place.  (The difference first, which is exact for near
+  // scores of any size.)  c: scale_log2.
+  __device__ __forceinline__ void weigh(f32x16& s, int t, float c, float inv_c) {
+    const float mx = largest(s);
+    if (__builtin_amdgcn_ballot_w64(mx - m[t] >= thr[t])) {
+      const float top = over_pair(mx, [](float x, float y) { return fmaxf(x, y); });
+      const bool fresh = thr[t] == -INFINITY, none = top == -INFINITY;  // no weight so far; none here
+      const float to = none ? m[t] : fmaxf(fresh ? -INFINITY : m[t], top - fminf(Elem<T>::kHead * inv_c, 1e30f));
+      const float f = fresh ? 0.f : __builtin_amdgcn_exp2f((m[t] - to) * c);
+      m[t] = to;
+      if (!none) thr[t] = fminf((Elem<T>::kHead + Elem<T>::kMargin) * inv_c, 1e30f);
+      l[t] *= f, lp[t] *= f;
 #pragma unroll
-        for (int t = 0; t < kRT; ++t) mask(s[t], t, at, lane);
-    };
-    scores(s, block, true);
-    hide();
-    bool over = false;
-#pragma unroll
-    for (int t = 0; t < kRT; ++t) over = over || largest(s[t]) >= thr[t];
-    if (__builtin_amdgcn_ballot_w64(over)) {
-      scores(s, block, false);
-      hide();
-#pragma unroll
-      for (int t = 0; t < kRT; ++t) {
-        const float top = over_pair(largest(s[t]), [](float x, float y) { return fmaxf(x, y); });
-        const bool fresh = thr[t] == -INFINITY, none = top == -INFINITY;  // no weight so far; none here
-        const float to = none ? m[t] : fmaxf(fresh ? -INFINITY : m[t], top - fminf(Elem<T>::kHead * inv_c, 1e30f));
-        const float f = fresh ? 0.f : __builtin_amdgcn_exp2f((m[t] - to) * c);
-        m[t] = to;
-        if (!none) thr[t] = fminf((Elem<T>::kHead + Elem<T>::kMargin) * inv_c, 1e30f);
-        l[t] *= f, lp[t] *= f;
-#pragma unroll
-        for (int j = 0; j < kOT; ++j) o[t][j] *= f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] -= to, below[t][r] = -to;
-      }
+      for (int j = 0; j < kOT; ++j) o[t][j] *= f;
     }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f((s[r] - m[t]) * c);
   }
 
   // Scores of keys that a row does not see; at: the block's first key.
@@ -444,11 +419,12 @@ struct State {
   __device__ __forceinline__ void step(const unsigned char* k, const unsigned char* v, int at, int least, float c, float inv_c,
                                        int lane) {
     f32x16 s[kRT];
-    offset_scores(s, k, at, least, c, inv_c, lane);
+    scores(s, k);
+    if (at + kBlock > least)
 #pragma unroll
-    for (int t = 0; t < kRT; ++t)
+      for (int t = 0; t < kRT; ++t) mask(s[t], t, at, lane);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[t][r] = __builtin_amdgcn_exp2f(s[t][r] * c);
+    for (int t = 0; t < kRT; ++t) weigh(s[t], t, c, inv_c);
     if constexpr (kExact) {
       output_exact(v, s, lane);
     } else {
@@ -801,7 +777,7 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
   bool far = false;
   f32x16 s[1];
   typename W::v8 part[kParts][2];
-  if (act > 0) w.scores(s, lds, false);
+  if (act > 0) w.scores(s, lds);
   // Half a step: block u, V of the one before it and K of the one after it in LDS.
   auto half = [&](int u, const unsigned char* v, const unsigned char* k, auto first) {
     constexpr bool kPV = !decltype(first)::value;
@@ -875,11 +851,13 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
 }
 
 // ---------------------------------------------------------------------------------------
-// Joining the parts of a job's rows: 16 lanes a row, 8 dims a lane.
+// Joining the parts of a job's rows: 16 lanes, 8 dims each, take every kSplit-th part of a row; kSplit such groups a row.
 
 constexpr int kLanes = kMaxD / 8;
+constexpr int kSplit = 4;
+constexpr int kJoinRows = kThreads / kLanes / kSplit;  // rows of a workgroup
 constexpr int kMine = kMaxParts / kLanes;  // parts whose statistics a lane has
-constexpr int kAtOnce = 4;                 // parts whose sums are loaded together (divides kLanes)
+constexpr int kAtOnce = kLanes / kSplit;   // parts whose sums a thread loads together
 
 // A row's parts: `count` of them, `stride` floats apart, the sums of part 0 at `sums` (this lane's dims) and its offset at
 // `stats` (the sums of weights kRows and 2 kRows further).
@@ -907,9 +885,12 @@ struct Joined {
   float M, l, lp;
 };
 
-// The sum over kSources lists of parts; c: the lane of the row.  (Dims past D: any that are there.)
+// The sum over kSources lists of parts, in the lanes of a row's first group; c: the lane in its group.  Every thread of the
+// workgroup comes here.  (Dims past D: any that are there.)
 template <int kSources>
-__device__ __forceinline__ Joined join(const Parts (&from)[kSources], int c, float scale_log2) {
+__device__ __forceinline__ Joined join(const Parts (&from)[kSources], float scale_log2) {
+  __shared__ f32x4 sh_sum[kThreads][2];
+  const int tid = threadIdx.x, c = tid % kLanes, group = tid / kLanes % kSplit;
   Joined y = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}, -INFINITY, 0.f, 0.f};
   float f[kSources][kMine], l[kSources][kMine], lp[kSources][kMine];
 #pragma unroll
@@ -940,24 +921,29 @@ __device__ __forceinline__ Joined join(const Parts (&from)[kSources], int c, flo
     for (int i = 0; i < kMine; ++i) {
       const int here = min(kLanes, from[n].count - i * kLanes);
       const float* const first = from[n].sums + i * kLanes * from[n].stride;
-      for (int s0 = 0; s0 < here; s0 += kAtOnce) {
-        f32x4 u[kAtOnce], v[kAtOnce];
-        float w[kAtOnce];
+      if (here <= 0) continue;
+      f32x4 u[kAtOnce], v[kAtOnce];
+      float w[kAtOnce];
 #pragma unroll
-        for (int s = 0; s < kAtOnce; ++s) {
-          const float* const at = first + min(s0 + s, here - 1) * from[n].stride;
-          u[s] = *reinterpret_cast<const f32x4*>(at), v[s] = *reinterpret_cast<const f32x4*>(at + 4);
-          w[s] = __shfl(f[n][i], s0 + s, kLanes);  // (past `here` there is a weight of 0: no part)
-        }
-#pragma unroll
-        for (int s = 0; s < kAtOnce; ++s)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            y.a[e] = w[s] == 0.f ? y.a[e] : fmaf(w[s], u[s][e], y.a[e]);
-            y.b[e] = w[s] == 0.f ? y.b[e] : fmaf(w[s], v[s][e], y.b[e]);
-          }
+      for (int s = 0; s < kAtOnce; ++s) {
+        const int at = s * kSplit + group;
+        const float* const row = first + min(at, here - 1) * from[n].stride;
+        u[s] = *reinterpret_cast<const f32x4*>(row), v[s] = *reinterpret_cast<const f32x4*>(row + 4);
+        w[s] = __shfl(f[n][i], at, kLanes);  // (past `here` there is a weight of 0: no part)
       }
+#pragma unroll
+      for (int s = 0; s < kAtOnce; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y.a[e] = w[s] == 0.f ? y.a[e] : fmaf(w[s], u[s][e], y.a[e]);
+          y.b[e] = w[s] == 0.f ? y.b[e] : fmaf(w[s], v[s][e], y.b[e]);
+        }
     }
+  sh_sum[tid][0] = y.a, sh_sum[tid][1] = y.b;
+  __syncthreads();
+  if (group == 0)
+#pragma unroll
+    for (int g = 1; g < kSplit; ++g) y.a += sh_sum[tid + g * kLanes][0], y.b += sh_sum[tid + g * kLanes][1];
   return y;
 }
 
@@ -1002,9 +988,13 @@ enum class Kind { kFew1, kFew2, kMany };
 __host__ __device__ constexpr int rows_of(Kind kind) {
   return kind == Kind::kFew1 ? kBlock : kind == Kind::kFew2 ? 2 * kBlock : kManyRows;
 }
-constexpr int kFewStages = 2;
+constexpr int few_stages(Kind kind) { return kind == Kind::kFew1 ? 1 : 2; }
 constexpr int lds_of(Kind kind, int kDH) {
-  return kind == Kind::kMany ? many_lds(kDH) : few_lds(kDH, kind == Kind::kFew1 ? 1 : 2, kFewStages);
+  return kind == Kind::kMany ? many_lds(kDH) : few_lds(kDH, kind == Kind::kFew1 ? 1 : 2, few_stages(kind));
+}
+
+constexpr int simd_waves(Kind kind, int kDH) {
+  return kind == Kind::kMany ? 2 : kind == Kind::kFew1 ? (kDH == 1 ? 4 : 2) : (kDH == 1 ? 2 : 1);
 }
 
 template <class T, int kDH, bool kAligned, Kind kKind, int kParts, bool kLse>
@@ -1012,7 +1002,7 @@ __device__ __forceinline__ void run(const Source& src, const Job& job, const Sin
   if constexpr (kKind == Kind::kMany)
     run_many<T, kDH, kAligned, kParts, kLse>(src, job, to, D, lds, st);
   else
-    run_few<T, kDH, kAligned, kKind == Kind::kFew1 ? 1 : 2, kFewStages>(src, job, to, D, lds, st);
+    run_few<T, kDH, kAligned, kKind == Kind::kFew1 ? 1 : 2, few_stages(kKind)>(src, job, to, D, lds, st);
 }
 
 // Part s of S of `blocks` blocks: whole rounds of the workgroup.
@@ -1025,7 +1015,7 @@ __device__ __forceinline__ void share(Job* job, int blocks, int s, int S) {
 }
 
 template <class T, int kDH, bool kAligned, Kind kKind, bool kLse>
-__global__ __launch_bounds__(kThreads, kKind == Kind::kMany ? 2 : 1) void attend_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(kThreads, simd_waves(kKind, kDH)) void attend_kernel(const AttendArgs a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[lds_of(kKind, kDH)];
   __shared__ Stats st;
   constexpr int kRows = rows_of(kKind);
@@ -1060,21 +1050,19 @@ __global__ __launch_bounds__(kThreads, kKind == Kind::kMany ? 2 : 1) void attend
 
 template <class T, Kind kKind>
 __global__ __launch_bounds__(kThreads) void attend_join_kernel(const AttendArgs a) {
-  constexpr int kRows = rows_of(kKind), kEach = kThreads / kLanes;
-  const int c = threadIdx.x % kLanes;
-  const int unit = blockIdx.x / (kRows / kEach), row = (int)(blockIdx.x % (kRows / kEach)) * kEach + (int)threadIdx.x / kLanes;
+  constexpr int kRows = rows_of(kKind), kBlocks = kRows / kJoinRows;
+  const int c = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const int unit = blockIdx.x / kBlocks, row = (int)(blockIdx.x % kBlocks) * kJoinRows + group / kSplit;
   const int head = unit / a.tiles, tile = unit - head * a.tiles, b = head / a.Hkv, kv = head - b * a.Hkv;
   const int r = tile * kRows + row, step = divide(r, a.by_group), h = kv * a.G + r - step * a.G;
-  if (step >= a.N) return;
   const int len = a.lens[b], n = a.lengths ? a.lengths[b] : a.N;
   const bool fits = len >= 0 && n >= 0 && n <= a.N && (long long)len + (a.causal ? n : 0) <= a.n_max;
   const bool past = fits && step >= n;
-  if (past && !a.pad) return;
-  const bool real = fits && !past;
   const int d = 8 * c < a.D ? c : 0;
   Parts p[1] = {parts_of(a.part, unit, a.parts, kRows, row, a.D, d)};
-  if (!real) p[0].count = 0;
-  const Joined y = join(p, c, a.scale_log2);
+  if (!fits || step >= n) p[0].count = 0;
+  const Joined y = join(p, a.scale_log2);
+  if (group % kSplit != 0 || step >= a.N || (past && !a.pad)) return;
   if (8 * c < a.D) store_row(static_cast<T*>(a.o) + b * a.os.b + h * a.os.h + step * a.os.n + 8 * c, y, past, !fits);
   if (c == 0 && a.lse) a.lse[((long long)b * a.Hkv * a.G + h) * a.N + step] = row_lse(y, a.scale, past, !fits);
 }
@@ -1107,7 +1095,7 @@ struct SharedArgs {
 };
 
 template <class T, int kDH, bool kAligned, Kind kKind>
-__global__ __launch_bounds__(kThreads) void shared_kernel(const SharedArgs a) {
+__global__ __launch_bounds__(kThreads, simd_waves(kKind, kDH)) void shared_kernel(const SharedArgs a) {
   constexpr int kPrefixLds = lds_of(kKind, kDH), kOwnLds = lds_of(Kind::kFew1, kDH);
   __shared__ __attribute__((aligned(1024))) unsigned char lds[kPrefixLds > kOwnLds ? kPrefixLds : kOwnLds];
   __shared__ Stats st;
@@ -1133,7 +1121,7 @@ __global__ __launch_bounds__(kThreads) void shared_kernel(const SharedArgs a) {
     job.row0 = tile * kRows, job.rows = a.each * a.G, job.seen = src.keys;
     share<kKind>(&job, (src.keys + kBlock - 1) / kBlock, s, parts);
     to.part = a.prefix_part + (((long long)head * a.prefix_tiles + tile) * parts + s) * kRows * (a.D + 3);
-    run<T, kDH, kAligned, kKind, 2, true>(src, job, to, a.D, lds, st);
+    run<T, kDH, kAligned, kKind, 1, true>(src, job, to, a.D, lds, st);
   } else {
     constexpr int kRows = rows_of(Kind::kFew1);
     const int append = a.kn != nullptr, len = ((uniform_ints)a.lens)[b];
@@ -1167,8 +1155,8 @@ __global__ __launch_bounds__(kThreads) void shared_kernel(const SharedArgs a) {
 template <class T, Kind kKind>
 __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs a, int rows) {
   constexpr int kRows = rows_of(kKind);
-  const int c = threadIdx.x % kLanes, at = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
-  if (at >= rows) return;
+  const int c = threadIdx.x % kLanes, group = threadIdx.x / kLanes, mine = blockIdx.x * kJoinRows + group / kSplit;
+  const int at = min(mine, rows - 1);
   const int H = a.Hkv * a.G, b = at / H, h = at - b * H, kv = h / a.G, g = h - kv * a.G, r = b / a.each;
   const int plen = a.prefix_lens[r], len = a.lens[b];
   const bool fits = plen >= 0 && plen <= a.prefix_max && len >= 0 && len <= a.n_max - (a.kn ? 1 : 0);
@@ -1177,7 +1165,8 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
   Parts p[2] = {
       parts_of(a.prefix_part, ((long long)r * a.Hkv + kv) * a.prefix_tiles + row / kRows, a.prefix_parts, kRows, row % kRows, a.D, d),
       parts_of(a.own_part, ((long long)b * a.Hkv + kv) * a.own_tiles + g / kBlock, a.own_parts, kBlock, g % kBlock, a.D, d)};
-  const Joined y = join(p, c, a.scale_log2);
+  const Joined y = join(p, a.scale_log2);
+  if (group % kSplit != 0 || mine >= rows) return;
   if (8 * c < a.D) store_row(static_cast<T*>(a.o) + b * a.os.b + h * a.os.h + 8 * c, y, false, !fits);
   if (c == 0 && a.lse) a.lse[at] = row_lse(y, a.scale, false, !fits);
 }
@@ -1190,11 +1179,11 @@ constexpr int kCu = 256;  // workgroups are counted for this many CUs, so that a
 static Kind choose_kind(long long rows) {
   return rows <= kBlock ? Kind::kFew1 : rows <= 2 * kBlock ? Kind::kFew2 : Kind::kMany;
 }
-// Workgroups that a job of up to n_max keys is divided over, where there are `jobs` of them.
-static int choose_parts(Kind kind, long long jobs, long long n_max) {
-  const long long least = kind == Kind::kMany ? 512 : 256;  // keys of a part
-  const long long want = 2 * kCu / std::max(1LL, jobs), most = n_max / least;
-  return (int)std::max(1LL, std::min({want, most, (long long)kMaxParts}));
+// Workgroups that a job of up to n_max keys is divided over, where there are `jobs` of them: `slots` a CU in all, parts of at
+// least `least` keys.
+static int choose_parts(long long slots, long long jobs, long long n_max, long long least) {
+  const long long parts = std::min({slots * kCu / std::max(1LL, jobs), n_max / least, (long long)kMaxParts});
+  return (int)std::max(1LL, parts);
 }
 static size_t part_bytes(Kind kind, long long jobs, int parts, int D) {
   return ((size_t)jobs * parts * rows_of(kind) * (D + 3) * 4 + 255) / 256 * 256;
@@ -1220,9 +1209,10 @@ static bool attend_plan(int B, int H, int Hkv, int N, int page, int M, int D, At
   x->tiles = (rows + each - 1) / each;
   if (x->tiles > INT32_MAX / ((long long)B * Hkv)) return false;
   x->jobs = x->tiles * B * Hkv;
-  x->parts = choose_parts(x->kind, x->jobs, n_max);
+  x->parts = choose_parts(x->kind == Kind::kFew2 ? 1 : 2, x->jobs, n_max, 256);
+  if (x->parts < 4 && n_max < 4096) x->parts = 1;
   x->bytes = x->parts > 1 ? part_bytes(x->kind, x->jobs, x->parts, D) : 0;
-  return x->jobs * x->parts <= INT32_MAX && x->jobs <= INT32_MAX / kManyRows;
+  return x->jobs * x->parts <= INT32_MAX && x->jobs <= INT32_MAX / kManyRows;  // (workgroups of either kernel)
 }
 
 template <class T, int kDH, bool kAligned>
@@ -1246,7 +1236,7 @@ static hipError_t launch_attend(const AttendArgs& a, const AttendPlan& x, hipStr
     aligned ? launch_attend<T, 2, true>(a, x, stream) : launch_attend<T, 2, false>(a, x, stream);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || x.parts == 1) return e;
-  const dim3 grid((unsigned)(x.jobs * (rows_of(x.kind) / (kThreads / kLanes))));
+  const dim3 grid((unsigned)(x.jobs * (rows_of(x.kind) / kJoinRows)));
   if (x.kind == Kind::kFew1)
     hipLaunchKernelGGL((attend_join_kernel<T, Kind::kFew1>), grid, dim3(kThreads), 0, stream, a);
   else if (x.kind == Kind::kFew2)
@@ -1272,8 +1262,8 @@ static bool shared_plan(int R, int B, int H, int Hkv, int page, int Mp, int M, i
   x->own_tiles = (G + kBlock - 1) / kBlock;
   x->prefix_jobs = x->prefix_tiles * R * Hkv;
   x->own_jobs = x->own_tiles * B * Hkv;
-  x->prefix_parts = choose_parts(x->kind, x->prefix_jobs, p_max);
-  x->own_parts = choose_parts(Kind::kFew1, x->own_jobs, n_max);
+  x->prefix_parts = choose_parts(x->kind == Kind::kFew1 ? 2 : 1, x->prefix_jobs, p_max, x->kind == Kind::kMany ? 512 : 128);
+  x->own_parts = choose_parts(2, x->own_jobs, n_max, 128);
   x->own_at = part_bytes(x->kind, x->prefix_jobs, x->prefix_parts, D);
   x->bytes = x->own_at + part_bytes(Kind::kFew1, x->own_jobs, x->own_parts, D);
   return x->prefix_jobs * x->prefix_parts + x->own_jobs * x->own_parts <= INT32_MAX;
@@ -1298,7 +1288,7 @@ static hipError_t launch_shared(const SharedArgs& a, const SharedPlan& x, int ro
     aligned ? launch_shared<T, 2, true>(a, x, stream) : launch_shared<T, 2, false>(a, x, stream);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const dim3 grid((rows + kThreads / kLanes - 1) / (kThreads / kLanes));
+  const dim3 grid((rows + kJoinRows - 1) / kJoinRows);
   if (x.kind == Kind::kFew1)
     hipLaunchKernelGGL((shared_join_kernel<T, Kind::kFew1>), grid, dim3(kThreads), 0, stream, a, rows);
   else if (x.kind == Kind::kFew2)

@@ -12,7 +12,11 @@
 //
 // Bound: HBM, every element read and written once.  A workgroup takes some tokens with all their heads: sines and
 // cosines of a token are computed once, into LDS, for all heads of queries and keys, as is where its rows lie (a
-// row's page among it); then each thread moves 16 bytes of a head, or two times 16 of a pair of halves.
+// row's page among it); then each thread moves the same 16 bytes of each token, or two times 16 of a pair of halves, so that
+// heads and places in them are told apart once.  (Told apart for each piece, 57 and 100 us for the appends below.)
+// Measured, from memory, us and TB/s read and written: 32001 tokens of 32 + 8 heads, half of each rotated, fp16, 132 (5.0;
+// a copy of as many bytes 127); 2 chunks of 8192 tokens into pages, queries too, 80 (5.0); 16 prompts of up to 1024 tokens,
+// 25 heads, into pages 31.3 (3.8: 40% of the padded batch's tokens are looked at and left); 8 tokens 3.2.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -34,7 +38,7 @@ constexpr int kThreads = 256;
 constexpr int kMaxD = 128;
 constexpr int kMaxTokens = 16;   // of a workgroup
 constexpr int kTensors = 3;      // of a launch
-constexpr int kItems = 4;        // of a thread in flight
+constexpr int kItems = 2;        // tokens of a thread in flight
 
 // One tensor of the launch.  Its heads' vectors are moved in items: `turned` of them rotate pairs, then `single` copy an
 // element each from dim r on, and `wide` copy 16 bytes.
@@ -56,6 +60,7 @@ struct Args {
   int rot, N, tokens;                // tokens: B * N
   int each, parts, count;            // tokens of a workgroup, workgroups that share them, tensors
   int items;                         // of a token
+  int side, slots;                   // tokens that the workgroup's threads take side by side; rounds of threads for them
   tfgfa::Division by_items;
   // Pages (tensors 0 and 1, K and V; tensor 2 is Q).
   const int* table;
@@ -115,7 +120,7 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(const Args a, int inte
     sh_sin[t * pairs + i] = s * a.magnitude * a.sign;
   }
   // The last threads, which have the fewest angles to compute, find the rows.
-  if (tid >= kThreads - kMaxTokens && kThreads - 1 - tid < here) {
+  if (kThreads - 1 - tid < here) {
     const int t = kThreads - 1 - tid, b = (u0 + t) / a.N, n = u0 + t - b * a.N;
 #pragma unroll
     for (int s = 0; s < kTensors; ++s) {
@@ -143,85 +148,90 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(const Args a, int inte
   }
   __syncthreads();
 
-  const int all = here * a.items;
-  for (int first = part * (kThreads * kItems); first < all; first += a.parts * (kThreads * kItems)) {
-    wide lo[kItems], hi[kItems];
-    E* to[kItems];
-    int at_lo[kItems], at_hi[kItems], angle[kItems], fate[kItems];  // at_hi: -1 no second piece, -2 one element; angle: -1 a copy
-#pragma unroll
-    for (int m = 0; m < kItems; ++m) {
-      const int item = first + m * kThreads + tid;
-      fate[m] = kSkip;
-      if (item >= all) continue;
-      const int t = divide(item, a.by_items);
-      int i = item - t * a.items;
-      const int s = a.count > 2 && i >= a.t[2].first ? 2 : a.count > 1 && i >= a.t[1].first ? 1 : 0;
-      // (Selected field by field: a pointer to one of the three would put the arguments in memory.)
-      auto of = [&](auto f) { return s == 2 ? f(a.t[2]) : s == 1 ? f(a.t[1]) : f(a.t[0]); };
-      i -= of([](const Tensor& x) { return x.first; });
-      const int turned = of([](const Tensor& x) { return x.turned; }), single = of([](const Tensor& x) { return x.single; });
-      const int per = turned + single + of([](const Tensor& x) { return x.wide; });
-      const int h = (int)(((float)i + 0.5f) * __builtin_amdgcn_rcpf((float)per));  // exact: i < 2^21
-      i -= h * per;
-      fate[m] = sh_fate[s][t];
-      const E* const x = static_cast<const E*>(of([](const Tensor& z) { return z.x; })) + sh_x[s][t] +
-                         h * of([](const Tensor& z) { return z.xh; });
-      to[m] = static_cast<E*>(of([](const Tensor& z) { return z.y; })) + sh_y[s][t] + h * of([](const Tensor& z) { return z.yh; });
-      angle[m] = -1;
-      if (i < turned) {
-        angle[m] = t * pairs + i * kEach;
-        if constexpr (kPairs == Pairs::kHalves) {
-          at_lo[m] = i * kWide, at_hi[m] = i * kWide + pairs;
-        } else if constexpr (kPairs == Pairs::kNeighbours) {
-          at_lo[m] = i * kWide, at_hi[m] = -1;
-        } else {
-          at_lo[m] = interleaved ? 2 * i : i, at_hi[m] = interleaved ? 2 * i + 1 : i + pairs;
-        }
-      } else if (i < turned + single) {
-        at_lo[m] = (turned ? a.rot : 0) + i - turned, at_hi[m] = -2;
+  // Each thread takes the same place of every `side`-th token: what tells the places apart is worked out once for them all.
+  for (int slot = part; slot < a.slots; slot += a.parts) {
+    const int place = slot * kThreads + tid, t0 = divide(place, a.by_items);
+    if (t0 >= a.side) continue;
+    int i = place - t0 * a.items;
+    const int s = a.count > 2 && i >= a.t[2].first ? 2 : a.count > 1 && i >= a.t[1].first ? 1 : 0;
+    // (Selected field by field: a pointer to one of the three would put the arguments in memory.)
+    auto of = [&](auto f) { return s == 2 ? f(a.t[2]) : s == 1 ? f(a.t[1]) : f(a.t[0]); };
+    i -= of([](const Tensor& z) { return z.first; });
+    const int turned = of([](const Tensor& z) { return z.turned; }), single = of([](const Tensor& z) { return z.single; });
+    const int per = turned + single + of([](const Tensor& z) { return z.wide; });
+    const int h = (int)(((float)i + 0.5f) * __builtin_amdgcn_rcpf((float)per));  // exact: i < 2^21
+    i -= h * per;
+    const bool rotates = i < turned;
+    int lo_at, hi_at = 0, angle = 0;
+    bool one = false, two = false;  // an element instead of a piece; a second one
+    if (rotates) {
+      angle = i * kEach;
+      if constexpr (kPairs == Pairs::kHalves) {
+        lo_at = i * kWide, hi_at = lo_at + pairs, two = true;
+      } else if constexpr (kPairs == Pairs::kNeighbours) {
+        lo_at = i * kWide;
       } else {
-        at_lo[m] = (turned ? a.rot : 0) + single + (i - turned - single) * kWide, at_hi[m] = -1;
+        lo_at = interleaved ? 2 * i : i, hi_at = interleaved ? 2 * i + 1 : i + pairs, one = two = true;
       }
-      if (fate[m] != kMove) continue;
-      if (at_hi[m] == -2 || (kPairs == Pairs::kAny && angle[m] >= 0))
-        lo[m][0] = x[at_lo[m]];
-      else
-        lo[m] = *reinterpret_cast<const wide*>(x + at_lo[m]);
-      if constexpr (kPairs == Pairs::kHalves) {
-        if (at_hi[m] >= 0) hi[m] = *reinterpret_cast<const wide*>(x + at_hi[m]);
-      } else if constexpr (kPairs == Pairs::kAny) {
-        if (at_hi[m] >= 0) hi[m][0] = x[at_hi[m]];
-      }
+    } else {
+      const int from = turned ? a.rot : 0;
+      one = i < turned + single;
+      lo_at = one ? from + i - turned : from + single + (i - turned - single) * kWide;
     }
+    const E* const x = static_cast<const E*>(of([](const Tensor& z) { return z.x; })) + h * of([](const Tensor& z) { return z.xh; }) + lo_at;
+    E* const y = static_cast<E*>(of([](const Tensor& z) { return z.y; })) + h * of([](const Tensor& z) { return z.yh; }) + lo_at;
+    const int apart = hi_at - lo_at;
+    for (int t = t0; t < here; t += a.side * kItems) {
+      wide lo[kItems], hi[kItems];
+      int fate[kItems];
 #pragma unroll
-    for (int m = 0; m < kItems; ++m) {
-      if (fate[m] == kSkip) continue;
-      if (fate[m] != kMove) {
-        const E fill = (E)(fate[m] == kNan ? __uint_as_float(0x7FC00000u) : 0.f);
-#pragma unroll
-        for (int e = 0; e < kWide; ++e) lo[m][e] = fill, hi[m][e] = fill;
-      } else if (angle[m] >= 0) {
-        const float* const c = sh_cos + angle[m];
-        const float* const s = sh_sin + angle[m];
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          const bool beside = kPairs == Pairs::kNeighbours;
-          const float xa = (float)lo[m][beside ? 2 * e : e], xb = (float)(beside ? lo[m][2 * e + 1] : hi[m][e]);
-          const E ya = (E)fmaf(xa, c[e], -(xb * s[e])), yb = (E)fmaf(xb, c[e], xa * s[e]);
-          if (beside)
-            lo[m][2 * e] = ya, lo[m][2 * e + 1] = yb;
-          else
-            lo[m][e] = ya, hi[m][e] = yb;
+      for (int m = 0; m < kItems; ++m) {
+        const int u = t + m * a.side;
+        fate[m] = u < here ? (kPaged ? sh_fate[s][u] : (int)kMove) : (int)kSkip;
+        if (fate[m] != kMove) continue;
+        const E* const from = x + sh_x[s][u];
+        if (one)
+          lo[m][0] = from[0];
+        else
+          lo[m] = *reinterpret_cast<const wide*>(from);
+        if constexpr (kPairs == Pairs::kHalves) {
+          if (two) hi[m] = *reinterpret_cast<const wide*>(from + apart);
+        } else if constexpr (kPairs == Pairs::kAny) {
+          if (two) hi[m][0] = from[apart];
         }
       }
-      if (at_hi[m] == -2 || (kPairs == Pairs::kAny && angle[m] >= 0))
-        to[m][at_lo[m]] = lo[m][0];
-      else
-        *reinterpret_cast<wide*>(to[m] + at_lo[m]) = lo[m];
-      if constexpr (kPairs == Pairs::kHalves) {
-        if (at_hi[m] >= 0) *reinterpret_cast<wide*>(to[m] + at_hi[m]) = hi[m];
-      } else if constexpr (kPairs == Pairs::kAny) {
-        if (at_hi[m] >= 0) to[m][at_hi[m]] = hi[m][0];
+#pragma unroll
+      for (int m = 0; m < kItems; ++m) {
+        const int u = t + m * a.side;
+        if (fate[m] == kSkip) continue;
+        if (fate[m] != kMove) {
+          const E fill = (E)(fate[m] == kNan ? __uint_as_float(0x7FC00000u) : 0.f);
+#pragma unroll
+          for (int e = 0; e < kWide; ++e) lo[m][e] = fill, hi[m][e] = fill;
+        } else if (rotates) {
+          const float* const c = sh_cos + u * pairs + angle;
+          const float* const sn = sh_sin + u * pairs + angle;
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) {
+            const bool beside = kPairs == Pairs::kNeighbours;
+            const float xa = (float)lo[m][beside ? 2 * e : e], xb = (float)(beside ? lo[m][2 * e + 1] : hi[m][e]);
+            const E ya = (E)fmaf(xa, c[e], -(xb * sn[e])), yb = (E)fmaf(xb, c[e], xa * sn[e]);
+            if (beside)
+              lo[m][2 * e] = ya, lo[m][2 * e + 1] = yb;
+            else
+              lo[m][e] = ya, hi[m][e] = yb;
+          }
+        }
+        E* const to = y + sh_y[s][u];
+        if (one)
+          to[0] = lo[m][0];
+        else
+          *reinterpret_cast<wide*>(to) = lo[m];
+        if constexpr (kPairs == Pairs::kHalves) {
+          if (two) *reinterpret_cast<wide*>(to + apart) = hi[m];
+        } else if constexpr (kPairs == Pairs::kAny) {
+          if (two) to[apart] = hi[m][0];
+        }
       }
     }
   }
@@ -275,11 +285,16 @@ static int launch(Args a, Pairs pairs, int interleaved, int cu, hipStream_t stre
   if (items == 0) return TFGFA_OK;
   a.items = (int)items;
   a.by_items = tfgfa::division_by(a.items);
-  // Tokens enough for every thread's items in flight, unless CUs would be left idle; then a token's items may be divided.
-  a.each = 1;
-  while (a.each < kMaxTokens && a.each * items < 2 * kThreads * kItems && a.tokens / (2 * a.each) >= 4 * cu) a.each *= 2;
+  a.side = (int)std::max(1LL, kThreads / items);
+  a.slots = (int)((a.side * items + kThreads - 1) / kThreads);
+  // As many tokens a workgroup as leave sixteen workgroups a CU; where there are fewer tokens, their places are divided.
+  // (With 8 a CU 32001 tokens of 40 heads take 145 us, with 16 132, with 32 137, with 64 169; 16 prompts of up to 1024
+  // tokens into pages 33.9, 31.3, 36.8, 55.)
+  a.each = a.side;
+  while (2 * a.each <= kMaxTokens && a.tokens / (2 * a.each) >= 16LL * cu) a.each *= 2;
+  a.each = std::min(a.each, kMaxTokens);
   const long long groups = (a.tokens + a.each - 1) / a.each;
-  a.parts = (int)std::max(1LL, std::min((a.each * items + kThreads * kItems - 1) / (kThreads * kItems), 4LL * cu / groups));
+  a.parts = (int)std::max(1LL, std::min<long long>(a.slots, 4LL * cu / groups));
   if (groups * a.parts > INT32_MAX) return TFGFA_ERR_TOO_LARGE;
   const dim3 grid((unsigned)(groups * a.parts));
   if (pairs == Pairs::kHalves)

@@ -520,7 +520,8 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     Everything else is as for :func:`decode_paged`: the pools, head layouts and types, ``k_new``/``v_new`` ((B, H_kv, D)),
     which become row ``cache_seqlens[b]`` of the sequence's own, ``out``, the lse.  A length that does not fit its table or a
     page id outside the pool yields NaN for the sequence, or for the whole group if it is the prefix's (checked on the
-    device).  ``workspace``: at least ``_C.decode_shared_workspace(R, B, H, H_kv, page, M_prefix, M, D)`` bytes, kept per
+    device).  A prefix's weights are rounded to the type for the product with V, as :func:`attention`'s are, where a group
+    has more than 64 query rows (B / R * H / H_kv).  ``workspace``: at least ``_C.decode_shared_workspace(R, B, H, H_kv, page, M_prefix, M, D)`` bytes, kept per
     device and stream where none is given.
     """
     if not _accepts_shared(q, k_pages, v_pages, prefix_table, prefix_lens, page_table, cache_seqlens, k_new, v_new, out):
