@@ -779,44 +779,65 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
   typename W::v8 part[kParts][2];
   if (act > 0) w.scores(s, lds);
   // Half a step: block u, V of the one before it and K of the one after it in LDS.
-  auto half = [&](int u, const unsigned char* v, const unsigned char* k, auto first) {
-    constexpr bool kPV = !decltype(first)::value;
-    if (u < act) {
-      if (u >= full) w.mask(s[0], 0, (job.first + u) * kBlock, lane);
-      w.template fused<kPV, kKeepL>(v, k, s[0], part, c, head, &far);
-    } else if (kPV && u == act && u > 0) {
-      typename W::v8 (*const all)[kParts][2] = &part;
-      w.output(v, *reinterpret_cast<typename W::v8 (*)[1][kParts][2]>(all));
-    }
+  auto block = [&](int u, const unsigned char* v, const unsigned char* k, auto first) {
+    if (u >= full) w.mask(s[0], 0, (job.first + u) * kBlock, lane);
+    w.template fused<!decltype(first)::value, kKeepL>(v, k, s[0], part, c, head, &far);
   };
-  auto step = [&](int j, auto slot, auto first) {
-    constexpr int kS = decltype(slot)::value;
-    unsigned char* const k_here = lds + kS * kSlot;
-    unsigned char* const k_next = lds + (kS ^ 1) * kSlot;
-    unsigned char* const v_here = lds + (2 + kS) * kSlot;
-    unsigned char* const v_last = lds + (2 + (kS ^ 1)) * kSlot;
-    half(2 * j, v_last + kHalf, k_here + kHalf, first);
+  auto last = [&](const unsigned char* v) {
+    typename W::v8 all[1][kParts][2];
+#pragma unroll
+    for (int n = 0; n < kParts; ++n) all[0][n][0] = part[n][0], all[0][n][1] = part[n][1];
+    w.output(v, all);
+  };
+  auto turn = [&](int j) {  // between the halves of step j
     tfgfa::wait_vmcnt<0>();
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (j + 1 < tiles) issue(values, j + 1, v_ids);
     if (j + 2 < tiles) issue(keys, j + 2, k_ids);
     v_ids = k_ids;
     if (j + 3 < tiles) k_ids = look_up(j + 3);
-    half(2 * j + 1, v_here, k_next, std::false_type());
+  };
+  auto k_of = [&](int slot) { return lds + slot * kSlot; };
+  auto v_of = [&](int slot) { return lds + (2 + slot) * kSlot; };
+  // Steps both of whose blocks the wave computes: no branches, so that the accumulators stay where they are.
+  auto step = [&](int j, auto slot, auto first) {
+    constexpr int kS = decltype(slot)::value;
+    block(2 * j, v_of(kS ^ 1) + kHalf, k_of(kS) + kHalf, first);
+    turn(j);
+    block(2 * j + 1, v_of(kS), k_of(kS ^ 1), std::false_type());
   };
   const std::integral_constant<int, 0> even{};
   const std::integral_constant<int, 1> odd{};
-  if (tiles > 0) step(0, even, std::true_type());
-  int j = 1;
+  const int steady = act / 2;
+  int j = 0;
+  if (steady > 0) {
+    step(0, even, std::true_type());
 #pragma unroll 1
-  for (; j + 1 < tiles; j += 2) {
-    step(j, odd, std::false_type());
-    step(j + 1, even, std::false_type());
+    for (j = 1; j + 1 < steady; j += 2) {
+      step(j, odd, std::false_type());
+      step(j + 1, even, std::false_type());
+    }
+    if (j < steady) {
+      step(j, odd, std::false_type());
+      ++j;
+    }
   }
-  if (j < tiles) step(j, odd, std::false_type());
-  if (act > 0 && act == 2 * tiles) {
-    typename W::v8 (*const all)[kParts][2] = &part;
-    w.output(lds + (2 + ((tiles - 1) & 1)) * kSlot + kHalf, *reinterpret_cast<typename W::v8 (*)[1][kParts][2]>(all));
+  // The wave's last block alone, or what is left of the block before; then loads for the other waves.
+  if (j < tiles) {
+    const unsigned char* const v_last = v_of((j & 1) ^ 1) + kHalf;
+    if (act & 1) {
+      if (act == 1)
+        block(0, v_last, k_of(0) + kHalf, std::true_type());
+      else
+        block(2 * j, v_last, k_of(j & 1) + kHalf, std::false_type());
+    } else if (act > 0) {
+      last(v_last);
+    }
+    turn(j);
+    if (act & 1) last(v_of(j & 1));
+    for (++j; j < tiles; ++j) turn(j);
+  } else if (act > 0) {
+    last(v_of((tiles - 1) & 1) + kHalf);
   }
   w.rescale(c);
   if (kParts > 1) w.lp[0] = w.l[0];
