@@ -1015,7 +1015,7 @@ constexpr int lds_of(Kind kind, int kDH) {
 }
 
 constexpr int simd_waves(Kind kind, int kDH) {
-  return kind == Kind::kMany ? 2 : kind == Kind::kFew1 ? (kDH == 1 ? 4 : 2) : (kDH == 1 ? 2 : 1);
+  return kind == Kind::kMany ? (kDH == 1 ? 3 : 2) : kind == Kind::kFew1 ? (kDH == 1 ? 4 : 2) : (kDH == 1 ? 2 : 1);
 }
 
 template <class T, int kDH, bool kAligned, Kind kKind, int kParts, bool kLse>
