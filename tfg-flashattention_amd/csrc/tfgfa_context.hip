@@ -11,8 +11,8 @@
 //   S^T[key][row] = K Q^T: lane (h, i) holds 16 keys of row i, so the softmax of a row is two lanes' own registers;
 //   O^T[dim][row] += V^T P^T: those 16 values are the B operand as they stand (the keys' order in the contraction is
 //   free), V's operand comes by transposing LDS reads.
-// K and V rows go from their pages to LDS by direct loads, 8 keys a transfer.  Where a page is a multiple of 8 keys, a
-// transfer has one page: its id and address are scalars, and rows past the end are past its descriptor, which gives zeros.
+// K and V rows go from their pages to LDS by direct loads.  Where a page is a multiple of 16 keys, so many have one page: its
+// id and address are scalars, and rows past the end are past its descriptor, which gives zeros.
 // Other pages: each lane has an address, of a row of zeros where there is no key.  A page id outside the pool gives a
 // row of NaN for K, so that NaN reaches the rows that see the key, and zeros for V.
 //
@@ -56,7 +56,7 @@ constexpr int kMaxD = 128;
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kBlock = 32;                    // keys of a block; rows of a wave's tile
-constexpr int kGroup = 8;                     // keys of a transfer
+constexpr int kGroup = 16;                    // keys whose rows are loaded together: of one page, where pages are multiples
 constexpr int kHalfBytes = kBlock * 128;      // K or V of a block, 64 dims
 constexpr int kManyRows = kWaves * kBlock;    // rows of a workgroup for many rows
 constexpr int kTile = 2 * kBlock;             // keys of its tile
@@ -139,84 +139,112 @@ __device__ __forceinline__ void lds_gather(uint64_t from, uint32_t lds_base) {
 
 __device__ __forceinline__ int swz_v(int row) { return (row & 3) << 1; }
 
-// Loads of kGroups groups of 8 keys, from group g0 of a block on.  A block in LDS: K's halves of 64 dims, then V's, each 32
+// Two transfers of one buffer, to LDS bytes `first` and `second` (tfgfa::lds_transfer, with one exchange of M0).
+__device__ __forceinline__ void lds_pair(i32x4 desc, uint32_t first, int off0, uint32_t second, int off1) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %3, %5, 0 offen lds\n\t"
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %4, %5, 0 offen lds\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(first), "s"(second), "v"(off0), "v"(off1), "s"(desc)
+      : "memory");
+}
+
+// Loads of kGroups groups of 16 keys, from group g0 of a block on.  A block in LDS: K's (or V's) halves of 64 dims, each 32
 // rows of 128 bytes; chunk c of row r at place c ^ swz (tfgfa_fwd.hip says why).  Lane l of a transfer fills chunk l % 8
-// of row l / 8 of the group.
+// of row l / 8 of its 8 rows.
 template <int kDH, bool kAligned, int kGroups>
 struct Loader {
-  int koff[kGroups][kDH], voff[kDH];  // aligned: byte offsets from the group's first row; otherwise in a row, or out of range
+  int koff[kGroups][2][kDH], voff[2][kDH];  // aligned: byte offsets from the group's first row; otherwise in a row, or out of range
   int g0, lane;
 
-  // Pages of a block's groups (one for each), or of its keys (lane l: key l % 32).
-  struct Ids {
-    int id[kAligned ? kGroups : 1];
+  // Where a block's rows are: of each group the page and its row in it, or (not aligned) of key l % 32 in lane l the page.
+  struct Place {
+    int page[kAligned ? kGroups : 1], row[kAligned ? kGroups : 1];
   };
 
   __device__ __forceinline__ void init(const Source& s, int D, int g0_, int lane_) {
     g0 = g0_, lane = lane_;
     const int r = lane >> 3, chunks = D >> 3;
 #pragma unroll
-    for (int dh = 0; dh < kDH; ++dh) {
+    for (int dh = 0; dh < kDH; ++dh)
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        const int c = 8 * dh + ((lane & 7) ^ tfgfa::swz_k((g0 + g) * kGroup + r));
-        koff[g][dh] = c < chunks ? (kAligned ? r * (int)s.ks.n : 0) + 16 * c : kOutOfRange;
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          const int c = 8 * dh + ((lane & 7) ^ tfgfa::swz_k((g0 + g) * kGroup + 8 * i + r));
+          koff[g][i][dh] = c < chunks ? (kAligned ? (8 * i + r) * (int)s.ks.n : 0) + 16 * c : kOutOfRange;
+        }
+        const int c = 8 * dh + ((lane & 7) ^ swz_v(r));
+        voff[i][dh] = c < chunks ? (kAligned ? (8 * i + r) * (int)s.vs.n : 0) + 16 * c : kOutOfRange;
       }
-      const int c = 8 * dh + ((lane & 7) ^ swz_v(r));
-      voff[dh] = c < chunks ? (kAligned ? r * (int)s.vs.n : 0) + 16 * c : kOutOfRange;
-    }
   }
-  // The pages of the block at key `at`.
-  __device__ __forceinline__ Ids look_up(const Source& s, int at) const {
-    Ids x;
+  // The place of the block at key `at`.
+  __device__ __forceinline__ Place look_up(const Source& s, int at) const {
+    Place x;
     if constexpr (kAligned) {
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        const int key = at + (g0 + g) * kGroup;
-        x.id[g] = uniform(key < s.keys ? ((uniform_ints)s.table)[divide(key, s.by_page)] : 0);
+        const int key = at + (g0 + g) * kGroup, column = divide(key, s.by_page);
+        x.page[g] = uniform(key < s.keys ? ((uniform_ints)s.table)[column] : 0);
+        x.row[g] = key - column * s.page;
       }
     } else {
       const int key = at + (lane & 31);
-      x.id[0] = key < s.keys ? s.table[divide(key, s.by_page)] : 0;
+      x.page[0] = key < s.keys ? s.table[divide(key, s.by_page)] : 0;
     }
     return x;
   }
   // K (kValue: V) of the block at key `at` to LDS byte `to`.
   template <bool kValue>
-  __device__ __forceinline__ void issue(const Source& s, int at, const Ids& x, uint32_t to) const {
+  __device__ __forceinline__ void issue(const Source& s, int at, const Place& x, uint32_t to) const {
     const Pages& st = kValue ? s.vs : s.ks;
     const char* const base = kValue ? s.v : s.k;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      const uint32_t there = to + (g0 + g) * 1024;
+      const uint32_t there = to + (g0 + g) * 2048;
       if constexpr (kAligned) {
-        const int key = at + (g0 + g) * kGroup, rows = uniform(min(kGroup, max(0, s.keys - key)));
-        const bool in = (uint32_t)x.id[g] < (uint32_t)s.P;
-        const uint64_t pid = (uint32_t)(in ? x.id[g] : 0), off = (uint32_t)(key - divide(key, s.by_page) * s.page);
-        const i32x4 desc = tfgfa::head_desc(base + pid * (uint64_t)st.p + off * (uint64_t)st.n, uniform(in ? rows : 0), (int)st.n);
+        const int rows = uniform(min(kGroup, max(0, s.keys - at - (g0 + g) * kGroup)));
+        const bool in = (uint32_t)x.page[g] < (uint32_t)s.P;
+        const uint64_t page = (uint32_t)(in ? x.page[g] : 0), row = (uint32_t)x.row[g];
+        const i32x4 desc = tfgfa::head_desc(base + page * (uint64_t)st.p + row * (uint64_t)st.n, uniform(in ? rows : 0), (int)st.n);
         if (kValue || in || rows == 0) {
 #pragma unroll
-          for (int dh = 0; dh < kDH; ++dh) tfgfa::lds_transfer(desc, there + dh * kHalfBytes, kValue ? voff[dh] : koff[g][dh]);
+          for (int dh = 0; dh < kDH; ++dh)
+            lds_pair(desc, there + dh * kHalfBytes, kValue ? voff[0][dh] : koff[g][0][dh], there + dh * kHalfBytes + 1024,
+                     kValue ? voff[1][dh] : koff[g][1][dh]);
         } else {
           const i32x4 nan = tfgfa::head_desc(kNanRow, 1, sizeof(kNanRow));
-          const int r = lane >> 3;
 #pragma unroll
           for (int dh = 0; dh < kDH; ++dh)
-            tfgfa::lds_transfer(nan, there + dh * kHalfBytes,
-                                koff[g][dh] == kOutOfRange || r >= rows ? kOutOfRange : koff[g][dh] - r * (int)st.n);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int r = 8 * i + (lane >> 3);
+              tfgfa::lds_transfer(nan, there + dh * kHalfBytes + 1024 * i,
+                                  koff[g][i][dh] == kOutOfRange || r >= rows ? kOutOfRange : koff[g][i][dh] - r * (int)st.n);
+            }
         }
       } else {
-        const int r = (g0 + g) * kGroup + (lane >> 3), key = at + r;
-        const int page = __shfl(x.id[0], r);
-        const bool seen = key < s.keys, in = seen && (uint32_t)page < (uint32_t)s.P;
-        const uint64_t pid = (uint32_t)(in ? page : 0), off = (uint32_t)(in ? key - divide(key, s.by_page) * s.page : 0);
-        const uint64_t zero = (uint64_t)(uintptr_t)kZeroRow;
-        const uint64_t row = in ? (uint64_t)(uintptr_t)base + pid * (uint64_t)st.p + off * (uint64_t)st.n
-                                : !kValue && seen ? (uint64_t)(uintptr_t)kNanRow : zero;
 #pragma unroll
-        for (int dh = 0; dh < kDH; ++dh) {
-          const int at_lane = kValue ? voff[dh] : koff[g][dh];
-          lds_gather(at_lane == kOutOfRange ? zero : row + at_lane, there + dh * kHalfBytes);
+        for (int i = 0; i < 2; ++i) {
+          const int r = (g0 + g) * kGroup + 8 * i + (lane >> 3), key = at + r;
+          const int page = __shfl(x.page[0], r);
+          const bool seen = key < s.keys, in = seen && (uint32_t)page < (uint32_t)s.P;
+          const uint64_t pid = (uint32_t)(in ? page : 0), off = (uint32_t)(in ? key - divide(key, s.by_page) * s.page : 0);
+          const uint64_t zero = (uint64_t)(uintptr_t)kZeroRow;
+          const uint64_t row = in ? (uint64_t)(uintptr_t)base + pid * (uint64_t)st.p + off * (uint64_t)st.n
+                                  : !kValue && seen ? (uint64_t)(uintptr_t)kNanRow : zero;
+#pragma unroll
+          for (int dh = 0; dh < kDH; ++dh) {
+            const int at_lane = kValue ? voff[i][dh] : koff[g][i][dh];
+            lds_gather(at_lane == kOutOfRange ? zero : row + at_lane, there + dh * kHalfBytes + 1024 * i);
+          }
         }
       }
     }
@@ -680,17 +708,17 @@ __device__ __forceinline__ void run_few(const Source& src, const Job& job, const
   State<T, kDH, kRT, 2> w;
   const float inv = 1.f / job.scale_log2;
   w.init(lane);
-  Loader<kDH, kAligned, 4> in;
-  typename Loader<kDH, kAligned, 4>::Ids ids = {};
+  Loader<kDH, kAligned, 2> in;
+  typename Loader<kDH, kAligned, 2>::Place place = {};
   in.init(src, D, 0, lane);
   auto issue = [&](int n, uint32_t to) {
-    in.template issue<false>(src, key(n), ids, to);
-    in.template issue<true>(src, key(n), ids, to + kBytes / 2);
-    if (n + 1 < count) ids = in.look_up(src, key(n + 1));
+    in.template issue<false>(src, key(n), place, to);
+    in.template issue<true>(src, key(n), place, to + kBytes / 2);
+    if (n + 1 < count) place = in.look_up(src, key(n + 1));
   };
   const int least = job.causal ? job.seen + divide(job.row0, job.by_group) + 1 : job.seen;
   auto pass = [&](auto exact) {
-    if (count > 0) ids = in.look_up(src, key(0));
+    if (count > 0) place = in.look_up(src, key(0));
 #pragma unroll
     for (int n = 0; n < kStages - 1; ++n)
       if (n < count) issue(n, ring_at + n * kBytes);
@@ -740,9 +768,9 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
   const float c = job.scale_log2;
   w.init(lane);
   if (tid == 0) sh_again = 0;
-  typedef Loader<kDH, kAligned, 2> In;                        // 16 keys of a tile: half a block
+  typedef Loader<kDH, kAligned, 1> In;                        // 16 keys of a tile: half a block
   In in;
-  in.init(src, D, (wave & 1) * 2, lane);
+  in.init(src, D, wave & 1, lane);
   const int mine = (wave >> 1) * kBlock;                      // the block's first key in the tile
   const int r0 = job.row0 + wave * kBlock, r1 = min(job.rows, r0 + kBlock) - 1;
   const int least = r0 >= job.rows ? 0 : job.causal ? job.seen + divide(r0, job.by_group) + 1 : job.seen;
@@ -750,25 +778,25 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
   // Blocks with a key that some row of the wave sees, and those with none that one does not.
   const int act = min(blocks, max(0, (most + kBlock - 1) / kBlock - job.first));
   const int full = min(act, max(0, least / kBlock - job.first));
-  auto issue = [&](auto value, int tile, const typename In::Ids& ids) {
+  auto issue = [&](auto value, int tile, const typename In::Place& place) {
     constexpr bool kValue = decltype(value)::value;
-    in.template issue<kValue>(src, key(tile) + mine, ids, ring_at + ((kValue ? 2 : 0) + (tile & 1)) * kSlot + (wave >> 1) * kHalf);
+    in.template issue<kValue>(src, key(tile) + mine, place, ring_at + ((kValue ? 2 : 0) + (tile & 1)) * kSlot + (wave >> 1) * kHalf);
   };
   auto look_up = [&](int tile) { return in.look_up(src, key(tile) + mine); };
   const std::false_type keys{};
   const std::true_type values{};
 
-  typename In::Ids k_ids = {}, v_ids = {};
+  typename In::Place k_at = {}, v_at = {};
   if (tiles > 0) {
-    v_ids = look_up(0);
-    issue(keys, 0, v_ids);
-    issue(values, 0, v_ids);
+    v_at = look_up(0);
+    issue(keys, 0, v_at);
+    issue(values, 0, v_at);
   }
   if (tiles > 1) {
-    v_ids = look_up(1);
-    issue(keys, 1, v_ids);
+    v_at = look_up(1);
+    issue(keys, 1, v_at);
   }
-  if (tiles > 2) k_ids = look_up(2);
+  if (tiles > 2) k_at = look_up(2);
   load_rows(w, job, r0, D, lane);
   tfgfa::wait_vmcnt<0>();
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -792,10 +820,10 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
   auto turn = [&](int j) {  // between the halves of step j
     tfgfa::wait_vmcnt<0>();
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (j + 1 < tiles) issue(values, j + 1, v_ids);
-    if (j + 2 < tiles) issue(keys, j + 2, k_ids);
-    v_ids = k_ids;
-    if (j + 3 < tiles) k_ids = look_up(j + 3);
+    if (j + 1 < tiles) issue(values, j + 1, v_at);
+    if (j + 2 < tiles) issue(keys, j + 2, k_at);
+    v_at = k_at;
+    if (j + 3 < tiles) k_at = look_up(j + 3);
   };
   auto k_of = [&](int slot) { return lds + slot * kSlot; };
   auto v_of = [&](int slot) { return lds + (2 + slot) * kSlot; };
@@ -850,9 +878,9 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
     w.clear();
 #pragma unroll 1
     for (int n = 0; n < tiles; ++n) {
-      const typename In::Ids ids = look_up(n);
-      issue(keys, n, ids);
-      issue(values, n, ids);
+      const typename In::Place place = look_up(n);
+      issue(keys, n, place);
+      issue(values, n, place);
       tfgfa::wait_vmcnt<0>();
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll 1
