@@ -76,9 +76,10 @@ extern "C" {
 #define TFGFA_ERR_STRIDE         8  /* strides outside what the entry point takes         */
 #define TFGFA_ERR_CACHE          9  /* k_new/v_new given without cache_seqlens            */
 #define TFGFA_ERR_DTYPE         10  /* dtype is not a TFGFA_DTYPE_* value                 */
-#define TFGFA_ERR_SCRATCH       11  /* tfserve_decode_paged: key_weights and a workspace that does not
-                                       hold its scores (tfgfa_decode_noalloc limits its split to its
-                                       scratch and does not return it)                      */
+#define TFGFA_ERR_SCRATCH       11  /* a workspace that does not hold what the call keeps in it: the scores
+                                       of tfserve_decode_paged with key_weights, the parts of
+                                       tfpages_decode_shared (tfgfa_decode_noalloc limits its split to
+                                       its scratch and does not return it)                    */
 
 /* Element types of q, k, v, o (fp32 accumulation and softmax either way). */
 #define TFGFA_DTYPE_BF16 0

@@ -33,7 +33,7 @@ extern "C" {
  * q, q_out: (B, H, N, D), k, k_out: (B, H_kv, N, D) or all NULL with H_kv 0; strides [b, h, n, d], last dimension
  * dense, the others not negative; what is written must not overlap.  q_out may be q itself with its strides, and k_out
  * k.  positions: int32 or int64 (position_bytes 4 or 8), element [b, n] at b * position_strides[0] + n *
- * position_strides[1]; or NULL: first + n.  D at most 128.
+ * position_strides[1]; or NULL: first + n.  D at most 128, B * N at most 2^27 (TFGFA_ERR_TOO_LARGE).
  */
 int tfpages_rotate(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int H,
                    const void* k, const int64_t* k_strides, void* k_out, const int64_t* k_out_strides, int H_kv,
@@ -51,7 +51,7 @@ int tfpages_rotate(const void* q, const int64_t* q_strides, void* q_out, const i
  * Visible on the device only: where cache_seqlens[b] < 0, n_b is not in [0, N] or their sum is past M * page, nothing
  * is written to the cache for the sequence and its rows of q_out are NaN; a page id outside [0, P) gets no row.
  * dtype: TFGFA_DTYPE_BF16 or TFGFA_DTYPE_F16; D a multiple of 8 up to 128; strides of k, v, q and q_out as for
- * tfserve_key_weights (multiples of 8, rows apart), pointers to 16 bytes.
+ * tfserve_key_weights (multiples of 8, rows apart), pointers to 16 bytes; B * N at most 2^27.
  */
 int tfpages_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, void* k_pages,
                    const int64_t* k_pages_strides, void* v_pages, const int64_t* v_pages_strides,

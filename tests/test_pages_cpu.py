@@ -73,6 +73,7 @@ def _rotate(lib, **kw):
     (dict(N=0), "OK"),
     (dict(H=0), "OK"),
     (dict(B=TOP, N=2), "ERR_TOO_LARGE"),
+    (dict(B=1 << 14, N=(1 << 13) + 1), "ERR_TOO_LARGE"),   # past 2^27 tokens
     (dict(q=0), "ERR_NULL_POINTER"),
     (dict(turns=0), "ERR_NULL_POINTER"),
     (dict(Hkv=2), "ERR_NULL_POINTER"),
@@ -118,7 +119,9 @@ def _append(lib, **kw):
     (dict(B=0), "OK"),
     (dict(N=0), "OK"),
     (dict(Hkv=0), "OK"),
+    (dict(Hkv=0, q=P, qo=P), "ERR_BAD_SHAPE"),
     (dict(B=TOP, N=2), "ERR_TOO_LARGE"),
+    (dict(B=1 << 14, N=(1 << 13) + 1), "ERR_TOO_LARGE"),   # past 2^27 tokens
     (dict(M=1 << 27), "ERR_TOO_LARGE"),
     (dict(k=0), "ERR_NULL_POINTER"),
     (dict(lens=0), "ERR_NULL_POINTER"),
@@ -170,6 +173,7 @@ def _attend(lib, **kw):
     (dict(M=1 << 27), "ERR_TOO_LARGE"),
     (dict(N=TOP), "ERR_TOO_LARGE"),
     (dict(B=TOP), "ERR_TOO_LARGE"),
+    (dict(B=1 << 23), "ERR_TOO_LARGE"),                             # 2^24 workgroups of 256 threads
     (dict(ks=(4096, 1024, 1 << 27, 1), page=1), "ERR_ALIGNMENT"),   # (the stride of one row is not taken)
     (dict(ks=(4096, 1024, 1 << 27, 1)), "ERR_TOO_LARGE"),           # 8 rows past 2^30 bytes
     (dict(q=0), "ERR_NULL_POINTER"),
@@ -216,6 +220,8 @@ def _shared(lib, **kw):
     (dict(H=0), "OK"),
     (dict(Mp=1 << 27), "ERR_TOO_LARGE"),
     (dict(M=1 << 27), "ERR_TOO_LARGE"),
+    (dict(R=1, B=1 << 23), "ERR_TOO_LARGE"),                 # 2^24 workgroups of 256 threads
+    (dict(R=1, B=1 << 22, H=32, Hkv=1), "ERR_TOO_LARGE"),    # and for the join
     (dict(q=0), "ERR_NULL_POINTER"),
     (dict(pl=0), "ERR_NULL_POINTER"),
     (dict(pt=0), "ERR_NULL_POINTER"),

@@ -1225,6 +1225,8 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
 
 constexpr int kCu = 256;  // workgroups are counted for this many CUs, so that a workspace's size does not depend on the device
 
+constexpr long long kMaxGroups = UINT32_MAX / kThreads;  // workgroups of a launch: fewer than 2^32 threads
+
 static Kind choose_kind(long long rows) {
   return rows <= kBlock ? Kind::kFew1 : rows <= 2 * kBlock ? Kind::kFew2 : Kind::kMany;
 }
@@ -1261,7 +1263,7 @@ static bool attend_plan(int B, int H, int Hkv, int N, int page, int M, int D, At
   x->parts = choose_parts(x->kind == Kind::kFew2 ? 1 : 2, x->jobs, n_max, 256);
   if (x->parts < 4 && n_max < 4096) x->parts = 1;
   x->bytes = x->parts > 1 ? part_bytes(x->kind, x->jobs, x->parts, D) : 0;
-  return x->jobs * x->parts <= INT32_MAX && x->jobs <= INT32_MAX / kManyRows;  // (workgroups of either kernel)
+  return x->jobs * x->parts <= kMaxGroups;  // (the join has at most kManyRows / kJoinRows a job, of few jobs)
 }
 
 template <class T, int kDH, bool kAligned>
@@ -1303,8 +1305,7 @@ struct SharedPlan {
 };
 static bool shared_plan(int R, int B, int H, int Hkv, int page, int Mp, int M, int D, SharedPlan* x) {
   const long long n_max = (long long)M * page, p_max = (long long)Mp * page, G = H / Hkv, rows = B / R * G;
-  if (n_max > INT32_MAX - (1 << 20) || p_max > INT32_MAX - (1 << 20) || rows > INT32_MAX - kManyRows ||
-      (long long)B * H > INT32_MAX - kThreads)
+  if (n_max > INT32_MAX - (1 << 20) || p_max > INT32_MAX - (1 << 20) || rows > INT32_MAX - kManyRows)
     return false;
   x->kind = choose_kind(rows);
   x->prefix_tiles = (rows + rows_of(x->kind) - 1) / rows_of(x->kind);
@@ -1315,7 +1316,7 @@ static bool shared_plan(int R, int B, int H, int Hkv, int page, int Mp, int M, i
   x->own_parts = choose_parts(2, x->own_jobs, n_max, 128);
   x->own_at = part_bytes(x->kind, x->prefix_jobs, x->prefix_parts, D);
   x->bytes = x->own_at + part_bytes(Kind::kFew1, x->own_jobs, x->own_parts, D);
-  return x->prefix_jobs * x->prefix_parts + x->own_jobs * x->own_parts <= INT32_MAX;
+  return x->prefix_jobs * x->prefix_parts + x->own_jobs * x->own_parts <= kMaxGroups && (long long)B * H <= kMaxGroups * kJoinRows;
 }
 
 template <class T, int kDH, bool kAligned>

@@ -37,6 +37,7 @@ using tfgfa::Rows;
 constexpr int kThreads = 256;
 constexpr int kMaxD = 128;
 constexpr int kMaxTokens = 16;   // of a workgroup
+constexpr int kMaxRun = 1 << 27;  // of a launch: workgroups of more than kMaxTokens / 2 then have fewer than 2^32 threads
 constexpr int kTensors = 3;      // of a launch
 constexpr int kItems = 2;        // tokens of a thread in flight
 
@@ -295,7 +296,6 @@ static int launch(Args a, Pairs pairs, int interleaved, int cu, hipStream_t stre
   a.each = std::min(a.each, kMaxTokens);
   const long long groups = (a.tokens + a.each - 1) / a.each;
   a.parts = (int)std::max(1LL, std::min<long long>(a.slots, 4LL * cu / groups));
-  if (groups * a.parts > INT32_MAX) return TFGFA_ERR_TOO_LARGE;
   const dim3 grid((unsigned)(groups * a.parts));
   if (pairs == Pairs::kHalves)
     hipLaunchKernelGGL((rotate_kernel<E, Pairs::kHalves, kPaged>), grid, dim3(kThreads), 0, stream, a, interleaved);
@@ -326,7 +326,7 @@ extern "C" int tfpages_rotate(const void* q, const int64_t* q_strides, void* q_o
   if (D < 1 || D > kMaxD || rot < 0 || rot > D || (rot & 1)) return TFGFA_ERR_HEAD_DIM;
   if (!(magnitude > 0.f) || !isfinite(magnitude)) return TFGFA_ERR_SCALE;
   if (B == 0 || N == 0 || (H == 0 && H_kv == 0)) return TFGFA_OK;
-  if ((long long)B * N > INT32_MAX - kMaxTokens) return TFGFA_ERR_TOO_LARGE;
+  if ((long long)B * N > kMaxRun) return TFGFA_ERR_TOO_LARGE;
   if (rot > 0 && !turns) return TFGFA_ERR_NULL_POINTER;
   if (positions && !position_strides) return TFGFA_ERR_NULL_POINTER;
   const uintptr_t size = dtype == TFPAGES_DTYPE_F32 ? 4 : 2;
@@ -382,9 +382,10 @@ extern "C" int tfpages_append(const void* k, const int64_t* k_strides, const voi
   if (D < 8 || D > kMaxD || (D & 7) || rot < 0 || rot > D || (rot & 1)) return TFGFA_ERR_HEAD_DIM;
   if (!(magnitude > 0.f) || !isfinite(magnitude)) return TFGFA_ERR_SCALE;
   if ((q == nullptr) != (q_out == nullptr)) return TFGFA_ERR_NULL_POINTER;
+  if (H_kv == 0 && q && H > 0) return TFGFA_ERR_BAD_SHAPE;  // queries of a cache without heads
   if (B == 0 || N == 0 || H_kv == 0) return TFGFA_OK;
   const long long n_max = (long long)M * page;
-  if ((long long)B * N > INT32_MAX - kMaxTokens || n_max > INT32_MAX - kMaxTokens) return TFGFA_ERR_TOO_LARGE;
+  if ((long long)B * N > kMaxRun || n_max > INT32_MAX - kMaxTokens) return TFGFA_ERR_TOO_LARGE;
   if (!k || !v || !k_pages || !v_pages || !cache_seqlens || (!page_table && M > 0) || !k_strides || !v_strides ||
       !k_pages_strides || !v_pages_strides || (rot > 0 && !turns))
     return TFGFA_ERR_NULL_POINTER;
