@@ -43,6 +43,7 @@ using tfgfa::Pages;
 using tfgfa::Rows;
 using tfgfa::Vecs;
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -615,7 +616,7 @@ constexpr int few_lds(int kDH, int kRT, int stages) {
   const int ring = kWaves * stages * 2 * kDH * kHalfBytes, rows = kWaves * kRT * kBlock * 64 * kDH * 4;
   return ring > rows ? ring : rows;
 }
-constexpr int many_lds(int kDH) { return kManyRows * 64 * kDH * 4; }  // the rows, and four tiles of 64 keys
+constexpr int many_lds(int kDH) { return 4 * kDH * 2 * kHalfBytes; }  // four tiles of 64 keys
 constexpr int kMaxRows = kWaves * 2 * kBlock;  // of statistics: four waves of 64 rows
 
 struct Stats {
@@ -643,23 +644,23 @@ __device__ __forceinline__ void load_rows(State<T, kDH, kRT, kParts>& w, const J
   }
 }
 
-// Row `row` of the workgroup's kRows rows, 8 dims from 8 c8 on, joined over kJoin waves' states (stride: rows apart), to its
+// Few rows: row `row` of the workgroup's kRows rows, 8 dims from 8 c8 on, joined over the waves' states (kRows apart), to its
 // place.
-template <class T, int kDH, int kJoin>
-__device__ __forceinline__ void put(const unsigned char* rows, const Stats& st, int stride, int row, int c8, const Job& job,
-                                    const Sink& to, int D, int kRows) {
+template <class T, int kDH, int kRows>
+__device__ __forceinline__ void put(const unsigned char* rows, const Stats& st, int row, int c8, const Job& job,
+                                    const Sink& to, int D) {
   constexpr int kPieces = 16 * kDH;
   const int r = job.row0 + row;
   const bool real = r < job.rows;
   if (!real && !(to.part == nullptr && to.fill != 0 && r < to.fill_to)) return;
   float M = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kJoin; ++w) M = fmaxf(M, st.m[w * stride + row]);
+  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, st.m[w * kRows + row]);
   float l = 0.f, lp = 0.f;
   f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int w = 0; w < kJoin; ++w) {
-    const int at = w * stride + row;
+  for (int w = 0; w < kWaves; ++w) {
+    const int at = w * kRows + row;
     const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((st.m[at] - M) * job.scale_log2);
     l = fmaf(f, st.l[at], l), lp = fmaf(f, st.lp[at], lp);
     const f32x4 x = *reinterpret_cast<const f32x4*>(rows + (at * kPieces + ((2 * c8) ^ (at % kPieces))) * 16);
@@ -749,13 +750,13 @@ __device__ __forceinline__ void run_few(const Source& src, const Job& job, const
   w.publish(lds + wave * kRows * 64 * kDH * 4, st.m + wave * kRows, st.l + wave * kRows, st.lp + wave * kRows, lane);
   __syncthreads();
   for (int e = tid; e < kRows * 8 * kDH; e += kThreads)
-    if (e % (8 * kDH) * 8 < D) put<T, kDH, kWaves>(lds, st, kRows, e / (8 * kDH), e % (8 * kDH), job, to, D, kRows);
+    if (e % (8 * kDH) * 8 < D) put<T, kDH, kRows>(lds, st, e / (8 * kDH), e % (8 * kDH), job, to, D);
 }
 
 // Many rows.  Two K tiles and two V tiles of 64 keys in LDS.  Step j of the workgroup: block 2j; wait for K of tile j + 1 and
 // V of tile j, barrier, load V of tile j + 1 and K of tile j + 2; block 2j + 1.
 template <class T, int kDH, bool kAligned, int kParts, bool kLse>
-__device__ __forceinline__ void run_many(const Source& src, const Job& job, const Sink& to, int D, unsigned char* lds, Stats& st) {
+__device__ __forceinline__ void run_many(const Source& src, const Job& job, const Sink& to, int D, unsigned char* lds) {
   constexpr int kHalf = kDH * kHalfBytes, kSlot = 2 * kHalf;  // K (or V) of a block, of a tile
   constexpr bool kKeepL = kLse || kParts > 1;                 // the sum of unrounded weights
   typedef State<T, kDH, 1, kParts> W;
@@ -893,10 +894,55 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
     }
   }
   __syncthreads();
-  w.publish(lds + wave * kBlock * 64 * kDH * 4, st.m + wave * kBlock, st.l + wave * kBlock, st.lp + wave * kBlock, lane);
-  __syncthreads();
-  for (int e = tid; e < kManyRows * 8 * kDH; e += kThreads)
-    if (e % (8 * kDH) * 8 < D) put<T, kDH, 1>(lds, st, 0, e / (8 * kDH), e % (8 * kDH), job, to, D, kManyRows);
+  // A row's dims are its two lanes': 4 of every 8 each.
+  const int i = lane & 31, h = lane >> 5, row = wave * kBlock + i, r = job.row0 + row;
+  const auto add = [](float x, float y) { return x + y; };
+  const float l = over_pair(w.l[0], add), lp = kParts == 1 ? over_pair(w.lp[0], add) : l;
+  const float m = w.thr[0] == -INFINITY ? -INFINITY : w.m[0];
+  const bool real = r < job.rows;
+  if (to.part) {
+    if (!real) return;
+#pragma unroll
+    for (int j = 0; j < 2 * kDH; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (32 * j + 8 * g < D)
+          *reinterpret_cast<f32x4*>(to.part + (long long)row * D + 32 * j + 8 * g + 4 * h) =
+              f32x4{w.o[0][j][4 * g], w.o[0][j][4 * g + 1], w.o[0][j][4 * g + 2], w.o[0][j][4 * g + 3]};
+    if (h == 0) {
+      float* const stats = to.part + (long long)kManyRows * D + row;
+      stats[0] = m, stats[kManyRows] = l, stats[2 * kManyRows] = lp;
+    }
+    return;
+  }
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  const int step_of = divide(r, job.by_group), head_of = r - step_of * job.G;
+  const bool stored = real || (to.fill != 0 && r < to.fill_to);
+  const float nan = __uint_as_float(0x7FC00000u), inv = lp == 0.f ? 0.f : 1.f / lp;
+  T* const out = static_cast<T*>(to.o) + step_of * to.o_step + head_of * to.o_head;
+#pragma unroll
+  for (int j = 0; j < 2 * kDH; ++j)
+#pragma unroll
+    for (int g = 0; g < 4; g += 2) {
+      uint32_t x[2][2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        v4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          y[e] = (T)(real ? (lp == 0.f ? 0.f : w.o[0][j][4 * (g + k) + e] * inv) : to.fill == 2 ? nan : 0.f);
+        const auto two = __builtin_bit_cast(u32x2, y);
+        x[k][0] = two[0], x[k][1] = two[1];
+      }
+      // The first lane takes dims 8 g .. of both, the second the next 8.
+      const auto a = __builtin_amdgcn_permlane32_swap(x[0][0], x[1][0], false, false);
+      const auto b = __builtin_amdgcn_permlane32_swap(x[0][1], x[1][1], false, false);
+      const int d = 32 * j + 8 * (g + h);
+      if (stored && d < D) *reinterpret_cast<u32x4*>(out + d) = u32x4{a[0], b[0], a[1], b[1]};
+    }
+  if (stored && h == 0 && to.lse)
+    to.lse[step_of * to.l_step + head_of * to.l_head] =
+        !real ? (to.fill == 2 ? nan : -INFINITY) : l == 0.f ? -INFINITY : fmaf(m, job.scale, log2f(l) * kLn2);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1049,7 +1095,7 @@ constexpr int simd_waves(Kind kind, int kDH) {
 template <class T, int kDH, bool kAligned, Kind kKind, int kParts, bool kLse>
 __device__ __forceinline__ void run(const Source& src, const Job& job, const Sink& to, int D, unsigned char* lds, Stats& st) {
   if constexpr (kKind == Kind::kMany)
-    run_many<T, kDH, kAligned, kParts, kLse>(src, job, to, D, lds, st);
+    run_many<T, kDH, kAligned, kParts, kLse>(src, job, to, D, lds);
   else
     run_few<T, kDH, kAligned, kKind == Kind::kFew1 ? 1 : 2, few_stages(kKind)>(src, job, to, D, lds, st);
 }
