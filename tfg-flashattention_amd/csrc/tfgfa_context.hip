@@ -16,8 +16,8 @@
 // Other pages: each lane has an address, of a row of zeros where there is no key.  A page id outside the pool gives a
 // row of NaN for K, so that NaN reaches the rows that see the key, and zeros for V.
 //
-// Few rows (up to 64 a job): each wave streams blocks of its own (wave w of a workgroup takes blocks w, w + 4, ..) through
-// a ring of its own, with no barrier, all rows in its registers; the four are joined through LDS.  Many rows: four waves
+// Few rows (up to 64 a job, 32 a workgroup): each wave streams blocks of its own (wave w of a workgroup takes blocks w, w + 4,
+// ..) through LDS of its own, with no barrier; the four are joined through LDS.  Many rows: four waves
 // of 32 rows share tiles of 64 keys.  A job's keys may be divided over workgroups, whose parts a second kernel joins.
 //
 // Hidden keys have weight 0, but 0 times an infinite or NaN value is NaN: a wave whose sums hold NaN at the end takes its
@@ -252,21 +252,21 @@ struct Loader {
   }
 };
 
-// A wave's rows: kRT tiles of 32, row i of tile t in lanes i and i + 32.
+// A wave's 32 rows, row i in lanes i and i + 32.
 // kParts: of the element type that a weight is split into for the product with V, each what rounding left of the ones
 // before (2: all but 2^-16 of a weight in bf16, 2^-22 in fp16).  With 1 the output is divided by the sum of the rounded weights, so that the
 // rounding of a weight that stands alone cancels; the log-sum-exp takes the unrounded ones.
-template <class T, int kDH, int kRT, int kParts>
+template <class T, int kDH, int kParts>
 struct State {
   typedef typename Elem<T>::v8 v8;
   typedef typename Elem<T>::v2 v2;
   static constexpr int kC = 4 * kDH;   // pieces of 16 dims
   static constexpr int kOT = 2 * kDH;  // output tiles of 32
-  v8 q[kRT][kC];
-  f32x16 o[kRT][kOT];
-  float m[kRT], thr[kRT];   // offset, and how far a score may pass it (-inf: the row has no weight yet)
-  float l[kRT], lp[kRT];    // this lane's sums of weights; kParts 1: of the rounded ones
-  int seen[kRT];            // keys that the row sees
+  v8 q[kC];
+  f32x16 o[kOT];
+  float m, thr;             // offset, and how far a score may pass it (-inf: the row has no weight yet)
+  float l, lp;              // this lane's sums of weights; kParts 1: of the rounded ones
+  int seen;                 // keys that the row sees
   int koff[4], voff[2][2];  // LDS offsets of the operands, in a block's first 64 dims
 
   __device__ __forceinline__ void init(int lane) {
@@ -283,27 +283,21 @@ struct State {
     clear();
   }
   __device__ __forceinline__ void clear() {
+    m = l = lp = 0.f, thr = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < kRT; ++t) {
-      m[t] = l[t] = lp[t] = 0.f, thr[t] = -INFINITY;
+    for (int j = 0; j < kOT; ++j)
 #pragma unroll
-      for (int j = 0; j < kOT; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[t][j][r] = 0.f;
-    }
+      for (int r = 0; r < 16; ++r) o[j][r] = 0.f;
   }
 
   // S^T of the block in LDS.
-  __device__ __forceinline__ void scores(f32x16 (&s)[kRT], const unsigned char* block) const {
+  __device__ __forceinline__ void scores(f32x16& s, const unsigned char* block) const {
 #pragma unroll
-    for (int t = 0; t < kRT; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+    for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
       const v8 a = key_operand(block, c);
-#pragma unroll
-      for (int t = 0; t < kRT; ++t) s[t] = Elem<T>::mfma(a, q[t][c], s[t]);
+      s = Elem<T>::mfma(a, q[c], s);
     }
   }
 
@@ -314,28 +308,28 @@ struct State {
     return fmaxf(x, s[15]);
   }
 
-  // Few rows, and the exact pass: weights 2^(c (s - m)) of tile t in place.  (The difference first, which is exact for near
+  // Few rows, and the exact pass: weights 2^(c (s - m)) in place.  (The difference first, which is exact for near
   // scores of any size.)  c: scale_log2.
-  __device__ __forceinline__ void weigh(f32x16& s, int t, float c, float inv_c) {
+  __device__ __forceinline__ void weigh(f32x16& s, float c, float inv_c) {
     const float mx = largest(s);
-    if (__builtin_amdgcn_ballot_w64(mx - m[t] >= thr[t])) {
+    if (__builtin_amdgcn_ballot_w64(mx - m >= thr)) {
       const float top = over_pair(mx, [](float x, float y) { return fmaxf(x, y); });
-      const bool fresh = thr[t] == -INFINITY, none = top == -INFINITY;  // no weight so far; none here
-      const float to = none ? m[t] : fmaxf(fresh ? -INFINITY : m[t], top - fminf(Elem<T>::kHead * inv_c, 1e30f));
-      const float f = fresh ? 0.f : __builtin_amdgcn_exp2f((m[t] - to) * c);
-      m[t] = to;
-      if (!none) thr[t] = fminf((Elem<T>::kHead + Elem<T>::kMargin) * inv_c, 1e30f);
-      l[t] *= f, lp[t] *= f;
+      const bool fresh = thr == -INFINITY, none = top == -INFINITY;  // no weight so far; none here
+      const float to = none ? m : fmaxf(fresh ? -INFINITY : m, top - fminf(Elem<T>::kHead * inv_c, 1e30f));
+      const float f = fresh ? 0.f : __builtin_amdgcn_exp2f((m - to) * c);
+      m = to;
+      if (!none) thr = fminf((Elem<T>::kHead + Elem<T>::kMargin) * inv_c, 1e30f);
+      l *= f, lp *= f;
 #pragma unroll
-      for (int j = 0; j < kOT; ++j) o[t][j] *= f;
+      for (int j = 0; j < kOT; ++j) o[j] *= f;
     }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f((s[r] - m[t]) * c);
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f((s[r] - m) * c);
   }
 
   // Scores of keys that a row does not see; at: the block's first key.
-  __device__ __forceinline__ void mask(f32x16& s, int t, int at, int lane) const {
-    const int left = seen[t] - at - 4 * (lane >> 5);
+  __device__ __forceinline__ void mask(f32x16& s, int at, int lane) const {
+    const int left = seen - at - 4 * (lane >> 5);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = 8 * (r / 4) + r % 4 < left ? s[r] : -INFINITY;
   }
@@ -384,43 +378,37 @@ struct State {
     }
     return x + y;
   }
-  __device__ __forceinline__ void split(const f32x16& w, int t, v8 (&part)[kParts][2]) {
+  __device__ __forceinline__ void split(const f32x16& w, v8 (&part)[kParts][2]) {
     float p[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) p[r] = w[r];
-    l[t] += sum16(p);
+    l += sum16(p);
     parts_of(p, part);
   }
 
   // O^T += V^T P^T.
-  __device__ __forceinline__ void output(const unsigned char* v, const v8 (&part)[kRT][kParts][2]) {
+  __device__ __forceinline__ void output(const unsigned char* v, const v8 (&part)[kParts][2]) {
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int j = 0; j < kOT; ++j) {
         const v8 a = values(v, j, c);
 #pragma unroll
-        for (int t = 0; t < kRT; ++t)
-#pragma unroll
-          for (int n = 0; n < kParts; ++n) o[t][j] = Elem<T>::mfma(a, part[t][n][c], o[t][j]);
+        for (int n = 0; n < kParts; ++n) o[j] = Elem<T>::mfma(a, part[n][c], o[j]);
       }
   }
 
   // The same with float32 products that leave weights of 0 out.
-  __device__ __forceinline__ void output_exact(const unsigned char* v, const f32x16 (&p)[kRT], int lane) {
+  __device__ __forceinline__ void output_exact(const unsigned char* v, const f32x16& p, int lane) {
     const int h = lane >> 5;
 #pragma unroll 1
     for (int r = 0; r < 16; ++r) {
-      float both[kRT][2];
+      float x = p[0];
 #pragma unroll
-      for (int t = 0; t < kRT; ++t) {
-        float x = p[t][0];
-#pragma unroll
-        for (int u = 1; u < 16; ++u) x = r == u ? p[t][u] : x;
-        const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        both[t][0] = __uint_as_float(y[0]), both[t][1] = __uint_as_float(y[1]);
-        l[t] += x, lp[t] += x;
-      }
+      for (int u = 1; u < 16; ++u) x = r == u ? p[u] : x;
+      const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+      const float both[2] = {__uint_as_float(y[0]), __uint_as_float(y[1])};
+      l += x, lp += x;
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
         const int key = 8 * (r / 4) + 4 * hh + r % 4;
@@ -432,12 +420,10 @@ struct State {
             typedef T v4 __attribute__((ext_vector_type(4)));
             const v4 x = *reinterpret_cast<const v4*>(v + (j >> 1) * kHalfBytes + key * 128 + (((d >> 3) ^ swz_v(key)) << 4) + 8 * h);
 #pragma unroll
-            for (int t = 0; t < kRT; ++t)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float y = both[t][hh];
-                o[t][j][4 * g + e] = y == 0.f ? o[t][j][4 * g + e] : fmaf(y, (float)x[e], o[t][j][4 * g + e]);
-              }
+            for (int e = 0; e < 4; ++e) {
+              const float y = both[hh];
+              o[j][4 * g + e] = y == 0.f ? o[j][4 * g + e] : fmaf(y, (float)x[e], o[j][4 * g + e]);
+            }
           }
       }
     }
@@ -447,24 +433,20 @@ struct State {
   template <bool kExact>
   __device__ __forceinline__ void step(const unsigned char* k, const unsigned char* v, int at, int least, float c, float inv_c,
                                        int lane) {
-    f32x16 s[kRT];
+    f32x16 s;
     scores(s, k);
-    if (at + kBlock > least)
-#pragma unroll
-      for (int t = 0; t < kRT; ++t) mask(s[t], t, at, lane);
-#pragma unroll
-    for (int t = 0; t < kRT; ++t) weigh(s[t], t, c, inv_c);
+    if (at + kBlock > least) mask(s, at, lane);
+    weigh(s, c, inv_c);
     if constexpr (kExact) {
       output_exact(v, s, lane);
     } else {
-      v8 part[kRT][kParts][2];
-#pragma unroll
-      for (int t = 0; t < kRT; ++t) split(s[t], t, part[t]);
+      v8 part[kParts][2];
+      split(s, part);
       output(v, part);
     }
   }
 
-  // Many rows (kRT = 1): blocks in a pipeline.  s: the scores of block u; part: the weights of block u - 1; v, k: V of block
+  // Many rows: blocks in a pipeline.  s: the scores of block u; part: the weights of block u - 1; v, k: V of block
   // u - 1 and K of block u + 1 in LDS.  The products of V run beside the exponentials, those of K beside the weights' sums
   // and rounding, one matrix instruction and a share of them at a time (a wave's VALU work overlaps its own matrix
   // instructions).  Offsets are in the log2 domain (m = thr): 2^(c s - m) is one v_fma and one v_exp.
@@ -480,13 +462,13 @@ struct State {
     if constexpr (kPV) vo[0] = values(v, 0, 0), vo[1] = values(v, 1, 0);
     __builtin_amdgcn_sched_barrier(0);
     float p[16];
-    const float neg = -m[0];
+    const float neg = -m;
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
       const int cc = i / kOT, j = i % kOT;
       if constexpr (kPV)
 #pragma unroll
-        for (int n = 0; n < kParts; ++n) o[0][j] = Elem<T>::mfma(vo[i & 1], part[n][cc], o[0][j]);
+        for (int n = 0; n < kParts; ++n) o[j] = Elem<T>::mfma(vo[i & 1], part[n][cc], o[j]);
       if (i + 2 < kPairs) {
         if constexpr (kPV) vo[i & 1] = values(v, (i + 2) % kOT, (i + 2) / kOT);
       } else {
@@ -504,35 +486,35 @@ struct State {
     for (int r = 0; r < 16; ++r) next[r] = 0.f;
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
-      next = Elem<T>::mfma(ko[i & 1], q[0][i], next);
+      next = Elem<T>::mfma(ko[i & 1], q[i], next);
       if (i + 2 < kC) ko[i & 1] = key_operand(k, i + 2);
       if (i == 0) {
         parts_of(p, part);
 #pragma unroll
         for (int n = 0; n < kParts; ++n) asm volatile("" : "+v"(part[n][0]), "+v"(part[n][1]));
       } else if (i == 1) {
-        float sum = add_rounded(part, lp[0]);
+        float sum = add_rounded(part, lp);
         // (As integers: past the bound, infinite or NaN.)
         if (__builtin_amdgcn_ballot_w64(__float_as_uint(sum) > __float_as_uint(kBound))) {
           const float top = over_pair(largest(s), [](float x, float y) { return fmaxf(x, y); });
           const float at = top * c;
           *far = *far || (fabsf(top) < INFINITY && !(fabsf(at) < INFINITY));
-          const float to = fmaxf(fmaxf(m[0], kLowest), at - head);
-          const float f = __builtin_amdgcn_exp2f(m[0] - to);
-          m[0] = to, lp[0] *= f, l[0] *= f;
+          const float to = fmaxf(fmaxf(m, kLowest), at - head);
+          const float f = __builtin_amdgcn_exp2f(m - to);
+          m = to, lp *= f, l *= f;
 #pragma unroll
-          for (int j = 0; j < kOT; ++j) o[0][j] *= f;
+          for (int j = 0; j < kOT; ++j) o[j] *= f;
 #pragma unroll
           for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -to));
           parts_of(p, part);
-          sum = add_rounded(part, lp[0]);
+          sum = add_rounded(part, lp);
         }
-        lp[0] = sum;
-        asm volatile("" : "+v"(lp[0]));
+        lp = sum;
+        asm volatile("" : "+v"(lp));
       }
       if (i == 2 && kLse) {
-        l[0] += sum16(p);
-        asm volatile("" : "+v"(l[0]));
+        l += sum16(p);
+        asm volatile("" : "+v"(l));
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -546,51 +528,45 @@ struct State {
   __device__ __forceinline__ bool any_nan() const {
     float x = 0.f;
 #pragma unroll
-    for (int t = 0; t < kRT; ++t)
+    for (int j = 0; j < kOT; ++j)
 #pragma unroll
-      for (int j = 0; j < kOT; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x = fmaf(o[t][j][r], 0.f, x);
+      for (int r = 0; r < 16; ++r) x = fmaf(o[j][r], 0.f, x);
     return __builtin_amdgcn_ballot_w64(x != x) != 0;
   }
 
   // Many rows: the offset from the log2 domain to scores without the scale.  What rounding it there leaves, m c - to, goes
   // into the sums, so that it is exact.
   __device__ __forceinline__ void rescale(float c) {
-    if (!(fabsf(m[0]) < INFINITY)) return;
-    if (m[0] <= kLowest) {  // scores of -inf alone
-      m[0] = -INFINITY;
+    if (!(fabsf(m) < INFINITY)) return;
+    if (m <= kLowest) {  // scores of -inf alone
+      m = -INFINITY;
       return;
     }
-    const float to = m[0] / c, f = __builtin_amdgcn_exp2f(-fmaf(to, c, -m[0]));
-    m[0] = to, l[0] *= f, lp[0] *= f;
+    const float to = m / c, f = __builtin_amdgcn_exp2f(-fmaf(to, c, -m));
+    m = to, l *= f, lp *= f;
 #pragma unroll
-    for (int j = 0; j < kOT; ++j) o[0][j] *= f;
+    for (int j = 0; j < kOT; ++j) o[j] *= f;
   }
 
   // Into LDS: rows of 64 kDH floats, 16-byte piece c of row r at place c ^ r % pieces; statistics beside.
   __device__ __forceinline__ void publish(unsigned char* rows, float* sm, float* sl, float* slp, int lane) const {
     constexpr int kPieces = 16 * kDH;
-    const int i = lane & 31, h = lane >> 5;
+    const int r = lane & 31, h = lane >> 5;
+    const float lt = over_pair(l, [](float x, float y) { return x + y; });
+    const float lpt = kParts == 1 ? over_pair(lp, [](float x, float y) { return x + y; }) : lt;
 #pragma unroll
-    for (int t = 0; t < kRT; ++t) {
-      const int r = t * kBlock + i;
-      const float lt = over_pair(l[t], [](float x, float y) { return x + y; });
-      const float lpt = kParts == 1 ? over_pair(lp[t], [](float x, float y) { return x + y; }) : lt;
+    for (int j = 0; j < kOT; ++j)
 #pragma unroll
-      for (int j = 0; j < kOT; ++j)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int c = 8 * j + 2 * g + h;
-          *reinterpret_cast<f32x4*>(rows + (r * kPieces + (c ^ (r % kPieces))) * 16) =
-              f32x4{o[t][j][4 * g], o[t][j][4 * g + 1], o[t][j][4 * g + 2], o[t][j][4 * g + 3]};
-        }
-      if (h == 0) sm[r] = thr[t] == -INFINITY ? -INFINITY : m[t], sl[r] = lt, slp[r] = lpt;
-    }
+      for (int g = 0; g < 4; ++g) {
+        const int c = 8 * j + 2 * g + h;
+        *reinterpret_cast<f32x4*>(rows + (r * kPieces + (c ^ (r % kPieces))) * 16) =
+            f32x4{o[j][4 * g], o[j][4 * g + 1], o[j][4 * g + 2], o[j][4 * g + 3]};
+      }
+    if (h == 0) sm[r] = thr == -INFINITY ? -INFINITY : m, sl[r] = lt, slp[r] = lpt;
   }
 };
 
-// A piece of work: rows [row0, row0 + 32 kRT or 128) of a job, blocks [first, last) of its keys.
+// A piece of work: rows [row0, row0 + 32 or 128) of a job, blocks [first, last) of its keys.
 struct Job {
   const void* q;                  // the job's first row; row r is r / G steps and r % G heads on
   long long q_step, q_head;
@@ -612,41 +588,35 @@ struct Sink {
   int fill_to, fill;              // rows from Job::rows up to here get zeros (fill 1) or NaN (fill 2)
 };
 
-constexpr int few_lds(int kDH, int kRT, int stages) {
-  const int ring = kWaves * stages * 2 * kDH * kHalfBytes, rows = kWaves * kRT * kBlock * 64 * kDH * 4;
-  return ring > rows ? ring : rows;
+constexpr int few_lds(int kDH) {  // a block of each wave, or its rows
+  const int blocks = kWaves * 2 * kDH * kHalfBytes, rows = kWaves * kBlock * 64 * kDH * 4;
+  return blocks > rows ? blocks : rows;
 }
 constexpr int many_lds(int kDH) { return 4 * kDH * 2 * kHalfBytes; }  // four tiles of 64 keys
-constexpr int kMaxRows = kWaves * 2 * kBlock;  // of statistics: four waves of 64 rows
 
 struct Stats {
-  float m[kMaxRows], l[kMaxRows], lp[kMaxRows];
+  float m[kWaves * kBlock], l[kWaves * kBlock], lp[kWaves * kBlock];
 };
 
-template <class T, int kDH, int kRT, int kParts>
-__device__ __forceinline__ void load_rows(State<T, kDH, kRT, kParts>& w, const Job& job, int first, int D, int lane) {
+template <class T, int kDH, int kParts>
+__device__ __forceinline__ void load_rows(State<T, kDH, kParts>& w, const Job& job, int first, int D, int lane) {
   typedef typename Elem<T>::v8 v8;
-  const int i = lane & 31, h = lane >> 5;
+  const int r = first + (lane & 31), h = lane >> 5, step = divide(r, job.by_group);
+  const T* const at = static_cast<const T*>(job.q) + step * job.q_step + (r - step * job.G) * job.q_head;
+  w.seen = r < job.rows ? job.seen + (job.causal ? step + 1 : 0) : 0;
 #pragma unroll
-  for (int t = 0; t < kRT; ++t) {
-    const int r = first + t * kBlock + i, step = divide(r, job.by_group);
-    const T* const at = static_cast<const T*>(job.q) + step * job.q_step + (r - step * job.G) * job.q_head;
-    w.seen[t] = r < job.rows ? job.seen + (job.causal ? step + 1 : 0) : 0;
-#pragma unroll
-    for (int c = 0; c < 4 * kDH; ++c) {
-      const int d = 16 * c + 8 * h;
-      w.q[t][c] = __builtin_bit_cast(v8, u32x4{0, 0, 0, 0});
-      if (r < job.rows && d < D) w.q[t][c] = *reinterpret_cast<const v8*>(at + d);
-    }
-    // Here, before the loop: the waits that the compiler places for these loads would empty the pipeline of direct ones.
-#pragma unroll
-    for (int c = 0; c < 4 * kDH; ++c) asm volatile("" ::"v"(w.q[t][c]));
+  for (int c = 0; c < 4 * kDH; ++c) {
+    const int d = 16 * c + 8 * h;
+    w.q[c] = __builtin_bit_cast(v8, u32x4{0, 0, 0, 0});
+    if (r < job.rows && d < D) w.q[c] = *reinterpret_cast<const v8*>(at + d);
   }
+  // Here, before the loop: the waits that the compiler places for these loads would empty the pipeline of direct ones.
+#pragma unroll
+  for (int c = 0; c < 4 * kDH; ++c) asm volatile("" ::"v"(w.q[c]));
 }
 
-// Few rows: row `row` of the workgroup's kRows rows, 8 dims from 8 c8 on, joined over the waves' states (kRows apart), to its
-// place.
-template <class T, int kDH, int kRows>
+// Few rows: row `row` of the workgroup's, 8 dims from 8 c8 on, joined over the waves' states, to its place.
+template <class T, int kDH>
 __device__ __forceinline__ void put(const unsigned char* rows, const Stats& st, int row, int c8, const Job& job,
                                     const Sink& to, int D) {
   constexpr int kPieces = 16 * kDH;
@@ -655,12 +625,12 @@ __device__ __forceinline__ void put(const unsigned char* rows, const Stats& st, 
   if (!real && !(to.part == nullptr && to.fill != 0 && r < to.fill_to)) return;
   float M = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, st.m[w * kRows + row]);
+  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, st.m[w * kBlock + row]);
   float l = 0.f, lp = 0.f;
   f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    const int at = w * kRows + row;
+    const int at = w * kBlock + row;
     const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((st.m[at] - M) * job.scale_log2);
     l = fmaf(f, st.l[at], l), lp = fmaf(f, st.lp[at], lp);
     const f32x4 x = *reinterpret_cast<const f32x4*>(rows + (at * kPieces + ((2 * c8) ^ (at % kPieces))) * 16);
@@ -676,8 +646,8 @@ __device__ __forceinline__ void put(const unsigned char* rows, const Stats& st, 
     *reinterpret_cast<f32x4*>(at) = a;
     *reinterpret_cast<f32x4*>(at + 4) = b;
     if (c8 == 0) {
-      float* const stats = to.part + (long long)kRows * D + row;
-      stats[0] = M, stats[kRows] = l, stats[2 * kRows] = lp;
+      float* const stats = to.part + (long long)kBlock * D + row;
+      stats[0] = M, stats[kBlock] = l, stats[2 * kBlock] = lp;
     }
     return;
   }
@@ -697,46 +667,32 @@ __device__ __forceinline__ void put(const unsigned char* rows, const Stats& st, 
 }
 
 // Few rows.
-template <class T, int kDH, bool kAligned, int kRT, int kStages>
+template <class T, int kDH, bool kAligned>
 __device__ __forceinline__ void run_few(const Source& src, const Job& job, const Sink& to, int D, unsigned char* lds, Stats& st) {
-  constexpr int kLoads = 8 * kDH;                       // transfers of a block
   constexpr int kBytes = 2 * kDH * kHalfBytes;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  unsigned char* const ring = lds + wave * kStages * kBytes;
-  const uint32_t ring_at = tfgfa::lds_addr(ring);
+  unsigned char* const block = lds + wave * kBytes;
+  const uint32_t block_at = tfgfa::lds_addr(block);
   const int count = max(0, (job.last - job.first - wave + kWaves - 1) / kWaves);
   auto key = [&](int n) { return (job.first + wave + n * kWaves) * kBlock; };
-  State<T, kDH, kRT, 2> w;
+  State<T, kDH, 2> w;
   const float inv = 1.f / job.scale_log2;
   w.init(lane);
   Loader<kDH, kAligned, 2> in;
   typename Loader<kDH, kAligned, 2>::Place place = {};
   in.init(src, D, 0, lane);
-  auto issue = [&](int n, uint32_t to) {
-    in.template issue<false>(src, key(n), place, to);
-    in.template issue<true>(src, key(n), place, to + kBytes / 2);
-    if (n + 1 < count) place = in.look_up(src, key(n + 1));
-  };
   const int least = job.causal ? job.seen + divide(job.row0, job.by_group) + 1 : job.seen;
   auto pass = [&](auto exact) {
     if (count > 0) place = in.look_up(src, key(0));
-#pragma unroll
-    for (int n = 0; n < kStages - 1; ++n)
-      if (n < count) issue(n, ring_at + n * kBytes);
     if (!decltype(exact)::value) load_rows(w, job, job.row0, D, lane);
-    int stage = 0;
 #pragma unroll 1
     for (int n = 0; n < count; ++n) {
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of the stage that is filled next
-      if (n + kStages - 1 < count) {
-        issue(n + kStages - 1, ring_at + (stage == 0 ? kStages - 1 : stage - 1) * kBytes);
-        tfgfa::wait_vmcnt<(kStages - 1) * kLoads>();
-      } else {
-        tfgfa::wait_vmcnt<0>();
-      }
-      const unsigned char* const block = ring + stage * kBytes;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of the block before
+      in.template issue<false>(src, key(n), place, block_at);
+      in.template issue<true>(src, key(n), place, block_at + kBytes / 2);
+      if (n + 1 < count) place = in.look_up(src, key(n + 1));
+      tfgfa::wait_vmcnt<0>();
       w.template step<decltype(exact)::value>(block, block + kBytes / 2, key(n), least, job.scale_log2, inv, lane);
-      stage = stage + 1 == kStages ? 0 : stage + 1;
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   };
@@ -745,12 +701,11 @@ __device__ __forceinline__ void run_few(const Source& src, const Job& job, const
     w.clear();
     pass(std::true_type());
   }
-  constexpr int kRows = kRT * kBlock;
-  __syncthreads();  // (the rows' places are the rings')
-  w.publish(lds + wave * kRows * 64 * kDH * 4, st.m + wave * kRows, st.l + wave * kRows, st.lp + wave * kRows, lane);
+  __syncthreads();  // (the rows' places are the blocks')
+  w.publish(lds + wave * kBlock * 64 * kDH * 4, st.m + wave * kBlock, st.l + wave * kBlock, st.lp + wave * kBlock, lane);
   __syncthreads();
-  for (int e = tid; e < kRows * 8 * kDH; e += kThreads)
-    if (e % (8 * kDH) * 8 < D) put<T, kDH, kRows>(lds, st, e / (8 * kDH), e % (8 * kDH), job, to, D);
+  for (int e = tid; e < kBlock * 8 * kDH; e += kThreads)
+    if (e % (8 * kDH) * 8 < D) put<T, kDH>(lds, st, e / (8 * kDH), e % (8 * kDH), job, to, D);
 }
 
 // Many rows.  Two K tiles and two V tiles of 64 keys in LDS.  Step j of the workgroup: block 2j; wait for K of tile j + 1 and
@@ -759,7 +714,7 @@ template <class T, int kDH, bool kAligned, int kParts, bool kLse>
 __device__ __forceinline__ void run_many(const Source& src, const Job& job, const Sink& to, int D, unsigned char* lds) {
   constexpr int kHalf = kDH * kHalfBytes, kSlot = 2 * kHalf;  // K (or V) of a block, of a tile
   constexpr bool kKeepL = kLse || kParts > 1;                 // the sum of unrounded weights
-  typedef State<T, kDH, 1, kParts> W;
+  typedef State<T, kDH, kParts> W;
   __shared__ int sh_again;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const uint32_t ring_at = tfgfa::lds_addr(lds);
@@ -801,23 +756,18 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
   load_rows(w, job, r0, D, lane);
   tfgfa::wait_vmcnt<0>();
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  w.m[0] = -INFINITY;
+  w.m = -INFINITY;
   const float head = fminf(Elem<T>::kHead, 1e30f * c);
   bool far = false;
-  f32x16 s[1];
+  f32x16 s;
   typename W::v8 part[kParts][2];
   if (act > 0) w.scores(s, lds);
   // Half a step: block u, V of the one before it and K of the one after it in LDS.
   auto block = [&](int u, const unsigned char* v, const unsigned char* k, auto first) {
-    if (u >= full) w.mask(s[0], 0, (job.first + u) * kBlock, lane);
-    w.template fused<!decltype(first)::value, kKeepL>(v, k, s[0], part, c, head, &far);
+    if (u >= full) w.mask(s, (job.first + u) * kBlock, lane);
+    w.template fused<!decltype(first)::value, kKeepL>(v, k, s, part, c, head, &far);
   };
-  auto last = [&](const unsigned char* v) {
-    typename W::v8 all[1][kParts][2];
-#pragma unroll
-    for (int n = 0; n < kParts; ++n) all[0][n][0] = part[n][0], all[0][n][1] = part[n][1];
-    w.output(v, all);
-  };
+  auto last = [&](const unsigned char* v) { w.output(v, part); };
   auto turn = [&](int j) {  // between the halves of step j
     tfgfa::wait_vmcnt<0>();
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -869,8 +819,8 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
     last(v_of((tiles - 1) & 1) + kHalf);
   }
   w.rescale(c);
-  if (kParts > 1) w.lp[0] = w.l[0];
-  w.thr[0] = 0.f;
+  if (kParts > 1) w.lp = w.l;
+  w.thr = 0.f;
   if ((__builtin_amdgcn_ballot_w64(far) != 0 || w.any_nan()) && lane == 0) sh_again = 1;
   __syncthreads();
   if (uniform(sh_again)) {
@@ -897,8 +847,8 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
   // A row's dims are its two lanes': 4 of every 8 each.
   const int i = lane & 31, h = lane >> 5, row = wave * kBlock + i, r = job.row0 + row;
   const auto add = [](float x, float y) { return x + y; };
-  const float l = over_pair(w.l[0], add), lp = kParts == 1 ? over_pair(w.lp[0], add) : l;
-  const float m = w.thr[0] == -INFINITY ? -INFINITY : w.m[0];
+  const float l = over_pair(w.l, add), lp = kParts == 1 ? over_pair(w.lp, add) : l;
+  const float m = w.thr == -INFINITY ? -INFINITY : w.m;
   const bool real = r < job.rows;
   if (to.part) {
     if (!real) return;
@@ -908,7 +858,7 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
       for (int g = 0; g < 4; ++g)
         if (32 * j + 8 * g < D)
           *reinterpret_cast<f32x4*>(to.part + (long long)row * D + 32 * j + 8 * g + 4 * h) =
-              f32x4{w.o[0][j][4 * g], w.o[0][j][4 * g + 1], w.o[0][j][4 * g + 2], w.o[0][j][4 * g + 3]};
+              f32x4{w.o[j][4 * g], w.o[j][4 * g + 1], w.o[j][4 * g + 2], w.o[j][4 * g + 3]};
     if (h == 0) {
       float* const stats = to.part + (long long)kManyRows * D + row;
       stats[0] = m, stats[kManyRows] = l, stats[2 * kManyRows] = lp;
@@ -930,7 +880,7 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
         v4 y;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          y[e] = (T)(real ? (lp == 0.f ? 0.f : w.o[0][j][4 * (g + k) + e] * inv) : to.fill == 2 ? nan : 0.f);
+          y[e] = (T)(real ? (lp == 0.f ? 0.f : w.o[j][4 * (g + k) + e] * inv) : to.fill == 2 ? nan : 0.f);
         const auto two = __builtin_bit_cast(u32x2, y);
         x[k][0] = two[0], x[k][1] = two[1];
       }
@@ -1079,17 +1029,14 @@ struct AttendArgs {
 };
 
 // How many rows a workgroup takes, and how.
-enum class Kind { kFew1, kFew2, kMany };
+enum class Kind { kFew, kMany };
 __host__ __device__ constexpr int rows_of(Kind kind) {
-  return kind == Kind::kFew1 ? kBlock : kind == Kind::kFew2 ? 2 * kBlock : kManyRows;
+  return kind == Kind::kFew ? kBlock : kManyRows;
 }
-constexpr int few_stages(Kind kind) { return kind == Kind::kFew1 ? 1 : 2; }
-constexpr int lds_of(Kind kind, int kDH) {
-  return kind == Kind::kMany ? many_lds(kDH) : few_lds(kDH, kind == Kind::kFew1 ? 1 : 2, few_stages(kind));
-}
+constexpr int lds_of(Kind kind, int kDH) { return kind == Kind::kMany ? many_lds(kDH) : few_lds(kDH); }
 
 constexpr int simd_waves(Kind kind, int kDH) {
-  return kind == Kind::kMany ? (kDH == 1 ? 3 : 2) : kind == Kind::kFew1 ? (kDH == 1 ? 4 : 2) : (kDH == 1 ? 2 : 1);
+  return kDH == 2 ? 2 : kind == Kind::kMany ? 3 : 4;
 }
 
 template <class T, int kDH, bool kAligned, Kind kKind, int kParts, bool kLse>
@@ -1097,7 +1044,24 @@ __device__ __forceinline__ void run(const Source& src, const Job& job, const Sin
   if constexpr (kKind == Kind::kMany)
     run_many<T, kDH, kAligned, kParts, kLse>(src, job, to, D, lds);
   else
-    run_few<T, kDH, kAligned, kKind == Kind::kFew1 ? 1 : 2, few_stages(kKind)>(src, job, to, D, lds, st);
+    run_few<T, kDH, kAligned>(src, job, to, D, lds, st);
+}
+
+// Which head, part and tile of rows a workgroup takes; in either order the workgroups of a head are on one XCD where 8 divides
+// the heads.
+struct Work {
+  int head, part, tile;
+};
+// Tile after tile.
+__device__ __forceinline__ Work by_tiles(int idx, int heads, int parts) {
+  const int rest = idx / heads, tile = rest / parts;
+  return {idx - rest * heads, rest - tile * parts, tile};
+}
+// The tiles of a part together, 8 parts at a time, so that its keys come from HBM once.
+__device__ __forceinline__ Work by_heads(int idx, int heads, int parts, int tiles) {
+  const int first = idx / (8 * tiles), in = idx - first * 8 * tiles, width = min(8, heads * parts - 8 * first);
+  const int tile = in / width, job = 8 * first + in - tile * width, part = job / heads;
+  return {job - part * heads, part, tile};
 }
 
 // Part s of S of `blocks` blocks: whole rounds of the workgroup.
@@ -1116,8 +1080,9 @@ __global__ __launch_bounds__(kThreads, simd_waves(kKind, kDH)) void attend_kerne
   constexpr int kRows = rows_of(kKind);
   // The longest first (the last tiles of a causal sequence); a key-value head's workgroups on one XCD where 8 divides
   // their number.
-  const int idx = blockIdx.x, rest = idx / a.heads, head = idx - rest * a.heads;
-  const int from_end = rest / a.parts, s = rest - from_end * a.parts, tile = a.tiles - 1 - from_end;
+  const bool together = kKind != Kind::kMany && a.tiles > 1;
+  const Work at = together ? by_heads(blockIdx.x, a.heads, a.parts, a.tiles) : by_tiles(blockIdx.x, a.heads, a.parts);
+  const int head = at.head, s = at.part, tile = a.tiles - 1 - at.tile;
   const int b = head / a.Hkv, kv = head - b * a.Hkv;
   const int len = ((uniform_ints)a.lens)[b], n = a.lengths ? ((uniform_ints)a.lengths)[b] : a.N;
   const bool fits = len >= 0 && n >= 0 && n <= a.N && (long long)len + (a.causal ? n : 0) <= a.n_max;
@@ -1191,7 +1156,7 @@ struct SharedArgs {
 
 template <class T, int kDH, bool kAligned, Kind kKind>
 __global__ __launch_bounds__(kThreads, simd_waves(kKind, kDH)) void shared_kernel(const SharedArgs a) {
-  constexpr int kPrefixLds = lds_of(kKind, kDH), kOwnLds = lds_of(Kind::kFew1, kDH);
+  constexpr int kPrefixLds = lds_of(kKind, kDH), kOwnLds = lds_of(Kind::kFew, kDH);
   __shared__ __attribute__((aligned(1024))) unsigned char lds[kPrefixLds > kOwnLds ? kPrefixLds : kOwnLds];
   __shared__ Stats st;
   Job job;
@@ -1203,7 +1168,10 @@ __global__ __launch_bounds__(kThreads, simd_waves(kKind, kDH)) void shared_kerne
   const bool prefix = (int)blockIdx.x < a.prefix_jobs;
   const int idx = prefix ? blockIdx.x : blockIdx.x - a.prefix_jobs;
   const int heads = prefix ? a.prefix_heads : a.own_heads, parts = prefix ? a.prefix_parts : a.own_parts;
-  const int rest = idx / heads, head = idx - rest * heads, tile = rest / parts, s = rest - tile * parts;
+  const int tiles = prefix ? a.prefix_tiles : a.own_tiles;
+  const bool together = tiles > 1 && !(prefix && kKind == Kind::kMany);
+  const Work at = together ? by_heads(idx, heads, parts, tiles) : by_tiles(idx, heads, parts);
+  const int head = at.head, tile = at.tile, s = at.part;
   const int b = head / a.Hkv, kv = head - b * a.Hkv;   // group or sequence
   Source src = {a.k + kv * a.ks.h, a.v + kv * a.vs.h, a.ks, a.vs, nullptr, a.by_page, a.page, a.P, 0};
   const long long first_head = (long long)kv * a.G;
@@ -1218,7 +1186,7 @@ __global__ __launch_bounds__(kThreads, simd_waves(kKind, kDH)) void shared_kerne
     to.part = a.prefix_part + (((long long)head * a.prefix_tiles + tile) * parts + s) * kRows * (a.D + 3);
     run<T, kDH, kAligned, kKind, 1, true>(src, job, to, a.D, lds, st);
   } else {
-    constexpr int kRows = rows_of(Kind::kFew1);
+    constexpr int kRows = rows_of(Kind::kFew);
     const int append = a.kn != nullptr, len = ((uniform_ints)a.lens)[b];
     const bool fits = len >= 0 && len <= a.n_max - append;
     src.table = a.table + b * a.table_stride;
@@ -1241,9 +1209,9 @@ __global__ __launch_bounds__(kThreads, simd_waves(kKind, kDH)) void shared_kerne
     }
     job.q = static_cast<const T*>(a.q) + b * a.qs.b + first_head * a.qs.h;
     job.row0 = tile * kRows, job.rows = a.G, job.seen = src.keys;
-    share<Kind::kFew1>(&job, (src.keys + kBlock - 1) / kBlock, s, parts);
+    share<Kind::kFew>(&job, (src.keys + kBlock - 1) / kBlock, s, parts);
     to.part = a.own_part + (((long long)head * a.own_tiles + tile) * parts + s) * kRows * (a.D + 3);
-    run<T, kDH, kAligned, Kind::kFew1, 2, true>(src, job, to, a.D, lds, st);
+    run<T, kDH, kAligned, Kind::kFew, 2, true>(src, job, to, a.D, lds, st);
   }
 }
 
@@ -1274,7 +1242,7 @@ constexpr int kCu = 256;  // workgroups are counted for this many CUs, so that a
 constexpr long long kMaxGroups = UINT32_MAX / kThreads;  // workgroups of a launch: fewer than 2^32 threads
 
 static Kind choose_kind(long long rows) {
-  return rows <= kBlock ? Kind::kFew1 : rows <= 2 * kBlock ? Kind::kFew2 : Kind::kMany;
+  return rows <= 2 * kBlock ? Kind::kFew : Kind::kMany;
 }
 // Workgroups that a job of up to n_max keys is divided over, where there are `jobs` of them: `slots` a CU in all, parts of at
 // least `least` keys.
@@ -1306,7 +1274,7 @@ static bool attend_plan(int B, int H, int Hkv, int N, int page, int M, int D, At
   x->tiles = (rows + each - 1) / each;
   if (x->tiles > INT32_MAX / ((long long)B * Hkv)) return false;
   x->jobs = x->tiles * B * Hkv;
-  x->parts = choose_parts(x->kind == Kind::kFew2 ? 1 : 2, x->jobs, n_max, 256);
+  x->parts = choose_parts(2, x->jobs, n_max, 256);
   if (x->parts < 4 && n_max < 4096) x->parts = 1;
   x->bytes = x->parts > 1 ? part_bytes(x->kind, x->jobs, x->parts, D) : 0;
   return x->jobs * x->parts <= kMaxGroups;  // (the join has at most kManyRows / kJoinRows a job, of few jobs)
@@ -1315,10 +1283,8 @@ static bool attend_plan(int B, int H, int Hkv, int N, int page, int M, int D, At
 template <class T, int kDH, bool kAligned>
 static void launch_attend(const AttendArgs& a, const AttendPlan& x, hipStream_t stream) {
   const dim3 grid((unsigned)(x.jobs * x.parts));
-  if (x.kind == Kind::kFew1)
-    hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kFew1, true>), grid, dim3(kThreads), 0, stream, a);
-  else if (x.kind == Kind::kFew2)
-    hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kFew2, true>), grid, dim3(kThreads), 0, stream, a);
+  if (x.kind == Kind::kFew)
+    hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kFew, true>), grid, dim3(kThreads), 0, stream, a);
   else if (a.lse)
     hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kMany, true>), grid, dim3(kThreads), 0, stream, a);
   else
@@ -1334,10 +1300,8 @@ static hipError_t launch_attend(const AttendArgs& a, const AttendPlan& x, hipStr
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || x.parts == 1) return e;
   const dim3 grid((unsigned)(x.jobs * (rows_of(x.kind) / kJoinRows)));
-  if (x.kind == Kind::kFew1)
-    hipLaunchKernelGGL((attend_join_kernel<T, Kind::kFew1>), grid, dim3(kThreads), 0, stream, a);
-  else if (x.kind == Kind::kFew2)
-    hipLaunchKernelGGL((attend_join_kernel<T, Kind::kFew2>), grid, dim3(kThreads), 0, stream, a);
+  if (x.kind == Kind::kFew)
+    hipLaunchKernelGGL((attend_join_kernel<T, Kind::kFew>), grid, dim3(kThreads), 0, stream, a);
   else
     hipLaunchKernelGGL((attend_join_kernel<T, Kind::kMany>), grid, dim3(kThreads), 0, stream, a);
   return hipGetLastError();
@@ -1358,20 +1322,18 @@ static bool shared_plan(int R, int B, int H, int Hkv, int page, int Mp, int M, i
   x->own_tiles = (G + kBlock - 1) / kBlock;
   x->prefix_jobs = x->prefix_tiles * R * Hkv;
   x->own_jobs = x->own_tiles * B * Hkv;
-  x->prefix_parts = choose_parts(x->kind == Kind::kFew1 ? 2 : 1, x->prefix_jobs, p_max, x->kind == Kind::kMany ? 512 : 128);
+  x->prefix_parts = choose_parts(x->kind == Kind::kFew ? 2 : 1, x->prefix_jobs, p_max, x->kind == Kind::kMany ? 512 : 128);
   x->own_parts = choose_parts(2, x->own_jobs, n_max, 128);
   x->own_at = part_bytes(x->kind, x->prefix_jobs, x->prefix_parts, D);
-  x->bytes = x->own_at + part_bytes(Kind::kFew1, x->own_jobs, x->own_parts, D);
+  x->bytes = x->own_at + part_bytes(Kind::kFew, x->own_jobs, x->own_parts, D);
   return x->prefix_jobs * x->prefix_parts + x->own_jobs * x->own_parts <= kMaxGroups && (long long)B * H <= kMaxGroups * kJoinRows;
 }
 
 template <class T, int kDH, bool kAligned>
 static void launch_shared(const SharedArgs& a, const SharedPlan& x, hipStream_t stream) {
   const dim3 grid((unsigned)(x.prefix_jobs * x.prefix_parts + x.own_jobs * x.own_parts));
-  if (x.kind == Kind::kFew1)
-    hipLaunchKernelGGL((shared_kernel<T, kDH, kAligned, Kind::kFew1>), grid, dim3(kThreads), 0, stream, a);
-  else if (x.kind == Kind::kFew2)
-    hipLaunchKernelGGL((shared_kernel<T, kDH, kAligned, Kind::kFew2>), grid, dim3(kThreads), 0, stream, a);
+  if (x.kind == Kind::kFew)
+    hipLaunchKernelGGL((shared_kernel<T, kDH, kAligned, Kind::kFew>), grid, dim3(kThreads), 0, stream, a);
   else
     hipLaunchKernelGGL((shared_kernel<T, kDH, kAligned, Kind::kMany>), grid, dim3(kThreads), 0, stream, a);
 }
@@ -1385,10 +1347,8 @@ static hipError_t launch_shared(const SharedArgs& a, const SharedPlan& x, int ro
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const dim3 grid((rows + kJoinRows - 1) / kJoinRows);
-  if (x.kind == Kind::kFew1)
-    hipLaunchKernelGGL((shared_join_kernel<T, Kind::kFew1>), grid, dim3(kThreads), 0, stream, a, rows);
-  else if (x.kind == Kind::kFew2)
-    hipLaunchKernelGGL((shared_join_kernel<T, Kind::kFew2>), grid, dim3(kThreads), 0, stream, a, rows);
+  if (x.kind == Kind::kFew)
+    hipLaunchKernelGGL((shared_join_kernel<T, Kind::kFew>), grid, dim3(kThreads), 0, stream, a, rows);
   else
     hipLaunchKernelGGL((shared_join_kernel<T, Kind::kMany>), grid, dim3(kThreads), 0, stream, a, rows);
   return hipGetLastError();
