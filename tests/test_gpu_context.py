@@ -570,6 +570,65 @@ def test_in_graphs_with_eager_calls_between():
         torch.cuda.synchronize()
 
 
+def _two_launch_calls(g):
+    """Calls that keep parts in a workspace between two launches, on inputs of their own."""
+    H, H_kv, D, page = 8, 2, 64, 16
+    pool = Pool(g, H_kv, D, page, BF, 1300)
+    long, _ = pool.texts([9000], 1.0)
+    prefix, _ = pool.texts([3000], 1.0)
+    own, _ = pool.texts([40, 0, 300, 17], 1.0, spare=1)
+    other, _ = pool.texts([5000], 1.0)
+    long, prefix, own, other = (x.to(DEV) for x in (long, prefix, own, other))
+    q4, q60 = _randn((1, H, 4, D), g, BF), _randn((1, H, 60, D), g, BF)
+    qs, q1 = _randn((4, H, D), g, BF), _randn((1, H, D), g, BF)
+    lens = {n: _i32(n) for n in ((8996,), (8940,), (3000,), (40, 0, 300, 17), (5000,))}
+    assert _C.attend_workspace(1, H, H_kv, 4, page, long.shape[1], D) > 0 and _C.attend_workspace(1, H, H_kv, 60, page, long.shape[1], D) > 0
+    return [lambda: fa.attend_paged(q4, pool.k, pool.v, long, lens[(8996,)], return_lse=True),
+            lambda: fa.attend_paged(q60, pool.k, pool.v, long, lens[(8940,)], return_lse=True),
+            lambda: fa.decode_shared(qs, pool.k, pool.v, prefix, lens[(3000,)], own, lens[(40, 0, 300, 17)], return_lse=True),
+            lambda: fa.decode_paged(q1, pool.k, pool.v, other, lens[(5000,)], return_lse=True)]
+
+
+def test_threads_share_a_stream_and_its_workspace():
+    """Calls of four threads on one stream, which share its workspace (a split decode step's among them): each gives what it
+    gives by itself."""
+    import threading
+
+    calls = _two_launch_calls(_gen(36))
+    refs = [call() for call in calls]
+    torch.cuda.synchronize()
+    got, stream = [[] for _ in calls], torch.cuda.current_stream()
+
+    def run(n):
+        with torch.cuda.stream(stream):
+            for _ in range(60):
+                got[n].append(calls[n]())
+
+    threads = [threading.Thread(target=run, args=(n,)) for n in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for n, ref in enumerate(refs):
+        assert len(got[n]) == 60
+        assert all(torch.equal(a, b) for outs in got[n] for a, b in zip(outs, ref)), n
+
+
+def test_two_streams_at_once():
+    """The same calls on two streams, which may run at the same time, each with a workspace of its own."""
+    calls = _two_launch_calls(_gen(37))
+    refs = [call() for call in calls]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(20):
+        for k, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got.append(((i + k) % len(calls), calls[(i + k) % len(calls)]()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for n, outs in got for a, b in zip(outs, refs[n]))
+
+
 def test_prompt_in_chunks_then_samples_of_it():
     """The operators as a program runs them: two prompts go in by chunks of unequal lengths (rotated keys into the pages,
     attention over what is there), then three samples of each continue behind the shared prompt token by token; every

@@ -426,3 +426,46 @@ def test_decode_shared_python_refuses(kw, match):
     a.update(kw)
     with pytest.raises(RuntimeError, match=match):
         fa.decode_shared(*[a.pop(n) for n in ("q", "k", "v", "pt", "pl", "table", "lens")], **a)
+
+
+class _OnDevice0(torch.Tensor):
+    """A tensor of the CPU that says it is on device 0."""
+
+    is_cuda = True
+
+    def get_device(self):
+        return 0
+
+
+@pytest.mark.parametrize("op", ["attend_paged", "decode_shared"])
+def test_workspace_lives_until_the_launch(monkeypatch, op):
+    """Another thread's call on the same stream may replace the kept workspace by a larger one before this call launches: the
+    buffer whose address the launch gets is still held then."""
+    import weakref
+
+    from custom_flash_attn import pages, serving
+
+    kept, first, launched = {}, [], []
+
+    def make(dev, nbytes):
+        buffer = kept["it"] = torch.empty(nbytes, dtype=torch.uint8)
+        first.append(weakref.ref(buffer))
+        return buffer
+
+    def launch(index, fn, *args):
+        kept["it"] = None   # (what the other thread does)
+        launched.append(args)
+        assert first[0]() is not None, "the workspace was let go before the launch"
+        assert args[-2:] == (first[0]().data_ptr(), first[0]().numel())
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(serving, "_current_stream", lambda index: 7)
+    monkeypatch.setattr(serving, "_decode_workspace", make)
+    monkeypatch.setattr(pages, "_launch_on", launch)
+    t = lambda *shape, dtype=torch.bfloat16: torch.zeros(shape, dtype=dtype).as_subclass(_OnDevice0)  # noqa: E731
+    i32 = dict(dtype=torch.int32)
+    if op == "attend_paged":
+        fa.attend_paged(t(1, 4, 3, 64), t(3, 2, 16, 64), t(3, 2, 16, 64), t(1, 1000, **i32), t(1, **i32))
+    else:
+        fa.decode_shared(t(4, 4, 64), t(3, 2, 16, 64), t(3, 2, 16, 64), t(2, 9, **i32), t(2, **i32), t(4, 2, **i32), t(4, **i32))
+    assert len(launched) == len(first) == 1

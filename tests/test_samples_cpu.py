@@ -69,6 +69,10 @@ def test_extend_refuses_budgets_and_full_tables(monkeypatch):
     x = torch.zeros(1, 6, 2, 16)
     c.extend(0, x, x, x, torch.zeros(1, 6, 2, 16))
     assert len(calls) == 2 and calls[0][0].shape == (1, 2, 6, 16) and calls[1][3] is c.table
+    c.reset()
+    with pytest.raises(ValueError, match="no place for 25 more tokens"):
+        c.prompt(0, torch.zeros(1, 25, 2, 16), torch.zeros(1, 25, 2, 16), torch.zeros(1, 25, 2, 16), None)
+    assert len(calls) == 2
 
 
 def test_a_budget_refuses_several_tokens_in_the_model():

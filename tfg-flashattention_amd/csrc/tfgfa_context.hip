@@ -12,16 +12,30 @@
 //   O^T[dim][row] += V^T P^T: those 16 values are the B operand as they stand (the keys' order in the contraction is
 //   free), V's operand comes by transposing LDS reads.
 // K and V rows go from their pages to LDS by direct loads.  Where a page is a multiple of 16 keys, so many have one page: its
-// id and address are scalars, and rows past the end are past its descriptor, which gives zeros.
+// id and address are scalars, and rows past the end are past its descriptor, which gives zeros.  (8 keys at a time the
+// scalar unit, which a CU's waves share, was as busy as the VALU: 8192 causal tokens of 16 heads took 178 us for 157.)
 // Other pages: each lane has an address, of a row of zeros where there is no key.  A page id outside the pool gives a
 // row of NaN for K, so that NaN reaches the rows that see the key, and zeros for V.
 //
-// Few rows (up to 64 a job, 32 a workgroup): each wave streams blocks of its own (wave w of a workgroup takes blocks w, w + 4,
+// Few rows (up to 64 a job, 32 a workgroup, the two workgroups of a job side by side): each wave streams blocks of its own (wave w of a workgroup takes blocks w, w + 4,
 // ..) through LDS of its own, with no barrier; the four are joined through LDS.  Many rows: four waves
 // of 32 rows share tiles of 64 keys.  A job's keys may be divided over workgroups, whose parts a second kernel joins.
 //
 // Hidden keys have weight 0, but 0 times an infinite or NaN value is NaN: a wave whose sums hold NaN at the end takes its
 // keys again with products on the VALU that leave weights of 0 out (so the common path checks nothing).
+//
+// Measured from memory, in graphs, us (a copy moves 5.0 TB/s here, a large bf16 product 1290 TFLOP/s):
+//   2048 tokens behind 14336, 32 heads on 8 of 128, fp16, lse     522   988 TFLOP/s: the exponentials and sums of a step hide
+//                                                                       behind its products but for a fifth
+//   8192 causal tokens of 16 heads of 64                          156   886 TFLOP/s: as many exponentials for half the products
+//   8 prompts of up to 800 tokens behind up to 224, 25 heads      29.4  8 steps of 64 keys a workgroup on average, against
+//                                                                       about 5 us of its first loads and its end
+//   8 tokens behind 30000, twice, 32 heads on 8 of 128            51    4.0 TB/s
+//   4 tokens behind 1020, 8 times, 25 heads                       13.6  29 MB; 200 workgroups, start and end 5 us
+//   64 sequences on a prefix of 32000, 32 heads on 8 of 128       72    2.9 TB/s: 256 rows a key make the prefix 571 TFLOP/s,
+//                                                                       one wave a SIMD, waiting for its tiles half the time
+//   16 sequences on each of 4 prefixes of 700, 25 heads           27.3  3.2 TB/s, the join of the parts 5 of it
+//   8 sequences on a prefix of 900, 12 heads                      10.1  two launches
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -1035,6 +1049,8 @@ __host__ __device__ constexpr int rows_of(Kind kind) {
 }
 constexpr int lds_of(Kind kind, int kDH) { return kind == Kind::kMany ? many_lds(kDH) : few_lds(kDH); }
 
+// Waves a SIMD, which bound the registers.  Many rows, heads of 64: 3 (8192 causal tokens of 16 heads 178 us, with 2 188); few
+// rows: 4 (64 sequences on 4 prefixes 24.7, with 2 and loads a block ahead 32).
 constexpr int simd_waves(Kind kind, int kDH) {
   return kDH == 2 ? 2 : kind == Kind::kMany ? 3 : 4;
 }
@@ -1241,6 +1257,9 @@ constexpr int kCu = 256;  // workgroups are counted for this many CUs, so that a
 
 constexpr long long kMaxGroups = UINT32_MAX / kThreads;  // workgroups of a launch: fewer than 2^32 threads
 
+// 33 to 64 rows: 40 tokens of 8 sequences, 25 heads, take 14.7 us as two tiles of few and 19.5 as a tile of many, two thirds empty;
+// 8 prefixes for 16 sequences each, heads of 128, 43.3 and 38.2, but then with weights rounded once.  65 to 128: 32 tokens of 32 sequences, 32 heads
+// on 8 of 128, take 69 as many and 101 as few, 100 tokens of 8 sequences 21.7 and 18.5.
 static Kind choose_kind(long long rows) {
   return rows <= 2 * kBlock ? Kind::kFew : Kind::kMany;
 }
@@ -1274,6 +1293,9 @@ static bool attend_plan(int B, int H, int Hkv, int N, int page, int M, int D, At
   x->tiles = (rows + each - 1) / each;
   if (x->tiles > INT32_MAX / ((long long)B * Hkv)) return false;
   x->jobs = x->tiles * B * Hkv;
+  // Two workgroups a CU, parts of 256 keys or more (512 tokens behind 16000, 32 heads on 8 of 128: 142 us, with one 157, with
+  // three 150).  Fewer than four parts of a short cache cost more in joining than they gain (4 tokens behind 1020, 8 times, 25
+  // heads: 13.7 us whole, 16.7 in two).
   x->parts = choose_parts(2, x->jobs, n_max, 256);
   if (x->parts < 4 && n_max < 4096) x->parts = 1;
   x->bytes = x->parts > 1 ? part_bytes(x->kind, x->jobs, x->parts, D) : 0;
@@ -1322,6 +1344,8 @@ static bool shared_plan(int R, int B, int H, int Hkv, int page, int Mp, int M, i
   x->own_tiles = (G + kBlock - 1) / kBlock;
   x->prefix_jobs = x->prefix_tiles * R * Hkv;
   x->own_jobs = x->own_tiles * B * Hkv;
+  // Few rows: two workgroups a CU for prefixes (2 of 30000 for 16 sequences each 59 us, with one 65; 1 of 8000 24, with one
+  // 20), many: one, with the sequences' own beside them (1 of 32000 for 64 sequences 70, with two 76).
   x->prefix_parts = choose_parts(x->kind == Kind::kFew ? 2 : 1, x->prefix_jobs, p_max, x->kind == Kind::kMany ? 512 : 128);
   x->own_parts = choose_parts(2, x->own_jobs, n_max, 128);
   x->own_at = part_bytes(x->kind, x->prefix_jobs, x->prefix_parts, D);

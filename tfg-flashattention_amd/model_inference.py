@@ -362,6 +362,7 @@ class PagedKVCache:
         import custom_flash_attn
 
         n = k.shape[1]
+        self._check_room(n)
         q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
         custom_flash_attn.append_paged(k, v, self.k[layer], self.v[layer], self.table, self.seqlens)
         if self.weights is None:
