@@ -23,7 +23,7 @@ _ROTATED = {torch.bfloat16: _C.DTYPE_BF16, torch.float16: _C.DTYPE_F16, torch.fl
 _INTS = (torch.int32, torch.int64)
 
 # Whether a function transform is active, and the forward-mode level (a torch without them has neither).
-_transform = getattr(torch._C._functorch, "peek_interpreter_stack", lambda: None)
+_transform = getattr(getattr(torch._C, "_functorch", None), "peek_interpreter_stack", lambda: None)
 
 
 def _view(t):
