@@ -18,7 +18,7 @@
 // row of NaN for K, so that NaN reaches the rows that see the key, and zeros for V.
 //
 // Few rows (up to 64 a job, 32 a workgroup, the two workgroups of a job side by side): each wave streams blocks of its own
-// (wave w of a workgroup takes blocks w, w + 4, ..) through LDS of its own, with no barrier; the four are joined through LDS.
+// (wave w of W in a workgroup takes blocks w, w + W, ..) through LDS of its own, with no barrier; they are joined through LDS.
 // Many rows: four waves of 32 rows share tiles of 64 keys, and store their rows from registers (through LDS 8 prompts take
 // 32.0 us for 29.5).  A job's keys may be divided over workgroups, whose parts a second kernel joins.
 //
@@ -603,14 +603,16 @@ struct Sink {
   int fill_to, fill;              // rows from Job::rows up to here get zeros (fill 1) or NaN (fill 2)
 };
 
-constexpr int few_lds(int kDH) {  // a block of each wave, or its rows
-  const int blocks = kWaves * 2 * kDH * kHalfBytes, rows = kWaves * kBlock * 64 * kDH * 4;
+constexpr int few_lds(int kDH, int waves) {  // a block of each wave, or its rows
+  const int blocks = waves * 2 * kDH * kHalfBytes, rows = waves * kBlock * 64 * kDH * 4;
   return blocks > rows ? blocks : rows;
 }
 constexpr int many_lds(int kDH) { return 4 * kDH * 2 * kHalfBytes; }  // four tiles of 64 keys
 
+// Of each wave's rows.
+template <int kW>
 struct Stats {
-  float m[kWaves * kBlock], l[kWaves * kBlock], lp[kWaves * kBlock];
+  float m[kW * kBlock], l[kW * kBlock], lp[kW * kBlock];
 };
 
 template <class T, int kDH, int kParts>
@@ -631,8 +633,8 @@ __device__ __forceinline__ void load_rows(State<T, kDH, kParts>& w, const Job& j
 }
 
 // Few rows: row `row` of the workgroup's, 8 dims from 8 c8 on, joined over the waves' states, to its place.
-template <class T, int kDH>
-__device__ __forceinline__ void put(const unsigned char* rows, const Stats& st, int row, int c8, const Job& job,
+template <class T, int kDH, int kW>
+__device__ __forceinline__ void put(const unsigned char* rows, const Stats<kW>& st, int row, int c8, const Job& job,
                                     const Sink& to, int D) {
   constexpr int kPieces = 16 * kDH;
   const int r = job.row0 + row;
@@ -640,11 +642,11 @@ __device__ __forceinline__ void put(const unsigned char* rows, const Stats& st, 
   if (!real && !(to.part == nullptr && to.fill != 0 && r < to.fill_to)) return;
   float M = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, st.m[w * kBlock + row]);
+  for (int w = 0; w < kW; ++w) M = fmaxf(M, st.m[w * kBlock + row]);
   float l = 0.f, lp = 0.f;
   f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < kW; ++w) {
     const int at = w * kBlock + row;
     const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((st.m[at] - M) * job.scale_log2);
     l = fmaf(f, st.l[at], l), lp = fmaf(f, st.lp[at], lp);
@@ -682,14 +684,15 @@ __device__ __forceinline__ void put(const unsigned char* rows, const Stats& st, 
 }
 
 // Few rows.
-template <class T, int kDH, bool kAligned>
-__device__ __forceinline__ void run_few(const Source& src, const Job& job, const Sink& to, int D, unsigned char* lds, Stats& st) {
+template <class T, int kDH, bool kAligned, int kW>
+__device__ __forceinline__ void run_few(const Source& src, const Job& job, const Sink& to, int D, unsigned char* lds,
+                                        Stats<kW>& st) {
   constexpr int kBytes = 2 * kDH * kHalfBytes;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   unsigned char* const block = lds + wave * kBytes;
   const uint32_t block_at = tfgfa::lds_addr(block);
-  const int count = max(0, (job.last - job.first - wave + kWaves - 1) / kWaves);
-  auto key = [&](int n) { return (job.first + wave + n * kWaves) * kBlock; };
+  const int count = max(0, (job.last - job.first - wave + kW - 1) / kW);
+  auto key = [&](int n) { return (job.first + wave + n * kW) * kBlock; };
   State<T, kDH, 2> w;
   const float inv = 1.f / job.scale_log2;
   w.init(lane);
@@ -719,8 +722,8 @@ __device__ __forceinline__ void run_few(const Source& src, const Job& job, const
   __syncthreads();  // (the rows' places are the blocks')
   w.publish(lds + wave * kBlock * 64 * kDH * 4, st.m + wave * kBlock, st.l + wave * kBlock, st.lp + wave * kBlock, lane);
   __syncthreads();
-  for (int e = tid; e < kBlock * 8 * kDH; e += kThreads)
-    if (e % (8 * kDH) * 8 < D) put<T, kDH>(lds, st, e / (8 * kDH), e % (8 * kDH), job, to, D);
+  for (int e = tid; e < kBlock * 8 * kDH; e += 64 * kW)
+    if (e % (8 * kDH) * 8 < D) put<T, kDH, kW>(lds, st, e / (8 * kDH), e % (8 * kDH), job, to, D);
 }
 
 // Many rows.  Two K tiles and two V tiles of 64 keys in LDS.  Step j of the workgroup: block 2j; wait for K of tile j + 1 and
@@ -1044,11 +1047,12 @@ struct AttendArgs {
 };
 
 // How many rows a workgroup takes, and how.
-enum class Kind { kFew, kMany };
+enum class Kind { kFew, kFewWide, kMany };
 __host__ __device__ constexpr int rows_of(Kind kind) {
-  return kind == Kind::kFew ? kBlock : kManyRows;
+  return kind == Kind::kMany ? kManyRows : kBlock;
 }
-constexpr int lds_of(Kind kind, int kDH) { return kind == Kind::kMany ? many_lds(kDH) : few_lds(kDH); }
+constexpr int waves_of(Kind kind) { return kind == Kind::kFewWide ? 8 : kWaves; }
+constexpr int lds_of(Kind kind, int kDH) { return kind == Kind::kMany ? many_lds(kDH) : few_lds(kDH, waves_of(kind)); }
 
 // Waves a SIMD, which bound the registers.  Many rows, heads of 64: 3 (8192 causal tokens of 16 heads 178 us, with 2 188); few
 // rows: 4 (64 sequences on 4 prefixes 24.7, with 2 and loads a block ahead 32).
@@ -1057,11 +1061,12 @@ constexpr int simd_waves(Kind kind, int kDH) {
 }
 
 template <class T, int kDH, bool kAligned, Kind kKind, int kParts, bool kLse>
-__device__ __forceinline__ void run(const Source& src, const Job& job, const Sink& to, int D, unsigned char* lds, Stats& st) {
+__device__ __forceinline__ void run(const Source& src, const Job& job, const Sink& to, int D, unsigned char* lds,
+                                    Stats<waves_of(kKind)>& st) {
   if constexpr (kKind == Kind::kMany)
     run_many<T, kDH, kAligned, kParts, kLse>(src, job, to, D, lds);
   else
-    run_few<T, kDH, kAligned>(src, job, to, D, lds, st);
+    run_few<T, kDH, kAligned, waves_of(kKind)>(src, job, to, D, lds, st);
 }
 
 // Which head, part and tile of rows a workgroup takes; in either order the workgroups of a head are on one XCD where 8 divides
@@ -1084,16 +1089,16 @@ __device__ __forceinline__ Work by_heads(int idx, int heads, int parts, int tile
 // Part s of S of `blocks` blocks: whole rounds of the workgroup.
 template <Kind kKind>
 __device__ __forceinline__ void share(Job* job, int blocks, int s, int S) {
-  constexpr int kRound = kKind == Kind::kMany ? 2 : kWaves;
+  constexpr int kRound = kKind == Kind::kMany ? 2 : waves_of(kKind);
   const int rounds = (blocks + kRound - 1) / kRound;
   job->first = kRound * (int)((long long)rounds * s / S);
   job->last = min(blocks, kRound * (int)((long long)rounds * (s + 1) / S));
 }
 
 template <class T, int kDH, bool kAligned, Kind kKind, bool kLse>
-__global__ __launch_bounds__(kThreads, simd_waves(kKind, kDH)) void attend_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(64 * waves_of(kKind), simd_waves(kKind, kDH)) void attend_kernel(const AttendArgs a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[lds_of(kKind, kDH)];
-  __shared__ Stats st;
+  __shared__ Stats<waves_of(kKind)> st;
   constexpr int kRows = rows_of(kKind);
   // The longest first (the last tiles of a causal sequence); a key-value head's workgroups on one XCD where 8 divides
   // their number.
@@ -1172,10 +1177,10 @@ struct SharedArgs {
 };
 
 template <class T, int kDH, bool kAligned, Kind kKind>
-__global__ __launch_bounds__(kThreads, simd_waves(kKind, kDH)) void shared_kernel(const SharedArgs a) {
+__global__ __launch_bounds__(64 * waves_of(kKind), simd_waves(kKind, kDH)) void shared_kernel(const SharedArgs a) {
   constexpr int kPrefixLds = lds_of(kKind, kDH), kOwnLds = lds_of(Kind::kFew, kDH);
   __shared__ __attribute__((aligned(1024))) unsigned char lds[kPrefixLds > kOwnLds ? kPrefixLds : kOwnLds];
-  __shared__ Stats st;
+  __shared__ Stats<waves_of(kKind)> st;
   Job job;
   Sink to;
   job.by_group = a.by_group, job.G = a.G, job.causal = 0;
@@ -1294,10 +1299,13 @@ static bool attend_plan(int B, int H, int Hkv, int N, int page, int M, int D, At
   x->tiles = (rows + each - 1) / each;
   if (x->tiles > INT32_MAX / ((long long)B * Hkv)) return false;
   x->jobs = x->tiles * B * Hkv;
+  // Eight waves a workgroup where a CU has one (12 tokens of 8 sequences, 32 heads on 8 of 128, 14.6 us, with four 18.5; 4
+  // tokens behind 1020, 8 times, 25 heads, 11.8 and 13.7; 2 behind 500, 64 times, 12 heads, 18.1 and 14.8, so not there).
+  if (x->kind == Kind::kFew && x->jobs <= kCu) x->kind = Kind::kFewWide;
   // Two workgroups a CU, parts of 256 keys or more (512 tokens behind 16000, 32 heads on 8 of 128: 142 us, with one 157, with
   // three 150).  Fewer than four parts of a short cache cost more in joining than they gain (4 tokens behind 1020, 8 times, 25
-  // heads: 13.7 us whole, 16.7 in two).
-  x->parts = choose_parts(2, x->jobs, n_max, 256);
+  // heads: 13.7 us whole, 16.7 in two, of four waves).
+  x->parts = choose_parts(x->kind == Kind::kFewWide ? 1 : 2, x->jobs, n_max, 256);
   if (x->parts < 4 && n_max < 4096) x->parts = 1;
   x->bytes = x->parts > 1 ? part_bytes(x->kind, x->jobs, x->parts, D) : 0;
   return x->jobs * x->parts <= kMaxGroups;  // (the join has at most kManyRows / kJoinRows a job, of few jobs)
@@ -1306,7 +1314,10 @@ static bool attend_plan(int B, int H, int Hkv, int N, int page, int M, int D, At
 template <class T, int kDH, bool kAligned>
 static void launch_attend(const AttendArgs& a, const AttendPlan& x, hipStream_t stream) {
   const dim3 grid((unsigned)(x.jobs * x.parts));
-  if (x.kind == Kind::kFew)
+  if (x.kind == Kind::kFewWide)
+    hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kFewWide, true>), grid, dim3(64 * waves_of(Kind::kFewWide)), 0,
+                       stream, a);
+  else if (x.kind == Kind::kFew)
     hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kFew, true>), grid, dim3(kThreads), 0, stream, a);
   else if (a.lse)
     hipLaunchKernelGGL((attend_kernel<T, kDH, kAligned, Kind::kMany, true>), grid, dim3(kThreads), 0, stream, a);
@@ -1323,7 +1334,7 @@ static hipError_t launch_attend(const AttendArgs& a, const AttendPlan& x, hipStr
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || x.parts == 1) return e;
   const dim3 grid((unsigned)(x.jobs * (rows_of(x.kind) / kJoinRows)));
-  if (x.kind == Kind::kFew)
+  if (x.kind != Kind::kMany)
     hipLaunchKernelGGL((attend_join_kernel<T, Kind::kFew>), grid, dim3(kThreads), 0, stream, a);
   else
     hipLaunchKernelGGL((attend_join_kernel<T, Kind::kMany>), grid, dim3(kThreads), 0, stream, a);
