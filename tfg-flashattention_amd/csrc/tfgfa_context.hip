@@ -31,8 +31,8 @@
 //   8192 causal tokens of 16 heads of 64                          156   886 TFLOP/s: as many exponentials for half the products
 //   8 prompts of up to 800 tokens behind up to 224, 25 heads      29.4  8 steps of 64 keys a workgroup on average, against
 //                                                                       about 5 us of its first loads and its end
-//   8 tokens behind 30000, twice, 32 heads on 8 of 128            51    4.0 TB/s
-//   4 tokens behind 1020, 8 times, 25 heads                       13.6  29 MB; 200 workgroups, start and end 5 us
+//   8 tokens behind 30000, twice, 32 heads on 8 of 128            50    4.1 TB/s
+//   4 tokens behind 1020, 8 times, 25 heads                       11.8  29 MB; 200 workgroups, start and end 5 us
 //   64 sequences on a prefix of 32000, 32 heads on 8 of 128       72    2.9 TB/s: 256 rows a key make the prefix 571 TFLOP/s,
 //                                                                       one wave a SIMD, waiting for its tiles half the time
 //   16 sequences on each of 4 prefixes of 700, 25 heads           27.3  3.2 TB/s, the join of the parts 5 of it
