@@ -23,7 +23,9 @@
 // 32.0 us for 29.5).  A job's keys may be divided over workgroups, whose parts a second kernel joins.
 //
 // Hidden keys have weight 0, but 0 times an infinite or NaN value is NaN: a wave whose sums hold NaN at the end takes its
-// keys again with products on the VALU that leave weights of 0 out (so the common path checks nothing).
+// keys again with products on the VALU that leave weights of 0 out (so the common path checks nothing).  So does a workgroup
+// of many rows, whose offsets are in the log2 domain, where one ends at 2^24 or past it: there rounding it moves all weights
+// (8192 causal tokens of 16 heads of 64 with such scores: 3.1 ms for 0.16).
 //
 // Measured from memory, in graphs, us (a copy moves 5.0 TB/s here, a large bf16 product 1290 TFLOP/s):
 //   2048 tokens behind 14336, 32 heads on 8 of 128, fp16, lse     522   988 TFLOP/s: the exponentials and sums of a step hide
@@ -466,12 +468,11 @@ struct State {
   // and rounding, one matrix instruction and a share of them at a time (a wave's VALU work overlaps its own matrix
   // instructions).  Offsets are in the log2 domain (m = thr): 2^(c s - m) is one v_fma and one v_exp.
   // The sum of the rounded weights tells when an offset has to move: a weight past the type's range, or a sum past kBound,
-  // is infinite, NaN or above it.  Where c s passes float32's range (scores past 2.3e38 / scale), `far` asks for the exact
-  // pass.
+  // is infinite, NaN or above it.
   static constexpr float kBound = std::is_same_v<T, __bf16> ? 0x1p64f : 0x1.fffffep127f;
   template <bool kPV, bool kLse>
   __device__ __forceinline__ void fused(const unsigned char* v, const unsigned char* k, f32x16& s, v8 (&part)[kParts][2],
-                                        float c, float head, bool* far) {
+                                        float c, float head) {
     constexpr int kPairs = 2 * kOT;
     v8 vo[2], ko[2];
     if constexpr (kPV) vo[0] = values(v, 0, 0), vo[1] = values(v, 1, 0);
@@ -512,9 +513,7 @@ struct State {
         // (As integers: past the bound, infinite or NaN.)
         if (__builtin_amdgcn_ballot_w64(__float_as_uint(sum) > __float_as_uint(kBound))) {
           const float top = over_pair(largest(s), [](float x, float y) { return fmaxf(x, y); });
-          const float at = top * c;
-          *far = *far || (fabsf(top) < INFINITY && !(fabsf(at) < INFINITY));
-          const float to = fmaxf(fmaxf(m, kLowest), at - head);
+          const float to = fmaxf(fmaxf(m, kLowest), top * c - head);
           const float f = __builtin_amdgcn_exp2f(m - to);
           m = to, lp *= f, l *= f;
 #pragma unroll
@@ -776,14 +775,13 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   w.m = -INFINITY;
   const float head = fminf(Elem<T>::kHead, 1e30f * c);
-  bool far = false;
   f32x16 s;
   typename W::v8 part[kParts][2];
   if (act > 0) w.scores(s, lds);
   // Half a step: block u, V of the one before it and K of the one after it in LDS.
   auto block = [&](int u, const unsigned char* v, const unsigned char* k, auto first) {
     if (u >= full) w.mask(s, (job.first + u) * kBlock, lane);
-    w.template fused<!decltype(first)::value, kKeepL>(v, k, s, part, c, head, &far);
+    w.template fused<!decltype(first)::value, kKeepL>(v, k, s, part, c, head);
   };
   auto last = [&](const unsigned char* v) { w.output(v, part); };
   auto turn = [&](int j) {  // between the halves of step j
@@ -836,6 +834,11 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
   } else if (act > 0) {
     last(v_of((tiles - 1) & 1) + kHalf);
   }
+  // The offset is c top - head rounded, weights are of c s exactly: the row's largest is 2^(head + what rounding left), at most
+  // 2^(head + 1) below kFar, and from there on may be past the type on either side.  Offsets only rise, and what an earlier
+  // one lost is 0 beside the last.  (kLowest, too, is what scores past float32's range in the log2 domain leave.)
+  constexpr float kFar = 0x1p24f;
+  const bool far = act > 0 && w.seen > job.first * kBlock && !(fabsf(w.m) < kFar);
   w.rescale(c);
   if (kParts > 1) w.lp = w.l;
   w.thr = 0.f;
