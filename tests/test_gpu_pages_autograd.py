@@ -1,0 +1,68 @@
+"""What the operators around a paged cache tell autograd: that tensors of the caller's were written (needs a GPU)."""
+import pytest
+import torch
+
+import custom_flash_attn as fa
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def _randn(*shape, dtype=F32):
+    return torch.randn(shape, device=DEV).to(dtype)
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _cache(B, H_kv, D=64, page=16, M=4):
+    k_pages, v_pages = (torch.zeros(B * M, H_kv, page, D, dtype=BF, device=DEV) for _ in range(2))
+    return k_pages, v_pages, torch.arange(B * M, dtype=torch.int32, device=DEV).view(B, M)
+
+
+def test_in_place_rotation_of_a_saved_tensor_is_noticed():
+    rotary = fa.Rotary(64, device=DEV)
+    q, k, w = _randn(1, 2, 5, 64), _randn(1, 2, 5, 64), _randn(1, 2, 5, 64).requires_grad_()
+    for x, given in ((q, dict(q_out=q)), (k, dict(q_out=torch.empty_like(q), k_out=k))):
+        y = w * x
+        fa.rotate(q, k, 0, rotary, **given)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    y = w * q                       # (nothing of q is written here)
+    fa.rotate(q, k, 0, rotary, k_out=k)
+    fa.rotate(q, k, 0, rotary)
+    y.sum().backward()
+    assert torch.equal(w.grad, q)
+
+
+def test_what_the_paged_operators_write_is_noticed():
+    B, H, H_kv, N, D = 2, 4, 2, 3, 64
+    k_pages, v_pages, table = _cache(B, H_kv)
+    q, k, v = _randn(B, H, N, D, dtype=BF), _randn(B, H_kv, N, D, dtype=BF), _randn(B, H_kv, N, D, dtype=BF)
+    lens, out, vec = _i32([5, 7]), torch.zeros(B, H, N, D, dtype=BF, device=DEV), torch.zeros(B, H, D, dtype=BF, device=DEV)
+    prefix, plens = table[:1, :1].contiguous(), _i32([5])
+    rotary = fa.Rotary(64, device=DEV)
+    calls = [
+        (lambda: fa.append_paged(k, v, k_pages, v_pages, table, lens, rotary=rotary, q=q, q_out=q), [k_pages, v_pages, q]),
+        (lambda: fa.append_paged(k, v, k_pages, v_pages, table, lens), [k_pages, v_pages]),
+        (lambda: fa.attend_paged(q, k_pages, v_pages, table, lens, out=out), [out]),
+        (lambda: fa.attend_paged(q, k_pages, v_pages, table, lens), []),
+        (lambda: fa.decode_shared(q[:, :, 0], k_pages, v_pages, prefix, plens, table, lens, k[:, :, 0], v[:, :, 0], out=vec),
+         [k_pages, v_pages, vec]),
+        (lambda: fa.decode_shared(q[:, :, 0], k_pages, v_pages, prefix, plens, table, lens, out=vec), [vec]),
+        (lambda: fa.decode_shared(q[:, :, 0], k_pages, v_pages, prefix, plens, table, lens), []),
+    ]
+    everything = [q, k, v, k_pages, v_pages, table, lens, out, vec, prefix, plens]
+    for n, (call, written) in enumerate(calls):
+        before = [t._version for t in everything]
+        call()
+        for i, (t, was) in enumerate(zip(everything, before)):
+            assert (t._version > was) == any(t is x for x in written), (n, i)
+    with torch.inference_mode():
+        pools = [x.clone() for x in (k_pages, v_pages)]
+        fa.append_paged(k, v, *pools, table, lens)
+    fa.append_paged(k, v, *pools, table, lens)   # inference tensors have no versions
+    torch.cuda.synchronize()

@@ -5,7 +5,8 @@ prefix.
 The reference's model has learned positions and keeps no cache (src/py/model_inference.py:166-228); nothing here has
 a counterpart in it.  The functions check their arguments (RuntimeError, before anything is launched), launch on the
 current stream of the tensors' device and do not synchronise.  :func:`rotate` has a gradient; the others are inference
-operators, whose results carry none.
+operators, whose results carry none.  Tensors of the caller's that are written (outputs, pools) count a version, as by torch's
+operators in place, so that a backward pass that needs their old values raises.
 """
 from __future__ import annotations
 
@@ -13,6 +14,7 @@ import math
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _C, _check_vec, _DTYPES, MAX_HEAD_DIM, _launch_on
 from .serving import (_accepts_pages, _check_pages, _check_seqlens, _check_table, _extent, _is_seqlens, _is_table,
@@ -274,6 +276,7 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions, rotary: Rotary, *
     if k is not None and k_out is None:
         k_out = torch.empty_like(k)
     _rotate(q, k, positions, rotary, q_out, k_out, False)
+    increment_version([x for x in outs if x is not None])
     return q_out if k is None else (q_out, k_out)
 
 
@@ -387,6 +390,7 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
                page_table.stride(0), cache_seqlens.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
                0 if positions is None else positions.data_ptr(), _view(q), _view(q_out), pad, turns, rot, interleaved,
                magnitude, B, 0 if q is None else q.shape[1], H_kv, N, P, page, page_table.shape[1], D, _DTYPES[k.dtype])
+    increment_version((k_pages, v_pages) if q is None or pad else (k_pages, v_pages, q_out))
     return q_out
 
 
@@ -459,6 +463,8 @@ def attend_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
                cache_seqlens.data_ptr(), 0 if lengths is None else lengths.data_ptr(), _view(out),
                0 if lse is None else lse.data_ptr(), pad, bool(causal), B, H, H_kv, N, P, page, M, D, _DTYPES[q.dtype], scale,
                *_extent(workspace))
+    if not pad:
+        increment_version(out)
     return (out, lse) if return_lse else out
 
 
@@ -529,8 +535,11 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     P, H_kv, page, D = k_pages.shape
     B, H, _ = q.shape
     (R, M_prefix), M, index = prefix_table.shape, page_table.shape[1], k_pages.get_device()
+    written = [] if k_new is None else [k_pages, v_pages]
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, H, D))
+    else:
+        written.append(out)
     lse = q.new_empty((B, H), dtype=torch.float32) if return_lse else None
     scale = (1.0 / math.sqrt(D)) if softmax_scale is None else float(softmax_scale)
     workspace = _workspace(workspace, index, 0 if workspace is not None else
@@ -540,4 +549,6 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                cache_seqlens.data_ptr(), _NONE3 if k_new is None else _view(k_new), _NONE3 if v_new is None else _view(v_new),
                _view(out), 0 if lse is None else lse.data_ptr(), R, B, H, H_kv, P, page, M_prefix, M, D, _DTYPES[q.dtype],
                scale, *_extent(workspace))
+    if written:
+        increment_version(written)
     return (out, lse) if return_lse else out
