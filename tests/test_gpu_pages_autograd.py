@@ -66,3 +66,27 @@ def test_what_the_paged_operators_write_is_noticed():
         fa.append_paged(k, v, *pools, table, lens)
     fa.append_paged(k, v, *pools, table, lens)   # inference tensors have no versions
     torch.cuda.synchronize()
+
+
+def test_outputs_that_require_a_gradient_are_refused():
+    B, H, N, D = 2, 2, 3, 64
+    k_pages, v_pages, table = _cache(B, H)
+    x, lens, rotary = _randn(B, H, N, D, dtype=BF), _i32([5, 7]), fa.Rotary(64, device=DEV)
+    out = torch.zeros_like(x).requires_grad_()
+    vec = torch.zeros(B, H, D, dtype=BF, device=DEV).requires_grad_()
+    pool = k_pages.clone().requires_grad_()
+    calls = [lambda: fa.rotate(x, None, 0, rotary, q_out=out),
+             lambda: fa.rotate(x, x, 0, rotary, k_out=out),
+             lambda: fa.append_paged(x, x, k_pages, v_pages, table, lens, rotary=rotary, q=x, q_out=out),
+             lambda: fa.append_paged(x, x, pool, v_pages, table, lens),
+             lambda: fa.append_paged(x, x, k_pages, pool, table, lens),
+             lambda: fa.attend_paged(x, k_pages, v_pages, table, lens, out=out),
+             lambda: fa.decode_shared(x[:, :, 0], k_pages, v_pages, table[:1], lens[:1], table, lens, out=vec),
+             lambda: fa.decode_shared(x[:, :, 0], pool, v_pages, table[:1], lens[:1], table, lens, x[:, :, 0], x[:, :, 0])]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            call()
+        with torch.no_grad():
+            call()
+    fa.attend_paged(x, pool, v_pages, table, lens)   # (only read)
+    torch.cuda.synchronize()

@@ -1,0 +1,61 @@
+"""More refusals of the operators around a paged cache, on the CPU: with tensors that say they are on a device, and nothing
+launched."""
+import pytest
+import torch
+
+import custom_flash_attn as fa
+from custom_flash_attn import pages
+
+BF, I32 = torch.bfloat16, torch.int32
+
+
+class _Dev(torch.Tensor):
+    """A CPU tensor that calls itself a device's."""
+
+    is_cuda = True
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        with torch._C.DisableTorchFunctionSubclass():
+            return func(*args, **(kwargs or {}))
+
+
+def _dev(*shape, dtype=BF):
+    return torch.zeros(shape, dtype=dtype).as_subclass(_Dev)
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """Calls that reach the launch."""
+    calls = []
+    monkeypatch.setattr(pages, "_launch_on", lambda index, fn, *args: calls.append(args))
+    monkeypatch.setattr(pages, "_workspace", lambda given, index, nbytes: None)
+    return calls
+
+
+def _grad(t):
+    return t.detach().requires_grad_().as_subclass(_Dev)
+
+
+def test_written_tensors_that_require_a_gradient(launches):
+    x, vec, pool, table, lens = _dev(2, 2, 3, 64), _dev(2, 2, 64), _dev(8, 2, 16, 64), _dev(2, 4, dtype=I32), _dev(2, dtype=I32)
+    rotary = fa.Rotary(64, device="cpu")
+    calls = [lambda: fa.rotate(x, None, 0, rotary, q_out=_grad(x)),
+             lambda: fa.rotate(x, x, 0, rotary, k_out=_grad(x)),
+             lambda: fa.append_paged(x, x, pool, pool, table, lens, rotary=rotary, q=x, q_out=_grad(x)),
+             lambda: fa.append_paged(x, x, _grad(pool), pool, table, lens),
+             lambda: fa.append_paged(x, x, pool, _grad(pool), table, lens),
+             lambda: fa.attend_paged(x, pool, pool, table, lens, out=_grad(x)),
+             lambda: fa.decode_shared(vec, pool, pool, table, lens, table, lens, out=_grad(vec)),
+             lambda: fa.decode_shared(vec, pool, _grad(pool), table, lens, table, lens, vec, vec)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            call()
+    assert not launches
+    with torch.no_grad():
+        for call in calls:
+            call()
+    assert len(launches) == len(calls)
+    fa.attend_paged(x, _grad(pool), pool, table, lens)                          # (only read)
+    fa.decode_shared(vec, _grad(pool), pool, table, lens, table, lens)
+    assert len(launches) == len(calls) + 2

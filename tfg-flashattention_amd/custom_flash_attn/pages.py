@@ -6,7 +6,8 @@ The reference's model has learned positions and keeps no cache (src/py/model_inf
 a counterpart in it.  The functions check their arguments (RuntimeError, before anything is launched), launch on the
 current stream of the tensors' device and do not synchronise.  :func:`rotate` has a gradient; the others are inference
 operators, whose results carry none.  Tensors of the caller's that are written (outputs, pools) count a version, as by torch's
-operators in place, so that a backward pass that needs their old values raises.
+operators in place, so that a backward pass that needs their old values raises; those that require a gradient are refused
+where gradients are recorded.
 """
 from __future__ import annotations
 
@@ -26,6 +27,15 @@ _INTS = (torch.int32, torch.int64)
 
 # Whether a function transform is active, and the forward-mode level (a torch without them has neither).
 _transform = getattr(getattr(torch._C, "_functorch", None), "peek_interpreter_stack", lambda: None)
+
+
+def _check_written(*tensors) -> None:
+    """Tensors that a call writes beside autograd (None: not given)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("a tensor that is written requires a gradient, which is not differentiable: call under "
+                                   "torch.no_grad() or give another")
 
 
 def _view(t):
@@ -271,6 +281,7 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions, rotary: Rotary, *
     if (_transform() is not None or getattr(forward_ad, "_current_level", -1) >= 0
             or (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)))):
         raise RuntimeError("q_out and k_out are not differentiable: rotate without them, or under torch.no_grad()")
+    _check_written(q_out, k_out)
     if q_out is None:
         q_out = torch.empty_like(q)
     if k is not None and k_out is None:
@@ -379,6 +390,7 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     """
     if not _accepts_append(k, v, k_pages, v_pages, page_table, cache_seqlens, lengths, rotary, positions, q, q_out):
         _check_append(k, v, k_pages, v_pages, page_table, cache_seqlens, lengths, rotary, positions, q, q_out)
+    _check_written(k_pages, v_pages, q_out)
     P, H_kv, page, D = k_pages.shape
     B, _, N, _ = k.shape
     pad = q_out is None
@@ -445,6 +457,7 @@ def attend_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     """
     if not _accepts_attend(q, k_pages, v_pages, page_table, cache_seqlens, lengths, out):
         _check_attend(q, k_pages, v_pages, page_table, cache_seqlens, lengths, out)
+    _check_written(out)
     P, H_kv, page, D = k_pages.shape
     B, H, N, _ = q.shape
     M, index = page_table.shape[1], k_pages.get_device()
@@ -535,11 +548,10 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     P, H_kv, page, D = k_pages.shape
     B, H, _ = q.shape
     (R, M_prefix), M, index = prefix_table.shape, page_table.shape[1], k_pages.get_device()
-    written = [] if k_new is None else [k_pages, v_pages]
+    written = ([] if k_new is None else [k_pages, v_pages]) + ([] if out is None else [out])
+    _check_written(*written)
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, H, D))
-    else:
-        written.append(out)
     lse = q.new_empty((B, H), dtype=torch.float32) if return_lse else None
     scale = (1.0 / math.sqrt(D)) if softmax_scale is None else float(softmax_scale)
     workspace = _workspace(workspace, index, 0 if workspace is not None else
