@@ -1,4 +1,5 @@
-"""What the operators around a paged cache tell autograd: that tensors of the caller's were written (needs a GPU)."""
+"""What the operators around a paged cache tell autograd: which results are part of a graph, and that tensors of the
+caller's were written (needs a GPU)."""
 import pytest
 import torch
 
@@ -90,3 +91,25 @@ def test_outputs_that_require_a_gradient_are_refused():
             call()
     fa.attend_paged(x, pool, v_pages, table, lens)   # (only read)
     torch.cuda.synchronize()
+
+
+def test_tangents_of_one_of_two_inputs():
+    """Forward mode where queries or keys alone have a tangent, by themselves, in a transform, and over a gradient."""
+    rotary, fad = fa.Rotary(64, device=DEV), torch.autograd.forward_ad
+    q, k, t = _randn(1, 4, 5, 64), _randn(1, 2, 5, 64), _randn(1, 4, 5, 64)
+    rq, rk, rt = (fa.rotate(x, None, 3, rotary) for x in (q, k, t))
+    for which in range(2):
+        with fad.dual_level():
+            pair = [q, k]
+            pair[which] = fad.make_dual(pair[which], t[:, :pair[which].shape[1]])
+            outs = [fad.unpack_dual(y) for y in fa.rotate(*pair, 3, rotary)]
+        assert torch.equal(outs[0].primal, rq) and torch.equal(outs[1].primal, rk)
+        assert torch.equal(outs[which].tangent, rt[:, :pair[which].shape[1]])
+        other = outs[1 - which].tangent
+        assert other is None or (other == 0).all()
+    (a, b), (da, db) = torch.func.jvp(lambda x: fa.rotate(x, k, 3, rotary), (q,), (t,))
+    assert torch.equal(a, rq) and torch.equal(b, rk) and torch.equal(da, rt) and (db == 0).all()
+    # The rotation keeps lengths: the gradient of its half square is x, the derivative of that t.  Two rotations of |x| up to
+    # 6, each off by 20 u (|x_a| + |x_b|).
+    _, h = torch.func.jvp(torch.func.grad(lambda x: (fa.rotate(x, k, 3, rotary)[0] ** 2).sum() / 2), (q,), (t,))
+    assert (h - t).abs().max() <= 2 * 20 * 2.0 ** -24 * 2 * float(t.abs().max())

@@ -205,7 +205,8 @@ def _keep(ctx, positions, rotary, transposed) -> None:
         ctx.save_for_forward(positions)
     else:
         ctx.first = positions
-    ctx.set_materialize_grads(False)
+    # (Forward mode needs a tangent for every result.)
+    ctx.set_materialize_grads(getattr(forward_ad, "_current_level", -1) >= 0)
 
 
 def _again(ctx, q, k, transposed: bool):
