@@ -113,3 +113,25 @@ def test_tangents_of_one_of_two_inputs():
     # 6, each off by 20 u (|x_a| + |x_b|).
     _, h = torch.func.jvp(torch.func.grad(lambda x: (fa.rotate(x, k, 3, rotary)[0] ** 2).sum() / 2), (q,), (t,))
     assert (h - t).abs().max() <= 2 * 20 * 2.0 ** -24 * 2 * float(t.abs().max())
+
+
+def test_rotation_of_an_input_without_gradient_is_outside_the_graph():
+    rotary = fa.Rotary(64, device=DEV)
+    q, k = _randn(1, 4, 5, 64), _randn(1, 2, 5, 64)
+    for first, second in ((True, False), (False, True), (True, True), (False, False)):
+        x, y = q.clone().requires_grad_(first), k.clone().requires_grad_(second)
+        a, b = fa.rotate(x, y, 3, rotary)
+        assert (a.requires_grad, b.requires_grad) == (first, second)
+        want = fa.rotate(q, k, 3, rotary)
+        assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+        for z, out in ((x, a), (y, b)):
+            if z.requires_grad:
+                g, = torch.autograd.grad(out.sum(), z, retain_graph=True)
+                assert torch.equal(g, torch.autograd.grad(fa.rotate(z, None, 3, rotary).sum(), z)[0])
+    # A tangent of one input only, beside a gradient of the other.
+    with torch.autograd.forward_ad.dual_level():
+        x = q.clone().requires_grad_()
+        a, b = fa.rotate(x, torch.autograd.forward_ad.make_dual(k, k), 3, rotary)
+        assert torch.equal(torch.autograd.forward_ad.unpack_dual(b).tangent, want[1])
+        g, = torch.autograd.grad(a.sum(), x)
+    assert torch.equal(g, torch.autograd.grad(fa.rotate(x, None, 3, rotary).sum(), x)[0])

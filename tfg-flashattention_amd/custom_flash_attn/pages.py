@@ -235,7 +235,10 @@ class _Rotate(_Linear):
     @staticmethod
     def forward(ctx, q, k, positions, rotary, transposed):
         _keep(ctx, positions, rotary, transposed)
-        return _new_rotated(q, k, positions, rotary, transposed)
+        outs = _new_rotated(q, k, positions, rotary, transposed)
+        if getattr(forward_ad, "_current_level", -1) < 0:  # (tangents go by the other way)
+            ctx.mark_non_differentiable(*[y for y, needed in zip(outs, ctx.needs_input_grad) if y is not None and not needed])
+        return outs
 
 
 class _RotateTransformed(_Linear):
