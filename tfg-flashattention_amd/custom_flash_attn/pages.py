@@ -187,13 +187,20 @@ def _rotate(q, k, positions, rotary, q_out, k_out, transposed: bool) -> None:
                transposed, B, N, D, _ROTATED[q.dtype])
 
 
+def _empty_like(x):
+    """A new tensor in the layout of ``x``, with a dense last dimension: torch's empty_like sorts strides, and puts another
+    dimension there where ``x``'s rows share elements (a window that slides by one)."""
+    y = torch.empty_like(x)
+    return y if y.stride(-1) == 1 or y.shape[-1] <= 1 else x.new_empty(x.shape)
+
+
 def _dense(x):
     """A gradient as the kernel takes it: an expanded last dimension, for one, is copied."""
     return x if x.shape[-1] <= 1 or x.stride(-1) == 1 else x.contiguous()
 
 
 def _new_rotated(q, k, positions, rotary, transposed: bool):
-    q_out, k_out = torch.empty_like(q), None if k is None else torch.empty_like(k)
+    q_out, k_out = _empty_like(q), None if k is None else _empty_like(k)
     _rotate(q, k, positions, rotary, q_out, k_out, transposed)
     return q_out, k_out
 
@@ -287,9 +294,9 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions, rotary: Rotary, *
         raise RuntimeError("q_out and k_out are not differentiable: rotate without them, or under torch.no_grad()")
     _check_written(q_out, k_out)
     if q_out is None:
-        q_out = torch.empty_like(q)
+        q_out = _empty_like(q)
     if k is not None and k_out is None:
-        k_out = torch.empty_like(k)
+        k_out = _empty_like(k)
     _rotate(q, k, positions, rotary, q_out, k_out, False)
     increment_version([x for x in outs if x is not None])
     return q_out if k is None else (q_out, k_out)
@@ -399,7 +406,7 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     B, _, N, _ = k.shape
     pad = q_out is None
     if q is not None and pad:
-        q_out = torch.empty_like(q)
+        q_out = _empty_like(q)
     turns, rot, interleaved, magnitude = (0, 0, False, 1.0) if rotary is None else (
         rotary._turns.data_ptr(), rotary.dim, rotary.interleaved, rotary.magnitude)
     _launch_on(k_pages.get_device(), _C.append, _view(k), _view(v), _view(k_pages), _view(v_pages), page_table.data_ptr(),
@@ -467,7 +474,7 @@ def attend_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     M, index = page_table.shape[1], k_pages.get_device()
     pad = out is None
     if pad:
-        out = torch.empty_like(q)
+        out = _empty_like(q)
     lse = None
     if return_lse:
         lse = q.new_empty((B, H, N), dtype=torch.float32)
