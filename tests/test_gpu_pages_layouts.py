@@ -1,4 +1,4 @@
-"""Layouts that the operators around a paged cache take and whose new results torch would lay out otherwise (needs a
+"""Layouts: inputs whose new results torch would lay out otherwise, and parts in their workspaces (needs a
 GPU)."""
 import pytest
 import torch
@@ -54,3 +54,33 @@ def test_one_token_expanded_over_heads(strides):
     assert torch.equal(fa.attend_paged(q, k_pages, v_pages, table, lens),
                        fa.attend_paged(q.contiguous(), k_pages, v_pages, table, lens))
     assert torch.equal(fa.rotate(q, None, 3, rotary), fa.rotate(q.contiguous(), None, 3, rotary))
+
+
+@pytest.mark.parametrize("H,H_kv,D,R,n", [(3, 3, 64, 1, 4), (6, 2, 128, 2, 5), (40, 1, 64, 1, 3), (5, 5, 72, 1, 70)])
+def test_workspaces_of_just_the_size(H, H_kv, D, R, n):
+    """Parts of few rows, of a tile and of several lie in the bytes that are asked for, and give what a larger workspace
+    gives."""
+    page, M_prefix, M, B = 16, 300, 40, R * n
+    g = torch.Generator().manual_seed(H + D)
+    k_pages, v_pages = (torch.randn(R * M_prefix + B * M, H_kv, page, D, generator=g).to(BF).to(DEV) for _ in range(2))
+    order = torch.randperm(R * M_prefix + B * M, generator=g).to(torch.int32).to(DEV)
+    prefix, table = order[:R * M_prefix].view(R, M_prefix), order[R * M_prefix:].view(B, M)
+    plens = torch.full((R,), M_prefix * page - 3, dtype=torch.int32, device=DEV)
+    lens = torch.arange(B, dtype=torch.int32, device=DEV) * 9
+    C = fa._C
+
+    def check(call, nbytes):
+        assert nbytes > 0
+        want = call(torch.empty(2 * nbytes, dtype=torch.uint8, device=DEV))
+        room = torch.full((nbytes + 256,), 255, dtype=torch.uint8, device=DEV)
+        got = call(room[:nbytes])
+        assert (room[nbytes:] == 255).all()
+        assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(got, want))
+
+    q = torch.randn(B, H, D, generator=g).to(BF).to(DEV)
+    check(lambda ws: fa.decode_shared(q, k_pages, v_pages, prefix, plens, table, lens, return_lse=True, workspace=ws),
+          C.decode_shared_workspace(R, B, H, H_kv, page, M_prefix, M, D))
+    for N in (1, 2, n):
+        x = torch.randn(R, H, N, D, generator=g).to(BF).to(DEV)
+        check(lambda ws: fa.attend_paged(x, k_pages, v_pages, prefix, plens - N, return_lse=True, workspace=ws),
+              C.attend_workspace(R, H, H_kv, N, page, M_prefix, D))

@@ -59,3 +59,22 @@ def test_written_tensors_that_require_a_gradient(launches):
     fa.attend_paged(x, _grad(pool), pool, table, lens)                          # (only read)
     fa.decode_shared(vec, _grad(pool), pool, table, lens, table, lens)
     assert len(launches) == len(calls) + 2
+
+
+def test_workspaces_hold_the_rows_that_there_are():
+    """A part keeps D sums, an offset and two sums of weights of each of its rows, in whole lines of 128 bytes, all of them in
+    256 bytes."""
+    C = pages._C
+
+    def at_most(jobs, parts, rows, D):
+        return jobs * parts * (rows * (D + 3) + 31) // 32 * 128 + 256
+
+    # (groups, sequences, query heads, key-value heads, page, prefix pages, pages, D): own parts of one row, of four, of 40 heads
+    # in two tiles; jobs enough for one part each.
+    assert C.decode_shared_workspace(1, 512, 32, 32, 16, 64, 8, 128) <= at_most(32 * 4, 2, 128, 128) + at_most(512 * 32, 1, 1, 128)
+    assert C.decode_shared_workspace(8, 512, 32, 8, 16, 64, 8, 128) <= at_most(8 * 8 * 2, 2, 128, 128) + at_most(512 * 8, 1, 4, 128)
+    assert C.decode_shared_workspace(1, 600, 40, 1, 16, 8, 8, 64) <= at_most(188, 1, 128, 64) + at_most(600 * 2, 1, 32, 64)
+    assert C.decode_shared_workspace(2, 6, 12, 12, 16, 2048, 8, 64) <= at_most(24, 21, 3, 64) + at_most(72, 1, 1, 64)
+    # One token of one query head a key-value head behind a long cache.
+    assert C.attend_workspace(1, 12, 12, 1, 16, 2048, 64) <= at_most(12, 32, 1, 64)
+    assert C.attend_workspace(1, 12, 12, 70, 16, 2048, 64) <= at_most(12, 32, 70, 64)

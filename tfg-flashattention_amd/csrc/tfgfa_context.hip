@@ -592,15 +592,20 @@ struct Job {
 };
 
 // Where its rows go: the outputs, or (part) its part of them: D floats a row of sums, and of each row the offset and the
-// sums of weights.
+// sums of weights, part_rows rows of each (those that there are: 512 sequences of 32 heads of 128 behind a prefix keep 10.5 MB
+// of their own, a tile's 32 rows each would be 275).
 struct Sink {
   void* o;
   long long o_step, o_head;       // elements
   float* lse;
   long long l_step, l_head;
   float* part;
+  int part_rows;
   int fill_to, fill;              // rows from Job::rows up to here get zeros (fill 1) or NaN (fill 2)
 };
+
+// Floats of a part: whole lines of 128 bytes.
+__host__ __device__ constexpr long long part_floats(int rows, int D) { return ((long long)rows * (D + 3) + 31) / 32 * 32; }
 
 constexpr int few_lds(int kDH, int waves) {  // a block of each wave, or its rows
   const int blocks = waves * 2 * kDH * kHalfBytes, rows = waves * kBlock * 64 * kDH * 4;
@@ -662,8 +667,8 @@ __device__ __forceinline__ void put(const unsigned char* rows, const Stats<kW>& 
     *reinterpret_cast<f32x4*>(at) = a;
     *reinterpret_cast<f32x4*>(at + 4) = b;
     if (c8 == 0) {
-      float* const stats = to.part + (long long)kBlock * D + row;
-      stats[0] = M, stats[kBlock] = l, stats[2 * kBlock] = lp;
+      float* const stats = to.part + (long long)to.part_rows * D + row;
+      stats[0] = M, stats[to.part_rows] = l, stats[2 * to.part_rows] = lp;
     }
     return;
   }
@@ -881,8 +886,8 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
           *reinterpret_cast<f32x4*>(to.part + (long long)row * D + 32 * j + 8 * g + 4 * h) =
               f32x4{w.o[j][4 * g], w.o[j][4 * g + 1], w.o[j][4 * g + 2], w.o[j][4 * g + 3]};
     if (h == 0) {
-      float* const stats = to.part + (long long)kManyRows * D + row;
-      stats[0] = m, stats[kManyRows] = l, stats[2 * kManyRows] = lp;
+      float* const stats = to.part + (long long)to.part_rows * D + row;
+      stats[0] = m, stats[to.part_rows] = l, stats[2 * to.part_rows] = lp;
     }
     return;
   }
@@ -926,7 +931,7 @@ constexpr int kMine = kMaxParts / kLanes;  // parts whose statistics a lane has
 constexpr int kAtOnce = kLanes / kSplit;   // parts whose sums a thread loads together
 
 // A row's parts: `count` of them, `stride` floats apart, the sums of part 0 at `sums` (this lane's dims) and its offset at
-// `stats` (the sums of weights kRows and 2 kRows further).
+// `stats` (the sums of weights `rows` and 2 `rows` further).
 struct Parts {
   const float* sums;
   const float* stats;
@@ -934,7 +939,7 @@ struct Parts {
   int count, rows;
 };
 __device__ __forceinline__ Parts parts_of(const float* part, long long job, int count, int rows, int row, int D, int c8) {
-  const long long stride = (long long)rows * (D + 3);
+  const long long stride = part_floats(rows, D);
   const float* const at = part + job * count * stride;
   return {at + (long long)row * D + 8 * c8, at + (long long)rows * D + row, stride, count, rows};
 }
@@ -1045,7 +1050,7 @@ struct AttendArgs {
   const int* lens;
   const int* lengths;
   Division by_page, by_group;
-  int page, P, n_max, N, G, Hkv, heads, D, causal, pad, tiles, parts;
+  int page, P, n_max, N, G, Hkv, heads, D, causal, pad, tiles, parts, part_rows;
   float scale, scale_log2;
 };
 
@@ -1128,7 +1133,8 @@ __global__ __launch_bounds__(64 * waves_of(kKind), simd_waves(kKind, kDH)) void 
   to.o_step = a.os.n, to.o_head = a.os.h;
   to.lse = a.lse ? a.lse + ((long long)b * a.Hkv * a.G + first_head) * a.N : nullptr;
   to.l_step = 1, to.l_head = a.N;
-  to.part = a.parts > 1 ? a.part + (unit * a.parts + s) * kRows * (a.D + 3) : nullptr;
+  to.part = a.parts > 1 ? a.part + (unit * a.parts + s) * part_floats(a.part_rows, a.D) : nullptr;
+  to.part_rows = a.part_rows;
   to.fill_to = a.N * a.G, to.fill = !fits ? 2 : a.pad;
   run<T, kDH, kAligned, kKind, 1, kLse>(src, job, to, a.D, lds, st);
 }
@@ -1144,7 +1150,7 @@ __global__ __launch_bounds__(kThreads) void attend_join_kernel(const AttendArgs 
   const bool fits = len >= 0 && n >= 0 && n <= a.N && (long long)len + (a.causal ? n : 0) <= a.n_max;
   const bool past = fits && step >= n;
   const int d = 8 * c < a.D ? c : 0;
-  Parts p[1] = {parts_of(a.part, unit, a.parts, kRows, row, a.D, d)};
+  Parts p[1] = {parts_of(a.part, unit, a.parts, a.part_rows, row, a.D, d)};
   if (!fits || step >= n) p[0].count = 0;
   const Joined y = join(p, a.scale_log2);
   if (group % kSplit != 0 || step >= a.N || (past && !a.pad)) return;
@@ -1174,8 +1180,8 @@ struct SharedArgs {
   long long prefix_stride, table_stride;
   Division by_page, by_group;
   int page, P, prefix_max, n_max, G, Hkv, R, each, D;   // each: sequences of a group
-  int prefix_heads, prefix_tiles, prefix_parts, prefix_jobs;
-  int own_heads, own_tiles, own_parts;
+  int prefix_heads, prefix_tiles, prefix_parts, prefix_part_rows, prefix_jobs;
+  int own_heads, own_tiles, own_parts, own_part_rows;
   float scale, scale_log2;
 };
 
@@ -1208,7 +1214,8 @@ __global__ __launch_bounds__(64 * waves_of(kKind), simd_waves(kKind, kDH)) void 
     job.q = static_cast<const T*>(a.q) + (long long)b * a.each * a.qs.b + first_head * a.qs.h;
     job.row0 = tile * kRows, job.rows = a.each * a.G, job.seen = src.keys;
     share<kKind>(&job, (src.keys + kBlock - 1) / kBlock, s, parts);
-    to.part = a.prefix_part + (((long long)head * a.prefix_tiles + tile) * parts + s) * kRows * (a.D + 3);
+    to.part_rows = a.prefix_part_rows;
+    to.part = a.prefix_part + (((long long)head * a.prefix_tiles + tile) * parts + s) * part_floats(a.prefix_part_rows, a.D);
     run<T, kDH, kAligned, kKind, 1, true>(src, job, to, a.D, lds, st);
   } else {
     constexpr int kRows = rows_of(Kind::kFew);
@@ -1235,7 +1242,8 @@ __global__ __launch_bounds__(64 * waves_of(kKind), simd_waves(kKind, kDH)) void 
     job.q = static_cast<const T*>(a.q) + b * a.qs.b + first_head * a.qs.h;
     job.row0 = tile * kRows, job.rows = a.G, job.seen = src.keys;
     share<Kind::kFew>(&job, (src.keys + kBlock - 1) / kBlock, s, parts);
-    to.part = a.own_part + (((long long)head * a.own_tiles + tile) * parts + s) * kRows * (a.D + 3);
+    to.part_rows = a.own_part_rows;
+    to.part = a.own_part + (((long long)head * a.own_tiles + tile) * parts + s) * part_floats(a.own_part_rows, a.D);
     run<T, kDH, kAligned, Kind::kFew, 2, true>(src, job, to, a.D, lds, st);
   }
 }
@@ -1251,8 +1259,9 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
   const int d = 8 * c < a.D ? c : 0;
   const int row = (b - r * a.each) * a.G + g;
   Parts p[2] = {
-      parts_of(a.prefix_part, ((long long)r * a.Hkv + kv) * a.prefix_tiles + row / kRows, a.prefix_parts, kRows, row % kRows, a.D, d),
-      parts_of(a.own_part, ((long long)b * a.Hkv + kv) * a.own_tiles + g / kBlock, a.own_parts, kBlock, g % kBlock, a.D, d)};
+      parts_of(a.prefix_part, ((long long)r * a.Hkv + kv) * a.prefix_tiles + row / kRows, a.prefix_parts, a.prefix_part_rows,
+               row % kRows, a.D, d),
+      parts_of(a.own_part, ((long long)b * a.Hkv + kv) * a.own_tiles + g / kBlock, a.own_parts, a.own_part_rows, g % kBlock, a.D, d)};
   const Joined y = join(p, a.scale_log2);
   if (group % kSplit != 0 || mine >= rows) return;
   if (8 * c < a.D) store_row(static_cast<T*>(a.o) + b * a.os.b + h * a.os.h + 8 * c, y, false, !fits);
@@ -1278,8 +1287,10 @@ static int choose_parts(long long slots, long long jobs, long long n_max, long l
   const long long parts = std::min({slots * kCu / std::max(1LL, jobs), n_max / least, (long long)kMaxParts});
   return (int)std::max(1LL, parts);
 }
-static size_t part_bytes(Kind kind, long long jobs, int parts, int D) {
-  return ((size_t)jobs * parts * rows_of(kind) * (D + 3) * 4 + 255) / 256 * 256;
+// Rows that a part keeps of a job of `rows`: those of its largest tile.
+static int part_rows(Kind kind, long long rows) { return (int)std::min<long long>(rows_of(kind), rows); }
+static size_t part_bytes(int rows, long long jobs, int parts, int D) {
+  return ((size_t)jobs * parts * part_floats(rows, D) * 4 + 255) / 256 * 256;
 }
 
 static bool heads_ok(int B, int H, int Hkv, int page, int M) {
@@ -1290,7 +1301,7 @@ static bool heads_ok(int B, int H, int Hkv, int page, int M) {
 struct AttendPlan {
   Kind kind;
   long long tiles, jobs;
-  int parts;
+  int parts, part_rows;
   size_t bytes;
 };
 // False: too large.
@@ -1310,7 +1321,8 @@ static bool attend_plan(int B, int H, int Hkv, int N, int page, int M, int D, At
   // heads: 13.7 us whole, 16.7 in two, of four waves).
   x->parts = choose_parts(x->kind == Kind::kFewWide ? 1 : 2, x->jobs, n_max, 256);
   if (x->parts < 4 && n_max < 4096) x->parts = 1;
-  x->bytes = x->parts > 1 ? part_bytes(x->kind, x->jobs, x->parts, D) : 0;
+  x->part_rows = part_rows(x->kind, rows);
+  x->bytes = x->parts > 1 ? part_bytes(x->part_rows, x->jobs, x->parts, D) : 0;
   return x->jobs * x->parts <= kMaxGroups;  // (the join has at most kManyRows / kJoinRows a job, of few jobs)
 }
 
@@ -1347,7 +1359,7 @@ static hipError_t launch_attend(const AttendArgs& a, const AttendPlan& x, hipStr
 struct SharedPlan {
   Kind kind;
   long long prefix_tiles, prefix_jobs, own_tiles, own_jobs;  // jobs: without their parts
-  int prefix_parts, own_parts;
+  int prefix_parts, prefix_part_rows, own_parts, own_part_rows;
   size_t own_at, bytes;
 };
 static bool shared_plan(int R, int B, int H, int Hkv, int page, int Mp, int M, int D, SharedPlan* x) {
@@ -1363,8 +1375,9 @@ static bool shared_plan(int R, int B, int H, int Hkv, int page, int Mp, int M, i
   // 20), many: one, with the sequences' own beside them (1 of 32000 for 64 sequences 70, with two 76).
   x->prefix_parts = choose_parts(x->kind == Kind::kFew ? 2 : 1, x->prefix_jobs, p_max, x->kind == Kind::kMany ? 512 : 128);
   x->own_parts = choose_parts(2, x->own_jobs, n_max, 128);
-  x->own_at = part_bytes(x->kind, x->prefix_jobs, x->prefix_parts, D);
-  x->bytes = x->own_at + part_bytes(Kind::kFew, x->own_jobs, x->own_parts, D);
+  x->prefix_part_rows = part_rows(x->kind, rows), x->own_part_rows = part_rows(Kind::kFew, G);
+  x->own_at = part_bytes(x->prefix_part_rows, x->prefix_jobs, x->prefix_parts, D);
+  x->bytes = x->own_at + part_bytes(x->own_part_rows, x->own_jobs, x->own_parts, D);
   return x->prefix_jobs * x->prefix_parts + x->own_jobs * x->own_parts <= kMaxGroups && (long long)B * H <= kMaxGroups * kJoinRows;
 }
 
@@ -1441,7 +1454,7 @@ extern "C" int tfpages_attend(const void* q, const int64_t* q_strides, const voi
   a.table = page_table, a.table_stride = B > 1 ? table_stride : 0, a.lens = cache_seqlens, a.lengths = lengths;
   a.by_page = tfgfa::division_by(page), a.by_group = tfgfa::division_by(H / H_kv);
   a.page = page, a.P = P, a.n_max = M * page, a.N = N, a.G = H / H_kv, a.Hkv = H_kv, a.heads = B * H_kv, a.D = D;
-  a.causal = causal, a.pad = pad != 0, a.tiles = (int)x.tiles, a.parts = x.parts;
+  a.causal = causal, a.pad = pad != 0, a.tiles = (int)x.tiles, a.parts = x.parts, a.part_rows = x.part_rows;
   a.scale = softmax_scale, a.scale_log2 = softmax_scale * kLog2e;
   const hipStream_t stream = (hipStream_t)hip_stream;
   const hipError_t e = dtype == TFGFA_DTYPE_BF16 ? launch_attend<__bf16>(a, x, stream) : launch_attend<_Float16>(a, x, stream);
@@ -1506,8 +1519,8 @@ extern "C" int tfpages_decode_shared(const void* q, const int64_t* q_strides, vo
   a.page = page, a.P = P, a.prefix_max = M_prefix * page, a.n_max = M * page, a.G = H / H_kv, a.Hkv = H_kv, a.R = R;
   a.each = B / R, a.D = D;
   a.prefix_heads = R * H_kv, a.prefix_tiles = (int)x.prefix_tiles, a.prefix_parts = x.prefix_parts;
-  a.prefix_jobs = (int)(x.prefix_jobs * x.prefix_parts);
-  a.own_heads = B * H_kv, a.own_tiles = (int)x.own_tiles, a.own_parts = x.own_parts;
+  a.prefix_part_rows = x.prefix_part_rows, a.prefix_jobs = (int)(x.prefix_jobs * x.prefix_parts);
+  a.own_heads = B * H_kv, a.own_tiles = (int)x.own_tiles, a.own_parts = x.own_parts, a.own_part_rows = x.own_part_rows;
   a.scale = softmax_scale, a.scale_log2 = softmax_scale * kLog2e;
   const hipStream_t stream = (hipStream_t)hip_stream;
   const hipError_t e = dtype == TFGFA_DTYPE_BF16 ? launch_shared<__bf16>(a, x, B * H, stream)
