@@ -78,3 +78,25 @@ def test_workspaces_hold_the_rows_that_there_are():
     # One token of one query head a key-value head behind a long cache.
     assert C.attend_workspace(1, 12, 12, 1, 16, 2048, 64) <= at_most(12, 32, 1, 64)
     assert C.attend_workspace(1, 12, 12, 70, 16, 2048, 64) <= at_most(12, 32, 70, 64)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(base=1e-320), "float64's range"),
+    (dict(scaling="base", factor=10.0, base=1e308), "float64's range"),      # a base past it: all frequencies 0 but the first
+    (dict(scaling="base", factor=1e-200, base=1e-200), "float64's range"),   # a base of 0
+    (dict(scaling="base", factor=1e300, dim=4), "float64's range"),
+    (dict(scaling="linear", factor=1e-320), "float64's range"),
+    (dict(scaling="bands", factor=1e-320, trained_length=10), "float64's range"),
+    (dict(scaling="bands", factor=2.0, trained_length=float("nan")), "trained_length"),
+])
+def test_rotary_refuses_numbers_past_its_range(kw, match):
+    kw = dict(kw)
+    with pytest.raises(RuntimeError, match=match):
+        fa.Rotary(kw.pop("dim", 64), device="cpu", **kw)
+
+
+def test_rotary_of_unusual_bases():
+    assert fa.Rotary(2, 1e-300, device="cpu").frequencies == (1.0,)
+    assert fa.Rotary(2, scaling="base", factor=1e300, device="cpu").frequencies == (1.0,)
+    assert fa.Rotary(4, 1e300, device="cpu").frequencies == (1.0, 1e-150)
+    assert fa.Rotary(4, 0.25, device="cpu").frequencies == (1.0, 2.0)

@@ -75,18 +75,23 @@ class Rotary:
                 raise RuntimeError(f"scaling must be None, 'linear', 'base' or 'bands', got {scaling!r}")
             if not (math.isfinite(factor) and factor > 0) or (scaling is None and factor != 1.0):
                 raise RuntimeError(f"factor must be finite and positive, and 1 without scaling, got {factor}")
-            if scaling == "base" and dim > 2:
-                base = base * factor ** (dim / (dim - 2))
-            f = [base ** (-2 * i / dim) for i in range(dim // 2)]
+            try:
+                if scaling == "base" and dim > 2:
+                    base = base * factor ** (dim / (dim - 2))
+                f = [base ** (-2 * i / dim) for i in range(dim // 2)] if 0 < base < math.inf else [math.inf]
+            except OverflowError:
+                f = [math.inf]
             if scaling == "linear":
                 f = [x / factor for x in f]
             elif scaling == "bands":
-                if trained_length is None or trained_length <= 0 or not 0 <= low < high < math.inf:
+                if trained_length is None or not trained_length > 0 or not 0 <= low < high < math.inf:
                     raise RuntimeError("scaling='bands' needs a positive trained_length and 0 <= low < high, got "
                                        f"{trained_length}, {low} and {high}")
                 for i, x in enumerate(f):
                     keep = min(1.0, max(0.0, (trained_length * x / (2 * math.pi) - low) / (high - low)))
                     f[i] = x / factor * (1 - keep) + x * keep
+            if not all(math.isfinite(x) for x in f):
+                raise RuntimeError(f"base and factor give frequencies past float64's range, got {base} and {factor}")
         self.dim, self.interleaved, self.magnitude, self.frequencies = dim, bool(interleaved), float(magnitude), tuple(f)
         self._turns = torch.tensor([_turn(x) for x in f], dtype=torch.int64).to(device)
 
