@@ -100,3 +100,14 @@ def test_rotary_of_unusual_bases():
     assert fa.Rotary(2, scaling="base", factor=1e300, device="cpu").frequencies == (1.0,)
     assert fa.Rotary(4, 1e300, device="cpu").frequencies == (1.0, 1e-150)
     assert fa.Rotary(4, 0.25, device="cpu").frequencies == (1.0, 2.0)
+
+
+def test_first_positions_of_64_bits(launches):
+    x, rotary = _dev(2, 2, 3, 64), fa.Rotary(64, device="cpu")
+    for p in (2 ** 63, -2 ** 63 - 1, 10 ** 30):
+        with pytest.raises(RuntimeError, match="64 bits"):
+            fa.rotate(x, None, p, rotary)
+    assert not launches
+    for p in (2 ** 63 - 1, -2 ** 63, 0, True):
+        fa.rotate(x, None, p, rotary)
+    assert len(launches) == 4

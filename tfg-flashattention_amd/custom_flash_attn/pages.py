@@ -124,6 +124,10 @@ def _are_positions(p, B: int, N: int, index: int) -> bool:
     return p.dtype in _INTS and p.get_device() == index and p.shape in ((N,), (B, N), (1, N))
 
 
+def _is_first(p) -> bool:
+    return type(p) is int and -2 ** 63 <= p < 2 ** 63
+
+
 def _accepts_rotate(q, k, positions, rotary, outs) -> bool:
     """Everything _check_rotate checks, as one test."""
     qs, index, dtype = q.shape, q.get_device(), q.dtype
@@ -139,7 +143,7 @@ def _accepts_rotate(q, k, positions, rotary, outs) -> bool:
         if out is not None and not (x is not None and out.shape == x.shape and out.dtype is dtype
                                     and out.get_device() == index and (out.stride(3) == 1 or qs[3] == 1)):
             return False
-    return type(positions) is int or (isinstance(positions, torch.Tensor) and _are_positions(positions, qs[0], qs[2], index))
+    return _is_first(positions) or (isinstance(positions, torch.Tensor) and _are_positions(positions, qs[0], qs[2], index))
 
 
 def _check_rotate(q, k, positions, rotary, outs) -> None:
@@ -175,6 +179,8 @@ def _check_rotate(q, k, positions, rotary, outs) -> None:
             raise RuntimeError(f"positions must be on {q.device}, got {positions.device}")
     elif not isinstance(positions, int):
         raise RuntimeError(f"positions must be a tensor or the first position, got {type(positions).__name__}")
+    elif not _is_first(int(positions)):
+        raise RuntimeError(f"the first position must be an integer of 64 bits, got {positions}")
 
 
 def _rotate(q, k, positions, rotary, q_out, k_out, transposed: bool) -> None:
