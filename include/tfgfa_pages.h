@@ -69,6 +69,7 @@ int tfpages_append(const void* k, const int64_t* k_strides, const void* v, const
  * causal, and all rows when not.  Tokens i >= n_b = lengths[b] (N without lengths) have no output: their rows of o
  * and lse become 0 and -inf with pad != 0, and are left as they were otherwise.
  * q, o: (B, H, N, D), strides [b, h, n, d] (multiples of 8, rows apart); lse: (B, H, N) contiguous or NULL.
+ * softmax_scale: positive, log2(e) times it finite.
  * A row whose scores are all -inf, or that sees no key, gives O = 0 and LSE = -inf.  Hidden rows and rows past the
  * cache's never reach a result.  Visible on the device only: where cache_seqlens[b] < 0, n_b is not in [0, N] or the
  * rows do not fit M * page, O and LSE of the sequence's N tokens are NaN; a page id outside [0, P) among the rows that a

@@ -1,9 +1,12 @@
 """More refusals of the operators around a paged cache, on the CPU: with tensors that say they are on a device, and nothing
 launched."""
+import ctypes
+
 import pytest
 import torch
 
 import custom_flash_attn as fa
+import test_pages_cpu as boundary
 from custom_flash_attn import pages
 
 BF, I32 = torch.bfloat16, torch.int32
@@ -111,3 +114,12 @@ def test_first_positions_of_64_bits(launches):
     for p in (2 ** 63 - 1, -2 ** 63, 0, True):
         fa.rotate(x, None, p, rotary)
     assert len(launches) == 4
+
+
+def test_scales_whose_binary_logarithm_form_is_infinite():
+    """Weights are 2^(scale log2 e (s - m)): a scale of 2.4e38 or more would be infinite in it, and equal scores NaN."""
+    lib = ctypes.CDLL(fa.library_path())
+    for call in (boundary._attend, boundary._shared):
+        assert call(lib, scale=2.4e38) == boundary._code("ERR_SCALE")
+        assert call(lib, scale=3.4e38) == boundary._code("ERR_SCALE")
+        assert call(lib, scale=2.3e38, q=0) == boundary._code("ERR_NULL_POINTER")

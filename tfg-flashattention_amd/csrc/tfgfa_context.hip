@@ -1429,7 +1429,7 @@ extern "C" int tfpages_attend(const void* q, const int64_t* q_strides, const voi
   if (dtype != TFGFA_DTYPE_BF16 && dtype != TFGFA_DTYPE_F16) return TFGFA_ERR_DTYPE;
   if (!heads_ok(B, H, H_kv, page, M) || N < 0 || P < 0) return TFGFA_ERR_BAD_SHAPE;
   if (D < 8 || D > kMaxD || (D & 7)) return TFGFA_ERR_HEAD_DIM;
-  if (!(softmax_scale > 0.f) || !isfinite(softmax_scale)) return TFGFA_ERR_SCALE;
+  if (!(softmax_scale > 0.f) || !isfinite(softmax_scale * kLog2e)) return TFGFA_ERR_SCALE;
   if (causal != 0 && causal != 1) return TFGFA_ERR_CAUSAL_FLAG;
   if (B == 0 || H == 0 || N == 0) return TFGFA_OK;
   if (P == 0) return TFGFA_ERR_BAD_SHAPE;
@@ -1482,7 +1482,7 @@ extern "C" int tfpages_decode_shared(const void* q, const int64_t* q_strides, vo
   if (!heads_ok(B, H, H_kv, page, M) || M_prefix < 0 || P < 0 || R < 0 || (R == 0 ? B != 0 : B % R != 0))
     return TFGFA_ERR_BAD_SHAPE;
   if (D < 8 || D > kMaxD || (D & 7)) return TFGFA_ERR_HEAD_DIM;
-  if (!(softmax_scale > 0.f) || !isfinite(softmax_scale)) return TFGFA_ERR_SCALE;
+  if (!(softmax_scale > 0.f) || !isfinite(softmax_scale * kLog2e)) return TFGFA_ERR_SCALE;
   if ((k_new == nullptr) != (v_new == nullptr)) return TFGFA_ERR_NULL_POINTER;
   if (B == 0 || H == 0) return TFGFA_OK;
   if (P == 0) return TFGFA_ERR_BAD_SHAPE;
