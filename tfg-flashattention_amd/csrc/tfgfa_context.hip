@@ -282,7 +282,7 @@ struct State {
   v8 q[kC];
   f32x16 o[kOT];
   float m, thr;             // offset, and how far a score may pass it (-inf: the row has no weight yet)
-  float l, lp;              // this lane's sums of weights; kParts 1: of the rounded ones
+  float l, lp;              // this lane's sums of weights, and (kParts 1) of the rounded ones
   int seen;                 // keys that the row sees
   int koff[4], voff[2][2];  // LDS offsets of the operands, in a block's first 64 dims
 
@@ -463,7 +463,7 @@ struct State {
     }
   }
 
-  // Many rows: blocks in a pipeline.  s: the scores of block u; part: the weights of block u - 1; v, k: V of block
+  // Many rows (kParts 1): blocks in a pipeline.  s: the scores of block u; part: the weights of block u - 1; v, k: V of block
   // u - 1 and K of block u + 1 in LDS.  The products of V run beside the exponentials, those of K beside the weights' sums
   // and rounding, one matrix instruction and a share of them at a time (a wave's VALU work overlaps its own matrix
   // instructions).  Offsets are in the log2 domain (m = thr): 2^(c s - m) is one v_fma and one v_exp.
@@ -482,9 +482,7 @@ struct State {
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
       const int cc = i / kOT, j = i % kOT;
-      if constexpr (kPV)
-#pragma unroll
-        for (int n = 0; n < kParts; ++n) o[j] = Elem<T>::mfma(vo[i & 1], part[n][cc], o[j]);
+      if constexpr (kPV) o[j] = Elem<T>::mfma(vo[i & 1], part[0][cc], o[j]);
       if (i + 2 < kPairs) {
         if constexpr (kPV) vo[i & 1] = values(v, (i + 2) % kOT, (i + 2) / kOT);
       } else {
@@ -506,8 +504,7 @@ struct State {
       if (i + 2 < kC) ko[i & 1] = key_operand(k, i + 2);
       if (i == 0) {
         parts_of(p, part);
-#pragma unroll
-        for (int n = 0; n < kParts; ++n) asm volatile("" : "+v"(part[n][0]), "+v"(part[n][1]));
+        asm volatile("" : "+v"(part[0][0]), "+v"(part[0][1]));
       } else if (i == 1) {
         float sum = add_rounded(part, lp);
         // (As integers: past the bound, infinite or NaN.)
@@ -562,12 +559,11 @@ struct State {
     for (int j = 0; j < kOT; ++j) o[j] *= f;
   }
 
-  // Into LDS: rows of 64 kDH floats, 16-byte piece c of row r at place c ^ r % pieces; statistics beside.
-  __device__ __forceinline__ void publish(unsigned char* rows, float* sm, float* sl, float* slp, int lane) const {
+  // Few rows (kParts 2), into LDS: rows of 64 kDH floats, 16-byte piece c of row r at place c ^ r % pieces; statistics beside.
+  __device__ __forceinline__ void publish(unsigned char* rows, float* sm, float* sl, int lane) const {
     constexpr int kPieces = 16 * kDH;
     const int r = lane & 31, h = lane >> 5;
     const float lt = over_pair(l, [](float x, float y) { return x + y; });
-    const float lpt = kParts == 1 ? over_pair(lp, [](float x, float y) { return x + y; }) : lt;
 #pragma unroll
     for (int j = 0; j < kOT; ++j)
 #pragma unroll
@@ -576,7 +572,7 @@ struct State {
         *reinterpret_cast<f32x4*>(rows + (r * kPieces + (c ^ (r % kPieces))) * 16) =
             f32x4{o[j][4 * g], o[j][4 * g + 1], o[j][4 * g + 2], o[j][4 * g + 3]};
       }
-    if (h == 0) sm[r] = thr == -INFINITY ? -INFINITY : m, sl[r] = lt, slp[r] = lpt;
+    if (h == 0) sm[r] = thr == -INFINITY ? -INFINITY : m, sl[r] = lt;
   }
 };
 
@@ -616,7 +612,7 @@ constexpr int many_lds(int kDH) { return 4 * kDH * 2 * kHalfBytes; }  // four ti
 // Of each wave's rows.
 template <int kW>
 struct Stats {
-  float m[kW * kBlock], l[kW * kBlock], lp[kW * kBlock];
+  float m[kW * kBlock], l[kW * kBlock];
 };
 
 template <class T, int kDH, int kParts>
@@ -647,13 +643,13 @@ __device__ __forceinline__ void put(const unsigned char* rows, const Stats<kW>& 
   float M = -INFINITY;
 #pragma unroll
   for (int w = 0; w < kW; ++w) M = fmaxf(M, st.m[w * kBlock + row]);
-  float l = 0.f, lp = 0.f;
+  float l = 0.f;
   f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int w = 0; w < kW; ++w) {
     const int at = w * kBlock + row;
     const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((st.m[at] - M) * job.scale_log2);
-    l = fmaf(f, st.l[at], l), lp = fmaf(f, st.lp[at], lp);
+    l = fmaf(f, st.l[at], l);
     const f32x4 x = *reinterpret_cast<const f32x4*>(rows + (at * kPieces + ((2 * c8) ^ (at % kPieces))) * 16);
     const f32x4 y = *reinterpret_cast<const f32x4*>(rows + (at * kPieces + ((2 * c8 + 1) ^ (at % kPieces))) * 16);
 #pragma unroll
@@ -668,18 +664,18 @@ __device__ __forceinline__ void put(const unsigned char* rows, const Stats<kW>& 
     *reinterpret_cast<f32x4*>(at + 4) = b;
     if (c8 == 0) {
       float* const stats = to.part + (long long)to.part_rows * D + row;
-      stats[0] = M, stats[to.part_rows] = l, stats[2 * to.part_rows] = lp;
+      stats[0] = M, stats[to.part_rows] = stats[2 * to.part_rows] = l;
     }
     return;
   }
   const int step = divide(r, job.by_group), head = r - step * job.G;
   const float nan = __uint_as_float(0x7FC00000u);
-  const float inv = lp == 0.f ? 0.f : 1.f / lp;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   typename Elem<T>::v8 out;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    out[e] = (T)(real ? (lp == 0.f ? 0.f : a[e] * inv) : to.fill == 2 ? nan : 0.f);
-    out[4 + e] = (T)(real ? (lp == 0.f ? 0.f : b[e] * inv) : to.fill == 2 ? nan : 0.f);
+    out[e] = (T)(real ? (l == 0.f ? 0.f : a[e] * inv) : to.fill == 2 ? nan : 0.f);
+    out[4 + e] = (T)(real ? (l == 0.f ? 0.f : b[e] * inv) : to.fill == 2 ? nan : 0.f);
   }
   *reinterpret_cast<typename Elem<T>::v8*>(static_cast<T*>(to.o) + step * to.o_step + head * to.o_head + 8 * c8) = out;
   if (c8 == 0 && to.lse)
@@ -724,7 +720,7 @@ __device__ __forceinline__ void run_few(const Source& src, const Job& job, const
     pass(std::true_type());
   }
   __syncthreads();  // (the rows' places are the blocks')
-  w.publish(lds + wave * kBlock * 64 * kDH * 4, st.m + wave * kBlock, st.l + wave * kBlock, st.lp + wave * kBlock, lane);
+  w.publish(lds + wave * kBlock * 64 * kDH * 4, st.m + wave * kBlock, st.l + wave * kBlock, lane);
   __syncthreads();
   for (int e = tid; e < kBlock * 8 * kDH; e += 64 * kW)
     if (e % (8 * kDH) * 8 < D) put<T, kDH, kW>(lds, st, e / (8 * kDH), e % (8 * kDH), job, to, D);
@@ -732,11 +728,10 @@ __device__ __forceinline__ void run_few(const Source& src, const Job& job, const
 
 // Many rows.  Two K tiles and two V tiles of 64 keys in LDS.  Step j of the workgroup: block 2j; wait for K of tile j + 1 and
 // V of tile j, barrier, load V of tile j + 1 and K of tile j + 2; block 2j + 1.
-template <class T, int kDH, bool kAligned, int kParts, bool kLse>
+template <class T, int kDH, bool kAligned, bool kLse>
 __device__ __forceinline__ void run_many(const Source& src, const Job& job, const Sink& to, int D, unsigned char* lds) {
   constexpr int kHalf = kDH * kHalfBytes, kSlot = 2 * kHalf;  // K (or V) of a block, of a tile
-  constexpr bool kKeepL = kLse || kParts > 1;                 // the sum of unrounded weights
-  typedef State<T, kDH, kParts> W;
+  typedef State<T, kDH, 1> W;
   __shared__ int sh_again;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const uint32_t ring_at = tfgfa::lds_addr(lds);
@@ -781,12 +776,12 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
   w.m = -INFINITY;
   const float head = fminf(Elem<T>::kHead, 1e30f * c);
   f32x16 s;
-  typename W::v8 part[kParts][2];
+  typename W::v8 part[1][2];
   if (act > 0) w.scores(s, lds);
   // Half a step: block u, V of the one before it and K of the one after it in LDS.
   auto block = [&](int u, const unsigned char* v, const unsigned char* k, auto first) {
     if (u >= full) w.mask(s, (job.first + u) * kBlock, lane);
-    w.template fused<!decltype(first)::value, kKeepL>(v, k, s, part, c, head);
+    w.template fused<!decltype(first)::value, kLse>(v, k, s, part, c, head);
   };
   auto last = [&](const unsigned char* v) { w.output(v, part); };
   auto turn = [&](int j) {  // between the halves of step j
@@ -845,7 +840,6 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
   constexpr float kFar = 0x1p24f;
   const bool far = act > 0 && w.seen > job.first * kBlock && !(fabsf(w.m) < kFar);
   w.rescale(c);
-  if (kParts > 1) w.lp = w.l;
   w.thr = 0.f;
   if ((__builtin_amdgcn_ballot_w64(far) != 0 || w.any_nan()) && lane == 0) sh_again = 1;
   __syncthreads();
@@ -873,7 +867,7 @@ __device__ __forceinline__ void run_many(const Source& src, const Job& job, cons
   // A row's dims are its two lanes': 4 of every 8 each.
   const int i = lane & 31, h = lane >> 5, row = wave * kBlock + i, r = job.row0 + row;
   const auto add = [](float x, float y) { return x + y; };
-  const float l = over_pair(w.l, add), lp = kParts == 1 ? over_pair(w.lp, add) : l;
+  const float l = over_pair(w.l, add), lp = over_pair(w.lp, add);
   const float m = w.thr == -INFINITY ? -INFINITY : w.m;
   const bool real = r < job.rows;
   if (to.part) {
@@ -1068,11 +1062,11 @@ constexpr int simd_waves(Kind kind, int kDH) {
   return kDH == 2 ? 2 : kind == Kind::kMany ? 3 : 4;
 }
 
-template <class T, int kDH, bool kAligned, Kind kKind, int kParts, bool kLse>
+template <class T, int kDH, bool kAligned, Kind kKind, bool kLse>
 __device__ __forceinline__ void run(const Source& src, const Job& job, const Sink& to, int D, unsigned char* lds,
                                     Stats<waves_of(kKind)>& st) {
   if constexpr (kKind == Kind::kMany)
-    run_many<T, kDH, kAligned, kParts, kLse>(src, job, to, D, lds);
+    run_many<T, kDH, kAligned, kLse>(src, job, to, D, lds);
   else
     run_few<T, kDH, kAligned, waves_of(kKind)>(src, job, to, D, lds, st);
 }
@@ -1136,7 +1130,7 @@ __global__ __launch_bounds__(64 * waves_of(kKind), simd_waves(kKind, kDH)) void 
   to.part = a.parts > 1 ? a.part + (unit * a.parts + s) * part_floats(a.part_rows, a.D) : nullptr;
   to.part_rows = a.part_rows;
   to.fill_to = a.N * a.G, to.fill = !fits ? 2 : a.pad;
-  run<T, kDH, kAligned, kKind, 1, kLse>(src, job, to, a.D, lds, st);
+  run<T, kDH, kAligned, kKind, kLse>(src, job, to, a.D, lds, st);
 }
 
 template <class T, Kind kKind>
@@ -1216,7 +1210,7 @@ __global__ __launch_bounds__(64 * waves_of(kKind), simd_waves(kKind, kDH)) void 
     share<kKind>(&job, (src.keys + kBlock - 1) / kBlock, s, parts);
     to.part_rows = a.prefix_part_rows;
     to.part = a.prefix_part + (((long long)head * a.prefix_tiles + tile) * parts + s) * part_floats(a.prefix_part_rows, a.D);
-    run<T, kDH, kAligned, kKind, 1, true>(src, job, to, a.D, lds, st);
+    run<T, kDH, kAligned, kKind, true>(src, job, to, a.D, lds, st);
   } else {
     constexpr int kRows = rows_of(Kind::kFew);
     const int append = a.kn != nullptr, len = ((uniform_ints)a.lens)[b];
@@ -1244,7 +1238,7 @@ __global__ __launch_bounds__(64 * waves_of(kKind), simd_waves(kKind, kDH)) void 
     share<Kind::kFew>(&job, (src.keys + kBlock - 1) / kBlock, s, parts);
     to.part_rows = a.own_part_rows;
     to.part = a.own_part + (((long long)head * a.own_tiles + tile) * parts + s) * part_floats(a.own_part_rows, a.D);
-    run<T, kDH, kAligned, Kind::kFew, 2, true>(src, job, to, a.D, lds, st);
+    run<T, kDH, kAligned, Kind::kFew, true>(src, job, to, a.D, lds, st);
   }
 }
 
