@@ -254,8 +254,9 @@ class _Rotate(_Linear):
     def forward(ctx, q, k, positions, rotary, transposed):
         _keep(ctx, positions, rotary, transposed)
         outs = _new_rotated(q, k, positions, rotary, transposed)
-        if getattr(forward_ad, "_current_level", -1) < 0:  # (tangents go by the other way)
-            ctx.mark_non_differentiable(*[y for y, needed in zip(outs, ctx.needs_input_grad) if y is not None and not needed])
+        needed = ctx.needs_input_grad
+        if k is not None and needed[0] != needed[1] and getattr(forward_ad, "_current_level", -1) < 0:  # (tangents: both)
+            ctx.mark_non_differentiable(outs[1 if needed[0] else 0])
         return outs
 
 
