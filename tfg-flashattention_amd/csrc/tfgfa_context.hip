@@ -14,7 +14,9 @@
 // K and V rows go from their pages to LDS by direct loads.  Where a page is a multiple of 16 keys, so many have one page: its
 // id and address are scalars, and rows past the end are past its descriptor, which gives zeros.  (8 keys at a time the
 // scalar unit, which a CU's waves share, was as busy as the VALU: 8192 causal tokens of 16 heads took 178 us for 157.)
-// Other pages: each lane has an address, of a row of zeros where there is no key.  A page id outside the pool gives a
+// Other pages: each lane has an address, of a row of zeros where there is no key (pages of 8, 24, 40 and 100 keys alike: 2048
+// tokens behind 14336 586 us for 510 to 530, 64 sequences on a prefix of 32000 95 for 72, 16 on each of 4 of 700 29.3 for 27.1,
+// 4 tokens behind 1020 13.2 for 11.8).  A page id outside the pool gives a
 // row of NaN for K, so that NaN reaches the rows that see the key, and zeros for V.
 //
 // Few rows (up to 64 a job, 32 a workgroup, the two workgroups of a job side by side): each wave streams blocks of its own
@@ -1056,8 +1058,9 @@ __host__ __device__ constexpr int rows_of(Kind kind) {
 constexpr int waves_of(Kind kind) { return kind == Kind::kFewWide ? 8 : kWaves; }
 constexpr int lds_of(Kind kind, int kDH) { return kind == Kind::kMany ? many_lds(kDH) : few_lds(kDH, waves_of(kind)); }
 
-// Waves a SIMD, which bound the registers.  Many rows, heads of 64: 3 (8192 causal tokens of 16 heads 178 us, with 2 188); few
-// rows: 4 (64 sequences on 4 prefixes 24.7, with 2 and loads a block ahead 32).
+// Waves a SIMD, which bound the registers.  Many rows, heads of 64: 3 (8192 causal tokens of 16 heads 178 us, with 2 188; 151 to
+// 157 since, by its steps without branches); few rows: 4, which their registers leave anyhow (64 sequences on 4 prefixes 27 us
+// with a bound of 4 and of 2).
 constexpr int simd_waves(Kind kind, int kDH) {
   return kDH == 2 ? 2 : kind == Kind::kMany ? 3 : 4;
 }

@@ -15,8 +15,9 @@
 // row's page among it); then each thread moves the same 16 bytes of each token, or two times 16 of a pair of halves, so that
 // heads and places in them are told apart once.  (Told apart for each piece, 57 and 100 us for the appends below.)
 // Measured, from memory, us and TB/s read and written: 32001 tokens of 32 + 8 heads, half of each rotated, fp16, 132 (5.0;
-// a copy of as many bytes 127); 2 chunks of 8192 tokens into pages, queries too, 80 (5.0); 16 prompts of up to 1024 tokens,
-// 25 heads, into pages 31.3 (3.8: 40% of the padded batch's tokens are looked at and left); 8 tokens 3.2.
+// a copy of as many bytes 127); 16000 of them in float32 138 (4.8); 2 chunks of 8192 tokens into pages, queries too, 80 (5.0); 16 prompts of up to 1024 tokens,
+// 25 heads, into pages 31.3 (3.8: 40% of the padded batch's tokens are looked at and left, and the 400 items of a token leave
+// 22% of two rounds of threads idle); 8 tokens 3.2.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -90,7 +91,10 @@ __device__ __forceinline__ void sin_cos(uint32_t p, float* s, float* c) {
 }
 
 // kHalves: pairs (i, i + r/2), an item two times kWide neighbouring dims; kNeighbours: pairs (2i, 2i + 1), an item kWide
-// dims; kAny: an item one pair, for sizes and layouts where neither is whole 16-byte pieces.
+// dims; kAny: an item one pair, for sizes and layouts where neither is whole 16-byte pieces: rotated dims that are no
+// multiple of 16 (halves) or 8 (neighbours) 16-bit elements, of 8 or 4 float32 ones, and unaligned views.  (32001 tokens of 32 + 8
+// heads of 128, fp16: 20 dims rotated in halves 221 us, 40 234, 20 of neighbours 227, for 130 to 132 with 64 or 128; heads of
+// 40 rotated whole 112, for the 41 of a copy; 16000 tokens in float32 175 with 20 dims, 138 with 64.)
 enum class Pairs { kHalves, kNeighbours, kAny };
 
 template <class E, Pairs kPairs, bool kPaged>

@@ -476,7 +476,8 @@ def attend_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     natural log, -inf for tokens that do not count).  A token that sees no row, or scores of -inf alone, has output 0 and
     lse -inf.  A sequence whose length or number of new tokens does not fit its table yields NaN for its tokens, a page id
     outside the pool for those that see its rows (checked on the device).  ``workspace`` as for :func:`decode`, of
-    ``_C.attend_workspace(B, H, H_kv, N, page, M, D)`` bytes; with a smaller one a tile of rows is one workgroup's.
+    ``_C.attend_workspace(B, H, H_kv, N, page, M, D)`` bytes; with a smaller one a tile of rows is one workgroup's.  Keys are
+    divided by the table's width: give the columns that the texts may use (a view of a table's first ones).
     """
     if not _accepts_attend(q, k_pages, v_pages, page_table, cache_seqlens, lengths, out):
         _check_attend(q, k_pages, v_pages, page_table, cache_seqlens, lengths, out)
@@ -563,8 +564,9 @@ def decode_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     which become row ``cache_seqlens[b]`` of the sequence's own, ``out``, the lse.  A length that does not fit its table or a
     page id outside the pool yields NaN for the sequence, or for the whole group if it is the prefix's (checked on the
     device).  A prefix's weights are rounded to the type for the product with V, as :func:`attention`'s are, where a group
-    has more than 64 query rows (B / R * H / H_kv).  ``workspace``: at least ``_C.decode_shared_workspace(R, B, H, H_kv, page, M_prefix, M, D)`` bytes, kept per
-    device and stream where none is given.
+    has more than 64 query rows (B / R * H / H_kv).  ``workspace``: at least ``_C.decode_shared_workspace(R, B, H, H_kv, page,
+    M_prefix, M, D)`` bytes, kept per device and stream where none is given.  Keys are divided by the tables' widths, as in
+    :func:`attend_paged`.
     """
     if not _accepts_shared(q, k_pages, v_pages, prefix_table, prefix_lens, page_table, cache_seqlens, k_new, v_new, out):
         _check_shared(q, k_pages, v_pages, prefix_table, prefix_lens, page_table, cache_seqlens, k_new, v_new, out)
